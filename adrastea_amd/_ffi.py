@@ -20,6 +20,9 @@ SYMBOLS = (
     "adr_dequantize_absmax_uint8", "adr_quantize_absmax_uint8", "adr_matmul_f16_plan",
     "adr_matmul_nt_fp16u8_plan", "adr_softmax_rows", "adr_error_stats_f16", "adr_error_stats_f32", "adr_attention_f16",
     "adr_attention_f16_ws", "adr_attention_f16_workspace_bytes", "adr_embed_uint8",
+    "adr_rotary_f16", "adr_append_f16",
+    "adr_attention_paged_f16", "adr_attention_paged_f16_ws", "adr_attention_paged_f16_workspace_bytes",
+    "adr_attention_packed_f16", "adr_attention_packed_f16_ws", "adr_attention_packed_f16_workspace_bytes",
     "adr_debug_knob", "adr_microbench_empty", "adr_microbench_mfma_f16", "adr_microbench_stream_read",
     "adr_strerror", "adr_abi_version",
 )
@@ -36,6 +39,30 @@ class TensorDesc(C.Structure):
     """adr_tensor_desc: index 0 is the innermost dimension (kernels.rs:28-47)."""
     _fields_ = [("ptr", C.c_void_p), ("dims", C.c_uint32), ("shape", C.c_uint32 * 7),
                 ("strides", C.c_uint32 * 7)]
+
+
+class PagedCacheDesc(C.Structure):
+    """adr_paged_cache"""
+    _fields_ = [("key", C.c_void_p), ("value", C.c_void_p),
+                *((f, C.c_int32) for f in ("pages", "kv_heads", "page_size", "d")),
+                *((f"stride_{t}{s}", C.c_int64) for t in "kv" for s in "xyzp")]
+
+
+class PagedBatchDesc(C.Structure):
+    """adr_paged_batch"""
+    _fields_ = [*((f, C.c_void_p) for f in ("row_offsets", "lengths", "table")),
+                *((f, C.c_int32) for f in ("sequences", "table_width", "table_pitch", "longest_rows", "longest"))]
+
+
+class PackedBatchDesc(C.Structure):
+    """adr_packed_batch"""
+    _fields_ = [*((f, C.c_void_p) for f in ("row_offsets", "key_offsets")),
+                *((f, C.c_int32) for f in ("sequences", "longest_rows", "longest"))]
+
+
+class RotaryDesc(C.Structure):
+    """adr_rotary"""
+    _fields_ = [("turns", C.c_void_p), ("dims", C.c_int32), ("layout", C.c_uint32), ("magnitude", C.c_float)]
 
 
 _lib = None
@@ -97,6 +124,15 @@ def lib():
     L.adr_attention_f16_ws.argtypes = L.adr_attention_f16.argtypes + [vp, C.c_int64]
     L.adr_attention_f16_workspace_bytes.argtypes = [i32] * 16 + [u32]
     L.adr_embed_uint8.argtypes = [vp, i32, i32, vp, vp, vp, vp, i32]
+    cache, batch, packed, rotary = PagedCacheDesc, PagedBatchDesc, PackedBatchDesc, RotaryDesc
+    L.adr_rotary_f16.argtypes = [vp, vp, vp, vp, rotary] + [i32] * 9
+    L.adr_append_f16.argtypes = [vp, cache, batch, vp, vp, vp, vp, vp, rotary] + [i32] * 14
+    L.adr_attention_paged_f16.argtypes = [vp, vp, vp, cache, batch] + [i32] * 8 + [f32, f32, u32]
+    L.adr_attention_paged_f16_ws.argtypes = L.adr_attention_paged_f16.argtypes + [vp, C.c_int64]
+    L.adr_attention_paged_f16_workspace_bytes.argtypes = [cache, batch, i32, i32]
+    L.adr_attention_packed_f16.argtypes = [vp, vp, vp, vp, vp, packed] + [i32] * 17 + [f32, f32, u32]
+    L.adr_attention_packed_f16_ws.argtypes = L.adr_attention_packed_f16.argtypes + [vp, C.c_int64]
+    L.adr_attention_packed_f16_workspace_bytes.argtypes = [packed] + [i32] * 5
     L.adr_strerror.argtypes = [C.c_int]
     L.adr_strerror.restype = C.c_char_p
     L.adr_abi_version.restype = C.c_int
@@ -105,6 +141,8 @@ def lib():
             getattr(L, name).restype = C.c_int
     L.adr_matmul_f16_workspace_bytes.restype = C.c_int64
     L.adr_attention_f16_workspace_bytes.restype = C.c_int64
+    L.adr_attention_paged_f16_workspace_bytes.restype = C.c_int64
+    L.adr_attention_packed_f16_workspace_bytes.restype = C.c_int64
     L.adr_held_workspace_limit.restype = C.c_int64
     L.adr_held_workspace_bytes.restype = C.c_int64
     L.adr_held_workspace_declined.restype = C.c_int64

@@ -6,6 +6,7 @@
 #include <mutex>
 
 #include "adr_common.hpp"
+#include "sequences.hpp"
 
 using namespace adr;
 
@@ -365,7 +366,8 @@ const char* adr_strerror(int code) {
              "ADR_NOALLOC_SCRATCH_BYTES; use adr_matmul_f16 or adr_matmul_f16_ws";
     case ADR_EUNSUPPORTED_LAYOUT:
       return "fused attention covers head dimension 64 or 128, unit x strides, y/z strides that "
-             "are multiples of 8 and 16-byte aligned pointers";
+             "are multiples of 8 and 16-byte aligned pointers (over pages and packed prompts: head "
+             "dimension 1 to 256, any strides), and a positive scale and temperature";
     default: return code > 0 ? hipGetErrorString((hipError_t)code) : "unknown error";
   }
 }
@@ -829,6 +831,255 @@ int64_t adr_attention_f16_workspace_bytes(int32_t heads, int32_t m, int32_t n, i
   if (nothing) return 0;
   const AttentionShape t = {heads, m, n, d, yz[0], yz[1], yz[2], yz[3], yz[4], yz[5], yz[6], yz[7], mask};
   return attention_plan(t, device_info_for_plan().cus, INT64_MAX).workspace_bytes;
+}
+
+// ---- several sequences at once -------------------------------------------------------------------
+
+namespace {
+
+// Sizes of a batch of `sequences` over `rows` packed rows; *nothing_to_do where no row belongs to one.
+int validate_rows(int32_t heads, int32_t kv_heads, int32_t rows, int32_t d, int32_t sequences, bool* nothing_to_do) {
+  *nothing_to_do = false;
+  if (heads < 0 || kv_heads < 0 || rows < 0 || d < 0 || sequences < 0) return ADR_EINVAL_SHAPE;
+  if (heads == 0 || rows == 0 || d == 0 || sequences == 0) {
+    *nothing_to_do = true;
+    return ADR_OK;
+  }
+  if (kv_heads == 0 || heads % kv_heads != 0) return ADR_EINVAL_SHAPE;
+  if ((int64_t)heads * rows > 0x7fffffff || sequences == 0x7fffffff) return ADR_EINVAL_SHAPE;
+  return ADR_OK;
+}
+
+int validate_cache(const adr_paged_cache& c, const adr_paged_batch& b) {
+  if (c.pages < 0 || c.page_size < 0 || b.table_width < 0 || b.table_pitch < b.table_width) return ADR_EINVAL_SHAPE;
+  if (c.page_size == 0 && b.table_width > 0) return ADR_EINVAL_SHAPE;
+  return ADR_OK;
+}
+
+bool words(const void* p) { return (uintptr_t)p % 4 == 0; }  // of 32 bits
+
+int validate_rotary(const adr_rotary& r, int32_t d) {
+  if (r.dims < 0 || r.dims > d || r.dims % 2 != 0 || r.dims > ADR_ROTARY_MAX_DIMS) return ADR_EINVAL_SHAPE;
+  if (r.layout > ADR_ROTARY_PAIRS) return ADR_EINVAL_ENUM;
+  return ADR_OK;
+}
+
+int attention_of_rows(hipStream_t stream, const SequencesArgs& a, float scale, float temp, bool held, void* workspace,
+                      int64_t workspace_bytes) {
+  if (a.d > 256 || !(scale > 0.0f) || !(temp > 0.0f) || !(scale / temp < 1.0e30f)) return ADR_EUNSUPPORTED_LAYOUT;
+  const DeviceInfo dev = device_info();
+  if (dev.status) return dev.status;
+  auto launch = [&](const SequencesPlan& plan, void* scratch) {
+    return (int)launch_attention_sequences(stream, a, plan, scratch);
+  };
+  if (!held) return launch(sequences_plan(a, dev.cus, workspace_bytes), workspace);
+  const SequencesPlan plan = sequences_plan(a, dev.cus, held_limit.load(std::memory_order_relaxed));
+  if (plan.workspace_bytes == 0) return launch(plan, nullptr);
+  if (held_allowed(stream)) {
+    std::lock_guard<std::mutex> lock(held_mutex);
+    if (Held* h = held_buffer(stream, plan.workspace_bytes)) {
+      const int rc = launch(plan, h->ptr);
+      held_used(h);
+      return rc;
+    }
+  }
+  return launch(sequences_plan(a, dev.cus, 0), nullptr);
+}
+
+int paged_args(SequencesArgs& a, const adr_paged_cache& c, const adr_paged_batch& b, int32_t heads, int32_t rows,
+               bool* nothing) {
+  if (int rc = validate_rows(heads, c.kv_heads, rows, c.d, b.sequences, nothing)) return rc;
+  if (int rc = validate_cache(c, b)) return rc;
+  if (*nothing) return ADR_OK;
+  a.k = (const half_t*)c.key, a.v = (const half_t*)c.value;
+  a.sk = {c.stride_kx, c.stride_ky, c.stride_kz, c.stride_kp};
+  a.sv = {c.stride_vx, c.stride_vy, c.stride_vz, c.stride_vp};
+  a.row_offsets = b.row_offsets, a.keys_of = b.lengths, a.table = b.table;
+  a.sequences = b.sequences, a.rows = rows;
+  a.heads = heads, a.kv_heads = c.kv_heads, a.group = heads / c.kv_heads, a.d = c.d;
+  a.table_width = b.table_width, a.table_pitch = b.table_pitch, a.pages = c.pages, a.page_size = c.page_size;
+  a.longest_rows = b.longest_rows, a.longest = b.longest;
+  return ADR_OK;
+}
+
+int packed_args(SequencesArgs& a, const adr_packed_batch& b, int32_t heads, int32_t kv_heads, int32_t rows, int32_t keys,
+                int32_t d, bool* nothing) {
+  if (int rc = validate_rows(heads, kv_heads, rows, d, b.sequences, nothing)) return rc;
+  if (keys < 0) return ADR_EINVAL_SHAPE;
+  if (*nothing) return ADR_OK;
+  a.row_offsets = b.row_offsets, a.keys_of = b.key_offsets;
+  a.sequences = b.sequences, a.rows = rows, a.keys = keys;
+  a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.d = d;
+  a.longest_rows = b.longest_rows, a.longest = b.longest;
+  return ADR_OK;
+}
+
+void set_rows(SequencesArgs& a, uint16_t* output, const uint16_t* query, const int32_t (&o)[3], const int32_t (&q)[3],
+              float scale, float temp, uint32_t mask) {
+  a.out = (half_t*)output, a.q = (const half_t*)query;
+  a.so_x = o[0], a.so_y = o[1], a.so_z = o[2];
+  a.sq_x = q[0], a.sq_y = q[1], a.sq_z = q[2];
+  a.c = (float)((double)scale * 1.44269504088896340736 / (double)temp);
+  a.mask = mask;
+}
+
+int attention_paged(adr_stream_t stream, uint16_t* output, const uint16_t* query, const adr_paged_cache& cache,
+                    const adr_paged_batch& batch, int32_t heads, int32_t rows, const int32_t (&o)[3],
+                    const int32_t (&q)[3], float scale, float temp, uint32_t mask, bool held, void* workspace,
+                    int64_t workspace_bytes) {
+  SequencesArgs a = {};
+  bool nothing;
+  if (int rc = paged_args(a, cache, batch, heads, rows, &nothing)) return rc;
+  if (mask > ADR_MASK_CAUSAL) return ADR_EINVAL_ENUM;
+  if (nothing) return ADR_OK;
+  // (a cache without pages, or a table without entries, need not exist)
+  if (!output || !query || !batch.row_offsets || !batch.lengths || (batch.table_width > 0 && !batch.table) ||
+      (cache.pages > 0 && (!cache.key || !cache.value)))
+    return ADR_ENULL;
+  if (!words(batch.row_offsets) || !words(batch.lengths) || !words(batch.table)) return ADR_EUNSUPPORTED_LAYOUT;
+  if (!a.table) a.table = batch.lengths;  // (of no entries: it only says that the keys are in pages)
+  set_rows(a, output, query, o, q, scale, temp, mask);
+  return attention_of_rows((hipStream_t)stream, a, scale, temp, held, workspace, workspace_bytes);
+}
+
+int attention_packed(adr_stream_t stream, uint16_t* output, const uint16_t* query, const uint16_t* key,
+                     const uint16_t* value, const adr_packed_batch& batch, int32_t heads, int32_t kv_heads, int32_t rows,
+                     int32_t keys, int32_t d, const int32_t (&o)[3], const int32_t (&q)[3], const int32_t (&k)[3],
+                     const int32_t (&v)[3], float scale, float temp, uint32_t mask, bool held, void* workspace,
+                     int64_t workspace_bytes) {
+  SequencesArgs a = {};
+  bool nothing;
+  if (int rc = packed_args(a, batch, heads, kv_heads, rows, keys, d, &nothing)) return rc;
+  if (mask > ADR_MASK_CAUSAL) return ADR_EINVAL_ENUM;
+  if (nothing) return ADR_OK;
+  if (!output || !query || !batch.row_offsets || !batch.key_offsets || (keys > 0 && (!key || !value))) return ADR_ENULL;
+  if (!words(batch.row_offsets) || !words(batch.key_offsets)) return ADR_EUNSUPPORTED_LAYOUT;
+  a.k = (const half_t*)key, a.v = (const half_t*)value;
+  a.sk = {k[0], k[1], k[2], 0};
+  a.sv = {v[0], v[1], v[2], 0};
+  set_rows(a, output, query, o, q, scale, temp, mask);
+  return attention_of_rows((hipStream_t)stream, a, scale, temp, held, workspace, workspace_bytes);
+}
+
+int validate_workspace(const void* workspace, int64_t bytes) {
+  if (bytes < 0 || (bytes > 0 && !workspace)) return ADR_ENULL;
+  return (uintptr_t)workspace % 16 != 0 ? ADR_EINVAL_SHAPE : ADR_OK;
+}
+
+}  // namespace
+
+int adr_rotary_f16(adr_stream_t stream, uint16_t* output, const uint16_t* input, const int32_t* positions,
+                   adr_rotary rotary, int32_t heads, int32_t rows, int32_t d, int32_t stride_ox, int32_t stride_oy,
+                   int32_t stride_oz, int32_t stride_ix, int32_t stride_iy, int32_t stride_iz) {
+  bool nothing;
+  if (int rc = validate_rows(heads, heads, rows, d, 1, &nothing)) return rc;
+  if (int rc = validate_rotary(rotary, d)) return rc;
+  if (nothing) return ADR_OK;
+  if (!output || !input || (rotary.dims > 0 && (!positions || !rotary.turns))) return ADR_ENULL;
+  if (!words(positions) || (uintptr_t)rotary.turns % 8 != 0) return ADR_EUNSUPPORTED_LAYOUT;
+  if (int rc = check_device()) return rc;
+  RotaryArgs a = {};
+  a.q_out = (half_t*)output, a.q = (const half_t*)input;
+  a.so_x = stride_ox, a.so_y = stride_oy, a.so_z = stride_oz;
+  a.sq_x = stride_ix, a.sq_y = stride_iy, a.sq_z = stride_iz;
+  a.positions = positions;
+  a.turns = rotary.turns, a.dims = rotary.dims, a.pairs = rotary.layout == ADR_ROTARY_PAIRS;
+  a.magnitude = rotary.magnitude;
+  a.heads = heads, a.rows = rows, a.d = d;
+  return (int)launch_rotary((hipStream_t)stream, a);
+}
+
+int adr_append_f16(adr_stream_t stream, adr_paged_cache cache, adr_paged_batch batch, const uint16_t* key,
+                   const uint16_t* value, uint16_t* query_out, const uint16_t* query, const int32_t* positions,
+                   adr_rotary rotary, int32_t heads, int32_t rows, int32_t stride_kx, int32_t stride_ky,
+                   int32_t stride_kz, int32_t stride_vx, int32_t stride_vy, int32_t stride_vz, int32_t stride_ox,
+                   int32_t stride_oy, int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz) {
+  bool nothing;
+  if (!query && !query_out) heads = cache.kv_heads;  // (no queries: their number does not count)
+  if (int rc = validate_rows(heads, cache.kv_heads, rows, cache.d, batch.sequences, &nothing)) return rc;
+  if (int rc = validate_cache(cache, batch)) return rc;
+  if (int rc = validate_rotary(rotary, cache.d)) return rc;
+  if (nothing) return ADR_OK;
+  if (!key || !value || !query != !query_out || !batch.row_offsets || !batch.lengths ||
+      (batch.table_width > 0 && !batch.table) || (cache.pages > 0 && (!cache.key || !cache.value)) ||
+      (rotary.dims > 0 && !rotary.turns))
+    return ADR_ENULL;
+  if (!words(positions) || !words(batch.row_offsets) || !words(batch.lengths) || !words(batch.table) ||
+      (uintptr_t)rotary.turns % 8 != 0)
+    return ADR_EUNSUPPORTED_LAYOUT;
+  if (int rc = check_device()) return rc;
+  RotaryArgs a = {};
+  a.q_out = (half_t*)query_out, a.q = (const half_t*)query;
+  a.so_x = stride_ox, a.so_y = stride_oy, a.so_z = stride_oz;
+  a.sq_x = stride_qx, a.sq_y = stride_qy, a.sq_z = stride_qz;
+  a.k = (const half_t*)key, a.v = (const half_t*)value;
+  a.sk_x = stride_kx, a.sk_y = stride_ky, a.sk_z = stride_kz;
+  a.sv_x = stride_vx, a.sv_y = stride_vy, a.sv_z = stride_vz;
+  a.positions = positions;
+  a.turns = rotary.turns, a.dims = rotary.dims, a.pairs = rotary.layout == ADR_ROTARY_PAIRS;
+  a.magnitude = rotary.magnitude;
+  a.heads = query ? heads : 0, a.kv_heads = cache.kv_heads, a.rows = rows, a.d = cache.d;
+  a.cache = cache, a.batch = batch;
+  return (int)launch_rotary((hipStream_t)stream, a);
+}
+
+int adr_attention_paged_f16(adr_stream_t stream, uint16_t* output, const uint16_t* query, adr_paged_cache cache,
+                            adr_paged_batch batch, int32_t heads, int32_t rows, int32_t stride_ox, int32_t stride_oy,
+                            int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz, float scale,
+                            float temp, uint32_t mask) {
+  return attention_paged(stream, output, query, cache, batch, heads, rows, {stride_ox, stride_oy, stride_oz},
+                         {stride_qx, stride_qy, stride_qz}, scale, temp, mask, true, nullptr, 0);
+}
+
+int adr_attention_paged_f16_ws(adr_stream_t stream, uint16_t* output, const uint16_t* query, adr_paged_cache cache,
+                               adr_paged_batch batch, int32_t heads, int32_t rows, int32_t stride_ox, int32_t stride_oy,
+                               int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz, float scale,
+                               float temp, uint32_t mask, void* workspace, int64_t workspace_bytes) {
+  if (int rc = validate_workspace(workspace, workspace_bytes)) return rc;
+  return attention_paged(stream, output, query, cache, batch, heads, rows, {stride_ox, stride_oy, stride_oz},
+                         {stride_qx, stride_qy, stride_qz}, scale, temp, mask, false, workspace, workspace_bytes);
+}
+
+int64_t adr_attention_paged_f16_workspace_bytes(adr_paged_cache cache, adr_paged_batch batch, int32_t heads,
+                                                int32_t rows) {
+  SequencesArgs a = {};
+  bool nothing;
+  if (int rc = paged_args(a, cache, batch, heads, rows, &nothing)) return rc;
+  return nothing ? 0 : sequences_plan(a, device_info_for_plan().cus, INT64_MAX).workspace_bytes;
+}
+
+int adr_attention_packed_f16(adr_stream_t stream, uint16_t* output, const uint16_t* query, const uint16_t* key,
+                             const uint16_t* value, adr_packed_batch batch, int32_t heads, int32_t kv_heads,
+                             int32_t rows, int32_t keys, int32_t d, int32_t stride_ox, int32_t stride_oy,
+                             int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz,
+                             int32_t stride_kx, int32_t stride_ky, int32_t stride_kz, int32_t stride_vx,
+                             int32_t stride_vy, int32_t stride_vz, float scale, float temp, uint32_t mask) {
+  return attention_packed(stream, output, query, key, value, batch, heads, kv_heads, rows, keys, d,
+                          {stride_ox, stride_oy, stride_oz}, {stride_qx, stride_qy, stride_qz},
+                          {stride_kx, stride_ky, stride_kz}, {stride_vx, stride_vy, stride_vz}, scale, temp, mask, true,
+                          nullptr, 0);
+}
+
+int adr_attention_packed_f16_ws(adr_stream_t stream, uint16_t* output, const uint16_t* query, const uint16_t* key,
+                                const uint16_t* value, adr_packed_batch batch, int32_t heads, int32_t kv_heads,
+                                int32_t rows, int32_t keys, int32_t d, int32_t stride_ox, int32_t stride_oy,
+                                int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz,
+                                int32_t stride_kx, int32_t stride_ky, int32_t stride_kz, int32_t stride_vx,
+                                int32_t stride_vy, int32_t stride_vz, float scale, float temp, uint32_t mask,
+                                void* workspace, int64_t workspace_bytes) {
+  if (int rc = validate_workspace(workspace, workspace_bytes)) return rc;
+  return attention_packed(stream, output, query, key, value, batch, heads, kv_heads, rows, keys, d,
+                          {stride_ox, stride_oy, stride_oz}, {stride_qx, stride_qy, stride_qz},
+                          {stride_kx, stride_ky, stride_kz}, {stride_vx, stride_vy, stride_vz}, scale, temp, mask, false,
+                          workspace, workspace_bytes);
+}
+
+int64_t adr_attention_packed_f16_workspace_bytes(adr_packed_batch batch, int32_t heads, int32_t kv_heads, int32_t rows,
+                                                 int32_t keys, int32_t d) {
+  SequencesArgs a = {};
+  bool nothing;
+  if (int rc = packed_args(a, batch, heads, kv_heads, rows, keys, d, &nothing)) return rc;
+  return nothing ? 0 : sequences_plan(a, device_info_for_plan().cus, INT64_MAX).workspace_bytes;
 }
 
 static int error_stats_common(adr_stream_t stream, adr_tensor_desc output, adr_tensor_desc lhs,

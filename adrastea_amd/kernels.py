@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
 import threading
 import warnings
 from dataclasses import dataclass, field
@@ -161,6 +162,176 @@ def lower_matmul(output: TensorLayout, left: TensorLayout, right: TensorLayout,
     return LoweredMatmul(*s[:4], s[4:7], s[7:10], s[10:], *tail)
 
 
+# ---- several sequences at once ---------------------------------------------------------------
+
+class RotaryLayout:
+    HALVES = 0   # value i is paired with value i + dims / 2
+    PAIRS = 1    # value 2 i with value 2 i + 1
+
+
+@dataclass(frozen=True)
+class RotaryScaling:
+    """How the frequencies base^(-2 i / dims) are changed for contexts longer than a model was trained on."""
+    kind: str = "identity"
+    parameters: Tuple[float, ...] = ()
+
+    @staticmethod
+    def Identity() -> "RotaryScaling":
+        return RotaryScaling()
+
+    @staticmethod
+    def Linear(factor: float) -> "RotaryScaling":
+        """Positions divided by `factor`."""
+        return RotaryScaling("linear", (float(factor),))
+
+    @staticmethod
+    def Base(factor: float) -> "RotaryScaling":
+        """The base grown so that the slowest pair turns `factor` times slower and the fastest as before."""
+        return RotaryScaling("base", (float(factor),))
+
+    @staticmethod
+    def Wavelength(factor: float, low: float, high: float, original: int) -> "RotaryScaling":
+        """Pairs that turn fewer than `low` times within `original` positions are slowed by `factor`, those that turn
+        more than `high` times are not, and those between are blended by their number of turns."""
+        return RotaryScaling("wavelength", (float(factor), float(low), float(high), float(original)))
+
+    @staticmethod
+    def Yarn(factor: float, original: int, fast: float = 32.0, slow: float = 1.0,
+             magnitude: Optional[float] = None) -> "RotaryScaling":
+        """A ramp over the pairs' indices, from the pair that turns `fast` times within `original` positions (kept) to
+        the one that turns `slow` times (slowed by `factor`), and the rotated values multiplied by `magnitude`
+        (default 0.1 ln(factor) + 1)."""
+        if magnitude is None:
+            magnitude = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+        return RotaryScaling("yarn", (float(factor), float(original), float(fast), float(slow), float(magnitude)))
+
+
+def rotary_frequencies(dims: int, base: float = 10000.0, scaling: RotaryScaling = RotaryScaling()):
+    """(radians a position for each of the dims / 2 pairs, magnitude), in Python's 64-bit floats."""
+    if dims < 0 or dims % 2 or not base > 0.0:
+        raise ValueError("rotary positions need an even number of values and a positive base")
+    p = scaling.parameters
+    if p and not p[0] > 0.0:
+        raise ValueError("the factor of a scaling is positive")
+    if scaling.kind == "base" and dims > 2:
+        base *= p[0] ** (dims / (dims - 2))
+    f = [base ** (-2.0 * i / dims) for i in range(dims // 2)]
+    if scaling.kind == "linear":
+        return [x / p[0] for x in f], 1.0
+    if scaling.kind == "wavelength":
+        factor, low, high, original = p
+        if not high > low:
+            raise ValueError("wavelength scaling needs high > low")
+        keep = [min(max((original * x / (2 * math.pi) - low) / (high - low), 0.0), 1.0) for x in f]
+        return [x * (k + (1.0 - k) / factor) for x, k in zip(f, keep)], 1.0
+    if scaling.kind == "yarn":
+        factor, original, fast, slow, magnitude = p
+
+        def index(turns):  # of the pair that turns so many times within the original context
+            return dims * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+        low, high = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), dims - 1)
+        slowed = [min(max((i - low) / max(high - low, 0.001), 0.0), 1.0) for i in range(dims // 2)]
+        return [x * (1.0 - s + s / factor) for x, s in zip(f, slowed)], magnitude
+    if scaling.kind not in ("identity", "base"):
+        raise ValueError(f"unknown rotary scaling {scaling.kind!r}")
+    return f, 1.0
+
+
+@dataclass(frozen=True)
+class Rotary:
+    """Rotary positions of a model: its frequencies in turns a position, on the device, made once."""
+    turns: object        # float64 tensor [dims / 2]
+    layout: int = RotaryLayout.HALVES
+    magnitude: float = 1.0
+
+    @staticmethod
+    def new(dims: int, base: float = 10000.0, layout: int = RotaryLayout.HALVES,
+            scaling: RotaryScaling = RotaryScaling()) -> "Rotary":
+        import torch
+        frequencies, magnitude = rotary_frequencies(dims, base, scaling)
+        turns = torch.tensor([f / (2 * math.pi) for f in frequencies], dtype=torch.float64).cuda()
+        return Rotary(turns, layout, magnitude)
+
+    @property
+    def _desc(self) -> _ffi.RotaryDesc:
+        import torch
+        assert self.turns.dtype == torch.float64 and self.turns.is_contiguous() and self.turns.dim() == 1
+        return _ffi.RotaryDesc(self.turns.data_ptr(), 2 * self.turns.numel(), self.layout, self.magnitude)
+
+
+_NO_ROTARY = _ffi.RotaryDesc(None, 0, 0, 1.0)
+
+
+@dataclass(frozen=True)
+class PagedCache:
+    """Keys and values of many sequences in pages: two [pages, kv_heads, page_size, d] views of the pools that
+    the program owns (a pool kept as [pages, page_size, kv_heads, d] is handed over as its permuted view)."""
+    key: TensorView
+    value: TensorView
+
+    @property
+    def _desc(self) -> _ffi.PagedCacheDesc:
+        k, v = self.key.layout, self.value.layout
+        assert len(k.dims) == 4 and k.dims == v.dims, "key and value pages are [pages, kv_heads, page_size, d] views"
+        p, h, s, d = k.dims
+        return _ffi.PagedCacheDesc(self.key.data_ptr(), self.value.data_ptr(), p, h, s, d,
+                                   *(t.strides[i] for t in (k, v) for i in (3, 2, 1, 0)))
+
+
+def _index(t, rank, what):
+    import torch
+    assert t.dtype == torch.int32 and t.dim() == rank and (t.numel() == 0 or t.stride(-1) == 1), \
+        f"{what}: an int32 tensor of rank {rank}, contiguous in its last dimension"
+    return t
+
+
+@dataclass(frozen=True)
+class PagedBatch:
+    """The sequences of one step over a paged cache: rows row_offsets[s] .. row_offsets[s + 1] - 1 belong to sequence s,
+    which has lengths[s] keys in the cache with those of this step, on the pages of table[s].  int32 tensors on the
+    device, which a program may refill from step to step (and between replays of a captured graph); longest_rows and
+    longest are what the host knows of the most rows and keys of a sequence (0: nothing), and only choose kernels."""
+    row_offsets: object  # [sequences + 1]
+    lengths: object      # [sequences]
+    table: object        # [sequences, pages of the longest]
+    longest_rows: int = 0
+    longest: int = 0
+
+    @property
+    def _desc(self) -> _ffi.PagedBatchDesc:
+        n = _index(self.lengths, 1, "lengths").shape[0]
+        assert _index(self.row_offsets, 1, "row_offsets").shape[0] == n + 1, "row_offsets has one entry more than lengths"
+        assert _index(self.table, 2, "table").shape[0] == n, "table has a row for each sequence"
+        pitch = self.table.stride(0) if n > 1 else self.table.shape[1]
+        return _ffi.PagedBatchDesc(self.row_offsets.data_ptr(), self.lengths.data_ptr(), self.table.data_ptr(), n,
+                                   self.table.shape[1], pitch, self.longest_rows, self.longest)
+
+
+@dataclass(frozen=True)
+class PackedBatch:
+    """Sequences whose rows, and whose keys, lie one behind the other (whole prompts: the same offsets twice)."""
+    row_offsets: object  # [sequences + 1]
+    key_offsets: object  # [sequences + 1]
+    longest_rows: int = 0
+    longest: int = 0
+
+    @property
+    def _desc(self) -> _ffi.PackedBatchDesc:
+        n = _index(self.row_offsets, 1, "row_offsets").shape[0]
+        assert n >= 1 and _index(self.key_offsets, 1, "key_offsets").shape[0] == n, "offsets of the same sequences"
+        return _ffi.PackedBatchDesc(self.row_offsets.data_ptr(), self.key_offsets.data_ptr(), n - 1, self.longest_rows,
+                                    self.longest)
+
+
+def _rows_view(view: TensorView, what: str):
+    """(heads, rows, d), (x, y, z) strides of a [heads, rows, d] view; rank 2: one head."""
+    dims, strides = view.layout.dims, view.layout.strides
+    assert len(dims) in (2, 3), f"{what}: a [heads, rows, d] view"
+    if len(dims) == 2:
+        return (1, *dims), (strides[1], strides[0], 0)
+    return dims, strides[::-1]
+
+
 # ---- the kernel interface ----------------------------------------------------------------------
 
 class CommonKernels:
@@ -305,6 +476,78 @@ class GpuKernels(CommonKernels):
               self._lib.adr_attention_f16_ws(*args, ws.data_ptr(), ws.numel()))
         if rc != 0:
             raise AdrasteaError(rc, "attention_f16")
+
+    # -- several sequences at once --
+    def rotary_f16(self, output, input, positions, rotary: Rotary):
+        """The rows of `input`, a [heads, rows, d] view, turned by positions[row] into `output` (which may be the same
+        view).  positions: int32 [rows]."""
+        dims, si = _rows_view(input, "input")
+        dims_out, so = _rows_view(output, "output")
+        assert dims_out == dims, "output and input have one shape"
+        assert _index(positions, 1, "positions").shape[0] == dims[1], "a position for each row"
+        rc = self._lib.adr_rotary_f16(_current_stream(), output.data_ptr(), input.data_ptr(), positions.data_ptr(),
+                                      rotary._desc, *dims, *so, *si)
+        if rc != 0:
+            raise AdrasteaError(rc, "rotary_f16")
+
+    def append_f16(self, cache: PagedCache, batch: PagedBatch, key, value, rotary: Optional[Rotary] = None,
+                   query_out=None, query=None, positions=None):
+        """The step's keys, turned, and values ([kv_heads, rows, d] views) into their pages, and its queries ([heads,
+        rows, d]) turned into `query_out`, which may be the same view.  Row j of the r of sequence s goes to
+        place lengths[s] - r + j and is turned by it, or by positions[row] (int32 [rows])."""
+        c, b = cache._desc, batch._desc
+        dims, sk = _rows_view(key, "key")
+        dims_v, sv = _rows_view(value, "value")
+        assert dims_v == dims and dims[0] == c.kv_heads and dims[2] == c.d, "key and value are [kv_heads, rows, d] views"
+        heads, sq, so = 0, (0, 0, 0), (0, 0, 0)
+        assert (query is None) == (query_out is None), "query and query_out go together"
+        if query is not None:
+            dims_q, sq = _rows_view(query, "query")
+            dims_o, so = _rows_view(query_out, "query_out")
+            heads = dims_q[0]
+            assert dims_o == dims_q and dims_q[1:] == dims[1:], "query and query_out are [heads, rows, d] views"
+        if positions is not None:
+            assert _index(positions, 1, "positions").shape[0] == dims[1], "a position for each row"
+        rc = self._lib.adr_append_f16(
+            _current_stream(), c, b, key.data_ptr(), value.data_ptr(), query_out.data_ptr() if heads else None,
+            query.data_ptr() if heads else None, positions.data_ptr() if positions is not None else None,
+            rotary._desc if rotary is not None else _NO_ROTARY, heads, dims[1], *sk, *sv, *so, *sq)
+        if rc != 0:
+            raise AdrasteaError(rc, "append_f16")
+
+    def attention_paged_f16(self, output, query, cache: PagedCache, batch: PagedBatch, scale: float,
+                            temperature: float = 1.0, mask: int = MatmulMask.CAUSAL):
+        """Attention of the step's rows ([heads, rows, d] views) over the cache: query head h reads key head
+        h / (heads / kv_heads), and under the mask the last row of a sequence sees all its keys."""
+        c, b = cache._desc, batch._desc
+        dims, sq = _rows_view(query, "query")
+        dims_o, so = _rows_view(output, "output")
+        assert dims_o == dims and dims[2] == c.d, "output and query are [heads, rows, d] views"
+        args = (_current_stream(), output.data_ptr(), query.data_ptr(), c, b, dims[0], dims[1], *so, *sq, float(scale),
+                float(temperature), int(mask))
+        ws = self._workspace
+        rc = (self._lib.adr_attention_paged_f16(*args) if ws is None else
+              self._lib.adr_attention_paged_f16_ws(*args, ws.data_ptr(), ws.numel()))
+        if rc != 0:
+            raise AdrasteaError(rc, "attention_paged_f16")
+
+    def attention_packed_f16(self, output, query, key, value, batch: PackedBatch, scale: float,
+                             temperature: float = 1.0, mask: int = MatmulMask.CAUSAL):
+        """Attention of packed rows ([heads, rows, d] views) over packed keys and values ([kv_heads, keys, d])."""
+        dims, sq = _rows_view(query, "query")
+        dims_o, so = _rows_view(output, "output")
+        dims_k, sk = _rows_view(key, "key")
+        dims_v, sv = _rows_view(value, "value")
+        assert dims_o == dims, "output and query are [heads, rows, d] views"
+        assert dims_v == dims_k and dims_k[2] == dims[2], "key and value are [kv_heads, keys, d] views"
+        args = (_current_stream(), output.data_ptr(), query.data_ptr(), key.data_ptr(), value.data_ptr(), batch._desc,
+                dims[0], dims_k[0], dims[1], dims_k[1], dims[2], *so, *sq, *sk, *sv, float(scale), float(temperature),
+                int(mask))
+        ws = self._workspace
+        rc = (self._lib.adr_attention_packed_f16(*args) if ws is None else
+              self._lib.adr_attention_packed_f16_ws(*args, ws.data_ptr(), ws.numel()))
+        if rc != 0:
+            raise AdrasteaError(rc, "attention_packed_f16")
 
     def _error_stats(self, fn, what, output, lhs, rhs):
         if _native is not None:
@@ -515,6 +758,18 @@ class MatmulTracer(CommonKernels):
     def attention_f16(self, output, query, key, value, scale, temperature=1.0,
                       mask=MatmulMask.NONE):
         self.inner.attention_f16(output, query, key, value, scale, temperature, mask)
+
+    def rotary_f16(self, output, input, positions, rotary):
+        self.inner.rotary_f16(output, input, positions, rotary)
+
+    def append_f16(self, cache, batch, key, value, rotary=None, query_out=None, query=None, positions=None):
+        self.inner.append_f16(cache, batch, key, value, rotary, query_out, query, positions)
+
+    def attention_paged_f16(self, output, query, cache, batch, scale, temperature=1.0, mask=MatmulMask.CAUSAL):
+        self.inner.attention_paged_f16(output, query, cache, batch, scale, temperature, mask)
+
+    def attention_packed_f16(self, output, query, key, value, batch, scale, temperature=1.0, mask=MatmulMask.CAUSAL):
+        self.inner.attention_packed_f16(output, query, key, value, batch, scale, temperature, mask)
 
     def error_stats_f16(self, output, lhs, rhs):
         self.inner.error_stats_f16(output, lhs, rhs)            # forwarded (kernels.rs:349-358)

@@ -10,8 +10,8 @@
  * with any other device current, every launching entry point returns ADR_EUNSUPPORTED_DEVICE
  * (the device's architecture, compute-unit and die counts are queried once per device and
  * cached).  Beside that cache the library keeps one piece of state: the pool of workspaces that
- * adr_matmul_f16, adr_matmul_nt_f16, adr_attention_f16 and (on request) adr_matmul_nt_fp16u8 draw
- * from, grown on demand and given back through adr_release_held_workspace*
+ * adr_matmul_f16, adr_matmul_nt_f16, adr_attention_f16, adr_attention_paged_f16,
+ * adr_attention_packed_f16 and (on request) adr_matmul_nt_fp16u8 draw from, grown on demand and given back through adr_release_held_workspace*
  * (adr_set_held_workspace_limit below; 0 switches it off).
  *
  * fp16 data is passed as uint16_t bit patterns (Rust `half::f16` is repr(transparent) u16).
@@ -384,6 +384,140 @@ int64_t adr_attention_f16_workspace_bytes(int32_t heads, int32_t m, int32_t n, i
                                           int32_t stride_oy, int32_t stride_oz, int32_t stride_qx, int32_t stride_qy,
                                           int32_t stride_qz, int32_t stride_kx, int32_t stride_ky, int32_t stride_kz,
                                           int32_t stride_vx, int32_t stride_vy, int32_t stride_vz, uint32_t mask);
+
+/*
+ * Serving several sequences at once (no counterpart in the reference, which runs one sequence
+ * without a cache: llama.rs:456-483).  Four operators that a step of a serving loop calls one after
+ * the other: rotary positions, the cache's new keys and values, and attention over the cache or over
+ * packed prompts.  What changes from step to step -- offsets, lengths, page numbers, positions -- is
+ * device memory, so that one captured graph serves many steps; sizes are the host's.
+ *
+ * Rows are packed: sequence s has rows row_offsets[s] .. row_offsets[s + 1] - 1 of the [heads, rows, d]
+ * views (strides x = dim -1, y = dim -2, z = dim -3 as above, any strides, negative ones included).
+ * Offsets are clamped to 0 .. rows; a sequence may have no rows; rows in front of the first and
+ * behind the last sequence are neither read nor written.
+ *
+ * adr_paged_cache: key and value pages as [pages, kv_heads, page_size, d] views of one pool each,
+ * strides in elements (x value, y slot, z head, p page), 64 bits.
+ * adr_paged_batch: sequence s has lengths[s] keys in the cache, those of its rows in this call
+ * included; key x lies in page table[s * table_pitch + x / page_size], slot x % page_size.  Lengths are
+ * taken as at most table_width * page_size and at least 0.  Entries beyond a sequence's length are not
+ * read.  longest_rows and longest are the largest number of rows and keys of any sequence as far as the
+ * host knows (0: unknown): they choose kernels and nothing else, every result is right whatever they say.
+ */
+typedef struct adr_paged_cache {
+  uint16_t* key;
+  uint16_t* value;
+  int32_t pages, kv_heads, page_size, d;
+  int64_t stride_kx, stride_ky, stride_kz, stride_kp;
+  int64_t stride_vx, stride_vy, stride_vz, stride_vp;
+} adr_paged_cache;
+typedef struct adr_paged_batch {
+  const int32_t* row_offsets; /* [sequences + 1] */
+  const int32_t* lengths;     /* [sequences] */
+  const int32_t* table;       /* [sequences, table_pitch], of which table_width entries a row are used */
+  int32_t sequences, table_width, table_pitch;
+  int32_t longest_rows, longest;
+} adr_paged_batch;
+/* Keys packed like the rows: sequence s has keys key_offsets[s] .. key_offsets[s + 1] - 1. */
+typedef struct adr_packed_batch {
+  const int32_t* row_offsets; /* [sequences + 1] */
+  const int32_t* key_offsets; /* [sequences + 1] */
+  int32_t sequences;
+  int32_t longest_rows, longest;
+} adr_packed_batch;
+
+/*
+ * Rotary positions: the first `dims` values of each head (the others pass) are turned in pairs, pair i
+ * by position * turns[i] full turns, and multiplied by `magnitude`:
+ *   (a, b) -> magnitude * (a cos - b sin, a sin + b cos).
+ * ADR_ROTARY_HALVES: a = x[i], b = x[i + dims / 2]; ADR_ROTARY_PAIRS: a = x[2i], b = x[2i + 1].
+ * `turns` is device memory, [dims / 2] doubles: frequency / (2 pi), with whatever scaling for long
+ * contexts the model asks for.  The angle is a 64-bit product reduced by its whole turns, so that
+ * positions of seven digits are as exact as small ones; negative positions turn back.  dims even, 0 .. d, at
+ * most ADR_ROTARY_MAX_DIMS.  fp32 arithmetic, one rounding.
+ * adr_rotary_f16: `output` and `input` are [heads, rows, d] views, and may be the same view;
+ * positions [rows].
+ */
+enum { ADR_ROTARY_HALVES = 0, ADR_ROTARY_PAIRS = 1 };
+#define ADR_ROTARY_MAX_DIMS 512
+typedef struct adr_rotary {
+  const double* turns;
+  int32_t dims;
+  uint32_t layout;
+  float magnitude;
+} adr_rotary;
+int adr_rotary_f16(adr_stream_t stream, uint16_t* output, const uint16_t* input, const int32_t* positions,
+                   adr_rotary rotary, int32_t heads, int32_t rows, int32_t d, int32_t stride_ox, int32_t stride_oy,
+                   int32_t stride_oz, int32_t stride_ix, int32_t stride_iy, int32_t stride_iz);
+
+/*
+ * A step's new keys and values into the cache: row j of sequence s, of its r rows, is key
+ * x = lengths[s] - r + j; `key` goes there rotated, `value` as it is ([kv_heads, rows, d] views).  `query`
+ * ([heads, rows, d]) is rotated into `query_out`, which may be the same view; both may be null.  The angle
+ * is that of position x, or of positions[row] where `positions` is not null.  rotary.dims == 0: nothing is
+ * turned.  Keys at x < 0, beyond the table, or on a page outside 0 .. pages - 1 are not written (so a
+ * table entry of -1 keeps a padded row out of the cache); the queries of such rows are written all the
+ * same.  Two rows that name the same slot leave either's key.
+ */
+int adr_append_f16(adr_stream_t stream, adr_paged_cache cache, adr_paged_batch batch, const uint16_t* key,
+                   const uint16_t* value, uint16_t* query_out, const uint16_t* query, const int32_t* positions,
+                   adr_rotary rotary, int32_t heads, int32_t rows, int32_t stride_kx, int32_t stride_ky,
+                   int32_t stride_kz, int32_t stride_vx, int32_t stride_vy, int32_t stride_vz, int32_t stride_ox,
+                   int32_t stride_oy, int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz);
+
+/*
+ * Attention of new rows over the cache: with r rows and n = lengths[s] keys, row j of sequence s and query
+ * head h
+ *   out[h, row, :] = sum_x softmax_x( scale * <query[h, row, :], key[x]> / temp ) * value[x],
+ * over the keys of kv head h / (heads / kv_heads), x <= j + n - r under ADR_MASK_CAUSAL (the last row
+ * sees all keys) and all x under ADR_MASK_NONE.  A row that sees no key, or whose scores are all -inf,
+ * becomes zeros; keys that a row does not see, and slots behind the last key, never reach it, whatever they
+ * hold (infinities and NaN included).  A key on a page outside 0 .. pages - 1 counts as NaN for the rows
+ * that see it.  Scores, softmax and sums in fp32; probabilities are rounded to fp16 for the matrix cores.
+ * d 1 .. 256, scale > 0, temp > 0 (ADR_EUNSUPPORTED_LAYOUT beyond), heads a multiple of kv_heads.  The fast
+ * kernels take d a multiple of 8 up to 128, x strides 1, the others multiples of 8 and not negative, slots at
+ * least d apart and less than 2^24, 16-byte aligned pointers, pages of 16, 32, 64 ... slots; everything else runs on
+ * a kernel of one wavefront per row.
+ * Where rows are few the keys of a sequence are shared by several workgroups whose parts pass through
+ * scratch memory and are added by a second launch, in a fixed order: from the library's pool
+ * (adr_set_held_workspace_limit; under capture, or where the pool cannot be used, keys are not shared), or
+ * in the _ws form from the caller's `workspace` (16-byte aligned), eagerly and under capture alike.  With less than
+ * _workspace_bytes reports they are cut into fewer parts, with 0 not at all.  The workspace carries nothing from call to
+ * call; calls (and graphs) sharing one must not overlap in time.
+ */
+int adr_attention_paged_f16(adr_stream_t stream, uint16_t* output, const uint16_t* query, adr_paged_cache cache,
+                            adr_paged_batch batch, int32_t heads, int32_t rows, int32_t stride_ox, int32_t stride_oy,
+                            int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz, float scale,
+                            float temp, uint32_t mask);
+int adr_attention_paged_f16_ws(adr_stream_t stream, uint16_t* output, const uint16_t* query, adr_paged_cache cache,
+                               adr_paged_batch batch, int32_t heads, int32_t rows, int32_t stride_ox, int32_t stride_oy,
+                               int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz, float scale,
+                               float temp, uint32_t mask, void* workspace, int64_t workspace_bytes);
+/* Bytes (>= 0; 0: no keys would be shared) or a negative ADR_E* code; reads no device memory. */
+int64_t adr_attention_paged_f16_workspace_bytes(adr_paged_cache cache, adr_paged_batch batch, int32_t heads,
+                                                int32_t rows);
+
+/*
+ * The same over keys and values packed like the rows: `key` and `value` are [kv_heads, keys, d] views.  Whole
+ * prompts have key_offsets equal to row_offsets; more keys than rows in a sequence are its past, seen
+ * by all its rows.  Offsets are clamped to 0 .. keys.
+ */
+int adr_attention_packed_f16(adr_stream_t stream, uint16_t* output, const uint16_t* query, const uint16_t* key,
+                             const uint16_t* value, adr_packed_batch batch, int32_t heads, int32_t kv_heads,
+                             int32_t rows, int32_t keys, int32_t d, int32_t stride_ox, int32_t stride_oy,
+                             int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz,
+                             int32_t stride_kx, int32_t stride_ky, int32_t stride_kz, int32_t stride_vx,
+                             int32_t stride_vy, int32_t stride_vz, float scale, float temp, uint32_t mask);
+int adr_attention_packed_f16_ws(adr_stream_t stream, uint16_t* output, const uint16_t* query, const uint16_t* key,
+                                const uint16_t* value, adr_packed_batch batch, int32_t heads, int32_t kv_heads,
+                                int32_t rows, int32_t keys, int32_t d, int32_t stride_ox, int32_t stride_oy,
+                                int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz,
+                                int32_t stride_kx, int32_t stride_ky, int32_t stride_kz, int32_t stride_vx,
+                                int32_t stride_vy, int32_t stride_vz, float scale, float temp, uint32_t mask,
+                                void* workspace, int64_t workspace_bytes);
+int64_t adr_attention_packed_f16_workspace_bytes(adr_packed_batch batch, int32_t heads, int32_t kv_heads, int32_t rows,
+                                                 int32_t keys, int32_t d);
 
 /*
  * Diagnostics (no counterpart in the reference).
