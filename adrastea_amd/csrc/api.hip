@@ -905,7 +905,7 @@ int paged_args(SequencesArgs& a, const adr_paged_cache& c, const adr_paged_batch
 int packed_args(SequencesArgs& a, const adr_packed_batch& b, int32_t heads, int32_t kv_heads, int32_t rows, int32_t keys,
                 int32_t d, bool* nothing) {
   if (int rc = validate_rows(heads, kv_heads, rows, d, b.sequences, nothing)) return rc;
-  if (keys < 0) return ADR_EINVAL_SHAPE;
+  if (keys < 0 || keys > MOST_KEYS) return ADR_EINVAL_SHAPE;
   if (*nothing) return ADR_OK;
   a.row_offsets = b.row_offsets, a.keys_of = b.key_offsets;
   a.sequences = b.sequences, a.rows = rows, a.keys = keys;
@@ -1045,6 +1045,7 @@ int64_t adr_attention_paged_f16_workspace_bytes(adr_paged_cache cache, adr_paged
   SequencesArgs a = {};
   bool nothing;
   if (int rc = paged_args(a, cache, batch, heads, rows, &nothing)) return rc;
+  a.so_x = a.sq_x = 1;
   return nothing ? 0 : sequences_plan(a, device_info_for_plan().cus, INT64_MAX).workspace_bytes;
 }
 
@@ -1079,6 +1080,8 @@ int64_t adr_attention_packed_f16_workspace_bytes(adr_packed_batch batch, int32_t
   SequencesArgs a = {};
   bool nothing;
   if (int rc = packed_args(a, batch, heads, kv_heads, rows, keys, d, &nothing)) return rc;
+  a.so_x = a.sq_x = 1;
+  a.sk = a.sv = {1, d, 0, 0};
   return nothing ? 0 : sequences_plan(a, device_info_for_plan().cus, INT64_MAX).workspace_bytes;
 }
 

@@ -27,6 +27,8 @@ struct RotaryArgs {
 };
 hipError_t launch_rotary(hipStream_t stream, const RotaryArgs& a);
 
+constexpr int MOST_KEYS = 1 << 30;  // of a sequence (a workgroup's tiles beyond the last key still count in 31 bits)
+
 // Attention of packed rows over pages or packed keys (table null).
 struct SequencesArgs {
   half_t* out;
@@ -45,7 +47,11 @@ struct SequencesArgs {
   float c;             // scale * log2(e) / temperature
   uint32_t mask;
 };
+// Which kernel, and how the keys are shared over workgroups (attention_sequences.hip).
 struct SequencesPlan {
+  enum Kind { ANY_LAYOUT, FEW_ROWS, TILES } kind;
+  int parts;      // of all sequences' work, for each key head; 0: no keys are shared
+  int min_steps;  // key tiles that a workgroup has at least, where keys are shared
   int64_t workspace_bytes;
 };
 SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail);

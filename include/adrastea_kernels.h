@@ -499,7 +499,7 @@ int64_t adr_attention_paged_f16_workspace_bytes(adr_paged_cache cache, adr_paged
                                                 int32_t rows);
 
 /*
- * The same over keys and values packed like the rows: `key` and `value` are [kv_heads, keys, d] views.  Whole
+ * The same over at most 2^30 keys and values packed like the rows: `key` and `value` are [kv_heads, keys, d] views.  Whole
  * prompts have key_offsets equal to row_offsets; more keys than rows in a sequence are its past, seen
  * by all its rows.  Offsets are clamped to 0 .. keys.
  */
