@@ -141,6 +141,8 @@ struct Piece {
   int slot;           // of the first part's results
 };
 
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 __device__ __forceinline__ int add_scan(int v) {  // inclusive, over the lanes of a wavefront
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
   v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
@@ -182,7 +184,7 @@ __device__ __forceinline__ bool find_piece(const SequencesArgs& a, const Share& 
       load(base);
     }
     for (int i = 1; i < 64; i <<= 1) work += __shfl_xor(work, i);
-    most = max(share.min_steps, (int)fminf(ceilf(work / (float)share.parts), 1.0e9f));
+    most = uniform(max(share.min_steps, (int)fminf(ceilf(work / (float)share.parts), 1.0e9f)));
     if (a.sequences > 64 * EACH) load(0);
   }
   int slot = 0;
@@ -200,27 +202,28 @@ __device__ __forceinline__ bool find_piece(const SequencesArgs& a, const Share& 
     const uint64_t behind = __ballot(upto > index);
     if (behind) {
       const int at = __builtin_ctzll(behind);
-      int i = index - (__shfl(upto, at) - __shfl(sum, at));
-      slot += __shfl(slots_upto, at) - __shfl(slots, at);
+      int i = index - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(sum, at));
+      slot += __builtin_amdgcn_readlane(slots_upto, at) - __builtin_amdgcn_readlane(slots, at);
 #pragma unroll
       for (int e = 0; e < EACH; e++) {
-        const int n = __shfl(count[e], at), p = __shfl(parts[e], at), b = __shfl(blocks[e], at);
+        const int n = __builtin_amdgcn_readlane(count[e], at), p = __builtin_amdgcn_readlane(parts[e], at), b = __builtin_amdgcn_readlane(blocks[e], at);
         if (i < n) {
           // (the last blocks first: under the mask they have the most keys)
           const int block = b - 1 - (DIVIDED ? i : i / p);
-          piece.q = sequence_at(a, base + at * EACH + e);
-          piece.block = block;
-          piece.parts = p;
-          piece.part = DIVIDED ? 0 : i % p;
-          piece.slot = slot + (b - 1 - block) * p;
+          const Sequence q = sequence_at(a, base + at * EACH + e);
+          piece.q = {uniform(q.index), uniform(q.row0), uniform(q.rows), uniform(q.key0), uniform(q.keys)};
+          piece.block = uniform(block);
+          piece.parts = uniform(p);
+          piece.part = uniform(DIVIDED ? 0 : i % p);
+          piece.slot = uniform(slot + (b - 1 - block) * p);
           return true;
         }
         i -= n;
         if (p > 1) slot += b * p;
       }
     }
-    index -= __shfl(upto, 63);
-    slot += __shfl(slots_upto, 63);
+    index -= __builtin_amdgcn_readlane(upto, 63);
+    slot += __builtin_amdgcn_readlane(slots_upto, 63);
     base += 64 * EACH;
     if (base < a.sequences) load(base);
   }
@@ -230,6 +233,13 @@ __device__ __forceinline__ bool find_piece(const SequencesArgs& a, const Share& 
 // One past the last key that some row of the block sees, and of one row.
 __device__ __forceinline__ int end_of_row(const SequencesArgs& a, const Sequence& q, int j) {
   return a.mask == ADR_MASK_CAUSAL ? clamp_to(j + q.keys - q.rows + 1, q.keys) : q.keys;
+}
+
+
+// A transfer's descriptor, in scalar registers: `bytes` from an address on.
+__device__ __forceinline__ u32x4_t descriptor(uint64_t p, int bytes) {
+  return u32x4_t{(uint32_t)uniform((int)(uint32_t)p), (uint32_t)uniform((int)((uint32_t)(p >> 32) & 0xffffu)),
+                 (uint32_t)uniform(bytes), 0x00020000u};
 }
 
 // Pages of 2^shift slots, 16 at least: 16 keys from a multiple of 16 on lie on one page, so that a transfer of 16 rows
@@ -261,17 +271,14 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Sequence
   const int hk = blockIdx.x % a.kv_heads;
   Piece pc;
   if (!find_piece<ROWS, KEYS, false>(a, share, blockIdx.x / a.kv_heads, lane, pc)) return;
-  const Sequence q = {__builtin_amdgcn_readfirstlane(pc.q.index), __builtin_amdgcn_readfirstlane(pc.q.row0),
-                      __builtin_amdgcn_readfirstlane(pc.q.rows), __builtin_amdgcn_readfirstlane(pc.q.key0),
-                      __builtin_amdgcn_readfirstlane(pc.q.keys)};
-  const int block = __builtin_amdgcn_readfirstlane(pc.block), part = __builtin_amdgcn_readfirstlane(pc.part),
-            parts = __builtin_amdgcn_readfirstlane(pc.parts), slot0 = __builtin_amdgcn_readfirstlane(pc.slot);
+  const Sequence q = pc.q;
+  const int block = pc.block, part = pc.part, parts = pc.parts, slot0 = pc.slot;
   const int rows = min(ROWS, q.rows * a.group - block * ROWS);          // of the block
   const int list_row = block * ROWS + min(frow, rows - 1), row = list_row / a.group, gh = list_row - row * a.group;
 
-  const int last_end = end_of_row(a, q, (block * ROWS + rows - 1) / a.group);  // of the block's last row
+  const int last_end = uniform(end_of_row(a, q, (block * ROWS + rows - 1) / a.group));  // of the block's last row
   const int all = (last_end + KEYS - 1) / KEYS;
-  const int tile0 = (int)((int64_t)all * part / parts), tile1 = (int)((int64_t)all * (part + 1) / parts);
+  const int tile0 = uniform((int)((int64_t)all * part / parts)), tile1 = uniform((int)((int64_t)all * (part + 1) / parts));
   const int row_end = min(last_end, tile1 * KEYS);
   const int tiles = max(0, (tile1 - tile0 - w + WAVES - 1) / WAVES);  // of this wavefront: tile0 + w + WAVES i
 
@@ -317,10 +324,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Sequence
         vo = key * a.sv.y;
       }
       const uint64_t pk = (uint64_t)(K + ko) - BIAS, pv = (uint64_t)(V + vo) - BIAS;
-      const u32x4_t dk = {(uint32_t)pk, (uint32_t)(pk >> 32) & 0xffffu,
-                          left > 0 ? (uint32_t)(((left - 1) * (int)a.sk.y + a.d) * 2 + BIAS) : 0u, 0x00020000u};
-      const u32x4_t dv = {(uint32_t)pv, (uint32_t)(pv >> 32) & 0xffffu,
-                          left > 0 ? (uint32_t)(((left - 1) * (int)a.sv.y + a.d) * 2 + BIAS) : 0u, 0x00020000u};
+      const u32x4_t dk = descriptor(pk, left > 0 ? ((left - 1) * (int)a.sk.y + a.d) * 2 + BIAS : 0);
+      const u32x4_t dv = descriptor(pv, left > 0 ? ((left - 1) * (int)a.sv.y + a.d) * 2 + BIAS : 0);
 #pragma unroll
       for (int j = 0; j < NI / 2; j += 2)
         dma_buffer_pair<0>(lds0 + (i & 1) * TILE + (h * (NI / 2) + j) * 1024, koff[j], koff[j + 1], dk);
@@ -496,6 +501,479 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Sequence
   }
 }
 
+// ---- many rows: prompts, and their pieces over what is in the cache ---------------------------------------
+//
+// A workgroup takes a block of 128 rows, wavefront w of it rows 32 w ... 32 w + 31 of the list, and walks tiles of 64
+// keys, double buffered in LDS by transfers from global memory; two workgroups share a compute unit.  Per tile a
+// wavefront computes S^T = K Q^T (MFMA 32x32x16, Q fragments resident in registers), so that every lane holds scores
+// of one row: the running maximum and sum are in-lane reductions plus one exchange with lane ^ 32, and a lane's own
+// last key is all that the mask needs.  The probabilities, narrowed to fp16, are already in the operand layout of the
+// second product O^T = V^T P^T, whose V^T fragments come from the row-major V tile by transposing LDS reads.  The two
+// products and the softmax between them are one instruction stream, as in attention_fwd_kernel (attention.hip, which
+// explains the arrangement): scores of tile i + 1 on the matrix cores beside the exponentials of tile i, P.V of tile i
+// beside the maximum of tile i + 1.  What is different here is where rows and keys come from: the heads of a group
+// share the block, so that a key row is read once for all of them and the part of a tile that the mask leaves empty
+// is 1 / group as wide, and each wavefront's 16 key rows of a tile have a base address of their own, on a page.
+template <int HD, bool PAGED>
+__global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a, Share share, Pages pages) {
+  constexpr int CPR = HD / 8, KEYS = 64, ROWS = 128;
+  constexpr int TILE = KEYS * HD * 2;  // bytes of one K or V tile
+  constexpr int NI = TILE / 1024 / 4;  // transfers per wavefront and tile: 16 rows
+  constexpr int DS = HD / 16;          // MFMA k-steps over the head dimension
+  constexpr int DT = HD / 32;          // 32-wide output column tiles
+  constexpr int ROWB = HD * 2;         // bytes per tile row
+  constexpr int BIAS = NI * 1024;      // bytes that descriptors start ahead, so that no offset is negative
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];  // K0 K1 V0 V1
+
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int frow = lane & 31, g = lane >> 5;
+  const bool causal = a.mask == ADR_MASK_CAUSAL;
+  // Consecutive workgroups go to different dies; where the key heads divide evenly, a die takes its share of them, so
+  // that the blocks which read the same keys meet in one L2.
+  int hk, index;
+  if (a.kv_heads % 8 == 0) {
+    const int each = a.kv_heads >> 3, seq = blockIdx.x >> 3;
+    hk = (blockIdx.x & 7) * each + seq % each;
+    index = seq / each;
+  } else {
+    hk = blockIdx.x % a.kv_heads;
+    index = blockIdx.x / a.kv_heads;
+  }
+  Piece pc;
+  if (!find_piece<ROWS, KEYS, false>(a, share, index, lane, pc)) return;
+  const Sequence q = pc.q;
+  const int block = pc.block, part = pc.part, parts = pc.parts, slot0 = pc.slot;
+  const int rows = min(ROWS, q.rows * a.group - block * ROWS);  // of the block
+  const int wave_rows = min(32, rows - w * 32);                 // of the wavefront (may be negative)
+  const int list0 = block * ROWS + w * 32;
+  // (lanes without a row of their own compute the block's last one)
+  const int list_row = block * ROWS + min(w * 32 + frow, rows - 1), row = list_row / a.group, gh = list_row - row * a.group;
+  const int lane_end = end_of_row(a, q, row);
+
+  const int last_end = uniform(end_of_row(a, q, (block * ROWS + rows - 1) / a.group));
+  const int all = (last_end + KEYS - 1) / KEYS;
+  const int tile0 = uniform((int)((int64_t)all * part / parts));
+  const int steps = uniform((int)((int64_t)all * (part + 1) / parts)) - tile0;
+  const int row_end = min(last_end, (tile0 + steps) * KEYS);
+  // Tiles that this wavefront computes: none without rows, none whose first key lies beyond its last row's.
+  int active = 0, first_edge = 0;
+  if (wave_rows > 0) {
+    active = uniform(clamp_to((end_of_row(a, q, (list0 + wave_rows - 1) / a.group) + KEYS - 1) / KEYS - tile0, steps));
+    // the first of them with keys that some row of the wavefront must not see
+    first_edge = uniform(end_of_row(a, q, list0 / a.group)) / KEYS - tile0;
+  }
+
+  const uint32_t lds0 = (uint32_t)(uintptr_t)ADR_LDS_PTR(smem);
+  const unsigned char* const sm = smem;
+  // Wavefront w transfers rows 16 w ... 16 w + 15 of a tile, 1 KiB at a time: byte offsets of a lane's chunks in those
+  // rows, less the j KiB that the instruction adds; chunks behind the head dimension come as zeros.
+  uint32_t koff[NI], voff[NI];
+#pragma unroll
+  for (int j = 0; j < NI; j++) {
+    int krow, kc;
+    k_chunk_inv<CPR>(j * 64 + lane, krow, kc);
+    const int vrow = (j * 64 + lane) / CPR, vc = (lane % CPR) ^ v_swz<CPR>(vrow);
+    koff[j] = kc * 8 < a.d ? (uint32_t)((krow * (int)a.sk.y + kc * 8) * 2 + BIAS - j * 1024) : 0x7fff0000u;
+    voff[j] = vc * 8 < a.d ? (uint32_t)((vrow * (int)a.sv.y + vc * 8) * 2 + BIAS - j * 1024) : 0x7fff0000u;
+  }
+  // The wavefront's next 16 key and value rows: base address, bytes from there to the last key (0 behind it), and the
+  // pages of 64 tiles at a time, a lane to each.
+  struct Next {
+    uint64_t base, p;
+    int64_t page_stride;
+    int bytes, key, stride, page;
+  };
+  bool lost = false;  // a key's page is not in the cache
+  auto place = [&](Next& t) __attribute__((always_inline)) {
+    const int n = ((t.key - 16 * w) >> 6) - tile0;
+    int left = min(row_end - t.key, 16);
+    if constexpr (PAGED) {
+      if ((n & 63) == 0) {
+        const int key = t.key + lane * KEYS;
+        t.page = 0;
+        if (key < row_end) {
+          t.page = a.table[(int64_t)q.index * a.table_pitch + (key >> pages.shift)];
+          if (t.page < 0 || t.page >= a.pages) lost = true, t.page = -1;
+        }
+      }
+      const int p = __builtin_amdgcn_readlane(t.page, n & 63), slot = t.key & ((1 << pages.shift) - 1);
+      if (p < 0) left = 0;
+      t.p = t.base + 2 * (p * t.page_stride + slot * (int64_t)t.stride);
+    } else {
+      t.p = t.base + 2 * (t.key * (int64_t)t.stride);
+    }
+    t.bytes = left > 0 ? ((left - 1) * t.stride + a.d) * 2 + BIAS : 0;
+  };
+  auto first_tile = [&](const half_t* base, int64_t stride, int64_t page_stride) __attribute__((always_inline)) {
+    Next t;
+    t.base = (uint64_t)(base + (PAGED ? 0 : q.key0 * stride)) - BIAS;
+    t.page_stride = page_stride;
+    t.stride = (int)stride;
+    t.key = tile0 * KEYS + 16 * w;
+    t.page = 0;
+    place(t);
+    return t;
+  };
+  half8_t qf[DS];  // (operand B of S^T = K Q^T: lane -> row frow, head-dimension group g)
+  const half_t* const qrow = a.q + (int64_t)(hk * a.group + gh) * a.sq_z + (int64_t)(q.row0 + row) * a.sq_y + g * 8;
+#pragma unroll
+  for (int ds = 0; ds < DS; ds++) {
+    qf[ds] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+    if (ds * 16 + g * 8 < a.d) qf[ds] = *(const half8_t*)(qrow + ds * 16);
+  }
+  Next nk = first_tile(a.k + hk * a.sk.z, a.sk.y, a.sk.p), nv = first_tile(a.v + hk * a.sv.z, a.sv.y, a.sv.p);
+  auto advance = [&](Next& t) __attribute__((always_inline)) {
+    t.key += KEYS;
+    place(t);
+  };
+  // Transfers 2 j and 2 j + 1 of the NI that bring a tile into buffer `buf` (0, 1: K; 2, 3: V).
+  auto transfer = [&](const Next& t, auto is_k, int buf, auto pair) __attribute__((always_inline)) {
+    constexpr int J = 2 * decltype(pair)::value;
+    const uint32_t dst = lds0 + w * (NI * 1024) + buf * TILE;
+    const u32x4_t desc = descriptor(t.p, t.bytes);
+    if constexpr (decltype(is_k)::value) dma_buffer_pair<J>(dst, koff[J], koff[J + 1], desc);
+    else dma_buffer_pair<J>(dst, voff[J], voff[J + 1], desc);
+  };
+  const std::true_type is_k{};
+  const std::false_type is_v{};
+  const std::integral_constant<int, 0> pair0{};
+  const std::integral_constant<int, NI / 2 - 1> pair1{};  // (the last pair; HD = 64 has one)
+  auto tile_transfers = [&](Next& t, auto k, int buf) __attribute__((always_inline)) {
+    transfer(t, k, buf, pair0);
+    if constexpr (NI > 2) transfer(t, k, buf, pair1);
+    advance(t);
+  };
+  // What is waited for at the end of each half: all transfers but those issued in it.
+  auto wait_landed = [&]() __attribute__((always_inline)) { wait_vm<NI>(); };
+
+  tile_transfers(nk, is_k, 0);
+  tile_transfers(nk, is_k, 1);
+  // LDS fragment offsets.  K: lane -> tile row frow (+32), chunk 2*ds + g.
+  int offK[DS];
+#pragma unroll
+  for (int ds = 0; ds < DS; ds++) offK[ds] = k_chunk_off<CPR>(frow, ds * 2 + g);
+#pragma unroll
+  for (int ds = 0; ds < DS; ds++) asm volatile("" : "+v"(qf[ds]));
+  wait_vm<NI>();  // the first K tile has landed
+  // V (transposing read): in each group of 16 lanes, lanes 4r..4r+3 address 16 consecutive halves of tile row r, and
+  // lane i of the group receives column i of that 4 x 16 block.  Group b = (lane / 16) % 2 takes columns 16b.. of the
+  // 32-column tile, g the rows 4g..4g+3.
+  int offV[DT];
+  {
+    const int s = lane & 15, b = (lane >> 4) & 1, r = s >> 2;
+    const int row = 4 * g + r;  // + 32*kt + 16*t + 8*h, all multiples of 8: row & 3 == r
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++) {
+      const int chunk = 4 * dt + 2 * b + ((s & 3) >> 1);
+      offV[dt] = row * ROWB + ((chunk ^ v_swz<CPR>(row)) << 4) + (s & 1) * 8;
+    }
+  }
+
+  float16_t o[DT], sa[2], sb[2];  // sums of P.V; scores of two tiles in turn
+  u32x4_t pf[2][2];                 // probabilities, two to a register
+#pragma unroll
+  for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) o[dt][r] = 0.0f;
+  float m_run = NO_SCORE, l_run = 0.0f;  // running maximum (log2 units) and this lane's sum
+
+  typedef short short4_t __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) short4_t lds_short4_t;
+  // A half tile is NG groups of four MFMAs.  A group's fragments are read a group ahead, and used in
+  // the opposite order, so that one wait covers all four.
+  constexpr int NG = DS / 2;
+  half8_t kf[NG][4], vf[NG][4];
+
+  auto read_k = [&](const unsigned char* cK, int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) kf[c][j] = *(const half8_t*)(cK + offK[2 * c + (j >> 1)] + (j & 1) * 32 * ROWB);
+  };
+  // which of the products with V the j-th of group c is: keys 32 kt + 16 t ..., columns 32 dt ...
+  auto pv_of = [](int c, int j, int& kt, int& t, int& dt) __attribute__((always_inline)) {
+    const int p = 4 * c + j;
+    kt = p / (2 * DT), t = p / DT % 2, dt = p % DT;
+  };
+  auto read_v = [&](const unsigned char* cV, int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      int kt, t, dt;
+      pv_of(c, j, kt, t, dt);
+      const unsigned char* p0 = cV + offV[dt] + (32 * kt + 16 * t) * ROWB;
+      const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)ADR_LDS_PTR(p0));
+      const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)ADR_LDS_PTR(p0 + 8 * ROWB));
+      vf[c][j] = __builtin_shufflevector(__builtin_bit_cast(half4_t, lo), __builtin_bit_cast(half4_t, hi),
+                                         0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  };
+
+  // First half of tile i: the scores of tile i + 1 on the matrix cores (K buffer KB), and the
+  // probabilities of tile i on the vector ALU.
+  auto half1 = [&](auto do_s, auto do_p, auto do_pv, auto kbuf, float16_t (&cur)[2], float16_t (&nxt)[2])
+                   __attribute__((always_inline)) {
+    constexpr bool S = decltype(do_s)::value, P = decltype(do_p)::value;
+    constexpr int KB = decltype(kbuf)::value, VB = 1 - KB;
+    const unsigned char* const cK = sm + KB * TILE;
+    const unsigned char* const cV = sm + (2 + VB) * TILE;
+    // Piece k of the softmax: VP scores, in three stages that run a piece apart, so that no instruction
+    // waits for the one before it: exponents (k + 1), powers of two (k), rounding and sum (k - 1).
+    // (The empty assembly keeps the stages where they are.  Sums by v_dot2 would be half the
+    // instructions, but those wait for the matrix cores.)
+    constexpr int NP = 4 * NG, VP = 32 / NP;
+    float sum[2] = {l_run, 0.0f};
+    float ex[VP], pw[VP];
+    auto stage_exponent = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < VP; e++) ex[e] = fmaf(cur[k * VP >> 4][(k * VP & 15) + e], a.c, -m_run);
+    };
+    auto stage_power = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < VP; e++) pw[e] = __builtin_amdgcn_exp2f(ex[e]);
+    };
+    auto stage_round = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < VP; e += 2) {
+        const int x = k * VP + e;
+        const float2_t e2 = {pw[e], pw[e + 1]};
+        uint32_t bits = __builtin_bit_cast(uint32_t, __builtin_convertvector(e2, half2_t));
+        sum[0] += pw[e];
+        sum[1] += pw[e + 1];
+        asm volatile("" : "+v"(bits), "+v"(sum[0]), "+v"(sum[1]));
+        pf[x >> 4][x >> 3 & 1][(x & 7) / 2] = bits;
+      }
+    };
+    if constexpr (HD == 128) __builtin_amdgcn_s_setprio(1);
+    if constexpr (P) stage_exponent(0);
+    if constexpr (S) {
+#pragma unroll
+      for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) nxt[kt][r] = 0.0f;
+    }
+#pragma unroll
+    for (int c = 0; c < NG; c++) {
+      if constexpr (S) {
+        if (c + 1 < NG) read_k(cK, c + 1);
+      }
+      if constexpr (decltype(do_pv)::value) {
+        if (c + 1 == NG) read_v(cV, 0);
+      }
+      if (c == 0) transfer(nv, is_v, 2 + KB, pair0);
+      if constexpr (NI > 2) {
+        if (c == NG / 2) transfer(nv, is_v, 2 + KB, pair1);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if constexpr (S) {
+          constexpr int last = 3;
+          const int f = last - j;
+          nxt[f & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[c][f], qf[2 * c + (f >> 1)], nxt[f & 1], 0, 0, 0);
+        }
+        if constexpr (P) {
+          const int k = 4 * c + j;
+          if (k > 0) stage_round(k - 1);
+          stage_power();
+          if (k + 1 < NP) stage_exponent(k + 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if constexpr (P) {
+      stage_round(NP - 1);
+      l_run = sum[0] + sum[1];
+      asm volatile("" : "+v"(l_run));
+    }
+    if constexpr (HD == 128) __builtin_amdgcn_s_setprio(0);
+    advance(nv);
+    wait_landed();
+    barrier();
+  };
+
+  // Second half of tile i: P.V of tile i on the matrix cores (V buffer VB), and the maximum of the
+  // scores of tile i + 1 on the vector ALU.
+  auto half2 = [&](int i, auto do_pv, auto do_max, auto do_s, auto vbuf, float16_t (&nxt)[2])
+                   __attribute__((always_inline)) {
+    constexpr bool PV = decltype(do_pv)::value, MAX = decltype(do_max)::value;
+    constexpr int VB = decltype(vbuf)::value, KB = VB;  // K buffer of tile i + 2
+    const unsigned char* const cV = sm + (2 + VB) * TILE;
+    const unsigned char* const cK = sm + KB * TILE;
+    if constexpr (MAX) {
+      if (i + 1 >= first_edge) {
+        // this lane's first masked key, counted from its own first one
+        int end = lane_end - (tile0 + i + 1) * KEYS - 4 * g;
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            asm volatile("" : "+v"(end));  // (one comparison at a time: 32 would take as many scalar register pairs)
+            if (32 * kt + 8 * (r >> 2) + (r & 3) >= end) nxt[kt][r] = -INFINITY;
+          }
+      }
+    }
+    // (the maximum from the second group on, when the scores are there; done before the last one)
+    constexpr int FIRST = NG == 4 ? 4 : 2, PER = NG == 4 ? 2 : 4;
+    float mx2[2] = {NO_SCORE, NO_SCORE}, mx = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NG; c++) {
+      if constexpr (PV) {
+        if (c + 1 < NG) read_v(cV, c + 1);
+      }
+      if constexpr (decltype(do_s)::value) {
+        if (c + 1 == NG) read_k(cK, 0);
+      }
+      if (c == 0) transfer(nk, is_k, 1 - KB, pair0);
+      if constexpr (NI > 2) {
+        if (c == NG / 2) transfer(nk, is_k, 1 - KB, pair1);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if constexpr (PV) {
+          constexpr int last = 3;
+          const int f = last - j;
+          int kt, t, dt;
+          pv_of(c, f, kt, t, dt);
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[c][f], __builtin_bit_cast(half8_t, pf[kt][t]), o[dt], 0, 0, 0);
+        }
+        if constexpr (MAX) {
+          const int first = (4 * c + j - FIRST) * PER * 2;
+          if (first >= 0 && first < 32) {
+#pragma unroll
+            for (int e = 0; e < PER; e++) {
+              const int x = first + 2 * e;
+              mx2[e & 1] = fmaxf(fmaxf(mx2[e & 1], nxt[x >> 4][x & 15]), nxt[x >> 4][(x & 15) + 1]);
+            }
+          }
+          if (first == 32) mx = pair_max(fmaxf(mx2[0], mx2[1])) * a.c;  // in log2 units (c > 0)
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if constexpr (MAX) {
+      // The exponent reference m_run follows the row maximum lazily: it moves only when some row
+      // of the wavefront outgrew it by more than 2^8 (probabilities up to 256 are as exact in fp16
+      // as those below 1), which after the first tiles is rare; the accumulator is rescaled only then.
+      if (__builtin_amdgcn_ballot_w64(mx > m_run + 8.0f) != 0) {
+        const float m_new = fmaxf(m_run, mx);
+        const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        l_run *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) o[dt][r] *= alpha;
+      }
+    }
+    advance(nk);
+    wait_landed();
+    barrier();
+  };
+  auto idle = [&](int i) __attribute__((always_inline)) {
+    tile_transfers(nv, is_v, 2 + ((i + 1) & 1));
+    wait_landed();
+    barrier();
+    tile_transfers(nk, is_k, (i + 1) & 1);
+    wait_landed();
+    barrier();
+  };
+
+  const std::true_type yes{};
+  const std::false_type no{};
+  const std::integral_constant<int, 0> even{};
+  const std::integral_constant<int, 1> odd{};
+
+  barrier();  // the first K tile has landed for every wavefront
+  int i = -1;
+  if (active > 0) {
+    read_k(sm, 0);
+    half1(yes, no, no, even, sb, sa);
+    half2(-1, no, yes, yes, odd, sa);
+    for (i = 0; i + 2 < active; i += 2) {
+      half1(yes, yes, yes, odd, sa, sb);
+      half2(i, yes, yes, yes, even, sb);
+      half1(yes, yes, yes, even, sb, sa);
+      half2(i + 1, yes, yes, yes, odd, sa);
+    }
+    if (i + 1 < active) {
+      half1(yes, yes, yes, odd, sa, sb);
+      half2(i, yes, yes, no, even, sb);
+      half1(no, yes, yes, even, sb, sa);
+      half2(i + 1, yes, no, no, odd, sa);
+    } else {
+      half1(no, yes, yes, odd, sa, sb);
+      half2(i, yes, no, no, even, sb);
+    }
+    i = active;
+  }
+  for (; i < steps; i++) idle(i);  // tiles this wavefront has no part in
+  wait_vm<0>();  // (transfers of no bytes write zeros)
+  barrier();     // every read of K and V tiles is done: LDS is free
+
+  float l_tot = pair_sum(l_run);
+  if constexpr (PAGED) {
+    // (a page that is not in the cache may be some rows' only: all of the block come out as NaN, and those that do not
+    // see it are computed again below)
+    int* const any_lost = (int*)smem;
+    if (tid == 0) *any_lost = 0;
+    __syncthreads();
+    if (__ballot(lost) && lane == 0) *any_lost = 1;
+    __syncthreads();
+    if (*any_lost) l_tot = NAN;
+    __syncthreads();
+  }
+  if (parts == 1) {
+    // out[row][32d + 8i + 4g + j] = o[d][4i + j] / l, by way of LDS, so that whole rows are stored
+    constexpr int PITCH = ROWB + 16;
+    static_assert(4 * 32 * PITCH <= 4 * TILE, "the output's slots fit the LDS");
+    unsigned char* const slot = smem + w * (32 * PITCH);
+    const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
+    bool finite = true;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        half4_t r;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float v = o[d][4 * i + j] * inv;
+          finite = finite && fabsf(v) < INFINITY;
+          r[j] = (half_t)v;
+        }
+        *(half4_t*)(slot + frow * PITCH + (32 * d + 8 * i + 4 * g) * 2) = r;
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the slot is the wavefront's own)
+    constexpr int RPI = 64 / CPR;  // rows of a store instruction
+    const int r0 = lane / CPR, col = lane % CPR * 8;
+#pragma unroll
+    for (int i = 0; i < 32 / RPI; i++) {
+      const int r = r0 + i * RPI, lr = list0 + r, token = lr / a.group, h = hk * a.group + lr - token * a.group;
+      if (r < wave_rows && col < a.d)
+        *(half8_t*)(a.out + (int64_t)h * a.so_z + (int64_t)(q.row0 + token) * a.so_y + col) =
+            *(const half8_t*)(slot + r * PITCH + col * 2);
+    }
+    // A value that is no number times the zero of a key that the row does not see is no zero: such rows are computed
+    // again from the keys that they see.
+    const uint64_t lanes = __ballot(!finite);
+    if (lanes && q.rows > 1 && causal) {
+      const uint32_t bad = (uint32_t)lanes | (uint32_t)(lanes >> 32);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (behind the stores above)
+      for (int r = 0; r < wave_rows; r++)
+        if (bad >> r & 1) row_by_wave(a, q, (list0 + r) / a.group, hk * a.group + (list0 + r) % a.group, lane);
+    }
+  } else if (frow < wave_rows) {
+    const int64_t prow = ((int64_t)(slot0 + part) * a.kv_heads + hk) * ROWS + w * 32 + frow;
+    float* const po = share.part_o + prow * HD + 4 * g;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float4_t r;
+#pragma unroll
+        for (int j = 0; j < 4; j++) r[j] = o[d][4 * i + j];
+        *(float4_t*)(po + 32 * d + 8 * i) = r;
+      }
+    if (g == 0) share.part_ml[prow] = make_float2(m_run, l_tot);
+  }
+}
+
 // Sums the parts of a divided block: a wavefront to a row, 16 rows to a workgroup, HD / 64 columns to a lane; parts in order.
 template <int HD, int ROWS, int KEYS>
 __global__ __launch_bounds__(256) void attention_join_kernel(SequencesArgs a, Share share) {
@@ -558,7 +1036,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(SequencesArgs a, Sh
 
 namespace {
 
-constexpr int FEW = 16, FEW_KEYS = 32, FEW_WAVES = 2;
+constexpr int FEW = 16, FEW_KEYS = 32, FEW_WAVES = 2, MANY = 128, MANY_KEYS = 64;
 // (a few more than the division above can come to: its sum of work is rounded)
 constexpr int SPARE = 8;
 
@@ -581,26 +1059,40 @@ int64_t slot_bytes(int rows, int hd) { return (int64_t)rows * (hd * 4 + 8); }
 SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
   SequencesPlan p = {SequencesPlan::ANY_LAYOUT, 0, 0, 0};
   if (!chunks(a)) return p;
-  p.kind = SequencesPlan::FEW_ROWS;
-  const int hd = a.d <= 64 ? 64 : 128;
-  const int64_t slot = slot_bytes(FEW, hd) * a.kv_heads;
+  const int longest_rows = a.longest_rows > 0 ? std::min(a.longest_rows, a.rows) : a.rows;
+  p.kind = (int64_t)longest_rows * a.group <= FEW ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES;
+  const bool few = p.kind == SequencesPlan::FEW_ROWS;
+  const int64_t slot = slot_bytes(few ? FEW : MANY, a.d <= 64 ? 64 : 128) * a.kv_heads;
   p.parts = std::max(1, 2 * cus / a.kv_heads);
-  p.parts = (int)std::max<int64_t>(0, std::min<int64_t>(p.parts, (avail / slot - SPARE) / 2));
   p.min_steps = 8;
+  if (!few && (int64_t)a.rows * a.heads / MANY >= 2 * cus) p.parts = 0;
+  p.parts = (int)std::max<int64_t>(0, std::min<int64_t>(p.parts, (avail / slot - SPARE) / 2));
   p.workspace_bytes = p.parts > 0 ? (2 * p.parts + SPARE) * slot : 0;
   return p;
 }
 
 template <int HD, bool PAGED>
-static hipError_t launch_few_rows(hipStream_t stream, const SequencesArgs& a, const Share& share) {
+static hipError_t launch_blocks(hipStream_t stream, const SequencesArgs& a, const SequencesPlan& p, void* workspace) {
+  const bool few = p.kind == SequencesPlan::FEW_ROWS;
+  const int rows = few ? FEW : MANY;
+  Share share = {p.parts, p.min_steps, (float*)workspace, nullptr};
+  if (p.parts > 0) share.part_ml = (float2*)((float*)workspace + ((int64_t)2 * p.parts + SPARE) * a.kv_heads * rows * HD);
   const Pages pages = {PAGED ? page_shift(a.page_size) : 0};
-  const int64_t blocks = (int64_t)a.rows * a.group / FEW + a.sequences + share.parts + SPARE;  // at most
-  if (blocks * a.kv_heads > 0x7fffffff / (64 * FEW_WAVES)) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, FEW_WAVES>), dim3((unsigned)(blocks * a.kv_heads)),
-                     dim3(64 * FEW_WAVES), 0, stream, a, share, pages);
-  if (share.parts > 0)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, FEW, FEW_KEYS>), dim3((unsigned)(share.parts * a.kv_heads)),
-                       dim3(256), 0, stream, a, share);
+  const int64_t blocks = ((int64_t)a.rows * a.group / rows + a.sequences + share.parts + SPARE) * a.kv_heads;  // at most
+  if (blocks > 0x7fffffff / 256) return hipErrorInvalidConfiguration;
+  const dim3 grid((unsigned)blocks);
+  if (few)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, FEW_WAVES>), grid, dim3(64 * FEW_WAVES), 0, stream,
+                       a, share, pages);
+  else
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, PAGED>), grid, dim3(256), 0, stream, a, share, pages);
+  if (p.parts > 0) {
+    const dim3 join((unsigned)(p.parts * a.kv_heads * (rows / 16)));
+    if (few)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, FEW, FEW_KEYS>), join, dim3(256), 0, stream, a, share);
+    else
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, MANY, MANY_KEYS>), join, dim3(256), 0, stream, a, share);
+  }
   return hipGetLastError();
 }
 
@@ -611,11 +1103,8 @@ hipError_t launch_attention_sequences(hipStream_t stream, const SequencesArgs& a
     hipLaunchKernelGGL(attention_any_layout_kernel, dim3((unsigned)grid), dim3(256), 0, stream, a);
     return hipGetLastError();
   }
-  const int hd = a.d <= 64 ? 64 : 128;
-  Share share = {p.parts, p.min_steps, (float*)workspace, nullptr};
-  if (p.parts > 0) share.part_ml = (float2*)((float*)workspace + ((int64_t)2 * p.parts + SPARE) * a.kv_heads * FEW * hd);
-  if (a.table) return hd == 128 ? launch_few_rows<128, true>(stream, a, share) : launch_few_rows<64, true>(stream, a, share);
-  return hd == 128 ? launch_few_rows<128, false>(stream, a, share) : launch_few_rows<64, false>(stream, a, share);
+  if (a.d <= 64) return a.table ? launch_blocks<64, true>(stream, a, p, workspace) : launch_blocks<64, false>(stream, a, p, workspace);
+  return a.table ? launch_blocks<128, true>(stream, a, p, workspace) : launch_blocks<128, false>(stream, a, p, workspace);
 }
 
 }  // namespace adr

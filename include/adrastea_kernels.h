@@ -401,7 +401,7 @@ int64_t adr_attention_f16_workspace_bytes(int32_t heads, int32_t m, int32_t n, i
  * strides in elements (x value, y slot, z head, p page), 64 bits.
  * adr_paged_batch: sequence s has lengths[s] keys in the cache, those of its rows in this call
  * included; key x lies in page table[s * table_pitch + x / page_size], slot x % page_size.  Lengths are
- * taken as at most table_width * page_size and at least 0.  Entries beyond a sequence's length are not
+ * taken as at least 0 and at most table_width * page_size and 2^30.  Entries beyond a sequence's length are not
  * read.  longest_rows and longest are the largest number of rows and keys of any sequence as far as the
  * host knows (0: unknown): they choose kernels and nothing else, every result is right whatever they say.
  */
