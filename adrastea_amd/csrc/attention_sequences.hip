@@ -55,6 +55,14 @@ __device__ __forceinline__ bool key_at(const SequencesArgs& a, const Sequence& q
 
 // One row of one query head by one wavefront, at any strides: 64 keys at a time, a lane to a key for the scores
 // and a lane to every 64th column for the sums.  Only keys that the row sees are read.  Probabilities stay in 32 bits.
+// A kernel's arguments, read from memory where they are used: kept in scalar registers from the start, those of a rare
+// path would push others out.  (They are the kernel's first parameter.)
+__device__ __forceinline__ const SequencesArgs& arguments_again() {
+  auto p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const SequencesArgs*)p;
+}
+
 constexpr int GENERAL_MAX_D = 256;
 __device__ __forceinline__ void row_by_wave(const SequencesArgs& a, const Sequence& q, int j, int h, int lane) {
   const int64_t row = (int64_t)q.row0 + j;
@@ -496,7 +504,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Sequence
     for (int r = w; r < rows; r += WAVES)
       if (*bad_rows >> r & 1) {
         const int lr = block * ROWS + r;
-        row_by_wave(a, q, lr / a.group, hk * a.group + lr % a.group, lane);
+        row_by_wave(arguments_again(), q, lr / a.group, hk * a.group + lr % a.group, lane);
       }
   }
 }
@@ -599,8 +607,6 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a
       const int p = __builtin_amdgcn_readlane(t.page, n & 63), slot = t.key & ((1 << pages.shift) - 1);
       if (p < 0) left = 0;
       t.p = t.base + 2 * (p * t.page_stride + slot * (int64_t)t.stride);
-    } else {
-      t.p = t.base + 2 * (t.key * (int64_t)t.stride);
     }
     t.bytes = left > 0 ? ((left - 1) * t.stride + a.d) * 2 + BIAS : 0;
   };
@@ -611,6 +617,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a
     t.stride = (int)stride;
     t.key = tile0 * KEYS + 16 * w;
     t.page = 0;
+    t.p = t.base + 2 * (t.key * stride);
     place(t);
     return t;
   };
@@ -624,6 +631,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a
   Next nk = first_tile(a.k + hk * a.sk.z, a.sk.y, a.sk.p), nv = first_tile(a.v + hk * a.sv.z, a.sv.y, a.sv.p);
   auto advance = [&](Next& t) __attribute__((always_inline)) {
     t.key += KEYS;
+    if constexpr (!PAGED) t.p += (uint32_t)t.stride * (KEYS * 2u);
     place(t);
   };
   // Transfers 2 j and 2 j + 1 of the NI that bring a tile into buffer `buf` (0, 1: K; 2, 3: V).
@@ -956,7 +964,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a
       const uint32_t bad = (uint32_t)lanes | (uint32_t)(lanes >> 32);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (behind the stores above)
       for (int r = 0; r < wave_rows; r++)
-        if (bad >> r & 1) row_by_wave(a, q, (list0 + r) / a.group, hk * a.group + (list0 + r) % a.group, lane);
+        if (bad >> r & 1) row_by_wave(arguments_again(), q, (list0 + r) / a.group, hk * a.group + (list0 + r) % a.group, lane);
     }
   } else if (frow < wave_rows) {
     const int64_t prow = ((int64_t)(slot0 + part) * a.kv_heads + hk) * ROWS + w * 32 + frow;
@@ -1021,7 +1029,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(SequencesArgs a, Sh
 #pragma unroll
     for (int j = 0; j < C; j++) finite = finite && fabsf(acc[j]) < INFINITY;
     if (__ballot(!finite) && pc.q.rows > 1 && a.mask == ADR_MASK_CAUSAL) {
-      row_by_wave(a, pc.q, token, h, lane);
+      row_by_wave(arguments_again(), pc.q, token, h, lane);
       continue;
     }
     if (lane * C < a.d)
