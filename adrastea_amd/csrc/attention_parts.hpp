@@ -82,6 +82,13 @@ __device__ __forceinline__ void dma_buffer_pair(uint32_t lds, uint32_t voff0, ui
                "buffer_load_dwordx4 %2, %3, 0 offen offset:%5 lds"
                :: "s"(lds), "v"(voff0), "v"(voff1), "s"(desc), "n"(FIRST * 1024), "n"(FIRST * 1024 + 1024) : "memory");
 }
+// The same for what is read once: the lines are the first to leave the caches.
+template <int FIRST>
+__device__ __forceinline__ void dma_buffer_pair_once(uint32_t lds, uint32_t voff0, uint32_t voff1, u32x4_t desc) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %3, 0 offen offset:%4 nt lds\n\t"
+               "buffer_load_dwordx4 %2, %3, 0 offen offset:%5 nt lds"
+               :: "s"(lds), "v"(voff0), "v"(voff1), "s"(desc), "n"(FIRST * 1024), "n"(FIRST * 1024 + 1024) : "memory");
+}
 __device__ __forceinline__ void dma_global(uint32_t lds, const void* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, off"
                :: "s"(lds), "v"(p) : "memory");

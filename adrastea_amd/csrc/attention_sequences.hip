@@ -16,13 +16,40 @@ namespace {
 
 constexpr float NO_SCORE = -1.0e30f;  // below any score of finite operands; exp2(-inf - NO_SCORE) is 0, not NaN
 
+// What a kernel is given.  Share of the work: see below.
+struct Job : SequencesArgs {
+  int page_shift;   // log2 of the slots of a page (16 at least: 16 keys from a multiple of 16 on lie on one page)
+  int parts;        // workgroups of a key head that share its work; 0: unshared
+  int shift;        // log2 of a piece's tiles
+  int least;        // pieces that a workgroup has at least
+  float* part_o;    // [2 * parts][key head][ROWS][HD] unnormalised sums
+  float2* part_ml;  // [2 * parts][key head][ROWS] (maximum in log2 units, sum)
+};
+
+// The job is read where it is used, by scalar loads from the kernel's arguments (of which it is the only one): kept in
+// registers from the start, what only the end of a kernel needs would push out what its loops need -- 25 scalar registers
+// were spilled into vector ones.  Loads do not move across arguments().
+typedef const __attribute__((address_space(4))) Job& Args;
+__device__ __forceinline__ Args arguments() {
+  auto p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const __attribute__((address_space(4))) Job*)p;
+}
+
+// The thread's index, likewise: what a kernel derives from it for one block is not kept for the next.
+__device__ __forceinline__ int thread_index() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
 // A sequence's rows and keys.
 struct Sequence {
   int index, row0, rows;  // first row of the [heads, rows, d] views
   int key0, keys;         // first key of packed ones
 };
 
-__device__ __forceinline__ Sequence sequence_at(const SequencesArgs& a, int s) {
+__device__ __forceinline__ Sequence sequence_at(Args a, int s) {
   Sequence q;
   q.index = s;
   q.row0 = clamp_to(a.row_offsets[s], a.rows);
@@ -39,7 +66,7 @@ __device__ __forceinline__ Sequence sequence_at(const SequencesArgs& a, int s) {
 }
 
 // Key x of the sequence as element offsets of its key and value rows (head 0); false: on no page of the cache.
-__device__ __forceinline__ bool key_at(const SequencesArgs& a, const Sequence& q, int x, int64_t& k, int64_t& v) {
+__device__ __forceinline__ bool key_at(Args a, const Sequence& q, int x, int64_t& k, int64_t& v) {
   if (!a.table) {
     k = (q.key0 + (int64_t)x) * a.sk.y;
     v = (q.key0 + (int64_t)x) * a.sv.y;
@@ -55,16 +82,8 @@ __device__ __forceinline__ bool key_at(const SequencesArgs& a, const Sequence& q
 
 // One row of one query head by one wavefront, at any strides: 64 keys at a time, a lane to a key for the scores
 // and a lane to every 64th column for the sums.  Only keys that the row sees are read.  Probabilities stay in 32 bits.
-// A kernel's arguments, read from memory where they are used: kept in scalar registers from the start, those of a rare
-// path would push others out.  (They are the kernel's first parameter.)
-__device__ __forceinline__ const SequencesArgs& arguments_again() {
-  auto p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(p));
-  return *(const SequencesArgs*)p;
-}
-
 constexpr int GENERAL_MAX_D = 256;
-__device__ __forceinline__ void row_by_wave(const SequencesArgs& a, const Sequence& q, int j, int h, int lane) {
+__device__ __forceinline__ void row_by_wave(Args a, const Sequence& q, int j, int h, int lane) {
   const int64_t row = (int64_t)q.row0 + j;
   const half_t* const Q = a.q + h * (int64_t)a.sq_z + row * a.sq_y;
   const half_t* const K = a.k + (h / a.group) * a.sk.z;
@@ -114,7 +133,8 @@ __device__ __forceinline__ void row_by_wave(const SequencesArgs& a, const Sequen
 }
 
 // Any layout: a wavefront per row and query head.
-__global__ __launch_bounds__(256) void attention_any_layout_kernel(SequencesArgs a) {
+__global__ __launch_bounds__(256) void attention_any_layout_kernel(Job) {
+  Args a = arguments();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int64_t i = (int64_t)blockIdx.x * 4 + wave; i < (int64_t)a.rows * a.heads; i += (int64_t)gridDim.x * 4) {
     const int h = (int)(i / a.rows), row = (int)(i - (int64_t)h * a.rows);
@@ -129,24 +149,22 @@ __global__ __launch_bounds__(256) void attention_any_layout_kernel(SequencesArgs
 //
 // The rows of a sequence times the query heads of a group, R = rows * group, are one list (row of the sequence
 // first, head of the group second), cut into blocks of ROWS: the heads of a group share every key that is read.
-// A workgroup takes one block of one key head, or one of several parts of its keys.  The host knows neither
-// the sequences' rows nor their keys, only how many workgroups fill the chip (`parts` for each key head), so the
-// division is made on the device, by every wavefront for itself and with the same result: with W the sum over all
-// blocks of their key tiles, no workgroup gets more than C = max(W / parts, min_steps) tiles, and a block
-// with more is divided evenly.  That is at most parts + blocks workgroups, and no sequence, however long among
-// short ones, holds up the others.  Divided blocks have their parts' results in consecutive slots of the workspace,
-// fewer than 2 * parts of them (each has more than C tiles, and there are W in all).
-struct Share {
-  int parts, min_steps;  // 0: nothing is divided
-  float* part_o;         // [slot][key head][ROWS][HD] unnormalised sums
-  float2* part_ml;       // [slot][key head][ROWS] (maximum in log2 units, sum)
+// The host knows neither the sequences' rows nor their keys, so the work is divided on the device, by every wavefront
+// for itself and with the same result.  Unshared: a workgroup takes one block of one key head.  Shared: all blocks' keys
+// are one line of pieces of 2^shift tiles, block after block, and each of `parts` workgroups of a key head takes the
+// same length of it: no sequence, however long among short ones, holds up the others, and a workgroup has its
+// start-up once.  A block that lies in one workgroup's stretch is finished there.  Of the others, a workgroup has at
+// most the first and the last in its stretch; their results go to its two slots of the workspace, and are joined by a
+// second launch, in order.
+struct Line {
+  int total, parts, shift;  // pieces, workgroups that have some, log2 of a piece's tiles
+  __device__ __forceinline__ int at(int part) const { return (int)((int64_t)total * part / parts); }
 };
 
-struct Piece {
+struct Block {
   Sequence q;
-  int block;          // of the sequence's rows
-  int part, parts;    // of its keys
-  int slot;           // of the first part's results
+  int block;           // of the sequence's list
+  int offset, pieces;  // of the block: where on the line the asked place lies in it, and all
 };
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -161,85 +179,85 @@ __device__ __forceinline__ int add_scan(int v) {  // inclusive, over the lanes o
   return v;
 }
 
-// Piece number `index` of the list above (DIVIDED: block number `index` of those that are divided); false: there are
-// fewer.  A lane takes 4 sequences of 256.
-template <int ROWS, int KEYS, bool DIVIDED>
-__device__ __forceinline__ bool find_piece(const SequencesArgs& a, const Share& share, int index, int lane, Piece& piece) {
-  constexpr int EACH = 4;
-  int blocks[EACH], tiles[EACH];
-  auto load = [&](int base) __attribute__((always_inline)) {
+// Rows of a block, keys of a tile, log2 of the tiles of a piece
+constexpr int FEW = 16, FEW_KEYS = 32, FEW_SHIFT = 2, FEW_WAVES = 2;  // (two tiles for each wavefront)
+constexpr int MANY = 128, MANY_KEYS = 64, MANY_SHIFT = 1;
+
+// The sequences on the line, 256 at a time: lane l has sequences base + 64 e + l, read from memory once for the whole
+// division where there are no more.
+template <int ROWS, int KEYS, bool SHARED>
+struct Roster {
+  static constexpr int EACH = 4;
+  typedef int each_t __attribute__((ext_vector_type(EACH)));
+  each_t row0, rows, key0, keys;
+  each_t upto;            // where on the line the sequence ends
+  int base, before, end;  // first sequence, and the part of the line that these are
+
+  static __device__ __forceinline__ int blocks_of(Args a, int rows) {
+    return (int)(((int64_t)rows * a.group + ROWS - 1) / ROWS);
+  }
+  // A block's pieces: one at least, so that rows without keys are somebody's.
+  static __device__ __forceinline__ int pieces_of(int keys, int shift) {
+    return SHARED ? max(1, (((keys + KEYS - 1) / KEYS) + (1 << shift) - 1) >> shift) : 1;
+  }
+  __device__ __forceinline__ void load(Args a, int shift, int lane, int first, int line) {
+    base = first;
+    before = end = line;
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
-      const int s = base + lane * EACH + e;
-      blocks[e] = tiles[e] = 0;
-      if (s < a.sequences) {
-        const Sequence q = sequence_at(a, s);
-        blocks[e] = (int)(((int64_t)q.rows * a.group + ROWS - 1) / ROWS);
-        tiles[e] = (q.keys + KEYS - 1) / KEYS;
+      row0[e] = rows[e] = key0[e] = keys[e] = 0;
+      if (base + 64 * e < a.sequences && base + 64 * e + lane < a.sequences) {
+        const Sequence q = sequence_at(a, base + 64 * e + lane);
+        row0[e] = q.row0, rows[e] = q.rows, key0[e] = q.key0, keys[e] = q.keys;
       }
     }
-  };
-  load(0);
-  int most = 0x7fffffff;  // C
-  if (share.parts > 0) {
-    // (in 32-bit floats: the sum need not be exact, only the same everywhere)
-    float work = 0.0f;
-    for (int base = 0;;) {
-#pragma unroll
-      for (int e = 0; e < EACH; e++) work += (float)blocks[e] * (float)tiles[e];
-      base += 64 * EACH;
-      if (base >= a.sequences) break;
-      load(base);
-    }
-    for (int i = 1; i < 64; i <<= 1) work += __shfl_xor(work, i);
-    most = uniform(max(share.min_steps, (int)fminf(ceilf(work / (float)share.parts), 1.0e9f)));
-    if (a.sequences > 64 * EACH) load(0);
-  }
-  int slot = 0;
-  for (int base = 0; base < a.sequences;) {
-    int count[EACH], parts[EACH], sum = 0, slots = 0;
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
-      parts[e] = tiles[e] <= most ? 1 : (tiles[e] + most - 1) / most;
-      const int divided = parts[e] > 1 ? blocks[e] : 0;
-      count[e] = DIVIDED ? divided : blocks[e] * parts[e];
-      sum += count[e];
-      slots += divided * parts[e];
-    }
-    const int upto = add_scan(sum), slots_upto = add_scan(slots);
-    const uint64_t behind = __ballot(upto > index);
-    if (behind) {
-      const int at = __builtin_ctzll(behind);
-      int i = index - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(sum, at));
-      slot += __builtin_amdgcn_readlane(slots_upto, at) - __builtin_amdgcn_readlane(slots, at);
-#pragma unroll
-      for (int e = 0; e < EACH; e++) {
-        const int n = __builtin_amdgcn_readlane(count[e], at), p = __builtin_amdgcn_readlane(parts[e], at), b = __builtin_amdgcn_readlane(blocks[e], at);
-        if (i < n) {
-          // (the last blocks first: under the mask they have the most keys)
-          const int block = b - 1 - (DIVIDED ? i : i / p);
-          const Sequence q = sequence_at(a, base + at * EACH + e);
-          piece.q = {uniform(q.index), uniform(q.row0), uniform(q.rows), uniform(q.key0), uniform(q.keys)};
-          piece.block = uniform(block);
-          piece.parts = uniform(p);
-          piece.part = uniform(DIVIDED ? 0 : i % p);
-          piece.slot = uniform(slot + (b - 1 - block) * p);
-          return true;
-        }
-        i -= n;
-        if (p > 1) slot += b * p;
+      upto[e] = end;
+      if (base + 64 * e < a.sequences) {
+        upto[e] += add_scan(blocks_of(a, rows[e]) * pieces_of(keys[e], shift));
+        end = __builtin_amdgcn_readlane(upto[e], 63);
       }
     }
-    index -= __builtin_amdgcn_readlane(upto, 63);
-    slot += __builtin_amdgcn_readlane(slots_upto, 63);
-    base += 64 * EACH;
-    if (base < a.sequences) load(base);
   }
-  return false;
-}
+  // The whole line.
+  __device__ __forceinline__ Line line_of(Args a, int lane) {
+    load(a, a.shift, lane, 0, 0);
+    while (base + 64 * EACH < a.sequences) load(a, a.shift, lane, base + 64 * EACH, end);
+    Line line = {end, max(1, end), a.shift};
+    if (SHARED) line.parts = max(1, min(a.parts, end / a.least));
+    return line;
+  }
+  // The block at `place` of the line; false: the line ends before.
+  __device__ __forceinline__ bool block_at(Args a, int shift, int place, int lane, Block& b) {
+    if (place < before) load(a, shift, lane, 0, 0);
+    while (place >= end) {
+      if (base + 64 * EACH >= a.sequences) return false;
+      load(a, shift, lane, base + 64 * EACH, end);
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+      const uint64_t behind = __ballot(upto[e] > place);
+      if (behind) {
+        const int at = __builtin_ctzll(behind);
+        b.q = {base + 64 * e + at, __builtin_amdgcn_readlane(row0[e], at), __builtin_amdgcn_readlane(rows[e], at),
+               __builtin_amdgcn_readlane(key0[e], at), __builtin_amdgcn_readlane(keys[e], at)};
+        const int blocks = blocks_of(a, b.q.rows), p = pieces_of(b.q.keys, shift);
+        const int in = place - (__builtin_amdgcn_readlane(upto[e], at) - blocks * p);
+        // (the last blocks first: under the mask they have the most keys)
+        const int i = SHARED ? uniform(in / p) : in;
+        b.block = blocks - 1 - i;
+        b.offset = in - i * p;
+        b.pieces = p;
+        return true;
+      }
+    }
+    return false;
+  }
+};
 
 // One past the last key that some row of the block sees, and of one row.
-__device__ __forceinline__ int end_of_row(const SequencesArgs& a, const Sequence& q, int j) {
+__device__ __forceinline__ int end_of_row(Args a, const Sequence& q, int j) {
   return a.mask == ADR_MASK_CAUSAL ? clamp_to(j + q.keys - q.rows + 1, q.keys) : q.keys;
 }
 
@@ -250,20 +268,14 @@ __device__ __forceinline__ u32x4_t descriptor(uint64_t p, int bytes) {
                  (uint32_t)uniform(bytes), 0x00020000u};
 }
 
-// Pages of 2^shift slots, 16 at least: 16 keys from a multiple of 16 on lie on one page, so that a transfer of 16 rows
-// has one base address.
-struct Pages {
-  int shift;
-};
-
 // ---- few rows: generation, a few tokens at once ----------------------------------------------------------
 //
 // A block of 16 rows against its keys: a read of the keys and values.  The workgroup's wavefronts walk tiles of
 // 32 keys in turn, each through two tiles' worth of LDS of its own, so that the loop has no barrier.  S^T = K Q^T, so
 // that a lane holds scores of one row, and O^T = V^T P^T, on MFMA 16x16x32; probabilities are rounded to fp16, the
 // matrix cores' operands, sums and scores stay in 32 bits.
-template <int HD, bool PAGED, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(SequencesArgs a, Share share, Pages pages) {
+template <int HD, bool PAGED, int WAVES, bool SHARED>
+__global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Job) {
   constexpr int CPR = HD / 8, KEYS = 32, ROWS = 16;
   constexpr int ROWB = HD * 2, TILE = KEYS * ROWB;  // bytes of a tile row, of a K or V tile
   constexpr int NI = TILE / 1024;                   // transfers per tile
@@ -274,19 +286,28 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Sequence
   static_assert(16 * (PITCH + 2) * 4 + 16 <= WAVE, "the partial results fit the tiles' LDS");
   __shared__ __attribute__((aligned(1024))) unsigned char smem[WAVES * WAVE];
 
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kv_heads = arguments().kv_heads, hk = blockIdx.x % kv_heads, wg = blockIdx.x / kv_heads;
+  Roster<ROWS, KEYS, SHARED> roster;
+  const Line line = roster.line_of(arguments(), threadIdx.x & 63);
+  if (wg >= line.parts) return;
+  const int stretch0 = SHARED ? line.at(wg) : wg, stretch1 = SHARED ? line.at(wg + 1) : wg + 1;
+  for (int place = stretch0, next_place;; place = next_place) {
+  Args a = arguments();
+  const int tid = thread_index(), lane = tid & 63, w = uniform(tid >> 6);
   const int frow = lane & 15, g = lane >> 4;
-  const int hk = blockIdx.x % a.kv_heads;
-  Piece pc;
-  if (!find_piece<ROWS, KEYS, false>(a, share, blockIdx.x / a.kv_heads, lane, pc)) return;
-  const Sequence q = pc.q;
-  const int block = pc.block, part = pc.part, parts = pc.parts, slot0 = pc.slot;
+  Block b;
+  if (!roster.block_at(a, a.shift, place, lane, b)) return;
+  const Sequence q = b.q;
+  const int block = b.block, pieces = min(stretch1 - place, b.pieces - b.offset);
+  const bool whole = pieces == b.pieces;
+  next_place = place + pieces;
   const int rows = min(ROWS, q.rows * a.group - block * ROWS);          // of the block
   const int list_row = block * ROWS + min(frow, rows - 1), row = list_row / a.group, gh = list_row - row * a.group;
 
   const int last_end = uniform(end_of_row(a, q, (block * ROWS + rows - 1) / a.group));  // of the block's last row
   const int all = (last_end + KEYS - 1) / KEYS;
-  const int tile0 = uniform((int)((int64_t)all * part / parts)), tile1 = uniform((int)((int64_t)all * (part + 1) / parts));
+  const int tile0 = whole ? 0 : min(all, b.offset << line.shift);
+  const int tile1 = b.offset + pieces == b.pieces ? all : min(all, (b.offset + pieces) << line.shift);
   const int row_end = min(last_end, tile1 * KEYS);
   const int tiles = max(0, (tile1 - tile0 - w + WAVES - 1) / WAVES);  // of this wavefront: tile0 + w + WAVES i
 
@@ -312,36 +333,34 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Sequence
     const int key = (tile0 + w + WAVES * (i + (lane >> 1))) * KEYS + 16 * (lane & 1);
     page = 0;
     if (key < row_end) {
-      page = a.table[(int64_t)q.index * a.table_pitch + (key >> pages.shift)];
+      page = a.table[(int64_t)q.index * a.table_pitch + (key >> a.page_shift)];
       if (page < 0 || page >= a.pages) lost = true, page = -1;
     }
   };
-  auto fetch = [&](int i) __attribute__((always_inline)) {
+  // Keys, or values, of tile i.
+  auto fetch = [&](int i, auto is_k) __attribute__((always_inline)) {
+    constexpr bool IS_K = decltype(is_k)::value;
+    const auto& st = IS_K ? a.sk : a.sv;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       const int key = (tile0 + w + WAVES * i) * KEYS + 16 * h;
       int left = min(row_end - key, 16);
-      int64_t ko, vo;
+      int64_t at = key * st.y;
       if constexpr (PAGED) {
-        const int p = __builtin_amdgcn_readlane(page, 2 * (i & 31) + h), slot = key & ((1 << pages.shift) - 1);
+        const int p = __builtin_amdgcn_readlane(page, 2 * (i & 31) + h), slot = key & ((1 << a.page_shift) - 1);
         if (p < 0) left = 0;
-        ko = p * a.sk.p + slot * a.sk.y;
-        vo = p * a.sv.p + slot * a.sv.y;
-      } else {
-        ko = key * a.sk.y;
-        vo = key * a.sv.y;
+        at = p * st.p + slot * st.y;
       }
-      const uint64_t pk = (uint64_t)(K + ko) - BIAS, pv = (uint64_t)(V + vo) - BIAS;
-      const u32x4_t dk = descriptor(pk, left > 0 ? ((left - 1) * (int)a.sk.y + a.d) * 2 + BIAS : 0);
-      const u32x4_t dv = descriptor(pv, left > 0 ? ((left - 1) * (int)a.sv.y + a.d) * 2 + BIAS : 0);
+      const u32x4_t desc = descriptor((uint64_t)((IS_K ? K : V) + at) - BIAS,
+                                      left > 0 ? ((left - 1) * (int)st.y + a.d) * 2 + BIAS : 0);
+      const uint32_t dst = lds0 + ((IS_K ? 0 : 2) + (i & 1)) * TILE + h * (NI / 2) * 1024;
+      const uint32_t(&off)[NI / 2] = IS_K ? koff : voff;
 #pragma unroll
-      for (int j = 0; j < NI / 2; j += 2)
-        dma_buffer_pair<0>(lds0 + (i & 1) * TILE + (h * (NI / 2) + j) * 1024, koff[j], koff[j + 1], dk);
-#pragma unroll
-      for (int j = 0; j < NI / 2; j += 2)
-        dma_buffer_pair<0>(lds0 + (2 + (i & 1)) * TILE + (h * (NI / 2) + j) * 1024, voff[j], voff[j + 1], dv);
+      for (int j = 0; j < NI / 2; j += 2) dma_buffer_pair_once<0>(dst + j * 1024, off[j], off[j + 1], desc);
     }
   };
+  const std::true_type is_k{};
+  const std::false_type is_v{};
 
   if constexpr (PAGED) look_up(0);
   half8_t qf[KS];
@@ -356,8 +375,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Sequence
   // (the loads above have landed before the transfers' own count begins)
 #pragma unroll
   for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(qf[ks]));
-  if (tiles > 0) fetch(0);
-  if (tiles > 1) fetch(1);
+  if (tiles > 0) fetch(0, is_k), fetch(0, is_v);
+  if (tiles > 1) fetch(1, is_k), fetch(1, is_v);
   int offK[KS], offV[DB];
 #pragma unroll
   for (int ks = 0; ks < KS; ks++) offK[ks] = k_chunk_off<CPR>(frow, ks * 4 + g);
@@ -375,9 +394,11 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Sequence
 #pragma unroll
   for (int db = 0; db < DB; db++) o[db] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
   const int end = min(end_of_row(a, q, row), row_end) - 4 * g;  // this lane's first key that its row does not see
-  // Tile i; `next`: there is a tile i + 1, `more`: and a tile i + 2.
+  // Tile i; `next`: there is a tile i + 1, `more`: and a tile i + 2, whose keys and values are asked for as soon as the
+  // fragments of this one's are in registers.
   auto tile = [&](int i, auto next, auto more) __attribute__((always_inline)) {
-    wait_vm<decltype(next)::value ? 2 * NI : 0>();  // tile i has landed (tile i + 1 may be in flight)
+    constexpr bool NEXT = decltype(next)::value, MORE = decltype(more)::value;
+    wait_vm<NEXT ? 3 * NI : NI>();  // its keys have landed
     const unsigned char* const cK = sm + (i & 1) * TILE;
     const unsigned char* const cV = sm + (2 + (i & 1)) * TILE;
     float4_t s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
@@ -388,6 +409,14 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Sequence
         const half8_t kf = *(const half8_t*)(cK + offK[ks] + kb * 16 * ROWB);
         s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[ks], s[kb], 0, 0, 0);
       }
+    if constexpr (MORE) {
+      if constexpr (PAGED) {
+        if (((i + 2) & 31) == 0) look_up(i + 2);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      fetch(i + 2, is_k);
+    }
+    wait_vm<MORE ? 3 * NI : NEXT ? 2 * NI : 0>();  // and its values
     half8_t vf[DB];
 #pragma unroll
     for (int db = 0; db < DB; db++) {
@@ -396,6 +425,12 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Sequence
       const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)ADR_LDS_PTR(p0 + 16 * ROWB));
       vf[db] = __builtin_shufflevector(__builtin_bit_cast(half4_t, lo), __builtin_bit_cast(half4_t, hi),
                                        0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    if constexpr (MORE) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int db = 0; db < DB; db++) asm volatile("" : "+v"(vf[db]));
+      fetch(i + 2, is_v);
     }
     const int left = end - (tile0 + w + WAVES * i) * KEYS;  // keys of this lane's row from its first one on
     float mx = NO_SCORE;
@@ -430,14 +465,6 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Sequence
       o[db] *= alpha;
       o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[db], __builtin_bit_cast(half8_t, pf), o[db], 0, 0, 0);
     }
-    // (the tile has been read: its fragments are in registers)
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if constexpr (decltype(more)::value) {
-      if constexpr (PAGED) {
-        if (((i + 2) & 31) == 0) look_up(i + 2);
-      }
-      fetch(i + 2);
-    }
   };
   const std::true_type yes{};
   const std::false_type no{};
@@ -446,6 +473,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Sequence
   if (i + 1 < tiles) tile(i++, yes, no);
   if (i < tiles) tile(i, no, no);
 
+  Args z = arguments();
   // Merge the wavefronts' results: [wavefront][row][HD] sums, and (maximum, sum) of every row.
   wait_vm<0>();
   __syncthreads();
@@ -478,8 +506,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Sequence
       l += ml[x].y * f;
       sum += *(const float4_t*)(xo + (x * 16 + r) * PITCH + col) * f;
     }
-    if (parts == 1) {
-      const int lr = block * ROWS + r, token = lr / a.group, h = hk * a.group + lr - token * a.group;
+    if (whole) {
+      const int lr = block * ROWS + r, token = lr / z.group, h = hk * z.group + lr - token * z.group;
       half4_t v;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       bool finite = true;
@@ -489,23 +517,28 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Sequence
         v[j] = (half_t)(sum[j] * inv);
       }
       if (!finite) atomicOr(bad_rows, 1 << r);
-      if (col < a.d)
-        *(half4_t*)(a.out + (int64_t)h * a.so_z + (int64_t)(q.row0 + token) * a.so_y + col) = v;
+      if (col < z.d)
+        *(half4_t*)(z.out + (int64_t)h * z.so_z + (int64_t)(q.row0 + token) * z.so_y + col) = v;
     } else {
-      const int64_t prow = ((int64_t)(slot0 + part) * a.kv_heads + hk) * ROWS + r;
-      *(float4_t*)(share.part_o + prow * HD + col) = sum;
-      if (col == 0) share.part_ml[prow] = make_float2(m_all, l);
+      const int64_t prow = ((int64_t)(2 * wg + (place != stretch0)) * z.kv_heads + hk) * ROWS + r;
+      *(float4_t*)(z.part_o + prow * HD + col) = sum;
+      if (col == 0) z.part_ml[prow] = make_float2(m_all, l);
     }
   }
   // A value that is no number times the zero of a key that the row does not see is no zero: such rows are computed
   // again from the keys that they see.
-  if (parts == 1 && q.rows > 1 && a.mask == ADR_MASK_CAUSAL) {
+  if (whole && q.rows > 1 && z.mask == ADR_MASK_CAUSAL) {
     __syncthreads();
     for (int r = w; r < rows; r += WAVES)
       if (*bad_rows >> r & 1) {
         const int lr = block * ROWS + r;
-        row_by_wave(arguments_again(), q, lr / a.group, hk * a.group + lr % a.group, lane);
+        row_by_wave(arguments(), q, lr / z.group, hk * z.group + lr % z.group, lane);
       }
+  }
+  if (!SHARED || next_place >= stretch1) break;
+  __syncthreads();  // (the next block's transfers go where the results are read)
+  Args n = arguments();
+  roster.load(n, n.shift, thread_index() & 63, 0, 0);  // (not kept in registers meanwhile)
   }
 }
 
@@ -522,8 +555,8 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Sequence
 // beside the maximum of tile i + 1.  What is different here is where rows and keys come from: the heads of a group
 // share the block, so that a key row is read once for all of them and the part of a tile that the mask leaves empty
 // is 1 / group as wide, and each wavefront's 16 key rows of a tile have a base address of their own, on a page.
-template <int HD, bool PAGED>
-__global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a, Share share, Pages pages) {
+template <int HD, bool PAGED, bool SHARED>
+__global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
   constexpr int CPR = HD / 8, KEYS = 64, ROWS = 128;
   constexpr int TILE = KEYS * HD * 2;  // bytes of one K or V tile
   constexpr int NI = TILE / 1024 / 4;  // transfers per wavefront and tile: 16 rows
@@ -533,24 +566,32 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a
   constexpr int BIAS = NI * 1024;      // bytes that descriptors start ahead, so that no offset is negative
   __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];  // K0 K1 V0 V1
 
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int frow = lane & 31, g = lane >> 5;
-  const bool causal = a.mask == ADR_MASK_CAUSAL;
   // Consecutive workgroups go to different dies; where the key heads divide evenly, a die takes its share of them, so
   // that the blocks which read the same keys meet in one L2.
+  const int kv_heads = arguments().kv_heads;
   int hk, index;
-  if (a.kv_heads % 8 == 0) {
-    const int each = a.kv_heads >> 3, seq = blockIdx.x >> 3;
+  if (kv_heads % 8 == 0) {
+    const int each = kv_heads >> 3, seq = blockIdx.x >> 3;
     hk = (blockIdx.x & 7) * each + seq % each;
     index = seq / each;
   } else {
-    hk = blockIdx.x % a.kv_heads;
-    index = blockIdx.x / a.kv_heads;
+    hk = blockIdx.x % kv_heads;
+    index = blockIdx.x / kv_heads;
   }
-  Piece pc;
-  if (!find_piece<ROWS, KEYS, false>(a, share, index, lane, pc)) return;
-  const Sequence q = pc.q;
-  const int block = pc.block, part = pc.part, parts = pc.parts, slot0 = pc.slot;
+  Roster<ROWS, KEYS, SHARED> roster;
+  const Line line = roster.line_of(arguments(), threadIdx.x & 63);
+  if (index >= line.parts) return;
+  const int stretch0 = SHARED ? line.at(index) : index, stretch1 = SHARED ? line.at(index + 1) : index + 1;
+  for (int place = stretch0, next_place;; place = next_place) {
+  Args a = arguments();
+  const int tid = thread_index(), lane = tid & 63, w = uniform(tid >> 6);
+  const int frow = lane & 31, g = lane >> 5;
+  Block b;
+  if (!roster.block_at(a, a.shift, place, lane, b)) return;
+  const Sequence q = b.q;
+  const int block = b.block, pieces = min(stretch1 - place, b.pieces - b.offset);
+  const bool whole = pieces == b.pieces;
+  next_place = place + pieces;
   const int rows = min(ROWS, q.rows * a.group - block * ROWS);  // of the block
   const int wave_rows = min(32, rows - w * 32);                 // of the wavefront (may be negative)
   const int list0 = block * ROWS + w * 32;
@@ -560,8 +601,8 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a
 
   const int last_end = uniform(end_of_row(a, q, (block * ROWS + rows - 1) / a.group));
   const int all = (last_end + KEYS - 1) / KEYS;
-  const int tile0 = uniform((int)((int64_t)all * part / parts));
-  const int steps = uniform((int)((int64_t)all * (part + 1) / parts)) - tile0;
+  const int tile0 = whole ? 0 : min(all, b.offset << line.shift);
+  const int steps = (b.offset + pieces == b.pieces ? all : min(all, (b.offset + pieces) << line.shift)) - tile0;
   const int row_end = min(last_end, (tile0 + steps) * KEYS);
   // Tiles that this wavefront computes: none without rows, none whose first key lies beyond its last row's.
   int active = 0, first_edge = 0;
@@ -592,7 +633,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a
     int bytes, key, stride, page;
   };
   bool lost = false;  // a key's page is not in the cache
-  auto place = [&](Next& t) __attribute__((always_inline)) {
+  auto locate = [&](Next& t) __attribute__((always_inline)) {
     const int n = ((t.key - 16 * w) >> 6) - tile0;
     int left = min(row_end - t.key, 16);
     if constexpr (PAGED) {
@@ -600,11 +641,11 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a
         const int key = t.key + lane * KEYS;
         t.page = 0;
         if (key < row_end) {
-          t.page = a.table[(int64_t)q.index * a.table_pitch + (key >> pages.shift)];
+          t.page = a.table[(int64_t)q.index * a.table_pitch + (key >> a.page_shift)];
           if (t.page < 0 || t.page >= a.pages) lost = true, t.page = -1;
         }
       }
-      const int p = __builtin_amdgcn_readlane(t.page, n & 63), slot = t.key & ((1 << pages.shift) - 1);
+      const int p = __builtin_amdgcn_readlane(t.page, n & 63), slot = t.key & ((1 << a.page_shift) - 1);
       if (p < 0) left = 0;
       t.p = t.base + 2 * (p * t.page_stride + slot * (int64_t)t.stride);
     }
@@ -618,7 +659,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a
     t.key = tile0 * KEYS + 16 * w;
     t.page = 0;
     t.p = t.base + 2 * (t.key * stride);
-    place(t);
+    locate(t);
     return t;
   };
   half8_t qf[DS];  // (operand B of S^T = K Q^T: lane -> row frow, head-dimension group g)
@@ -632,7 +673,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a
   auto advance = [&](Next& t) __attribute__((always_inline)) {
     t.key += KEYS;
     if constexpr (!PAGED) t.p += (uint32_t)t.stride * (KEYS * 2u);
-    place(t);
+    locate(t);
   };
   // Transfers 2 j and 2 j + 1 of the NI that bring a tile into buffer `buf` (0, 1: K; 2, 3: V).
   auto transfer = [&](const Next& t, auto is_k, int buf, auto pair) __attribute__((always_inline)) {
@@ -915,6 +956,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a
   wait_vm<0>();  // (transfers of no bytes write zeros)
   barrier();     // every read of K and V tiles is done: LDS is free
 
+  Args z = arguments();
   float l_tot = pair_sum(l_run);
   if constexpr (PAGED) {
     // (a page that is not in the cache may be some rows' only: all of the block come out as NaN, and those that do not
@@ -927,7 +969,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a
     if (*any_lost) l_tot = NAN;
     __syncthreads();
   }
-  if (parts == 1) {
+  if (whole) {
     // out[row][32d + 8i + 4g + j] = o[d][4i + j] / l, by way of LDS, so that whole rows are stored
     constexpr int PITCH = ROWB + 16;
     static_assert(4 * 32 * PITCH <= 4 * TILE, "the output's slots fit the LDS");
@@ -952,23 +994,23 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a
     const int r0 = lane / CPR, col = lane % CPR * 8;
 #pragma unroll
     for (int i = 0; i < 32 / RPI; i++) {
-      const int r = r0 + i * RPI, lr = list0 + r, token = lr / a.group, h = hk * a.group + lr - token * a.group;
-      if (r < wave_rows && col < a.d)
-        *(half8_t*)(a.out + (int64_t)h * a.so_z + (int64_t)(q.row0 + token) * a.so_y + col) =
+      const int r = r0 + i * RPI, lr = list0 + r, token = lr / z.group, h = hk * z.group + lr - token * z.group;
+      if (r < wave_rows && col < z.d)
+        *(half8_t*)(z.out + (int64_t)h * z.so_z + (int64_t)(q.row0 + token) * z.so_y + col) =
             *(const half8_t*)(slot + r * PITCH + col * 2);
     }
     // A value that is no number times the zero of a key that the row does not see is no zero: such rows are computed
     // again from the keys that they see.
     const uint64_t lanes = __ballot(!finite);
-    if (lanes && q.rows > 1 && causal) {
+    if (lanes && q.rows > 1 && z.mask == ADR_MASK_CAUSAL) {
       const uint32_t bad = (uint32_t)lanes | (uint32_t)(lanes >> 32);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (behind the stores above)
       for (int r = 0; r < wave_rows; r++)
-        if (bad >> r & 1) row_by_wave(arguments_again(), q, (list0 + r) / a.group, hk * a.group + (list0 + r) % a.group, lane);
+        if (bad >> r & 1) row_by_wave(arguments(), q, (list0 + r) / z.group, hk * z.group + (list0 + r) % z.group, lane);
     }
   } else if (frow < wave_rows) {
-    const int64_t prow = ((int64_t)(slot0 + part) * a.kv_heads + hk) * ROWS + w * 32 + frow;
-    float* const po = share.part_o + prow * HD + 4 * g;
+    const int64_t prow = ((int64_t)(2 * index + (place != stretch0)) * z.kv_heads + hk) * ROWS + w * 32 + frow;
+    float* const po = z.part_o + prow * HD + 4 * g;
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -978,63 +1020,91 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(SequencesArgs a
         for (int j = 0; j < 4; j++) r[j] = o[d][4 * i + j];
         *(float4_t*)(po + 32 * d + 8 * i) = r;
       }
-    if (g == 0) share.part_ml[prow] = make_float2(m_run, l_tot);
+    if (g == 0) z.part_ml[prow] = make_float2(m_run, l_tot);
+  }
+  if (!SHARED || next_place >= stretch1) break;
+  __syncthreads();  // (the next block's transfers go where the results are read)
+  Args n = arguments();
+  roster.load(n, n.shift, thread_index() & 63, 0, 0);  // (not kept in registers meanwhile)
   }
 }
 
-// Sums the parts of a divided block: a wavefront to a row, 16 rows to a workgroup, HD / 64 columns to a lane; parts in order.
+// Sums the parts of the blocks that lie in several workgroups' stretches, in order: a thread to 4 columns of a row, as
+// many rows at once as 256 threads have.  Workgroup `bound` of a key head looks where stretch `bound` begins, and takes the
+// block that lies around that place if no stretch before begins in it.
 template <int HD, int ROWS, int KEYS>
-__global__ __launch_bounds__(256) void attention_join_kernel(SequencesArgs a, Share share) {
-  constexpr int C = HD / 64;
-  typedef float vec_t __attribute__((ext_vector_type(C)));
-  typedef half_t hvec_t __attribute__((ext_vector_type(C)));
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+__global__ __launch_bounds__(256) void attention_join_kernel(Job) {
+  constexpr int COLS = HD / 4, AT_ONCE = 256 / COLS < ROWS ? 256 / COLS : ROWS, GROUPS = ROWS / AT_ONCE;
+  __shared__ int bad_rows;  // whose result is not finite
+  const int tid = threadIdx.x, lane = tid & 63;
+  Args a = arguments();
   const int hk = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
-  constexpr int GROUPS = ROWS / 16;
-  Piece pc;
-  if (!find_piece<ROWS, KEYS, true>(a, share, rest / GROUPS, lane, pc)) return;
-  const int rows = min(ROWS, pc.q.rows * a.group - pc.block * ROWS);
-  for (int r = rest % GROUPS * 16 + w; r < min(rows, rest % GROUPS * 16 + 16); r += 4) {
-    const int64_t first = ((int64_t)pc.slot * a.kv_heads + hk) * ROWS + r, step = (int64_t)a.kv_heads * ROWS;
-    vec_t acc = 0.0f;
+  Roster<ROWS, KEYS, true> roster;
+  const Line line = roster.line_of(a, lane);
+  const int bound = rest / GROUPS + 1;
+  if (bound >= line.parts) return;
+  Block b;
+  if (!roster.block_at(a, a.shift, line.at(bound), lane, b) || b.offset == 0) return;
+  const int begin = line.at(bound) - b.offset, before = line.at(bound - 1);
+  if (before > begin) return;
+  const int rows = min(ROWS, b.q.rows * a.group - b.block * ROWS), r0 = rest % GROUPS * AT_ONCE;
+  if (r0 >= rows) return;
+  // stretches bound - 1 ... last; the first of them has the block behind others, unless it begins with it
+  const int last = (int)(((int64_t)(begin + b.pieces) * line.parts - 1) / line.total), parts = last - bound + 2;
+  const int slot = 2 * (bound - 1) + (before != begin);
+  const int r = r0 + tid / COLS, col = tid % COLS * 4;
+  if (tid == 0) bad_rows = 0;
+  __syncthreads();
+  if (r < rows && r - r0 < AT_ONCE) {
+    auto row_of = [&](int part) __attribute__((always_inline)) {
+      return ((int64_t)(part == 0 ? slot : 2 * (bound - 1 + part)) * a.kv_heads + hk) * ROWS + r;
+    };
+    constexpr int UNROLL = 8;
     float m = NO_SCORE, l = 0.0f;
-    for (int s0 = 0; s0 < pc.parts; s0 += 64) {
-      const float2 ml = s0 + lane < pc.parts ? share.part_ml[first + (s0 + lane) * step] : make_float2(NO_SCORE, 0.0f);
-      float top = ml.x;
-      for (int i = 1; i < 64; i <<= 1) top = fmaxf(top, __shfl_xor(top, i));
-      const float m_new = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - m_new);
-      m = m_new;
-      const float f = __builtin_amdgcn_exp2f(ml.x - m);
-      float sum = ml.y * f;
-      for (int i = 1; i < 64; i <<= 1) sum += __shfl_xor(sum, i);
-      l = l * alpha + sum;
-      acc *= alpha;
-      const int n = min(64, pc.parts - s0);
-      for (int s = 0; s < n; s += 8) {
-        vec_t v[8];
+    for (int s = 0; s < parts; s += UNROLL) {
+      float2 ml[UNROLL];
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-          v[j] = *(const vec_t*)(share.part_o + (first + (s0 + min(s + j, n - 1)) * step) * HD + lane * C);
+      for (int j = 0; j < UNROLL; j++) ml[j] = a.part_ml[row_of(min(s + j, parts - 1))];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float fj = __shfl(f, s + j);
-          if (s + j < n) acc += v[j] * fj;
-        }
-      }
+      for (int j = 0; j < UNROLL; j++) m = fmaxf(m, ml[j].x);
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    acc *= inv;
-    const int lr = pc.block * ROWS + r, token = lr / a.group, h = hk * a.group + lr - token * a.group;
+    float4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < parts; s += UNROLL) {
+      float2 ml[UNROLL];
+      float4_t v[UNROLL];
+#pragma unroll
+      for (int j = 0; j < UNROLL; j++) {
+        const int64_t row = row_of(min(s + j, parts - 1));
+        ml[j] = a.part_ml[row];
+        v[j] = *(const float4_t*)(a.part_o + row * HD + col);
+      }
+#pragma unroll
+      for (int j = 0; j < UNROLL; j++)
+        if (s + j < parts) {
+          const float f = __builtin_amdgcn_exp2f(ml[j].x - m);
+          l += ml[j].y * f;
+          acc += v[j] * f;
+        }
+    }
+    acc *= l == 0.0f ? 0.0f : 1.0f / l;
+    const int lr = b.block * ROWS + r, token = lr / a.group, h = hk * a.group + lr - token * a.group;
+    half4_t out;
     bool finite = true;
 #pragma unroll
-    for (int j = 0; j < C; j++) finite = finite && fabsf(acc[j]) < INFINITY;
-    if (__ballot(!finite) && pc.q.rows > 1 && a.mask == ADR_MASK_CAUSAL) {
-      row_by_wave(arguments_again(), pc.q, token, h, lane);
-      continue;
+    for (int j = 0; j < 4; j++) {
+      finite = finite && fabsf(acc[j]) < INFINITY;
+      out[j] = (half_t)acc[j];
     }
-    if (lane * C < a.d)
-      *(hvec_t*)(a.out + (int64_t)h * a.so_z + (int64_t)(pc.q.row0 + token) * a.so_y + lane * C) =
-          __builtin_convertvector(acc, hvec_t);
+    if (!finite) atomicOr(&bad_rows, 1 << (r - r0));
+    if (col < a.d) *(half4_t*)(a.out + (int64_t)h * a.so_z + (int64_t)(b.q.row0 + token) * a.so_y + col) = out;
+  }
+  if (b.q.rows > 1 && a.mask == ADR_MASK_CAUSAL) {  // (as above)
+    __syncthreads();
+    for (int x = tid >> 6; x < AT_ONCE; x += 4)
+      if (bad_rows >> x & 1) {
+        const int lr = b.block * ROWS + r0 + x;
+        row_by_wave(arguments(), b.q, lr / a.group, hk * a.group + lr % a.group, lane);
+      }
   }
 }
 
@@ -1043,10 +1113,6 @@ __global__ __launch_bounds__(256) void attention_join_kernel(SequencesArgs a, Sh
 // ---- the choice ---------------------------------------------------------------------------------------------
 
 namespace {
-
-constexpr int FEW = 16, FEW_KEYS = 32, FEW_WAVES = 2, MANY = 128, MANY_KEYS = 64;
-// (a few more than the division above can come to: its sum of work is rounded)
-constexpr int SPARE = 8;
 
 int page_shift(int page_size) { return page_size >= 16 && (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1; }
 
@@ -1065,17 +1131,22 @@ int64_t slot_bytes(int rows, int hd) { return (int64_t)rows * (hd * 4 + 8); }
 }  // namespace
 
 SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
-  SequencesPlan p = {SequencesPlan::ANY_LAYOUT, 0, 0, 0};
+  SequencesPlan p = {SequencesPlan::ANY_LAYOUT, 0, 0, 0, 0};
   if (!chunks(a)) return p;
   const int longest_rows = a.longest_rows > 0 ? std::min(a.longest_rows, a.rows) : a.rows;
   p.kind = (int64_t)longest_rows * a.group <= FEW ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES;
   const bool few = p.kind == SequencesPlan::FEW_ROWS;
   const int64_t slot = slot_bytes(few ? FEW : MANY, a.d <= 64 ? 64 : 128) * a.kv_heads;
   p.parts = std::max(1, 2 * cus / a.kv_heads);
-  p.min_steps = 8;
+  p.least = 2;
+  // (pieces grow where there could be more of them than the line counts)
+  const int64_t most_keys = a.table ? std::min((int64_t)a.table_width * a.page_size, (int64_t)MOST_KEYS) : a.keys;
+  const double most_tiles = ((double)a.rows * a.group / (few ? FEW : MANY) + a.sequences) * (most_keys / (few ? FEW_KEYS : MANY_KEYS) + 2.0);
+  for (p.shift = few ? FEW_SHIFT : MANY_SHIFT; most_tiles > ldexp(0x1p29, p.shift) && p.shift < 25; p.shift++) {}
   if (!few && (int64_t)a.rows * a.heads / MANY >= 2 * cus) p.parts = 0;
-  p.parts = (int)std::max<int64_t>(0, std::min<int64_t>(p.parts, (avail / slot - SPARE) / 2));
-  p.workspace_bytes = p.parts > 0 ? (2 * p.parts + SPARE) * slot : 0;
+  p.parts = (int)std::min<int64_t>(p.parts, avail / (2 * slot));
+  if (p.parts < 2) p.parts = 0;
+  p.workspace_bytes = 2 * p.parts * slot;
   return p;
 }
 
@@ -1083,23 +1154,29 @@ template <int HD, bool PAGED>
 static hipError_t launch_blocks(hipStream_t stream, const SequencesArgs& a, const SequencesPlan& p, void* workspace) {
   const bool few = p.kind == SequencesPlan::FEW_ROWS;
   const int rows = few ? FEW : MANY;
-  Share share = {p.parts, p.min_steps, (float*)workspace, nullptr};
-  if (p.parts > 0) share.part_ml = (float2*)((float*)workspace + ((int64_t)2 * p.parts + SPARE) * a.kv_heads * rows * HD);
-  const Pages pages = {PAGED ? page_shift(a.page_size) : 0};
-  const int64_t blocks = ((int64_t)a.rows * a.group / rows + a.sequences + share.parts + SPARE) * a.kv_heads;  // at most
+  Job job;
+  (SequencesArgs&)job = a;
+  job.page_shift = PAGED ? page_shift(a.page_size) : 0;
+  job.parts = p.parts, job.shift = p.shift, job.least = p.least;
+  job.part_o = (float*)workspace;
+  job.part_ml = p.parts > 0 ? (float2*)((float*)workspace + (int64_t)2 * p.parts * a.kv_heads * rows * HD) : nullptr;
+  // Unshared: as many as there can be blocks.
+  const int64_t blocks = (p.parts > 0 ? p.parts : (int64_t)a.rows * a.group / rows + a.sequences) * a.kv_heads;
   if (blocks > 0x7fffffff / 256) return hipErrorInvalidConfiguration;
-  const dim3 grid((unsigned)blocks);
-  if (few)
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, FEW_WAVES>), grid, dim3(64 * FEW_WAVES), 0, stream,
-                       a, share, pages);
-  else
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, PAGED>), grid, dim3(256), 0, stream, a, share, pages);
-  if (p.parts > 0) {
-    const dim3 join((unsigned)(p.parts * a.kv_heads * (rows / 16)));
-    if (few)
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, FEW, FEW_KEYS>), join, dim3(256), 0, stream, a, share);
-    else
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, MANY, MANY_KEYS>), join, dim3(256), 0, stream, a, share);
+  const int at_once = std::min(rows, 1024 / HD);  // rows of the joining workgroups
+  const dim3 grid((unsigned)blocks), join((unsigned)(p.parts * a.kv_heads * (rows / at_once)));
+  if (few && p.parts > 0) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, FEW_WAVES, true>), grid, dim3(64 * FEW_WAVES), 0,
+                       stream, job);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, FEW, FEW_KEYS>), join, dim3(256), 0, stream, job);
+  } else if (few) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, FEW_WAVES, false>), grid, dim3(64 * FEW_WAVES), 0,
+                       stream, job);
+  } else if (p.parts > 0) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, PAGED, true>), grid, dim3(256), 0, stream, job);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, MANY, MANY_KEYS>), join, dim3(256), 0, stream, job);
+  } else {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, PAGED, false>), grid, dim3(256), 0, stream, job);
   }
   return hipGetLastError();
 }
@@ -1108,7 +1185,9 @@ hipError_t launch_attention_sequences(hipStream_t stream, const SequencesArgs& a
   if (p.kind == SequencesPlan::ANY_LAYOUT) {
     const int64_t waves = (int64_t)a.rows * a.heads;
     const int64_t grid = std::min<int64_t>((waves + 3) / 4, 1 << 22);
-    hipLaunchKernelGGL(attention_any_layout_kernel, dim3((unsigned)grid), dim3(256), 0, stream, a);
+    Job job = {};
+    (SequencesArgs&)job = a;
+    hipLaunchKernelGGL(attention_any_layout_kernel, dim3((unsigned)grid), dim3(256), 0, stream, job);
     return hipGetLastError();
   }
   if (a.d <= 64) return a.table ? launch_blocks<64, true>(stream, a, p, workspace) : launch_blocks<64, false>(stream, a, p, workspace);

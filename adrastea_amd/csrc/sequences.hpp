@@ -50,8 +50,9 @@ struct SequencesArgs {
 // Which kernel, and how the keys are shared over workgroups (attention_sequences.hip).
 struct SequencesPlan {
   enum Kind { ANY_LAYOUT, FEW_ROWS, TILES } kind;
-  int parts;      // of all sequences' work, for each key head; 0: no keys are shared
-  int min_steps;  // key tiles that a workgroup has at least, where keys are shared
+  int parts;  // workgroups of each key head that share all its work; 0: one for each block of rows
+  int shift;  // log2 of the key tiles of a piece of the work
+  int least;  // pieces that each workgroup has at least
   int64_t workspace_bytes;
 };
 SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail);
