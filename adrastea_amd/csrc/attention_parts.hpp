@@ -82,12 +82,21 @@ __device__ __forceinline__ void dma_buffer_pair(uint32_t lds, uint32_t voff0, ui
                "buffer_load_dwordx4 %2, %3, 0 offen offset:%5 lds"
                :: "s"(lds), "v"(voff0), "v"(voff1), "s"(desc), "n"(FIRST * 1024), "n"(FIRST * 1024 + 1024) : "memory");
 }
-// The same for what is read once: the lines are the first to leave the caches.
-template <int FIRST>
-__device__ __forceinline__ void dma_buffer_pair_once(uint32_t lds, uint32_t voff0, uint32_t voff1, u32x4_t desc) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %3, 0 offen offset:%4 nt lds\n\t"
-               "buffer_load_dwordx4 %2, %3, 0 offen offset:%5 nt lds"
-               :: "s"(lds), "v"(voff0), "v"(voff1), "s"(desc), "n"(FIRST * 1024), "n"(FIRST * 1024 + 1024) : "memory");
+// N transfers in a row of what is read once (its lines are the first to leave the caches); the j-th one's offset of j KiB
+// counts on both sides.
+template <int N>
+__device__ __forceinline__ void dma_buffer_once(uint32_t lds, const uint32_t (&voff)[N], u32x4_t desc) {
+  static_assert(N == 2 || N == 4, "16 rows of 64 or 128 values");
+  if constexpr (N == 4)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %5, 0 offen nt lds\n\t"
+                 "buffer_load_dwordx4 %2, %5, 0 offen offset:1024 nt lds\n\t"
+                 "buffer_load_dwordx4 %3, %5, 0 offen offset:2048 nt lds\n\t"
+                 "buffer_load_dwordx4 %4, %5, 0 offen offset:3072 nt lds"
+                 :: "s"(lds), "v"(voff[0]), "v"(voff[1]), "v"(voff[2]), "v"(voff[3]), "s"(desc) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %3, 0 offen nt lds\n\t"
+                 "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 nt lds"
+                 :: "s"(lds), "v"(voff[0]), "v"(voff[1]), "s"(desc) : "memory");
 }
 __device__ __forceinline__ void dma_global(uint32_t lds, const void* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, off"

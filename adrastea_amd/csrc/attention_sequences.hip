@@ -282,7 +282,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Job) {
   constexpr int KS = HD / 32, DB = HD / 16;         // k-steps of S, blocks of 16 output columns
   constexpr int WAVE = 4 * TILE;                    // K0 K1 V0 V1 of a wavefront
   constexpr int PITCH = HD + 4;                     // of the partial results' rows, in floats
-  constexpr int BIAS = 1024;                        // bytes that descriptors start ahead, so that no offset is negative
+  constexpr int BIAS = NI / 2 * 1024;               // bytes that descriptors start ahead, so that no offset is negative
   static_assert(16 * (PITCH + 2) * 4 + 16 <= WAVE, "the partial results fit the tiles' LDS");
   __shared__ __attribute__((aligned(1024))) unsigned char smem[WAVES * WAVE];
 
@@ -323,46 +323,48 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Job) {
     int krow, kc;
     k_chunk_inv<CPR>(j * 64 + lane, krow, kc);
     const int vrow = (j * 64 + lane) / CPR, vc = (lane % CPR) ^ v_swz8<CPR>(vrow);
-    koff[j] = kc * 8 < a.d ? (uint32_t)((krow * (int)a.sk.y + kc * 8) * 2 + BIAS - (j & 1) * 1024) : 0x7fff0000u;
-    voff[j] = vc * 8 < a.d ? (uint32_t)((vrow * (int)a.sv.y + vc * 8) * 2 + BIAS - (j & 1) * 1024) : 0x7fff0000u;
+    koff[j] = kc * 8 < a.d ? (uint32_t)((krow * (int)a.sk.y + kc * 8) * 2 + BIAS - j * 1024) : 0x7fff0000u;
+    voff[j] = vc * 8 < a.d ? (uint32_t)((vrow * (int)a.sv.y + vc * 8) * 2 + BIAS - j * 1024) : 0x7fff0000u;
   }
-  // The pages of 32 of the wavefront's tiles at a time, a lane to each 16 keys.
-  int page = 0;
+  // Where the keys and values of 32 of the wavefront's tiles lie, a lane to each 16 keys: their addresses are worked
+  // out by the vector ALU once, not by scalar instructions for each tile.  (Addresses are even: an odd one says that there
+  // are keys.)
+  uint64_t k_at = 0, v_at = 0;
   bool lost = false;  // a key's page is not in the cache
   auto look_up = [&](int i) __attribute__((always_inline)) {
     const int key = (tile0 + w + WAVES * (i + (lane >> 1))) * KEYS + 16 * (lane & 1);
-    page = 0;
+    k_at = v_at = 0;  // (no keys)
     if (key < row_end) {
-      page = a.table[(int64_t)q.index * a.table_pitch + (key >> a.page_shift)];
-      if (page < 0 || page >= a.pages) lost = true, page = -1;
+      int64_t ko = key * a.sk.y, vo = key * a.sv.y;
+      bool good = true;
+      if constexpr (PAGED) {
+        const int page = a.table[(int64_t)q.index * a.table_pitch + (key >> a.page_shift)];
+        const int slot = key & ((1 << a.page_shift) - 1);
+        good = page >= 0 && page < a.pages;
+        ko = page * a.sk.p + slot * a.sk.y;
+        vo = page * a.sv.p + slot * a.sv.y;
+      }
+      lost |= !good;
+      if (good) k_at = ((uint64_t)(K + ko) - BIAS) | 1, v_at = ((uint64_t)(V + vo) - BIAS) | 1;
     }
   };
   // Keys, or values, of tile i.
   auto fetch = [&](int i, auto is_k) __attribute__((always_inline)) {
     constexpr bool IS_K = decltype(is_k)::value;
-    const auto& st = IS_K ? a.sk : a.sv;
+    const int stride = (int)(IS_K ? a.sk.y : a.sv.y);
+    const uint64_t at = IS_K ? k_at : v_at;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      const int key = (tile0 + w + WAVES * i) * KEYS + 16 * h;
-      int left = min(row_end - key, 16);
-      int64_t at = key * st.y;
-      if constexpr (PAGED) {
-        const int p = __builtin_amdgcn_readlane(page, 2 * (i & 31) + h), slot = key & ((1 << a.page_shift) - 1);
-        if (p < 0) left = 0;
-        at = p * st.p + slot * st.y;
-      }
-      const u32x4_t desc = descriptor((uint64_t)((IS_K ? K : V) + at) - BIAS,
-                                      left > 0 ? ((left - 1) * (int)st.y + a.d) * 2 + BIAS : 0);
-      const uint32_t dst = lds0 + ((IS_K ? 0 : 2) + (i & 1)) * TILE + h * (NI / 2) * 1024;
-      const uint32_t(&off)[NI / 2] = IS_K ? koff : voff;
-#pragma unroll
-      for (int j = 0; j < NI / 2; j += 2) dma_buffer_pair_once<0>(dst + j * 1024, off[j], off[j + 1], desc);
+      const int l = 2 * (i & 31) + h, left = min(row_end - (tile0 + w + WAVES * i) * KEYS - 16 * h, 16);
+      const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)at, l), hi = __builtin_amdgcn_readlane((uint32_t)(at >> 32), l);
+      const u32x4_t desc = {lo & ~1u, hi & 0xffffu, lo & 1 ? (uint32_t)(((left - 1) * stride + a.d) * 2 + BIAS) : 0u, 0x00020000u};
+      dma_buffer_once<NI / 2>(lds0 + ((IS_K ? 0 : 2) + (i & 1)) * TILE + h * (NI / 2) * 1024, IS_K ? koff : voff, desc);
     }
   };
   const std::true_type is_k{};
   const std::false_type is_v{};
 
-  if constexpr (PAGED) look_up(0);
+  look_up(0);
   half8_t qf[KS];
   const half_t* const qrow =
       a.q + (int64_t)(hk * a.group + gh) * a.sq_z + (int64_t)(q.row0 + row) * a.sq_y;
@@ -410,9 +412,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Job) {
         s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[ks], s[kb], 0, 0, 0);
       }
     if constexpr (MORE) {
-      if constexpr (PAGED) {
-        if (((i + 2) & 31) == 0) look_up(i + 2);
-      }
+      if (((i + 2) & 31) == 0) look_up(i + 2);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       fetch(i + 2, is_k);
     }
@@ -625,31 +625,35 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
     koff[j] = kc * 8 < a.d ? (uint32_t)((krow * (int)a.sk.y + kc * 8) * 2 + BIAS - j * 1024) : 0x7fff0000u;
     voff[j] = vc * 8 < a.d ? (uint32_t)((vrow * (int)a.sv.y + vc * 8) * 2 + BIAS - j * 1024) : 0x7fff0000u;
   }
-  // The wavefront's next 16 key and value rows: base address, bytes from there to the last key (0 behind it), and the
-  // pages of 64 tiles at a time, a lane to each.
+  // The wavefront's next 16 key and value rows: address, and bytes from there to the last key (0 behind it).  On
+  // pages, the addresses of 64 tiles at a time, a lane to each, worked out by the vector ALU.  (Addresses are even: an
+  // odd one says that there is one.)
   struct Next {
-    uint64_t base, p;
+    uint64_t base, p, pages;
     int64_t page_stride;
-    int bytes, key, stride, page;
+    int bytes, key, stride;
   };
   bool lost = false;  // a key's page is not in the cache
   auto locate = [&](Next& t) __attribute__((always_inline)) {
-    const int n = ((t.key - 16 * w) >> 6) - tile0;
-    int left = min(row_end - t.key, 16);
+    const int left = min(row_end - t.key, 16);
+    t.bytes = left > 0 ? ((left - 1) * t.stride + a.d) * 2 + BIAS : 0;
     if constexpr (PAGED) {
+      const int n = ((t.key - 16 * w) >> 6) - tile0;
       if ((n & 63) == 0) {
         const int key = t.key + lane * KEYS;
-        t.page = 0;
+        t.pages = 0;
         if (key < row_end) {
-          t.page = a.table[(int64_t)q.index * a.table_pitch + (key >> a.page_shift)];
-          if (t.page < 0 || t.page >= a.pages) lost = true, t.page = -1;
+          const int page = a.table[(int64_t)q.index * a.table_pitch + (key >> a.page_shift)];
+          const int slot = key & ((1 << a.page_shift) - 1);
+          if (page < 0 || page >= a.pages) lost = true;
+          else t.pages = (t.base + 2 * (page * t.page_stride + slot * (int64_t)t.stride)) | 1;
         }
       }
-      const int p = __builtin_amdgcn_readlane(t.page, n & 63), slot = t.key & ((1 << a.page_shift) - 1);
-      if (p < 0) left = 0;
-      t.p = t.base + 2 * (p * t.page_stride + slot * (int64_t)t.stride);
+      const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)t.pages, n & 63);
+      const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(t.pages >> 32), n & 63);
+      t.p = (uint64_t)hi << 32 | (lo & ~1u);
+      if (!(lo & 1)) t.bytes = 0;
     }
-    t.bytes = left > 0 ? ((left - 1) * t.stride + a.d) * 2 + BIAS : 0;
   };
   auto first_tile = [&](const half_t* base, int64_t stride, int64_t page_stride) __attribute__((always_inline)) {
     Next t;
@@ -657,7 +661,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
     t.page_stride = page_stride;
     t.stride = (int)stride;
     t.key = tile0 * KEYS + 16 * w;
-    t.page = 0;
+    t.pages = 0;
     t.p = t.base + 2 * (t.key * stride);
     locate(t);
     return t;
@@ -1052,39 +1056,54 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Job) {
   // stretches bound - 1 ... last; the first of them has the block behind others, unless it begins with it
   const int last = (int)(((int64_t)(begin + b.pieces) * line.parts - 1) / line.total), parts = last - bound + 2;
   const int slot = 2 * (bound - 1) + (before != begin);
-  const int r = r0 + tid / COLS, col = tid % COLS * 4;
+  // Few rows leave threads over: these share the parts.
+  const int items = min(rows - r0, AT_ONCE) * COLS, sharers = 256 / items, sharer = tid / items, item = tid - sharer * items;
+  const int r = r0 + item / COLS, col = item % COLS * 4;
+  __shared__ float4_t sums[256];
+  __shared__ float2 mls[256];
   if (tid == 0) bad_rows = 0;
-  __syncthreads();
-  if (r < rows && r - r0 < AT_ONCE) {
-    auto row_of = [&](int part) __attribute__((always_inline)) {
-      return ((int64_t)(part == 0 ? slot : 2 * (bound - 1 + part)) * a.kv_heads + hk) * ROWS + r;
-    };
+  auto row_of = [&](int part) __attribute__((always_inline)) {
+    return ((int64_t)(part == 0 ? slot : 2 * (bound - 1 + part)) * a.kv_heads + hk) * ROWS + r;
+  };
+  float m = NO_SCORE, l = 0.0f;
+  float4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (sharer < sharers) {
     constexpr int UNROLL = 8;
-    float m = NO_SCORE, l = 0.0f;
-    for (int s = 0; s < parts; s += UNROLL) {
-      float2 ml[UNROLL];
-#pragma unroll
-      for (int j = 0; j < UNROLL; j++) ml[j] = a.part_ml[row_of(min(s + j, parts - 1))];
-#pragma unroll
-      for (int j = 0; j < UNROLL; j++) m = fmaxf(m, ml[j].x);
-    }
-    float4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < parts; s += UNROLL) {
+    for (int s = sharer; s < parts; s += UNROLL * sharers) {
       float2 ml[UNROLL];
       float4_t v[UNROLL];
 #pragma unroll
       for (int j = 0; j < UNROLL; j++) {
-        const int64_t row = row_of(min(s + j, parts - 1));
+        const int64_t row = row_of(min(s + j * sharers, parts - 1));
         ml[j] = a.part_ml[row];
         v[j] = *(const float4_t*)(a.part_o + row * HD + col);
       }
+      float top = m;
+#pragma unroll
+      for (int j = 0; j < UNROLL; j++) top = fmaxf(top, ml[j].x);  // (the last part may be among them several times)
+      const float alpha = __builtin_amdgcn_exp2f(m - top);
+      m = top;
+      l *= alpha;
+      acc *= alpha;
 #pragma unroll
       for (int j = 0; j < UNROLL; j++)
-        if (s + j < parts) {
+        if (s + j * sharers < parts) {
           const float f = __builtin_amdgcn_exp2f(ml[j].x - m);
           l += ml[j].y * f;
           acc += v[j] * f;
         }
+    }
+  }
+  sums[tid] = acc;
+  mls[tid] = make_float2(m, l);
+  __syncthreads();
+  if (sharer == 0) {
+    for (int s = 1; s < sharers; s++) {
+      const float2 ml = mls[s * items + item];
+      const float top = fmaxf(m, ml.x), f0 = __builtin_amdgcn_exp2f(m - top), f1 = __builtin_amdgcn_exp2f(ml.x - top);
+      m = top;
+      l = l * f0 + ml.y * f1;
+      acc = acc * f0 + sums[s * items + item] * f1;
     }
     acc *= l == 0.0f ? 0.0f : 1.0f / l;
     const int lr = b.block * ROWS + r, token = lr / a.group, h = hk * a.group + lr - token * a.group;
@@ -1138,7 +1157,7 @@ SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
   const bool few = p.kind == SequencesPlan::FEW_ROWS;
   const int64_t slot = slot_bytes(few ? FEW : MANY, a.d <= 64 ? 64 : 128) * a.kv_heads;
   p.parts = std::max(1, 2 * cus / a.kv_heads);
-  p.least = 2;
+  p.least = 1;
   // (pieces grow where there could be more of them than the line counts)
   const int64_t most_keys = a.table ? std::min((int64_t)a.table_width * a.page_size, (int64_t)MOST_KEYS) : a.keys;
   const double most_tiles = ((double)a.rows * a.group / (few ? FEW : MANY) + a.sequences) * (most_keys / (few ? FEW_KEYS : MANY_KEYS) + 2.0);

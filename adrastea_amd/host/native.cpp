@@ -21,7 +21,8 @@ PyObject *layout_type, *view_type;                      // the classes of tensor
 PyObject *of_general, *permute_general, *cast_general;  // their definitions of the methods below
 PyObject *current_device, *raw_stream;                  // torch's functions
 PyObject *s_shape, *s_stride, *s_dims, *s_strides, *s_storage, *s_layout, *s_offset, *s_data_ptr, *s_load, *s_store,
-    *s_mask, *s_op, *s_scale, *s_beta, *s_bias, *s_is_contiguous;
+    *s_mask, *s_op, *s_scale, *s_beta, *s_bias, *s_is_contiguous, *s_get_device, *s_key, *s_value, *s_row_offsets, *s_lengths,
+    *s_table, *s_key_offsets, *s_longest_rows, *s_longest, *s_turns, *s_rotary_layout, *s_magnitude;
 
 decltype(&adr_matmul_f16) matmul_fn;
 decltype(&adr_attention_f16) attention_fn;
@@ -30,6 +31,10 @@ decltype(&adr_matmul_nt_fp16u8) matmul_u8_fn;
 decltype(&adr_quantize_absmax_u8) quantize_fn;
 decltype(&adr_dequantize_absmax_u8) dequantize_fn;
 decltype(&adr_error_stats_f16) error_stats_fn[2];
+decltype(&adr_rotary_f16) rotary_fn;
+decltype(&adr_append_f16) append_fn;
+decltype(&adr_attention_paged_f16) paged_fn;
+decltype(&adr_attention_packed_f16) packed_fn;
 
 // A reference that is given back at the end of its scope.
 struct Ref {
@@ -425,6 +430,198 @@ PyObject* error_stats(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromLong(rc);
 }
 
+// ---- several sequences at once.  The handles of kernels.py have checked types and devices of their tensors when they
+// were made; sizes, strides and addresses are read at each call.
+
+// torch's current stream on its current device, and that device
+bool read_device(int64_t& device, adr_stream_t& s) {
+  const Ref dev(PyObject_CallNoArgs(current_device));
+  if (!as_int(dev, device)) return false;
+  const Ref raw(PyObject_CallOneArg(raw_stream, dev));
+  int64_t v;
+  if (!as_int(raw, v)) return false;
+  s = (adr_stream_t)(uintptr_t)v;
+  return true;
+}
+
+bool on_device(PyObject* tensor, int64_t device) {
+  int64_t v;
+  return call_int(tensor, s_get_device, v) && v == device;
+}
+
+// A [heads, rows, d] view (rank 2: one head) of a tensor on `device`
+struct Rows {
+  int32_t heads, rows, d, x, y, z;
+  void* ptr;
+};
+bool read_rows(PyObject* view, int64_t device, Rows& r) {
+  Layout l;
+  if ((PyObject*)Py_TYPE(view) != view_type || !read_layout(view, l) || (l.rank != 2 && l.rank != 3) || !read_ptr(view, r.ptr))
+    return false;
+  const Ref storage(attr(view, s_storage));
+  if (!storage.p || !on_device(storage, device)) return false;
+  for (int i = 0; i < l.rank; i++)
+    if (l.dims[i] > INT32_MAX || l.strides[i] > INT32_MAX || l.strides[i] < INT32_MIN) return false;
+  r.heads = l.rank == 3 ? (int32_t)l.dims[0] : 1;
+  r.rows = (int32_t)last(l.dims, l, 2), r.d = (int32_t)last(l.dims, l, 1);
+  r.x = (int32_t)last(l.strides, l, 1), r.y = (int32_t)last(l.strides, l, 2), r.z = l.rank == 3 ? (int32_t)l.strides[0] : 0;
+  return true;
+}
+
+// A tensor of `rank` dimensions on `device`: sizes and address
+bool read_index(PyObject* tensor, int rank, int64_t device, int64_t (&dims)[MAX_RANK], void*& ptr) {
+  if (!tensor) return false;
+  const Ref shape(attr(tensor, s_shape));
+  return shape.p && PyTuple_Check(shape) && read_ints(shape, dims, rank) && on_device(tensor, device) && read_ptr(tensor, ptr);
+}
+
+bool read_int32(PyObject* o, PyObject* name, int32_t& v) {
+  const Ref r(attr(o, name));
+  int64_t x;
+  if (!as_int(r, x) || x > INT32_MAX || x < INT32_MIN) return false;
+  v = (int32_t)x;
+  return true;
+}
+
+bool read_cache(PyObject* o, int64_t device, adr_paged_cache& c) {
+  Layout l[2];
+  const Ref views[2] = {Ref(attr(o, s_key)), Ref(attr(o, s_value))};
+  void* p[2];
+  for (int i = 0; i < 2; i++) {
+    if (!views[i].p || (PyObject*)Py_TYPE(views[i].p) != view_type || !read_layout(views[i], l[i]) || l[i].rank != 4 ||
+        !read_ptr(views[i], p[i]))
+      return false;
+    const Ref storage(attr(views[i], s_storage));
+    if (!storage.p || !on_device(storage, device)) return false;
+  }
+  for (int i = 0; i < 4; i++)
+    if (l[0].dims[i] != l[1].dims[i] || l[0].dims[i] > INT32_MAX) return false;
+  c = {(uint16_t*)p[0], (uint16_t*)p[1], (int32_t)l[0].dims[0], (int32_t)l[0].dims[1], (int32_t)l[0].dims[2],
+       (int32_t)l[0].dims[3], l[0].strides[3], l[0].strides[2], l[0].strides[1], l[0].strides[0],
+       l[1].strides[3], l[1].strides[2], l[1].strides[1], l[1].strides[0]};
+  return true;
+}
+
+bool read_paged_batch(PyObject* o, int64_t device, adr_paged_batch& b) {
+  const Ref offsets(attr(o, s_row_offsets)), lengths(attr(o, s_lengths)), table(attr(o, s_table));
+  int64_t n[MAX_RANK], m[MAX_RANK], t[MAX_RANK], stride[MAX_RANK];
+  void *po, *pl, *pt;
+  if (!read_index(offsets, 1, device, n, po) || !read_index(lengths, 1, device, m, pl) || !read_index(table, 2, device, t, pt) ||
+      n[0] != m[0] + 1 || t[0] != m[0] || m[0] < 1 || t[0] > INT32_MAX || t[1] > INT32_MAX)
+    return false;
+  const Ref strides(call(table, s_stride));
+  int rank = 2;
+  if (!strides.p || !read_ints(strides, stride, rank) || stride[1] != 1 || stride[0] > INT32_MAX || stride[0] < t[1]) return false;
+  b = {(const int32_t*)po, (const int32_t*)pl, (const int32_t*)pt, (int32_t)m[0], (int32_t)t[1], (int32_t)stride[0], 0, 0};
+  return read_int32(o, s_longest_rows, b.longest_rows) && read_int32(o, s_longest, b.longest);
+}
+
+bool read_rotary(PyObject* o, int64_t device, adr_rotary& r) {
+  const Ref turns(attr(o, s_turns)), magnitude(attr(o, s_magnitude));
+  int64_t n[MAX_RANK];
+  void* p;
+  double m;
+  int32_t layout;
+  if (!read_index(turns, 1, device, n, p) || n[0] > INT32_MAX / 2 || !read_double(magnitude, m) ||
+      !read_int32(o, s_rotary_layout, layout))
+    return false;
+  r = {(const double*)p, (int32_t)n[0] * 2, (uint32_t)layout, (float)m};
+  return true;
+}
+
+// rotary_f16(output, input, positions, rotary)
+PyObject* rotary_f16(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t device, count[MAX_RANK];
+  adr_stream_t stream;
+  Rows o, x;
+  adr_rotary r;
+  void* p;
+  if (n != 4 || !rotary_fn || !read_device(device, stream) || !read_rows(a[0], device, o) || !read_rows(a[1], device, x) ||
+      !read_index(a[2], 1, device, count, p) || !read_rotary(a[3], device, r) || o.heads != x.heads || o.rows != x.rows ||
+      o.d != x.d || count[0] != x.rows)
+    return general();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = rotary_fn(stream, (uint16_t*)o.ptr, (const uint16_t*)x.ptr, (const int32_t*)p, r, x.heads, x.rows, x.d, o.x, o.y, o.z,
+                 x.x, x.y, x.z);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// append_f16(cache, batch, key, value, rotary, query_out, query, positions); the last four may be None
+PyObject* append_f16(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t device, count[MAX_RANK];
+  adr_stream_t stream;
+  adr_paged_cache c;
+  adr_paged_batch b;
+  adr_rotary r = {nullptr, 0, 0, 1.0f};
+  Rows k, v, o = {}, q = {};
+  void* p = nullptr;
+  if (n != 8 || !append_fn || !read_device(device, stream) || !read_cache(a[0], device, c) ||
+      !read_paged_batch(a[1], device, b) || !read_rows(a[2], device, k) || !read_rows(a[3], device, v) || k.heads != v.heads ||
+      k.rows != v.rows || k.d != v.d || k.heads != c.kv_heads || k.d != c.d || (a[5] == Py_None) != (a[6] == Py_None))
+    return general();
+  if (a[4] != Py_None && !read_rotary(a[4], device, r)) return general();
+  if (a[6] != Py_None && (!read_rows(a[5], device, o) || !read_rows(a[6], device, q) || o.heads != q.heads || o.rows != q.rows ||
+                          o.d != q.d || q.rows != k.rows || q.d != k.d))
+    return general();
+  if (a[7] != Py_None && (!read_index(a[7], 1, device, count, p) || count[0] != k.rows)) return general();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = append_fn(stream, c, b, (const uint16_t*)k.ptr, (const uint16_t*)v.ptr, (uint16_t*)o.ptr, (const uint16_t*)q.ptr,
+                 (const int32_t*)p, r, q.heads, k.rows, k.x, k.y, k.z, v.x, v.y, v.z, o.x, o.y, o.z, q.x, q.y, q.z);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// attention_paged_f16(output, query, cache, batch, scale, temperature, mask)
+PyObject* attention_paged_f16(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t device, mask;
+  adr_stream_t stream;
+  adr_paged_cache c;
+  adr_paged_batch b;
+  Rows o, q;
+  double scale, temp;
+  if (n != 7 || !paged_fn || !read_device(device, stream) || !read_rows(a[0], device, o) || !read_rows(a[1], device, q) ||
+      !read_cache(a[2], device, c) || !read_paged_batch(a[3], device, b) || !read_double(a[4], scale) ||
+      !read_double(a[5], temp) || !as_int(a[6], mask) || o.heads != q.heads || o.rows != q.rows || o.d != q.d || q.d != c.d)
+    return general();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = paged_fn(stream, (uint16_t*)o.ptr, (const uint16_t*)q.ptr, c, b, q.heads, q.rows, o.x, o.y, o.z, q.x, q.y, q.z,
+                (float)scale, (float)temp, (uint32_t)mask);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// attention_packed_f16(output, query, key, value, batch, scale, temperature, mask)
+PyObject* attention_packed_f16(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t device, mask, rows[MAX_RANK], keys[MAX_RANK];
+  adr_stream_t stream;
+  adr_packed_batch b;
+  Rows o, q, k, v;
+  double scale, temp;
+  void *pr, *pk;
+  if (n != 8 || !packed_fn || !read_device(device, stream) || !read_rows(a[0], device, o) || !read_rows(a[1], device, q) ||
+      !read_rows(a[2], device, k) || !read_rows(a[3], device, v) || !read_double(a[5], scale) || !read_double(a[6], temp) ||
+      !as_int(a[7], mask) || o.heads != q.heads || o.rows != q.rows || o.d != q.d || k.heads != v.heads || k.rows != v.rows ||
+      k.d != v.d || k.d != q.d)
+    return general();
+  const Ref row_offsets(attr(a[4], s_row_offsets)), key_offsets(attr(a[4], s_key_offsets));
+  if (!read_index(row_offsets, 1, device, rows, pr) || !read_index(key_offsets, 1, device, keys, pk) || rows[0] != keys[0] ||
+      rows[0] < 1 || rows[0] > INT32_MAX || !read_int32(a[4], s_longest_rows, b.longest_rows) ||
+      !read_int32(a[4], s_longest, b.longest))
+    return general();
+  b.row_offsets = (const int32_t*)pr, b.key_offsets = (const int32_t*)pk, b.sequences = (int32_t)rows[0] - 1;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = packed_fn(stream, (uint16_t*)o.ptr, (const uint16_t*)q.ptr, (const uint16_t*)k.ptr, (const uint16_t*)v.ptr, b, q.heads,
+                 k.heads, q.rows, k.rows, q.d, o.x, o.y, o.z, q.x, q.y, q.z, k.x, k.y, k.z, v.x, v.y, v.z, (float)scale,
+                 (float)temp, (uint32_t)mask);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
 #define ADR_METHOD(f) (PyCFunction)(void (*)(void))f, METH_FASTCALL | METH_KEYWORDS
 PyMethodDef of_def = {"of", ADR_METHOD(view_of), "View of a torch tensor with its own sizes and strides."};
 PyMethodDef permute_def = {"permute", ADR_METHOD(view_permute), nullptr};
@@ -475,6 +672,17 @@ PyObject* bind(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
+// bind_sequences(addresses of the functions over several sequences): beside bind, whose torch functions they use
+PyObject* bind_sequences(PyObject*, PyObject* args) {
+  unsigned long long p[4];
+  if (!PyArg_ParseTuple(args, "KKKK", p, p + 1, p + 2, p + 3)) return nullptr;
+  rotary_fn = (decltype(rotary_fn))p[0];
+  append_fn = (decltype(append_fn))p[1];
+  paged_fn = (decltype(paged_fn))p[2];
+  packed_fn = (decltype(packed_fn))p[3];
+  Py_RETURN_NONE;
+}
+
 #define ADR_FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"install", install, METH_VARARGS, nullptr},
                          {"bind", bind, METH_VARARGS, nullptr},
@@ -485,6 +693,11 @@ PyMethodDef methods[] = {{"install", install, METH_VARARGS, nullptr},
                          ADR_FAST(quantize_absmax_uint8),
                          ADR_FAST(dequantize_absmax_uint8),
                          ADR_FAST(error_stats),
+                         {"bind_sequences", bind_sequences, METH_VARARGS, nullptr},
+                         ADR_FAST(rotary_f16),
+                         ADR_FAST(append_f16),
+                         ADR_FAST(attention_paged_f16),
+                         ADR_FAST(attention_packed_f16),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
@@ -495,7 +708,10 @@ PyMODINIT_FUNC PyInit__native() {
       {&s_shape, "shape"}, {&s_stride, "stride"}, {&s_dims, "dims"}, {&s_strides, "strides"}, {&s_storage, "storage"},
       {&s_layout, "layout"}, {&s_offset, "offset"}, {&s_data_ptr, "data_ptr"}, {&s_load, "load_"}, {&s_store, "store_"},
       {&s_mask, "mask_"}, {&s_op, "op"}, {&s_scale, "scale"}, {&s_beta, "beta"}, {&s_bias, "bias"},
-      {&s_is_contiguous, "is_contiguous"}};
+      {&s_is_contiguous, "is_contiguous"}, {&s_get_device, "get_device"}, {&s_key, "key"}, {&s_value, "value"},
+      {&s_row_offsets, "row_offsets"}, {&s_lengths, "lengths"}, {&s_table, "table"}, {&s_key_offsets, "key_offsets"},
+      {&s_longest_rows, "longest_rows"}, {&s_longest, "longest"}, {&s_turns, "turns"}, {&s_rotary_layout, "layout"},
+      {&s_magnitude, "magnitude"}};
   for (const auto& n : names)
     if (!(*n.at = PyUnicode_InternFromString(n.name))) return nullptr;
   return PyModule_Create(&module);

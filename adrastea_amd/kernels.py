@@ -244,6 +244,11 @@ class Rotary:
     layout: int = RotaryLayout.HALVES
     magnitude: float = 1.0
 
+    def __post_init__(self):
+        import torch
+        assert self.turns.dtype == torch.float64 and self.turns.dim() == 1 and self.turns.is_contiguous(), \
+            "turns: a contiguous float64 tensor of rank 1"
+
     @staticmethod
     def new(dims: int, base: float = 10000.0, layout: int = RotaryLayout.HALVES,
             scaling: RotaryScaling = RotaryScaling()) -> "Rotary":
@@ -254,8 +259,7 @@ class Rotary:
 
     @property
     def _desc(self) -> _ffi.RotaryDesc:
-        import torch
-        assert self.turns.dtype == torch.float64 and self.turns.is_contiguous() and self.turns.dim() == 1
+        _here(self.turns)
         return _ffi.RotaryDesc(self.turns.data_ptr(), 2 * self.turns.numel(), self.layout, self.magnitude)
 
 
@@ -269,13 +273,26 @@ class PagedCache:
     key: TensorView
     value: TensorView
 
+    def __post_init__(self):
+        k, v = self.key.layout, self.value.layout
+        assert len(k.dims) == 4 and k.dims == v.dims, "key and value pages are [pages, kv_heads, page_size, d] views"
+
     @property
     def _desc(self) -> _ffi.PagedCacheDesc:
         k, v = self.key.layout, self.value.layout
-        assert len(k.dims) == 4 and k.dims == v.dims, "key and value pages are [pages, kv_heads, page_size, d] views"
+        _here(self.key.storage, self.value.storage)
         p, h, s, d = k.dims
         return _ffi.PagedCacheDesc(self.key.data_ptr(), self.value.data_ptr(), p, h, s, d,
                                    *(t.strides[i] for t in (k, v) for i in (3, 2, 1, 0)))
+
+
+def _here(*storages) -> None:
+    """Device memory of the current device: what a launch there may be given."""
+    import torch
+    device = torch.cuda.current_device()
+    for s in storages:
+        at = getattr(s, "get_device", None)
+        assert at is None or at() == device, f"memory of device {at()} in a call on device {device} (-1: the host)"
 
 
 def _index(t, rank, what):
@@ -297,11 +314,15 @@ class PagedBatch:
     longest_rows: int = 0
     longest: int = 0
 
-    @property
-    def _desc(self) -> _ffi.PagedBatchDesc:
+    def __post_init__(self):
         n = _index(self.lengths, 1, "lengths").shape[0]
         assert _index(self.row_offsets, 1, "row_offsets").shape[0] == n + 1, "row_offsets has one entry more than lengths"
         assert _index(self.table, 2, "table").shape[0] == n, "table has a row for each sequence"
+
+    @property
+    def _desc(self) -> _ffi.PagedBatchDesc:
+        n = self.lengths.shape[0]
+        _here(self.row_offsets, self.lengths, self.table)
         pitch = self.table.stride(0) if n > 1 else self.table.shape[1]
         return _ffi.PagedBatchDesc(self.row_offsets.data_ptr(), self.lengths.data_ptr(), self.table.data_ptr(), n,
                                    self.table.shape[1], pitch, self.longest_rows, self.longest)
@@ -315,10 +336,14 @@ class PackedBatch:
     longest_rows: int = 0
     longest: int = 0
 
-    @property
-    def _desc(self) -> _ffi.PackedBatchDesc:
+    def __post_init__(self):
         n = _index(self.row_offsets, 1, "row_offsets").shape[0]
         assert n >= 1 and _index(self.key_offsets, 1, "key_offsets").shape[0] == n, "offsets of the same sequences"
+
+    @property
+    def _desc(self) -> _ffi.PackedBatchDesc:
+        n = self.row_offsets.shape[0]
+        _here(self.row_offsets, self.key_offsets)
         return _ffi.PackedBatchDesc(self.row_offsets.data_ptr(), self.key_offsets.data_ptr(), n - 1, self.longest_rows,
                                     self.longest)
 
@@ -327,6 +352,7 @@ def _rows_view(view: TensorView, what: str):
     """(heads, rows, d), (x, y, z) strides of a [heads, rows, d] view; rank 2: one head."""
     dims, strides = view.layout.dims, view.layout.strides
     assert len(dims) in (2, 3), f"{what}: a [heads, rows, d] view"
+    _here(view.storage)
     if len(dims) == 2:
         return (1, *dims), (strides[1], strides[0], 0)
     return dims, strides[::-1]
@@ -369,8 +395,18 @@ def _native_binding() -> tuple:
             torch.cuda.current_device, torch._C._cuda_getCurrentRawStream)
 
 
+_NATIVE_SEQUENCE_CALLS = ("adr_rotary_f16", "adr_append_f16", "adr_attention_paged_f16", "adr_attention_packed_f16")
+
+
+@functools.lru_cache(maxsize=None)
+def _native_sequence_binding() -> tuple:
+    lib = _ffi.lib()
+    return tuple(C.cast(getattr(lib, name), C.c_void_p).value for name in _NATIVE_SEQUENCE_CALLS)
+
+
 def _bind_native() -> None:
     _native.bind(*_native_binding())
+    _native.bind_sequences(*_native_sequence_binding())
 
 
 class GpuKernels(CommonKernels):
@@ -481,10 +517,14 @@ class GpuKernels(CommonKernels):
     def rotary_f16(self, output, input, positions, rotary: Rotary):
         """The rows of `input`, a [heads, rows, d] view, turned by positions[row] into `output` (which may be the same
         view).  positions: int32 [rows]."""
+        _index(positions, 1, "positions")
+        if self._lowered("rotary_f16", output, input, positions, rotary):
+            return
         dims, si = _rows_view(input, "input")
         dims_out, so = _rows_view(output, "output")
         assert dims_out == dims, "output and input have one shape"
-        assert _index(positions, 1, "positions").shape[0] == dims[1], "a position for each row"
+        assert positions.shape[0] == dims[1], "a position for each row"
+        _here(positions)
         rc = self._lib.adr_rotary_f16(_current_stream(), output.data_ptr(), input.data_ptr(), positions.data_ptr(),
                                       rotary._desc, *dims, *so, *si)
         if rc != 0:
@@ -495,6 +535,10 @@ class GpuKernels(CommonKernels):
         """The step's keys, turned, and values ([kv_heads, rows, d] views) into their pages, and its queries ([heads,
         rows, d]) turned into `query_out`, which may be the same view.  Row j of the r of sequence s goes to
         place lengths[s] - r + j and is turned by it, or by positions[row] (int32 [rows])."""
+        if positions is not None:
+            _index(positions, 1, "positions")
+        if self._lowered("append_f16", cache, batch, key, value, rotary, query_out, query, positions):
+            return
         c, b = cache._desc, batch._desc
         dims, sk = _rows_view(key, "key")
         dims_v, sv = _rows_view(value, "value")
@@ -507,7 +551,8 @@ class GpuKernels(CommonKernels):
             heads = dims_q[0]
             assert dims_o == dims_q and dims_q[1:] == dims[1:], "query and query_out are [heads, rows, d] views"
         if positions is not None:
-            assert _index(positions, 1, "positions").shape[0] == dims[1], "a position for each row"
+            assert positions.shape[0] == dims[1], "a position for each row"
+            _here(positions)
         rc = self._lib.adr_append_f16(
             _current_stream(), c, b, key.data_ptr(), value.data_ptr(), query_out.data_ptr() if heads else None,
             query.data_ptr() if heads else None, positions.data_ptr() if positions is not None else None,
@@ -519,6 +564,8 @@ class GpuKernels(CommonKernels):
                             temperature: float = 1.0, mask: int = MatmulMask.CAUSAL):
         """Attention of the step's rows ([heads, rows, d] views) over the cache: query head h reads key head
         h / (heads / kv_heads), and under the mask the last row of a sequence sees all its keys."""
+        if self._workspace is None and self._lowered("attention_paged_f16", output, query, cache, batch, scale, temperature, mask):
+            return
         c, b = cache._desc, batch._desc
         dims, sq = _rows_view(query, "query")
         dims_o, so = _rows_view(output, "output")
@@ -534,6 +581,9 @@ class GpuKernels(CommonKernels):
     def attention_packed_f16(self, output, query, key, value, batch: PackedBatch, scale: float,
                              temperature: float = 1.0, mask: int = MatmulMask.CAUSAL):
         """Attention of packed rows ([heads, rows, d] views) over packed keys and values ([kv_heads, keys, d])."""
+        if self._workspace is None and self._lowered("attention_packed_f16", output, query, key, value, batch, scale,
+                                                     temperature, mask):
+            return
         dims, sq = _rows_view(query, "query")
         dims_o, so = _rows_view(output, "output")
         dims_k, sk = _rows_view(key, "key")

@@ -553,11 +553,16 @@ def test_another_stream(kern):
 def test_refusals_of_the_python_interface(kern):
     p = Paged([(2, 20)], 4, 2, 64, 16)
     out, q = heads_view(p.out_t), heads_view(p.q_t)
-    long = PagedBatch(p.batch.row_offsets.long(), p.batch.lengths, p.batch.table)
-    for bad in (long, PagedBatch(p.batch.row_offsets[:1], p.batch.lengths, p.batch.table),
-                PagedBatch(p.batch.row_offsets, p.batch.lengths, p.batch.table.t())):
+    b = p.batch
+    for bad in ((b.row_offsets.long(), b.lengths, b.table), (b.row_offsets[:1], b.lengths, b.table),
+                (b.row_offsets, b.lengths, b.table.t())):
         with pytest.raises(AssertionError):
-            kern.attention_paged_f16(out, q, p.cache, bad, 0.1)
+            PagedBatch(*bad)
+    for elsewhere in (PagedBatch(b.row_offsets.cpu(), b.lengths, b.table), PagedBatch(b.row_offsets, b.lengths, b.table.cpu())):
+        with pytest.raises(AssertionError):
+            kern.attention_paged_f16(out, q, p.cache, elsewhere, 0.1)
+    with pytest.raises(AssertionError):
+        kern.attention_paged_f16(out, heads_view(p.q_t.cpu()), p.cache, b, 0.1)
     with pytest.raises(AssertionError):
         kern.attention_paged_f16(heads_view(p.out_t[:, :2]), q, p.cache, p.batch, 0.1)
     with pytest.raises(AdrasteaError) as e:
