@@ -22,8 +22,10 @@ struct Job : SequencesArgs {
   int parts;        // workgroups of a key head that share its work; 0: unshared
   int shift;        // log2 of a piece's tiles
   int least;        // pieces that a workgroup has at least
+  double per_head;  // 1 / group
   float* part_o;    // [2 * parts][key head][ROWS][HD] unnormalised sums
   float2* part_ml;  // [2 * parts][key head][ROWS] (maximum in log2 units, sum)
+  struct Seam* seams;  // [parts][key head]
 };
 
 // The job is read where it is used, by scalar loads from the kernel's arguments (of which it is the only one): kept in
@@ -35,6 +37,11 @@ __device__ __forceinline__ Args arguments() {
   asm volatile("" : "+s"(p));
   return *(const __attribute__((address_space(4))) Job*)p;
 }
+
+// A list row's row: the quotient is at least 0.5 / group away from the next integer, far more than the product's error.
+__device__ __forceinline__ int row_of_list(Args a, int list_row) { return (int)(((double)list_row + 0.5) * a.per_head); }
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // The thread's index, likewise: what a kernel derives from it for one block is not kept for the next.
 __device__ __forceinline__ int thread_index() {
@@ -158,7 +165,16 @@ __global__ __launch_bounds__(256) void attention_any_layout_kernel(Job) {
 // second launch, in order.
 struct Line {
   int total, parts, shift;  // pieces, workgroups that have some, log2 of a piece's tiles
-  __device__ __forceinline__ int at(int part) const { return (int)((int64_t)total * part / parts); }
+  // (exact: the product has fewer than 53 bits, and a quotient that is no integer lies too far below the next one)
+  __device__ __forceinline__ int at(int part) const { return uniform((int)((double)total * (double)part / (double)parts)); }
+};
+
+// What the second launch needs of the place where a stretch begins, if that is inside a block and no stretch before
+// begins inside the same one: the block, and which slots its parts are in.
+struct Seam {
+  int parts, slot;  // 0: nothing begins here.  The first part's slot; the others' are those of the following stretches' beginnings
+  Sequence q;
+  int block;
 };
 
 struct Block {
@@ -167,7 +183,6 @@ struct Block {
   int offset, pieces;  // of the block: where on the line the asked place lies in it, and all
 };
 
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 __device__ __forceinline__ int add_scan(int v) {  // inclusive, over the lanes of a wavefront
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
@@ -256,6 +271,19 @@ struct Roster {
   }
 };
 
+// The seam at the beginning of stretch `part`, which lies in block b.
+__device__ __forceinline__ Seam seam_at(const Line& line, int part, int place, const Block& b) {
+  Seam s = {0, 0, b.q, b.block};
+  if (part == 0 || b.offset == 0) return s;
+  const int begin = place - b.offset, before = line.at(part - 1);
+  if (before > begin) return s;
+  // stretches part - 1 ... last; the first of them has the block behind others, unless it begins with it
+  const int last = uniform((int)(((double)(begin + b.pieces) * (double)line.parts - 1.0) / (double)line.total));
+  s.parts = last - part + 2;
+  s.slot = 2 * (part - 1) + (before != begin);
+  return s;
+}
+
 // One past the last key that some row of the block sees, and of one row.
 __device__ __forceinline__ int end_of_row(Args a, const Sequence& q, int j) {
   return a.mask == ADR_MASK_CAUSAL ? clamp_to(j + q.keys - q.rows + 1, q.keys) : q.keys;
@@ -275,7 +303,7 @@ __device__ __forceinline__ u32x4_t descriptor(uint64_t p, int bytes) {
 // that a lane holds scores of one row, and O^T = V^T P^T, on MFMA 16x16x32; probabilities are rounded to fp16, the
 // matrix cores' operands, sums and scores stay in 32 bits.
 template <int HD, bool PAGED, int WAVES, bool SHARED>
-__global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Job) {
+__global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) {
   constexpr int CPR = HD / 8, KEYS = 32, ROWS = 16;
   constexpr int ROWB = HD * 2, TILE = KEYS * ROWB;  // bytes of a tile row, of a K or V tile
   constexpr int NI = TILE / 1024;                   // transfers per tile
@@ -284,12 +312,17 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Job) {
   constexpr int PITCH = HD + 4;                     // of the partial results' rows, in floats
   constexpr int BIAS = NI / 2 * 1024;               // bytes that descriptors start ahead, so that no offset is negative
   static_assert(16 * (PITCH + 2) * 4 + 16 <= WAVE, "the partial results fit the tiles' LDS");
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[WAVES * WAVE];
+  // (WAVES * WAVE bytes, asked for at the launch: told of them, the compiler would count one wavefront to a SIMD, hand it
+  // the accumulation registers as well and move every sum in and out of those)
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
 
   const int kv_heads = arguments().kv_heads, hk = blockIdx.x % kv_heads, wg = blockIdx.x / kv_heads;
   Roster<ROWS, KEYS, SHARED> roster;
   const Line line = roster.line_of(arguments(), threadIdx.x & 63);
-  if (wg >= line.parts) return;
+  if (wg >= line.parts) {
+    if (SHARED && threadIdx.x == 0) arguments().seams[wg * kv_heads + hk].parts = 0;
+    return;
+  }
   const int stretch0 = SHARED ? line.at(wg) : wg, stretch1 = SHARED ? line.at(wg + 1) : wg + 1;
   for (int place = stretch0, next_place;; place = next_place) {
   Args a = arguments();
@@ -301,10 +334,11 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Job) {
   const int block = b.block, pieces = min(stretch1 - place, b.pieces - b.offset);
   const bool whole = pieces == b.pieces;
   next_place = place + pieces;
+  if (SHARED && place == stretch0 && tid == 0) a.seams[wg * kv_heads + hk] = seam_at(line, wg, place, b);
   const int rows = min(ROWS, q.rows * a.group - block * ROWS);          // of the block
-  const int list_row = block * ROWS + min(frow, rows - 1), row = list_row / a.group, gh = list_row - row * a.group;
+  const int list_row = block * ROWS + min(frow, rows - 1), row = row_of_list(a, list_row), gh = list_row - row * a.group;
 
-  const int last_end = uniform(end_of_row(a, q, (block * ROWS + rows - 1) / a.group));  // of the block's last row
+  const int last_end = uniform(end_of_row(a, q, row_of_list(a, block * ROWS + rows - 1)));  // of the block's last row
   const int all = (last_end + KEYS - 1) / KEYS;
   const int tile0 = whole ? 0 : min(all, b.offset << line.shift);
   const int tile1 = b.offset + pieces == b.pieces ? all : min(all, (b.offset + pieces) << line.shift);
@@ -445,9 +479,17 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Job) {
     swap_halves(x, y);
     x = fmaxf(x, y), y = x;
     swap_rows(x, y);
-    const float m_new = fmaxf(m_run, fmaxf(x, y) * a.c), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-    m_run = m_new;
-    float sum = 0.0f;
+    // The exponents' reference follows the maximum lazily: it moves when some row has outgrown it by more than 2^8
+    // (probabilities up to 256 are as exact in fp16 as those below 1), and only then are the sums rescaled.
+    const float top = fmaxf(x, y) * a.c;
+    if (__builtin_amdgcn_ballot_w64(top > m_run + 8.0f) != 0) {
+      const float m_new = fmaxf(m_run, top), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; db++) o[db] *= alpha;
+    }
+    float sum[2] = {0.0f, 0.0f};
     u32x4_t pf;
 #pragma unroll
     for (int kb = 0; kb < 2; kb++)
@@ -455,16 +497,16 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Job) {
       for (int r = 0; r < 4; r += 2) {
         float2_t e;
 #pragma unroll
-        for (int j = 0; j < 2; j++) e[j] = __builtin_amdgcn_exp2f(fmaf(s[kb][r + j], a.c, -m_new));
-        sum += e[0] + e[1];
+        for (int j = 0; j < 2; j++) {
+          e[j] = __builtin_amdgcn_exp2f(fmaf(s[kb][r + j], a.c, -m_run));
+          sum[j] += e[j];
+        }
         pf[kb * 2 + r / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(e, half2_t));
       }
-    l_run = l_run * alpha + sum;
+    l_run += sum[0] + sum[1];
 #pragma unroll
-    for (int db = 0; db < DB; db++) {
-      o[db] *= alpha;
+    for (int db = 0; db < DB; db++)
       o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[db], __builtin_bit_cast(half8_t, pf), o[db], 0, 0, 0);
-    }
   };
   const std::true_type yes{};
   const std::false_type no{};
@@ -507,7 +549,7 @@ __global__ __launch_bounds__(64 * WAVES) void attention_few_rows_kernel(Job) {
       sum += *(const float4_t*)(xo + (x * 16 + r) * PITCH + col) * f;
     }
     if (whole) {
-      const int lr = block * ROWS + r, token = lr / z.group, h = hk * z.group + lr - token * z.group;
+      const int lr = block * ROWS + r, token = row_of_list(z, lr), h = hk * z.group + lr - token * z.group;
       half4_t v;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       bool finite = true;
@@ -580,7 +622,10 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
   }
   Roster<ROWS, KEYS, SHARED> roster;
   const Line line = roster.line_of(arguments(), threadIdx.x & 63);
-  if (index >= line.parts) return;
+  if (index >= line.parts) {
+    if (SHARED && threadIdx.x == 0) arguments().seams[index * kv_heads + hk].parts = 0;
+    return;
+  }
   const int stretch0 = SHARED ? line.at(index) : index, stretch1 = SHARED ? line.at(index + 1) : index + 1;
   for (int place = stretch0, next_place;; place = next_place) {
   Args a = arguments();
@@ -592,14 +637,15 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
   const int block = b.block, pieces = min(stretch1 - place, b.pieces - b.offset);
   const bool whole = pieces == b.pieces;
   next_place = place + pieces;
+  if (SHARED && place == stretch0 && tid == 0) a.seams[index * kv_heads + hk] = seam_at(line, index, place, b);
   const int rows = min(ROWS, q.rows * a.group - block * ROWS);  // of the block
   const int wave_rows = min(32, rows - w * 32);                 // of the wavefront (may be negative)
   const int list0 = block * ROWS + w * 32;
   // (lanes without a row of their own compute the block's last one)
-  const int list_row = block * ROWS + min(w * 32 + frow, rows - 1), row = list_row / a.group, gh = list_row - row * a.group;
+  const int list_row = block * ROWS + min(w * 32 + frow, rows - 1), row = row_of_list(a, list_row), gh = list_row - row * a.group;
   const int lane_end = end_of_row(a, q, row);
 
-  const int last_end = uniform(end_of_row(a, q, (block * ROWS + rows - 1) / a.group));
+  const int last_end = uniform(end_of_row(a, q, row_of_list(a, block * ROWS + rows - 1)));
   const int all = (last_end + KEYS - 1) / KEYS;
   const int tile0 = whole ? 0 : min(all, b.offset << line.shift);
   const int steps = (b.offset + pieces == b.pieces ? all : min(all, (b.offset + pieces) << line.shift)) - tile0;
@@ -607,9 +653,9 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
   // Tiles that this wavefront computes: none without rows, none whose first key lies beyond its last row's.
   int active = 0, first_edge = 0;
   if (wave_rows > 0) {
-    active = uniform(clamp_to((end_of_row(a, q, (list0 + wave_rows - 1) / a.group) + KEYS - 1) / KEYS - tile0, steps));
+    active = uniform(clamp_to((end_of_row(a, q, row_of_list(a, list0 + wave_rows - 1)) + KEYS - 1) / KEYS - tile0, steps));
     // the first of them with keys that some row of the wavefront must not see
-    first_edge = uniform(end_of_row(a, q, list0 / a.group)) / KEYS - tile0;
+    first_edge = uniform(end_of_row(a, q, row_of_list(a, list0))) / KEYS - tile0;
   }
 
   const uint32_t lds0 = (uint32_t)(uintptr_t)ADR_LDS_PTR(smem);
@@ -998,7 +1044,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
     const int r0 = lane / CPR, col = lane % CPR * 8;
 #pragma unroll
     for (int i = 0; i < 32 / RPI; i++) {
-      const int r = r0 + i * RPI, lr = list0 + r, token = lr / z.group, h = hk * z.group + lr - token * z.group;
+      const int r = r0 + i * RPI, lr = list0 + r, token = row_of_list(z, lr), h = hk * z.group + lr - token * z.group;
       if (r < wave_rows && col < z.d)
         *(half8_t*)(z.out + (int64_t)h * z.so_z + (int64_t)(q.row0 + token) * z.so_y + col) =
             *(const half8_t*)(slot + r * PITCH + col * 2);
@@ -1033,29 +1079,20 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
   }
 }
 
-// Sums the parts of the blocks that lie in several workgroups' stretches, in order: a thread to 4 columns of a row, as
-// many rows at once as 256 threads have.  Workgroup `bound` of a key head looks where stretch `bound` begins, and takes the
-// block that lies around that place if no stretch before begins in it.
-template <int HD, int ROWS, int KEYS>
+// Sums the parts of the blocks that lie in several workgroups' stretches, in order: a workgroup to a seam, a thread to 4
+// columns of a row, as many rows at once as 256 threads have.
+template <int HD, int ROWS>
 __global__ __launch_bounds__(256) void attention_join_kernel(Job) {
   constexpr int COLS = HD / 4, AT_ONCE = 256 / COLS < ROWS ? 256 / COLS : ROWS, GROUPS = ROWS / AT_ONCE;
   __shared__ int bad_rows;  // whose result is not finite
   const int tid = threadIdx.x, lane = tid & 63;
   Args a = arguments();
   const int hk = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
-  Roster<ROWS, KEYS, true> roster;
-  const Line line = roster.line_of(a, lane);
-  const int bound = rest / GROUPS + 1;
-  if (bound >= line.parts) return;
-  Block b;
-  if (!roster.block_at(a, a.shift, line.at(bound), lane, b) || b.offset == 0) return;
-  const int begin = line.at(bound) - b.offset, before = line.at(bound - 1);
-  if (before > begin) return;
+  const Seam b = a.seams[(rest / GROUPS + 1) * a.kv_heads + hk];
+  const int parts = b.parts, slot = b.slot, next = 2 * (rest / GROUPS);
+  if (parts == 0) return;
   const int rows = min(ROWS, b.q.rows * a.group - b.block * ROWS), r0 = rest % GROUPS * AT_ONCE;
   if (r0 >= rows) return;
-  // stretches bound - 1 ... last; the first of them has the block behind others, unless it begins with it
-  const int last = (int)(((int64_t)(begin + b.pieces) * line.parts - 1) / line.total), parts = last - bound + 2;
-  const int slot = 2 * (bound - 1) + (before != begin);
   // Few rows leave threads over: these share the parts.
   const int items = min(rows - r0, AT_ONCE) * COLS, sharers = 256 / items, sharer = tid / items, item = tid - sharer * items;
   const int r = r0 + item / COLS, col = item % COLS * 4;
@@ -1063,7 +1100,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Job) {
   __shared__ float2 mls[256];
   if (tid == 0) bad_rows = 0;
   auto row_of = [&](int part) __attribute__((always_inline)) {
-    return ((int64_t)(part == 0 ? slot : 2 * (bound - 1 + part)) * a.kv_heads + hk) * ROWS + r;
+    return ((int64_t)(part == 0 ? slot : next + 2 * part) * a.kv_heads + hk) * ROWS + r;
   };
   float m = NO_SCORE, l = 0.0f;
   float4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -1106,7 +1143,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Job) {
       acc = acc * f0 + sums[s * items + item] * f1;
     }
     acc *= l == 0.0f ? 0.0f : 1.0f / l;
-    const int lr = b.block * ROWS + r, token = lr / a.group, h = hk * a.group + lr - token * a.group;
+    const int lr = b.block * ROWS + r, token = row_of_list(a, lr), h = hk * a.group + lr - token * a.group;
     half4_t out;
     bool finite = true;
 #pragma unroll
@@ -1163,9 +1200,10 @@ SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
   const double most_tiles = ((double)a.rows * a.group / (few ? FEW : MANY) + a.sequences) * (most_keys / (few ? FEW_KEYS : MANY_KEYS) + 2.0);
   for (p.shift = few ? FEW_SHIFT : MANY_SHIFT; most_tiles > ldexp(0x1p29, p.shift) && p.shift < 25; p.shift++) {}
   if (!few && (int64_t)a.rows * a.heads / MANY >= 2 * cus) p.parts = 0;
-  p.parts = (int)std::min<int64_t>(p.parts, avail / (2 * slot));
+  const int64_t part = 2 * slot + (int64_t)sizeof(Seam) * a.kv_heads;
+  p.parts = (int)std::min<int64_t>(p.parts, avail / part);
   if (p.parts < 2) p.parts = 0;
-  p.workspace_bytes = 2 * p.parts * slot;
+  p.workspace_bytes = p.parts * part;
   return p;
 }
 
@@ -1178,22 +1216,26 @@ static hipError_t launch_blocks(hipStream_t stream, const SequencesArgs& a, cons
   job.page_shift = PAGED ? page_shift(a.page_size) : 0;
   job.parts = p.parts, job.shift = p.shift, job.least = p.least;
   job.part_o = (float*)workspace;
-  job.part_ml = p.parts > 0 ? (float2*)((float*)workspace + (int64_t)2 * p.parts * a.kv_heads * rows * HD) : nullptr;
+  job.per_head = 1.0 / a.group;
+  const int64_t part_rows = (int64_t)2 * p.parts * a.kv_heads * rows;
+  job.part_ml = (float2*)(job.part_o + (p.parts > 0 ? part_rows * HD : 0));
+  job.seams = (Seam*)(job.part_ml + (p.parts > 0 ? part_rows : 0));
   // Unshared: as many as there can be blocks.
   const int64_t blocks = (p.parts > 0 ? p.parts : (int64_t)a.rows * a.group / rows + a.sequences) * a.kv_heads;
   if (blocks > 0x7fffffff / 256) return hipErrorInvalidConfiguration;
   const int at_once = std::min(rows, 1024 / HD);  // rows of the joining workgroups
-  const dim3 grid((unsigned)blocks), join((unsigned)(p.parts * a.kv_heads * (rows / at_once)));
+  const dim3 grid((unsigned)blocks), join((unsigned)((p.parts - 1) * a.kv_heads * (rows / at_once)));
+  const size_t lds = (size_t)FEW_WAVES * 4 * FEW_KEYS * HD * 2;
   if (few && p.parts > 0) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, FEW_WAVES, true>), grid, dim3(64 * FEW_WAVES), 0,
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, FEW_WAVES, true>), grid, dim3(64 * FEW_WAVES), lds,
                        stream, job);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, FEW, FEW_KEYS>), join, dim3(256), 0, stream, job);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, FEW>), join, dim3(256), 0, stream, job);
   } else if (few) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, FEW_WAVES, false>), grid, dim3(64 * FEW_WAVES), 0,
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, FEW_WAVES, false>), grid, dim3(64 * FEW_WAVES), lds,
                        stream, job);
   } else if (p.parts > 0) {
     hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, PAGED, true>), grid, dim3(256), 0, stream, job);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, MANY, MANY_KEYS>), join, dim3(256), 0, stream, job);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, MANY>), join, dim3(256), 0, stream, job);
   } else {
     hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, PAGED, false>), grid, dim3(256), 0, stream, job);
   }
