@@ -195,7 +195,7 @@ __device__ __forceinline__ int add_scan(int v) {  // inclusive, over the lanes o
 }
 
 // Rows of a block, keys of a tile, log2 of the tiles of a piece
-constexpr int FEW = 16, FEW_KEYS = 32, FEW_SHIFT = 2, FEW_WAVES = 2;  // (two tiles for each wavefront)
+constexpr int FEW = 16, FEW_KEYS = 32, FEW_SHIFT = 2;
 constexpr int MANY = 128, MANY_KEYS = 64, MANY_SHIFT = 1;
 
 // The sequences on the line, 256 at a time: lane l has sequences base + 64 e + l, read from memory once for the whole
@@ -1182,25 +1182,43 @@ bool chunks(const SequencesArgs& a) {
          strides % 8 == 0 && strides >= 0 && near(a.sk.y) && near(a.sv.y) && (!a.table || page_shift(a.page_size) >= 0);
 }
 
-int64_t slot_bytes(int rows, int hd) { return (int64_t)rows * (hd * 4 + 8); }
-
 }  // namespace
 
 SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
-  SequencesPlan p = {SequencesPlan::ANY_LAYOUT, 0, 0, 0, 0};
+  SequencesPlan p = {SequencesPlan::ANY_LAYOUT, 0, 0, 0, 0, 0};
   if (!chunks(a)) return p;
   const int longest_rows = a.longest_rows > 0 ? std::min(a.longest_rows, a.rows) : a.rows;
   p.kind = (int64_t)longest_rows * a.group <= FEW ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES;
   const bool few = p.kind == SequencesPlan::FEW_ROWS;
-  const int64_t slot = slot_bytes(few ? FEW : MANY, a.d <= 64 ? 64 : 128) * a.kv_heads;
-  p.parts = std::max(1, 2 * cus / a.kv_heads);
-  p.least = 1;
-  // (pieces grow where there could be more of them than the line counts)
+  const int rows = few ? FEW : MANY, keys = few ? FEW_KEYS : MANY_KEYS, hd = a.d <= 64 ? 64 : 128;
   const int64_t most_keys = a.table ? std::min((int64_t)a.table_width * a.page_size, (int64_t)MOST_KEYS) : a.keys;
-  const double most_tiles = ((double)a.rows * a.group / (few ? FEW : MANY) + a.sequences) * (most_keys / (few ? FEW_KEYS : MANY_KEYS) + 2.0);
+  const double longest = a.longest > 0 ? std::min<double>(a.longest, most_keys) : most_keys;
+  // blocks: of all key heads, as far as the host can tell
+  const double blocks = std::max((double)a.rows * a.heads / rows, (double)std::min(a.rows, a.sequences) * a.kv_heads);
+  p.least = 1;
+  if (few) {
+    // Two launches take the host and the device some 4 us more than one, and shared keys leave no workgroup with more
+    // than the others.  us, fitted to 16 shapes of 12 to 32 heads, 1 to 256 sequences and 250 to 4000 keys: a block
+    // by itself, four wavefronts to it, 4 + 8.5 per 1000 keys of 128 (one of 500 keys 7.8, shared 9.2; 700 9.1, 9.2; 1000
+    // 14, 10.7); with more blocks than compute units the longest is a tail behind the others (100 sequences of up to 1000
+    // keys, 8 key heads: 41.3, shared 43.7; up to 4000 145, 129).
+    const double alone = longest * hd * 6.6e-5, all = blocks * longest * hd * 4 / 6e6;
+    p.waves = blocks <= cus ? 4 : 2;
+    const bool unshared = blocks <= cus ? 4.0 + alone < 9.3 + all / 2 : alone < 9.0;
+    // Shared: 64 KiB of tiles in flight on a compute unit.  More only crowd each other in the caches (eight sequences of 50000 to
+    // 110000 keys: two workgroups of 64 KiB to a unit 389 us, one 366), but hide the start of short stretches (256
+    // sequences of up to 1000 keys: 98.8, 105).
+    const int each = (hd == 64 ? 2 : 1) * (blocks >= 4.0 * cus ? 2 : 1);
+    p.parts = unshared ? 0 : std::max(1, each * cus / a.kv_heads);
+    if (p.parts > 0) p.waves = 2;
+  } else {
+    p.waves = 4;
+    p.parts = blocks >= 2.0 * cus || longest <= 384 ? 0 : std::max(1, 2 * cus / a.kv_heads);
+  }
+  // (pieces grow where there could be more of them than the line counts)
+  const double most_tiles = ((double)a.rows * a.group / rows + a.sequences) * (most_keys / keys + 2.0);
   for (p.shift = few ? FEW_SHIFT : MANY_SHIFT; most_tiles > ldexp(0x1p29, p.shift) && p.shift < 25; p.shift++) {}
-  if (!few && (int64_t)a.rows * a.heads / MANY >= 2 * cus) p.parts = 0;
-  const int64_t part = 2 * slot + (int64_t)sizeof(Seam) * a.kv_heads;
+  const int64_t part = (2 * (int64_t)rows * (hd * 4 + 8) + (int64_t)sizeof(Seam)) * a.kv_heads;
   p.parts = (int)std::min<int64_t>(p.parts, avail / part);
   if (p.parts < 2) p.parts = 0;
   p.workspace_bytes = p.parts * part;
@@ -1225,14 +1243,15 @@ static hipError_t launch_blocks(hipStream_t stream, const SequencesArgs& a, cons
   if (blocks > 0x7fffffff / 256) return hipErrorInvalidConfiguration;
   const int at_once = std::min(rows, 1024 / HD);  // rows of the joining workgroups
   const dim3 grid((unsigned)blocks), join((unsigned)((p.parts - 1) * a.kv_heads * (rows / at_once)));
-  const size_t lds = (size_t)FEW_WAVES * 4 * FEW_KEYS * HD * 2;
+  const dim3 few_threads(64 * p.waves);
+  const size_t few_lds = (size_t)p.waves * 4 * FEW_KEYS * HD * 2;
   if (few && p.parts > 0) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, FEW_WAVES, true>), grid, dim3(64 * FEW_WAVES), lds,
-                       stream, job);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, 2, true>), grid, few_threads, few_lds, stream, job);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, FEW>), join, dim3(256), 0, stream, job);
+  } else if (few && p.waves == 2) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, 2, false>), grid, few_threads, few_lds, stream, job);
   } else if (few) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, FEW_WAVES, false>), grid, dim3(64 * FEW_WAVES), lds,
-                       stream, job);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, 4, false>), grid, few_threads, few_lds, stream, job);
   } else if (p.parts > 0) {
     hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, PAGED, true>), grid, dim3(256), 0, stream, job);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, MANY>), join, dim3(256), 0, stream, job);

@@ -50,6 +50,7 @@ struct SequencesArgs {
 // Which kernel, and how the keys are shared over workgroups (attention_sequences.hip).
 struct SequencesPlan {
   enum Kind { ANY_LAYOUT, FEW_ROWS, TILES } kind;
+  int waves;  // wavefronts of a workgroup
   int parts;  // workgroups of each key head that share all its work; 0: one for each block of rows
   int shift;  // log2 of the key tiles of a piece of the work
   int least;  // pieces that each workgroup has at least
