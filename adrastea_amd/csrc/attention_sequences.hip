@@ -20,12 +20,12 @@ constexpr float NO_SCORE = -1.0e30f;  // below any score of finite operands; exp
 struct Job : SequencesArgs {
   int page_shift;   // log2 of the slots of a page (16 at least: 16 keys from a multiple of 16 on lie on one page)
   int parts;        // workgroups of a key head that share its work; 0: unshared
-  int shift;        // log2 of a piece's tiles
-  int least;        // pieces that a workgroup has at least
+  int shift;        // few rows: log2 of a piece's tiles
+  int least;        // pieces (many rows: tiles) that a workgroup has at least
   double per_head;  // 1 / group
-  float* part_o;    // [2 * parts][key head][ROWS][HD] unnormalised sums
-  float2* part_ml;  // [2 * parts][key head][ROWS] (maximum in log2 units, sum)
-  struct Seam* seams;  // [parts][key head]
+  float* part_o;    // [slot][key head][ROWS][HD] unnormalised sums
+  float2* part_ml;  // [slot][key head][ROWS] (maximum in log2 units, sum)
+  struct Seam* seams;  // [parts][key head], of many rows half as many
 };
 
 // The job is read where it is used, by scalar loads from the kernel's arguments (of which it is the only one): kept in
@@ -169,10 +169,10 @@ struct Line {
   __device__ __forceinline__ int at(int part) const { return uniform((int)((double)total * (double)part / (double)parts)); }
 };
 
-// What the second launch needs of the place where a stretch begins, if that is inside a block and no stretch before
-// begins inside the same one: the block, and which slots its parts are in.
+// What the second launch needs of a divided block: of few rows, at the place where a stretch begins inside a block and no
+// stretch before begins inside the same one.
 struct Seam {
-  int parts, slot;  // 0: nothing begins here.  The first part's slot; the others' are those of the following stretches' beginnings
+  int parts, slot;  // 0 parts: nothing to do here
   Sequence q;
   int block;
 };
@@ -182,7 +182,6 @@ struct Block {
   int block;           // of the sequence's list
   int offset, pieces;  // of the block: where on the line the asked place lies in it, and all
 };
-
 
 __device__ __forceinline__ int add_scan(int v) {  // inclusive, over the lanes of a wavefront
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
@@ -196,7 +195,7 @@ __device__ __forceinline__ int add_scan(int v) {  // inclusive, over the lanes o
 
 // Rows of a block, keys of a tile, log2 of the tiles of a piece
 constexpr int FEW = 16, FEW_KEYS = 32, FEW_SHIFT = 2;
-constexpr int MANY = 128, MANY_KEYS = 64, MANY_SHIFT = 1;
+constexpr int MANY = 128, MANY_KEYS = 64;
 
 // The sequences on the line, 256 at a time: lane l has sequences base + 64 e + l, read from memory once for the whole
 // division where there are no more.
@@ -282,6 +281,79 @@ __device__ __forceinline__ Seam seam_at(const Line& line, int part, int place, c
   s.parts = last - part + 2;
   s.slot = 2 * (part - 1) + (before != begin);
   return s;
+}
+
+// The share of a workgroup of the kernel for many rows.
+struct Part {
+  Block b;
+  int part, parts;  // of the block's keys
+  int slot;         // of the first part's results: those of a block follow each other
+  int seam;         // divided blocks before this one
+  int seams;        // divided blocks of all
+};
+
+// Part number `index`, of at most 256 sequences (SHARED); false: there are fewer.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ bool part_at(Args a, int index, int lane, Part& p) {
+  constexpr int EACH = 4, UNDIVIDED = 1 << 26;
+  int rows[EACH], keys[EACH], row0[EACH], key0[EACH], blocks[EACH], tiles[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; e++) {
+    row0[e] = rows[e] = key0[e] = keys[e] = 0;
+    if (64 * e < a.sequences && 64 * e + lane < a.sequences) {
+      const Sequence q = sequence_at(a, 64 * e + lane);
+      row0[e] = q.row0, rows[e] = q.rows, key0[e] = q.key0, keys[e] = q.keys;
+    }
+    blocks[e] = (int)(((int64_t)rows[e] * a.group + ROWS - 1) / ROWS);
+    tiles[e] = (keys[e] + KEYS - 1) / KEYS;
+  }
+  auto all_lanes = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(add_scan(v), 63); };
+  // (parts of a block at C tiles to each: exact, as a list row's row is)
+  auto parts_of = [&](int tiles, double inv, int most) __attribute__((always_inline)) {
+    return max(1, (int)(((double)(tiles + most - 1) + 0.5) * inv));
+  };
+  int work = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; e++) work += blocks[e] * min(tiles[e], 1 << 20);  // (blocks: fewer than 2^10)
+  work = all_lanes(work);
+  int most = max(a.least, (work + a.parts - 1) / a.parts);
+  double inv = 0.0;
+  for (int tries = 0;; tries++) {
+    inv = 1.0 / (double)most;
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; e++) n += blocks[e] * parts_of(tiles[e], inv, most);
+    n = all_lanes(n);
+    if (n <= a.parts || most >= UNDIVIDED) break;
+    // (larger in proportion, and so through in a few tries; where there are too many blocks nothing is divided in the end)
+    most = tries < 8 ? max(most + 1, uniform((int)fmin((double)most * n / a.parts, (double)UNDIVIDED))) : UNDIVIDED;
+  }
+  int at = -1, before = 0, slots = 0, seams = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; e++)
+    if (64 * e < a.sequences) {
+      const int each = parts_of(tiles[e], inv, most), mine = blocks[e] * each, divided = each > 1 ? blocks[e] : 0;
+      const int upto = before + add_scan(mine), slots_upto = add_scan(divided * each), seams_upto = add_scan(divided);
+      const uint64_t behind = __ballot(upto > index);
+      if (at < 0 && behind) {
+        at = __builtin_ctzll(behind);
+        const int n = __builtin_amdgcn_readlane(blocks[e], at), parts = __builtin_amdgcn_readlane(each, at);
+        const int in = index - (__builtin_amdgcn_readlane(upto, at) - n * parts), i = uniform(in / parts);
+        p.b.q = {64 * e + at, __builtin_amdgcn_readlane(row0[e], at), __builtin_amdgcn_readlane(rows[e], at),
+                 __builtin_amdgcn_readlane(key0[e], at), __builtin_amdgcn_readlane(keys[e], at)};
+        // (the last blocks first: under the mask they have the most keys)
+        p.b.block = n - 1 - i;
+        p.parts = parts;
+        p.part = in - i * parts;
+        p.slot = slots + __builtin_amdgcn_readlane(slots_upto - divided * each, at) + (parts > 1 ? i * parts : 0);
+        p.seam = seams + __builtin_amdgcn_readlane(seams_upto - divided, at) + (parts > 1 ? i : 0);
+      }
+      before = __builtin_amdgcn_readlane(upto, 63);
+      slots += __builtin_amdgcn_readlane(slots_upto, 63);
+      seams += __builtin_amdgcn_readlane(seams_upto, 63);
+    }
+  p.seams = seams;
+  return at >= 0;
 }
 
 // One past the last key that some row of the block sees, and of one row.
@@ -607,6 +679,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
   constexpr int ROWB = HD * 2;         // bytes per tile row
   constexpr int BIAS = NI * 1024;      // bytes that descriptors start ahead, so that no offset is negative
   __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];  // K0 K1 V0 V1
+  __shared__ int lost_keys[4];  // of each wavefront
 
   // Consecutive workgroups go to different dies; where the key heads divide evenly, a die takes its share of them, so
   // that the blocks which read the same keys meet in one L2.
@@ -620,24 +693,23 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
     hk = blockIdx.x % kv_heads;
     index = blockIdx.x / kv_heads;
   }
-  Roster<ROWS, KEYS, SHARED> roster;
-  const Line line = roster.line_of(arguments(), threadIdx.x & 63);
-  if (index >= line.parts) {
-    if (SHARED && threadIdx.x == 0) arguments().seams[index * kv_heads + hk].parts = 0;
-    return;
-  }
-  const int stretch0 = SHARED ? line.at(index) : index, stretch1 = SHARED ? line.at(index + 1) : index + 1;
-  for (int place = stretch0, next_place;; place = next_place) {
   Args a = arguments();
-  const int tid = thread_index(), lane = tid & 63, w = uniform(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
   const int frow = lane & 31, g = lane >> 5;
-  Block b;
-  if (!roster.block_at(a, a.shift, place, lane, b)) return;
-  const Sequence q = b.q;
-  const int block = b.block, pieces = min(stretch1 - place, b.pieces - b.offset);
-  const bool whole = pieces == b.pieces;
-  next_place = place + pieces;
-  if (SHARED && place == stretch0 && tid == 0) a.seams[index * kv_heads + hk] = seam_at(line, index, place, b);
+  Part pt = {{}, 0, 1, 0, 0, 0};
+  if constexpr (SHARED) {
+    const bool some = part_at<ROWS, KEYS>(a, index, lane, pt);
+    // (the second launch has a workgroup to each two slots)
+    if (tid == 0 && index >= pt.seams && index < a.parts / 2) a.seams[index * kv_heads + hk].parts = 0;
+    if (!some) return;
+    if (tid == 0 && pt.part == 0 && pt.parts > 1) a.seams[pt.seam * kv_heads + hk] = Seam{pt.parts, pt.slot, pt.b.q, pt.b.block};
+  } else {
+    Roster<ROWS, KEYS, false> roster;
+    roster.load(a, 0, lane, 0, 0);
+    if (!roster.block_at(a, 0, index, lane, pt.b)) return;
+  }
+  const Sequence q = pt.b.q;
+  const int block = pt.b.block, part = pt.part, parts = pt.parts, slot0 = pt.slot;
   const int rows = min(ROWS, q.rows * a.group - block * ROWS);  // of the block
   const int wave_rows = min(32, rows - w * 32);                 // of the wavefront (may be negative)
   const int list0 = block * ROWS + w * 32;
@@ -647,8 +719,9 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
 
   const int last_end = uniform(end_of_row(a, q, row_of_list(a, block * ROWS + rows - 1)));
   const int all = (last_end + KEYS - 1) / KEYS;
-  const int tile0 = whole ? 0 : min(all, b.offset << line.shift);
-  const int steps = (b.offset + pieces == b.pieces ? all : min(all, (b.offset + pieces) << line.shift)) - tile0;
+  // (exact, as above)
+  auto cut = [&](int i) __attribute__((always_inline)) { return uniform((int)((double)all * (double)i / (double)parts)); };
+  const int tile0 = SHARED ? cut(part) : 0, steps = (SHARED ? cut(part + 1) : all) - tile0;
   const int row_end = min(last_end, (tile0 + steps) * KEYS);
   // Tiles that this wavefront computes: none without rows, none whose first key lies beyond its last row's.
   int active = 0, first_edge = 0;
@@ -673,27 +746,30 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
   }
   // The wavefront's next 16 key and value rows: address, and bytes from there to the last key (0 behind it).  On
   // pages, the addresses of 64 tiles at a time, a lane to each, worked out by the vector ALU.  (Addresses are even: an
-  // odd one says that there is one.)
+  // odd one says that there is one.)  Keys are ahead of values: theirs bring the pages, which the values take over.
   struct Next {
     uint64_t base, p, pages;
     int64_t page_stride;
     int bytes, key, stride;
   };
   bool lost = false;  // a key's page is not in the cache
-  auto locate = [&](Next& t) __attribute__((always_inline)) {
+  int page = 0;
+  auto locate = [&](Next& t, auto is_k) __attribute__((always_inline)) {
     const int left = min(row_end - t.key, 16);
     t.bytes = left > 0 ? ((left - 1) * t.stride + a.d) * 2 + BIAS : 0;
     if constexpr (PAGED) {
       const int n = ((t.key - 16 * w) >> 6) - tile0;
       if ((n & 63) == 0) {
         const int key = t.key + lane * KEYS;
-        t.pages = 0;
-        if (key < row_end) {
-          const int page = a.table[(int64_t)q.index * a.table_pitch + (key >> a.page_shift)];
-          const int slot = key & ((1 << a.page_shift) - 1);
-          if (page < 0 || page >= a.pages) lost = true;
-          else t.pages = (t.base + 2 * (page * t.page_stride + slot * (int64_t)t.stride)) | 1;
+        if constexpr (decltype(is_k)::value) {
+          page = -1;
+          if (key < row_end) {
+            page = a.table[(int64_t)q.index * a.table_pitch + (key >> a.page_shift)];
+            if (page < 0 || page >= a.pages) lost = true, page = -1;
+          }
         }
+        const int slot = key & ((1 << a.page_shift) - 1);
+        t.pages = page < 0 ? 0 : (t.base + 2 * (page * t.page_stride + slot * (int64_t)t.stride)) | 1;
       }
       const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)t.pages, n & 63);
       const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(t.pages >> 32), n & 63);
@@ -701,7 +777,9 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
       if (!(lo & 1)) t.bytes = 0;
     }
   };
-  auto first_tile = [&](const half_t* base, int64_t stride, int64_t page_stride) __attribute__((always_inline)) {
+  const std::true_type is_k{};
+  const std::false_type is_v{};
+  auto first_tile = [&](const half_t* base, int64_t stride, int64_t page_stride, auto k) __attribute__((always_inline)) {
     Next t;
     t.base = (uint64_t)(base + (PAGED ? 0 : q.key0 * stride)) - BIAS;
     t.page_stride = page_stride;
@@ -709,7 +787,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
     t.key = tile0 * KEYS + 16 * w;
     t.pages = 0;
     t.p = t.base + 2 * (t.key * stride);
-    locate(t);
+    locate(t, k);
     return t;
   };
   half8_t qf[DS];  // (operand B of S^T = K Q^T: lane -> row frow, head-dimension group g)
@@ -719,11 +797,11 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
     qf[ds] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
     if (ds * 16 + g * 8 < a.d) qf[ds] = *(const half8_t*)(qrow + ds * 16);
   }
-  Next nk = first_tile(a.k + hk * a.sk.z, a.sk.y, a.sk.p), nv = first_tile(a.v + hk * a.sv.z, a.sv.y, a.sv.p);
-  auto advance = [&](Next& t) __attribute__((always_inline)) {
+  Next nk = first_tile(a.k + hk * a.sk.z, a.sk.y, a.sk.p, is_k), nv = first_tile(a.v + hk * a.sv.z, a.sv.y, a.sv.p, is_v);
+  auto advance = [&](Next& t, auto k) __attribute__((always_inline)) {
     t.key += KEYS;
     if constexpr (!PAGED) t.p += (uint32_t)t.stride * (KEYS * 2u);
-    locate(t);
+    locate(t, k);
   };
   // Transfers 2 j and 2 j + 1 of the NI that bring a tile into buffer `buf` (0, 1: K; 2, 3: V).
   auto transfer = [&](const Next& t, auto is_k, int buf, auto pair) __attribute__((always_inline)) {
@@ -733,14 +811,12 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
     if constexpr (decltype(is_k)::value) dma_buffer_pair<J>(dst, koff[J], koff[J + 1], desc);
     else dma_buffer_pair<J>(dst, voff[J], voff[J + 1], desc);
   };
-  const std::true_type is_k{};
-  const std::false_type is_v{};
   const std::integral_constant<int, 0> pair0{};
   const std::integral_constant<int, NI / 2 - 1> pair1{};  // (the last pair; HD = 64 has one)
   auto tile_transfers = [&](Next& t, auto k, int buf) __attribute__((always_inline)) {
     transfer(t, k, buf, pair0);
     if constexpr (NI > 2) transfer(t, k, buf, pair1);
-    advance(t);
+    advance(t, k);
   };
   // What is waited for at the end of each half: all transfers but those issued in it.
   auto wait_landed = [&]() __attribute__((always_inline)) { wait_vm<NI>(); };
@@ -882,7 +958,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
       asm volatile("" : "+v"(l_run));
     }
     if constexpr (HD == 128) __builtin_amdgcn_s_setprio(0);
-    advance(nv);
+    advance(nv, is_v);
     wait_landed();
     barrier();
   };
@@ -961,7 +1037,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
           for (int r = 0; r < 16; r++) o[dt][r] *= alpha;
       }
     }
-    advance(nk);
+    advance(nk, is_k);
     wait_landed();
     barrier();
   };
@@ -1004,22 +1080,20 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
   }
   for (; i < steps; i++) idle(i);  // tiles this wavefront has no part in
   wait_vm<0>();  // (transfers of no bytes write zeros)
-  barrier();     // every read of K and V tiles is done: LDS is free
+  if constexpr (PAGED) {
+    if (lane == 0) lost_keys[w] = __ballot(lost) != 0;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+  barrier();  // every read of K and V tiles is done: LDS is free
 
   Args z = arguments();
   float l_tot = pair_sum(l_run);
   if constexpr (PAGED) {
     // (a page that is not in the cache may be some rows' only: all of the block come out as NaN, and those that do not
     // see it are computed again below)
-    int* const any_lost = (int*)smem;
-    if (tid == 0) *any_lost = 0;
-    __syncthreads();
-    if (__ballot(lost) && lane == 0) *any_lost = 1;
-    __syncthreads();
-    if (*any_lost) l_tot = NAN;
-    __syncthreads();
+    if (lost_keys[0] | lost_keys[1] | lost_keys[2] | lost_keys[3]) l_tot = NAN;
   }
-  if (whole) {
+  if (!SHARED || parts == 1) {
     // out[row][32d + 8i + 4g + j] = o[d][4i + j] / l, by way of LDS, so that whole rows are stored
     constexpr int PITCH = ROWB + 16;
     static_assert(4 * 32 * PITCH <= 4 * TILE, "the output's slots fit the LDS");
@@ -1044,6 +1118,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
     const int r0 = lane / CPR, col = lane % CPR * 8;
 #pragma unroll
     for (int i = 0; i < 32 / RPI; i++) {
+      if (i * RPI >= wave_rows) break;
       const int r = r0 + i * RPI, lr = list0 + r, token = row_of_list(z, lr), h = hk * z.group + lr - token * z.group;
       if (r < wave_rows && col < z.d)
         *(half8_t*)(z.out + (int64_t)h * z.so_z + (int64_t)(q.row0 + token) * z.so_y + col) =
@@ -1059,7 +1134,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
         if (bad >> r & 1) row_by_wave(arguments(), q, (list0 + r) / z.group, hk * z.group + (list0 + r) % z.group, lane);
     }
   } else if (frow < wave_rows) {
-    const int64_t prow = ((int64_t)(2 * index + (place != stretch0)) * z.kv_heads + hk) * ROWS + w * 32 + frow;
+    const int64_t prow = ((int64_t)(slot0 + part) * z.kv_heads + hk) * ROWS + w * 32 + frow;
     float* const po = z.part_o + prow * HD + 4 * g;
 #pragma unroll
     for (int d = 0; d < DT; d++)
@@ -1072,11 +1147,6 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
       }
     if (g == 0) z.part_ml[prow] = make_float2(m_run, l_tot);
   }
-  if (!SHARED || next_place >= stretch1) break;
-  __syncthreads();  // (the next block's transfers go where the results are read)
-  Args n = arguments();
-  roster.load(n, n.shift, thread_index() & 63, 0, 0);  // (not kept in registers meanwhile)
-  }
 }
 
 // Sums the parts of the blocks that lie in several workgroups' stretches, in order: a workgroup to a seam, a thread to 4
@@ -1088,8 +1158,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Job) {
   const int tid = threadIdx.x, lane = tid & 63;
   Args a = arguments();
   const int hk = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
-  const Seam b = a.seams[(rest / GROUPS + 1) * a.kv_heads + hk];
-  const int parts = b.parts, slot = b.slot, next = 2 * (rest / GROUPS);
+  // (few rows: stretch s begins in slot 2 s, and the part before the seam is in front of that or of the one before)
+  constexpr bool STRETCHES = ROWS == FEW;
+  const int seam = rest / GROUPS + STRETCHES;
+  const Seam b = a.seams[seam * a.kv_heads + hk];
+  const int parts = b.parts, slot = b.slot, next = STRETCHES ? 2 * (seam - 1) : slot, step = STRETCHES ? 2 : 1;
   if (parts == 0) return;
   const int rows = min(ROWS, b.q.rows * a.group - b.block * ROWS), r0 = rest % GROUPS * AT_ONCE;
   if (r0 >= rows) return;
@@ -1100,7 +1173,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Job) {
   __shared__ float2 mls[256];
   if (tid == 0) bad_rows = 0;
   auto row_of = [&](int part) __attribute__((always_inline)) {
-    return ((int64_t)(part == 0 ? slot : next + 2 * part) * a.kv_heads + hk) * ROWS + r;
+    return ((int64_t)(part == 0 ? slot : next + step * part) * a.kv_heads + hk) * ROWS + r;
   };
   float m = NO_SCORE, l = 0.0f;
   float4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -1212,13 +1285,22 @@ SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
     p.parts = unshared ? 0 : std::max(1, each * cus / a.kv_heads);
     if (p.parts > 0) p.waves = 2;
   } else {
+    // A tile takes a workgroup about a microsecond (0.75 at 64 values) whatever its rows are, two on a compute unit 1.4 as
+    // long.  Shared: the parts' way through memory, 130 KB for a workgroup, is weighed against the tiles that each has.
     p.waves = 4;
-    p.parts = blocks >= 2.0 * cus || longest <= 384 ? 0 : std::max(1, 2 * cus / a.kv_heads);
+    p.least = 4;
+    const double tile = hd == 64 ? 0.75 : 0.96, way = hd == 64 ? 0.0135 : 0.027;
+    const double tiles = longest / MANY_KEYS + 1, work = blocks * tiles;
+    const double n = std::min(2.0 * cus, std::max(blocks, sqrt(work * tile / way)));
+    const bool unshared = a.sequences > 256 || blocks >= 2.0 * cus ||
+                          7 + tiles * tile <= 11 + (n > cus ? 1.4 : 1.0) * work * tile / n + n * way;
+    p.parts = unshared ? 0 : (int)(n / a.kv_heads);
   }
   // (pieces grow where there could be more of them than the line counts)
   const double most_tiles = ((double)a.rows * a.group / rows + a.sequences) * (most_keys / keys + 2.0);
-  for (p.shift = few ? FEW_SHIFT : MANY_SHIFT; most_tiles > ldexp(0x1p29, p.shift) && p.shift < 25; p.shift++) {}
-  const int64_t part = (2 * (int64_t)rows * (hd * 4 + 8) + (int64_t)sizeof(Seam)) * a.kv_heads;
+  for (p.shift = FEW_SHIFT; most_tiles > ldexp(0x1p29, p.shift) && p.shift < 25; p.shift++) {}
+  // (slots: two to a stretch of few rows, one to a part of many)
+  const int64_t part = ((few ? 2 : 1) * (int64_t)rows * (hd * 4 + 8) + (int64_t)sizeof(Seam)) * a.kv_heads;
   p.parts = (int)std::min<int64_t>(p.parts, avail / part);
   if (p.parts < 2) p.parts = 0;
   p.workspace_bytes = p.parts * part;
@@ -1235,14 +1317,15 @@ static hipError_t launch_blocks(hipStream_t stream, const SequencesArgs& a, cons
   job.parts = p.parts, job.shift = p.shift, job.least = p.least;
   job.part_o = (float*)workspace;
   job.per_head = 1.0 / a.group;
-  const int64_t part_rows = (int64_t)2 * p.parts * a.kv_heads * rows;
+  const int64_t part_rows = (int64_t)(few ? 2 : 1) * p.parts * a.kv_heads * rows;
   job.part_ml = (float2*)(job.part_o + (p.parts > 0 ? part_rows * HD : 0));
   job.seams = (Seam*)(job.part_ml + (p.parts > 0 ? part_rows : 0));
-  // Unshared: as many as there can be blocks.
-  const int64_t blocks = (p.parts > 0 ? p.parts : (int64_t)a.rows * a.group / rows + a.sequences) * a.kv_heads;
+  // Unshared: as many as there can be blocks.  Shared: a stretch to each, or a part.
+  const int64_t most = (int64_t)a.rows * a.group / rows + a.sequences;  // blocks of a key head
+  const int64_t blocks = (p.parts == 0 ? most : few ? p.parts : std::max<int64_t>(p.parts, most)) * a.kv_heads;
   if (blocks > 0x7fffffff / 256) return hipErrorInvalidConfiguration;
   const int at_once = std::min(rows, 1024 / HD);  // rows of the joining workgroups
-  const dim3 grid((unsigned)blocks), join((unsigned)((p.parts - 1) * a.kv_heads * (rows / at_once)));
+  const dim3 grid((unsigned)blocks), join((unsigned)((few ? p.parts - 1 : p.parts / 2) * a.kv_heads * (rows / at_once)));
   const dim3 few_threads(64 * p.waves);
   const size_t few_lds = (size_t)p.waves * 4 * FEW_KEYS * HD * 2;
   if (few && p.parts > 0) {
