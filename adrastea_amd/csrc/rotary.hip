@@ -7,6 +7,7 @@
 // turns are taken off in 64 bits, and what is left, at most half a turn, goes through the 32-bit sincospi.
 // Each is computed once per row and pair, by a thread of its own, and shared by all heads through LDS.
 #include <algorithm>
+#include <type_traits>
 
 #include "sequences.hpp"
 
@@ -21,34 +22,127 @@ struct RowPlace {   // of one row of the workgroup
   int64_t k, v;     // element offset of its slot in the cache (head 0); -1: not written
 };
 
-// The grid's geometry, chosen by the host.
-struct RotaryShape {
+struct RotaryJob : RotaryArgs {
   int rows_per_wg;
-  int q_items, k_items, v_items;  // work items of one head: 8 or 16 values, or one or two
-  int row_items;                  // of a row
+  int items;  // of a head
 };
 
-// VEC: 16 bytes at a time -- one item is a pair of chunks of 8 values (halves), a chunk of 4 pairs (pairs), or
-// a chunk that passes.  Otherwise an item is one pair or one value that passes, at any stride.
-template <bool VEC>
-__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, RotaryShape shape) {
+// The job, read from the kernel's arguments (of which it is the only one) where it is used.  Loads do not move across this:
+// kept in registers from the start, all of it would not fit the scalar ones.
+typedef const __attribute__((address_space(4))) RotaryJob& Args;
+__device__ __forceinline__ Args arguments() {
+  auto p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const __attribute__((address_space(4))) RotaryJob*)p;
+}
+
+// Queries, keys and values are one list of heads, and each head the same list of items.  VEC: 16 bytes at a time --
+// an item is a pair of chunks of 8 values (halves), a chunk of 4 pairs (pairs), or a chunk that passes.  Otherwise it is one
+// pair or one value that passes, at any stride.  Values have the same items, with nothing turned.
+//
+// Bound by memory, and before that by what it takes to find an item: so a thread has the same item of all the heads
+// that it goes through, and from head to head only the addresses change.  Items asked for ahead cost registers that
+// are wavefronts (us with four ahead, two, none: 4099 rows of 40 heads of 128, pairs, half of the head 21.4, 19.7, 17.4), and
+// nobody waits for the stores at the end (17.3 -> 16.4).  CACHE false: queries only.
+template <bool VEC, bool CACHE>
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryJob) {
+  Args a = arguments();
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   RowPlace* const place = (RowPlace*)smem;                                     // [rows_per_wg]
   float2* const turn = (float2*)(smem + MAX_ROWS * sizeof(RowPlace));          // [rows_per_wg][dims / 2]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int R = shape.rows_per_wg, half = a.dims >> 1;
+  const int R = a.rows_per_wg, half = a.dims >> 1, items = a.items;
+  typedef typename std::conditional<VEC, half8_t, half_t>::type chunk_t;
 
-  for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < a.rows; row0 += (int64_t)gridDim.x * R) {
-  for (int r = wave; r < R; r += 4) {
-    RowPlace p = {-1, 0, -1, -1};
-    const int64_t row64 = row0 + r;
-    if (row64 < a.rows) {
-      const int row = (int)row64;
-      p.row = row;
-      if (a.k) {
+  const int q_heads = a.q ? a.heads : 0, kv_heads = CACHE ? a.kv_heads : 0, heads = q_heads + 2 * kv_heads;
+  const int side_by_side = items < 256 ? 256 / items : 1;  // heads at once
+  const int first = items < 256 ? tid / items : 0;
+  const int item0 = first < side_by_side ? tid - first * items : items;  // (threads left over have none)
+  chunk_t v = {}, v2 = {};
+
+  // Item `in` of a head: its chunks' first values, whether there are two, whether they are turned (but for values).
+  struct Item {
+    int in, x, x2;
+    bool pair, two;
+  };
+  auto item_at = [&](int in) __attribute__((always_inline)) {
+    constexpr int W = VEC ? 8 : 1;  // values of a chunk
+    const int count = VEC && !a.pairs ? half >> 3 : VEC ? a.dims >> 3 : half;
+    Item t;
+    t.in = in;
+    t.pair = in < count;
+    t.two = t.pair && !(VEC && a.pairs);
+    t.x = !t.pair ? (in - count) * W + a.dims : !VEC && a.pairs ? 2 * in : in * W;
+    t.x2 = t.x + (a.pairs ? 1 : half);
+    return t;
+  };
+  auto read = [&](const Item& t, int64_t row, int h) __attribute__((always_inline)) {
+    const int k = CACHE ? h - q_heads : -1, w = CACHE ? k - kv_heads : -1;
+    const half_t* const base = k < 0 ? a.q : w < 0 ? a.k : a.v;
+    const int z = k < 0 ? a.sq_z : w < 0 ? a.sk_z : a.sv_z, y = k < 0 ? a.sq_y : w < 0 ? a.sk_y : a.sv_y;
+    const half_t* const from = base + (int64_t)(k < 0 ? h : w < 0 ? k : w) * z + row * y;
+    if constexpr (VEC) {
+      v = *(const half8_t*)(from + t.x);
+      if (t.two) v2 = *(const half8_t*)(from + t.x2);
+    } else {
+      const int64_t x = k < 0 ? a.sq_x : w < 0 ? a.sk_x : a.sv_x;
+      v = from[t.x * x];
+      if (t.two) v2 = from[t.x2 * x];
+    }
+  };
+  auto write = [&](const Item& t, int64_t row0, int r, int h) __attribute__((always_inline)) {
+    const int k = CACHE ? h - q_heads : -1, w = CACHE ? k - kv_heads : -1;
+    const RowPlace p = place[r];
+    const int64_t at = k < 0 ? (row0 + r) * a.so_y + h * (int64_t)a.so_z
+                             : w < 0 ? p.k + k * a.cache.stride_kz : p.v + w * a.cache.stride_vz;
+    if (p.row < 0 || (k >= 0 && (w < 0 ? p.k : p.v) < 0)) return;
+    half_t* const to = (k < 0 ? a.q_out : (half_t*)(w < 0 ? a.cache.key : a.cache.value)) + at;
+    const float2* const cs = turn + r * half;
+    const bool turned = t.pair && w < 0;
+    if constexpr (VEC) {
+      half8_t o = v, o2 = v2;
+      if (turned && a.pairs) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float2 c = cs[t.in * 4 + e];
+          const float xa = (float)v[2 * e], xb = (float)v[2 * e + 1];
+          o[2 * e] = (half_t)(xa * c.x - xb * c.y);
+          o[2 * e + 1] = (half_t)(xa * c.y + xb * c.x);
+        }
+      } else if (turned) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float2 c = cs[t.in * 8 + e];
+          const float xa = (float)v[e], xb = (float)v2[e];
+          o[e] = (half_t)(xa * c.x - xb * c.y);
+          o2[e] = (half_t)(xa * c.y + xb * c.x);
+        }
+      }
+      *(half8_t*)(to + t.x) = o;
+      if (t.two) *(half8_t*)(to + t.x2) = o2;
+    } else {
+      const int64_t x = k < 0 ? a.so_x : w < 0 ? a.cache.stride_kx : a.cache.stride_vx;
+      half_t o = v, o2 = v2;
+      if (turned) {
+        const float2 c = cs[t.in];
+        const float xa = (float)v, xb = (float)v2;
+        o = (half_t)(xa * c.x - xb * c.y);
+        o2 = (half_t)(xa * c.y + xb * c.x);
+      }
+      to[t.x * x] = o;
+      if (t.two) to[t.x2 * x] = o2;
+    }
+  };
+
+  for (int64_t row0 = (int64_t)blockIdx.x * R;;) {
+    const int rows = (int)min((int64_t)R, a.rows - row0);
+    for (int r = wave; r < rows; r += 4) {
+      const int row = (int)row0 + r;
+      RowPlace p = {row, 0, -1, -1};
+      if constexpr (CACHE) {
         const int s = sequence_of_row(a.batch.row_offsets, a.batch.sequences, row, lane);
-        const int first = clamp_to(a.batch.row_offsets[s], a.rows), end = clamp_to(a.batch.row_offsets[s + 1], a.rows);
-        if (row < first || row >= end) {
+        const int begin = clamp_to(a.batch.row_offsets[s], a.rows), end = clamp_to(a.batch.row_offsets[s + 1], a.rows);
+        if (row < begin || row >= end) {
           p.row = -1;
         } else {
           const int64_t x = (int64_t)a.batch.lengths[s] - end + row;
@@ -64,97 +158,29 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, RotaryShape s
         }
       }
       if (a.positions) p.position = a.positions[row];
+      if (lane == 0) place[r] = p;
     }
-    if (lane == 0) place[r] = p;
-  }
-  __syncthreads();
-  for (int i = tid; i < R * half; i += 256) {
-    const int r = i / half, f = i - r * half;
-    const double t = (double)place[r].position * a.turns[f];
-    float sine, cosine;
-    sincospif((float)(2.0 * (t - rint(t))), &sine, &cosine);
-    turn[i] = make_float2(cosine * a.magnitude, sine * a.magnitude);
-  }
-  __syncthreads();
-
-  const int q_all = a.heads * shape.q_items, k_all = a.kv_heads * shape.k_items;
-  for (int i = tid; i < R * shape.row_items; i += 256) {
-    const int r = i / shape.row_items;
-    int item = i - r * shape.row_items;
-    const RowPlace p = place[r];
-    if (p.row < 0) continue;
-    const half_t* src;
-    half_t* dst;
-    int64_t src_x, dst_x;
-    bool rotated = true;
-    if (item < q_all) {
-      const int h = item / shape.q_items;
-      item -= h * shape.q_items;
-      src = a.q + (int64_t)h * a.sq_z + (int64_t)p.row * a.sq_y;
-      dst = a.q_out + (int64_t)h * a.so_z + (int64_t)p.row * a.so_y;
-      src_x = a.sq_x, dst_x = a.so_x;
-    } else if (item < q_all + k_all) {
-      item -= q_all;
-      const int h = item / shape.k_items;
-      item -= h * shape.k_items;
-      if (p.k < 0) continue;
-      src = a.k + (int64_t)h * a.sk_z + (int64_t)p.row * a.sk_y;
-      dst = (half_t*)a.cache.key + p.k + h * a.cache.stride_kz;
-      src_x = a.sk_x, dst_x = a.cache.stride_kx;
-    } else {
-      item -= q_all + k_all;
-      const int h = item / shape.v_items;
-      item -= h * shape.v_items;
-      if (p.v < 0) continue;
-      src = a.v + (int64_t)h * a.sv_z + (int64_t)p.row * a.sv_y;
-      dst = (half_t*)a.cache.value + p.v + h * a.cache.stride_vz;
-      src_x = a.sv_x, dst_x = a.cache.stride_vx;
-      rotated = false;
+    __syncthreads();
+    for (int i = tid; i < rows * half; i += 256) {
+      const int r = i / half, f = i - r * half;
+      const double t = (double)place[r].position * a.turns[f];
+      float sine, cosine;
+      sincospif((float)(2.0 * (t - rint(t))), &sine, &cosine);
+      turn[i] = make_float2(cosine * a.magnitude, sine * a.magnitude);
     }
-    const float2* const cs = turn + r * half;
-    if constexpr (VEC) {
-      const int turned = !rotated ? 0 : a.pairs ? a.dims >> 3 : a.dims >> 4;  // items of this head that are turned
-      if (item >= turned) {
-        const int x = (rotated ? a.dims : 0) + (item - turned) * 8;
-        *(half8_t*)(dst + x) = *(const half8_t*)(src + x);
-      } else if (a.pairs) {
-        const half8_t v = *(const half8_t*)(src + item * 8);
-        half8_t o;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float2 t = cs[item * 4 + e];
-          const float x = (float)v[2 * e], y = (float)v[2 * e + 1];
-          o[2 * e] = (half_t)(x * t.x - y * t.y);
-          o[2 * e + 1] = (half_t)(x * t.y + y * t.x);
-        }
-        *(half8_t*)(dst + item * 8) = o;
-      } else {
-        const half8_t va = *(const half8_t*)(src + item * 8), vb = *(const half8_t*)(src + half + item * 8);
-        half8_t oa, ob;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float2 t = cs[item * 8 + e];
-          const float x = (float)va[e], y = (float)vb[e];
-          oa[e] = (half_t)(x * t.x - y * t.y);
-          ob[e] = (half_t)(x * t.y + y * t.x);
-        }
-        *(half8_t*)(dst + item * 8) = oa;
-        *(half8_t*)(dst + half + item * 8) = ob;
-      }
-    } else {
-      if (!rotated || item >= half) {
-        const int x = rotated ? item - half + a.dims : item;
-        dst[x * dst_x] = src[x * src_x];
-      } else {
-        const int xa = a.pairs ? 2 * item : item, xb = a.pairs ? xa + 1 : item + half;
-        const float2 t = cs[item];
-        const float x = (float)src[xa * src_x], y = (float)src[xb * src_x];
-        dst[xa * dst_x] = (half_t)(x * t.x - y * t.y);
-        dst[xb * dst_x] = (half_t)(x * t.y + y * t.x);
+    __syncthreads();
+    for (int in = item0; in < items; in += 256) {
+      const Item t = item_at(in);
+      for (int r = 0, h = first;; h += side_by_side) {
+        while (h >= heads) h -= heads, r++;
+        if (r >= rows) break;
+        read(t, row0 + r, h);
+        write(t, row0, r, h);
       }
     }
-  }
-  __syncthreads();  // (the next rows' places and angles go where these are read)
+    row0 += (int64_t)gridDim.x * R;
+    if (row0 >= a.rows) break;
+    __syncthreads();  // (the next rows' places and angles go where these are read)
   }
 }
 
@@ -183,25 +209,25 @@ hipError_t launch_rotary(hipStream_t stream, const RotaryArgs& a) {
   const bool vec = vectors_fit(a);
   const int turned = !vec ? a.dims / 2 : a.pairs ? a.dims / 8 : a.dims / 16;
   const int passing = vec ? (a.d - a.dims) / 8 : a.d - a.dims;
-  // (in place, what passes is there already)
-  const bool in_place = a.q == a.q_out && a.sq_x == a.so_x && a.sq_y == a.so_y && a.sq_z == a.so_z;
-  RotaryShape s = {};
-  s.q_items = a.q ? turned + (in_place ? 0 : passing) : 0;
-  s.k_items = a.k ? turned + passing : 0;
-  s.v_items = a.k ? (vec ? a.d / 8 : a.d) : 0;
-  const int64_t items = (int64_t)a.heads * s.q_items + (int64_t)a.kv_heads * (s.k_items + s.v_items);
+  RotaryJob s = {};
+  (RotaryArgs&)s = a;
+  s.items = turned + passing;
+  const int64_t items = s.items * ((int64_t)(a.q ? a.heads : 0) + 2 * (int64_t)(a.k ? a.kv_heads : 0));
   if (items == 0) return hipSuccess;
   if (items * MAX_ROWS > 0x7fffffff) return hipErrorInvalidConfiguration;
-  s.row_items = (int)items;
-  // Rows of a workgroup: as many as give its 256 threads an item each, within the LDS of their angles.
+  // Rows of a workgroup: as many as give its 256 threads four items each, within the LDS of their angles, and not so
+  // many that there would be fewer than eight workgroups for each of 256 compute units.
   const int half = a.dims / 2;
-  int R = (int)std::min<int64_t>(std::max<int64_t>(256 / items, 1), a.k ? 4 : MAX_ROWS);
-  while (R > 1 && R * half > 2048) R >>= 1;
+  int R = (int)std::min<int64_t>(std::max<int64_t>(1024 / items, 1), MAX_ROWS);
+  while (R > 1 && (R * half > 2048 || (R * items > 256 && a.rows / R < 2048))) R >>= 1;
   s.rows_per_wg = R;
   const int64_t grid = std::min<int64_t>(((int64_t)a.rows + R - 1) / R, 1 << 22);  // (a launch has fewer than 2^32 threads)
   const size_t lds = MAX_ROWS * sizeof(RowPlace) + (size_t)R * half * sizeof(float2);
-  if (vec) hipLaunchKernelGGL(rotary_kernel<true>, dim3((unsigned)grid), dim3(256), lds, stream, a, s);
-  else hipLaunchKernelGGL(rotary_kernel<false>, dim3((unsigned)grid), dim3(256), lds, stream, a, s);
+  const dim3 blocks((unsigned)grid), threads(256);
+  if (vec && a.k) hipLaunchKernelGGL(HIP_KERNEL_NAME(rotary_kernel<true, true>), blocks, threads, lds, stream, s);
+  else if (vec) hipLaunchKernelGGL(HIP_KERNEL_NAME(rotary_kernel<true, false>), blocks, threads, lds, stream, s);
+  else if (a.k) hipLaunchKernelGGL(HIP_KERNEL_NAME(rotary_kernel<false, true>), blocks, threads, lds, stream, s);
+  else hipLaunchKernelGGL(HIP_KERNEL_NAME(rotary_kernel<false, false>), blocks, threads, lds, stream, s);
   return hipGetLastError();
 }
 
