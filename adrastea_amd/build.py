@@ -125,24 +125,36 @@ def build_legacy_modules(force: bool = False) -> list:
     return outs
 
 
-HOST_TEST_SRC = os.path.join(os.path.dirname(HERE), "tests", "cpp", "test_host.cpp")
-HOST_TEST_BIN = os.path.join(os.path.dirname(HERE), "tests", "cpp", "bin", "test_host")
+CPP_TESTS = os.path.join(os.path.dirname(HERE), "tests", "cpp")
+HOST_TEST_SRC = os.path.join(CPP_TESTS, "test_host.cpp")
+HOST_TEST_BIN = os.path.join(CPP_TESTS, "bin", "test_host")
+SEQUENCES_TEST_SRC = os.path.join(CPP_TESTS, "test_sequences.cpp")
+SEQUENCES_TEST_BIN = os.path.join(CPP_TESTS, "bin", "test_sequences")
 
 
-def build_host_test(force: bool = False) -> str:
-    """Compiles the C++ host-side test (header-only host/*.hpp over the C ABI) with g++."""
-    deps = [HOST_TEST_SRC, LIB] + [os.path.join(HERE, "host", f) for f in os.listdir(os.path.join(HERE, "host"))]
-    if (not force and os.path.exists(HOST_TEST_BIN)
-            and all(os.path.getmtime(d) <= os.path.getmtime(HOST_TEST_BIN) for d in deps)):
-        return HOST_TEST_BIN
-    os.makedirs(os.path.dirname(HOST_TEST_BIN), exist_ok=True)
-    cmd = ["g++", "-std=c++17", "-O1", "-Wall", "-o", HOST_TEST_BIN, HOST_TEST_SRC, "-L" + LIBDIR,
+def _build_host_test(force: bool, src: str, out: str) -> str:
+    deps = [src, LIB] + [os.path.join(HERE, "host", f) for f in os.listdir(os.path.join(HERE, "host"))]
+    if (not force and os.path.exists(out)
+            and all(os.path.getmtime(d) <= os.path.getmtime(out) for d in deps)):
+        return out
+    os.makedirs(os.path.dirname(out), exist_ok=True)
+    cmd = ["g++", "-std=c++17", "-O1", "-Wall", "-o", out, src, "-L" + LIBDIR,
            "-ladrastea_kernels_hip", "-ldl", "-Wl,-rpath,$ORIGIN/../../../adrastea_amd/lib",
            "-Wl,-rpath,/opt/rocm/lib"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for the host test:\n{r.stdout}\n{r.stderr}")
-    return HOST_TEST_BIN
+    return out
+
+
+def build_sequences_test(force: bool = False) -> str:
+    return _build_host_test(force, SEQUENCES_TEST_SRC, SEQUENCES_TEST_BIN)
+
+
+def build_host_test(force: bool = False) -> str:
+    """Compiles the C++ host-side tests (header-only host/*.hpp over the C ABI) with g++."""
+    build_sequences_test(force)
+    return _build_host_test(force, HOST_TEST_SRC, HOST_TEST_BIN)
 
 
 NATIVE_SRC = os.path.join(HERE, "host", "native.cpp")

@@ -85,6 +85,27 @@ inline LoweredMatmul lower_matmul(const TensorLayout& out, const TensorLayout& l
   return r;
 }
 
+// ---- several sequences at once (not in the reference) ----
+
+// Keys and values of many sequences in pages: [pages, kv_heads, page_size, d] views of the caller's pools.
+struct PagedCache {
+  TensorView<f16> key, value;
+  adr_paged_cache lower() const {
+    const auto &k = key.layout, &v = value.layout;
+    if (k.dims.size() != 4 || k.dims != v.dims) throw std::logic_error("PagedCache: [pages, kv_heads, page_size, d] views");
+    adr_paged_cache c{};
+    c.key = key.ptr, c.value = value.ptr;
+    c.pages = (int32_t)k.dims[0], c.kv_heads = (int32_t)k.dims[1], c.page_size = (int32_t)k.dims[2], c.d = (int32_t)k.dims[3];
+    c.stride_kx = (int64_t)k.strides[3], c.stride_ky = (int64_t)k.strides[2], c.stride_kz = (int64_t)k.strides[1], c.stride_kp = (int64_t)k.strides[0];
+    c.stride_vx = (int64_t)v.strides[3], c.stride_vy = (int64_t)v.strides[2], c.stride_vz = (int64_t)v.strides[1], c.stride_vp = (int64_t)v.strides[0];
+    return c;
+  }
+};
+// Device memory of the caller: see adr_paged_batch and adr_packed_batch.
+using PagedBatch = adr_paged_batch;
+using PackedBatch = adr_packed_batch;
+using Rotary = adr_rotary;
+
 struct CommonKernels {
   virtual ~CommonKernels() = default;
   virtual void matmul_f16(TensorView<f16>& output, const TensorView<const f16>& left,
@@ -179,6 +200,73 @@ class GpuKernels : public CommonKernels {
     if (lf.size(-1) != rf.size(-1)) throw std::logic_error("error_stats: length mismatch");
     int rc = adr_error_stats_f32(stream_, descriptor(out), descriptor(lf), descriptor(rf));
     if (rc) throw AdrasteaError(rc, "error_stats_f32");
+  }
+  // A [heads, rows, d] view (rank 2: one head) as the C ABI takes it.
+  struct Rows {
+    int32_t heads, rows, d, x, y, z;
+  };
+  template <typename T>
+  static Rows rows_of(const TensorView<T>& v, const char* what) {
+    const auto& l = v.layout;
+    if (l.dims.size() != 2 && l.dims.size() != 3) throw std::logic_error(std::string(what) + ": [heads, rows, d] views");
+    const bool h = l.dims.size() == 3;
+    return {h ? (int32_t)l.size(-3) : 1, (int32_t)l.size(-2), (int32_t)l.size(-1), (int32_t)l.stride(-1), (int32_t)l.stride(-2),
+            h ? (int32_t)l.stride(-3) : 0};
+  }
+  static void same(const Rows& a, const Rows& b, const char* what) {
+    if (a.heads != b.heads || a.rows != b.rows || a.d != b.d) throw std::logic_error(std::string(what) + ": shape mismatch");
+  }
+  // The rows of `input` turned by positions[row] (device memory, [rows]) into `output`, which may be the same view.
+  void rotary_f16(TensorView<f16>& output, const TensorView<const f16>& input, const int32_t* positions, const Rotary& rotary) {
+    const Rows o = rows_of(output, "rotary_f16"), i = rows_of(input, "rotary_f16");
+    same(o, i, "rotary_f16");
+    int rc = adr_rotary_f16(stream_, output.ptr, input.ptr, positions, rotary, i.heads, i.rows, i.d, o.x, o.y, o.z, i.x, i.y, i.z);
+    if (rc) throw AdrasteaError(rc, "rotary_f16");
+  }
+  // The step's keys, turned, and values into their pages, and its queries turned into `query_out` (both null: none).
+  void append_f16(const PagedCache& cache, const PagedBatch& batch, const TensorView<const f16>& key, const TensorView<const f16>& value,
+                  const Rotary& rotary, TensorView<f16>* query_out = nullptr, const TensorView<const f16>* query = nullptr,
+                  const int32_t* positions = nullptr) {
+    const adr_paged_cache c = cache.lower();
+    const Rows k = rows_of(key, "append_f16"), v = rows_of(value, "append_f16");
+    same(k, v, "append_f16");
+    if (k.heads != c.kv_heads || k.d != c.d || !query != !query_out) throw std::logic_error("append_f16: shape mismatch");
+    Rows q{}, o{};
+    if (query) {
+      q = rows_of(*query, "append_f16"), o = rows_of(*query_out, "append_f16");
+      same(q, o, "append_f16");
+      if (q.rows != k.rows || q.d != k.d) throw std::logic_error("append_f16: shape mismatch");
+    }
+    int rc = adr_append_f16(stream_, c, batch, key.ptr, value.ptr, query ? query_out->ptr : nullptr, query ? query->ptr : nullptr,
+                            positions, rotary, q.heads, k.rows, k.x, k.y, k.z, v.x, v.y, v.z, o.x, o.y, o.z, q.x, q.y, q.z);
+    if (rc) throw AdrasteaError(rc, "append_f16");
+  }
+  void attention_paged_f16(TensorView<f16>& output, const TensorView<const f16>& query, const PagedCache& cache, const PagedBatch& batch,
+                           float scale, float temperature = 1.0f, MatmulMask mask = MatmulMask::Causal) {
+    const adr_paged_cache c = cache.lower();
+    const Rows o = rows_of(output, "attention_paged_f16"), q = rows_of(query, "attention_paged_f16");
+    same(o, q, "attention_paged_f16");
+    if (q.d != c.d) throw std::logic_error("attention_paged_f16: shape mismatch");
+    auto call = [&](auto fn, auto... workspace) {
+      return fn(stream_, output.ptr, query.ptr, c, batch, q.heads, q.rows, o.x, o.y, o.z, q.x, q.y, q.z, scale, temperature,
+                (uint32_t)mask, workspace...);
+    };
+    int rc = workspace_bytes_ > 0 ? call(adr_attention_paged_f16_ws, workspace_, workspace_bytes_) : call(adr_attention_paged_f16);
+    if (rc) throw AdrasteaError(rc, "attention_paged_f16");
+  }
+  void attention_packed_f16(TensorView<f16>& output, const TensorView<const f16>& query, const TensorView<const f16>& key,
+                            const TensorView<const f16>& value, const PackedBatch& batch, float scale, float temperature = 1.0f,
+                            MatmulMask mask = MatmulMask::Causal) {
+    const char* what = "attention_packed_f16";
+    const Rows o = rows_of(output, what), q = rows_of(query, what), k = rows_of(key, what), v = rows_of(value, what);
+    same(o, q, what), same(k, v, what);
+    if (k.d != q.d) throw std::logic_error("attention_packed_f16: shape mismatch");
+    auto call = [&](auto fn, auto... workspace) {
+      return fn(stream_, output.ptr, query.ptr, key.ptr, value.ptr, batch, q.heads, k.heads, q.rows, k.rows, q.d, o.x, o.y, o.z, q.x,
+                q.y, q.z, k.x, k.y, k.z, v.x, v.y, v.z, scale, temperature, (uint32_t)mask, workspace...);
+    };
+    int rc = workspace_bytes_ > 0 ? call(adr_attention_packed_f16_ws, workspace_, workspace_bytes_) : call(adr_attention_packed_f16);
+    if (rc) throw AdrasteaError(rc, what);
   }
   std::string plan(const TensorLayout& o, const TensorLayout& l, const TensorLayout& r, const MatmulOptions& opt) const {
     LoweredMatmul w = lower_matmul(o, l, r, opt);

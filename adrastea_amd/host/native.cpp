@@ -19,10 +19,10 @@ constexpr int MAX_RANK = 7;  // of a descriptor; views of higher rank take the g
 
 PyObject *layout_type, *view_type;                      // the classes of tensor.py
 PyObject *of_general, *permute_general, *cast_general;  // their definitions of the methods below
-PyObject *current_device, *raw_stream;                  // torch's functions
+PyObject *current_device, *raw_stream, *int32_type;     // torch's functions, torch.int32
 PyObject *s_shape, *s_stride, *s_dims, *s_strides, *s_storage, *s_layout, *s_offset, *s_data_ptr, *s_load, *s_store,
     *s_mask, *s_op, *s_scale, *s_beta, *s_bias, *s_is_contiguous, *s_get_device, *s_key, *s_value, *s_row_offsets, *s_lengths,
-    *s_table, *s_key_offsets, *s_longest_rows, *s_longest, *s_turns, *s_rotary_layout, *s_magnitude;
+    *s_table, *s_key_offsets, *s_longest_rows, *s_longest, *s_turns, *s_rotary_layout, *s_magnitude, *s_dtype;
 
 decltype(&adr_matmul_f16) matmul_fn;
 decltype(&adr_attention_f16) attention_fn;
@@ -475,6 +475,16 @@ bool read_index(PyObject* tensor, int rank, int64_t device, int64_t (&dims)[MAX_
   return shape.p && PyTuple_Check(shape) && read_ints(shape, dims, rank) && on_device(tensor, device) && read_ptr(tensor, ptr);
 }
 
+// positions[rows]: contiguous, int32
+bool read_positions(PyObject* tensor, int64_t device, int64_t rows, void*& ptr) {
+  int64_t n[MAX_RANK], stride[MAX_RANK];
+  const Ref type(attr(tensor, s_dtype));
+  if (type.p != int32_type || !read_index(tensor, 1, device, n, ptr) || n[0] != rows) return false;
+  const Ref strides(call(tensor, s_stride));
+  int rank = 1;
+  return strides.p && read_ints(strides, stride, rank) && stride[0] == 1;
+}
+
 bool read_int32(PyObject* o, PyObject* name, int32_t& v) {
   const Ref r(attr(o, name));
   int64_t x;
@@ -531,14 +541,14 @@ bool read_rotary(PyObject* o, int64_t device, adr_rotary& r) {
 
 // rotary_f16(output, input, positions, rotary)
 PyObject* rotary_f16(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  int64_t device, count[MAX_RANK];
+  int64_t device;
   adr_stream_t stream;
   Rows o, x;
   adr_rotary r;
   void* p;
   if (n != 4 || !rotary_fn || !read_device(device, stream) || !read_rows(a[0], device, o) || !read_rows(a[1], device, x) ||
-      !read_index(a[2], 1, device, count, p) || !read_rotary(a[3], device, r) || o.heads != x.heads || o.rows != x.rows ||
-      o.d != x.d || count[0] != x.rows)
+      !read_positions(a[2], device, x.rows, p) || !read_rotary(a[3], device, r) || o.heads != x.heads || o.rows != x.rows ||
+      o.d != x.d)
     return general();
   int rc;
   Py_BEGIN_ALLOW_THREADS
@@ -550,7 +560,7 @@ PyObject* rotary_f16(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // append_f16(cache, batch, key, value, rotary, query_out, query, positions); the last four may be None
 PyObject* append_f16(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  int64_t device, count[MAX_RANK];
+  int64_t device;
   adr_stream_t stream;
   adr_paged_cache c;
   adr_paged_batch b;
@@ -565,7 +575,7 @@ PyObject* append_f16(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (a[6] != Py_None && (!read_rows(a[5], device, o) || !read_rows(a[6], device, q) || o.heads != q.heads || o.rows != q.rows ||
                           o.d != q.d || q.rows != k.rows || q.d != k.d))
     return general();
-  if (a[7] != Py_None && (!read_index(a[7], 1, device, count, p) || count[0] != k.rows)) return general();
+  if (a[7] != Py_None && !read_positions(a[7], device, k.rows, p)) return general();
   int rc;
   Py_BEGIN_ALLOW_THREADS
   rc = append_fn(stream, c, b, (const uint16_t*)k.ptr, (const uint16_t*)v.ptr, (uint16_t*)o.ptr, (const uint16_t*)q.ptr,
@@ -672,10 +682,13 @@ PyObject* bind(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
-// bind_sequences(addresses of the functions over several sequences): beside bind, whose torch functions they use
+// bind_sequences(addresses of the functions over several sequences, torch.int32): beside bind, whose torch functions they use
 PyObject* bind_sequences(PyObject*, PyObject* args) {
   unsigned long long p[4];
-  if (!PyArg_ParseTuple(args, "KKKK", p, p + 1, p + 2, p + 3)) return nullptr;
+  PyObject* type;
+  if (!PyArg_ParseTuple(args, "KKKKO", p, p + 1, p + 2, p + 3, &type)) return nullptr;
+  Py_INCREF(type);
+  Py_XSETREF(int32_type, type);
   rotary_fn = (decltype(rotary_fn))p[0];
   append_fn = (decltype(append_fn))p[1];
   paged_fn = (decltype(paged_fn))p[2];
@@ -711,7 +724,7 @@ PyMODINIT_FUNC PyInit__native() {
       {&s_is_contiguous, "is_contiguous"}, {&s_get_device, "get_device"}, {&s_key, "key"}, {&s_value, "value"},
       {&s_row_offsets, "row_offsets"}, {&s_lengths, "lengths"}, {&s_table, "table"}, {&s_key_offsets, "key_offsets"},
       {&s_longest_rows, "longest_rows"}, {&s_longest, "longest"}, {&s_turns, "turns"}, {&s_rotary_layout, "layout"},
-      {&s_magnitude, "magnitude"}};
+      {&s_magnitude, "magnitude"}, {&s_dtype, "dtype"}};
   for (const auto& n : names)
     if (!(*n.at = PyUnicode_InternFromString(n.name))) return nullptr;
   return PyModule_Create(&module);

@@ -400,8 +400,9 @@ _NATIVE_SEQUENCE_CALLS = ("adr_rotary_f16", "adr_append_f16", "adr_attention_pag
 
 @functools.lru_cache(maxsize=None)
 def _native_sequence_binding() -> tuple:
+    import torch
     lib = _ffi.lib()
-    return tuple(C.cast(getattr(lib, name), C.c_void_p).value for name in _NATIVE_SEQUENCE_CALLS)
+    return (*(C.cast(getattr(lib, name), C.c_void_p).value for name in _NATIVE_SEQUENCE_CALLS), torch.int32)
 
 
 def _bind_native() -> None:
@@ -517,13 +518,12 @@ class GpuKernels(CommonKernels):
     def rotary_f16(self, output, input, positions, rotary: Rotary):
         """The rows of `input`, a [heads, rows, d] view, turned by positions[row] into `output` (which may be the same
         view).  positions: int32 [rows]."""
-        _index(positions, 1, "positions")
         if self._lowered("rotary_f16", output, input, positions, rotary):
             return
         dims, si = _rows_view(input, "input")
         dims_out, so = _rows_view(output, "output")
         assert dims_out == dims, "output and input have one shape"
-        assert positions.shape[0] == dims[1], "a position for each row"
+        assert _index(positions, 1, "positions").shape[0] == dims[1], "a position for each row"
         _here(positions)
         rc = self._lib.adr_rotary_f16(_current_stream(), output.data_ptr(), input.data_ptr(), positions.data_ptr(),
                                       rotary._desc, *dims, *so, *si)
@@ -535,8 +535,6 @@ class GpuKernels(CommonKernels):
         """The step's keys, turned, and values ([kv_heads, rows, d] views) into their pages, and its queries ([heads,
         rows, d]) turned into `query_out`, which may be the same view.  Row j of the r of sequence s goes to
         place lengths[s] - r + j and is turned by it, or by positions[row] (int32 [rows])."""
-        if positions is not None:
-            _index(positions, 1, "positions")
         if self._lowered("append_f16", cache, batch, key, value, rotary, query_out, query, positions):
             return
         c, b = cache._desc, batch._desc
@@ -551,7 +549,7 @@ class GpuKernels(CommonKernels):
             heads = dims_q[0]
             assert dims_o == dims_q and dims_q[1:] == dims[1:], "query and query_out are [heads, rows, d] views"
         if positions is not None:
-            assert positions.shape[0] == dims[1], "a position for each row"
+            assert _index(positions, 1, "positions").shape[0] == dims[1], "a position for each row"
             _here(positions)
         rc = self._lib.adr_append_f16(
             _current_stream(), c, b, key.data_ptr(), value.data_ptr(), query_out.data_ptr() if heads else None,
