@@ -89,8 +89,9 @@ __device__ __forceinline__ bool key_at(Args a, const Sequence& q, int x, int64_t
 
 // One row of one query head by one wavefront, at any strides: 64 keys at a time, a lane to a key for the scores
 // and a lane to every 64th column for the sums.  Only keys that the row sees are read.  Probabilities stay in 32 bits.
+// (Columns col0 ... col1 - 1 are stored.)
 constexpr int GENERAL_MAX_D = 256;
-__device__ __forceinline__ void row_by_wave(Args a, const Sequence& q, int j, int h, int lane) {
+__device__ __forceinline__ void row_by_wave(Args a, const Sequence& q, int j, int h, int lane, int col0 = 0, int col1 = GENERAL_MAX_D) {
   const int64_t row = (int64_t)q.row0 + j;
   const half_t* const Q = a.q + h * (int64_t)a.sq_z + row * a.sq_y;
   const half_t* const K = a.k + (h / a.group) * a.sk.z;
@@ -136,7 +137,8 @@ __device__ __forceinline__ void row_by_wave(Args a, const Sequence& q, int j, in
   half_t* const O = a.out + h * (int64_t)a.so_z + row * a.so_y;
 #pragma unroll
   for (int c = 0; c < GENERAL_MAX_D / 64; c++)
-    if (c * 64 + lane < a.d) O[(c * 64 + lane) * (int64_t)a.so_x] = (half_t)(o[c] * inv);
+    if (c * 64 + lane < a.d && c * 64 + lane >= col0 && c * 64 + lane < col1)
+      O[(c * 64 + lane) * (int64_t)a.so_x] = (half_t)(o[c] * inv);
 }
 
 // Any layout: a wavefront per row and query head.
@@ -191,6 +193,17 @@ __device__ __forceinline__ int add_scan(int v) {  // inclusive, over the lanes o
   v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
   v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
   return v;
+}
+
+__device__ __forceinline__ int min_of_all(int v) {
+  constexpr int NONE = 0x7fffffff;
+  v = min(v, __builtin_amdgcn_update_dpp(NONE, v, 0x111, 0xf, 0xf, false));  // row_shr:1
+  v = min(v, __builtin_amdgcn_update_dpp(NONE, v, 0x112, 0xf, 0xf, false));
+  v = min(v, __builtin_amdgcn_update_dpp(NONE, v, 0x114, 0xf, 0xf, false));
+  v = min(v, __builtin_amdgcn_update_dpp(NONE, v, 0x118, 0xf, 0xf, false));
+  v = min(v, __builtin_amdgcn_update_dpp(NONE, v, 0x142, 0xa, 0xf, false));  // row_bcast:15
+  v = min(v, __builtin_amdgcn_update_dpp(NONE, v, 0x143, 0xc, 0xf, false));  // row_bcast:31
+  return __builtin_amdgcn_readlane(v, 63);
 }
 
 // Rows of a block, keys of a tile, log2 of the tiles of a piece
@@ -320,13 +333,18 @@ __device__ __forceinline__ bool part_at(Args a, int index, int lane, Part& p) {
   double inv = 0.0;
   for (int tries = 0;; tries++) {
     inv = 1.0 / (double)most;
-    int n = 0;
+    int n = 0, fewer = UNDIVIDED;  // the least that some block has a part less with
 #pragma unroll
-    for (int e = 0; e < EACH; e++) n += blocks[e] * parts_of(tiles[e], inv, most);
+    for (int e = 0; e < EACH; e++) {
+      const int each = parts_of(tiles[e], inv, most);
+      n += blocks[e] * each;
+      if (blocks[e] > 0 && each > 1) fewer = min(fewer, (int)((float)tiles[e] * __builtin_amdgcn_rcpf((float)(each - 1))) + 1);
+    }
     n = all_lanes(n);
     if (n <= a.parts || most >= UNDIVIDED) break;
     // (larger in proportion, and so through in a few tries; where there are too many blocks nothing is divided in the end)
-    most = tries < 8 ? max(most + 1, uniform((int)fmin((double)most * n / a.parts, (double)UNDIVIDED))) : UNDIVIDED;
+    most = tries < 8 ? max(max(most + 1, min_of_all(fewer)), uniform((int)fmin((double)most * n / a.parts, (double)UNDIVIDED)))
+                     : UNDIVIDED;
   }
   int at = -1, before = 0, slots = 0, seams = 0;
 #pragma unroll
@@ -669,8 +687,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
 // beside the maximum of tile i + 1.  What is different here is where rows and keys come from: the heads of a group
 // share the block, so that a key row is read once for all of them and the part of a tile that the mask leaves empty
 // is 1 / group as wide, and each wavefront's 16 key rows of a tile have a base address of their own, on a page.
-template <int HD, bool PAGED, bool SHARED>
-__global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
+template <int HD, bool PAGED, bool SHARED, int GROUPS>
+__global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
   constexpr int CPR = HD / 8, KEYS = 64, ROWS = 128;
   constexpr int TILE = KEYS * HD * 2;  // bytes of one K or V tile
   constexpr int NI = TILE / 1024 / 4;  // transfers per wavefront and tile: 16 rows
@@ -678,8 +696,8 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
   constexpr int DT = HD / 32;          // 32-wide output column tiles
   constexpr int ROWB = HD * 2;         // bytes per tile row
   constexpr int BIAS = NI * 1024;      // bytes that descriptors start ahead, so that no offset is negative
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];  // K0 K1 V0 V1
-  __shared__ int lost_keys[4];  // of each wavefront
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[GROUPS * 4 * TILE];  // K0 K1 V0 V1 of each group
+  __shared__ int lost_keys[4 * GROUPS];  // of each wavefront
 
   // Consecutive workgroups go to different dies; where the key heads divide evenly, a die takes its share of them, so
   // that the blocks which read the same keys meet in one L2.
@@ -694,7 +712,7 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
     index = blockIdx.x / kv_heads;
   }
   Args a = arguments();
-  const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63, group = GROUPS == 1 ? 0 : uniform(tid >> 8), w = uniform(tid >> 6 & 3);
   const int frow = lane & 31, g = lane >> 5;
   Part pt = {{}, 0, 1, 0, 0, 0};
   if constexpr (SHARED) {
@@ -721,18 +739,20 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
   const int all = (last_end + KEYS - 1) / KEYS;
   // (exact, as above)
   auto cut = [&](int i) __attribute__((always_inline)) { return uniform((int)((double)all * (double)i / (double)parts)); };
-  const int tile0 = SHARED ? cut(part) : 0, steps = (SHARED ? cut(part + 1) : all) - tile0;
-  const int row_end = min(last_end, (tile0 + steps) * KEYS);
+  const int part0 = SHARED ? cut(part) : 0, part_tiles = (SHARED ? cut(part + 1) : all) - part0;
+  // (of each group; the second may have one less)
+  const int steps = (part_tiles + GROUPS - 1) / GROUPS, tile0 = part0 + group * steps;
+  const int row_end = min(last_end, min(part0 + part_tiles, tile0 + steps) * KEYS);
   // Tiles that this wavefront computes: none without rows, none whose first key lies beyond its last row's.
   int active = 0, first_edge = 0;
   if (wave_rows > 0) {
-    active = uniform(clamp_to((end_of_row(a, q, row_of_list(a, list0 + wave_rows - 1)) + KEYS - 1) / KEYS - tile0, steps));
+    active = uniform(clamp_to((end_of_row(a, q, row_of_list(a, list0 + wave_rows - 1)) + KEYS - 1) / KEYS - tile0, min(steps, part0 + part_tiles - tile0)));
     // the first of them with keys that some row of the wavefront must not see
     first_edge = uniform(end_of_row(a, q, row_of_list(a, list0))) / KEYS - tile0;
   }
 
-  const uint32_t lds0 = (uint32_t)(uintptr_t)ADR_LDS_PTR(smem);
-  const unsigned char* const sm = smem;
+  unsigned char* const sm = smem + group * (4 * TILE);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)ADR_LDS_PTR(smem) + group * (4 * TILE);
   // Wavefront w transfers rows 16 w ... 16 w + 15 of a tile, 1 KiB at a time: byte offsets of a lane's chunks in those
   // rows, less the j KiB that the instruction adds; chunks behind the head dimension come as zeros.
   uint32_t koff[NI], voff[NI];
@@ -1081,71 +1101,121 @@ __global__ __launch_bounds__(256, 2) void attention_tiles_kernel(Job) {
   for (; i < steps; i++) idle(i);  // tiles this wavefront has no part in
   wait_vm<0>();  // (transfers of no bytes write zeros)
   if constexpr (PAGED) {
-    if (lane == 0) lost_keys[w] = __ballot(lost) != 0;
+    if (lane == 0) lost_keys[4 * group + w] = __ballot(lost) != 0;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
   barrier();  // every read of K and V tiles is done: LDS is free
+
+  // The groups' sums are joined by way of LDS: each finishes half of the columns.
+  constexpr int MINE = DT / GROUPS;
+  constexpr int EXCHANGE = GROUPS == 1 ? 0 : 256 * MINE * 64;  // bytes from a group
+  float16_t res[MINE];
+  if constexpr (GROUPS == 2) {
+    __shared__ float2 mls[2][256];
+    const int at = tid & 255;
+    float4_t* const theirs = (float4_t*)(smem + (1 - group) * (4 * TILE)) + at;
+    float4_t* const ours = (float4_t*)sm + at;
+    auto give = [&](auto first) __attribute__((always_inline)) {
+#pragma unroll
+      for (int d = 0; d < MINE; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float16_t& v = o[decltype(first)::value + d];
+          ours[(4 * d + i) * 256] = float4_t{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+        }
+    };
+    if (group == 0) give(std::integral_constant<int, MINE>{});
+    else give(std::integral_constant<int, 0>{});
+    mls[group][at] = make_float2(m_run, l_run);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    barrier();
+    const float2 ml = mls[1 - group][at];
+    const float top = fmaxf(m_run, ml.x), f0 = __builtin_amdgcn_exp2f(m_run - top), f1 = __builtin_amdgcn_exp2f(ml.x - top);
+    m_run = top;
+    l_run = l_run * f0 + ml.y * f1;
+    auto take = [&](auto first) __attribute__((always_inline)) {
+#pragma unroll
+      for (int d = 0; d < MINE; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float16_t& v = o[decltype(first)::value + d];
+          const float4_t x = theirs[(4 * d + i) * 256];
+#pragma unroll
+          for (int j = 0; j < 4; j++) res[d][4 * i + j] = v[4 * i + j] * f0 + x[j] * f1;
+        }
+    };
+    if (group == 0) take(std::integral_constant<int, 0>{});
+    else take(std::integral_constant<int, MINE>{});
+  } else {
+#pragma unroll
+    for (int d = 0; d < DT; d++) res[d] = o[d];
+  }
 
   Args z = arguments();
   float l_tot = pair_sum(l_run);
   if constexpr (PAGED) {
     // (a page that is not in the cache may be some rows' only: all of the block come out as NaN, and those that do not
     // see it are computed again below)
-    if (lost_keys[0] | lost_keys[1] | lost_keys[2] | lost_keys[3]) l_tot = NAN;
+    int any = 0;
+#pragma unroll
+    for (int i = 0; i < 4 * GROUPS; i++) any |= lost_keys[i];
+    if (any) l_tot = NAN;
   }
+  const int col0 = group * (32 * MINE);
   if (!SHARED || parts == 1) {
-    // out[row][32d + 8i + 4g + j] = o[d][4i + j] / l, by way of LDS, so that whole rows are stored
-    constexpr int PITCH = ROWB + 16;
-    static_assert(4 * 32 * PITCH <= 4 * TILE, "the output's slots fit the LDS");
-    unsigned char* const slot = smem + w * (32 * PITCH);
+    // out[row][32d + 8i + 4g + j] = res[d][4i + j] / l, by way of LDS, so that whole rows are stored
+    constexpr int PITCH = ROWB / GROUPS + 16, CHUNKS = CPR / GROUPS;
+    static_assert(EXCHANGE + 4 * 32 * PITCH <= 4 * TILE, "the output's slots fit the LDS");
+    unsigned char* const slot = sm + EXCHANGE + w * (32 * PITCH);
     const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
     bool finite = true;
 #pragma unroll
-    for (int d = 0; d < DT; d++)
+    for (int d = 0; d < MINE; d++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        half4_t r;
+        half4_t h;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          const float v = o[d][4 * i + j] * inv;
+          const float v = res[d][4 * i + j] * inv;
           finite = finite && fabsf(v) < INFINITY;
-          r[j] = (half_t)v;
+          h[j] = (half_t)v;
         }
-        *(half4_t*)(slot + frow * PITCH + (32 * d + 8 * i + 4 * g) * 2) = r;
+        *(half4_t*)(slot + frow * PITCH + (32 * d + 8 * i + 4 * g) * 2) = h;
       }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the slot is the wavefront's own)
-    constexpr int RPI = 64 / CPR;  // rows of a store instruction
-    const int r0 = lane / CPR, col = lane % CPR * 8;
+    constexpr int RPI = 64 / CHUNKS;  // rows of a store instruction
+    const int r0 = lane / CHUNKS, col = lane % CHUNKS * 8;
 #pragma unroll
     for (int i = 0; i < 32 / RPI; i++) {
       if (i * RPI >= wave_rows) break;
       const int r = r0 + i * RPI, lr = list0 + r, token = row_of_list(z, lr), h = hk * z.group + lr - token * z.group;
-      if (r < wave_rows && col < z.d)
-        *(half8_t*)(z.out + (int64_t)h * z.so_z + (int64_t)(q.row0 + token) * z.so_y + col) =
+      if (r < wave_rows && col0 + col < z.d)
+        *(half8_t*)(z.out + (int64_t)h * z.so_z + (int64_t)(q.row0 + token) * z.so_y + col0 + col) =
             *(const half8_t*)(slot + r * PITCH + col * 2);
     }
     // A value that is no number times the zero of a key that the row does not see is no zero: such rows are computed
-    // again from the keys that they see.
+    // again from the keys that they see, a group's columns of them.
     const uint64_t lanes = __ballot(!finite);
     if (lanes && q.rows > 1 && z.mask == ADR_MASK_CAUSAL) {
       const uint32_t bad = (uint32_t)lanes | (uint32_t)(lanes >> 32);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (behind the stores above)
       for (int r = 0; r < wave_rows; r++)
-        if (bad >> r & 1) row_by_wave(arguments(), q, (list0 + r) / z.group, hk * z.group + (list0 + r) % z.group, lane);
+        if (bad >> r & 1)
+          row_by_wave(arguments(), q, (list0 + r) / z.group, hk * z.group + (list0 + r) % z.group, lane, col0, col0 + 32 * MINE);
     }
   } else if (frow < wave_rows) {
     const int64_t prow = ((int64_t)(slot0 + part) * z.kv_heads + hk) * ROWS + w * 32 + frow;
-    float* const po = z.part_o + prow * HD + 4 * g;
+    float* const po = z.part_o + prow * HD + col0 + 4 * g;
 #pragma unroll
-    for (int d = 0; d < DT; d++)
+    for (int d = 0; d < MINE; d++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        float4_t r;
+        float4_t v;
 #pragma unroll
-        for (int j = 0; j < 4; j++) r[j] = o[d][4 * i + j];
-        *(float4_t*)(po + 32 * d + 8 * i) = r;
+        for (int j = 0; j < 4; j++) v[j] = res[d][4 * i + j];
+        *(float4_t*)(po + 32 * d + 8 * i) = v;
       }
-    if (g == 0) z.part_ml[prow] = make_float2(m_run, l_tot);
+    if (g == 0 && group == 0) z.part_ml[prow] = make_float2(m_run, l_tot);
   }
 }
 
@@ -1266,8 +1336,11 @@ SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
   const int rows = few ? FEW : MANY, keys = few ? FEW_KEYS : MANY_KEYS, hd = a.d <= 64 ? 64 : 128;
   const int64_t most_keys = a.table ? std::min((int64_t)a.table_width * a.page_size, (int64_t)MOST_KEYS) : a.keys;
   const double longest = a.longest > 0 ? std::min<double>(a.longest, most_keys) : most_keys;
-  // blocks: of all key heads, as far as the host can tell
-  const double blocks = std::max((double)a.rows * a.heads / rows, (double)std::min(a.rows, a.sequences) * a.kv_heads);
+  // Blocks of all key heads, as far as the host can tell: a sequence's last one is full by half, but where one sequence has
+  // most of the rows, the others' only ones.
+  const int sequences = std::min(a.rows, a.sequences);
+  const double full = (double)a.rows * a.group / rows, ends = (double)longest_rows * sequences > 4.0 * a.rows ? sequences : sequences / 2.0;
+  const double blocks = a.kv_heads * (few ? std::max(full, (double)sequences) : sequences <= 1 ? ceil(full) : std::max(full + ends, (double)sequences));
   p.least = 1;
   if (few) {
     // Two launches take the host and the device some 4 us more than one, and shared keys leave no workgroup with more
@@ -1285,16 +1358,32 @@ SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
     p.parts = unshared ? 0 : std::max(1, each * cus / a.kv_heads);
     if (p.parts > 0) p.waves = 2;
   } else {
-    // A tile takes a workgroup about a microsecond (0.75 at 64 values) whatever its rows are, two on a compute unit 1.4 as
-    // long.  Shared: the parts' way through memory, 130 KB for a workgroup, is weighed against the tiles that each has.
-    p.waves = 4;
+    // Five ways: one or two groups of wavefronts to a block; keys shared over workgroups or not, and if so, as many as there
+    // are compute units or twice that.  us, fitted to pieces of 64 to 2048 rows over 500 to 8000 keys, 8 key heads of 128
+    // and 4 of 64, and to batches of pieces and tokens: start and end, a tile `one` with a compute unit to itself and `two`
+    // for two tiles beside each other, of two groups or of two workgroups, and the parts' way through memory, 130 KB for a
+    // workgroup.  (1024 rows over 8025 keys, 256 blocks: a group 144, two 134, shared 143; 512 rows: 122, 99, shared by
+    // two groups 78, by twice as many single ones 79; 256 rows: 117, 95, 47.5, 50.5; 64 rows, shared by two groups 27.9, by
+    // as many single ones 25.3.)
+    const double one = hd == 64 ? 0.67 : 1.1, two = hd == 64 ? 1.02 : 2.0, way = hd == 64 ? 0.012 : 0.018;
+    // (several sequences: taken to be three quarters as long as the longest)
+    const double tiles = longest / MANY_KEYS + 1, work = blocks * tiles * (a.sequences == 1 ? 1.0 : 0.75);
+    double best = 7 + (blocks <= cus ? one : two) * tiles;
+    p.waves = 4, p.parts = 0;
     p.least = 4;
-    const double tile = hd == 64 ? 0.75 : 0.96, way = hd == 64 ? 0.0135 : 0.027;
-    const double tiles = longest / MANY_KEYS + 1, work = blocks * tiles;
-    const double n = std::min(2.0 * cus, std::max(blocks, sqrt(work * tile / way)));
-    const bool unshared = a.sequences > 256 || blocks >= 2.0 * cus ||
-                          7 + tiles * tile <= 11 + (n > cus ? 1.4 : 1.0) * work * tile / n + n * way;
-    p.parts = unshared ? 0 : (int)(n / a.kv_heads);
+    if (blocks <= cus && 8 + two * tiles / 2 < best) best = 8 + two * tiles / 2, p.waves = 8;
+    auto shared = [&](int waves, double most, double start, double tile) {
+      double n = std::min(most, sqrt(work * tile / way));
+      // (the blocks of one sequence are of one size, and go into equally many parts; of several, one goes into half a part
+      // too few in the mean)
+      if (a.sequences == 1) n = floor(n / blocks) * blocks;
+      if (a.sequences > 256 || n < (a.sequences == 1 ? 2.0 : 1.5) * blocks) return;
+      const double us = start + work * tile / (a.sequences == 1 ? n : n - blocks / 2) + n * way;
+      if (us < best) best = us, p.waves = waves, p.parts = (int)(n / a.kv_heads + 0.5);
+    };
+    shared(4, cus * 15 / 16.0, 12, one);  // (with as many as there are units some share one: 26.0, 240 of them 24.8)
+    shared(4, 2.0 * cus, 12, two);
+    shared(8, cus, 14, two / 2);
   }
   // (pieces grow where there could be more of them than the line counts)
   const double most_tiles = ((double)a.rows * a.group / rows + a.sequences) * (most_keys / keys + 2.0);
@@ -1326,20 +1415,23 @@ static hipError_t launch_blocks(hipStream_t stream, const SequencesArgs& a, cons
   if (blocks > 0x7fffffff / 256) return hipErrorInvalidConfiguration;
   const int at_once = std::min(rows, 1024 / HD);  // rows of the joining workgroups
   const dim3 grid((unsigned)blocks), join((unsigned)((few ? p.parts - 1 : p.parts / 2) * a.kv_heads * (rows / at_once)));
-  const dim3 few_threads(64 * p.waves);
+  const dim3 threads(64 * p.waves);
   const size_t few_lds = (size_t)p.waves * 4 * FEW_KEYS * HD * 2;
   if (few && p.parts > 0) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, 2, true>), grid, few_threads, few_lds, stream, job);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, 2, true>), grid, threads, few_lds, stream, job);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, FEW>), join, dim3(256), 0, stream, job);
   } else if (few && p.waves == 2) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, 2, false>), grid, few_threads, few_lds, stream, job);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, 2, false>), grid, threads, few_lds, stream, job);
   } else if (few) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, 4, false>), grid, few_threads, few_lds, stream, job);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_few_rows_kernel<HD, PAGED, 4, false>), grid, threads, few_lds, stream, job);
   } else if (p.parts > 0) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, PAGED, true>), grid, dim3(256), 0, stream, job);
+    if (p.waves == 8) hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, PAGED, true, 2>), grid, threads, 0, stream, job);
+    else hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, PAGED, true, 1>), grid, threads, 0, stream, job);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, MANY>), join, dim3(256), 0, stream, job);
+  } else if (p.waves == 8) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, PAGED, false, 2>), grid, threads, 0, stream, job);
   } else {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, PAGED, false>), grid, dim3(256), 0, stream, job);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, PAGED, false, 1>), grid, threads, 0, stream, job);
   }
   return hipGetLastError();
 }
