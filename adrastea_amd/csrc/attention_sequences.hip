@@ -1332,6 +1332,9 @@ SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
   if (!chunks(a)) return p;
   const int longest_rows = a.longest_rows > 0 ? std::min(a.longest_rows, a.rows) : a.rows;
   p.kind = (int64_t)longest_rows * a.group <= FEW ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES;
+  const int forced = knob(KNOB_SEQUENCES);  // (1: any layout; 2 ... 4: few rows; 5 ... 8: many; adr_debug_knob says which)
+  if (forced == 1) return SequencesPlan{SequencesPlan::ANY_LAYOUT, 0, 0, 0, 0, 0};
+  if (forced) p.kind = forced <= 4 ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES;
   const bool few = p.kind == SequencesPlan::FEW_ROWS;
   const int rows = few ? FEW : MANY, keys = few ? FEW_KEYS : MANY_KEYS, hd = a.d <= 64 ? 64 : 128;
   const int64_t most_keys = a.table ? std::min((int64_t)a.table_width * a.page_size, (int64_t)MOST_KEYS) : a.keys;
@@ -1384,6 +1387,12 @@ SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
     shared(4, cus * 15 / 16.0, 12, one);  // (with as many as there are units some share one: 26.0, 240 of them 24.8)
     shared(4, 2.0 * cus, 12, two);
     shared(8, cus, 14, two / 2);
+  }
+  if (forced) {  // (shared in small parts, so that short sequences are divided too)
+    const bool divides = forced == 4 || (forced > 6 && a.sequences <= 256 && full + sequences < 1000);
+    p.waves = forced == 3 || forced == 5 || forced == 7 ? 4 : forced == 6 || forced == 8 ? 8 : 2;
+    p.parts = divides ? std::max(16, cus / a.kv_heads) : 0;
+    p.least = 1;
   }
   // (pieces grow where there could be more of them than the line counts)
   const double most_tiles = ((double)a.rows * a.group / rows + a.sequences) * (most_keys / keys + 2.0);

@@ -557,8 +557,12 @@ int adr_matmul_f16_ws_plan(char* name, int32_t cap, int32_t batches, int32_t m, 
  * GEMM (0: the dispatch decides; 1 + i: tile i of 256x192, 256x128, 128x128, 128x64, 64x64, 128x64
  * with K split over two groups of wavefronts, 64x64 with K split over four; 8: the register-staged
  * kernels that otherwise serve a K that is no multiple of 64; 9: the passes of 64 rows for products
- * of 17 to 256 rows); a forced tile also keeps products of 17 to 256 rows off those passes.  Unknown
- * ids return ADR_EINVAL_ENUM.
+ * of 17 to 256 rows); a forced tile also keeps products of 17 to 256 rows off those passes.  id 2: the kernel of the
+ * attention over several sequences, where the layout is one the matrix-core kernels take (1: a
+ * wavefront per row, as for other layouts; blocks of few rows: 2, 3 unshared with two or four
+ * wavefronts, 4 shared keys; blocks of many rows: 5, 6 unshared with one or two groups of
+ * wavefronts, 7, 8 shared keys; shared keys need a workspace, without one they are unshared).
+ * Unknown ids return ADR_EINVAL_ENUM.
  */
 int adr_debug_knob(int32_t id, int32_t value);
 

@@ -19,13 +19,21 @@ def kern():
     return GpuKernels()
 
 
-@pytest.fixture(params=["unshared", "pool", "workspace"])
+FORMS = ["a row to a wavefront", "few rows, 2 waves", "few rows, 4 waves", "few rows, shared", "many rows", "many rows, 2 groups",
+         "many rows, shared", "many rows, 2 groups, shared"]   # by value of adr_debug_knob(2, 1 + i)
+
+
+@pytest.fixture(params=["unshared", "pool", "workspace", *FORMS])
 def shared_keys(request):
-    """Kernels whose keys are not shared over workgroups, shared through the library's pool, or through their own buffer."""
+    """Kernels whose keys are not shared over workgroups, shared through the library's pool, or through their own buffer;
+    and each form of the kernels by itself, whatever the sizes are."""
     lib = _ffi.lib()
-    lib.adr_set_held_workspace_limit(_ffi.HELD_WORKSPACE_DEFAULT_BYTES if request.param == "pool" else 0)
+    forced = FORMS.index(request.param) + 1 if request.param in FORMS else 0
+    assert lib.adr_debug_knob(2, forced) == 0
+    lib.adr_set_held_workspace_limit(_ffi.HELD_WORKSPACE_DEFAULT_BYTES if request.param == "pool" or forced else 0)
     yield GpuKernels(workspace_bytes=(96 << 20) if request.param == "workspace" else 0)
     lib.adr_set_held_workspace_limit(0)
+    lib.adr_debug_knob(2, 0)
 
 
 def dev(a):
@@ -292,6 +300,59 @@ def test_many_sequences(shared_keys):
     p.check(0.125, CAUSAL)
 
 
+def wide_attention(q, k, v, scale, causal=True):
+    """The definition in 64 bits on the GPU, for sizes that the one in numpy takes too long for: q [heads, r, d]."""
+    heads, r, d = q.shape
+    kv, n, _ = k.shape
+    out = torch.empty(heads, r, d, dtype=torch.float64, device="cuda")
+    hidden = (torch.arange(n, device="cuda")[None, :] > torch.arange(n - r, n, device="cuda")[:, None]) if causal else None
+    for h in range(heads):
+        s = (q[h].double() @ k[h // (heads // kv)].double().t().contiguous()) * scale
+        if causal:
+            s.masked_fill_(hidden, -float("inf"))
+        out[h] = torch.softmax(s, -1) @ v[h // (heads // kv)].double()
+    return out
+
+
+# more rows and keys than one workgroup's: blocks that are divided several times, one sequence among many, a batch of tokens
+LARGE = [([(700, 2900)], 8, 2, 128, 16), ([(300, 5100)], 8, 1, 64, 64), ([(500, 1800), *[(1, 37 * i + 1) for i in range(40)]], 8, 4, 64, 32),
+         ([(1, 150 * i) for i in range(1, 60)], 4, 4, 128, 16), ([(4, 9000), (3, 20), (4, 4000)], 4, 2, 128, 16),
+         ([(130, 1000)] * 5, 6, 2, 128, 128), ([(1, 40000)], 16, 2, 64, 16)]
+
+
+@pytest.mark.parametrize("case", LARGE, ids=["%dx_%dx%d_h%d_%d_d%d" % (len(c[0]), *c[0][0], *c[1:4]) for c in LARGE])
+def test_large_batches(shared_keys, case):
+    seqs, heads, kv, d, page = case
+    gen = torch.Generator(device="cuda").manual_seed(70)
+    rows, longest = sum(r for r, _ in seqs), max(n for _, n in seqs)
+    pages, table = ref.pages_of([n for _, n in seqs], page, np.random.default_rng(71))
+    table_t = ints(table)
+    pool = torch.randn(2, pages, page, kv, d, dtype=torch.float16, device="cuda", generator=gen)
+    q = torch.randn(rows, heads, d, dtype=torch.float16, device="cuda", generator=gen)
+    at, scale = ref.offsets([r for r, _ in seqs]), 1.0 / np.sqrt(d)
+    cache = PagedCache(*(TensorView.of(t).permute([0, 2, 1, 3]) for t in pool))
+    batch = PagedBatch(ints(at), ints([n for _, n in seqs]), table_t, max(r for r, _ in seqs), longest)
+    starts = ref.offsets([n for _, n in seqs])
+    packed = torch.empty(2, int(starts[-1]), kv, d, dtype=torch.float16, device="cuda")
+    for i, (_, n) in enumerate(seqs):
+        packed[:, starts[i]:starts[i + 1]] = pool[:, table_t[i, :-(-n // page)].long()].reshape(2, -1, kv, d)[:, :n]
+    packed_batch = PackedBatch(batch.row_offsets, ints(starts), batch.longest_rows, longest)
+    for mask in (CAUSAL, NONE):
+        paged, from_packed = torch.empty_like(q), torch.empty_like(q)
+        for again in range(2):   # (the same bits: nothing depends on who comes first)
+            out, other = torch.empty_like(q), torch.empty_like(q)
+            shared_keys.attention_paged_f16(heads_view(out), heads_view(q), cache, batch, scale, 1.0, mask)
+            shared_keys.attention_packed_f16(heads_view(other), heads_view(q), *(heads_view(x) for x in packed), packed_batch, scale,
+                                             1.0, mask)
+            assert again == 0 or (torch.equal(out, paged) and torch.equal(other, from_packed))
+            paged, from_packed = out, other
+        for i, (r, n) in enumerate(seqs):
+            k, v = (x[starts[i]:starts[i + 1]].permute(1, 0, 2).contiguous() for x in packed)
+            want = wide_attention(q[at[i]:at[i + 1]].permute(1, 0, 2).contiguous(), k, v, scale, mask == CAUSAL).permute(1, 0, 2).cpu()
+            for got in (paged, from_packed):
+                assert ref.close_enough(got[at[i]:at[i + 1]].cpu().numpy(), want.numpy(), float(v.abs().max()), n), (i, mask)
+
+
 def test_offsets_beyond_32_bits(shared_keys):
     """Pages whose element offsets pass 2^31 and 2^32, through a page stride that spreads few pages over a large buffer."""
     kv, page, d, stride = 2, 16, 64, 1 << 30
@@ -538,6 +599,42 @@ def test_a_captured_step_serves_later_ones():
             kk, vv = (ref.gathered(t, table[s], lengths_now[s]) for t in (k_np, v_np))
             want = ref.attention(q_np[s][:, None], kk, vv, scale)[:, 0]
             assert ref.close_enough(replayed[s].cpu().numpy(), want, np.abs(vv).max(), lengths_now[s])
+
+
+def test_two_streams_at_once(shared_keys):
+    """Calls that run beside each other on two streams, each with its own part of the library's pool."""
+    if shared_keys._workspace is not None:
+        pytest.skip("an instance with a workspace serves one stream")
+    ps = [Paged([(1, 3000), (1, 70)], 4, 2, 128, 16, seed=61), Paged([(90, 2000), (1, 5)], 4, 2, 64, 16, seed=62)]
+    streams = [torch.cuda.Stream() for _ in ps]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for p, s in zip(ps, streams):
+            with torch.cuda.stream(s):
+                shared_keys.attention_paged_f16(heads_view(p.out_t), heads_view(p.q_t), p.cache, p.batch, 0.1)
+    torch.cuda.synchronize()
+    for p in ps:
+        p.check(0.1, CAUSAL)
+
+
+def test_two_graphs_share_a_workspace():
+    """Two captured calls with one instance's buffer, replayed by turns on a stream."""
+    k = GpuKernels(workspace_bytes=64 << 20)
+    ps = [Paged([(1, 3000), (1, 70)], 4, 2, 128, 16, seed=63), Paged([(90, 2000), (1, 5)], 4, 2, 64, 16, seed=64)]
+    graphs = []
+    for p in ps:
+        k.attention_paged_f16(heads_view(p.out_t), heads_view(p.q_t), p.cache, p.batch, 0.1)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            k.attention_paged_f16(heads_view(p.out_t), heads_view(p.q_t), p.cache, p.batch, 0.1)
+    for _ in range(4):
+        for p, g in zip(ps, graphs):
+            p.out_t[:p.row_offsets[-1]] = 0
+            g.replay()
+    torch.cuda.synchronize()
+    for p in ps:
+        p.check(0.1, CAUSAL)
 
 
 def test_another_stream(kern):
