@@ -57,17 +57,20 @@ struct Sequence {
 };
 
 __device__ __forceinline__ Sequence sequence_at(Args a, int s) {
+  // (all four loads at once: one way to memory)
+  const bool paged = a.table != nullptr;
+  const int r0 = a.row_offsets[s], r1 = a.row_offsets[s + 1], k0 = a.keys_of[s], k1 = a.keys_of[s + (paged ? 0 : 1)];
   Sequence q;
   q.index = s;
-  q.row0 = clamp_to(a.row_offsets[s], a.rows);
-  q.rows = max(clamp_to(a.row_offsets[s + 1], a.rows) - q.row0, 0);
-  if (a.table) {
-    q.key0 = 0;
+  q.row0 = clamp_to(r0, a.rows);
+  q.rows = max(clamp_to(r1, a.rows) - q.row0, 0);
+  if (paged) {
     const int64_t room = min((int64_t)a.table_width * a.page_size, (int64_t)MOST_KEYS);
-    q.keys = (int)min((int64_t)max(a.keys_of[s], 0), room);
+    q.key0 = 0;
+    q.keys = (int)min((int64_t)max(k0, 0), room);
   } else {
-    q.key0 = clamp_to(a.keys_of[s], a.keys);
-    q.keys = max(clamp_to(a.keys_of[s + 1], a.keys) - q.key0, 0);
+    q.key0 = clamp_to(k0, a.keys);
+    q.keys = max(clamp_to(k1, a.keys) - q.key0, 0);
   }
   return q;
 }
@@ -439,6 +442,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
   const half_t* const V = a.v + hk * a.sv.z + (PAGED ? 0 : q.key0 * a.sv.y);
   const uint32_t lds0 = (uint32_t)(uintptr_t)ADR_LDS_PTR(smem) + w * WAVE;
   const unsigned char* const sm = smem + w * WAVE;
+  // The queries' fragments, by way of the second tile of values, which comes after them: nothing waits for them before the
+  // first keys are on their way.  (Chunks behind the head dimension are zeros below.)
+  const int d = a.d, k_stride = (int)a.sk.y, v_stride = (int)a.sv.y;
+  const half_t* const qrow =
+      a.q + (int64_t)(hk * a.group + gh) * a.sq_z + (int64_t)(q.row0 + row) * a.sq_y;
+#pragma unroll
+  for (int ks = 0; ks < KS; ks++) {
+    const int col = ks * 32 + g * 8;
+    dma_global(lds0 + 3 * TILE + ks * 1024, qrow + (col < d ? col : 0));
+  }
   // Byte offsets of a lane's chunks in 16 rows (the second 16 rows of a tile repeat them); chunks behind the head
   // dimension lie behind every descriptor's end and come as zeros.
   uint32_t koff[NI / 2], voff[NI / 2];
@@ -447,8 +460,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
     int krow, kc;
     k_chunk_inv<CPR>(j * 64 + lane, krow, kc);
     const int vrow = (j * 64 + lane) / CPR, vc = (lane % CPR) ^ v_swz8<CPR>(vrow);
-    koff[j] = kc * 8 < a.d ? (uint32_t)((krow * (int)a.sk.y + kc * 8) * 2 + BIAS - j * 1024) : 0x7fff0000u;
-    voff[j] = vc * 8 < a.d ? (uint32_t)((vrow * (int)a.sv.y + vc * 8) * 2 + BIAS - j * 1024) : 0x7fff0000u;
+    const uint32_t ko = (uint32_t)((krow * k_stride + kc * 8) * 2 + BIAS - j * 1024);
+    const uint32_t vo = (uint32_t)((vrow * v_stride + vc * 8) * 2 + BIAS - j * 1024);
+    koff[j] = kc * 8 < d ? ko : 0x7fff0000u;
+    voff[j] = vc * 8 < d ? vo : 0x7fff0000u;
   }
   // Where the keys and values of 32 of the wavefront's tiles lie, a lane to each 16 keys: their addresses are worked
   // out by the vector ALU once, not by scalar instructions for each tile.  (Addresses are even: an odd one says that there
@@ -475,13 +490,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
   // Keys, or values, of tile i.
   auto fetch = [&](int i, auto is_k) __attribute__((always_inline)) {
     constexpr bool IS_K = decltype(is_k)::value;
-    const int stride = (int)(IS_K ? a.sk.y : a.sv.y);
+    const int stride = IS_K ? k_stride : v_stride;
     const uint64_t at = IS_K ? k_at : v_at;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       const int l = 2 * (i & 31) + h, left = min(row_end - (tile0 + w + WAVES * i) * KEYS - 16 * h, 16);
       const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)at, l), hi = __builtin_amdgcn_readlane((uint32_t)(at >> 32), l);
-      const u32x4_t desc = {lo & ~1u, hi & 0xffffu, lo & 1 ? (uint32_t)(((left - 1) * stride + a.d) * 2 + BIAS) : 0u, 0x00020000u};
+      const u32x4_t desc = {lo & ~1u, hi & 0xffffu, lo & 1 ? (uint32_t)(((left - 1) * stride + d) * 2 + BIAS) : 0u, 0x00020000u};
       dma_buffer_once<NI / 2>(lds0 + ((IS_K ? 0 : 2) + (i & 1)) * TILE + h * (NI / 2) * 1024, IS_K ? koff : voff, desc);
     }
   };
@@ -489,20 +504,22 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
   const std::false_type is_v{};
 
   look_up(0);
+  // (the lookup's load has landed before the transfers' own count begins)
+  if (tiles > 0) fetch(0, is_k), fetch(0, is_v);
+  if (tiles > 1) fetch(1, is_k);
+  if (tiles > 1) wait_vm<3 * NI>();
+  else if (tiles > 0) wait_vm<2 * NI>();
+  else wait_vm<0>();
   half8_t qf[KS];
-  const half_t* const qrow =
-      a.q + (int64_t)(hk * a.group + gh) * a.sq_z + (int64_t)(q.row0 + row) * a.sq_y;
 #pragma unroll
   for (int ks = 0; ks < KS; ks++) {
-    const int col = ks * 32 + g * 8;
-    qf[ks] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
-    if (col < a.d) qf[ks] = *(const half8_t*)(qrow + col);
+    qf[ks] = *(const half8_t*)(sm + 3 * TILE + ks * 1024 + lane * 16);
+    if (ks * 32 + g * 8 >= d) qf[ks] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
   }
-  // (the loads above have landed before the transfers' own count begins)
 #pragma unroll
   for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(qf[ks]));
-  if (tiles > 0) fetch(0, is_k), fetch(0, is_v);
-  if (tiles > 1) fetch(1, is_k), fetch(1, is_v);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  if (tiles > 1) fetch(1, is_v);
   int offK[KS], offV[DB];
 #pragma unroll
   for (int ks = 0; ks < KS; ks++) offK[ks] = k_chunk_off<CPR>(frow, ks * 4 + g);
@@ -734,6 +751,18 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
   // (lanes without a row of their own compute the block's last one)
   const int list_row = block * ROWS + min(w * 32 + frow, rows - 1), row = row_of_list(a, list_row), gh = list_row - row * a.group;
   const int lane_end = end_of_row(a, q, row);
+  unsigned char* const sm = smem + group * (4 * TILE);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)ADR_LDS_PTR(smem) + group * (4 * TILE);
+  const int d = a.d, k_stride = (int)a.sk.y, v_stride = (int)a.sv.y;
+  // The queries' fragments, by way of the values' LDS, so that nothing waits for them before the first keys are on their
+  // way.  (Chunks behind the head dimension are zeros below.)
+  static_assert(4 * DS * 1024 <= 2 * TILE, "the queries fit the values' tiles");
+  const half_t* const qrow = a.q + (int64_t)(hk * a.group + gh) * a.sq_z + (int64_t)(q.row0 + row) * a.sq_y;
+#pragma unroll
+  for (int ds = 0; ds < DS; ds++) {
+    const int col = ds * 16 + g * 8;
+    dma_global(lds0 + 2 * TILE + (w * DS + ds) * 1024, qrow + (col < d ? col : 0));
+  }
 
   const int last_end = uniform(end_of_row(a, q, row_of_list(a, block * ROWS + rows - 1)));
   const int all = (last_end + KEYS - 1) / KEYS;
@@ -751,8 +780,6 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     first_edge = uniform(end_of_row(a, q, row_of_list(a, list0))) / KEYS - tile0;
   }
 
-  unsigned char* const sm = smem + group * (4 * TILE);
-  const uint32_t lds0 = (uint32_t)(uintptr_t)ADR_LDS_PTR(smem) + group * (4 * TILE);
   // Wavefront w transfers rows 16 w ... 16 w + 15 of a tile, 1 KiB at a time: byte offsets of a lane's chunks in those
   // rows, less the j KiB that the instruction adds; chunks behind the head dimension come as zeros.
   uint32_t koff[NI], voff[NI];
@@ -761,8 +788,10 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     int krow, kc;
     k_chunk_inv<CPR>(j * 64 + lane, krow, kc);
     const int vrow = (j * 64 + lane) / CPR, vc = (lane % CPR) ^ v_swz<CPR>(vrow);
-    koff[j] = kc * 8 < a.d ? (uint32_t)((krow * (int)a.sk.y + kc * 8) * 2 + BIAS - j * 1024) : 0x7fff0000u;
-    voff[j] = vc * 8 < a.d ? (uint32_t)((vrow * (int)a.sv.y + vc * 8) * 2 + BIAS - j * 1024) : 0x7fff0000u;
+    const uint32_t ko = (uint32_t)((krow * k_stride + kc * 8) * 2 + BIAS - j * 1024);
+    const uint32_t vo = (uint32_t)((vrow * v_stride + vc * 8) * 2 + BIAS - j * 1024);
+    koff[j] = kc * 8 < d ? ko : 0x7fff0000u;
+    voff[j] = vc * 8 < d ? vo : 0x7fff0000u;
   }
   // The wavefront's next 16 key and value rows: address, and bytes from there to the last key (0 behind it).  On
   // pages, the addresses of 64 tiles at a time, a lane to each, worked out by the vector ALU.  (Addresses are even: an
@@ -776,7 +805,7 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
   int page = 0;
   auto locate = [&](Next& t, auto is_k) __attribute__((always_inline)) {
     const int left = min(row_end - t.key, 16);
-    t.bytes = left > 0 ? ((left - 1) * t.stride + a.d) * 2 + BIAS : 0;
+    t.bytes = left > 0 ? ((left - 1) * t.stride + d) * 2 + BIAS : 0;
     if constexpr (PAGED) {
       const int n = ((t.key - 16 * w) >> 6) - tile0;
       if ((n & 63) == 0) {
@@ -810,13 +839,6 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     locate(t, k);
     return t;
   };
-  half8_t qf[DS];  // (operand B of S^T = K Q^T: lane -> row frow, head-dimension group g)
-  const half_t* const qrow = a.q + (int64_t)(hk * a.group + gh) * a.sq_z + (int64_t)(q.row0 + row) * a.sq_y + g * 8;
-#pragma unroll
-  for (int ds = 0; ds < DS; ds++) {
-    qf[ds] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
-    if (ds * 16 + g * 8 < a.d) qf[ds] = *(const half8_t*)(qrow + ds * 16);
-  }
   Next nk = first_tile(a.k + hk * a.sk.z, a.sk.y, a.sk.p, is_k), nv = first_tile(a.v + hk * a.sv.z, a.sv.y, a.sv.p, is_v);
   auto advance = [&](Next& t, auto k) __attribute__((always_inline)) {
     t.key += KEYS;
@@ -847,9 +869,16 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
   int offK[DS];
 #pragma unroll
   for (int ds = 0; ds < DS; ds++) offK[ds] = k_chunk_off<CPR>(frow, ds * 2 + g);
+  wait_vm<NI>();  // the queries and the first K tile have landed
+  half8_t qf[DS];  // (operand B of S^T = K Q^T: lane -> row frow, head-dimension group g)
+#pragma unroll
+  for (int ds = 0; ds < DS; ds++) {
+    qf[ds] = *(const half8_t*)(sm + 2 * TILE + (w * DS + ds) * 1024 + lane * 16);
+    if (ds * 16 + g * 8 >= d) qf[ds] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+  }
 #pragma unroll
   for (int ds = 0; ds < DS; ds++) asm volatile("" : "+v"(qf[ds]));
-  wait_vm<NI>();  // the first K tile has landed
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (values come there behind the next barrier)
   // V (transposing read): in each group of 16 lanes, lanes 4r..4r+3 address 16 consecutive halves of tile row r, and
   // lane i of the group receives column i of that 4 x 16 block.  Group b = (lane / 16) % 2 takes columns 16b.. of the
   // 32-column tile, g the rows 4g..4g+3.
@@ -1168,7 +1197,7 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     static_assert(EXCHANGE + 4 * 32 * PITCH <= 4 * TILE, "the output's slots fit the LDS");
     unsigned char* const slot = sm + EXCHANGE + w * (32 * PITCH);
     const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
-    bool finite = true;
+    float zero[2] = {0.0f, 0.0f};  // (NaN behind a value that is not finite)
 #pragma unroll
     for (int d = 0; d < MINE; d++)
 #pragma unroll
@@ -1177,7 +1206,7 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const float v = res[d][4 * i + j] * inv;
-          finite = finite && fabsf(v) < INFINITY;
+          zero[j & 1] = fmaf(v, 0.0f, zero[j & 1]);
           h[j] = (half_t)v;
         }
         *(half4_t*)(slot + frow * PITCH + (32 * d + 8 * i + 4 * g) * 2) = h;
@@ -1185,17 +1214,21 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the slot is the wavefront's own)
     constexpr int RPI = 64 / CHUNKS;  // rows of a store instruction
     const int r0 = lane / CHUNKS, col = lane % CHUNKS * 8;
+    int token = row_of_list(z, list0 + r0), head = list0 + r0 - token * z.group;  // of the group
+    const int more_tokens = row_of_list(z, RPI), more_heads = RPI - more_tokens * z.group;
+    half_t* const out = z.out + (int64_t)(hk * z.group) * z.so_z + (int64_t)q.row0 * z.so_y + col0 + col;
 #pragma unroll
     for (int i = 0; i < 32 / RPI; i++) {
       if (i * RPI >= wave_rows) break;
-      const int r = r0 + i * RPI, lr = list0 + r, token = row_of_list(z, lr), h = hk * z.group + lr - token * z.group;
+      const int r = r0 + i * RPI;
       if (r < wave_rows && col0 + col < z.d)
-        *(half8_t*)(z.out + (int64_t)h * z.so_z + (int64_t)(q.row0 + token) * z.so_y + col0 + col) =
-            *(const half8_t*)(slot + r * PITCH + col * 2);
+        *(half8_t*)(out + (int64_t)head * z.so_z + (int64_t)token * z.so_y) = *(const half8_t*)(slot + r * PITCH + col * 2);
+      token += more_tokens, head += more_heads;
+      if (head >= z.group) head -= z.group, token++;
     }
     // A value that is no number times the zero of a key that the row does not see is no zero: such rows are computed
     // again from the keys that they see, a group's columns of them.
-    const uint64_t lanes = __ballot(!finite);
+    const uint64_t lanes = __ballot(!(zero[0] + zero[1] == 0.0f));
     if (lanes && q.rows > 1 && z.mask == ADR_MASK_CAUSAL) {
       const uint32_t bad = (uint32_t)lanes | (uint32_t)(lanes >> 32);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (behind the stores above)
