@@ -394,7 +394,12 @@ __device__ __forceinline__ u32x4_t descriptor(uint64_t p, int bytes) {
 // A block of 16 rows against its keys: a read of the keys and values.  The workgroup's wavefronts walk tiles of
 // 32 keys in turn, each through two tiles' worth of LDS of its own, so that the loop has no barrier.  S^T = K Q^T, so
 // that a lane holds scores of one row, and O^T = V^T P^T, on MFMA 16x16x32; probabilities are rounded to fp16, the
-// matrix cores' operands, sums and scores stay in 32 bits.
+// matrix cores' operands, sums and scores stay in 32 bits.  (fp16 probabilities cost 2^-11 of each; a product in 32 bits would be
+// no matrix product, and its values are fp16 anyway.)
+//
+// Bound by memory: 16 rows of every key read once leave the matrix cores 5 % busy.  64 sequences of 3 to 4000 keys (32 / 8
+// heads of 128, 504 MB) 88.5 us = 5.7 TB/s, eight of 50000 to 110000 (40 / 8, 2.36 GB) 366 us = 6.4 TB/s, where a plain read
+// reaches 7.0 to 7.3; one of 777 keys (32 / 32) 9.7 us, of which two launches are 8.8 on the host.
 template <int HD, bool PAGED, int WAVES, bool SHARED>
 __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) {
   constexpr int CPR = HD / 8, KEYS = 32, ROWS = 16;
@@ -704,6 +709,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
 // beside the maximum of tile i + 1.  What is different here is where rows and keys come from: the heads of a group
 // share the block, so that a key row is read once for all of them and the part of a tile that the mask leaves empty
 // is 1 / group as wide, and each wavefront's 16 key rows of a tile have a base address of their own, on a page.
+//
+// GROUPS == 2: eight wavefronts, of which four take the first half of the block's keys and four the second, each through
+// tiles of its own; both ends meet in LDS.  Two workgroups beside each other do as much, but that takes twice as many blocks,
+// or parts that go through memory: 1024 rows over 8025 keys (256 blocks) 134 us, by halves through memory 143, one group on
+// each compute unit 144.
+//
+// Bound by power, and by issue as in attention_fwd_kernel: one prompt of 16384 rows (32 / 8 heads of 128) 2001 us = 1099
+// TFLOP/s with the matrix cores busy 69 % of cycles at 1.6 GHz, where a product of 8192^3 reaches 1408.  Short blocks are
+// bound by their beginnings and ends: us of a block among others, 2.0 from the end of one to the start of the next in its place,
+// 1.8 to find its sequence, 1.9 for addresses, 1.8 until the first keys are there, 1.9 a tile, 2.4 for the results (nine prompts
+// of 100 to 3996 rows, 25 tiles a block in the mean, 446 us = 934 TFLOP/s; the tiles of wavefronts whose rows end early, and of rows
+// that the mask hides, are in these figures as work that is not counted).
 template <int HD, bool PAGED, bool SHARED, int GROUPS>
 __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
   constexpr int CPR = HD / 8, KEYS = 64, ROWS = 128;
