@@ -258,7 +258,7 @@ struct Roster {
     if (SHARED) line.parts = max(1, min(a.parts, end / a.least));
     return line;
   }
-  // The block at `place` of the line; false: the line ends before.
+  // The block at `place` of the line; false: the line ends before (or offsets that decrease made it longer than it counts).
   __device__ __forceinline__ bool block_at(Args a, int shift, int place, int lane, Block& b) {
     if (place < before) load(a, shift, lane, 0, 0);
     while (place >= end) {
@@ -279,7 +279,7 @@ struct Roster {
         b.block = blocks - 1 - i;
         b.offset = in - i * p;
         b.pieces = p;
-        return true;
+        return in >= 0 && b.block >= 0;
       }
     }
     return false;
@@ -294,7 +294,7 @@ __device__ __forceinline__ Seam seam_at(const Line& line, int part, int place, c
   if (before > begin) return s;
   // stretches part - 1 ... last; the first of them has the block behind others, unless it begins with it
   const int last = uniform((int)(((double)(begin + b.pieces) * (double)line.parts - 1.0) / (double)line.total));
-  s.parts = last - part + 2;
+  s.parts = min(last, line.parts - 1) - part + 2;
   s.slot = 2 * (part - 1) + (before != begin);
   return s;
 }
@@ -339,7 +339,7 @@ __device__ __forceinline__ bool part_at(Args a, int index, int lane, Part& p) {
     int n = 0, fewer = UNDIVIDED;  // the least that some block has a part less with
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
-      const int each = parts_of(tiles[e], inv, most);
+      const int each = min(parts_of(tiles[e], inv, most), a.parts + 1);  // (so that the sum stays within 32 bits)
       n += blocks[e] * each;
       if (blocks[e] > 0 && each > 1) fewer = min(fewer, (int)((float)tiles[e] * __builtin_amdgcn_rcpf((float)(each - 1))) + 1);
     }
@@ -427,7 +427,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
   const int tid = thread_index(), lane = tid & 63, w = uniform(tid >> 6);
   const int frow = lane & 15, g = lane >> 4;
   Block b;
-  if (!roster.block_at(a, a.shift, place, lane, b)) return;
+  if (!roster.block_at(a, a.shift, place, lane, b)) {
+    if (SHARED && place == stretch0 && tid == 0) a.seams[wg * kv_heads + hk].parts = 0;
+    return;
+  }
   const Sequence q = b.q;
   const int block = b.block, pieces = min(stretch1 - place, b.pieces - b.offset);
   const bool whole = pieces == b.pieces;
@@ -1469,7 +1472,7 @@ static hipError_t launch_blocks(hipStream_t stream, const SequencesArgs& a, cons
   job.part_ml = (float2*)(job.part_o + (p.parts > 0 ? part_rows * HD : 0));
   job.seams = (Seam*)(job.part_ml + (p.parts > 0 ? part_rows : 0));
   // Unshared: as many as there can be blocks.  Shared: a stretch to each, or a part.
-  const int64_t most = (int64_t)a.rows * a.group / rows + a.sequences;  // blocks of a key head
+  const int64_t most = (int64_t)a.rows * a.group / rows + std::min(a.rows, a.sequences);  // blocks of a key head
   const int64_t blocks = (p.parts == 0 ? most : few ? p.parts : std::max<int64_t>(p.parts, most)) * a.kv_heads;
   if (blocks > 0x7fffffff / 256) return hipErrorInvalidConfiguration;
   const int at_once = std::min(rows, 1024 / HD);  // rows of the joining workgroups

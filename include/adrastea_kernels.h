@@ -394,14 +394,15 @@ int64_t adr_attention_f16_workspace_bytes(int32_t heads, int32_t m, int32_t n, i
  *
  * Rows are packed: sequence s has rows row_offsets[s] .. row_offsets[s + 1] - 1 of the [heads, rows, d]
  * views (strides x = dim -1, y = dim -2, z = dim -3 as above, any strides, negative ones included).
- * Offsets are clamped to 0 .. rows; a sequence may have no rows; rows in front of the first and
- * behind the last sequence are neither read nor written.
+ * Offsets are clamped to 0 .. rows and do not decrease (where they do, rows that several sequences claim,
+ * or none, hold any of their results, or none); a sequence may have no rows; rows in front of the first
+ * and behind the last sequence are neither read nor written.
  *
  * adr_paged_cache: key and value pages as [pages, kv_heads, page_size, d] views of one pool each,
  * strides in elements (x value, y slot, z head, p page), 64 bits.
  * adr_paged_batch: sequence s has lengths[s] keys in the cache, those of its rows in this call
- * included; key x lies in page table[s * table_pitch + x / page_size], slot x % page_size.  Lengths are
- * taken as at least 0 and at most table_width * page_size and 2^30.  Entries beyond a sequence's length are not
+ * included; key x lies in page table[s * table_pitch + x / page_size], slot x % page_size.  The attention
+ * takes lengths as at least 0 and at most table_width * page_size and 2^30.  Entries beyond a sequence's length are not
  * read.  longest_rows and longest are the largest number of rows and keys of any sequence as far as the
  * host knows (0: unknown): they choose kernels and nothing else, every result is right whatever they say.
  */
@@ -471,10 +472,11 @@ int adr_append_f16(adr_stream_t stream, adr_paged_cache cache, adr_paged_batch b
  * head h
  *   out[h, row, :] = sum_x softmax_x( scale * <query[h, row, :], key[x]> / temp ) * value[x],
  * over the keys of kv head h / (heads / kv_heads), x <= j + n - r under ADR_MASK_CAUSAL (the last row
- * sees all keys) and all x under ADR_MASK_NONE.  A row that sees no key, or whose scores are all -inf,
- * becomes zeros; keys that a row does not see, and slots behind the last key, never reach it, whatever they
+ * sees all keys) and all x under ADR_MASK_NONE.  A row that sees no key, or whose scores are all -inf
+ * while its values are finite, becomes zeros; keys that a row does not see, and slots behind the last key, never reach it, whatever they
  * hold (infinities and NaN included).  A key on a page outside 0 .. pages - 1 counts as NaN for the rows
  * that see it.  Scores, softmax and sums in fp32; probabilities are rounded to fp16 for the matrix cores.
+ * `output` overlaps none of the others.
  * d 1 .. 256, scale > 0, temp > 0 (ADR_EUNSUPPORTED_LAYOUT beyond), heads a multiple of kv_heads.  The fast
  * kernels take d a multiple of 8 up to 128, x strides 1, the others multiples of 8 and not negative, slots at
  * least d apart and less than 2^24, 16-byte aligned pointers, pages of 16, 32, 64 ... slots; everything else runs on

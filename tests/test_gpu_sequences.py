@@ -601,6 +601,22 @@ def test_a_captured_step_serves_later_ones():
             assert ref.close_enough(replayed[s].cpu().numpy(), want, np.abs(vv).max(), lengths_now[s])
 
 
+def test_offsets_that_decrease(shared_keys):
+    """Rows that only one sequence claims are right; the others hold some result, and nothing else is written."""
+    p = Paged([(10, 300), (0, 40), (10, 500)], 4, 2, 64, 16, seed=65)
+    want = p.want(0.125, CAUSAL)
+    # (sequence 1 ends before it begins; sequence 2 begins among the rows of sequence 0)
+    p.seqs = [(10, 300), (0, 40), (15, 500)]
+    batch = PagedBatch(ints([0, 10, 5, 20]), p.batch.lengths, p.batch.table)
+    shared_keys.attention_paged_f16(heads_view(p.out_t), heads_view(p.q_t), p.cache, batch, 0.125)
+    got = p.out_t.cpu().numpy()
+    k, v = (ref.gathered(x, p.table[2], 500) for x in (p.k, p.v))
+    behind = ref.attention(p.q[5:20].transpose(1, 0, 2), k, v, 0.125).transpose(1, 0, 2)
+    top = np.nanmax(np.abs(p.v.astype(np.float64)))
+    assert ref.close_enough(got[:5], want[:5], top, 300) and ref.close_enough(got[10:20], behind[5:], top, 500)
+    assert np.isfinite(got[5:10]).all() and (got[20:] == SENTINEL).all()
+
+
 def test_two_streams_at_once(shared_keys):
     """Calls that run beside each other on two streams, each with its own part of the library's pool."""
     if shared_keys._workspace is not None:
