@@ -123,6 +123,30 @@ struct CommonKernels {
                                const TensorView<const f16>& rhs) = 0;
   virtual void error_stats_f32(TensorView<float>& output, const TensorView<const float>& lhs,
                                const TensorView<const float>& rhs) = 0;
+  // Several sequences at once (an interface of its own, for implementations that offer it): see adr_rotary_f16,
+  // adr_append_f16, adr_attention_paged_f16 and adr_attention_packed_f16.
+  // The rows of `input` turned by positions[row] (device memory, [rows]) into `output`, which may be the same view.
+  virtual void rotary_f16(TensorView<f16>& /*output*/, const TensorView<const f16>& /*input*/, const int32_t* /*positions*/,
+                          const Rotary& /*rotary*/) {
+    throw AdrasteaError(ADR_ENOTIMPL, "rotary_f16");
+  }
+  // The step's keys, turned, and values into their pages, and its queries turned into `query_out` (both null: none).
+  virtual void append_f16(const PagedCache& /*cache*/, const PagedBatch& /*batch*/, const TensorView<const f16>& /*key*/,
+                          const TensorView<const f16>& /*value*/, const Rotary& /*rotary*/, TensorView<f16>* /*query_out*/ = nullptr,
+                          const TensorView<const f16>* /*query*/ = nullptr, const int32_t* /*positions*/ = nullptr) {
+    throw AdrasteaError(ADR_ENOTIMPL, "append_f16");
+  }
+  virtual void attention_paged_f16(TensorView<f16>& /*output*/, const TensorView<const f16>& /*query*/, const PagedCache& /*cache*/,
+                                   const PagedBatch& /*batch*/, float /*scale*/, float /*temperature*/ = 1.0f,
+                                   MatmulMask /*mask*/ = MatmulMask::Causal) {
+    throw AdrasteaError(ADR_ENOTIMPL, "attention_paged_f16");
+  }
+  virtual void attention_packed_f16(TensorView<f16>& /*output*/, const TensorView<const f16>& /*query*/,
+                                    const TensorView<const f16>& /*key*/, const TensorView<const f16>& /*value*/,
+                                    const PackedBatch& /*batch*/, float /*scale*/, float /*temperature*/ = 1.0f,
+                                    MatmulMask /*mask*/ = MatmulMask::Causal) {
+    throw AdrasteaError(ADR_ENOTIMPL, "attention_packed_f16");
+  }
 };
 
 // TensorGpuDescriptor::from (kernels.rs:38-55): dims and strides reversed, innermost first.
@@ -216,17 +240,16 @@ class GpuKernels : public CommonKernels {
   static void same(const Rows& a, const Rows& b, const char* what) {
     if (a.heads != b.heads || a.rows != b.rows || a.d != b.d) throw std::logic_error(std::string(what) + ": shape mismatch");
   }
-  // The rows of `input` turned by positions[row] (device memory, [rows]) into `output`, which may be the same view.
-  void rotary_f16(TensorView<f16>& output, const TensorView<const f16>& input, const int32_t* positions, const Rotary& rotary) {
+  void rotary_f16(TensorView<f16>& output, const TensorView<const f16>& input, const int32_t* positions,
+                  const Rotary& rotary) override {
     const Rows o = rows_of(output, "rotary_f16"), i = rows_of(input, "rotary_f16");
     same(o, i, "rotary_f16");
     int rc = adr_rotary_f16(stream_, output.ptr, input.ptr, positions, rotary, i.heads, i.rows, i.d, o.x, o.y, o.z, i.x, i.y, i.z);
     if (rc) throw AdrasteaError(rc, "rotary_f16");
   }
-  // The step's keys, turned, and values into their pages, and its queries turned into `query_out` (both null: none).
   void append_f16(const PagedCache& cache, const PagedBatch& batch, const TensorView<const f16>& key, const TensorView<const f16>& value,
                   const Rotary& rotary, TensorView<f16>* query_out = nullptr, const TensorView<const f16>* query = nullptr,
-                  const int32_t* positions = nullptr) {
+                  const int32_t* positions = nullptr) override {
     const adr_paged_cache c = cache.lower();
     const Rows k = rows_of(key, "append_f16"), v = rows_of(value, "append_f16");
     same(k, v, "append_f16");
@@ -242,7 +265,7 @@ class GpuKernels : public CommonKernels {
     if (rc) throw AdrasteaError(rc, "append_f16");
   }
   void attention_paged_f16(TensorView<f16>& output, const TensorView<const f16>& query, const PagedCache& cache, const PagedBatch& batch,
-                           float scale, float temperature = 1.0f, MatmulMask mask = MatmulMask::Causal) {
+                           float scale, float temperature = 1.0f, MatmulMask mask = MatmulMask::Causal) override {
     const adr_paged_cache c = cache.lower();
     const Rows o = rows_of(output, "attention_paged_f16"), q = rows_of(query, "attention_paged_f16");
     same(o, q, "attention_paged_f16");
@@ -256,7 +279,7 @@ class GpuKernels : public CommonKernels {
   }
   void attention_packed_f16(TensorView<f16>& output, const TensorView<const f16>& query, const TensorView<const f16>& key,
                             const TensorView<const f16>& value, const PackedBatch& batch, float scale, float temperature = 1.0f,
-                            MatmulMask mask = MatmulMask::Causal) {
+                            MatmulMask mask = MatmulMask::Causal) override {
     const char* what = "attention_packed_f16";
     const Rows o = rows_of(output, what), q = rows_of(query, what), k = rows_of(key, what), v = rows_of(value, what);
     same(o, q, what), same(k, v, what);
@@ -308,6 +331,23 @@ class MatmulTracer : public CommonKernels {
   }
   void error_stats_f16(TensorView<float>& out, const TensorView<const f16>& l, const TensorView<const f16>& r) override { inner_.error_stats_f16(out, l, r); }
   void error_stats_f32(TensorView<float>& out, const TensorView<const float>& l, const TensorView<const float>& r) override { inner_.error_stats_f32(out, l, r); }
+  void rotary_f16(TensorView<f16>& o, const TensorView<const f16>& i, const int32_t* positions, const Rotary& rotary) override {
+    inner_.rotary_f16(o, i, positions, rotary);
+  }
+  void append_f16(const PagedCache& cache, const PagedBatch& batch, const TensorView<const f16>& k, const TensorView<const f16>& v,
+                  const Rotary& rotary, TensorView<f16>* query_out = nullptr, const TensorView<const f16>* query = nullptr,
+                  const int32_t* positions = nullptr) override {
+    inner_.append_f16(cache, batch, k, v, rotary, query_out, query, positions);
+  }
+  void attention_paged_f16(TensorView<f16>& o, const TensorView<const f16>& q, const PagedCache& cache, const PagedBatch& batch,
+                           float scale, float t = 1.0f, MatmulMask mask = MatmulMask::Causal) override {
+    inner_.attention_paged_f16(o, q, cache, batch, scale, t, mask);
+  }
+  void attention_packed_f16(TensorView<f16>& o, const TensorView<const f16>& q, const TensorView<const f16>& k,
+                            const TensorView<const f16>& v, const PackedBatch& batch, float scale, float t = 1.0f,
+                            MatmulMask mask = MatmulMask::Causal) override {
+    inner_.attention_packed_f16(o, q, k, v, batch, scale, t, mask);
+  }
 
  private:
   void rec(const TensorView<f16>& o, const TensorView<const f16>& l, const TensorView<const f16>& r) {

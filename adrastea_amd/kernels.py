@@ -735,9 +735,26 @@ def attention_workspace_bytes(output: TensorLayout, query: TensorLayout, key: Te
     return int(n)
 
 
+def attention_paged_workspace_bytes(cache: PagedCache, batch: PagedBatch, heads: int, rows: int) -> int:
+    """Scratch bytes adr_attention_paged_f16_ws would use for `rows` packed rows of `heads` query heads (0: it would share no
+    keys)."""
+    n = _ffi.lib().adr_attention_paged_f16_workspace_bytes(cache._desc, batch._desc, heads, rows)
+    if n < 0:
+        raise AdrasteaError(int(n), "attention_paged_f16_workspace_bytes")
+    return int(n)
+
+
+def attention_packed_workspace_bytes(batch: PackedBatch, heads: int, kv_heads: int, rows: int, keys: int, d: int) -> int:
+    """Scratch bytes adr_attention_packed_f16_ws would use for these sizes (0: it would share no keys)."""
+    n = _ffi.lib().adr_attention_packed_f16_workspace_bytes(batch._desc, heads, kv_heads, rows, keys, d)
+    if n < 0:
+        raise AdrasteaError(int(n), "attention_packed_f16_workspace_bytes")
+    return int(n)
+
+
 def set_held_workspace_limit(nbytes: int) -> None:
-    """Bytes per buffer of the workspace pool that adr_matmul_f16, adr_matmul_nt_f16 and
-    adr_attention_f16 (and, on request, adr_matmul_nt_fp16u8) draw from, one buffer per (device, stream); 0 switches it off."""
+    """Bytes per buffer of the workspace pool that adr_matmul_f16, adr_matmul_nt_f16, adr_attention_f16, adr_attention_paged_f16 and
+    adr_attention_packed_f16 (and, on request, adr_matmul_nt_fp16u8) draw from, one buffer per (device, stream); 0 switches it off."""
     rc = _ffi.lib().adr_set_held_workspace_limit(int(nbytes))
     if rc != 0:
         raise AdrasteaError(int(rc), "set_held_workspace_limit")

@@ -28,7 +28,8 @@ static void cpu_tests() {
   CHECK(throws([&] { PagedCache{cache.key, {P, TensorLayout::row_major({5, 2, 16, 64})}}.lower(); }));
   CHECK(throws([&] { PagedCache{{P, TensorLayout::row_major({6, 2, 64})}, {P, TensorLayout::row_major({6, 2, 64})}}.lower(); }));
 
-  GpuKernels k;
+  GpuKernels gpu;
+  MatmulTracer k(gpu);  // (forwards them)
   const PagedBatch batch{(const int32_t*)P, (const int32_t*)P, (const int32_t*)P, 2, 3, 3, 1, 48};
   TensorView<f16> out(P, TensorLayout::row_major({4, 3, 64})), fewer(P, TensorLayout::row_major({4, 2, 64}));
   const TensorView<const f16> q(P, out.layout), kv(P, TensorLayout::row_major({2, 3, 64})), wide(P, TensorLayout::row_major({4, 3, 72}));
@@ -45,6 +46,25 @@ static void cpu_tests() {
   } catch (const AdrasteaError& e) {
     CHECK(e.code == ADR_EUNSUPPORTED_LAYOUT);
   }
+  struct Other : CommonKernels {  // an implementation from before these calls
+    void matmul_f16(TensorView<f16>&, const TensorView<const f16>&, const TensorView<const f16>&, const MatmulOptions&) override {}
+    void matmul_f16_slow(TensorView<f16>&, const TensorView<const f16>&, const TensorView<const f16>&, const MatmulOptions&) override {}
+    void softmax_rows_inplace(TensorView<f16>&, float) override {}
+    void attention_f16(TensorView<f16>&, const TensorView<const f16>&, const TensorView<const f16>&, const TensorView<const f16>&, float,
+                       float, MatmulMask) override {}
+    void error_stats_f16(TensorView<float>&, const TensorView<const f16>&, const TensorView<const f16>&) override {}
+    void error_stats_f32(TensorView<float>&, const TensorView<const float>&, const TensorView<const float>&) override {}
+  } other;
+  MatmulTracer over_other(other);
+  int refused = 0;
+  auto code = [&](auto call) {
+    try { call(); } catch (const AdrasteaError& e) { refused += e.code == ADR_ENOTIMPL; }
+  };
+  code([&] { over_other.rotary_f16(out, q, (const int32_t*)P, none); });
+  code([&] { over_other.append_f16(cache, batch, kv, kv, none); });
+  code([&] { over_other.attention_paged_f16(out, q, cache, batch, 0.1f); });
+  code([&] { over_other.attention_packed_f16(out, q, kv, kv, PackedBatch{}, 0.1f); });
+  CHECK(refused == 4);
 }
 
 static void gpu_tests() {
@@ -77,7 +97,8 @@ static void gpu_tests() {
   TensorView<f16> out((f16*)put(q.data(), q.size() * 2), view(heads));
   const TensorView<const f16> qv((const f16*)put(q.data(), q.size() * 2), view(heads)), kview((const f16*)put(k.data(), k.size() * 2), view(kv)),
       vview((const f16*)put(v.data(), v.size() * 2), view(kv));
-  GpuKernels kernels;
+  GpuKernels gpu;
+  MatmulTracer kernels(gpu);
   kernels.append_f16(cache, batch, kview, vview, Rotary{nullptr, 0, ADR_ROTARY_HALVES, 1.0f});
   kernels.attention_paged_f16(out, qv, cache, batch, 0.125f);
   CHECK(sync() == 0);

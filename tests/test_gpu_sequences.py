@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from adrastea_amd import (AdrasteaError, GpuKernels, MatmulMask, MatmulTracer, PackedBatch, PagedBatch, PagedCache, Rotary,
+from adrastea_amd import (AdrasteaError, attention_packed_workspace_bytes, attention_paged_workspace_bytes, GpuKernels, MatmulMask, MatmulTracer, PackedBatch, PagedBatch, PagedCache, Rotary,
                           RotaryLayout, RotaryScaling, TensorLayout, TensorView, _ffi, rotary_frequencies)
 import sequences_reference as ref
 
@@ -599,6 +599,41 @@ def test_a_captured_step_serves_later_ones():
             kk, vv = (ref.gathered(t, table[s], lengths_now[s]) for t in (k_np, v_np))
             want = ref.attention(q_np[s][:, None], kk, vv, scale)[:, 0]
             assert ref.close_enough(replayed[s].cpu().numpy(), want, np.abs(vv).max(), lengths_now[s])
+
+
+@pytest.mark.parametrize("seqs", [[(1, 3000), (1, 70)], [(60, 3000)], [(300, 1900), (1, 1700)]])
+def test_workspace_bytes(kern, seqs):
+    """What is reported is what is used: the same bits with it as through the pool; with less, or none, still right."""
+    p = Paged(seqs, 8, 2, 128, 16, seed=66)
+    batch = PagedBatch(p.batch.row_offsets, p.batch.lengths, p.batch.table, max(r for r, _ in seqs), 3000)
+    keys = [torch.from_numpy(np.concatenate([ref.gathered(x, p.table[i], n) for i, (_, n) in enumerate(seqs)], 1)).cuda()
+            for x in (p.k, p.v)]
+    packed = PackedBatch(batch.row_offsets, ints(ref.offsets(p.lengths)), batch.longest_rows, 3000)
+    paged_bytes = attention_paged_workspace_bytes(p.cache, batch, 8, p.rows)
+    packed_bytes = attention_packed_workspace_bytes(packed, 8, 2, p.rows, sum(p.lengths), 128)
+    assert paged_bytes > 0 and packed_bytes > 0
+
+    def run(k, paged):
+        p.out_t.fill_(SENTINEL)
+        if paged:
+            k.attention_paged_f16(heads_view(p.out_t), heads_view(p.q_t), p.cache, batch, 0.1)
+        else:
+            k.attention_packed_f16(heads_view(p.out_t), heads_view(p.q_t), *map(TensorView.of, keys), packed, 0.1)
+        p.check(0.1, CAUSAL)
+        return p.out_t.clone()
+    lib = _ffi.lib()
+    for paged, nbytes in ((True, paged_bytes), (False, packed_bytes)):
+        lib.adr_set_held_workspace_limit(_ffi.HELD_WORKSPACE_DEFAULT_BYTES)
+        pool = run(kern, paged)
+        lib.adr_set_held_workspace_limit(0)
+        n = p.row_offsets[-1]
+        assert torch.equal(run(GpuKernels(workspace_bytes=nbytes), paged)[:n], pool[:n])
+        for part in (nbytes // 2, nbytes // 7, 64):
+            run(GpuKernels(workspace_bytes=part), paged)
+    with pytest.raises(AdrasteaError):
+        attention_paged_workspace_bytes(p.cache, batch, 7, p.rows)     # (7 heads, 2 key heads)
+    with pytest.raises(AdrasteaError):
+        attention_packed_workspace_bytes(packed, 8, 2, -1, 5, 128)
 
 
 def test_offsets_that_decrease(shared_keys):
