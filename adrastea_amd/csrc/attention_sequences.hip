@@ -38,6 +38,20 @@ __device__ __forceinline__ Args arguments() {
   return *(const __attribute__((address_space(4))) Job*)p;
 }
 
+// What the start of a block needs, by one wait for all of it.
+template <bool PAGED>
+__device__ __forceinline__ void early(Args a) {
+  if constexpr (PAGED)
+    asm volatile("" ::"s"(a.kv_heads), "s"(a.row_offsets), "s"(a.keys_of), "s"(a.rows), "s"(a.sequences), "s"(a.group),
+                 "s"(a.per_head), "s"(a.mask), "s"(a.d), "s"(a.q), "s"(a.sq_y), "s"(a.sq_z), "s"(a.k), "s"(a.v), "s"(a.sk.y),
+                 "s"(a.sk.z), "s"(a.sv.y), "s"(a.sv.z), "s"(a.sk.p), "s"(a.sv.p), "s"(a.table), "s"(a.table_width),
+                 "s"(a.page_size), "s"(a.table_pitch), "s"(a.pages), "s"(a.page_shift));
+  else
+    asm volatile("" ::"s"(a.kv_heads), "s"(a.row_offsets), "s"(a.keys_of), "s"(a.rows), "s"(a.sequences), "s"(a.group),
+                 "s"(a.per_head), "s"(a.mask), "s"(a.d), "s"(a.q), "s"(a.sq_y), "s"(a.sq_z), "s"(a.k), "s"(a.v), "s"(a.sk.y),
+                 "s"(a.sk.z), "s"(a.sv.y), "s"(a.sv.z), "s"(a.keys));
+}
+
 // A list row's row: the quotient is at least 0.5 / group away from the next integer, far more than the product's error.
 __device__ __forceinline__ int row_of_list(Args a, int list_row) { return (int)(((double)list_row + 0.5) * a.per_head); }
 
@@ -56,9 +70,8 @@ struct Sequence {
   int key0, keys;         // first key of packed ones
 };
 
-__device__ __forceinline__ Sequence sequence_at(Args a, int s) {
+__device__ __forceinline__ Sequence sequence_at(Args a, int s, bool paged) {
   // (all four loads at once: one way to memory)
-  const bool paged = a.table != nullptr;
   const int r0 = a.row_offsets[s], r1 = a.row_offsets[s + 1], k0 = a.keys_of[s], k1 = a.keys_of[s + (paged ? 0 : 1)];
   Sequence q;
   q.index = s;
@@ -150,7 +163,7 @@ __global__ __launch_bounds__(256) void attention_any_layout_kernel(Job) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int64_t i = (int64_t)blockIdx.x * 4 + wave; i < (int64_t)a.rows * a.heads; i += (int64_t)gridDim.x * 4) {
     const int h = (int)(i / a.rows), row = (int)(i - (int64_t)h * a.rows);
-    const Sequence q = sequence_at(a, sequence_of_row(a.row_offsets, a.sequences, row, lane));
+    const Sequence q = sequence_at(a, sequence_of_row(a.row_offsets, a.sequences, row, lane), a.table != nullptr);
     if (row < q.row0 || row >= q.row0 + q.rows) continue;
     row_by_wave(a, q, row - q.row0, h, lane);
   }
@@ -215,7 +228,7 @@ constexpr int MANY = 128, MANY_KEYS = 64;
 
 // The sequences on the line, 256 at a time: lane l has sequences base + 64 e + l, read from memory once for the whole
 // division where there are no more.
-template <int ROWS, int KEYS, bool SHARED>
+template <int ROWS, int KEYS, bool PAGED, bool SHARED>
 struct Roster {
   static constexpr int EACH = 4;
   typedef int each_t __attribute__((ext_vector_type(EACH)));
@@ -237,7 +250,7 @@ struct Roster {
     for (int e = 0; e < EACH; e++) {
       row0[e] = rows[e] = key0[e] = keys[e] = 0;
       if (base + 64 * e < a.sequences && base + 64 * e + lane < a.sequences) {
-        const Sequence q = sequence_at(a, base + 64 * e + lane);
+        const Sequence q = sequence_at(a, base + 64 * e + lane, PAGED);
         row0[e] = q.row0, rows[e] = q.rows, key0[e] = q.key0, keys[e] = q.keys;
       }
     }
@@ -309,7 +322,7 @@ struct Part {
 };
 
 // Part number `index`, of at most 256 sequences (SHARED); false: there are fewer.
-template <int ROWS, int KEYS>
+template <int ROWS, int KEYS, bool PAGED>
 __device__ __forceinline__ bool part_at(Args a, int index, int lane, Part& p) {
   constexpr int EACH = 4, UNDIVIDED = 1 << 26;
   int rows[EACH], keys[EACH], row0[EACH], key0[EACH], blocks[EACH], tiles[EACH];
@@ -317,7 +330,7 @@ __device__ __forceinline__ bool part_at(Args a, int index, int lane, Part& p) {
   for (int e = 0; e < EACH; e++) {
     row0[e] = rows[e] = key0[e] = keys[e] = 0;
     if (64 * e < a.sequences && 64 * e + lane < a.sequences) {
-      const Sequence q = sequence_at(a, 64 * e + lane);
+      const Sequence q = sequence_at(a, 64 * e + lane, PAGED);
       row0[e] = q.row0, rows[e] = q.rows, key0[e] = q.key0, keys[e] = q.keys;
     }
     blocks[e] = (int)(((int64_t)rows[e] * a.group + ROWS - 1) / ROWS);
@@ -415,7 +428,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
 
   const int kv_heads = arguments().kv_heads, hk = blockIdx.x % kv_heads, wg = blockIdx.x / kv_heads;
-  Roster<ROWS, KEYS, SHARED> roster;
+  Roster<ROWS, KEYS, PAGED, SHARED> roster;
   const Line line = roster.line_of(arguments(), threadIdx.x & 63);
   if (wg >= line.parts) {
     if (SHARED && threadIdx.x == 0) arguments().seams[wg * kv_heads + hk].parts = 0;
@@ -738,7 +751,9 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
 
   // Consecutive workgroups go to different dies; where the key heads divide evenly, a die takes its share of them, so
   // that the blocks which read the same keys meet in one L2.
-  const int kv_heads = arguments().kv_heads;
+  Args a = arguments();
+  early<PAGED>(a);
+  const int kv_heads = a.kv_heads;
   int hk, index;
   if (kv_heads % 8 == 0) {
     const int each = kv_heads >> 3, seq = blockIdx.x >> 3;
@@ -748,18 +763,17 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     hk = blockIdx.x % kv_heads;
     index = blockIdx.x / kv_heads;
   }
-  Args a = arguments();
   const int tid = threadIdx.x, lane = tid & 63, group = GROUPS == 1 ? 0 : uniform(tid >> 8), w = uniform(tid >> 6 & 3);
   const int frow = lane & 31, g = lane >> 5;
   Part pt = {{}, 0, 1, 0, 0, 0};
   if constexpr (SHARED) {
-    const bool some = part_at<ROWS, KEYS>(a, index, lane, pt);
+    const bool some = part_at<ROWS, KEYS, PAGED>(a, index, lane, pt);
     // (the second launch has a workgroup to each two slots)
     if (tid == 0 && index >= pt.seams && index < a.parts / 2) a.seams[index * kv_heads + hk].parts = 0;
     if (!some) return;
     if (tid == 0 && pt.part == 0 && pt.parts > 1) a.seams[pt.seam * kv_heads + hk] = Seam{pt.parts, pt.slot, pt.b.q, pt.b.block};
   } else {
-    Roster<ROWS, KEYS, false> roster;
+    Roster<ROWS, KEYS, PAGED, false> roster;
     roster.load(a, 0, lane, 0, 0);
     if (!roster.block_at(a, 0, index, lane, pt.b)) return;
   }
