@@ -38,10 +38,16 @@ __device__ __forceinline__ Args arguments() {
   return *(const __attribute__((address_space(4))) Job*)p;
 }
 
-// What the start of a block needs, by one wait for all of it.
-template <bool PAGED>
+// What the start of a block needs, or (ALL false) the division of the work, by one wait for all of it.
+template <bool PAGED, bool ALL = true>
 __device__ __forceinline__ void early(Args a) {
-  if constexpr (PAGED)
+  if constexpr (!ALL && PAGED)
+    asm volatile("" ::"s"(a.kv_heads), "s"(a.row_offsets), "s"(a.keys_of), "s"(a.rows), "s"(a.sequences), "s"(a.group),
+                 "s"(a.parts), "s"(a.shift), "s"(a.least), "s"(a.table_width), "s"(a.page_size));
+  else if constexpr (!ALL)
+    asm volatile("" ::"s"(a.kv_heads), "s"(a.row_offsets), "s"(a.keys_of), "s"(a.rows), "s"(a.sequences), "s"(a.group),
+                 "s"(a.parts), "s"(a.shift), "s"(a.least), "s"(a.keys));
+  else if constexpr (PAGED)
     asm volatile("" ::"s"(a.kv_heads), "s"(a.row_offsets), "s"(a.keys_of), "s"(a.rows), "s"(a.sequences), "s"(a.group),
                  "s"(a.per_head), "s"(a.mask), "s"(a.d), "s"(a.q), "s"(a.sq_y), "s"(a.sq_z), "s"(a.k), "s"(a.v), "s"(a.sk.y),
                  "s"(a.sk.z), "s"(a.sv.y), "s"(a.sv.z), "s"(a.sk.p), "s"(a.sv.p), "s"(a.table), "s"(a.table_width),
@@ -427,16 +433,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
   // the accumulation registers as well and move every sum in and out of those)
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
 
-  const int kv_heads = arguments().kv_heads, hk = blockIdx.x % kv_heads, wg = blockIdx.x / kv_heads;
+  Args first = arguments();
+  early<PAGED, !SHARED>(first);
+  const int kv_heads = first.kv_heads, hk = blockIdx.x % kv_heads, wg = blockIdx.x / kv_heads;
   Roster<ROWS, KEYS, PAGED, SHARED> roster;
-  const Line line = roster.line_of(arguments(), threadIdx.x & 63);
+  const Line line = roster.line_of(first, threadIdx.x & 63);
   if (wg >= line.parts) {
     if (SHARED && threadIdx.x == 0) arguments().seams[wg * kv_heads + hk].parts = 0;
     return;
   }
   const int stretch0 = SHARED ? line.at(wg) : wg, stretch1 = SHARED ? line.at(wg + 1) : wg + 1;
   for (int place = stretch0, next_place;; place = next_place) {
-  Args a = arguments();
+  Args a = SHARED ? arguments() : first;
   const int tid = thread_index(), lane = tid & 63, w = uniform(tid >> 6);
   const int frow = lane & 15, g = lane >> 4;
   Block b;
@@ -444,6 +452,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
     if (SHARED && place == stretch0 && tid == 0) a.seams[wg * kv_heads + hk].parts = 0;
     return;
   }
+  if constexpr (SHARED)  // (by one wait, as above)
+    asm volatile("" ::"s"(a.seams), "s"(a.group), "s"(a.per_head), "s"(a.mask), "s"(a.d), "s"(a.q), "s"(a.sq_y), "s"(a.sq_z),
+                 "s"(a.k), "s"(a.v), "s"(a.sk.y), "s"(a.sk.z), "s"(a.sv.y), "s"(a.sv.z));
   const Sequence q = b.q;
   const int block = b.block, pieces = min(stretch1 - place, b.pieces - b.offset);
   const bool whole = pieces == b.pieces;
