@@ -417,8 +417,8 @@ __device__ __forceinline__ u32x4_t descriptor(uint64_t p, int bytes) {
 // no matrix product, and its values are fp16 anyway.)
 //
 // Bound by memory: 16 rows of every key read once leave the matrix cores 5 % busy.  64 sequences of 3 to 4000 keys (32 / 8
-// heads of 128, 504 MB) 88.5 us = 5.7 TB/s, eight of 50000 to 110000 (40 / 8, 2.36 GB) 366 us = 6.4 TB/s, where a plain read
-// reaches 7.0 to 7.3; one of 777 keys (32 / 32) 9.7 us, of which two launches are 8.8 on the host.
+// heads of 128, 504 MB) 88.2 us = 5.7 TB/s, eight of 50000 to 110000 (40 / 8, 2.36 GB) 365 us = 6.4 TB/s, where a plain read
+// reaches 7.0 to 7.3; one of 777 keys (32 / 32) 9.5 us, of which two launches are 8.8 on the host.
 template <int HD, bool PAGED, int WAVES, bool SHARED>
 __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) {
   constexpr int CPR = HD / 8, KEYS = 32, ROWS = 16;
@@ -745,8 +745,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
 // Bound by power, and by issue as in attention_fwd_kernel: one prompt of 16384 rows (32 / 8 heads of 128) 2001 us = 1099
 // TFLOP/s with the matrix cores busy 69 % of cycles at 1.6 GHz, where a product of 8192^3 reaches 1408.  Short blocks are
 // bound by their beginnings and ends: us of a block among others, 2.0 from the end of one to the start of the next in its place,
-// 1.8 to find its sequence, 1.9 for addresses, 1.8 until the first keys are there, 1.9 a tile, 2.4 for the results (nine prompts
-// of 100 to 3996 rows, 25 tiles a block in the mean, 446 us = 934 TFLOP/s; the tiles of wavefronts whose rows end early, and of rows
+// 1.8 to find its sequence, 1.9 for addresses (before arguments came by one wait), 1.8 until the first keys are there, 1.9 a
+// tile, 2.4 for the results (nine prompts of 100 to 3996 rows, 25 tiles a block in the mean, 436 us = 957 TFLOP/s; the tiles of wavefronts whose rows end early, and of rows
 // that the mask hides, are in these figures as work that is not counted).
 template <int HD, bool PAGED, bool SHARED, int GROUPS>
 __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {

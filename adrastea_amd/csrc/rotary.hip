@@ -43,7 +43,10 @@ __device__ __forceinline__ Args arguments() {
 // Bound by memory, and before that by what it takes to find an item: so a thread has the same item of all the heads
 // that it goes through, and from head to head only the addresses change.  Items asked for ahead cost registers that
 // are wavefronts (us with four ahead, two, none: 4099 rows of 40 heads of 128, pairs, half of the head 21.4, 19.7, 17.4), and
-// nobody waits for the stores at the end (17.3 -> 16.4).  CACHE false: queries only.
+// nobody waits for the stores at the end (17.3 -> 16.4).  15.3 to 17.0 us = 4.9 to 5.5 TB/s; four prompts of 700 to 2500 rows into
+// the cache (32 / 8 heads of 128) 39.3 us = 4.4 TB/s.  Nontemporal stores would take 15.1 and 31.6, but what is written here is
+// what the attention behind it reads: both together four prompts of 2000 rows 191.2 us, with them 195.4, eight heads of their own
+// 80.0 and 84.8.  CACHE false: queries only.
 template <bool VEC, bool CACHE>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryJob) {
   Args a = arguments();
