@@ -718,8 +718,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
   }
   if (!SHARED || next_place >= stretch1) break;
   __syncthreads();  // (the next block's transfers go where the results are read)
-  Args n = arguments();
-  roster.load(n, n.shift, thread_index() & 63, 0, 0);  // (not kept in registers meanwhile)
   }
 }
 
