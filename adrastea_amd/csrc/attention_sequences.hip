@@ -743,9 +743,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
 // Bound by power, and by issue as in attention_fwd_kernel: one prompt of 16384 rows (32 / 8 heads of 128) 2001 us = 1099
 // TFLOP/s with the matrix cores busy 69 % of cycles at 1.6 GHz, where a product of 8192^3 reaches 1408.  Short blocks are
 // bound by their beginnings and ends: us of a block among others, 2.0 from the end of one to the start of the next in its place,
-// 1.8 to find its sequence, 1.9 for addresses (before arguments came by one wait), 1.8 until the first keys are there, 1.9 a
-// tile, 2.4 for the results (nine prompts of 100 to 3996 rows, 25 tiles a block in the mean, 436 us = 957 TFLOP/s; the tiles of wavefronts whose rows end early, and of rows
-// that the mask hides, are in these figures as work that is not counted).
+// 1.4 to find its sequence, 1.7 for addresses, 1.8 until the first keys are there, 1.9 a tile, 2.4 for the results.  Nine prompts
+// of 100 to 3996 rows, 25 tiles a block in the mean, 436 us = 957 TFLOP/s (what wavefronts whose rows end early, and rows that
+// the mask hides, compute of a tile is in the time and not in the operations).
 template <int HD, bool PAGED, bool SHARED, int GROUPS>
 __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
   constexpr int CPR = HD / 8, KEYS = 64, ROWS = 128;
@@ -1408,7 +1408,8 @@ SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
   if (!chunks(a)) return p;
   const int longest_rows = a.longest_rows > 0 ? std::min(a.longest_rows, a.rows) : a.rows;
   p.kind = (int64_t)longest_rows * a.group <= FEW ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES;
-  const int forced = knob(KNOB_SEQUENCES);  // (1: any layout; 2 ... 4: few rows; 5 ... 8: many; adr_debug_knob says which)
+  // (1: any layout; 2 ... 4: few rows; 5 ... 8: many; adr_debug_knob says which.  Other values force nothing.)
+  const int forced = knob(KNOB_SEQUENCES) >= 1 && knob(KNOB_SEQUENCES) <= 8 ? knob(KNOB_SEQUENCES) : 0;
   if (forced == 1) return SequencesPlan{SequencesPlan::ANY_LAYOUT, 0, 0, 0, 0, 0};
   if (forced) p.kind = forced <= 4 ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES;
   const bool few = p.kind == SequencesPlan::FEW_ROWS;

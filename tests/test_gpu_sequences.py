@@ -292,6 +292,18 @@ def test_hints_never_change_what_is_computed(shared_keys):
         p.check(scale, CAUSAL)
 
 
+@pytest.mark.parametrize("value", [-1, 9, 1 << 30])
+def test_unknown_forms_force_nothing(kern, value):
+    lib = _ffi.lib()
+    p = Paged([(1, 700), (70, 300)], 8, 2, 128, 16, seed=13)
+    try:
+        assert lib.adr_debug_knob(2, value) == 0
+        kern.attention_paged_f16(heads_view(p.out_t), heads_view(p.q_t), p.cache, p.batch, 0.1)
+    finally:
+        lib.adr_debug_knob(2, 0)
+    p.check(0.1, CAUSAL)
+
+
 def test_many_sequences(shared_keys):
     rng = np.random.default_rng(10)
     seqs = [(int(rng.integers(0, 3)), int(rng.integers(0, 60))) for _ in range(700)]
