@@ -89,13 +89,13 @@ __device__ __forceinline__ void dma_buffer_once(uint32_t lds, const uint32_t (&v
   static_assert(N == 2 || N == 4, "16 rows of 64 or 128 values");
   if constexpr (N == 4)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %5, 0 offen nt lds\n\t"
-                 "buffer_load_dwordx4 %2, %5, 0 offen offset:1024 nt lds\n\t"
-                 "buffer_load_dwordx4 %3, %5, 0 offen offset:2048 nt lds\n\t"
-                 "buffer_load_dwordx4 %4, %5, 0 offen offset:3072 nt lds"
+                 "buffer_load_dwordx4 %2, %5, 0 offen offset:0x400 nt lds\n\t"
+                 "buffer_load_dwordx4 %3, %5, 0 offen offset:0x800 nt lds\n\t"
+                 "buffer_load_dwordx4 %4, %5, 0 offen offset:0xc00 nt lds"
                  :: "s"(lds), "v"(voff[0]), "v"(voff[1]), "v"(voff[2]), "v"(voff[3]), "s"(desc) : "memory");
   else
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %3, 0 offen nt lds\n\t"
-                 "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 nt lds"
+                 "buffer_load_dwordx4 %2, %3, 0 offen offset:0x400 nt lds"
                  :: "s"(lds), "v"(voff[0]), "v"(voff[1]), "s"(desc) : "memory");
 }
 __device__ __forceinline__ void dma_global(uint32_t lds, const void* p) {
