@@ -367,7 +367,8 @@ const char* adr_strerror(int code) {
     case ADR_EUNSUPPORTED_LAYOUT:
       return "fused attention covers head dimension 64 or 128, unit x strides, y/z strides that "
              "are multiples of 8 and 16-byte aligned pointers (over pages and packed prompts: head "
-             "dimension 1 to 256, any strides), and a positive scale and temperature";
+             "dimension 1 to 256, any strides), and a positive scale and temperature (there with a "
+             "quotient of 2^-126 to 2^58)";
     default: return code > 0 ? hipGetErrorString((hipError_t)code) : "unknown error";
   }
 }
@@ -864,9 +865,16 @@ int validate_rotary(const adr_rotary& r, int32_t d) {
   return ADR_OK;
 }
 
+// The factor of the scores, a normal number in 32 bits: hidden scores of -inf stay -inf where it is multiplied with them, and
+// no score of finite operands comes near the kernels' mark for none (NO_SCORE).
+bool factor_fits(float scale, float temp) {
+  const double f = (double)scale / (double)temp;
+  return scale > 0.0f && temp > 0.0f && f >= 0x1p-126 && f <= 0x1p58;
+}
+
 int attention_of_rows(hipStream_t stream, const SequencesArgs& a, float scale, float temp, bool held, void* workspace,
                       int64_t workspace_bytes) {
-  if (a.d > 256 || !(scale > 0.0f) || !(temp > 0.0f) || !(scale / temp < 1.0e30f)) return ADR_EUNSUPPORTED_LAYOUT;
+  if (a.d > 256 || !factor_fits(scale, temp)) return ADR_EUNSUPPORTED_LAYOUT;
   const DeviceInfo dev = device_info();
   if (dev.status) return dev.status;
   auto launch = [&](const SequencesPlan& plan, void* scratch) {

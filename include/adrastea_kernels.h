@@ -477,7 +477,7 @@ int adr_append_f16(adr_stream_t stream, adr_paged_cache cache, adr_paged_batch b
  * hold (infinities and NaN included).  A key on a page outside 0 .. pages - 1 counts as NaN for the rows
  * that see it.  Scores, softmax and sums in fp32; probabilities are rounded to fp16 for the matrix cores.
  * `output` overlaps none of the others.
- * d 1 .. 256, scale > 0, temp > 0 (ADR_EUNSUPPORTED_LAYOUT beyond), heads a multiple of kv_heads.  The fast
+ * d 1 .. 256, scale > 0, temp > 0, scale / temp 2^-126 .. 2^58 (ADR_EUNSUPPORTED_LAYOUT beyond), heads a multiple of kv_heads.  The fast
  * kernels take d a multiple of 8 up to 128, x strides 1, the others multiples of 8 and not negative, slots at
  * least d apart and less than 2^24, 16-byte aligned pointers, pages of 16, 32, 64 ... slots; everything else runs on
  * a kernel of one wavefront per row.

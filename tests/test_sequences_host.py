@@ -2,6 +2,7 @@
 import math
 
 import pytest
+import torch
 
 from adrastea_amd import RotaryScaling, _ffi, rotary_frequencies
 from sequences_reference import yarn_reference
@@ -140,3 +141,18 @@ def test_scalings_that_make_no_sense_are_refused():
                 lambda: rotary_frequencies(8, scaling=RotaryScaling("cubic", (1.0,)))):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("scale,temp", [(1.0, math.inf), (1e-20, 1e20), (2.0 ** -126, 1.5), (2.0 ** -140, 1.0), (2.0 ** 59, 1.0), (1e29, 1.0),
+                                        (2.0 ** 30, 2.0 ** -30), (1e38, 1e-38), (math.inf, math.inf)])
+def test_a_factor_of_the_scores_out_of_range(scale, temp):
+    """Where scale / temp is no normal number in 32 bits, hidden scores would not stay -inf; where it is huge, finite ones would
+    pass the kernels' mark for none."""
+    assert paged(scale=scale, temp=temp) == LAYOUT and packed(scale=scale, temp=temp) == LAYOUT
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are not real")
+@pytest.mark.parametrize("scale,temp", [(2.0 ** -126, 1.0), (2.0 ** 58, 1.0), (1.0, 1e30), (2.0 ** -149, 2.0 ** -60)])
+def test_the_ends_of_its_range(scale, temp):
+    """Accepted as far as the arguments go: without a GPU, what is refused is the device."""
+    assert paged(scale=scale, temp=temp) not in (0, LAYOUT) and packed(scale=scale, temp=temp) not in (0, LAYOUT)
