@@ -14,7 +14,15 @@
 namespace adr {
 namespace {
 
-constexpr float NO_SCORE = -1.0e30f;  // below any score of finite operands; exp2(-inf - NO_SCORE) is 0, not NaN
+// Below any score of finite operands (256 * 65504^2 < 2^41, times at most 2^58 log2(e)); exp2(-inf - NO_SCORE) is 0, not NaN.
+constexpr float NO_SCORE = -1.0e30f;
+
+// A row's probabilities are 2^(s c - R), where s c - R is one fma, exact but for its last step, and R the largest s c that
+// was seen.  That is itself rounded: at 2^31 by up to 2^7, so that the largest probability could be 2^128 or 2^-128.  A step above
+// what was found, R is no smaller than the largest s c at least, and no probability or sum is infinite that should not be;
+// rows whose R is beyond FAR_SCORE in the end, where it can be larger by more than 2, are computed again by row_by_wave.
+constexpr float FAR_SCORE = 0x1p24f;
+__device__ __forceinline__ float above(float top) { return fmaf(fabsf(top), 0x1p-23f, top); }
 
 // What a kernel is given.  Share of the work: see below.
 struct Job : SequencesArgs {
@@ -110,8 +118,8 @@ __device__ __forceinline__ bool key_at(Args a, const Sequence& q, int x, int64_t
 }
 
 // One row of one query head by one wavefront, at any strides: 64 keys at a time, a lane to a key for the scores
-// and a lane to every 64th column for the sums.  Only keys that the row sees are read.  Probabilities stay in 32 bits.
-// (Columns col0 ... col1 - 1 are stored.)
+// and a lane to every 64th column for the sums.  Only keys that the row sees are read.  Probabilities stay in 32 bits, and
+// scores unscaled until their maximum is subtracted: right for scores of any size.  (Columns col0 ... col1 - 1 are stored.)
 constexpr int GENERAL_MAX_D = 256;
 __device__ __forceinline__ void row_by_wave(Args a, const Sequence& q, int j, int h, int lane, int col0 = 0, int col1 = GENERAL_MAX_D) {
   const int64_t row = (int64_t)q.row0 + j;
@@ -130,13 +138,13 @@ __device__ __forceinline__ void row_by_wave(Args a, const Sequence& q, int j, in
       s = 0.0f;
       if (good)
         for (int i = 0; i < a.d; i++) s = fmaf((float)Q[i * (int64_t)a.sq_x], (float)K[ko + i * a.sk.x], s);
-      s = good ? s * a.c : NAN;
+      if (!good) s = NAN;
     }
     float top = s;
     for (int i = 32; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));  // (not the NaNs)
-    const float m_new = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - m_new);
+    const float m_new = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f((m - m_new) * a.c);
     m = m_new;
-    const float p = __builtin_amdgcn_exp2f(s - m);
+    const float p = __builtin_amdgcn_exp2f((s - m) * a.c);
     l = l * alpha + p;
 #pragma unroll
     for (int c = 0; c < GENERAL_MAX_D / 64; c++) o[c] *= alpha;
@@ -620,7 +628,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
     swap_rows(x, y);
     // The exponents' reference follows the maximum lazily: it moves when some row has outgrown it by more than 2^8
     // (probabilities up to 256 are as exact in fp16 as those below 1), and only then are the sums rescaled.
-    const float top = fmaxf(x, y) * a.c;
+    const float top = above(fmaxf(x, y) * a.c);
     if (__builtin_amdgcn_ballot_w64(top > m_run + 8.0f) != 0) {
       const float m_new = fmaxf(m_run, top), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
@@ -698,7 +706,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
         v[j] = (half_t)(sum[j] * inv);
       }
       if (!finite) atomicOr(bad_rows, 1 << r);
-      if (col < z.d)
+      if (col < z.d && fabsf(m_all) <= FAR_SCORE)
         *(half4_t*)(z.out + (int64_t)h * z.so_z + (int64_t)(q.row0 + token) * z.so_y + col) = v;
     } else {
       const int64_t prow = ((int64_t)(2 * wg + (place != stretch0)) * z.kv_heads + hk) * ROWS + r;
@@ -706,12 +714,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
       if (col == 0) z.part_ml[prow] = make_float2(m_all, l);
     }
   }
-  // A value that is no number times the zero of a key that the row does not see is no zero: such rows are computed
-  // again from the keys that they see.
-  if (whole && q.rows > 1 && z.mask == ADR_MASK_CAUSAL) {
-    __syncthreads();
+  if (whole) {
+    float m_all = NO_SCORE;
+#pragma unroll
+    for (int x = 0; x < WAVES; x++) m_all = fmaxf(m_all, xml[x * 16 + frow].x);
+    int again = (int)__ballot(fabsf(m_all) > FAR_SCORE);  // (not stored above)
+    // A value that is no number times the zero of a key that the row does not see is no zero: such rows are computed
+    // again from the keys that they see.
+    if (q.rows > 1 && z.mask == ADR_MASK_CAUSAL) {
+      __syncthreads();
+      again |= *bad_rows;
+    }
     for (int r = w; r < rows; r += WAVES)
-      if (*bad_rows >> r & 1) {
+      if (again >> r & 1) {
         const int lr = block * ROWS + r;
         row_by_wave(arguments(), q, lr / z.group, hk * z.group + lr % z.group, lane);
       }
@@ -1109,7 +1124,7 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
               mx2[e & 1] = fmaxf(fmaxf(mx2[e & 1], nxt[x >> 4][x & 15]), nxt[x >> 4][(x & 15) + 1]);
             }
           }
-          if (first == 32) mx = pair_max(fmaxf(mx2[0], mx2[1])) * a.c;  // in log2 units (c > 0)
+          if (first == 32) mx = above(pair_max(fmaxf(mx2[0], mx2[1])) * a.c);  // in log2 units (c > 0)
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -1271,8 +1286,9 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     }
     // A value that is no number times the zero of a key that the row does not see is no zero: such rows are computed
     // again from the keys that they see, a group's columns of them.
-    const uint64_t lanes = __ballot(!(zero[0] + zero[1] == 0.0f));
-    if (lanes && q.rows > 1 && z.mask == ADR_MASK_CAUSAL) {
+    const uint64_t lanes = __ballot(fabsf(m_run) > FAR_SCORE ||
+                                    (!(zero[0] + zero[1] == 0.0f) && q.rows > 1 && z.mask == ADR_MASK_CAUSAL));
+    if (lanes) {
       const uint32_t bad = (uint32_t)lanes | (uint32_t)(lanes >> 32);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (behind the stores above)
       for (int r = 0; r < wave_rows; r++)
@@ -1370,17 +1386,16 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Job) {
       finite = finite && fabsf(acc[j]) < INFINITY;
       out[j] = (half_t)acc[j];
     }
-    if (!finite) atomicOr(&bad_rows, 1 << (r - r0));
+    const bool far = fabsf(m) > FAR_SCORE;
+    if (far || (!finite && b.q.rows > 1 && a.mask == ADR_MASK_CAUSAL)) atomicOr(&bad_rows, 1 << (r - r0));  // (as above)
     if (col < a.d) *(half4_t*)(a.out + (int64_t)h * a.so_z + (int64_t)(b.q.row0 + token) * a.so_y + col) = out;
   }
-  if (b.q.rows > 1 && a.mask == ADR_MASK_CAUSAL) {  // (as above)
-    __syncthreads();
-    for (int x = tid >> 6; x < AT_ONCE; x += 4)
-      if (bad_rows >> x & 1) {
-        const int lr = b.block * ROWS + r0 + x;
-        row_by_wave(arguments(), b.q, lr / a.group, hk * a.group + lr % a.group, lane);
-      }
-  }
+  __syncthreads();
+  for (int x = tid >> 6; x < AT_ONCE; x += 4)
+    if (bad_rows >> x & 1) {
+      const int lr = b.block * ROWS + r0 + x;
+      row_by_wave(arguments(), b.q, lr / a.group, hk * a.group + lr % a.group, lane);
+    }
 }
 
 }  // namespace

@@ -1,0 +1,46 @@
+"""Attention over several sequences where numbers are large, small or not finite, through every form of the kernels, against
+what the definition gives in 64 bits."""
+import numpy as np
+import pytest
+
+from test_gpu_sequences import CAUSAL, NONE, Packed, dev, heads_view, shared_keys  # noqa: F401 (fixtures)
+
+pytestmark = pytest.mark.gpu
+
+
+def packed_call(k, p, scale, mask=CAUSAL, temp=1.0):
+    p.q_t, p.k_t, p.v_t = dev(p.q), dev(p.k), dev(p.v)
+    k.attention_packed_f16(heads_view(p.out_t), heads_view(p.q_t), heads_view(p.k_t), heads_view(p.v_t), p.batch, scale, temp, mask)
+    return p.out_t.cpu().numpy()[:p.row_offsets[-1]]
+
+
+@pytest.mark.parametrize("mask", [CAUSAL, NONE], ids=["causal", "full"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kind", ["high", "low", "rising"])
+def test_scores_of_any_size(shared_keys, kind, d, mask):
+    """Scores of 2^29 to 2^32 in log2 units, where a step of 32 bits is 2^6 to 2^9: keys differ by 2^20 d / 64 and more, so that
+    each row's result is the value of its largest key.  (Scores are exact: 2^14 times d integers of 11 bits.)  `rising`: the
+    first keys far below zero, the others near it."""
+    p = Packed([(1, 700), (40, 300), (1, 3), (200, 330), (2, 75)], 4, 2, d, seed=d)
+    rng = np.random.default_rng(90)
+    p.q[:p.row_offsets[-1]] = 2.0 ** 14
+    height = np.empty((p.keys, p.kv))
+    for i, (_, n) in enumerate(p.seqs):
+        for h in range(p.kv):
+            some = rng.permutation(np.arange(700, 700 + n))
+            height[p.key_offsets[i]:p.key_offsets[i + 1], h] = some
+            if kind == "low":
+                height[p.key_offsets[i]:p.key_offsets[i + 1], h] *= -1
+            elif kind == "rising" and n > 100:
+                height[p.key_offsets[i]:p.key_offsets[i + 1], h] = np.sort(some) - (700 + n - 3)
+    height[-1] = np.nan
+    p.k[:] = height[:, :, None]
+    got = packed_call(shared_keys, p, 1.0, mask)
+    for i, (r, n) in enumerate(p.seqs):
+        for j in range(r):
+            end = j + n - r + 1 if mask == CAUSAL else n
+            best = p.key_offsets[i] + height[p.key_offsets[i]:p.key_offsets[i] + end].argmax(0)   # of each key head
+            want = p.v[best, np.arange(p.kv)].repeat(2, 0).astype(np.float64)
+            # (one weight, rounded to fp16 against its unrounded self, and the result's rounding: half a step each, with
+            # their product and the 32-bit quotient's 2^-22)
+            assert (np.abs(got[p.row_offsets[i] + j] - want) <= np.abs(want) * (2.0 ** -10 + 2.0 ** -20) + 2.0 ** -24).all(), (i, j)
