@@ -17,10 +17,16 @@ namespace {
 // Below any score of finite operands (256 * 65504^2 < 2^41, times at most 2^58 log2(e)); exp2(-inf - NO_SCORE) is 0, not NaN.
 constexpr float NO_SCORE = -1.0e30f;
 
-// A row's probabilities are 2^(s c - R), where s c - R is one fma, exact but for its last step, and R the largest s c that
-// was seen.  That is itself rounded: at 2^31 by up to 2^7, so that the largest probability could be 2^128 or 2^-128.  A step above
-// what was found, R is no smaller than the largest s c at least, and no probability or sum is infinite that should not be;
-// rows whose R is beyond FAR_SCORE in the end, where it can be larger by more than 2, are computed again by row_by_wave.
+// A row's probabilities are 2^(s c - R), rounded to fp16 for the second product.  R follows the largest s c that was seen: 7 below it
+// where it moves, and it moves, with the sums rescaled, when that has grown to more than 15 above, which after the first tiles is
+// rare.  So the largest probability is 2^7 to 2^15 (65504 is fp16's largest number), and one of 2^-14 is still as exact
+// as 1 is; below, the error of 2^-25 is 2^-32 of the largest, and keys that weigh as little are lost altogether.  (With R up
+// to 8 below, each of 6000 keys that weigh 2^-25.5 was lost: 2^-13 of the result.)
+constexpr float BELOW = 7.0f, GROWN = 15.0f;
+// s c - R is one fma, exact but for its last step, but the largest s c is itself rounded: at 2^31 by up to 2^7, so that the
+// largest probability could be 2^128 or 2^-128.  A step above what was found, it is no smaller than it should be at least, and no
+// probability or sum is infinite that should not be; rows whose R is beyond FAR_SCORE in the end, where it can be larger by
+// more than 2, are computed again by row_by_wave.
 constexpr float FAR_SCORE = 0x1p24f;
 __device__ __forceinline__ float above(float top) { return fmaf(fabsf(top), 0x1p-23f, top); }
 
@@ -626,11 +632,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
     swap_halves(x, y);
     x = fmaxf(x, y), y = x;
     swap_rows(x, y);
-    // The exponents' reference follows the maximum lazily: it moves when some row has outgrown it by more than 2^8
-    // (probabilities up to 256 are as exact in fp16 as those below 1), and only then are the sums rescaled.
     const float top = above(fmaxf(x, y) * a.c);
-    if (__builtin_amdgcn_ballot_w64(top > m_run + 8.0f) != 0) {
-      const float m_new = fmaxf(m_run, top), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+    if (__builtin_amdgcn_ballot_w64(top > m_run + GROWN) != 0) {
+      const float m_new = fmaxf(m_run, top - BELOW), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
       l_run *= alpha;
 #pragma unroll
@@ -1130,11 +1134,8 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
       }
     }
     if constexpr (MAX) {
-      // The exponent reference m_run follows the row maximum lazily: it moves only when some row
-      // of the wavefront outgrew it by more than 2^8 (probabilities up to 256 are as exact in fp16
-      // as those below 1), which after the first tiles is rare; the accumulator is rescaled only then.
-      if (__builtin_amdgcn_ballot_w64(mx > m_run + 8.0f) != 0) {
-        const float m_new = fmaxf(m_run, mx);
+      if (__builtin_amdgcn_ballot_w64(mx > m_run + GROWN) != 0) {
+        const float m_new = fmaxf(m_run, mx - BELOW);
         const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
         m_run = m_new;
         l_run *= alpha;

@@ -44,3 +44,21 @@ def test_scores_of_any_size(shared_keys, kind, d, mask):
             # (one weight, rounded to fp16 against its unrounded self, and the result's rounding: half a step each, with
             # their product and the 32-bit quotient's 2^-22)
             assert (np.abs(got[p.row_offsets[i] + j] - want) <= np.abs(want) * (2.0 ** -10 + 2.0 ** -20) + 2.0 ** -24).all(), (i, j)
+
+
+@pytest.mark.parametrize("rows,keys", [(1, 6000), (70, 6000)])
+@pytest.mark.parametrize("depth", [18.0, 25.5, 30.0])
+def test_many_keys_of_little_weight(shared_keys, rows, keys, depth):
+    """One key that outweighs each of the others by 2^depth, and whose value is zero: what is left is the others'."""
+    p = Packed([(rows, keys)], 2, 1, 64, seed=7)
+    p.q[:rows], p.k[:keys] = 0.0, 0.0
+    p.q[:rows, :, 0], p.k[1:keys, :, 0] = 1.0, -1.0
+    p.v[0], p.v[1:keys] = 0.0, 1.0
+    got = packed_call(shared_keys, p, depth * np.log(2.0)).astype(np.float64)
+    others = np.arange(keys - rows, keys, dtype=np.float64) * 2.0 ** -depth     # keys behind the first that each row sees
+    want = others / (1.0 + others)
+    # Weights below fp16's normal numbers are off by half of their step, 2^-25, where the largest is at least 2^7: 2^-32 of it
+    # for each key; above, 2^-11 of each.  32-bit sums of at most 6000 terms: 6000 2^-24 of themselves.  The exponent (5 bits, 32-bit
+    # scale): 2^-18.  The result's rounding.
+    bound = others * (2.0 ** -11 + 6000 * 2.0 ** -23 + 2.0 ** -18) + np.arange(keys - rows, keys) * 2.0 ** -32 + want * 2.0 ** -11 + 2.0 ** -25
+    assert (np.abs(got - want[:, None, None]) <= bound[:, None, None]).all()
