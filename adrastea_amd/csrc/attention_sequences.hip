@@ -30,6 +30,31 @@ constexpr float BELOW = 7.0f, GROWN = 15.0f;
 constexpr float FAR_SCORE = 0x1p24f;
 __device__ __forceinline__ float above(float top) { return fmaf(fabsf(top), 0x1p-23f, top); }
 
+// A weighted mean of values, rounded to fp16.  Its weights are off by up to 2^-11 each (fp16 in the second product, 32 bits in their
+// sum), so that a mean of values near the largest number of fp16 can lie as far beyond it, and would be rounded to
+// infinity: it is that number.
+constexpr float LARGEST = 65504.0f;
+__device__ __forceinline__ half_t mean_of(float v) {
+  return (half_t)(fabsf(v) < LARGEST * 1.01f ? __builtin_amdgcn_fmed3f(v, -LARGEST, LARGEST) : v);
+}
+// Four of them; false: not all are finite.  (One that is rounded to infinity is rare, and looked at again.)
+__device__ __forceinline__ bool round_means(half4_t& h, const float4_t& v, float factor) {
+  bool finite = true;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    h[j] = (half_t)(v[j] * factor);
+    finite = finite && fabsf((float)h[j]) < INFINITY;
+  }
+  if (finite) return true;
+  finite = true;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    h[j] = mean_of(v[j] * factor);
+    finite = finite && fabsf((float)h[j]) < INFINITY;
+  }
+  return finite;
+}
+
 // What a kernel is given.  Share of the work: see below.
 struct Job : SequencesArgs {
   int page_shift;   // log2 of the slots of a page (16 at least: 16 keys from a multiple of 16 on lie on one page)
@@ -174,7 +199,7 @@ __device__ __forceinline__ void row_by_wave(Args a, const Sequence& q, int j, in
 #pragma unroll
   for (int c = 0; c < GENERAL_MAX_D / 64; c++)
     if (c * 64 + lane < a.d && c * 64 + lane >= col0 && c * 64 + lane < col1)
-      O[(c * 64 + lane) * (int64_t)a.so_x] = (half_t)(o[c] * inv);
+      O[(c * 64 + lane) * (int64_t)a.so_x] = mean_of(o[c] * inv);
 }
 
 // Any layout: a wavefront per row and query head.
@@ -703,13 +728,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
       const int lr = block * ROWS + r, token = row_of_list(z, lr), h = hk * z.group + lr - token * z.group;
       half4_t v;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      bool finite = true;
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        finite = finite && fabsf(sum[j] * inv) < INFINITY;
-        v[j] = (half_t)(sum[j] * inv);
-      }
-      if (!finite) atomicOr(bad_rows, 1 << r);
+      if (!round_means(v, sum, inv)) atomicOr(bad_rows, 1 << r);
       if (col < z.d && fabsf(m_all) <= FAR_SCORE)
         *(half4_t*)(z.out + (int64_t)h * z.so_z + (int64_t)(q.row0 + token) * z.so_y + col) = v;
     } else {
@@ -1256,7 +1275,7 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     static_assert(EXCHANGE + 4 * 32 * PITCH <= 4 * TILE, "the output's slots fit the LDS");
     unsigned char* const slot = sm + EXCHANGE + w * (32 * PITCH);
     const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
-    float zero[2] = {0.0f, 0.0f};  // (NaN behind a value that is not finite)
+    float zero[2] = {0.0f, 0.0f};  // (NaN behind a result that is not finite)
 #pragma unroll
     for (int d = 0; d < MINE; d++)
 #pragma unroll
@@ -1264,12 +1283,24 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
         half4_t h;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          const float v = res[d][4 * i + j] * inv;
-          zero[j & 1] = fmaf(v, 0.0f, zero[j & 1]);
-          h[j] = (half_t)v;
+          h[j] = (half_t)(res[d][4 * i + j] * inv);
+          zero[j & 1] = fmaf((float)h[j], 0.0f, zero[j & 1]);
         }
         *(half4_t*)(slot + frow * PITCH + (32 * d + 8 * i + 4 * g) * 2) = h;
       }
+    bool finite = zero[0] + zero[1] == 0.0f;
+    if (__ballot(!finite)) {
+      finite = true;
+#pragma unroll
+      for (int d = 0; d < MINE; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          half4_t h;
+          const float4_t v = {res[d][4 * i], res[d][4 * i + 1], res[d][4 * i + 2], res[d][4 * i + 3]};
+          finite &= round_means(h, v, inv);
+          *(half4_t*)(slot + frow * PITCH + (32 * d + 8 * i + 4 * g) * 2) = h;
+        }
+    }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the slot is the wavefront's own)
     constexpr int RPI = 64 / CHUNKS;  // rows of a store instruction
     const int r0 = lane / CHUNKS, col = lane % CHUNKS * 8;
@@ -1288,7 +1319,7 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     // A value that is no number times the zero of a key that the row does not see is no zero: such rows are computed
     // again from the keys that they see, a group's columns of them.
     const uint64_t lanes = __ballot(fabsf(m_run) > FAR_SCORE ||
-                                    (!(zero[0] + zero[1] == 0.0f) && q.rows > 1 && z.mask == ADR_MASK_CAUSAL));
+                                    (!finite && q.rows > 1 && z.mask == ADR_MASK_CAUSAL));
     if (lanes) {
       const uint32_t bad = (uint32_t)lanes | (uint32_t)(lanes >> 32);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (behind the stores above)
@@ -1378,15 +1409,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Job) {
       l = l * f0 + ml.y * f1;
       acc = acc * f0 + sums[s * items + item] * f1;
     }
-    acc *= l == 0.0f ? 0.0f : 1.0f / l;
     const int lr = b.block * ROWS + r, token = row_of_list(a, lr), h = hk * a.group + lr - token * a.group;
     half4_t out;
-    bool finite = true;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      finite = finite && fabsf(acc[j]) < INFINITY;
-      out[j] = (half_t)acc[j];
-    }
+    const bool finite = round_means(out, acc, l == 0.0f ? 0.0f : 1.0f / l);
     const bool far = fabsf(m) > FAR_SCORE;
     if (far || (!finite && b.q.rows > 1 && a.mask == ADR_MASK_CAUSAL)) atomicOr(&bad_rows, 1 << (r - r0));  // (as above)
     if (col < a.d) *(half4_t*)(a.out + (int64_t)h * a.so_z + (int64_t)(b.q.row0 + token) * a.so_y + col) = out;

@@ -62,3 +62,19 @@ def test_many_keys_of_little_weight(shared_keys, rows, keys, depth):
     # scale): 2^-18.  The result's rounding.
     bound = others * (2.0 ** -11 + 6000 * 2.0 ** -23 + 2.0 ** -18) + np.arange(keys - rows, keys) * 2.0 ** -32 + want * 2.0 ** -11 + 2.0 ** -25
     assert (np.abs(got - want[:, None, None]) <= bound[:, None, None]).all()
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("rows", [1, 70])
+def test_the_largest_values_stay_finite(shared_keys, sign, rows):
+    """Values that are all the largest number of fp16: every weighted mean of them is that number.  One weight, in a later
+    tile than the row's first key, is a little more than half a step above a number of fp16, and the only large one."""
+    keys = 300
+    p = Packed([(rows, keys), (60, 62), (140, 300)], 2, 1, 64, seed=8)
+    p.v[:] = sign * 65504.0
+    p.q[:rows], p.k[:keys] = 0.0, 0.0
+    p.q[:rows, :, 0], p.k[1:keys, :, 0], p.k[128, :, 0] = 1.0, -100.0, 1.0
+    for mask in (CAUSAL, NONE):
+        got = packed_call(shared_keys, p, (7.0 + np.log2(1.0 + 2.0 ** -11 + 2.0 ** -13)) * np.log(2.0), mask).astype(np.float64)
+        # (weights rounded to fp16 against their unrounded sum, 2^-11, then the result's rounding)
+        assert np.isfinite(got).all() and (np.abs(got - sign * 65504.0) <= 65504.0 * (2.0 ** -10 + 2.0 ** -20)).all()
