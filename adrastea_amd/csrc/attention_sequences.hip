@@ -1442,6 +1442,12 @@ bool chunks(const SequencesArgs& a) {
          strides % 8 == 0 && strides >= 0 && near(a.sk.y) && near(a.sv.y) && (!a.table || page_shift(a.page_size) >= 0);
 }
 
+// Blocks of all key heads that there can be, and as many as a launch of 256 threads to each may have.
+int64_t most_blocks(const SequencesArgs& a, int rows) {
+  return ((int64_t)a.rows * a.group / rows + std::min(a.rows, a.sequences)) * a.kv_heads;
+}
+constexpr int64_t LAUNCH_BLOCKS = 0x7fffffff / 256;
+
 }  // namespace
 
 SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
@@ -1519,6 +1525,8 @@ SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
   const int64_t part = ((few ? 2 : 1) * (int64_t)rows * (hd * 4 + 8) + (int64_t)sizeof(Seam)) * a.kv_heads;
   p.parts = (int)std::min<int64_t>(p.parts, avail / part);
   if (p.parts < 2) p.parts = 0;
+  // (hundreds of thousands of sequences with a block to each: the kernel whose wavefronts take one row after the other)
+  if (p.parts == 0 && most_blocks(a, rows) > LAUNCH_BLOCKS) return SequencesPlan{SequencesPlan::ANY_LAYOUT, 0, 0, 0, 0, 0};
   p.workspace_bytes = p.parts * part;
   return p;
 }
@@ -1537,9 +1545,9 @@ static hipError_t launch_blocks(hipStream_t stream, const SequencesArgs& a, cons
   job.part_ml = (float2*)(job.part_o + (p.parts > 0 ? part_rows * HD : 0));
   job.seams = (Seam*)(job.part_ml + (p.parts > 0 ? part_rows : 0));
   // Unshared: as many as there can be blocks.  Shared: a stretch to each, or a part.
-  const int64_t most = (int64_t)a.rows * a.group / rows + std::min(a.rows, a.sequences);  // blocks of a key head
-  const int64_t blocks = (p.parts == 0 ? most : few ? p.parts : std::max<int64_t>(p.parts, most)) * a.kv_heads;
-  if (blocks > 0x7fffffff / 256) return hipErrorInvalidConfiguration;
+  const int64_t most = most_blocks(a, rows), shared = (int64_t)p.parts * a.kv_heads;
+  const int64_t blocks = p.parts == 0 ? most : few ? shared : std::max(shared, most);
+  if (blocks > LAUNCH_BLOCKS) return hipErrorInvalidConfiguration;
   const int at_once = std::min(rows, 1024 / HD);  // rows of the joining workgroups
   const dim3 grid((unsigned)blocks), join((unsigned)((few ? p.parts - 1 : p.parts / 2) * a.kv_heads * (rows / at_once)));
   const dim3 threads(64 * p.waves);

@@ -479,8 +479,8 @@ int adr_append_f16(adr_stream_t stream, adr_paged_cache cache, adr_paged_batch b
  * `output` overlaps none of the others.
  * d 1 .. 256, scale > 0, temp > 0, scale / temp 2^-126 .. 2^58 (ADR_EUNSUPPORTED_LAYOUT beyond), heads a multiple of kv_heads.  The fast
  * kernels take d a multiple of 8 up to 128, x strides 1, the others multiples of 8 and not negative, slots at
- * least d apart and less than 2^24, 16-byte aligned pointers, pages of 16, 32, 64 ... slots; everything else runs on
- * a kernel of one wavefront per row.
+ * least d apart and less than 2^24, 16-byte aligned pointers, pages of 16, 32, 64 ... slots; everything else, and
+ * calls with more blocks of rows than a launch has workgroups (millions), run on a kernel of one wavefront per row.
  * Where rows are few the keys of a sequence are shared by several workgroups whose parts pass through
  * scratch memory and are added by a second launch, in a fixed order: from the library's pool
  * (adr_set_held_workspace_limit; under capture, or where the pool cannot be used, keys are not shared), or

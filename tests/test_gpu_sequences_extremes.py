@@ -2,8 +2,10 @@
 what the definition gives in 64 bits."""
 import numpy as np
 import pytest
+import torch
 
-from test_gpu_sequences import CAUSAL, NONE, Packed, dev, heads_view, shared_keys  # noqa: F401 (fixtures)
+from adrastea_amd import PackedBatch
+from test_gpu_sequences import CAUSAL, NONE, Packed, dev, heads_view, kern, shared_keys  # noqa: F401 (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +80,14 @@ def test_the_largest_values_stay_finite(shared_keys, sign, rows):
         got = packed_call(shared_keys, p, (7.0 + np.log2(1.0 + 2.0 ** -11 + 2.0 ** -13)) * np.log(2.0), mask).astype(np.float64)
         # (weights rounded to fp16 against their unrounded sum, 2^-11, then the result's rounding)
         assert np.isfinite(got).all() and (np.abs(got - sign * 65504.0) <= 65504.0 * (2.0 ** -10 + 2.0 ** -20)).all()
+
+
+def test_more_sequences_than_a_launch_has_workgroups(kern):  # noqa: F811
+    """Many sequences of one row that sees one key: each row's result is its value, to the bit."""
+    n, heads, d = 280000, 32, 8
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    q, k, v = torch.randn(3, n, heads, d, dtype=torch.float16, device="cuda", generator=gen)
+    out = torch.zeros_like(q)
+    at = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    kern.attention_packed_f16(*(heads_view(t) for t in (out, q, k, v)), PackedBatch(at, at), 0.3)
+    assert torch.equal(out, v)
