@@ -441,6 +441,31 @@ __device__ __forceinline__ int end_of_row(Args a, const Sequence& q, int j) {
 }
 
 
+// A value that is no number times the zero of a key that a row does not see is no zero, and a page that is not in the cache is
+// noticed for a block as a whole.  So where rows of a block come out as no numbers, the first of them seeing the keys before
+// x0, this looks, by all lanes, whether some key of x0 ... x1 - 1, the block's last, holds such a value or has no page: then the rows
+// are computed again from the keys that they see.  Otherwise it is their own result.  (For whole chunks of 16 bytes.)  One row
+// after the other is slow, and these are a block's: a prompt of 4096 rows (32 / 8 heads of 128, 0.17 ms) whose first value is NaN
+// 0.2 ms, whose 2000th or last one is 31 or 75 ms; with all rows that are no numbers computed again each took 75 to 89 ms.
+__device__ __forceinline__ bool hidden_reaches(Args a, const Sequence& q, int hk, int x0, int x1, int lane) {
+  const half_t* const V = a.v + hk * a.sv.z;
+  bool lost = false;
+  float zero = 0.0f;
+  for (int x = x0 + lane; x < x1; x += 64) {
+    int64_t ko, vo;
+    if (!key_at(a, q, x, ko, vo)) {
+      lost = true;
+      break;
+    }
+    for (int i = 0; i < a.d; i += 8) {
+      const half8_t v = *(const half8_t*)(V + vo + i);
+#pragma unroll
+      for (int e = 0; e < 8; e++) zero = fmaf((float)v[e], 0.0f, zero);
+    }
+  }
+  return __ballot(lost || !(zero == 0.0f)) != 0;
+}
+
 // A transfer's descriptor, in scalar registers: `bytes` from an address on.
 __device__ __forceinline__ u32x4_t descriptor(uint64_t p, int bytes) {
   return u32x4_t{(uint32_t)uniform((int)(uint32_t)p), (uint32_t)uniform((int)((uint32_t)(p >> 32) & 0xffffu)),
@@ -742,11 +767,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
 #pragma unroll
     for (int x = 0; x < WAVES; x++) m_all = fmaxf(m_all, xml[x * 16 + frow].x);
     int again = (int)__ballot(fabsf(m_all) > FAR_SCORE);  // (not stored above)
-    // A value that is no number times the zero of a key that the row does not see is no zero: such rows are computed
-    // again from the keys that they see.
     if (q.rows > 1 && z.mask == ADR_MASK_CAUSAL) {
       __syncthreads();
-      again |= *bad_rows;
+      const int bad = uniform(*bad_rows);
+      if (bad && hidden_reaches(z, q, hk, end_of_row(z, q, row_of_list(z, block * ROWS + __builtin_ctz(bad))),
+                                end_of_row(z, q, row_of_list(z, block * ROWS + rows - 1)), lane))
+        again |= bad;
     }
     for (int r = w; r < rows; r += WAVES)
       if (again >> r & 1) {
@@ -1261,8 +1287,8 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
   Args z = arguments();
   float l_tot = pair_sum(l_run);
   if constexpr (PAGED) {
-    // (a page that is not in the cache may be some rows' only: all of the block come out as NaN, and those that do not
-    // see it are computed again below)
+    // (a page that is not in the cache may be some rows' only: all of the block come out as NaN, and where some do not see
+    // it they are computed again below)
     int any = 0;
 #pragma unroll
     for (int i = 0; i < 4 * GROUPS; i++) any |= lost_keys[i];
@@ -1316,15 +1342,18 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
       token += more_tokens, head += more_heads;
       if (head >= z.group) head -= z.group, token++;
     }
-    // A value that is no number times the zero of a key that the row does not see is no zero: such rows are computed
-    // again from the keys that they see, a group's columns of them.
-    const uint64_t lanes = __ballot(fabsf(m_run) > FAR_SCORE ||
-                                    (!finite && q.rows > 1 && z.mask == ADR_MASK_CAUSAL));
-    if (lanes) {
-      const uint32_t bad = (uint32_t)lanes | (uint32_t)(lanes >> 32);
+    // Rows that are computed again, a group's columns of them.
+    const uint64_t wrong = __ballot(!finite), far = __ballot(fabsf(m_run) > FAR_SCORE);
+    if ((wrong | far) && wave_rows > 0) {
+      uint32_t again = (uint32_t)far | (uint32_t)(far >> 32);
+      const uint32_t bad = (uint32_t)wrong | (uint32_t)(wrong >> 32);
+      if (bad && q.rows > 1 && z.mask == ADR_MASK_CAUSAL &&
+          hidden_reaches(z, q, hk, end_of_row(z, q, row_of_list(z, list0 + min(__builtin_ctz(bad), wave_rows - 1))),
+                         end_of_row(z, q, row_of_list(z, block * ROWS + rows - 1)), lane))
+        again |= bad;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (behind the stores above)
       for (int r = 0; r < wave_rows; r++)
-        if (bad >> r & 1)
+        if (again >> r & 1)
           row_by_wave(arguments(), q, (list0 + r) / z.group, hk * z.group + (list0 + r) % z.group, lane, col0, col0 + 32 * MINE);
     }
   } else if (frow < wave_rows) {
@@ -1348,7 +1377,8 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
 template <int HD, int ROWS>
 __global__ __launch_bounds__(256) void attention_join_kernel(Job) {
   constexpr int COLS = HD / 4, AT_ONCE = 256 / COLS < ROWS ? 256 / COLS : ROWS, GROUPS = ROWS / AT_ONCE;
-  __shared__ int bad_rows;  // whose result is not finite
+  __shared__ int bad_rows;  // whose result is not finite; 16 bits on, whose scores are beyond FAR_SCORE
+  static_assert(AT_ONCE <= 16, "a bit to each");
   const int tid = threadIdx.x, lane = tid & 63;
   Args a = arguments();
   const int hk = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads;
@@ -1412,13 +1442,19 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Job) {
     const int lr = b.block * ROWS + r, token = row_of_list(a, lr), h = hk * a.group + lr - token * a.group;
     half4_t out;
     const bool finite = round_means(out, acc, l == 0.0f ? 0.0f : 1.0f / l);
-    const bool far = fabsf(m) > FAR_SCORE;
-    if (far || (!finite && b.q.rows > 1 && a.mask == ADR_MASK_CAUSAL)) atomicOr(&bad_rows, 1 << (r - r0));  // (as above)
+    if (!finite) atomicOr(&bad_rows, 1 << (r - r0));
+    if (fabsf(m) > FAR_SCORE) atomicOr(&bad_rows, 0x10000 << (r - r0));
     if (col < a.d) *(half4_t*)(a.out + (int64_t)h * a.so_z + (int64_t)(b.q.row0 + token) * a.so_y + col) = out;
   }
   __syncthreads();
+  int again = uniform(bad_rows) >> 16 & 0xffff;
+  const int bad = uniform(bad_rows) & 0xffff;
+  if (bad && b.q.rows > 1 && a.mask == ADR_MASK_CAUSAL &&
+      hidden_reaches(a, b.q, hk, end_of_row(a, b.q, row_of_list(a, b.block * ROWS + r0 + __builtin_ctz(bad))),
+                     end_of_row(a, b.q, row_of_list(a, b.block * ROWS + rows - 1)), lane))
+    again |= bad;
   for (int x = tid >> 6; x < AT_ONCE; x += 4)
-    if (bad_rows >> x & 1) {
+    if (again >> x & 1) {
       const int lr = b.block * ROWS + r0 + x;
       row_by_wave(arguments(), b.q, lr / a.group, hk * a.group + lr % a.group, lane);
     }

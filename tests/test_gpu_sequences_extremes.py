@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from adrastea_amd import PackedBatch
+import sequences_reference as ref
 from test_gpu_sequences import CAUSAL, NONE, Packed, dev, heads_view, kern, shared_keys  # noqa: F401 (fixtures)
 
 pytestmark = pytest.mark.gpu
@@ -91,3 +92,54 @@ def test_more_sequences_than_a_launch_has_workgroups(kern):  # noqa: F811
     at = torch.arange(n + 1, dtype=torch.int32, device="cuda")
     kern.attention_packed_f16(*(heads_view(t) for t in (out, q, k, v)), PackedBatch(at, at), 0.3)
     assert torch.equal(out, v)
+
+
+@pytest.mark.parametrize("seen,hidden", [(3, None), (None, 1), (3, 1), (None, 2), (5, 2)])
+@pytest.mark.parametrize("rows,keys", [(9, 200), (150, 150), (70, 400)])
+def test_no_numbers_before_and_behind_a_row(shared_keys, rows, keys, seen, hidden):
+    """Values that are no numbers, in columns of their own: at a key that all rows see, and at one of the last, which only the
+    rows behind it see.  Every row has them in exactly these columns, and numbers in the others."""
+    p = Packed([(3, 3), (rows, keys), (2, 9)], 4, 2, 128, seed=rows)
+    first = p.key_offsets[1]
+    gone = np.zeros((rows, p.d), bool)
+    clean = p.v.copy()
+    if seen is not None:
+        p.v[first + keys - rows - (0 if rows == keys else seen), :, 5] = np.inf
+        gone[:, 5] = True
+    if hidden is not None:
+        p.v[first + keys - hidden, :, 70] = -np.inf
+        gone[rows - hidden:, 70] = True
+    got = packed_call(shared_keys, p, 0.1)
+    a = p.row_offsets[1]
+    assert (np.isfinite(got[a:a + rows]) == ~gone[:, None, :]).all()
+    assert np.isfinite(got[:a]).all() and np.isfinite(got[a + rows:]).all()
+    p.v = clean
+    want = p.want(0.1, CAUSAL)[:p.row_offsets[-1]]
+    got[a:a + rows] = np.where(gone[:, None, :], want[a:a + rows], got[a:a + rows])
+    assert ref.close_enough(got, want, np.abs(clean[:-1].astype(np.float64)).max(), keys)
+
+
+@pytest.mark.parametrize("what", ["key", "value"])
+def test_a_prompt_of_no_numbers_takes_no_longer(kern, what):  # noqa: F811
+    """Rows that come out as NaN because they see one are not computed twice: 500 times the time when they were."""
+    n, heads, kv, d = 4096, 32, 8, 128
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    q, out = torch.randn(2, n, heads, d, dtype=torch.float16, device="cuda", generator=gen)
+    k, v = torch.randn(2, n, kv, d, dtype=torch.float16, device="cuda", generator=gen)
+    at = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    batch = PackedBatch(at, at, n, n)
+
+    def fastest():
+        times = []
+        for _ in range(4):
+            begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            begin.record()
+            kern.attention_packed_f16(*(heads_view(t) for t in (out, q, k, v)), batch, 0.1)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(begin.elapsed_time(end))
+        return min(times)
+    numbers = fastest()
+    (k if what == "key" else v)[7] = float("nan")
+    assert fastest() < 20 * numbers
+    assert out[7:].isnan().all() and out[:7].isfinite().all()
