@@ -87,6 +87,14 @@ inline LoweredMatmul lower_matmul(const TensorLayout& out, const TensorLayout& l
 
 // ---- several sequences at once (not in the reference) ----
 
+// A size or a stride as the C ABI takes it; strides of a dimension of one are never used, and may be anything.
+inline int32_t int32_of(size_t v, const char* what, bool used = true) {
+  const int64_t x = (int64_t)v;
+  if (x >= INT32_MIN && x <= INT32_MAX) return (int32_t)x;
+  if (used) throw std::logic_error(std::string(what) + ": " + std::to_string(x) + " does not fit 32 bits");
+  return 0;
+}
+
 // Keys and values of many sequences in pages: [pages, kv_heads, page_size, d] views of the caller's pools.
 struct PagedCache {
   TensorView<f16> key, value;
@@ -95,7 +103,8 @@ struct PagedCache {
     if (k.dims.size() != 4 || k.dims != v.dims) throw std::logic_error("PagedCache: [pages, kv_heads, page_size, d] views");
     adr_paged_cache c{};
     c.key = key.ptr, c.value = value.ptr;
-    c.pages = (int32_t)k.dims[0], c.kv_heads = (int32_t)k.dims[1], c.page_size = (int32_t)k.dims[2], c.d = (int32_t)k.dims[3];
+    auto size = [&](int i) { return int32_of(k.dims[i], "PagedCache"); };
+    c.pages = size(0), c.kv_heads = size(1), c.page_size = size(2), c.d = size(3);
     c.stride_kx = (int64_t)k.strides[3], c.stride_ky = (int64_t)k.strides[2], c.stride_kz = (int64_t)k.strides[1], c.stride_kp = (int64_t)k.strides[0];
     c.stride_vx = (int64_t)v.strides[3], c.stride_vy = (int64_t)v.strides[2], c.stride_vz = (int64_t)v.strides[1], c.stride_vp = (int64_t)v.strides[0];
     return c;
@@ -234,8 +243,9 @@ class GpuKernels : public CommonKernels {
     const auto& l = v.layout;
     if (l.dims.size() != 2 && l.dims.size() != 3) throw std::logic_error(std::string(what) + ": [heads, rows, d] views");
     const bool h = l.dims.size() == 3;
-    return {h ? (int32_t)l.size(-3) : 1, (int32_t)l.size(-2), (int32_t)l.size(-1), (int32_t)l.stride(-1), (int32_t)l.stride(-2),
-            h ? (int32_t)l.stride(-3) : 0};
+    auto size = [&](long i) { return int32_of(l.size(i), what); };
+    auto stride = [&](long i) { return int32_of(l.stride(i), what, l.size(i) > 1); };
+    return {h ? size(-3) : 1, size(-2), size(-1), stride(-1), stride(-2), h ? stride(-3) : 0};
   }
   static void same(const Rows& a, const Rows& b, const char* what) {
     if (a.heads != b.heads || a.rows != b.rows || a.d != b.d) throw std::logic_error(std::string(what) + ": shape mismatch");

@@ -260,6 +260,7 @@ class Rotary:
     @property
     def _desc(self) -> _ffi.RotaryDesc:
         _here(self.turns)
+        _int32("turns", 2 * self.turns.numel())
         return _ffi.RotaryDesc(self.turns.data_ptr(), 2 * self.turns.numel(), self.layout, self.magnitude)
 
 
@@ -282,6 +283,7 @@ class PagedCache:
         k, v = self.key.layout, self.value.layout
         _here(self.key.storage, self.value.storage)
         p, h, s, d = k.dims
+        _int32("sizes of the pages", p, h, s, d)
         return _ffi.PagedCacheDesc(self.key.data_ptr(), self.value.data_ptr(), p, h, s, d,
                                    *(t.strides[i] for t in (k, v) for i in (3, 2, 1, 0)))
 
@@ -293,6 +295,18 @@ def _here(*storages) -> None:
     for s in storages:
         at = getattr(s, "get_device", None)
         assert at is None or at() == device, f"memory of device {at()} in a call on device {device} (-1: the host)"
+
+
+def _int32(what: str, *values: int) -> None:
+    """The C interface has 32 bits for them, and ctypes drops the others without a word."""
+    for v in values:
+        if not -2 ** 31 <= v < 2 ** 31:
+            raise ValueError(f"{what}: {v} does not fit 32 bits")
+
+
+def _hint(v: int) -> int:
+    """(Hints choose kernels and nothing else: what is too large for 32 bits says the same as their largest number.)"""
+    return min(max(v, -2 ** 31), 2 ** 31 - 1)
 
 
 def _index(t, rank, what):
@@ -324,8 +338,9 @@ class PagedBatch:
         n = self.lengths.shape[0]
         _here(self.row_offsets, self.lengths, self.table)
         pitch = self.table.stride(0) if n > 1 else self.table.shape[1]
+        _int32("sequences and table", n, self.table.shape[1], pitch)
         return _ffi.PagedBatchDesc(self.row_offsets.data_ptr(), self.lengths.data_ptr(), self.table.data_ptr(), n,
-                                   self.table.shape[1], pitch, self.longest_rows, self.longest)
+                                   self.table.shape[1], pitch, _hint(self.longest_rows), _hint(self.longest))
 
 
 @dataclass(frozen=True)
@@ -344,8 +359,9 @@ class PackedBatch:
     def _desc(self) -> _ffi.PackedBatchDesc:
         n = self.row_offsets.shape[0]
         _here(self.row_offsets, self.key_offsets)
-        return _ffi.PackedBatchDesc(self.row_offsets.data_ptr(), self.key_offsets.data_ptr(), n - 1, self.longest_rows,
-                                    self.longest)
+        _int32("sequences", n)
+        return _ffi.PackedBatchDesc(self.row_offsets.data_ptr(), self.key_offsets.data_ptr(), n - 1, _hint(self.longest_rows),
+                                    _hint(self.longest))
 
 
 def _rows_view(view: TensorView, what: str):
@@ -353,6 +369,9 @@ def _rows_view(view: TensorView, what: str):
     dims, strides = view.layout.dims, view.layout.strides
     assert len(dims) in (2, 3), f"{what}: a [heads, rows, d] view"
     _here(view.storage)
+    # (of a dimension of one the stride is never used, and may be anything)
+    strides = tuple(0 if n <= 1 and not -2 ** 31 <= s < 2 ** 31 else s for n, s in zip(dims, strides))
+    _int32(what, *dims, *strides)
     if len(dims) == 2:
         return (1, *dims), (strides[1], strides[0], 0)
     return dims, strides[::-1]
@@ -738,6 +757,7 @@ def attention_workspace_bytes(output: TensorLayout, query: TensorLayout, key: Te
 def attention_paged_workspace_bytes(cache: PagedCache, batch: PagedBatch, heads: int, rows: int) -> int:
     """Scratch bytes adr_attention_paged_f16_ws would use for `rows` packed rows of `heads` query heads (0: it would share no
     keys)."""
+    _int32("heads and rows", heads, rows)
     n = _ffi.lib().adr_attention_paged_f16_workspace_bytes(cache._desc, batch._desc, heads, rows)
     if n < 0:
         raise AdrasteaError(int(n), "attention_paged_f16_workspace_bytes")
@@ -746,6 +766,7 @@ def attention_paged_workspace_bytes(cache: PagedCache, batch: PagedBatch, heads:
 
 def attention_packed_workspace_bytes(batch: PackedBatch, heads: int, kv_heads: int, rows: int, keys: int, d: int) -> int:
     """Scratch bytes adr_attention_packed_f16_ws would use for these sizes (0: it would share no keys)."""
+    _int32("heads, rows and keys", heads, kv_heads, rows, keys, d)
     n = _ffi.lib().adr_attention_packed_f16_workspace_bytes(batch._desc, heads, kv_heads, rows, keys, d)
     if n < 0:
         raise AdrasteaError(int(n), "attention_packed_f16_workspace_bytes")

@@ -214,3 +214,105 @@ def test_memory_of_another_device(both):
                         ("attention_packed_f16", q, q, q, q, PackedBatch(p.row_offsets, Elsewhere(p.key_offsets)), 0.1, 1.0, 1)]:
         assert both(name, *args) == (None, None), (name, args)
     same(both("rotary_f16", q, q, at, r))
+
+
+FAR = 1 << 31
+
+
+def spread(*strides, dims=(6, 2, 64), offset=0):
+    return TensorView(half(6 * 2 * 64), TensorLayout(dims, strides), offset)
+
+
+def test_strides_and_sizes_of_more_than_32_bits(both):
+    """Neither path passes on what the C interface would take for another number."""
+    q, o, c, b, at, r, k = rows(6, 2, 64), rows(6, 2, 64), cache(), batch(), ints(4, 5), rotary(), rows(2, 2, 64)
+    p = PackedBatch(ints(0, 1, 2), ints(0, 1, 2))
+    two = (2, 2, 64)
+    for strides in ((FAR, 64, 1), ((1 << 32) + 64, 64, 1), (-FAR - 1, 64, 1), (128, FAR, 1), (128, 64, 1 << 33)):
+        x, y = spread(*strides), spread(*strides, dims=two)
+        for name, *args in [("rotary_f16", x, q, at, r), ("rotary_f16", o, x, at, r), ("append_f16", c, b, y, k, r, None, None, None),
+                            ("append_f16", c, b, k, y, r, None, None, None), ("append_f16", c, b, k, k, r, o, x, None),
+                            ("append_f16", c, b, k, k, r, x, q, at), ("attention_paged_f16", x, q, c, b, 0.1, 1.0, 1),
+                            ("attention_paged_f16", o, x, c, b, 0.1, 1.0, 1), ("attention_packed_f16", o, q, y, k, p, 0.1, 1.0, 1),
+                            ("attention_packed_f16", o, q, k, y, p, 0.1, 1.0, 1), ("attention_packed_f16", o, x, k, k, p, 0.1, 1.0, 1)]:
+            with pytest.raises(ValueError):
+                both(name, *args)
+    long = spread(64, 64, 1, dims=(2, FAR, 64))   # (never read: its address is all that a call takes)
+    with pytest.raises(ValueError):
+        both("attention_packed_f16", o, q, long, long, p, 0.1, 1.0, 1)
+    pages = TensorView(half(64), TensorLayout((FAR, 2, 16, 64), (2048, 1024, 64, 1)))
+    with pytest.raises(ValueError):
+        both("attention_paged_f16", o, q, PagedCache(pages, pages), b, 0.1, 1.0, 1)
+
+
+def test_what_fits_is_passed_on(both):
+    """The ends of 32 bits, strides that no element uses, and hints of any size."""
+    q, c, b = rows(6, 2, 64), cache(), batch()
+    for z in (FAR - 1, -FAR):
+        assert str(z) in same(both("attention_paged_f16", spread(z, 64, 1), q, c, b, 0.1, 1.0, 1)).split()
+    one = spread(1 << 40, 64, 1, dims=(1, 2, 64))
+    assert both("rotary_f16", one, one, ints(1, 2), rotary())[1].split()[-6:] == ["1", "64", "0", "1", "64", "0"]
+    seen = both("attention_paged_f16", q, q, c, batch(longest_rows=1 << 40, longest=1 << 31), 0.1, 1.0, 1)[1].split()
+    assert seen.count(str(FAR - 1)) == 2
+
+
+def test_sizes_of_a_workspace_have_32_bits():
+    p = PackedBatch.__new__(PackedBatch)
+    for args in ((1 << 32, 2, 50, 50, 64), (4, 2, 1 << 31, 50, 64), (4, 2, 50, (1 << 32) + 1, 64)):
+        with pytest.raises(ValueError):
+            kernels.attention_packed_workspace_bytes(p, *args)
+    with pytest.raises(ValueError):
+        kernels.attention_paged_workspace_bytes(None, None, 4, 1 << 31)
+
+
+CPP = r"""
+#include "adrastea_amd/host/kernels.hpp"
+#include <cstdio>
+using namespace adrastea;
+static f16* const P = (f16*)4096;  // never read
+static int wrong = 0;
+template <typename F> static void refuses(const char* what, F f) {
+  try { f(); } catch (const std::logic_error&) { return; } catch (const std::exception&) {}
+  printf("passed on: %s\n", what), wrong++;
+}
+int main() {
+  GpuKernels k;
+  const size_t far = size_t(1) << 31, z[] = {far, (far << 1) + 64, (size_t)(-(long)far - 1)};
+  const PagedCache cache{{P, TensorLayout::row_major({6, 2, 16, 64})}, {P, TensorLayout::row_major({6, 2, 16, 64})}};
+  const PagedBatch batch{(const int32_t*)P, (const int32_t*)P, (const int32_t*)P, 2, 3, 3, 1, 48};
+  const PackedBatch packed{(const int32_t*)P, (const int32_t*)P, 2, 1, 48};
+  const Rotary none{nullptr, 0, ADR_ROTARY_HALVES, 1.0f};
+  TensorView<f16> out(P, TensorLayout::row_major({4, 3, 64}));
+  const TensorView<const f16> q(P, out.layout), kv(P, TensorLayout::row_major({2, 3, 64}));
+  for (size_t s : z) {
+    TensorView<f16> o(P, TensorLayout({4, 3, 64}, {s, 64, 1}));
+    const TensorView<const f16> x(P, o.layout), y(P, TensorLayout({2, 3, 64}, {s, 64, 1})), v(P, TensorLayout({2, 3, 64}, {192, s, 1}));
+    refuses("rotary, output", [&] { k.rotary_f16(o, q, (const int32_t*)P, none); });
+    refuses("rotary, input", [&] { k.rotary_f16(out, x, (const int32_t*)P, none); });
+    refuses("append, key", [&] { k.append_f16(cache, batch, y, kv, none); });
+    refuses("append, value", [&] { k.append_f16(cache, batch, kv, v, none); });
+    refuses("append, query", [&] { k.append_f16(cache, batch, kv, kv, none, &out, &x); });
+    refuses("paged", [&] { k.attention_paged_f16(out, x, cache, batch, 0.1f); });
+    refuses("packed", [&] { k.attention_packed_f16(out, q, y, kv, packed, 0.1f); });
+    refuses("packed, values", [&] { k.attention_packed_f16(out, q, kv, v, packed, 0.1f); });
+  }
+  const TensorLayout pages({far, 2, 16, 64}, {2048, 1024, 64, 1});
+  refuses("pages", [&] { PagedCache{{P, pages}, {P, pages}}.lower(); });
+  const TensorView<const f16> one(P, TensorLayout({1, 3, 64}, {far, 64, 1}));   // (a stride that no element uses)
+  if (GpuKernels::rows_of(one, "").z != 0) printf("unused stride\n"), wrong++;
+  const TensorView<const f16> back(P, TensorLayout({2, 3, 64}, {(size_t)-192l, 64, 1}));
+  if (GpuKernels::rows_of(back, "").z != -192) printf("negative stride\n"), wrong++;
+  return wrong;
+}
+"""
+
+
+def test_strides_and_sizes_through_the_host_mirror(tmp_path):
+    if shutil.which("g++") is None:
+        pytest.skip("no C++ compiler")
+    (tmp_path / "sizes.cpp").write_text(CPP)
+    lib = os.path.dirname(_ffi.LIB_PATH)
+    subprocess.run(["g++", "-std=c++17", "-I" + ROOT, "-o", str(tmp_path / "sizes"), str(tmp_path / "sizes.cpp"), "-L" + lib,
+                    "-l:" + os.path.basename(_ffi.LIB_PATH), "-Wl,-rpath," + lib, "-Wl,--allow-shlib-undefined"], check=True)
+    r = subprocess.run([str(tmp_path / "sizes")], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout
