@@ -19,7 +19,8 @@ constexpr int MAX_RANK = 7;  // of a descriptor; views of higher rank take the g
 
 PyObject *layout_type, *view_type;                      // the classes of tensor.py
 PyObject *of_general, *permute_general, *cast_general;  // their definitions of the methods below
-PyObject *current_device, *raw_stream, *int32_type;     // torch's functions, torch.int32
+PyObject *current_device, *raw_stream;                  // torch's functions
+PyObject *int32_type, *float16_type;                    // torch's types
 PyObject *s_shape, *s_stride, *s_dims, *s_strides, *s_storage, *s_layout, *s_offset, *s_data_ptr, *s_load, *s_store,
     *s_mask, *s_op, *s_scale, *s_beta, *s_bias, *s_is_contiguous, *s_get_device, *s_key, *s_value, *s_row_offsets, *s_lengths,
     *s_table, *s_key_offsets, *s_longest_rows, *s_longest, *s_turns, *s_rotary_layout, *s_magnitude, *s_dtype;
@@ -460,6 +461,8 @@ bool read_rows(PyObject* view, int64_t device, Rows& r) {
     return false;
   const Ref storage(attr(view, s_storage));
   if (!storage.p || !on_device(storage, device)) return false;
+  const Ref type(attr(storage, s_dtype));
+  if (type.p != float16_type) return false;  // (others that are let pass go the general way)
   for (int i = 0; i < l.rank; i++)
     if (l.dims[i] > INT32_MAX || l.strides[i] > INT32_MAX || l.strides[i] < INT32_MIN) return false;
   r.heads = l.rank == 3 ? (int32_t)l.dims[0] : 1;
@@ -687,6 +690,10 @@ PyObject* bind_sequences(PyObject*, PyObject* args) {
   unsigned long long p[4];
   PyObject* type;
   if (!PyArg_ParseTuple(args, "KKKKO", p, p + 1, p + 2, p + 3, &type)) return nullptr;
+  const Ref torch(PyImport_ImportModule("torch"));
+  PyObject* const half = torch.p ? PyObject_GetAttrString(torch, "float16") : nullptr;
+  if (!half) return nullptr;
+  Py_XSETREF(float16_type, half);
   Py_INCREF(type);
   Py_XSETREF(int32_type, type);
   rotary_fn = (decltype(rotary_fn))p[0];

@@ -277,6 +277,8 @@ class PagedCache:
     def __post_init__(self):
         k, v = self.key.layout, self.value.layout
         assert len(k.dims) == 4 and k.dims == v.dims, "key and value pages are [pages, kv_heads, page_size, d] views"
+        _halves("key pages", self.key)
+        _halves("value pages", self.value)
 
     @property
     def _desc(self) -> _ffi.PagedCacheDesc:
@@ -302,6 +304,14 @@ def _int32(what: str, *values: int) -> None:
     for v in values:
         if not -2 ** 31 <= v < 2 ** 31:
             raise ValueError(f"{what}: {v} does not fit 32 bits")
+
+
+def _halves(what: str, view) -> None:
+    """Values of fp16, or their bits in 16-bit integers: the kernels would read and write any other type as if it were."""
+    import torch
+    dtype = getattr(view.storage, "dtype", None)
+    if dtype not in (torch.float16, torch.int16, torch.uint16) and (dtype is not None or view.storage.element_size() != 2):
+        raise TypeError(f"{what}: values of {dtype}, not of fp16")
 
 
 def _hint(v: int) -> int:
@@ -369,6 +379,7 @@ def _rows_view(view: TensorView, what: str):
     dims, strides = view.layout.dims, view.layout.strides
     assert len(dims) in (2, 3), f"{what}: a [heads, rows, d] view"
     _here(view.storage)
+    _halves(what, view)
     # (of a dimension of one the stride is never used, and may be anything)
     strides = tuple(0 if n <= 1 and not -2 ** 31 <= s < 2 ** 31 else s for n, s in zip(dims, strides))
     _int32(what, *dims, *strides)

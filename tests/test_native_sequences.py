@@ -316,3 +316,30 @@ def test_strides_and_sizes_through_the_host_mirror(tmp_path):
                     "-l:" + os.path.basename(_ffi.LIB_PATH), "-Wl,-rpath," + lib, "-Wl,--allow-shlib-undefined"], check=True)
     r = subprocess.run([str(tmp_path / "sizes")], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stdout
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64, torch.uint8, torch.int32])
+def test_values_of_another_type(both, dtype):
+    """Nothing but fp16 is read, or written, as fp16."""
+    def other(view):
+        return TensorView(torch.zeros(view.storage.shape, dtype=dtype), view.layout)
+    q, c, b, at, r, k = rows(6, 2, 64), cache(), batch(), ints(4, 5), rotary(), rows(2, 2, 64)
+    p = PackedBatch(ints(0, 1, 2), ints(0, 1, 2))
+    for name, *args in [("rotary_f16", other(q), q, at, r), ("rotary_f16", q, other(q), at, r),
+                        ("append_f16", c, b, other(k), k, r, None, None, None), ("append_f16", c, b, k, other(k), r, None, None, None),
+                        ("append_f16", c, b, k, k, r, other(q), q, None), ("append_f16", c, b, k, k, r, q, other(q), None),
+                        ("attention_paged_f16", other(q), q, c, b, 0.1, 1.0, 1), ("attention_paged_f16", q, other(q), c, b, 0.1, 1.0, 1),
+                        ("attention_packed_f16", other(q), q, k, k, p, 0.1, 1.0, 1), ("attention_packed_f16", q, other(q), k, k, p, 0.1, 1.0, 1),
+                        ("attention_packed_f16", q, q, other(k), k, p, 0.1, 1.0, 1), ("attention_packed_f16", q, q, k, other(k), p, 0.1, 1.0, 1)]:
+        assert both(name, *args) == (None, None), (name, args)
+    for pools in ((other(c.key), c.value), (c.key, other(c.value))):
+        with pytest.raises(TypeError):
+            PagedCache(*pools)
+
+
+@pytest.mark.parametrize("dtype", [torch.int16, torch.uint16])
+def test_bits_of_fp16(both, dtype):
+    """fp16 kept as 16-bit integers, as the C interface has it, is taken by the general path."""
+    x = TensorView(torch.zeros(2, 6, 64, dtype=dtype), TensorLayout((6, 2, 64), (64, 384, 1)))
+    native, general = both("rotary_f16", x, x, ints(4, 5), rotary())
+    assert native is None and general.split()[-9:] == ["6", "2", "64", "1", "384", "64", "1", "384", "64"]
