@@ -1003,6 +1003,7 @@ int adr_append_f16(adr_stream_t stream, adr_paged_cache cache, adr_paged_batch b
                    int32_t stride_kz, int32_t stride_vx, int32_t stride_vy, int32_t stride_vz, int32_t stride_ox,
                    int32_t stride_oy, int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz) {
   bool nothing;
+  if (heads == 0) query = query_out = nullptr;
   if (!query && !query_out) heads = cache.kv_heads;  // (no queries: their number does not count)
   if (int rc = validate_rows(heads, cache.kv_heads, rows, cache.d, batch.sequences, &nothing)) return rc;
   if (int rc = validate_cache(cache, batch)) return rc;

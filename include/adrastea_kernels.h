@@ -455,7 +455,7 @@ int adr_rotary_f16(adr_stream_t stream, uint16_t* output, const uint16_t* input,
 /*
  * A step's new keys and values into the cache: row j of sequence s, of its r rows, is key
  * x = lengths[s] - r + j; `key` goes there rotated, `value` as it is ([kv_heads, rows, d] views).  `query`
- * ([heads, rows, d]) is rotated into `query_out`, which may be the same view; both may be null.  The angle
+ * ([heads, rows, d]) is rotated into `query_out`, which may be the same view; both may be null, or have 0 heads.  The angle
  * is that of position x, or of positions[row] where `positions` is not null.  rotary.dims == 0: nothing is
  * turned.  Keys at x < 0, beyond the table, or on a page outside 0 .. pages - 1 are not written (so a
  * table entry of -1 keeps a padded row out of the cache); the queries of such rows are written all the

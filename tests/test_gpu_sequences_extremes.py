@@ -4,9 +4,9 @@ import numpy as np
 import pytest
 import torch
 
-from adrastea_amd import PackedBatch
+from adrastea_amd import PackedBatch, Rotary, _ffi
 import sequences_reference as ref
-from test_gpu_sequences import CAUSAL, NONE, Packed, dev, heads_view, kern, shared_keys  # noqa: F401 (fixtures)
+from test_gpu_sequences import CAUSAL, NONE, Packed, Paged, dev, heads_view, kern, shared_keys  # noqa: F401 (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -143,3 +143,20 @@ def test_a_prompt_of_no_numbers_takes_no_longer(kern, what):  # noqa: F811
     (k if what == "key" else v)[7] = float("nan")
     assert fastest() < 20 * numbers
     assert out[7:].isnan().all() and out[:7].isfinite().all()
+
+
+def test_append_of_no_query_heads():
+    """With addresses of queries, but no heads of them, the keys and values go to their pages as without."""
+    p = Paged([(3, 20), (1, 17)], 4, 2, 64, 16, seed=21)
+    key, value = torch.randn(2, p.rows, 2, 64, dtype=torch.float16, device="cuda")
+    rotary = Rotary.new(64)
+    rows = (1, 128, 64)  # strides of key and value
+    written = []
+    for q in (None, p.q_t.data_ptr()):
+        p.k_t.zero_(), p.v_t.zero_()
+        rc = _ffi.lib().adr_append_f16(torch.cuda.current_stream().cuda_stream, p.cache._desc, p.batch._desc, key.data_ptr(),
+                                       value.data_ptr(), q, q, None, rotary._desc, 0, p.rows, *rows, *rows, 1, 256, 64, 1, 256, 64)
+        assert rc == 0
+        written.append((p.k_t.clone(), p.v_t.clone()))
+    for without, with_address in zip(*written):
+        assert torch.equal(without, with_address) and without.any()

@@ -156,3 +156,14 @@ def test_a_factor_of_the_scores_out_of_range(scale, temp):
 def test_the_ends_of_its_range(scale, temp):
     """Accepted as far as the arguments go: without a GPU, what is refused is the device."""
     assert paged(scale=scale, temp=temp) not in (0, LAYOUT) and packed(scale=scale, temp=temp) not in (0, LAYOUT)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are not real")
+def test_append_of_no_query_heads_is_no_call_of_nothing():
+    """Keys and values are there to be written: without a GPU, that is an error of the device and not a success."""
+    lib = _ffi.lib()
+    r = _ffi.RotaryDesc(P, 64, 0, 1.0)
+    strides = (1, 64, 320) * 4
+    without = lib.adr_append_f16(None, cache(), batch(), P, P, None, None, None, r, 0, 5, *strides)
+    assert without not in (0, SHAPE, NULL) and lib.adr_append_f16(None, cache(), batch(), P, P, P, P, None, r, 0, 5, *strides) == without
+    assert lib.adr_append_f16(None, cache(kv_heads=0), batch(), P, P, P, P, None, r, 0, 5, *strides) == 0
