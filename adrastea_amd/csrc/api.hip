@@ -902,7 +902,9 @@ int paged_args(SequencesArgs& a, const adr_paged_cache& c, const adr_paged_batch
   a.k = (const half_t*)c.key, a.v = (const half_t*)c.value;
   a.sk = {c.stride_kx, c.stride_ky, c.stride_kz, c.stride_kp};
   a.sv = {c.stride_vx, c.stride_vy, c.stride_vz, c.stride_vp};
-  a.row_offsets = b.row_offsets, a.keys_of = b.lengths, a.table = b.table;
+  static const int32_t unknown = 0;
+  a.row_offsets = b.row_offsets, a.keys_of = b.lengths;
+  a.table = b.table ? b.table : &unknown;  // (says that the keys are in pages; no launch is given it)
   a.sequences = b.sequences, a.rows = rows;
   a.heads = heads, a.kv_heads = c.kv_heads, a.group = heads / c.kv_heads, a.d = c.d;
   a.table_width = b.table_width, a.table_pitch = b.table_pitch, a.pages = c.pages, a.page_size = c.page_size;
@@ -945,7 +947,7 @@ int attention_paged(adr_stream_t stream, uint16_t* output, const uint16_t* query
       (cache.pages > 0 && (!cache.key || !cache.value)))
     return ADR_ENULL;
   if (!words(batch.row_offsets) || !words(batch.lengths) || !words(batch.table)) return ADR_EUNSUPPORTED_LAYOUT;
-  if (!a.table) a.table = batch.lengths;  // (of no entries: it only says that the keys are in pages)
+  if (!batch.table) a.table = batch.lengths;  // (of no entries)
   set_rows(a, output, query, o, q, scale, temp, mask);
   return attention_of_rows((hipStream_t)stream, a, scale, temp, held, workspace, workspace_bytes);
 }

@@ -167,3 +167,15 @@ def test_append_of_no_query_heads_is_no_call_of_nothing():
     without = lib.adr_append_f16(None, cache(), batch(), P, P, None, None, None, r, 0, 5, *strides)
     assert without not in (0, SHAPE, NULL) and lib.adr_append_f16(None, cache(), batch(), P, P, P, P, None, r, 0, 5, *strides) == without
     assert lib.adr_append_f16(None, cache(kv_heads=0), batch(), P, P, P, P, None, r, 0, 5, *strides) == 0
+
+
+def test_workspace_bytes_before_there_is_a_table():
+    """Sizes are enough to ask: the addresses of a batch that is yet to be allocated change nothing."""
+    lib = _ffi.lib()
+    for heads, rows, sequences, width in ((32, 1, 1, 500), (32, 16, 16, 250), (32, 256, 1, 600), (8, 5, 3, 2)):
+        c = cache(pages=10000, kv_heads=8 if heads == 32 else 2, d=128, ky=128, kz=2048, kp=16384)
+        sizes = dict(sequences=sequences, table_width=width, table_pitch=width)
+        want = lib.adr_attention_paged_f16_workspace_bytes(c, batch(**sizes), heads, rows)
+        unknown = batch(row_offsets=None, lengths=None, table=None, **sizes)
+        assert lib.adr_attention_paged_f16_workspace_bytes(c, unknown, heads, rows) == want
+        assert want > 0 or heads == 8
