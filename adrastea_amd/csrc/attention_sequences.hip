@@ -26,8 +26,9 @@ constexpr float BELOW = 7.0f, GROWN = 15.0f;
 // s c - R is one fma, exact but for its last step, but the largest s c is itself rounded: at 2^31 by up to 2^7, so that the
 // largest probability could be 2^128 or 2^-128.  A step above what was found, it is no smaller than it should be at least, and no
 // probability or sum is infinite that should not be; rows whose R is beyond FAR_SCORE in the end, where it can be larger by
-// more than 2, are computed again by row_by_wave.
+// more than 2, are computed again by row_by_wave.  (An infinite one has made the row NaN, as it should be.)
 constexpr float FAR_SCORE = 0x1p24f;
+__device__ __forceinline__ bool is_far(float r) { return fabsf(r) > FAR_SCORE && fabsf(r) < INFINITY; }
 __device__ __forceinline__ float above(float top) { return fmaf(fabsf(top), 0x1p-23f, top); }
 
 // A weighted mean of values, rounded to fp16.  Its weights are off by up to 2^-11 each (fp16 in the second product, 32 bits in their
@@ -754,7 +755,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
       half4_t v;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       if (!round_means(v, sum, inv)) atomicOr(bad_rows, 1 << r);
-      if (col < z.d && fabsf(m_all) <= FAR_SCORE)
+      if (col < z.d && !is_far(m_all))
         *(half4_t*)(z.out + (int64_t)h * z.so_z + (int64_t)(q.row0 + token) * z.so_y + col) = v;
     } else {
       const int64_t prow = ((int64_t)(2 * wg + (place != stretch0)) * z.kv_heads + hk) * ROWS + r;
@@ -766,7 +767,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
     float m_all = NO_SCORE;
 #pragma unroll
     for (int x = 0; x < WAVES; x++) m_all = fmaxf(m_all, xml[x * 16 + frow].x);
-    int again = (int)__ballot(fabsf(m_all) > FAR_SCORE);  // (not stored above)
+    int again = (int)__ballot(is_far(m_all));  // (not stored above)
     if (q.rows > 1 && z.mask == ADR_MASK_CAUSAL) {
       __syncthreads();
       const int bad = uniform(*bad_rows);
@@ -1343,7 +1344,7 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
       if (head >= z.group) head -= z.group, token++;
     }
     // Rows that are computed again, a group's columns of them.
-    const uint64_t wrong = __ballot(!finite), far = __ballot(fabsf(m_run) > FAR_SCORE);
+    const uint64_t wrong = __ballot(!finite), far = __ballot(is_far(m_run));
     if ((wrong | far) && wave_rows > 0) {
       uint32_t again = (uint32_t)far | (uint32_t)(far >> 32);
       const uint32_t bad = (uint32_t)wrong | (uint32_t)(wrong >> 32);
@@ -1443,7 +1444,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Job) {
     half4_t out;
     const bool finite = round_means(out, acc, l == 0.0f ? 0.0f : 1.0f / l);
     if (!finite) atomicOr(&bad_rows, 1 << (r - r0));
-    if (fabsf(m) > FAR_SCORE) atomicOr(&bad_rows, 0x10000 << (r - r0));
+    if (is_far(m)) atomicOr(&bad_rows, 0x10000 << (r - r0));
     if (col < a.d) *(half4_t*)(a.out + (int64_t)h * a.so_z + (int64_t)(b.q.row0 + token) * a.so_y + col) = out;
   }
   __syncthreads();

@@ -119,7 +119,7 @@ def test_no_numbers_before_and_behind_a_row(shared_keys, rows, keys, seen, hidde
     assert ref.close_enough(got, want, np.abs(clean[:-1].astype(np.float64)).max(), keys)
 
 
-@pytest.mark.parametrize("what", ["key", "value"])
+@pytest.mark.parametrize("what", ["key", "value", "score"])
 def test_a_prompt_of_no_numbers_takes_no_longer(kern, what):  # noqa: F811
     """Rows that come out as NaN because they see one are not computed twice: 500 times the time when they were."""
     n, heads, kv, d = 4096, 32, 8, 128
@@ -140,7 +140,11 @@ def test_a_prompt_of_no_numbers_takes_no_longer(kern, what):  # noqa: F811
             times.append(begin.elapsed_time(end))
         return min(times)
     numbers = fastest()
-    (k if what == "key" else v)[7] = float("nan")
+    if what == "score":   # (infinite, of every row)
+        q[:, :, 0] = q[:, :, 0].abs() + 1.0
+        k[7, :, 0] = float("inf")
+    else:
+        (k if what == "key" else v)[7] = float("nan")
     assert fastest() < 20 * numbers
     assert out[7:].isnan().all() and out[:7].isfinite().all()
 
@@ -160,3 +164,19 @@ def test_append_of_no_query_heads():
         written.append((p.k_t.clone(), p.v_t.clone()))
     for without, with_address in zip(*written):
         assert torch.equal(without, with_address) and without.any()
+
+
+@pytest.mark.parametrize("mask", [CAUSAL, NONE], ids=["causal", "full"])
+@pytest.mark.parametrize("rows,keys", [(1, 300), (40, 300), (200, 210)])
+def test_infinite_scores(shared_keys, rows, keys, mask):
+    """A score of +inf leaves no number in the rows that see it; one of -inf is a key that weighs nothing."""
+    p = Packed([(rows, keys), (3, 50)], 4, 2, 64, seed=keys)
+    p.q[:, :, 0] = np.abs(p.q[:, :, 0]) + np.float16(1.0)
+    at = keys - rows + rows // 2      # (which half of the rows see)
+    p.k[at, :, 0], p.k[3, :, 0] = np.inf, -np.inf
+    got = packed_call(shared_keys, p, 0.125, mask)
+    seen = np.zeros(p.row_offsets[-1], bool)
+    seen[rows // 2 if mask == CAUSAL else 0:rows] = True
+    assert np.isnan(got[seen]).all() and np.isfinite(got[~seen]).all()
+    want = p.want(0.125, mask)[:p.row_offsets[-1]]
+    assert ref.close_enough(got[~seen], want[~seen], np.abs(p.v[:-1].astype(np.float64)).max(), keys)
