@@ -457,12 +457,13 @@ struct Rows {
 };
 bool read_rows(PyObject* view, int64_t device, Rows& r) {
   Layout l;
-  if ((PyObject*)Py_TYPE(view) != view_type || !read_layout(view, l) || (l.rank != 2 && l.rank != 3) || !read_ptr(view, r.ptr))
-    return false;
-  const Ref storage(attr(view, s_storage));
-  if (!storage.p || !on_device(storage, device)) return false;
+  if ((PyObject*)Py_TYPE(view) != view_type || !read_layout(view, l) || (l.rank != 2 && l.rank != 3)) return false;
+  const Ref storage(attr(view, s_storage)), offset(attr(view, s_offset));
   const Ref type(attr(storage, s_dtype));
-  if (type.p != float16_type) return false;  // (others that are let pass go the general way)
+  int64_t address, at;
+  if (!type.p || type.p != float16_type) return false;  // (others that are let pass go the general way)
+  if (!on_device(storage, device) || !call_int(storage, s_data_ptr, address) || !as_int(offset, at)) return false;
+  r.ptr = (void*)(uintptr_t)(address + at * 2);
   for (int i = 0; i < l.rank; i++)
     if (l.dims[i] > INT32_MAX || l.strides[i] > INT32_MAX || l.strides[i] < INT32_MIN) return false;
   r.heads = l.rank == 3 ? (int32_t)l.dims[0] : 1;

@@ -343,3 +343,13 @@ def test_bits_of_fp16(both, dtype):
     x = TensorView(torch.zeros(2, 6, 64, dtype=dtype), TensorLayout((6, 2, 64), (64, 384, 1)))
     native, general = both("rotary_f16", x, x, ints(4, 5), rotary())
     assert native is None and general.split()[-9:] == ["6", "2", "64", "1", "384", "64", "1", "384", "64"]
+
+
+def test_views_that_begin_inside_their_storage(both):
+    """As query, key and value views of one projection are."""
+    qkv = TensorView.of(half(2, 10, 64)).permute([1, 0, 2])
+    q, k, v = qkv.take([6, -1, -1]), qkv.skip([6, 0, 0]).take([2, -1, -1]), qkv.skip([8, 0, 0])
+    same(both("append_f16", cache(), batch(), k, v, rotary(), q, q, None))
+    p = PackedBatch(ints(0, 1, 2), ints(0, 1, 2))
+    seen = same(both("attention_packed_f16", q, q, k, v, p, 0.1, 1.0, 1)).split()
+    assert [int(x, 16) - int(seen[2], 16) for x in seen[3:5]] == [6 * 64 * 2, 8 * 64 * 2]
