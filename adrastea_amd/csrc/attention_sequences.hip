@@ -483,7 +483,7 @@ __device__ __forceinline__ u32x4_t descriptor(uint64_t p, int bytes) {
 //
 // Bound by memory: 16 rows of every key read once leave the matrix cores 5 % busy.  64 sequences of 3 to 4000 keys (32 / 8
 // heads of 128, 504 MB) 88.2 us = 5.7 TB/s, eight of 50000 to 110000 (40 / 8, 2.36 GB) 365 us = 6.4 TB/s, where a plain read
-// reaches 7.0 to 7.3; one of 777 keys (32 / 32) 9.5 us, of which two launches are 8.8 on the host.
+// reaches 7.0 to 7.3; one of 777 keys (32 / 32) 9.6 to 10.4 us, of which two launches are 8.8 on the host.
 template <int HD, bool PAGED, int WAVES, bool SHARED>
 __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) {
   constexpr int CPR = HD / 8, KEYS = 32, ROWS = 16;
@@ -803,14 +803,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
 // GROUPS == 2: eight wavefronts, of which four take the first half of the block's keys and four the second, each through
 // tiles of its own; both ends meet in LDS.  Two workgroups beside each other do as much, but that takes twice as many blocks,
 // or parts that go through memory: 1024 rows over 8025 keys (256 blocks) 134 us, by halves through memory 143, one group on
-// each compute unit 144.
+// each compute unit 144 (all three on one machine).
 //
-// Bound by power, and by issue as in attention_fwd_kernel: one prompt of 16384 rows (32 / 8 heads of 128) 2001 us = 1099
-// TFLOP/s with the matrix cores busy 69 % of cycles at 1.6 GHz, where a product of 8192^3 reaches 1408.  Short blocks are
+// Bound by issue as in attention_fwd_kernel, and where all is loop by power: one prompt of 16384 rows (32 / 8 heads of 128) 2006
+// to 2196 us by machine = 1096 to 1000 TFLOP/s, with the matrix cores busy 69 % of cycles at 1.6 GHz, where a product of 8192^3
+// reaches 1408.  The 256 blocks above, two groups each, leave some of that power: 53 % at 1.8 GHz, 136 to 146 us.  Short blocks are
 // bound by their beginnings and ends: us of a block among others, 2.0 from the end of one to the start of the next in its place,
 // 1.4 to find its sequence, 1.7 for addresses, 1.8 until the first keys are there, 1.9 a tile, 2.4 for the results.  Nine prompts
-// of 100 to 3996 rows, 25 tiles a block in the mean, 436 us = 957 TFLOP/s (what wavefronts whose rows end early, and rows that
-// the mask hides, compute of a tile is in the time and not in the operations).
+// of 100 to 3996 rows, 25 tiles a block in the mean, 447 to 477 us = 933 to 874 TFLOP/s (what wavefronts whose rows end early, and
+// rows that the mask hides, compute of a tile is in the time and not in the operations).  HD = 128 keeps 24 to 38 vector registers
+// in scratch memory at those beginnings and ends, none in the loop; HD = 64 none.
 template <int HD, bool PAGED, bool SHARED, int GROUPS>
 __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
   constexpr int CPR = HD / 8, KEYS = 64, ROWS = 128;

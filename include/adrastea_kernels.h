@@ -395,8 +395,8 @@ int64_t adr_attention_f16_workspace_bytes(int32_t heads, int32_t m, int32_t n, i
  * Rows are packed: sequence s has rows row_offsets[s] .. row_offsets[s + 1] - 1 of the [heads, rows, d]
  * views (strides x = dim -1, y = dim -2, z = dim -3 as above, any strides, negative ones included).
  * Offsets are clamped to 0 .. rows and do not decrease (where they do, rows that several sequences claim,
- * or none, hold any of their results, or none); a sequence may have no rows; rows in front of the first
- * and behind the last sequence are neither read nor written.
+ * or none, hold any of their results, or none); a sequence may have no rows; what rows in front of the first
+ * and behind the last sequence hold does not matter, and they are not written.
  *
  * adr_paged_cache: key and value pages as [pages, kv_heads, page_size, d] views of one pool each,
  * strides in elements (x value, y slot, z head, p page), 64 bits.
@@ -475,7 +475,9 @@ int adr_append_f16(adr_stream_t stream, adr_paged_cache cache, adr_paged_batch b
  * sees all keys) and all x under ADR_MASK_NONE.  A row that sees no key, or whose scores are all -inf
  * while its values are finite, becomes zeros; keys that a row does not see, and slots behind the last key, never reach it, whatever they
  * hold (infinities and NaN included).  A key on a page outside 0 .. pages - 1 counts as NaN for the rows
- * that see it.  Scores, softmax and sums in fp32; probabilities are rounded to fp16 for the matrix cores.
+ * that see it.  Scores, softmax and sums in fp32; probabilities are rounded to fp16 for the matrix cores (2^-11 of each; below
+ * 2^-21 of a row's largest, 2^-32 of that).  Finite operands give finite results, whatever the size of the scores; rows with scores beyond
+ * 2^24 / log2(e), and rows beside a hidden value that is not finite, are slow.
  * `output` overlaps none of the others.
  * d 1 .. 256, scale > 0, temp > 0, scale / temp 2^-126 .. 2^58 (ADR_EUNSUPPORTED_LAYOUT beyond), heads a multiple of kv_heads.  The fast
  * kernels take d a multiple of 8 up to 128, x strides 1, the others multiples of 8 and not negative, slots at
