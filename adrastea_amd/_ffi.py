@@ -23,6 +23,9 @@ SYMBOLS = (
     "adr_rotary_f16", "adr_append_f16",
     "adr_attention_paged_f16", "adr_attention_paged_f16_ws", "adr_attention_paged_f16_workspace_bytes",
     "adr_attention_packed_f16", "adr_attention_packed_f16_ws", "adr_attention_packed_f16_workspace_bytes",
+    "adr_norm_rotary_f16", "adr_append_norm_f16", "adr_append_u8", "adr_read_u8",
+    "adr_attention_paged_u8", "adr_attention_paged_u8_ws", "adr_attention_paged_u8_workspace_bytes",
+    "adr_attention_tree_f16", "adr_attention_tree_f16_ws", "adr_attention_tree_u8", "adr_attention_tree_u8_ws",
     "adr_debug_knob", "adr_microbench_empty", "adr_microbench_mfma_f16", "adr_microbench_stream_read",
     "adr_strerror", "adr_abi_version",
 )
@@ -33,6 +36,7 @@ ADR_EUNSUPPORTED_DEVICE, ADR_EUNSUPPORTED_LAYOUT, ADR_ESCRATCH = -6, -7, -8
 KNOB_GEMM_TILE = 0
 NOALLOC_SCRATCH_BYTES = 16 * 1024 * 1024
 HELD_WORKSPACE_DEFAULT_BYTES = 128 * 1024 * 1024
+ROTARY_MAX_AXES = 8
 
 
 class TensorDesc(C.Structure):
@@ -63,6 +67,30 @@ class PackedBatchDesc(C.Structure):
 class RotaryDesc(C.Structure):
     """adr_rotary"""
     _fields_ = [("turns", C.c_void_p), ("dims", C.c_int32), ("layout", C.c_uint32), ("magnitude", C.c_float)]
+
+
+class RotaryAxesDesc(C.Structure):
+    """adr_rotary_axes"""
+    _fields_ = [("turns", C.c_void_p), ("axis", C.c_void_p), ("dims", C.c_int32), ("layout", C.c_uint32), ("magnitude", C.c_float),
+                ("axes", C.c_int32)]
+
+
+class HeadNormDesc(C.Structure):
+    """adr_head_norm"""
+    _fields_ = [("weight", C.c_void_p), ("eps", C.c_float)]
+
+
+class PagedCacheU8Desc(C.Structure):
+    """adr_paged_cache_u8"""
+    _fields_ = [*((f, C.c_void_p) for f in ("key", "key_scale", "value", "value_scale")),
+                *((f, C.c_int32) for f in ("pages", "kv_heads", "page_size", "d")),
+                *((f"stride_{t}{s}", C.c_int64) for t in "kv" for s in "xyzp"),
+                *((f"stride_{t}s{s}", C.c_int64) for t in "kv" for s in "yzp")]
+
+
+class DraftTreeDesc(C.Structure):
+    """adr_draft_tree"""
+    _fields_ = [("bits", C.c_void_p), ("words", C.c_int32), ("pitch", C.c_int32)]
 
 
 _lib = None
@@ -133,6 +161,18 @@ def lib():
     L.adr_attention_packed_f16.argtypes = [vp, vp, vp, vp, vp, packed] + [i32] * 17 + [f32, f32, u32]
     L.adr_attention_packed_f16_ws.argtypes = L.adr_attention_packed_f16.argtypes + [vp, C.c_int64]
     L.adr_attention_packed_f16_workspace_bytes.argtypes = [packed] + [i32] * 5
+    codes, axes, norm, tree = PagedCacheU8Desc, RotaryAxesDesc, HeadNormDesc, DraftTreeDesc
+    L.adr_norm_rotary_f16.argtypes = [vp, vp, vp, vp, i32, axes, norm] + [i32] * 9
+    L.adr_append_norm_f16.argtypes = [vp, cache, batch, vp, vp, vp, vp, vp, i32, axes, norm, norm] + [i32] * 14
+    L.adr_append_u8.argtypes = [vp, codes, batch, vp, vp, vp, vp, vp, i32, axes, norm, norm] + [i32] * 14
+    L.adr_read_u8.argtypes = [vp, vp, vp, codes, batch] + [i32] * 7
+    L.adr_attention_paged_u8.argtypes = [vp, vp, vp, codes, batch] + [i32] * 8 + [f32, f32, u32]
+    L.adr_attention_paged_u8_ws.argtypes = L.adr_attention_paged_u8.argtypes + [vp, C.c_int64]
+    L.adr_attention_paged_u8_workspace_bytes.argtypes = [codes, batch, i32, i32]
+    L.adr_attention_tree_f16.argtypes = [vp, vp, vp, cache, batch, tree] + [i32] * 8 + [f32, f32]
+    L.adr_attention_tree_f16_ws.argtypes = L.adr_attention_tree_f16.argtypes + [vp, C.c_int64]
+    L.adr_attention_tree_u8.argtypes = [vp, vp, vp, codes, batch, tree] + [i32] * 8 + [f32, f32]
+    L.adr_attention_tree_u8_ws.argtypes = L.adr_attention_tree_u8.argtypes + [vp, C.c_int64]
     L.adr_strerror.argtypes = [C.c_int]
     L.adr_strerror.restype = C.c_char_p
     L.adr_abi_version.restype = C.c_int
@@ -143,6 +183,7 @@ def lib():
     L.adr_attention_f16_workspace_bytes.restype = C.c_int64
     L.adr_attention_paged_f16_workspace_bytes.restype = C.c_int64
     L.adr_attention_packed_f16_workspace_bytes.restype = C.c_int64
+    L.adr_attention_paged_u8_workspace_bytes.restype = C.c_int64
     L.adr_held_workspace_limit.restype = C.c_int64
     L.adr_held_workspace_bytes.restype = C.c_int64
     L.adr_held_workspace_declined.restype = C.c_int64

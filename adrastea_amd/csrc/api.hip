@@ -6,6 +6,7 @@
 #include <mutex>
 
 #include "adr_common.hpp"
+#include "append.hpp"
 #include "sequences.hpp"
 
 using namespace adr;
@@ -851,7 +852,8 @@ int validate_rows(int32_t heads, int32_t kv_heads, int32_t rows, int32_t d, int3
   return ADR_OK;
 }
 
-int validate_cache(const adr_paged_cache& c, const adr_paged_batch& b) {
+extern "C++" template <typename Cache>
+int validate_cache(const Cache& c, const adr_paged_batch& b) {
   if (c.pages < 0 || c.page_size < 0 || b.table_width < 0 || b.table_pitch < b.table_width) return ADR_EINVAL_SHAPE;
   if (c.page_size == 0 && b.table_width > 0) return ADR_EINVAL_SHAPE;
   return ADR_OK;
@@ -877,11 +879,13 @@ int attention_of_rows(hipStream_t stream, const SequencesArgs& a, float scale, f
   if (a.d > 256 || !factor_fits(scale, temp)) return ADR_EUNSUPPORTED_LAYOUT;
   const DeviceInfo dev = device_info();
   if (dev.status) return dev.status;
+  const bool u8 = a.k_scale != nullptr;
   auto launch = [&](const SequencesPlan& plan, void* scratch) {
-    return (int)launch_attention_sequences(stream, a, plan, scratch);
+    return (int)(u8 ? launch_attention_u8(stream, a, plan, scratch) : launch_attention_sequences(stream, a, plan, scratch));
   };
-  if (!held) return launch(sequences_plan(a, dev.cus, workspace_bytes), workspace);
-  const SequencesPlan plan = sequences_plan(a, dev.cus, held_limit.load(std::memory_order_relaxed));
+  auto plan_with = [&](int64_t bytes) { return u8 ? sequences_u8_plan(a, dev.cus, bytes) : sequences_plan(a, dev.cus, bytes); };
+  if (!held) return launch(plan_with(workspace_bytes), workspace);
+  const SequencesPlan plan = plan_with(held_limit.load(std::memory_order_relaxed));
   if (plan.workspace_bytes == 0) return launch(plan, nullptr);
   if (held_allowed(stream)) {
     std::lock_guard<std::mutex> lock(held_mutex);
@@ -891,17 +895,30 @@ int attention_of_rows(hipStream_t stream, const SequencesArgs& a, float scale, f
       return rc;
     }
   }
-  return launch(sequences_plan(a, dev.cus, 0), nullptr);
+  return launch(plan_with(0), nullptr);
 }
 
-int paged_args(SequencesArgs& a, const adr_paged_cache& c, const adr_paged_batch& b, int32_t heads, int32_t rows,
-               bool* nothing) {
+extern "C++" bool complete(const adr_paged_cache& c) { return c.pages == 0 || (c.key && c.value); }
+extern "C++" bool complete(const adr_paged_cache_u8& c) { return c.pages == 0 || (c.key && c.value && c.key_scale && c.value_scale); }
+
+extern "C++" void set_scales(SequencesArgs&, const adr_paged_cache&) {}
+extern "C++" void set_scales(SequencesArgs& a, const adr_paged_cache_u8& c) {
+  static const half_t none = 0;
+  a.k_scale = c.key_scale ? (const half_t*)c.key_scale : &none;  // (says that there are codes; nothing reads it)
+  a.v_scale = (const half_t*)c.value_scale;
+  a.sks = {0, c.stride_ksy, c.stride_ksz, c.stride_ksp};
+  a.svs = {0, c.stride_vsy, c.stride_vsz, c.stride_vsp};
+}
+
+extern "C++" template <typename Cache>
+int paged_args(SequencesArgs& a, const Cache& c, const adr_paged_batch& b, int32_t heads, int32_t rows, bool* nothing) {
   if (int rc = validate_rows(heads, c.kv_heads, rows, c.d, b.sequences, nothing)) return rc;
   if (int rc = validate_cache(c, b)) return rc;
   if (*nothing) return ADR_OK;
   a.k = (const half_t*)c.key, a.v = (const half_t*)c.value;
   a.sk = {c.stride_kx, c.stride_ky, c.stride_kz, c.stride_kp};
   a.sv = {c.stride_vx, c.stride_vy, c.stride_vz, c.stride_vp};
+  set_scales(a, c);
   static const int32_t unknown = 0;
   a.row_offsets = b.row_offsets, a.keys_of = b.lengths;
   a.table = b.table ? b.table : &unknown;  // (says that the keys are in pages; no launch is given it)
@@ -933,18 +950,25 @@ void set_rows(SequencesArgs& a, uint16_t* output, const uint16_t* query, const i
   a.mask = mask;
 }
 
-int attention_paged(adr_stream_t stream, uint16_t* output, const uint16_t* query, const adr_paged_cache& cache,
+extern "C++" template <typename Cache>
+int attention_paged(adr_stream_t stream, uint16_t* output, const uint16_t* query, const Cache& cache,
                     const adr_paged_batch& batch, int32_t heads, int32_t rows, const int32_t (&o)[3],
                     const int32_t (&q)[3], float scale, float temp, uint32_t mask, bool held, void* workspace,
-                    int64_t workspace_bytes) {
+                    int64_t workspace_bytes, const adr_draft_tree* tree = nullptr) {
   SequencesArgs a = {};
   bool nothing;
   if (int rc = paged_args(a, cache, batch, heads, rows, &nothing)) return rc;
-  if (mask > ADR_MASK_CAUSAL) return ADR_EINVAL_ENUM;
+  if (!tree && mask > ADR_MASK_CAUSAL) return ADR_EINVAL_ENUM;
+  if (tree && (tree->words < 0 || tree->pitch < tree->words)) return ADR_EINVAL_SHAPE;
   if (nothing) return ADR_OK;
+  if (tree) {
+    if (tree->words > 0 && !tree->bits) return ADR_ENULL;
+    if (!words(tree->bits)) return ADR_EUNSUPPORTED_LAYOUT;
+    mask = MASK_TREE;
+    a.tree = tree->bits, a.tree_words = tree->words, a.tree_pitch = tree->pitch;
+  }
   // (a cache without pages, or a table without entries, need not exist)
-  if (!output || !query || !batch.row_offsets || !batch.lengths || (batch.table_width > 0 && !batch.table) ||
-      (cache.pages > 0 && (!cache.key || !cache.value)))
+  if (!output || !query || !batch.row_offsets || !batch.lengths || (batch.table_width > 0 && !batch.table) || !complete(cache))
     return ADR_ENULL;
   if (!words(batch.row_offsets) || !words(batch.lengths) || !words(batch.table)) return ADR_EUNSUPPORTED_LAYOUT;
   if (!batch.table) a.table = batch.lengths;  // (of no entries)
@@ -1095,6 +1119,177 @@ int64_t adr_attention_packed_f16_workspace_bytes(adr_packed_batch batch, int32_t
   a.sk = a.sv = {1, d, 0, 0};
   return nothing ? 0 : sequences_plan(a, device_info_for_plan().cus, INT64_MAX).workspace_bytes;
 }
+
+namespace {
+
+int validate_axes(const adr_rotary_axes& r, int32_t d, const int32_t* positions, int32_t pitch, int32_t rows) {
+  if (int rc = validate_rotary(adr_rotary{r.turns, r.dims, r.layout, r.magnitude}, d)) return rc;
+  if (r.axes < 1 || r.axes > ADR_ROTARY_MAX_AXES) return ADR_EINVAL_SHAPE;
+  return positions && r.axes > 1 && pitch < rows ? ADR_EINVAL_SHAPE : ADR_OK;
+}
+
+bool eps_fits(const adr_head_norm& n) { return !n.weight || (n.eps >= 0.0f && n.eps <= 3.402823466e38f); }
+
+void set_turns(PlaceArgs& a, const adr_rotary_axes& r, const int32_t* positions, int32_t pitch) {
+  a.positions = positions, a.positions_pitch = pitch;
+  a.turns = r.turns, a.axis = r.axes > 1 ? r.axis : nullptr, a.axes = r.axes;
+  a.dims = r.dims, a.pairs = r.layout == ADR_ROTARY_PAIRS, a.magnitude = r.magnitude;
+}
+
+// What the kernels read as such, at its natural alignment.
+bool turns_aligned(const adr_rotary_axes& r, const int32_t* positions) {
+  return words(positions) && words(r.axis) && (uintptr_t)r.turns % 8 == 0;
+}
+
+extern "C++" template <typename Cache>
+int append_normed(adr_stream_t stream, const Cache& cache, PlaceArgs& a, const adr_paged_batch& batch, const uint16_t* key,
+                  const uint16_t* value, uint16_t* query_out, const uint16_t* query, const int32_t* positions,
+                  int32_t positions_pitch, const adr_rotary_axes& rotary, const adr_head_norm& query_norm,
+                  const adr_head_norm& key_norm, int32_t heads, int32_t rows, const int32_t (&k)[3], const int32_t (&v)[3],
+                  const int32_t (&o)[3], const int32_t (&q)[3]) {
+  bool nothing;
+  if (heads == 0) query = query_out = nullptr;
+  if (!query && !query_out) heads = cache.kv_heads;  // (no queries: their number does not count)
+  if (int rc = validate_rows(heads, cache.kv_heads, rows, cache.d, batch.sequences, &nothing)) return rc;
+  if (int rc = validate_cache(cache, batch)) return rc;
+  if (int rc = validate_axes(rotary, cache.d, positions, positions_pitch, rows)) return rc;
+  if (!eps_fits(key_norm) || (query && !eps_fits(query_norm))) return ADR_EINVAL_SHAPE;
+  if (nothing) return ADR_OK;
+  if (!key || !value || !query != !query_out || !batch.row_offsets || !batch.lengths ||
+      (batch.table_width > 0 && !batch.table) || !complete(cache) || (rotary.dims > 0 && !rotary.turns))
+    return ADR_ENULL;
+  if (!words(batch.row_offsets) || !words(batch.lengths) || !words(batch.table) || !turns_aligned(rotary, positions))
+    return ADR_EUNSUPPORTED_LAYOUT;
+  if (int rc = check_device()) return rc;
+  a.q_out = (half_t*)query_out, a.q = (const half_t*)query;
+  a.so_x = o[0], a.so_y = o[1], a.so_z = o[2];
+  a.sq_x = q[0], a.sq_y = q[1], a.sq_z = q[2];
+  a.k = (const half_t*)key, a.v = (const half_t*)value;
+  a.sk_x = k[0], a.sk_y = k[1], a.sk_z = k[2];
+  a.sv_x = v[0], a.sv_y = v[1], a.sv_z = v[2];
+  set_turns(a, rotary, positions, positions_pitch);
+  if (query) a.q_weight = (const half_t*)query_norm.weight, a.q_eps = query_norm.eps;
+  a.k_weight = (const half_t*)key_norm.weight, a.k_eps = key_norm.eps;
+  a.heads = query ? heads : 0, a.kv_heads = cache.kv_heads, a.rows = rows, a.d = cache.d;
+  a.batch = batch;
+  return (int)launch_place((hipStream_t)stream, a);
+}
+
+}  // namespace
+
+int adr_norm_rotary_f16(adr_stream_t stream, uint16_t* output, const uint16_t* input, const int32_t* positions,
+                        int32_t positions_pitch, adr_rotary_axes rotary, adr_head_norm norm, int32_t heads, int32_t rows,
+                        int32_t d, int32_t stride_ox, int32_t stride_oy, int32_t stride_oz, int32_t stride_ix,
+                        int32_t stride_iy, int32_t stride_iz) {
+  bool nothing;
+  if (int rc = validate_rows(heads, heads, rows, d, 1, &nothing)) return rc;
+  if (int rc = validate_axes(rotary, d, positions, positions_pitch, rows)) return rc;
+  if (!eps_fits(norm)) return ADR_EINVAL_SHAPE;
+  if (nothing) return ADR_OK;
+  if (!output || !input || (rotary.dims > 0 && (!positions || !rotary.turns))) return ADR_ENULL;
+  if (!turns_aligned(rotary, positions)) return ADR_EUNSUPPORTED_LAYOUT;
+  if (int rc = check_device()) return rc;
+  PlaceArgs a = {};
+  a.q_out = (half_t*)output, a.q = (const half_t*)input;
+  a.so_x = stride_ox, a.so_y = stride_oy, a.so_z = stride_oz;
+  a.sq_x = stride_ix, a.sq_y = stride_iy, a.sq_z = stride_iz;
+  set_turns(a, rotary, positions, positions_pitch);
+  a.q_weight = (const half_t*)norm.weight, a.q_eps = norm.eps;
+  a.heads = heads, a.rows = rows, a.d = d;
+  return (int)launch_place((hipStream_t)stream, a);
+}
+
+int adr_append_norm_f16(adr_stream_t stream, adr_paged_cache cache, adr_paged_batch batch, const uint16_t* key,
+                        const uint16_t* value, uint16_t* query_out, const uint16_t* query, const int32_t* positions,
+                        int32_t positions_pitch, adr_rotary_axes rotary, adr_head_norm query_norm, adr_head_norm key_norm,
+                        int32_t heads, int32_t rows, int32_t stride_kx, int32_t stride_ky, int32_t stride_kz,
+                        int32_t stride_vx, int32_t stride_vy, int32_t stride_vz, int32_t stride_ox, int32_t stride_oy,
+                        int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz) {
+  PlaceArgs a = {};
+  a.cache = cache;
+  return append_normed(stream, cache, a, batch, key, value, query_out, query, positions, positions_pitch, rotary, query_norm,
+                       key_norm, heads, rows, {stride_kx, stride_ky, stride_kz}, {stride_vx, stride_vy, stride_vz},
+                       {stride_ox, stride_oy, stride_oz}, {stride_qx, stride_qy, stride_qz});
+}
+
+int adr_append_u8(adr_stream_t stream, adr_paged_cache_u8 cache, adr_paged_batch batch, const uint16_t* key,
+                  const uint16_t* value, uint16_t* query_out, const uint16_t* query, const int32_t* positions,
+                  int32_t positions_pitch, adr_rotary_axes rotary, adr_head_norm query_norm, adr_head_norm key_norm,
+                  int32_t heads, int32_t rows, int32_t stride_kx, int32_t stride_ky, int32_t stride_kz, int32_t stride_vx,
+                  int32_t stride_vy, int32_t stride_vz, int32_t stride_ox, int32_t stride_oy, int32_t stride_oz,
+                  int32_t stride_qx, int32_t stride_qy, int32_t stride_qz) {
+  PlaceArgs a = {};
+  a.codes = cache, a.in_codes = true;
+  return append_normed(stream, cache, a, batch, key, value, query_out, query, positions, positions_pitch, rotary, query_norm,
+                       key_norm, heads, rows, {stride_kx, stride_ky, stride_kz}, {stride_vx, stride_vy, stride_vz},
+                       {stride_ox, stride_oy, stride_oz}, {stride_qx, stride_qy, stride_qz});
+}
+
+int adr_read_u8(adr_stream_t stream, uint16_t* key, uint16_t* value, adr_paged_cache_u8 cache, adr_paged_batch batch,
+                int32_t rows, int32_t stride_kx, int32_t stride_ky, int32_t stride_kz, int32_t stride_vx, int32_t stride_vy,
+                int32_t stride_vz) {
+  bool nothing;
+  if (int rc = validate_rows(cache.kv_heads, cache.kv_heads, rows, cache.d, batch.sequences, &nothing)) return rc;
+  if (int rc = validate_cache(cache, batch)) return rc;
+  if (nothing) return ADR_OK;
+  if (!key || !value || !batch.row_offsets || !batch.lengths || (batch.table_width > 0 && !batch.table) || !complete(cache))
+    return ADR_ENULL;
+  if (!words(batch.row_offsets) || !words(batch.lengths) || !words(batch.table)) return ADR_EUNSUPPORTED_LAYOUT;
+  if (int rc = check_device()) return rc;
+  ReadArgs a = {};
+  a.k = (half_t*)key, a.v = (half_t*)value;
+  a.sk_x = stride_kx, a.sk_y = stride_ky, a.sk_z = stride_kz;
+  a.sv_x = stride_vx, a.sv_y = stride_vy, a.sv_z = stride_vz;
+  a.rows = rows, a.cache = cache, a.batch = batch;
+  return (int)launch_read_u8((hipStream_t)stream, a);
+}
+
+int adr_attention_paged_u8(adr_stream_t stream, uint16_t* output, const uint16_t* query, adr_paged_cache_u8 cache,
+                           adr_paged_batch batch, int32_t heads, int32_t rows, int32_t stride_ox, int32_t stride_oy,
+                           int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz, float scale,
+                           float temp, uint32_t mask) {
+  return attention_paged(stream, output, query, cache, batch, heads, rows, {stride_ox, stride_oy, stride_oz},
+                         {stride_qx, stride_qy, stride_qz}, scale, temp, mask, true, nullptr, 0);
+}
+
+int adr_attention_paged_u8_ws(adr_stream_t stream, uint16_t* output, const uint16_t* query, adr_paged_cache_u8 cache,
+                              adr_paged_batch batch, int32_t heads, int32_t rows, int32_t stride_ox, int32_t stride_oy,
+                              int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz, float scale,
+                              float temp, uint32_t mask, void* workspace, int64_t workspace_bytes) {
+  if (int rc = validate_workspace(workspace, workspace_bytes)) return rc;
+  return attention_paged(stream, output, query, cache, batch, heads, rows, {stride_ox, stride_oy, stride_oz},
+                         {stride_qx, stride_qy, stride_qz}, scale, temp, mask, false, workspace, workspace_bytes);
+}
+
+int64_t adr_attention_paged_u8_workspace_bytes(adr_paged_cache_u8 cache, adr_paged_batch batch, int32_t heads,
+                                               int32_t rows) {
+  SequencesArgs a = {};
+  bool nothing;
+  if (int rc = paged_args(a, cache, batch, heads, rows, &nothing)) return rc;
+  a.so_x = a.sq_x = 1;
+  return nothing ? 0 : sequences_u8_plan(a, device_info_for_plan().cus, INT64_MAX).workspace_bytes;
+}
+
+#define ADR_TREE_ENTRIES(suffix, cache_t)                                                                                        \
+  int adr_attention_tree_##suffix(adr_stream_t stream, uint16_t* output, const uint16_t* query, cache_t cache,                  \
+                                  adr_paged_batch batch, adr_draft_tree tree, int32_t heads, int32_t rows, int32_t stride_ox,   \
+                                  int32_t stride_oy, int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz, \
+                                  float scale, float temp) {                                                                    \
+    return attention_paged(stream, output, query, cache, batch, heads, rows, {stride_ox, stride_oy, stride_oz},                 \
+                           {stride_qx, stride_qy, stride_qz}, scale, temp, 0, true, nullptr, 0, &tree);                         \
+  }                                                                                                                             \
+  int adr_attention_tree_##suffix##_ws(adr_stream_t stream, uint16_t* output, const uint16_t* query, cache_t cache,             \
+                                       adr_paged_batch batch, adr_draft_tree tree, int32_t heads, int32_t rows,                 \
+                                       int32_t stride_ox, int32_t stride_oy, int32_t stride_oz, int32_t stride_qx,              \
+                                       int32_t stride_qy, int32_t stride_qz, float scale, float temp, void* workspace,          \
+                                       int64_t workspace_bytes) {                                                               \
+    if (int rc = validate_workspace(workspace, workspace_bytes)) return rc;                                                     \
+    return attention_paged(stream, output, query, cache, batch, heads, rows, {stride_ox, stride_oy, stride_oz},                 \
+                           {stride_qx, stride_qy, stride_qz}, scale, temp, 0, false, workspace, workspace_bytes, &tree);        \
+  }
+ADR_TREE_ENTRIES(f16, adr_paged_cache)
+ADR_TREE_ENTRIES(u8, adr_paged_cache_u8)
+#undef ADR_TREE_ENTRIES
 
 static int error_stats_common(adr_stream_t stream, adr_tensor_desc output, adr_tensor_desc lhs,
                               adr_tensor_desc rhs, bool f32) {

@@ -27,6 +27,9 @@ struct RotaryArgs {
 };
 hipError_t launch_rotary(hipStream_t stream, const RotaryArgs& a);
 
+// Rows are drafted tokens, and the last keys of their sequence: a row sees all keys before those, and of those what its bits say.
+constexpr uint32_t MASK_TREE = 2;
+
 constexpr int MOST_KEYS = 1 << 30;  // of a sequence (a workgroup's tiles beyond the last key still count in 31 bits)
 
 // Attention of packed rows over pages or packed keys (table null).
@@ -46,6 +49,12 @@ struct SequencesArgs {
   int longest_rows, longest;
   float c;             // scale * log2(e) / temperature
   uint32_t mask;
+  // In 8 bits: k and v are codes, and these their scales (y slot, z head, p page); null: k and v are fp16.
+  const half_t* k_scale;
+  const half_t* v_scale;
+  KvStrides sks, svs;
+  const int* tree;     // MASK_TREE: [rows, tree_words] bits of the drafted tokens that a row sees
+  int tree_words, tree_pitch;
 };
 // Which kernel, and how the keys are shared over workgroups (attention_sequences.hip).
 struct SequencesPlan {
@@ -59,6 +68,9 @@ struct SequencesPlan {
 SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail);
 hipError_t launch_attention_sequences(hipStream_t stream, const SequencesArgs& a, const SequencesPlan& p,
                                       void* workspace);
+// The same where keys and values are codes (attention_u8.hip).
+SequencesPlan sequences_u8_plan(const SequencesArgs& a, int cus, int64_t avail);
+hipError_t launch_attention_u8(hipStream_t stream, const SequencesArgs& a, const SequencesPlan& p, void* workspace);
 
 
 // The last of `sequences` whose first row is not behind `row`, by all lanes of a wavefront: 64 offsets a

@@ -268,6 +268,92 @@ _NO_ROTARY = _ffi.RotaryDesc(None, 0, 0, 1.0)
 
 
 @dataclass(frozen=True)
+class RotaryAxes:
+    """Rotary positions on several axes (time, height and width, say): Rotary, and for each pair the axis whose position
+    turns it."""
+    turns: object        # float64 tensor [dims / 2]
+    axis: object         # int32 tensor [dims / 2], of 0 .. axes - 1
+    axes: int
+    layout: int = RotaryLayout.HALVES
+    magnitude: float = 1.0
+
+    def __post_init__(self):
+        import torch
+        assert self.turns.dtype == torch.float64 and self.turns.dim() == 1 and self.turns.is_contiguous(), \
+            "turns: a contiguous float64 tensor of rank 1"
+        assert _index(self.axis, 1, "axis").shape == self.turns.shape, "axis has an entry for each pair"
+        assert 1 <= self.axes <= _ffi.ROTARY_MAX_AXES, f"1 to {_ffi.ROTARY_MAX_AXES} axes"
+
+    @staticmethod
+    def new(dims: int, sections, base: float = 10000.0, layout: int = RotaryLayout.HALVES,
+            scaling: RotaryScaling = RotaryScaling(), own_frequencies: bool = False) -> "RotaryAxes":
+        """The first sections[0] pairs follow the first axis, the next sections[1] the second, and so on, at the frequencies that
+        the pairs have under one axis; with own_frequencies each axis has those of a head of its pairs alone."""
+        import torch
+        sections = [int(n) for n in sections]
+        if min(sections, default=-1) < 0 or 2 * sum(sections) != dims or len(sections) > _ffi.ROTARY_MAX_AXES:
+            raise ValueError(f"the sections of 1 to {_ffi.ROTARY_MAX_AXES} axes are the dims / 2 pairs")
+        frequencies, magnitude = rotary_frequencies(dims, base, scaling)
+        if own_frequencies:
+            frequencies = [f for n in sections for f in rotary_frequencies(2 * n, base, scaling)[0]]
+        turns = torch.tensor([f / (2 * math.pi) for f in frequencies], dtype=torch.float64).cuda()
+        axis = torch.tensor([a for a, n in enumerate(sections) for _ in range(n)], dtype=torch.int32).cuda()
+        return RotaryAxes(turns, axis, len(sections), layout, magnitude)
+
+    @property
+    def _desc(self) -> _ffi.RotaryAxesDesc:
+        _here(self.turns, self.axis)
+        _int32("turns", 2 * self.turns.numel())
+        return _ffi.RotaryAxesDesc(self.turns.data_ptr(), self.axis.data_ptr(), 2 * self.turns.numel(), self.layout, self.magnitude,
+                                   self.axes)
+
+
+def _axes_desc(rotary) -> _ffi.RotaryAxesDesc:
+    """Of a RotaryAxes, a Rotary (one axis) or None (nothing is turned)."""
+    if isinstance(rotary, RotaryAxes):
+        return rotary._desc
+    r = rotary._desc if rotary is not None else _NO_ROTARY
+    return _ffi.RotaryAxesDesc(r.turns, None, r.dims, r.layout, r.magnitude, 1)
+
+
+@dataclass(frozen=True)
+class HeadNorm:
+    """Each head divided by its root mean square and multiplied by a weight: x / sqrt(mean(x^2) + eps) * weight."""
+    weight: object       # fp16 tensor [d], on the device
+    eps: float = 1e-6
+
+    def __post_init__(self):
+        import torch
+        assert self.weight.dtype == torch.float16 and self.weight.dim() == 1 and self.weight.is_contiguous(), \
+            "weight: a contiguous fp16 tensor of rank 1"
+        if not 0.0 <= self.eps <= 3.4e38:
+            raise ValueError("eps is a finite number, and not negative")
+
+
+_NO_NORM = _ffi.HeadNormDesc(None, 0.0)
+
+
+def _norm_desc(norm: Optional[HeadNorm], d: int) -> _ffi.HeadNormDesc:
+    if norm is None:
+        return _NO_NORM
+    _here(norm.weight)
+    assert norm.weight.shape[0] == d, "a norm's weight has an entry for each value of a head"
+    return _ffi.HeadNormDesc(norm.weight.data_ptr(), norm.eps)
+
+
+def _axis_positions(positions, axes: int, rows: int):
+    """Address and pitch of positions [axes, rows], or [rows] for one axis."""
+    rank = positions.dim()
+    assert rank == 2 or (rank == 1 and axes == 1), "positions: [axes, rows]"
+    shape = _index(positions, rank, "positions").shape
+    assert shape[-1] == rows and (rank == 1 or shape[0] == axes), "a position on each axis for each row"
+    _here(positions)
+    pitch = positions.stride(0) if rank == 2 and axes > 1 else rows
+    _int32("positions", pitch)
+    return positions.data_ptr(), pitch
+
+
+@dataclass(frozen=True)
 class PagedCache:
     """Keys and values of many sequences in pages: two [pages, kv_heads, page_size, d] views of the pools that
     the program owns (a pool kept as [pages, page_size, kv_heads, d] is handed over as its permuted view)."""
@@ -288,6 +374,73 @@ class PagedCache:
         _int32("sizes of the pages", p, h, s, d)
         return _ffi.PagedCacheDesc(self.key.data_ptr(), self.value.data_ptr(), p, h, s, d,
                                    *(t.strides[i] for t in (k, v) for i in (3, 2, 1, 0)))
+
+
+@dataclass(frozen=True)
+class PagedCacheU8:
+    """Keys and values in 8 bits: [pages, kv_heads, page_size, d] views of codes, and [pages, kv_heads, page_size] views of their
+    scales.  Code c stands for (c - 127.5) * scale."""
+    key: TensorView
+    key_scale: TensorView
+    value: TensorView
+    value_scale: TensorView
+
+    def __post_init__(self):
+        import torch
+        k, v = self.key.layout, self.value.layout
+        assert len(k.dims) == 4 and k.dims == v.dims, "key and value pages are [pages, kv_heads, page_size, d] views"
+        assert self.key_scale.layout.dims == k.dims[:3] and self.value_scale.layout.dims == k.dims[:3], \
+            "scales are [pages, kv_heads, page_size] views"
+        for what, t in (("key", self.key), ("value", self.value)):
+            if t.storage.dtype != torch.uint8:
+                raise TypeError(f"{what} pages: values of {t.storage.dtype}, not codes in uint8")
+        _halves("key scales", self.key_scale)
+        _halves("value scales", self.value_scale)
+
+    @property
+    def _desc(self) -> _ffi.PagedCacheU8Desc:
+        views = (self.key, self.key_scale, self.value, self.value_scale)
+        k, ks, v, vs = (t.layout for t in views)
+        _here(*(t.storage for t in views))
+        p, h, s, d = k.dims
+        _int32("sizes of the pages", p, h, s, d)
+        return _ffi.PagedCacheU8Desc(*(t.data_ptr() for t in views), p, h, s, d,
+                                     *(t.strides[i] for t in (k, v) for i in (3, 2, 1, 0)),
+                                     *(t.strides[i] for t in (ks, vs) for i in (2, 1, 0)))
+
+
+@dataclass(frozen=True)
+class DraftTree:
+    """What drafted tokens see of each other: bit i % 32 of word i / 32 of a row says that it sees the i-th drafted token of its
+    sequence (its ancestors and itself).  int32 on the device, [rows, words], packed like the rows of a step."""
+    bits: object
+
+    def __post_init__(self):
+        _index(self.bits, 2, "bits")
+
+    @staticmethod
+    def of(parents) -> "DraftTree":
+        """From the drafts of a step's sequences: for each, the index of the token that each drafted token follows, in front of
+        it, or -1 where that is what is in the cache."""
+        import torch
+        words = max([(len(p) + 31) // 32 for p in parents] + [1])
+        rows = []
+        for p in parents:
+            seen = []
+            for j, parent in enumerate(p):
+                if not -1 <= parent < j:
+                    raise ValueError("a drafted token follows one in front of it, or -1")
+                seen.append((seen[parent] if parent >= 0 else 0) | 1 << j)
+            rows += [[(s >> 32 * w & 0xffffffff) - (s >> 32 * w + 31 & 1) * (1 << 32) for w in range(words)] for s in seen]
+        return DraftTree(torch.tensor(rows, dtype=torch.int32).reshape(len(rows), words).cuda())
+
+    def _desc_of(self, rows: int) -> _ffi.DraftTreeDesc:
+        _here(self.bits)
+        n, words = self.bits.shape
+        assert n == rows, "bits for each row"
+        pitch = self.bits.stride(0) if n > 1 else words
+        _int32("bits", words, pitch)
+        return _ffi.DraftTreeDesc(self.bits.data_ptr(), words, pitch)
 
 
 def _here(*storages) -> None:
@@ -627,6 +780,94 @@ class GpuKernels(CommonKernels):
         if rc != 0:
             raise AdrasteaError(rc, "attention_packed_f16")
 
+    # -- heads normed and turned, a cache in 8 bits, drafted trees --
+    def norm_rotary_f16(self, output, input, positions=None, rotary=None, norm: Optional[HeadNorm] = None):
+        """The heads of `input`, a [heads, rows, d] view, normed and then turned into `output` (which may be the same view).
+        rotary: a RotaryAxes, a Rotary or None; positions: int32 [axes, rows] (or [rows])."""
+        dims, si = _rows_view(input, "input")
+        dims_out, so = _rows_view(output, "output")
+        assert dims_out == dims, "output and input have one shape"
+        r = _axes_desc(rotary)
+        at, pitch = (None, 0) if positions is None else _axis_positions(positions, r.axes, dims[1])
+        rc = self._lib.adr_norm_rotary_f16(_current_stream(), output.data_ptr(), input.data_ptr(), at, pitch, r,
+                                           _norm_desc(norm, dims[2]), *dims, *so, *si)
+        if rc != 0:
+            raise AdrasteaError(rc, "norm_rotary_f16")
+
+    def _append(self, fn, what, cache, batch, key, value, rotary, query_out, query, positions, query_norm, key_norm):
+        c, b = cache._desc, batch._desc
+        dims, sk = _rows_view(key, "key")
+        dims_v, sv = _rows_view(value, "value")
+        assert dims_v == dims and dims[0] == c.kv_heads and dims[2] == c.d, "key and value are [kv_heads, rows, d] views"
+        heads, sq, so = 0, (0, 0, 0), (0, 0, 0)
+        assert (query is None) == (query_out is None), "query and query_out go together"
+        if query is not None:
+            dims_q, sq = _rows_view(query, "query")
+            dims_o, so = _rows_view(query_out, "query_out")
+            heads = dims_q[0]
+            assert dims_o == dims_q and dims_q[1:] == dims[1:], "query and query_out are [heads, rows, d] views"
+        r = _axes_desc(rotary)
+        at, pitch = (None, 0) if positions is None else _axis_positions(positions, r.axes, dims[1])
+        rc = fn(_current_stream(), c, b, key.data_ptr(), value.data_ptr(), query_out.data_ptr() if heads else None,
+                query.data_ptr() if heads else None, at, pitch, r, _norm_desc(query_norm, c.d), _norm_desc(key_norm, c.d),
+                heads, dims[1], *sk, *sv, *so, *sq)
+        if rc != 0:
+            raise AdrasteaError(rc, what)
+
+    def append_norm_f16(self, cache: PagedCache, batch: PagedBatch, key, value, rotary=None, query_out=None, query=None,
+                        positions=None, query_norm: Optional[HeadNorm] = None, key_norm: Optional[HeadNorm] = None):
+        """append_f16 of heads that are normed before they are turned, by positions on several axes (int32 [axes, rows]) where
+        rotary is a RotaryAxes."""
+        self._append(self._lib.adr_append_norm_f16, "append_norm_f16", cache, batch, key, value, rotary, query_out, query,
+                     positions, query_norm, key_norm)
+
+    def append_u8(self, cache: PagedCacheU8, batch: PagedBatch, key, value, rotary=None, query_out=None, query=None,
+                  positions=None, query_norm: Optional[HeadNorm] = None, key_norm: Optional[HeadNorm] = None):
+        """append_norm_f16 into a cache in 8 bits: keys as normed and turned, and values, each with a scale of its own for each
+        head, within half a scale of what they were."""
+        self._append(self._lib.adr_append_u8, "append_u8", cache, batch, key, value, rotary, query_out, query, positions,
+                     query_norm, key_norm)
+
+    def read_u8(self, key_out, value_out, cache: PagedCacheU8, batch: PagedBatch):
+        """What the codes of the batch's rows stand for, into [kv_heads, rows, d] views: row j of the r of sequence s is key
+        lengths[s] - r + j.  (As many rows as keys: all of them.)"""
+        c, b = cache._desc, batch._desc
+        dims, sk = _rows_view(key_out, "key_out")
+        dims_v, sv = _rows_view(value_out, "value_out")
+        assert dims_v == dims and dims[0] == c.kv_heads and dims[2] == c.d, "key_out and value_out are [kv_heads, rows, d] views"
+        rc = self._lib.adr_read_u8(_current_stream(), key_out.data_ptr(), value_out.data_ptr(), c, b, dims[1], *sk, *sv)
+        if rc != 0:
+            raise AdrasteaError(rc, "read_u8")
+
+    def _attention_paged(self, what, output, query, cache, batch, before, after):
+        c, b = cache._desc, batch._desc
+        dims, sq = _rows_view(query, "query")
+        dims_o, so = _rows_view(output, "output")
+        assert dims_o == dims and dims[2] == c.d, "output and query are [heads, rows, d] views"
+        args = (_current_stream(), output.data_ptr(), query.data_ptr(), c, b, *(f(dims[1]) for f in before), dims[0], dims[1], *so,
+                *sq, *after)
+        ws = self._workspace
+        rc = (getattr(self._lib, "adr_" + what)(*args) if ws is None else
+              getattr(self._lib, "adr_" + what + "_ws")(*args, ws.data_ptr(), ws.numel()))
+        if rc != 0:
+            raise AdrasteaError(rc, what)
+
+    def attention_paged_u8(self, output, query, cache: PagedCacheU8, batch: PagedBatch, scale: float, temperature: float = 1.0,
+                           mask: int = MatmulMask.CAUSAL):
+        """attention_paged_f16 over a cache in 8 bits."""
+        self._attention_paged("attention_paged_u8", output, query, cache, batch, (), (float(scale), float(temperature), int(mask)))
+
+    def attention_tree_f16(self, output, query, cache: PagedCache, batch: PagedBatch, tree: DraftTree, scale: float,
+                           temperature: float = 1.0):
+        """Attention of drafted tokens, which are the last keys of their sequences: each row sees all keys in front of the
+        draft, and of the draft what its bits say."""
+        self._attention_paged("attention_tree_f16", output, query, cache, batch, (tree._desc_of,), (float(scale), float(temperature)))
+
+    def attention_tree_u8(self, output, query, cache: PagedCacheU8, batch: PagedBatch, tree: DraftTree, scale: float,
+                          temperature: float = 1.0):
+        """attention_tree_f16 over a cache in 8 bits."""
+        self._attention_paged("attention_tree_u8", output, query, cache, batch, (tree._desc_of,), (float(scale), float(temperature)))
+
     def _error_stats(self, fn, what, output, lhs, rhs):
         if _native is not None:
             rc = _native.error_stats(output, lhs, rhs, int(what == "error_stats_f32"))
@@ -775,6 +1016,16 @@ def attention_paged_workspace_bytes(cache: PagedCache, batch: PagedBatch, heads:
     return int(n)
 
 
+def attention_paged_u8_workspace_bytes(cache: PagedCacheU8, batch: PagedBatch, heads: int, rows: int) -> int:
+    """Scratch bytes adr_attention_paged_u8_ws would use for `rows` packed rows of `heads` query heads (0: it would share no
+    keys)."""
+    _int32("heads and rows", heads, rows)
+    n = _ffi.lib().adr_attention_paged_u8_workspace_bytes(cache._desc, batch._desc, heads, rows)
+    if n < 0:
+        raise AdrasteaError(int(n), "attention_paged_u8_workspace_bytes")
+    return int(n)
+
+
 def attention_packed_workspace_bytes(batch: PackedBatch, heads: int, kv_heads: int, rows: int, keys: int, d: int) -> int:
     """Scratch bytes adr_attention_packed_f16_ws would use for these sizes (0: it would share no keys)."""
     _int32("heads, rows and keys", heads, kv_heads, rows, keys, d)
@@ -867,6 +1118,29 @@ class MatmulTracer(CommonKernels):
 
     def attention_packed_f16(self, output, query, key, value, batch, scale, temperature=1.0, mask=MatmulMask.CAUSAL):
         self.inner.attention_packed_f16(output, query, key, value, batch, scale, temperature, mask)
+
+    def norm_rotary_f16(self, output, input, positions=None, rotary=None, norm=None):
+        self.inner.norm_rotary_f16(output, input, positions, rotary, norm)
+
+    def append_norm_f16(self, cache, batch, key, value, rotary=None, query_out=None, query=None, positions=None, query_norm=None,
+                        key_norm=None):
+        self.inner.append_norm_f16(cache, batch, key, value, rotary, query_out, query, positions, query_norm, key_norm)
+
+    def append_u8(self, cache, batch, key, value, rotary=None, query_out=None, query=None, positions=None, query_norm=None,
+                  key_norm=None):
+        self.inner.append_u8(cache, batch, key, value, rotary, query_out, query, positions, query_norm, key_norm)
+
+    def read_u8(self, key_out, value_out, cache, batch):
+        self.inner.read_u8(key_out, value_out, cache, batch)
+
+    def attention_paged_u8(self, output, query, cache, batch, scale, temperature=1.0, mask=MatmulMask.CAUSAL):
+        self.inner.attention_paged_u8(output, query, cache, batch, scale, temperature, mask)
+
+    def attention_tree_f16(self, output, query, cache, batch, tree, scale, temperature=1.0):
+        self.inner.attention_tree_f16(output, query, cache, batch, tree, scale, temperature)
+
+    def attention_tree_u8(self, output, query, cache, batch, tree, scale, temperature=1.0):
+        self.inner.attention_tree_u8(output, query, cache, batch, tree, scale, temperature)
 
     def error_stats_f16(self, output, lhs, rhs):
         self.inner.error_stats_f16(output, lhs, rhs)            # forwarded (kernels.rs:349-358)

@@ -10,8 +10,8 @@
  * with any other device current, every launching entry point returns ADR_EUNSUPPORTED_DEVICE
  * (the device's architecture, compute-unit and die counts are queried once per device and
  * cached).  Beside that cache the library keeps one piece of state: the pool of workspaces that
- * adr_matmul_f16, adr_matmul_nt_f16, adr_attention_f16, adr_attention_paged_f16,
- * adr_attention_packed_f16 and (on request) adr_matmul_nt_fp16u8 draw from, grown on demand and given back through adr_release_held_workspace*
+ * adr_matmul_f16, adr_matmul_nt_f16, adr_attention_f16, adr_attention_paged_f16, adr_attention_packed_f16,
+ * adr_attention_paged_u8, adr_attention_tree_f16, adr_attention_tree_u8 and (on request) adr_matmul_nt_fp16u8 draw from, grown on demand and given back through adr_release_held_workspace*
  * (adr_set_held_workspace_limit below; 0 switches it off).
  *
  * fp16 data is passed as uint16_t bit patterns (Rust `half::f16` is repr(transparent) u16).
@@ -522,6 +522,130 @@ int adr_attention_packed_f16_ws(adr_stream_t stream, uint16_t* output, const uin
                                 void* workspace, int64_t workspace_bytes);
 int64_t adr_attention_packed_f16_workspace_bytes(adr_packed_batch batch, int32_t heads, int32_t kv_heads, int32_t rows,
                                                  int32_t keys, int32_t d);
+
+/*
+ * Norms of queries and keys for each head, with the rotation in the same pass, of one or several axes (no counterpart in the
+ * reference).
+ *
+ * adr_head_norm: before it is turned, a head x of d values becomes x / sqrt(mean(x^2) + eps) * weight; `weight` is device memory,
+ * [d] fp16, contiguous; null: the heads are not normed.  eps >= 0, finite (ADR_EINVAL_SHAPE).  A head of zeros under eps = 0 is NaN.
+ * adr_rotary_axes: adr_rotary for images and video, whose rows have a position on each of `axes` axes (1 ..
+ * ADR_ROTARY_MAX_AXES): pair i is turned by positions[axis[i] * positions_pitch + row] * turns[i] full turns.  `axis` is device
+ * memory, [dims / 2], entries outside 0 .. axes - 1 count as 0; null: all pairs follow the first axis.  How the pairs are
+ * divided, and whether each axis has frequencies of its own, is in `axis` and `turns`.
+ *
+ * adr_norm_rotary_f16: as adr_rotary_f16, with both; positions [axes][positions_pitch], of which `rows` entries each are used.
+ * adr_append_norm_f16: as adr_append_f16, with both: `query_norm` for the queries, `key_norm` for the keys, values as they are.
+ * Without `positions` every axis is at the row's place in the cache.  32-bit arithmetic (angles in 64), one rounding.
+ */
+#define ADR_ROTARY_MAX_AXES 8
+typedef struct adr_rotary_axes {
+  const double* turns;
+  const int32_t* axis;
+  int32_t dims;
+  uint32_t layout;
+  float magnitude;
+  int32_t axes;
+} adr_rotary_axes;
+typedef struct adr_head_norm {
+  const uint16_t* weight;
+  float eps;
+} adr_head_norm;
+int adr_norm_rotary_f16(adr_stream_t stream, uint16_t* output, const uint16_t* input, const int32_t* positions,
+                        int32_t positions_pitch, adr_rotary_axes rotary, adr_head_norm norm, int32_t heads, int32_t rows,
+                        int32_t d, int32_t stride_ox, int32_t stride_oy, int32_t stride_oz, int32_t stride_ix,
+                        int32_t stride_iy, int32_t stride_iz);
+int adr_append_norm_f16(adr_stream_t stream, adr_paged_cache cache, adr_paged_batch batch, const uint16_t* key,
+                        const uint16_t* value, uint16_t* query_out, const uint16_t* query, const int32_t* positions,
+                        int32_t positions_pitch, adr_rotary_axes rotary, adr_head_norm query_norm, adr_head_norm key_norm,
+                        int32_t heads, int32_t rows, int32_t stride_kx, int32_t stride_ky, int32_t stride_kz,
+                        int32_t stride_vx, int32_t stride_vy, int32_t stride_vz, int32_t stride_ox, int32_t stride_oy,
+                        int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz);
+
+/*
+ * A paged cache in 8 bits (no counterpart in the reference): the codes of adr_dequantize_absmax_u8, with one fp16 scale for
+ * each key and for each value of a head: code c stands for (c - 127.5) * scale.  Codes are [pages, kv_heads, page_size, d] views,
+ * scales [pages, kv_heads, page_size] (strides y slot, z head, p page), all strides in elements.
+ *
+ * adr_append_u8: adr_append_norm_f16 into such a cache.  What is quantised is the key as normed and turned, in 64 bits and not
+ * rounded before: with top the largest |y| of the head, scale = the smallest fp16 number that is top / 127.5 at least, 513.5 at
+ * most, and code = 128 + floor(y / scale) within 0 .. 255.  So a value is off by at most half a scale (values beyond 65471, the
+ * largest of the format, become that), and a head of zeros has scale 0.  A head with an infinity or NaN has scale NaN.
+ *
+ * adr_read_u8: the way back, of the same rows that adr_append_u8 would write: row j of the r of sequence s is key lengths[s] - r + j,
+ * and fp16((code - 127.5) * scale) goes to its row of `key` and `value` ([kv_heads, rows, d] views).  A batch whose sequences
+ * have as many rows as keys reads all of them.  Rows whose key is on no page of the cache become NaN; rows of no sequence are left.
+ */
+typedef struct adr_paged_cache_u8 {
+  uint8_t* key;
+  uint16_t* key_scale;
+  uint8_t* value;
+  uint16_t* value_scale;
+  int32_t pages, kv_heads, page_size, d;
+  int64_t stride_kx, stride_ky, stride_kz, stride_kp;
+  int64_t stride_vx, stride_vy, stride_vz, stride_vp;
+  int64_t stride_ksy, stride_ksz, stride_ksp;
+  int64_t stride_vsy, stride_vsz, stride_vsp;
+} adr_paged_cache_u8;
+int adr_append_u8(adr_stream_t stream, adr_paged_cache_u8 cache, adr_paged_batch batch, const uint16_t* key,
+                  const uint16_t* value, uint16_t* query_out, const uint16_t* query, const int32_t* positions,
+                  int32_t positions_pitch, adr_rotary_axes rotary, adr_head_norm query_norm, adr_head_norm key_norm,
+                  int32_t heads, int32_t rows, int32_t stride_kx, int32_t stride_ky, int32_t stride_kz, int32_t stride_vx,
+                  int32_t stride_vy, int32_t stride_vz, int32_t stride_ox, int32_t stride_oy, int32_t stride_oz,
+                  int32_t stride_qx, int32_t stride_qy, int32_t stride_qz);
+int adr_read_u8(adr_stream_t stream, uint16_t* key, uint16_t* value, adr_paged_cache_u8 cache, adr_paged_batch batch,
+                int32_t rows, int32_t stride_kx, int32_t stride_ky, int32_t stride_kz, int32_t stride_vx, int32_t stride_vy,
+                int32_t stride_vz);
+
+/*
+ * Attention over a cache in 8 bits: as adr_attention_paged_f16 over the values that the codes stand for, which are not rounded
+ * to fp16 where scores are computed, and once where they are summed.  A key of which either scale is no finite number, or the
+ * value's is beyond 513.5, counts as NaN for the rows that see it and does not reach the others; rows of queries that are not
+ * all finite are NaN where they see a key.
+ * The fast kernels take d a multiple of 16 up to 128, x strides 1, the codes' other strides multiples of 16 (the queries' and the
+ * output's of 8) and not negative, slots at least d apart and less than 2^24, 16-byte aligned pointers, pages of 16, 32,
+ * 64 ... slots; everything else runs on a kernel of one wavefront per row.  Scales that follow each other from slot to slot, a page's
+ * from a multiple of 16 bytes on, are read 16 bytes at a time, others one by one.
+ */
+int adr_attention_paged_u8(adr_stream_t stream, uint16_t* output, const uint16_t* query, adr_paged_cache_u8 cache,
+                           adr_paged_batch batch, int32_t heads, int32_t rows, int32_t stride_ox, int32_t stride_oy,
+                           int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz, float scale,
+                           float temp, uint32_t mask);
+int adr_attention_paged_u8_ws(adr_stream_t stream, uint16_t* output, const uint16_t* query, adr_paged_cache_u8 cache,
+                              adr_paged_batch batch, int32_t heads, int32_t rows, int32_t stride_ox, int32_t stride_oy,
+                              int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz, float scale,
+                              float temp, uint32_t mask, void* workspace, int64_t workspace_bytes);
+int64_t adr_attention_paged_u8_workspace_bytes(adr_paged_cache_u8 cache, adr_paged_batch batch, int32_t heads,
+                                               int32_t rows);
+
+/*
+ * Attention of drafted tokens that form a tree (no counterpart in the reference): the rows of a sequence are a draft, and the last
+ * of its keys, in the same order (adr_append_f16 puts them there, with their depths as `positions`).  Row j of the r of a
+ * sequence sees all keys in front of the last r, and of those key i where bit i % 32 of word i / 32 of its bits is set (its
+ * ancestors and itself): bits are [rows, words], rows `pitch` words apart, packed like the rows of the queries; tokens beyond
+ * 32 * words are not seen.  Otherwise as adr_attention_paged_f16 and adr_attention_paged_u8, whose
+ * _workspace_bytes hold for these too.
+ */
+typedef struct adr_draft_tree {
+  const int32_t* bits;
+  int32_t words, pitch;
+} adr_draft_tree;
+int adr_attention_tree_f16(adr_stream_t stream, uint16_t* output, const uint16_t* query, adr_paged_cache cache,
+                           adr_paged_batch batch, adr_draft_tree tree, int32_t heads, int32_t rows, int32_t stride_ox,
+                           int32_t stride_oy, int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz,
+                           float scale, float temp);
+int adr_attention_tree_f16_ws(adr_stream_t stream, uint16_t* output, const uint16_t* query, adr_paged_cache cache,
+                              adr_paged_batch batch, adr_draft_tree tree, int32_t heads, int32_t rows, int32_t stride_ox,
+                              int32_t stride_oy, int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz,
+                              float scale, float temp, void* workspace, int64_t workspace_bytes);
+int adr_attention_tree_u8(adr_stream_t stream, uint16_t* output, const uint16_t* query, adr_paged_cache_u8 cache,
+                          adr_paged_batch batch, adr_draft_tree tree, int32_t heads, int32_t rows, int32_t stride_ox,
+                          int32_t stride_oy, int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz,
+                          float scale, float temp);
+int adr_attention_tree_u8_ws(adr_stream_t stream, uint16_t* output, const uint16_t* query, adr_paged_cache_u8 cache,
+                             adr_paged_batch batch, adr_draft_tree tree, int32_t heads, int32_t rows, int32_t stride_ox,
+                             int32_t stride_oy, int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz,
+                             float scale, float temp, void* workspace, int64_t workspace_bytes);
 
 /*
  * Diagnostics (no counterpart in the reference).
