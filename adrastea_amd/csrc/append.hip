@@ -20,7 +20,8 @@ namespace {
 enum Cache { NO_CACHE, F16, U8 };
 
 struct PlaceJob : PlaceArgs {
-  int splits, heads_each;  // groups of lanes that share a row's heads, and heads of each
+  int lanes;   // that a head needs, of W
+  int splits;  // wavefronts that share a row's heads
 };
 
 // ---- sums over the lanes of a head --------------------------------------------------------------------------
@@ -121,6 +122,8 @@ __device__ __forceinline__ T inverse_of(half_t s) {
   return (float)s > 0.0f ? (T)1 / (T)(float)s : (T)0;
 }
 
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // ---- where a row's key goes -----------------------------------------------------------------------------------
 
 struct Slot {
@@ -158,15 +161,22 @@ __device__ __forceinline__ Slot slot_of(const adr_paged_batch& b, int rows, int 
 
 // ---- 16 bytes at a time -------------------------------------------------------------------------------------
 
-// W lanes have a head, each the 16 values that are turned together and so need no exchange: of halves chunk l of 8 values and its
-// partner, of pairs two chunks side by side; chunks that pass follow, two to a lane.  A lane has the same values of all
-// heads that its group goes through, so that angles and weights are made once for a row and stay in registers.  The heads of
-// a row are shared by `splits` groups: as many as it takes to fill the machine.
+// A wavefront has a row, or shares it with others where rows are few.  W lanes have a head, and the 64 / W heads that a wavefront
+// works on lie side by side; a lane has the 16 values that are turned together and so need no exchange: of halves chunk l
+// of 8 values and its partner, of pairs two chunks side by side; chunks that pass follow, two to a lane.  So angles and weights
+// stay in registers from head to head: each angle is computed by one lane of the wavefront, and comes to the others by way of LDS.
+//
+// Loads and stores of the loops are under no condition, so that the next head's loads are waited for and not the stores in front
+// of them: lanes that are left over do what the last one with values does, and store the same.
 template <int CACHE, int W>
 __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
-  constexpr int GROUPS = 64 / W;  // of a wavefront
-  const int lane = threadIdx.x & 63, l = lane & (W - 1);
-  const int q_heads = a.q ? a.heads : 0, kv_heads = CACHE == NO_CACHE ? 0 : a.kv_heads, all = q_heads + 2 * kv_heads;
+  typedef typename std::conditional<CACHE == U8, double, float>::type angle_t;
+  constexpr int GROUPS = 64 / W, MOST_PAIRS = 8 * W;
+  __shared__ Turn<angle_t> shared_turns[4][MOST_PAIRS];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), l = min(lane & (W - 1), a.lanes - 1);
+  Turn<angle_t>* const turns = shared_turns[wave];
+  const bool mine = (lane & (W - 1)) < a.lanes;
+  const int end_q = a.q ? a.heads : 0, end_k = end_q + (CACHE == NO_CACHE ? 0 : a.kv_heads), all = 2 * end_k - end_q;
   // The lane's chunks (first values), and which are turned.
   const int joined = a.pairs ? 0 : a.dims >> 4;
   int x0, x1;
@@ -181,91 +191,114 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
     x0 = a.dims + 16 * (l - joined), x1 = x0 + 8;
     turn0 = turn1 = false;
   }
-  const bool has0 = x0 < a.d, has1 = x1 < a.d;
-  const int pair0 = 8 * l;  // the first of the lane's pairs
-  const int64_t tasks = (int64_t)a.rows * a.splits;
-  for (int64_t base = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * GROUPS; base < tasks; base += (int64_t)gridDim.x * 4 * GROUPS) {
-    const int first = (int)(base / a.splits), last = (int)((min(base + GROUPS, tasks) - 1) / a.splits);
-    const int64_t task = base + lane / W;
-    const bool some = task < tasks;
-    const int row = some ? (int)(task / a.splits) : last, split = some ? (int)(task - (int64_t)row * a.splits) : 0;
-    const int h0 = split * a.heads_each, h1 = some ? min(h0 + a.heads_each, all) : 0;
-    half8_t n0 = {}, n1 = {};
+  const bool one = x1 >= a.d;  // (the last of an odd number: its chunk twice)
+  if (one) x1 = x0, turn1 = false;
+  const float per_value = 1.0f / (float)a.d;
+  const uint32_t tasks = (uint32_t)a.rows * a.splits;  // (splits are more than one where there are few rows)
+  for (uint64_t task = (uint64_t)blockIdx.x * 4 + wave; task < tasks; task += (uint64_t)gridDim.x * 4) {
+    const int row = uniform((int)((uint32_t)task / (uint32_t)a.splits)), split = uniform((int)((uint32_t)task - (uint32_t)row * a.splits));
+    const int step = GROUPS * a.splits, h0 = split * GROUPS + lane / W;
+    // The chunks of a head, asked for a head ahead (behind the last one, that again).
+    half8_t n0, n1;
     auto read = [&](int h) __attribute__((always_inline)) {
-      if (h >= h1) return;
-      const int k = h - q_heads, v = k - kv_heads;
-      const half_t* from = k < 0   ? a.q + h * (int64_t)a.sq_z + row * (int64_t)a.sq_y
-                           : v < 0 ? a.k + k * (int64_t)a.sk_z + row * (int64_t)a.sk_y
-                                   : a.v + v * (int64_t)a.sv_z + row * (int64_t)a.sv_y;
-      if (has0) n0 = *(const half8_t*)(from + x0);
-      if (has1) n1 = *(const half8_t*)(from + x1);
+      const half_t* from = h < end_q ? a.q + h * (int64_t)a.sq_z + row * (int64_t)a.sq_y
+                           : h < end_k ? a.k + (h - end_q) * (int64_t)a.sk_z + row * (int64_t)a.sk_y
+                                       : a.v + (h - end_k) * (int64_t)a.sv_z + row * (int64_t)a.sv_y;
+      n0 = *(const half8_t*)(from + x0);
+      n1 = *(const half8_t*)(from + x1);
     };
-    read(h0);
+    read(min(h0, all - 1));
     Slot at = {row, 0, -1, 0};
     if constexpr (CACHE != NO_CACHE) {
       const int pages = CACHE == U8 ? a.codes.pages : a.cache.pages, size = CACHE == U8 ? a.codes.page_size : a.cache.page_size;
-      at = slot_of(a.batch, a.rows, pages, size, first, last, row, lane);
+      at = slot_of(a.batch, a.rows, pages, size, row, row, row, lane);
+      if (uniform(at.row) < 0) continue;
     }
-    if (at.row < 0) continue;  // (no lane is asked for anything behind this)
+    for (int i = lane; i < a.dims >> 1; i += 64)
+      turns[i] = turn_of<angle_t>(position_of(a, row, i, at.position), a.turns[i], a.magnitude);
+    __builtin_amdgcn_wave_barrier();
+    const int end = CACHE != NO_CACHE && uniform(at.page) < 0 ? end_q : all;  // (keys and values without a slot go nowhere)
+    if (h0 >= end) continue;
 
-    // Norm and turn 16 values, in the bits of T.
-    auto turned = [&](auto zero, const half8_t& c0, const half8_t& c1, const half8_t& w0, const half8_t& w1, bool norm, float eps,
-                      const auto& turns, auto (&y)[16]) __attribute__((always_inline)) {
-      typedef decltype(zero) T;
-#pragma unroll
-      for (int e = 0; e < 8; e++) y[e] = (T)(float)c0[e], y[8 + e] = (T)(float)c1[e];
-      if (norm) {
-        T sum = 0;
-#pragma unroll
-        for (int e = 0; e < 16; e++) sum = fused(y[e], y[e], sum);
-        const T factor = (T)1 / root(sum_of<W>(sum) / (T)a.d + (T)eps);
-#pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = y[e] * factor * (T)(float)w0[e], y[8 + e] = y[8 + e] * factor * (T)(float)w1[e];
-      }
-      if (a.pairs) {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (e < 4 ? turn0 : turn1) {
-            const T u = y[2 * e], v = y[2 * e + 1];
-            y[2 * e] = u * turns[e].cosine - v * turns[e].sine;
-            y[2 * e + 1] = u * turns[e].sine + v * turns[e].cosine;
-          }
-      } else if (turn0) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const T u = y[e], v = y[8 + e];
-          y[e] = u * turns[e].cosine - v * turns[e].sine;
-          y[8 + e] = u * turns[e].sine + v * turns[e].cosine;
-        }
-      }
-    };
-    auto angles = [&](auto& turns) __attribute__((always_inline)) {
-      typedef typename std::remove_reference<decltype(turns[0].sine)>::type T;
+    // The lane's eight pairs.
+    auto angles = [&](auto& mine8) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        turns[e] = {1, 0};
-        if (e < 4 || !a.pairs ? turn0 : turn1)
-          turns[e] = turn_of<T>(position_of(a, row, pair0 + e, at.position), a.turns[pair0 + e], a.magnitude);
+        mine8[e] = {1, 0};
+        if (e < 4 || !a.pairs ? turn0 : turn1) mine8[e] = {turns[8 * l + e].cosine, turns[8 * l + e].sine};
       }
     };
-    auto rounded = [&](const float (&y)[16], half8_t& o0, half8_t& o1) __attribute__((always_inline)) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) o0[e] = (half_t)y[e], o1[e] = (half_t)y[8 + e];
-    };
     auto store16 = [&](half_t* to, const half8_t& o0, const half8_t& o1) __attribute__((always_inline)) {
-      if (has0) *(half8_t*)(to + x0) = o0;
-      if (has1) *(half8_t*)(to + x1) = o1;
+      *(half8_t*)(to + x0) = o0;
+      *(half8_t*)(to + x1) = o1;
+    };
+    // Norm and turn 16 values in 32 bits: weights are part of the cosines and sines, and the norm's factor is applied at the end.
+    struct Coefficients {
+      float uc[8], us[8], vc[8], vs[8];  // of each pair (u, v): u w cos, u w sin, v w cos, v w sin
+    };
+    auto coefficients = [&](const half_t* weight, Coefficients& f) __attribute__((always_inline)) {
+      Turn<float> t[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        t[e] = {1, 0};
+        if (e < 4 || !a.pairs ? turn0 : turn1) t[e] = {(float)turns[8 * l + e].cosine, (float)turns[8 * l + e].sine};
+      }
+      half8_t w0, w1;
+#pragma unroll
+      for (int e = 0; e < 8; e++) w0[e] = w1[e] = (half_t)1;
+      if (weight) w0 = *(const half8_t*)(weight + x0), w1 = *(const half8_t*)(weight + x1);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float wu = (float)(!a.pairs ? w0[e] : e < 4 ? w0[2 * e & 7] : w1[2 * e & 7]);
+        const float wv = (float)(!a.pairs ? w1[e] : e < 4 ? w0[(2 * e + 1) & 7] : w1[(2 * e + 1) & 7]);
+        f.uc[e] = wu * t[e].cosine, f.us[e] = wu * t[e].sine;
+        f.vc[e] = wv * t[e].cosine, f.vs[e] = wv * t[e].sine;
+      }
+    };
+    auto place_rounded = [&](half_t* to, const half8_t& c0, const half8_t& c1, bool norm, float eps, const Coefficients& f)
+                             __attribute__((always_inline)) {
+      float factor = 1.0f;
+      if (norm) {
+        float sum = 0.0f, sum1 = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) sum = fmaf((float)c0[e], (float)c0[e], sum), sum1 = fmaf((float)c1[e], (float)c1[e], sum1);
+        sum = !mine ? 0.0f : one ? sum : sum + sum1;
+        factor = __builtin_amdgcn_rsqf(fmaf(sum_of<W>(sum), per_value, eps));
+      }
+      half8_t o0, o1;
+      auto turn = [&](float u, float v, int e, bool is_turned, half_t& ou, half_t& ov) __attribute__((always_inline)) {
+        const float tu = u * f.uc[e], tv = v * f.vc[e];
+        // (what passes has a cosine of 1, and is not mixed with its neighbour's infinity)
+        ou = (half_t)((is_turned ? fmaf(-v, f.vs[e], tu) : tu) * factor);
+        ov = (half_t)((is_turned ? fmaf(u, f.us[e], tv) : tv) * factor);
+      };
+      if (a.pairs) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          half_t x, y;
+          turn((float)c0[2 * e], (float)c0[2 * e + 1], e, turn0, x, y);
+          o0[2 * e] = x, o0[2 * e + 1] = y;
+          turn((float)c1[2 * e], (float)c1[2 * e + 1], e + 4, turn1, x, y);
+          o1[2 * e] = one ? o0[2 * e] : x, o1[2 * e + 1] = one ? o0[2 * e + 1] : y;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          half_t x, y;
+          turn((float)c0[e], (float)c1[e], e, turn0, x, y);
+          o0[e] = x, o1[e] = y;
+        }
+      }
+      store16(to, o0, o1);
     };
     // 16 values as codes, and the head's scale.
-    auto store8 = [&](auto zero, const auto (&y)[16], uint8_t* codes, half_t* scale) __attribute__((always_inline)) {
+    auto place_codes = [&](auto zero, const auto (&y)[16], uint8_t* codes, half_t* scale) __attribute__((always_inline)) {
       typedef decltype(zero) T;
       T top = 0, none = 0;
 #pragma unroll
       for (int e = 0; e < 16; e++) {
-        const bool mine = e < 8 ? has0 : has1;
-        const T v = mine ? y[e] : (T)0;
-        top = larger(top, v < 0 ? -v : v);
-        none = fused(v, (T)0, none);  // (NaN behind what is not finite)
+        top = larger(top, y[e] < 0 ? -y[e] : y[e]);
+        none = fused(y[e], (T)0, none);  // (NaN behind what is not finite)
       }
       top = max_of<W>(top), none = sum_of<W>(none);
       const half_t s = scale_of(none == 0 ? top : (T)INFINITY);
@@ -273,80 +306,94 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
       uint32_t c[4] = {};
 #pragma unroll
       for (int e = 0; e < 16; e++) c[e / 4] |= code_of(y[e], (T)(float)s, inv) << 8 * (e % 4);
-      if (has0) *(u32x2_t*)(codes + x0) = u32x2_t{c[0], c[1]};
-      if (has1) *(u32x2_t*)(codes + x1) = u32x2_t{c[2], c[3]};
-      if (l == 0) *scale = s;
+      *(u32x2_t*)(codes + x0) = u32x2_t{c[0], c[1]};
+      *(u32x2_t*)(codes + x1) = u32x2_t{c[2], c[3]};
+      *scale = s;
     };
 
     int h = h0;
-    half8_t w0 = {}, w1 = {};
-    auto weights = [&](const half_t* w) __attribute__((always_inline)) {
-      if (w && has0) w0 = *(const half8_t*)(w + x0);
-      if (w && has1) w1 = *(const half8_t*)(w + x1);
-    };
-    if (h < min(h1, q_heads + (CACHE == F16 ? kv_heads : 0))) {
-      Turn<float> turns[8];
-      angles(turns);
-      weights(a.q_weight);
-      for (; h < min(h1, q_heads); h++) {
-        const half8_t c0 = n0, c1 = n1;
-        read(h + 1);
-        float y[16];
-        half8_t o0, o1;
-        turned(0.0f, c0, c1, w0, w1, a.q_weight != nullptr, a.q_eps, turns, y);
-        rounded(y, o0, o1);
-        store16(a.q_out + h * (int64_t)a.so_z + row * (int64_t)a.so_y, o0, o1);
-      }
-      if constexpr (CACHE == F16) {
-        weights(a.k_weight);
-        for (; h < min(h1, q_heads + kv_heads); h++) {
+    if (h < min(end, CACHE == F16 ? end_k : end_q)) {
+      Coefficients f;
+      if (h < end_q) {
+        coefficients(a.q_weight, f);
+        half_t* to = a.q_out + h * (int64_t)a.so_z + row * (int64_t)a.so_y;
+        for (; h < end_q; h += step, to += (int64_t)step * a.so_z) {
           const half8_t c0 = n0, c1 = n1;
-          read(h + 1);
-          float y[16];
-          half8_t o0, o1;
-          turned(0.0f, c0, c1, w0, w1, a.k_weight != nullptr, a.k_eps, turns, y);
-          rounded(y, o0, o1);
-          const adr_paged_cache& c = a.cache;
-          if (at.page >= 0)
-            store16((half_t*)c.key + at.page * c.stride_kp + at.slot * c.stride_ky + (h - q_heads) * c.stride_kz, o0, o1);
+          read(min(h + step, all - 1));
+          place_rounded(to, c0, c1, a.q_weight != nullptr, a.q_eps, f);
+        }
+      }
+      if (CACHE == F16 && h < min(end, end_k)) {
+        coefficients(a.k_weight, f);
+        const adr_paged_cache& c = a.cache;
+        half_t* const to = (half_t*)c.key + at.page * c.stride_kp + at.slot * c.stride_ky;
+        for (; h < end_k; h += step) {
+          const half8_t c0 = n0, c1 = n1;
+          read(min(h + step, all - 1));
+          place_rounded(to + (h - end_q) * c.stride_kz, c0, c1, a.k_weight != nullptr, a.k_eps, f);
         }
       }
     }
     if constexpr (CACHE == U8) {
       const adr_paged_cache_u8& c = a.codes;
-      if (h < min(h1, q_heads + kv_heads)) {
-        Turn<double> turns[8];
-        angles(turns);
-        weights(a.k_weight);
-        for (; h < min(h1, q_heads + kv_heads); h++) {
+      if (h < min(end, end_k)) {
+        Turn<double> t[8];
+        angles(t);
+        half8_t w0 = {}, w1 = {};
+        if (a.k_weight) w0 = *(const half8_t*)(a.k_weight + x0), w1 = *(const half8_t*)(a.k_weight + x1);
+        uint8_t* const to = c.key + at.page * c.stride_kp + at.slot * c.stride_ky;
+        half_t* const scale = (half_t*)c.key_scale + at.page * c.stride_ksp + at.slot * c.stride_ksy;
+        for (; h < end_k; h += step) {
           const half8_t c0 = n0, c1 = n1;
-          read(h + 1);
+          read(min(h + step, all - 1));
           double y[16];
-          turned(0.0, c0, c1, w0, w1, a.k_weight != nullptr, a.k_eps, turns, y);
-          if (at.page >= 0)
-            store8(0.0, y, c.key + at.page * c.stride_kp + at.slot * c.stride_ky + (h - q_heads) * c.stride_kz,
-                   (half_t*)c.key_scale + at.page * c.stride_ksp + at.slot * c.stride_ksy + (h - q_heads) * c.stride_ksz);
+#pragma unroll
+          for (int e = 0; e < 8; e++) y[e] = (double)(float)c0[e], y[8 + e] = (double)(float)c1[e];
+          if (a.k_weight) {
+            double sum = 0.0, sum1 = 0.0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) sum = fma(y[e], y[e], sum), sum1 = fma(y[8 + e], y[8 + e], sum1);
+            sum = !mine ? 0.0 : one ? sum : sum + sum1;
+            const double factor = 1.0 / sqrt(sum_of<W>(sum) / (double)a.d + (double)a.k_eps);
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = y[e] * factor * (double)(float)w0[e], y[8 + e] = y[8 + e] * factor * (double)(float)w1[e];
+          }
+          if (a.pairs) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              const double u = y[2 * e], v = y[2 * e + 1], x = u * t[e].cosine - v * t[e].sine, z = u * t[e].sine + v * t[e].cosine;
+              y[2 * e] = (e < 4 ? turn0 : turn1) ? x : e >= 4 && one ? y[2 * e - 8] : u;
+              y[2 * e + 1] = (e < 4 ? turn0 : turn1) ? z : e >= 4 && one ? y[2 * e - 7] : v;
+            }
+          } else if (turn0) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              const double u = y[e], v = y[8 + e];
+              y[e] = u * t[e].cosine - v * t[e].sine;
+              y[8 + e] = u * t[e].sine + v * t[e].cosine;
+            }
+          }
+          place_codes(0.0, y, to + (h - end_q) * c.stride_kz, scale + (h - end_q) * c.stride_ksz);
         }
       }
-      for (; h < h1; h++) {
+      uint8_t* const to = c.value + at.page * c.stride_vp + at.slot * c.stride_vy;
+      half_t* const scale = (half_t*)c.value_scale + at.page * c.stride_vsp + at.slot * c.stride_vsy;
+      for (; h < end; h += step) {
         const half8_t c0 = n0, c1 = n1;
-        read(h + 1);
+        read(min(h + step, all - 1));
         float y[16];
 #pragma unroll
         for (int e = 0; e < 8; e++) y[e] = (float)c0[e], y[8 + e] = (float)c1[e];
-        const int v = h - q_heads - kv_heads;
-        if (at.page >= 0)
-          store8(0.0f, y, c.value + at.page * c.stride_vp + at.slot * c.stride_vy + v * c.stride_vz,
-                 (half_t*)c.value_scale + at.page * c.stride_vsp + at.slot * c.stride_vsy + v * c.stride_vsz);
+        place_codes(0.0f, y, to + (h - end_k) * c.stride_vz, scale + (h - end_k) * c.stride_vsz);
       }
     }
     if constexpr (CACHE == F16) {
       const adr_paged_cache& c = a.cache;
-      for (; h < h1; h++) {
+      half_t* const to = (half_t*)c.value + at.page * c.stride_vp + at.slot * c.stride_vy;
+      for (; h < end; h += step) {
         const half8_t c0 = n0, c1 = n1;
-        read(h + 1);
-        const int v = h - q_heads - kv_heads;
-        if (at.page >= 0) store16((half_t*)c.value + at.page * c.stride_vp + at.slot * c.stride_vy + v * c.stride_vz, c0, c1);
+        read(min(h + step, all - 1));
+        store16(to + (h - end_k) * c.stride_vz, c0, c1);
       }
     }
   }
@@ -524,14 +571,13 @@ hipError_t launch_place_into(hipStream_t stream, const PlaceArgs& a) {
     return hipGetLastError();
   }
   const int lanes = a.pairs ? (a.d + 15) / 16 : a.dims / 16 + (a.d - a.dims + 15) / 16;
+  job.lanes = lanes;
   const int W = lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : 32;
-  // Groups that share a row's heads: one for each where there are few rows, fewer where the rows alone make 16 wavefronts for
-  // each of 256 compute units.
-  const int64_t groups = (int64_t)256 * 16 * (64 / W);
-  int64_t splits = std::min<int64_t>(std::max<int64_t>((groups + a.rows - 1) / a.rows, 1), heads);
-  job.heads_each = (int)((heads + splits - 1) / splits);
-  job.splits = (int)((heads + job.heads_each - 1) / job.heads_each);
-  const unsigned grid = (unsigned)std::min<int64_t>(((int64_t)a.rows * job.splits * W + 255) / 256, MOST);
+  // Wavefronts that share a row: one for each of its steps where there are few rows, fewer where the rows alone make 16
+  // wavefronts for each of 256 compute units.
+  const int64_t steps = (heads + 64 / W - 1) / (64 / W);
+  job.splits = (int)std::min<int64_t>(std::max<int64_t>((256 * 16 + a.rows - 1) / a.rows, 1), steps);
+  const unsigned grid = (unsigned)std::min<int64_t>(((int64_t)a.rows * job.splits + 3) / 4, MOST);
   if (W == 4) hipLaunchKernelGGL(HIP_KERNEL_NAME(place_kernel<CACHE, 4>), dim3(grid), dim3(256), 0, stream, job);
   else if (W == 8) hipLaunchKernelGGL(HIP_KERNEL_NAME(place_kernel<CACHE, 8>), dim3(grid), dim3(256), 0, stream, job);
   else if (W == 16) hipLaunchKernelGGL(HIP_KERNEL_NAME(place_kernel<CACHE, 16>), dim3(grid), dim3(256), 0, stream, job);
