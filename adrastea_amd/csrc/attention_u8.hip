@@ -4,7 +4,10 @@
 //   out = sum_x softmax_x(scale s / temp) (V[x] - 127.5) vs[x]
 //
 // Codes less 128 are exact in fp16, so scores are 32-bit sums of exact products, which begin at sum(q) / 2 and are multiplied by
-// the key's scale once; (V - 128) vs + vs / 2 is one fused step to fp16, the values that the codes stand for, rounded once.
+// the key's scale once.  A value's scale is a power of two times a factor below 2: (V - 127.5) 2^e is exact in fp16 too, and the
+// factor goes into the probability, so that nothing is rounded that is not in 16 bits.  (With values rounded to fp16 the results
+// of a batch of tokens were 0.00033 off in the mean, of their root mean square, now 0.00028, where the last rounding to fp16 alone is
+// 0.00021.)
 // A key whose scales are no finite numbers, or which is on no page, has NaN for a key's scale and 0 for a value's: rows that see
 // it become NaN, and to the others it is a finite value of weight 0.
 //
@@ -29,6 +32,24 @@ __device__ __forceinline__ half8_t centred(uint32_t w0, uint32_t w1) {
     r[2 * i] = h[0], r[2 * i + 1] = h[1];
   }
   return r;
+}
+
+// Probabilities have a factor below 2 more than in attention_sequences.hip.
+constexpr float GROWN_U8 = GROWN - 1.0f;
+
+// The powers of two in eight scales (2^-14 at least), and what is left of them, for scales below 2^15.
+__device__ __forceinline__ void split_scales(half8_t s, half8_t& power, half8_t& factor) {
+  const u32x4_t bits = __builtin_bit_cast(u32x4_t, s);
+  u32x4_t p, r;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+    const ushort2_t e = __builtin_elementwise_max(__builtin_bit_cast(ushort2_t, bits[i] & 0x7c007c00u), ushort2_t{0x0400, 0x0400});
+    p[i] = __builtin_bit_cast(uint32_t, e);
+    r[i] = __builtin_bit_cast(uint32_t, (ushort2_t)(ushort2_t{0x7800, 0x7800} - e));
+  }
+  power = __builtin_bit_cast(half8_t, p);
+  factor = s * __builtin_bit_cast(half8_t, r);
 }
 
 // Where in a 256-byte line of the value tile a 16-byte chunk lies: the transposing reads of 32 lanes take a chunk each of rows
@@ -324,13 +345,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
     x = fmaxf(x, y), y = x;
     swap_rows(x, y);
     const float top = above(fmaxf(x, y) * a.c);
-    if (__builtin_amdgcn_ballot_w64(top > m_run + GROWN) != 0) {
+    if (__builtin_amdgcn_ballot_w64(top > m_run + GROWN_U8) != 0) {
       const float m_new = fmaxf(m_run, top - BELOW), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
       l_run *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; db++) o[db] *= alpha;
     }
+    half8_t power, factor;
+    split_scales(__builtin_shufflevector(vs[0], vs[1], 0, 1, 2, 3, 4, 5, 6, 7), power, factor);
     float sum[2] = {0.0f, 0.0f};
     u32x4_t pf;
 #pragma unroll
@@ -342,15 +365,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
         for (int j = 0; j < 2; j++) {
           e[j] = __builtin_amdgcn_exp2f(fmaf(s[kb][r + j], a.c, -m_run));
           sum[j] += e[j];
+          e[j] *= (float)factor[4 * kb + r + j];
         }
         pf[kb * 2 + r / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(e, half2_t));
       }
     l_run += sum[0] + sum[1];
-    const half8_t scale = __builtin_shufflevector(vs[0], vs[1], 0, 1, 2, 3, 4, 5, 6, 7);
-    const half8_t half_scale = scale * (half_t)0.5f;
+    const half8_t half_power = power * (half_t)0.5f;
 #pragma unroll
     for (int db = 0; db < DB; db++) {
-      const half8_t v = __builtin_elementwise_fma(centred((uint32_t)vc[db][0], (uint32_t)vc[db][1]), scale, half_scale);
+      const half8_t v = __builtin_elementwise_fma(centred((uint32_t)vc[db][0], (uint32_t)vc[db][1]), power, half_power);
       o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, __builtin_bit_cast(half8_t, pf), o[db], 0, 0, 0);
     }
   };
