@@ -1,14 +1,17 @@
 // Attention over a paged cache in 8 bits: code c of key x stands for (c - 127.5) ks[x], of its value for (c - 127.5) vs[x].
 //
-//   s[x] = <q, K[x] - 127.5> ks[x]                    = (<q, K[x] - 128> + sum(q) / 2) ks[x]
-//   out = sum_x softmax_x(scale s / temp) (V[x] - 127.5) vs[x]
+//   s[x] = <q, K[x] - 127.5> ks[x],   out = sum_x w[x] (V[x] - 127.5) / sum_x softmax weights,   w[x] = weight of x times vs[x]
 //
-// Codes less 128 are exact in fp16, so scores are 32-bit sums of exact products, which begin at sum(q) / 2 and are multiplied by
-// the key's scale once.  A value's scale is a power of two times a factor below 2: (V - 127.5) 2^e is exact in fp16 too, and the
-// factor goes into the probability, so that nothing is rounded that is not in 16 bits.  (With values rounded to fp16 the results
-// of a batch of tokens were 0.00033 off in the mean, of their root mean square, now 0.00028, where the last rounding to fp16 alone is
-// 0.00021.)
-// A key whose scales are no finite numbers, or which is on no page, has NaN for a key's scale and 0 for a value's: rows that see
+// The matrix cores are given the codes as they are: a byte, widened, is the fp16 number c 2^-24, exact, and below the normal
+// numbers, which are not flushed.  So scores are 32-bit sums of exact products that begin at -127.5 sum(q) and are multiplied by the
+// key's scale once; a value's scale goes into the probability, the only thing that is rounded, and 127.5 times the sum of the
+// rounded probabilities (one more product, with ones) is taken off at the end.  (With values rounded to fp16 the results of a batch of
+// tokens were 0.00033 off in the mean, of their root mean square, now 0.00027, where the last rounding to fp16 alone is 0.00021.)
+//
+// What is kept within fp16's range is thus the probability times the value's scale: a row's reference follows the largest
+// s c + log2 vs, as attention_sequences.hip says of s c, with vs taken as 2^-25 where it is less (a key of such values may have
+// all the weight; then the others' part of the result is below fp16's numbers).
+// A key whose scales are no numbers of the format, or which is on no page, has NaN for a key's scale and 0 for a value's: rows that see
 // it become NaN, and to the others it is a finite value of weight 0.
 //
 // Who does what, the softmax and the parts that are joined are those of attention_sequences.hip.
@@ -22,35 +25,16 @@ namespace {
 
 __global__ __launch_bounds__(256) void attention_u8_any_layout_kernel(Job) { rows_one_by_one<true>(arguments()); }
 
-// Eight codes, less 128: 0x6400 | c is the fp16 number 1024 + c.
-__device__ __forceinline__ half8_t centred(uint32_t w0, uint32_t w1) {
-  const half2_t bias = {(half_t)1152.0f, (half_t)1152.0f};
-  half8_t r;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const half2_t h = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, i < 2 ? w0 : w1, i & 1 ? 0x04030402u : 0x04010400u)) - bias;
-    r[2 * i] = h[0], r[2 * i + 1] = h[1];
-  }
-  return r;
+// Eight codes c as c 2^-24.
+__device__ __forceinline__ half8_t widened(uint32_t w0, uint32_t w1) {
+  const u32x4_t r = {__builtin_amdgcn_perm(0u, w0, 0x0c010c00u), __builtin_amdgcn_perm(0u, w0, 0x0c030c02u),
+                     __builtin_amdgcn_perm(0u, w1, 0x0c010c00u), __builtin_amdgcn_perm(0u, w1, 0x0c030c02u)};
+  return __builtin_bit_cast(half8_t, r);
 }
+constexpr float WIDENED = 0x1p-24f;
 
-// Probabilities have a factor below 2 more than in attention_sequences.hip.
-constexpr float GROWN_U8 = GROWN - 1.0f;
-
-// The powers of two in eight scales (2^-14 at least), and what is left of them, for scales below 2^15.
-__device__ __forceinline__ void split_scales(half8_t s, half8_t& power, half8_t& factor) {
-  const u32x4_t bits = __builtin_bit_cast(u32x4_t, s);
-  u32x4_t p, r;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
-    const ushort2_t e = __builtin_elementwise_max(__builtin_bit_cast(ushort2_t, bits[i] & 0x7c007c00u), ushort2_t{0x0400, 0x0400});
-    p[i] = __builtin_bit_cast(uint32_t, e);
-    r[i] = __builtin_bit_cast(uint32_t, (ushort2_t)(ushort2_t{0x7800, 0x7800} - e));
-  }
-  power = __builtin_bit_cast(half8_t, p);
-  factor = s * __builtin_bit_cast(half8_t, r);
-}
+// The largest probability times scale may be this much above the reference, in log2 units.
+constexpr float GROWN_U8 = GROWN - 0.5f;
 
 // Where in a 256-byte line of the value tile a 16-byte chunk lies: the transposing reads of 32 lanes take a chunk each of rows
 // 4 g ... 4 g + 3 and 16 + 4 g ... 16 + 4 g + 3 of two g, and these 16 are on different banks.
@@ -68,47 +52,40 @@ __device__ __forceinline__ void transfer_once(uint32_t lds, const uint32_t (&vof
                  :: "s"(lds), "v"(voff[0]), "s"(desc) : "memory");
 }
 
-// The scales of 16 keys of a page from slot `slot` on, those behind `left` 0; for values, what does not fit 0 as well.  `bad`: a
-// bit for each key that has one that does not fit.
+// The scales of 16 keys of a page, of which `left` are there (what comes for the others does not count).
 struct Scales {
   u32x4_t lo, hi;
 };
-template <typename Fits>
-__device__ __forceinline__ Scales read_scales(const half_t* p, int64_t step, bool side_by_side, int left, Fits fits, uint32_t& bad) {
-  uint16_t v[16];
+__device__ __forceinline__ Scales read_scales(const half_t* p, int64_t step, bool side_by_side, int left) {
+  Scales s;
   if (side_by_side) {
-    const u32x4_t lo = *(const u32x4_t*)p, hi = *(const u32x4_t*)(p + 8);
-    __builtin_memcpy(v, &lo, 16);
-    __builtin_memcpy(v + 8, &hi, 16);
+    s.lo = *(const u32x4_t*)p, s.hi = *(const u32x4_t*)(p + 8);
   } else {
+    uint16_t v[16];
 #pragma unroll
     for (int e = 0; e < 16; e++) v[e] = half_to_bits(p[min(e, left - 1) * step]);
+    __builtin_memcpy(&s, v, 32);
   }
-  bad = 0;
-#pragma unroll
-  for (int e = 0; e < 16; e++) {
-    if (e >= left) v[e] = 0;
-    if (!fits(bits_to_half(v[e]))) bad |= 1u << e;
-  }
-  Scales s;
-  __builtin_memcpy(&s.lo, v, 16);
-  __builtin_memcpy(&s.hi, v + 8, 16);
   return s;
 }
 
 // ---- few rows: generation, a few tokens or a small draft at once ---------------------------------------------
 //
-// A block of 16 rows against its keys, as attention_few_rows_kernel: tiles of 32 keys, two of each wavefront's in LDS.  A tile's
+// A block of 16 rows against its keys, as attention_few_rows_kernel: tiles of 32 keys, four of each wavefront's in LDS.  A tile's
 // codes go from LDS to registers as they are, values through the transposing read of bytes, and become fp16 there.
-template <int HD, int WAVES, bool SHARED, bool TREE>
+constexpr int few_ahead(int) { return 8; }
+constexpr int few_bytes(int hd, int depth) { return 2 * depth * FEW_KEYS * hd + 3 * 2 * few_ahead(hd) * FEW_KEYS * 2; }  // of LDS, a wavefront
+
+template <int HD, int WAVES, int DEPTH, bool SHARED, bool TREE>
 __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Job) {
   constexpr int CPR = HD / 16, KEYS = 32, ROWS = 16;
   constexpr int ROWB = HD, TILE = KEYS * ROWB;      // bytes of a tile row, of a K or V tile
   constexpr int NI = TILE / 1024;                   // transfers per tile
   constexpr int KP = HD / 64, DB = HD / 16;         // pairs of k-steps of S, blocks of 16 output columns
-  constexpr int AHEAD = 16;                         // tiles whose addresses are looked up at once
-  constexpr int SCALES = 4 * TILE;                  // K0 K1 V0 V1 of a wavefront, then 32 tiles' scales, of keys and of values
-  constexpr int WAVE = SCALES + 4 * AHEAD * KEYS * 2;
+  constexpr int AHEAD = few_ahead(HD);              // tiles whose addresses are looked up at once
+  constexpr int SCALES = 2 * DEPTH * TILE;          // K0 ... V0 ... of a wavefront, then twice as many tiles' scales:
+  constexpr int KIND = 2 * AHEAD * KEYS * 2;        // bytes of those of keys, of values, and of their logarithms
+  constexpr int WAVE = few_bytes(HD, DEPTH);
   constexpr int PITCH = HD + 4;                     // of the partial results' rows, in floats
   constexpr int BIAS = NI / 2 * 1024;               // bytes that descriptors start ahead, so that no offset is negative
   static_assert(16 * (PITCH + 2) * 4 + 16 <= WAVE, "the partial results fit the tiles' LDS");
@@ -151,14 +128,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
 
   const uint32_t lds0 = (uint32_t)(uintptr_t)ADR_LDS_PTR(smem) + w * WAVE;
   unsigned char* const sm = smem + w * WAVE;
-  // The queries' fragments, by way of the second tile of values: of 64 columns a lane has 16, 8 to each of two k-steps, as
+  // The queries' fragments, by way of the last tile of values: of 64 columns a lane has 16, 8 to each of two k-steps, as
   // it reads 16 codes of a key at once.  (Chunks behind the head dimension are zeros below.)
   const int d = a.d, k_stride = (int)a.sk.y, v_stride = (int)a.sv.y;
   const half_t* const qrow = a.q + (int64_t)(hk * a.group + gh) * a.sq_z + (int64_t)(q.row0 + row) * a.sq_y;
 #pragma unroll
   for (int ks = 0; ks < 2 * KP; ks++) {
     const int col = (ks >> 1) * 64 + g * 16 + (ks & 1) * 8;
-    dma_global(lds0 + 3 * TILE + ks * 1024, qrow + (col < d ? col : 0));
+    dma_global(lds0 + SCALES - TILE + ks * 1024, qrow + (col < d ? col : 0));
   }
   // Byte offsets of a lane's chunks in 16 rows; chunks behind the head dimension lie behind every descriptor's end and come
   // as zeros.  Values' chunks are placed differently in the second 16 rows.
@@ -178,26 +155,24 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
   // scales, which go to LDS.  (Code addresses are as they come; bit 63 says that there are keys.)
   const bool side_by_side = a.sks.y == 1 && a.svs.y == 1 && (a.sks.z | a.sks.p | a.svs.z | a.svs.p) % 8 == 0 &&
                             ((uintptr_t)a.k_scale | (uintptr_t)a.v_scale) % 16 == 0;
-  uint32_t at_lo = 0, at_hi = 0;
+  uint32_t at_lo = 0, at_hi = 0, bad = 0;
+  Scales looked_up;
   auto look_up = [&](int i) __attribute__((always_inline)) {
     Args c = arguments();
-    const int t = i + (lane >> 1 & 15), key = (tile0 + w + WAVES * t) * KEYS + 16 * (lane & 1), left = row_end - key;
+    const int t = i + (lane >> 1 & (AHEAD - 1)), key = (tile0 + w + WAVES * t) * KEYS + 16 * (lane & 1), left = row_end - key;
     const bool is_v = lane >= 32;
     uint64_t at = 0;  // (no keys)
-    Scales s = {};
-    uint32_t bad = 0;
-    if (left > 0) {
+    looked_up = {}, bad = 0;
+    if (left > 0 && (lane & 31) < 2 * AHEAD) {
       const int page = c.table[(int64_t)q.index * c.table_pitch + (key >> c.page_shift)];
       const int slot = key & ((1 << c.page_shift) - 1);
       if (page >= 0 && page < c.pages) {
         if (is_v) {
           at = (uint64_t)c.v + hk * c.sv.z + page * c.sv.p + slot * c.sv.y - BIAS;
-          s = read_scales(c.v_scale + hk * c.svs.z + page * c.svs.p + slot * c.svs.y, c.svs.y, side_by_side, left,
-                          value_scale_fits, bad);
+          looked_up = read_scales(c.v_scale + hk * c.svs.z + page * c.svs.p + slot * c.svs.y, c.svs.y, side_by_side, left);
         } else {
           at = (uint64_t)c.k + hk * c.sk.z + page * c.sk.p + slot * c.sk.y - BIAS;
-          s = read_scales(c.k_scale + hk * c.sks.z + page * c.sks.p + slot * c.sks.y, c.sks.y, side_by_side, left,
-                          key_scale_fits, bad);
+          looked_up = read_scales(c.k_scale + hk * c.sks.z + page * c.sks.p + slot * c.sks.y, c.sks.y, side_by_side, left);
         }
         at |= 1ull << 63;
       } else {
@@ -205,17 +180,38 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
       }
     }
     at_lo = (uint32_t)at, at_hi = (uint32_t)(at >> 32);
-    bad |= __shfl_xor((int)bad, 32);
-    if (bad) {
-      uint16_t v[16];
-      __builtin_memcpy(v, &s, 32);
+  };
+  // The scales that were looked up, to LDS: of keys that a tile does not have 0, and of those that count as NaN as said above.
+  // (Apart from the above, so that the first transfers do not wait for them.)
+  auto keep_scales = [&](int i) __attribute__((always_inline)) {
+    const int t = i + (lane >> 1 & (AHEAD - 1)), left = row_end - (tile0 + w + WAVES * t) * KEYS - 16 * (lane & 1);
+    const bool is_v = lane >= 32;
+    uint16_t v[16];
+    __builtin_memcpy(v, &looked_up, 32);
 #pragma unroll
-      for (int e = 0; e < 16; e++)
-        if (bad >> e & 1) v[e] = is_v ? 0 : 0x7e00;
-      __builtin_memcpy(&s, v, 32);
+    for (int e = 0; e < 16; e++) {
+      if (e >= left) v[e] = 0;
+      if (!scale_fits(bits_to_half(v[e]))) bad |= 1u << e;
     }
-    u32x4_t* const to = (u32x4_t*)(sm + SCALES + (is_v ? 2 * AHEAD * KEYS * 2 : 0) + ((t & (2 * AHEAD - 1)) * KEYS + 16 * (lane & 1)) * 2);
-    to[0] = s.lo, to[1] = s.hi;
+    bad |= __shfl_xor((int)bad, 32);
+#pragma unroll
+    for (int e = 0; e < 16; e++)
+      if (bad >> e & 1) v[e] = is_v ? 0 : 0x7e00;
+    if ((lane & 31) < 2 * AHEAD) {
+      unsigned char* const to = sm + SCALES + ((t & (2 * AHEAD - 1)) * KEYS + 16 * (lane & 1)) * 2;
+      Scales s;
+      __builtin_memcpy(&s, v, 32);
+      u32x4_t* const here = (u32x4_t*)(to + (is_v ? KIND : 0));
+      here[0] = s.lo, here[1] = s.hi;
+      if (is_v) {
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+          v[e] = half_to_bits((half_t)__builtin_amdgcn_logf(fmaxf(fabsf((float)bits_to_half(v[e])), 0x1p-25f)));
+        __builtin_memcpy(&s, v, 32);
+        u32x4_t* const logs = (u32x4_t*)(to + 2 * KIND);
+        logs[0] = s.lo, logs[1] = s.hi;
+      }
+    }
   };
   // Keys, or values, of tile i.
   auto fetch = [&](int i, auto is_k) __attribute__((always_inline)) {
@@ -226,42 +222,56 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
       const int l = (IS_K ? 0 : 32) + 2 * (i & (AHEAD - 1)) + h, left = min(row_end - (tile0 + w + WAVES * i) * KEYS - 16 * h, 16);
       const uint32_t lo = __builtin_amdgcn_readlane(at_lo, l), hi = __builtin_amdgcn_readlane(at_hi, l);
       const u32x4_t desc = {lo, hi & 0xffffu, hi >> 31 ? (uint32_t)((left - 1) * stride + d + BIAS) : 0u, 0x00020000u};
-      transfer_once<NI / 2>(lds0 + ((IS_K ? 0 : 2) + (i & 1)) * TILE + h * (NI / 2) * 1024, IS_K ? koff : voff[h], desc);
+      transfer_once<NI / 2>(lds0 + ((IS_K ? 0 : DEPTH) + (i & (DEPTH - 1))) * TILE + h * (NI / 2) * 1024, IS_K ? koff : voff[h], desc);
     }
   };
   const std::true_type is_k{};
   const std::false_type is_v{};
 
+  // All transfers but the last n of K or V tiles have landed (n: at most 2 DEPTH - 1).
+  auto wait_tiles = [&](int n) __attribute__((always_inline)) {
+    static_assert((DEPTH == 2 || DEPTH == 4) && (2 * DEPTH - 1) * NI < 64, "as many as are told apart here");
+    if (DEPTH > 2 && n == 7) wait_vm<7 * NI>();
+    else if (DEPTH > 2 && n == 6) wait_vm<6 * NI>();
+    else if (DEPTH > 2 && n == 5) wait_vm<5 * NI>();
+    else if (DEPTH > 2 && n == 4) wait_vm<4 * NI>();
+    else if (n == 3) wait_vm<3 * NI>();
+    else if (n == 2) wait_vm<2 * NI>();
+    else if (n == 1) wait_vm<NI>();
+    else wait_vm<0>();
+  };
+
   look_up(0);
   asm volatile("" : "+v"(at_lo), "+v"(at_hi));
-  // (the lookup's loads have landed before the transfers' own count begins)
-  if (tiles > 0) fetch(0, is_k), fetch(0, is_v);
-  if (tiles > 1) fetch(1, is_k);
-  if (tiles > 1) wait_vm<3 * NI>();
-  else if (tiles > 0) wait_vm<2 * NI>();
-  else wait_vm<0>();
+#pragma unroll
+  for (int t = 0; t < DEPTH; t++) {
+    if (t < tiles) fetch(t, is_k);
+    if (t < tiles && t + 1 < DEPTH) fetch(t, is_v);
+  }
+  keep_scales(0);
+  wait_tiles(2 * min(tiles, DEPTH) - (tiles >= DEPTH));
   half8_t qf[2 * KP];
-  float half_sum = 0.0f;
+  float first_sum = 0.0f;
 #pragma unroll
   for (int ks = 0; ks < 2 * KP; ks++) {
-    qf[ks] = *(const half8_t*)(sm + 3 * TILE + ks * 1024 + lane * 16);
+    qf[ks] = *(const half8_t*)(sm + SCALES - TILE + ks * 1024 + lane * 16);
     if ((ks >> 1) * 64 + g * 16 + (ks & 1) * 8 >= d) qf[ks] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
   }
 #pragma unroll
   for (int ks = 0; ks < 2 * KP; ks++) asm volatile("" : "+v"(qf[ks]));
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  if (tiles > 1) fetch(1, is_v);
+  if (tiles >= DEPTH) fetch(DEPTH - 1, is_v);
 #pragma unroll
   for (int ks = 0; ks < 2 * KP; ks++)
 #pragma unroll
-    for (int e = 0; e < 8; e++) half_sum += (float)qf[ks][e];
+    for (int e = 0; e < 8; e++) first_sum += (float)qf[ks][e];
   {
-    float x = half_sum, y = x;  // over the four lanes that share a row
+    float x = first_sum, y = x;  // over the four lanes that share a row
     swap_halves(x, y);
     x = x + y, y = x;
     swap_rows(x, y);
-    half_sum = 0.5f * (x + y);
-    if (!(fabsf(half_sum) < INFINITY)) half_sum = NAN;
+    first_sum = -127.5f * WIDENED * (x + y);
+    if (!(fabsf(first_sum) < INFINITY)) first_sum = NAN;
   }
   int offK[KP], offV[DB];
 #pragma unroll
@@ -281,79 +291,91 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
 #pragma unroll
   for (int db = 0; db < DB; db++) o[db] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
   const int end = min(end_of_row(a, q, row), row_end) - 4 * g;  // this lane's first key that its row does not see
-  // Tile i; `next`: there is a tile i + 1, `more`: and a tile i + 2.
-  auto tile = [&](int i, auto next, auto more) __attribute__((always_inline)) {
-    constexpr bool NEXT = decltype(next)::value, MORE = decltype(more)::value;
-    wait_vm<NEXT ? 3 * NI : NI>();  // its keys have landed
-    const unsigned char* const cK = sm + (i & 1) * TILE;
-    const unsigned char* const cV = sm + (2 + (i & 1)) * TILE;
+  // (of the block's first row, which sees the fewest; of a draft, what is in front of it)
+  const int common_end = min(row_end, uniform(TREE ? end_of_common(a, q, 0) : end_of_row(a, q, row_of_list(a, block * ROWS))));
+  const float c = a.c / WIDENED;  // (scores are times 2^-24)
+  float4_t ones = {0.0f, 0.0f, 0.0f, 0.0f};
+  half8_t all_ones;
+#pragma unroll
+  for (int e = 0; e < 8; e++) all_ones[e] = (half_t)1;
+  for (int i = 0; i < tiles; i++) {
+    const int ahead = min(tiles - i, DEPTH);  // tiles that are in LDS or on their way
+    const bool more = i + DEPTH < tiles;      // the next of them is asked for as soon as the fragments of this one are in registers
+    wait_tiles(2 * ahead - 1);                // its keys have landed
+    const unsigned char* const cK = sm + (i & (DEPTH - 1)) * TILE;
+    const unsigned char* const cV = sm + (DEPTH + (i & (DEPTH - 1))) * TILE;
     u32x4_t kc[2][KP];
-    half4_t ks[2], vs[2];
+    half4_t ks[2], vs[2], log_vs[2];
 #pragma unroll
     for (int kb = 0; kb < 2; kb++) {
 #pragma unroll
       for (int kp = 0; kp < KP; kp++) kc[kb][kp] = *(const u32x4_t*)(cK + offK[kp] + kb * 16 * ROWB);
       const unsigned char* const scales = sm + SCALES + ((i & (2 * AHEAD - 1)) * KEYS + 16 * kb + 4 * g) * 2;
       ks[kb] = *(const half4_t*)scales;
-      vs[kb] = *(const half4_t*)(scales + 2 * AHEAD * KEYS * 2);
+      vs[kb] = *(const half4_t*)(scales + KIND);
+      log_vs[kb] = *(const half4_t*)(scales + 2 * KIND);
     }
     float4_t s[2];
 #pragma unroll
-    for (int kb = 0; kb < 2; kb++) s[kb] = float4_t{half_sum, half_sum, half_sum, half_sum};
+    for (int kb = 0; kb < 2; kb++) s[kb] = float4_t{first_sum, first_sum, first_sum, first_sum};
 #pragma unroll
     for (int kp = 0; kp < KP; kp++)
 #pragma unroll
       for (int h = 0; h < 2; h++)
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
-          s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(centred(kc[kb][kp][2 * h], kc[kb][kp][2 * h + 1]), qf[2 * kp + h], s[kb], 0, 0, 0);
-    if constexpr (MORE) {
+          s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(widened(kc[kb][kp][2 * h], kc[kb][kp][2 * h + 1]), qf[2 * kp + h], s[kb], 0, 0, 0);
+    if (more) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (((i + 2) & (AHEAD - 1)) == 0) {
-        look_up(i + 2);
+      const bool looks = ((i + DEPTH) & (AHEAD - 1)) == 0;
+      if (looks) {
+        look_up(i + DEPTH);
         asm volatile("" : "+v"(at_lo), "+v"(at_hi));
       }
-      fetch(i + 2, is_k);
+      fetch(i + DEPTH, is_k);
+      if (looks) keep_scales(i + DEPTH);
     }
-    wait_vm<MORE ? 3 * NI : NEXT ? 2 * NI : 0>();  // and its values
+    wait_tiles(more ? 2 * DEPTH - 1 : 2 * ahead - 2);  // and its values
     int2_t vc[DB];
 #pragma unroll
     for (int db = 0; db < DB; db++) vc[db] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2_t*)ADR_LDS_PTR(cV + offV[db]));
-    if constexpr (MORE) {
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-      for (int db = 0; db < DB; db++) asm volatile("" : "+v"(vc[db]));
-      fetch(i + 2, is_v);
-    }
-    const int left = end - (tile0 + w + WAVES * i) * KEYS;  // keys of this lane's row from its first one on
-    uint32_t seen = ~0u;
-    if constexpr (TREE) {
-      const int drafted = (tile0 + w + WAVES * i) * KEYS - (q.keys - q.rows);  // of the tile's first key
-      if (drafted > -KEYS) seen = tree_window(a, q.row0 + row, drafted) >> 4 * g;
+    for (int db = 0; db < DB; db++) asm volatile("" : "+v"(vc[db]));
+    if (more) fetch(i + DEPTH, is_v);
+    const int key0 = (tile0 + w + WAVES * i) * KEYS;
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) s[kb][r] *= (float)ks[kb][r];
+    if (key0 + KEYS > common_end) {  // keys that some row does not see
+      const int left = end - key0;   // of this lane's row from its first one on
+      uint32_t seen = ~0u;
+      if constexpr (TREE) seen = tree_window(a, q.row0 + row, key0 - (q.keys - q.rows)) >> 4 * g;
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          if (16 * kb + r >= left || (TREE && !(seen >> (16 * kb + r) & 1))) s[kb][r] = -INFINITY;
     }
     float mx = NO_SCORE;
 #pragma unroll
     for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        s[kb][r] *= (float)ks[kb][r];
-        if (16 * kb + r >= left || (TREE && !(seen >> (16 * kb + r) & 1))) s[kb][r] = -INFINITY;
-        mx = fmaxf(mx, s[kb][r]);
-      }
+      for (int r = 0; r < 4; r++) mx = fmaxf(mx, fmaf(s[kb][r], c, (float)log_vs[kb][r]));
     float x = mx, y = mx;  // over the four lanes that share a row
     swap_halves(x, y);
     x = fmaxf(x, y), y = x;
     swap_rows(x, y);
-    const float top = above(fmaxf(x, y) * a.c);
+    const float top = above(fmaxf(x, y));
     if (__builtin_amdgcn_ballot_w64(top > m_run + GROWN_U8) != 0) {
       const float m_new = fmaxf(m_run, top - BELOW), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
       l_run *= alpha;
+      ones *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; db++) o[db] *= alpha;
     }
-    half8_t power, factor;
-    split_scales(__builtin_shufflevector(vs[0], vs[1], 0, 1, 2, 3, 4, 5, 6, 7), power, factor);
     float sum[2] = {0.0f, 0.0f};
     u32x4_t pf;
 #pragma unroll
@@ -363,26 +385,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
         float2_t e;
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-          e[j] = __builtin_amdgcn_exp2f(fmaf(s[kb][r + j], a.c, -m_run));
+          e[j] = __builtin_amdgcn_exp2f(fmaf(s[kb][r + j], c, -m_run));
           sum[j] += e[j];
-          e[j] *= (float)factor[4 * kb + r + j];
+          e[j] *= (float)vs[kb][r + j];
         }
         pf[kb * 2 + r / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(e, half2_t));
       }
     l_run += sum[0] + sum[1];
-    const half8_t half_power = power * (half_t)0.5f;
+    ones = __builtin_amdgcn_mfma_f32_16x16x32_f16(all_ones, __builtin_bit_cast(half8_t, pf), ones, 0, 0, 0);
 #pragma unroll
-    for (int db = 0; db < DB; db++) {
-      const half8_t v = __builtin_elementwise_fma(centred((uint32_t)vc[db][0], (uint32_t)vc[db][1]), power, half_power);
-      o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, __builtin_bit_cast(half8_t, pf), o[db], 0, 0, 0);
-    }
-  };
-  const std::true_type yes{};
-  const std::false_type no{};
-  int i = 0;
-  for (; i + 2 < tiles; i++) tile(i, yes, yes);
-  if (i + 1 < tiles) tile(i++, yes, no);
-  if (i < tiles) tile(i, no, no);
+    for (int db = 0; db < DB; db++)
+      o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(widened((uint32_t)vc[db][0], (uint32_t)vc[db][1]),
+                                                     __builtin_bit_cast(half8_t, pf), o[db], 0, 0, 0);
+  }
 
   Args z = arguments();
   // Merge the wavefronts' results: [wavefront][row][HD] sums, and (maximum, sum) of every row.
@@ -396,7 +411,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
   swap_rows(x, y);
   if (g == 0) xml[w * 16 + frow] = make_float2(m_run, x + y);
 #pragma unroll
-  for (int db = 0; db < DB; db++) *(float4_t*)(xo + (w * 16 + frow) * PITCH + 16 * db + 4 * g) = o[db];
+  for (int db = 0; db < DB; db++)
+    *(float4_t*)(xo + (w * 16 + frow) * PITCH + 16 * db + 4 * g) = o[db] * (1.0f / WIDENED) - ones * 127.5f;
   __syncthreads();
   for (int e = tid; e < rows * (HD / 4); e += 64 * WAVES) {
     const int r = e / (HD / 4), col = e % (HD / 4) * 4;
@@ -475,7 +491,7 @@ SequencesPlan sequences_u8_plan(const SequencesArgs& a, int cus, int64_t avail) 
   (void)longest_rows;
   const double alone = longest * hd * 3.3e-5, all = blocks * longest * hd * 2 / 6e6;
   const bool unshared = blocks <= cus ? 4.0 + alone < 9.3 + all / 2 : alone < 9.0;
-  const int each = hd == 64 ? 2 : 1;
+  const int each = hd == 64 ? 8 : 4;
   p.parts = unshared ? 0 : std::max(1, each * cus / a.kv_heads);
   const int forced = knob(KNOB_SEQUENCES) >= 2 && knob(KNOB_SEQUENCES) <= 8 ? knob(KNOB_SEQUENCES) : 0;
   if (forced) p.parts = forced == 4 ? std::max(16, cus / a.kv_heads) : 0;
@@ -488,6 +504,8 @@ SequencesPlan sequences_u8_plan(const SequencesArgs& a, int cus, int64_t avail) 
   p.workspace_bytes = p.parts * part;
   return p;
 }
+
+constexpr int SHARED_DEPTH = 2;
 
 template <int HD, bool TREE>
 static hipError_t launch_blocks(hipStream_t stream, const SequencesArgs& a, const SequencesPlan& p, void* workspace) {
@@ -503,13 +521,12 @@ static hipError_t launch_blocks(hipStream_t stream, const SequencesArgs& a, cons
   const int64_t blocks = p.parts == 0 ? most_blocks(a, FEW) : (int64_t)p.parts * a.kv_heads;
   if (blocks > LAUNCH_BLOCKS) return hipErrorInvalidConfiguration;
   const int at_once = std::min(FEW, 1024 / HD);
-  const dim3 grid((unsigned)blocks), join((unsigned)((p.parts - 1) * a.kv_heads * (FEW / at_once))), threads(256);
-  const size_t lds = 4 * ((size_t)4 * FEW_KEYS * HD + 4096);
+  const dim3 grid((unsigned)blocks), join((unsigned)((p.parts - 1) * a.kv_heads * (FEW / at_once)));
   if (p.parts > 0) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_u8_few_rows_kernel<HD, 4, true, TREE>), grid, threads, lds, stream, job);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_u8_few_rows_kernel<HD, 2, SHARED_DEPTH, true, TREE>), grid, dim3(128), 2 * few_bytes(HD, SHARED_DEPTH), stream, job);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, FEW, true>), join, dim3(256), 0, stream, job);
   } else {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_u8_few_rows_kernel<HD, 4, false, TREE>), grid, threads, lds, stream, job);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_u8_few_rows_kernel<HD, 4, 4, false, TREE>), grid, dim3(256), 4 * few_bytes(HD, 4), stream, job);
   }
   return hipGetLastError();
 }

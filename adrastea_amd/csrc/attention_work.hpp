@@ -210,9 +210,8 @@ __device__ __forceinline__ void row_by_wave(Args a, const Sequence& q, int j, in
       O[(c * 64 + lane) * (int64_t)a.so_x] = mean_of(o[c] * inv);
 }
 
-// The same over codes.  A key counts as NaN where a scale of it is no finite number, or a value's so large that its codes are not.
-__device__ __forceinline__ bool key_scale_fits(half_t s) { return fabsf((float)s) < INFINITY; }
-__device__ __forceinline__ bool value_scale_fits(half_t s) { return fabsf((float)s) <= 513.5f; }
+// The same over codes.  A key counts as NaN where a scale of it is larger than those of the format, or no number.
+__device__ __forceinline__ bool scale_fits(half_t s) { return fabsf((float)s) <= 513.5f; }
 
 __device__ __forceinline__ void row_by_wave_u8(Args a, const Sequence& q, int j, int h, int lane, int col0 = 0, int col1 = GENERAL_MAX_D) {
   const int64_t row = (int64_t)q.row0 + j;
@@ -235,7 +234,7 @@ __device__ __forceinline__ void row_by_wave_u8(Args a, const Sequence& q, int j,
       if (page >= 0 && page < a.pages) {
         const half_t ks = a.k_scale[page * a.sks.p + slot * a.sks.y + hk * a.sks.z];
         const half_t vs = a.v_scale[page * a.svs.p + slot * a.svs.y + hk * a.svs.z];
-        good = key_scale_fits(ks) && value_scale_fits(vs);
+        good = scale_fits(ks) && scale_fits(vs);
         if (good) {
           const int64_t ko = page * a.sk.p + slot * a.sk.y;
           float sum = 0.0f, none = 0.0f;

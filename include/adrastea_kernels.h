@@ -598,10 +598,9 @@ int adr_read_u8(adr_stream_t stream, uint16_t* key, uint16_t* value, adr_paged_c
                 int32_t stride_vz);
 
 /*
- * Attention over a cache in 8 bits: as adr_attention_paged_f16 over the values that the codes stand for, which are not rounded
- * to fp16 where scores are computed, and once where they are summed.  A key of which either scale is no finite number, or the
- * value's is beyond 513.5, counts as NaN for the rows that see it and does not reach the others; rows of queries that are not
- * all finite are NaN where they see a key.
+ * Attention over a cache in 8 bits: as adr_attention_paged_f16 over the values that the codes stand for, which are not
+ * rounded.  A key of which either scale is beyond 513.5, infinite or NaN counts as NaN for the rows that see it and does not reach
+ * the others; rows of queries that are not all finite are NaN where they see a key.
  * The fast kernels take d a multiple of 16 up to 128, x strides 1, the codes' other strides multiples of 16 (the queries' and the
  * output's of 8) and not negative, slots at least d apart and less than 2^24, 16-byte aligned pointers, pages of 16, 32,
  * 64 ... slots; everything else runs on a kernel of one wavefront per row.  Scales that follow each other from slot to slot, a page's

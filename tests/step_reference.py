@@ -87,9 +87,11 @@ def attention(q, k, v, scale, temp, seen):
 
 
 def close_enough(got, want, value_max, keys, codes):
-    """As for the cache in 16 bits (sequences_reference.py), and where values are made of codes their rounding to fp16: 2^-11 of
-    sum w |v| <= value_max, and 2^-25.  Scores of codes are 32-bit sums too, of products that add up to those of the values and
-    half a scale for each query value: within the bound there, for which 2^5 is far from reached."""
+    """As for the cache in 16 bits (sequences_reference.py).  Values of codes are not rounded, but a step of 2^-11 more of sum
+    w |v| <= value_max is allowed (and 2^-25) for a kernel that rounds them to fp16 first.  Scores of codes are 32-bit sums of
+    d <= 128 products of codes up to 255, which begin at -127.5 sum(q): in the tests here sum |q| <= 110, scales <= 0.03 and
+    the factor is 1 / sqrt(d) >= 0.08, so that all of it adds up to less than 110 * 382 * 0.03 * 0.125 < 2^8 / 1.6 for d = 64 and
+    less than 2^7 for d = 128; an error of d 2^-24 of that is below 2^-11 in each exponent, as there."""
     want = np.asarray(want, np.float64)
     extra = value_max * 2.0 ** -11 + 2.0 ** -25 if codes else 0.0
     bound = (np.abs(want) * 2.0 ** -11 + 2.0 ** -25 + extra +

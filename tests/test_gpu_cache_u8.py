@@ -121,6 +121,9 @@ class Paged:
             out[a:a + r] = ref.attention(self.q[a:a + r].transpose(1, 0, 2), k, v, scale, temp, mask == CAUSAL).transpose(1, 0, 2)
         return out
 
+    def cache_scale(self, which, i, h, n):
+        return ref.gathered(self.cache.scales[which][..., None], self.cache.table[i], n)[h, :, 0].astype(np.float64)
+
     def check(self, scale, mask, temp=1.0):
         want, got = self.want(scale, mask, temp), self.out_t.cpu().numpy()
         n = self.row_offsets[-1]
@@ -289,7 +292,7 @@ def test_what_a_row_does_not_see_never_reaches_it(shared_keys, rows, keys, d):
     scale = 1.0 / np.sqrt(d)
     place = (p.cache.table[0, (keys - 1) // 16], slice(None), (keys - 1) % 16)
     clean = p.cache.scales.copy()
-    for which, bad in ((0, np.nan), (0, np.inf), (1, np.nan), (1, -np.inf), (1, 600.0)):
+    for which, bad in ((0, np.nan), (0, np.inf), (0, 514.0), (1, np.nan), (1, -np.inf), (1, 600.0)):
         p.cache.scales[:] = clean
         p.cache.scales[(which, *place)] = bad
         p.cache.upload()
@@ -326,6 +329,45 @@ def test_pages_outside_the_cache_are_nan_and_never_read(shared_keys):
         assert np.isnan(got[1:4]).all()
         rest = [0, 4, 5]
         assert step.close_enough(got[rest], want[rest], 127.5 * 0.03, 100, True)
+
+
+def test_values_of_very_different_sizes(shared_keys):
+    """A key with most of the weight whose values are tiny, or zero, beside keys of large values and little weight, and the other way
+    round: each as exact as the rest of the row allows.  Bounds: sums of the weights' roundings, 2^-11 of each |w v| and 2^-32 of the
+    row's largest |w v|'s scale a key, over the 32-bit sums' (keys + 127) 2^-23 of what they add up to, and the result's own."""
+    d, n = 64, 600
+    for first, rest, near in ((2.0 ** -24, 513.5, 8.0), (0.0, 513.5, 20.0), (513.5, 2.0 ** -24, -30.0), (0.01, 1e-6, -16.0), (1e-6, 0.01, 16.0),
+                              (0.0, 0.0, 1.0), (513.5, 2.0 ** -20, -60.0)):
+        p = Paged([(1, n), (2, n)], 2, 2, d, 16, seed=3)
+        for i in range(2):
+            for x in range(n):
+                at = (slice(None), p.cache.table[i, x // 16], slice(None), x % 16)
+                p.cache.scales[1][at[1:]] = first if x == 77 else rest
+                p.cache.scales[0][at[1:]] = 0.02
+                p.cache.codes[0][at[1:]] = 128 if x != 77 else 255
+        p.cache.upload()
+        p.q[:p.row_offsets[-1]] = 1.0
+        # the score of key 77 is `near` log2 units above the others'
+        step_of = 64 * 127 * float(np.float16(0.02))
+        scale = abs(near) * np.log(2) / step_of
+        if near < 0:
+            p.q[:p.row_offsets[-1]] = -1.0
+        shared_keys.attention_paged_u8(heads_view(p.out_t), heads_view(dev(p.q)), p.cache.handle, p.batch, scale)
+        got = p.out_t.cpu().numpy()
+        for i, (r, m) in enumerate(p.seqs):
+            k, v = p.cache.values(i, m)
+            for j in range(r):
+                row, end = p.row_offsets[i] + j, j + m - r + 1
+                for h in range(2):
+                    s = k[h, :end] @ p.q[row, h].astype(np.float64) * scale
+                    w = np.exp(s - s.max())
+                    w /= w.sum()
+                    want = w @ v[h, :end]
+                    each = (w[:, None] * np.abs(v[h, :end])).sum(0)
+                    sizes = w * p.cache_scale(1, i, h, end)
+                    bound = (np.abs(want) * 2.0 ** -11 + 2.0 ** -25 + each * 2.0 ** -11 + 127.5 * sizes.max() * end * 2.0 ** -32 +
+                             127.5 * sizes.sum() * (end + 127) * 2.0 ** -23 + each * 2.0 ** -11)
+                    assert (np.abs(got[row, h] - want) <= bound).all(), (first, rest, near, row, h)
 
 
 def test_scores_of_any_size_and_values_near_the_largest(shared_keys):
