@@ -71,21 +71,21 @@ __device__ __forceinline__ Scales read_scales(const half_t* p, int64_t step, boo
 
 // ---- few rows: generation, a few tokens or a small draft at once ---------------------------------------------
 //
-// A block of 16 rows against its keys, as attention_few_rows_kernel: tiles of 32 keys, four of each wavefront's in LDS.  A tile's
+// A block of 16 rows against its keys, as attention_few_rows_kernel: tiles of 32 keys, two of each wavefront's in LDS.  A tile's
 // codes go from LDS to registers as they are, values through the transposing read of bytes, and become fp16 there.
-constexpr int few_ahead(int) { return 8; }
-constexpr int few_bytes(int hd, int depth) { return 2 * depth * FEW_KEYS * hd + 3 * 2 * few_ahead(hd) * FEW_KEYS * 2; }  // of LDS, a wavefront
+constexpr int FEW_AHEAD = 8;
+constexpr int few_bytes(int hd) { return 4 * FEW_KEYS * hd + 3 * 2 * FEW_AHEAD * FEW_KEYS * 2; }  // of LDS, a wavefront
 
-template <int HD, int WAVES, int DEPTH, bool SHARED, bool TREE>
+template <int HD, int WAVES, bool SHARED, bool TREE>
 __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Job) {
   constexpr int CPR = HD / 16, KEYS = 32, ROWS = 16;
   constexpr int ROWB = HD, TILE = KEYS * ROWB;      // bytes of a tile row, of a K or V tile
   constexpr int NI = TILE / 1024;                   // transfers per tile
   constexpr int KP = HD / 64, DB = HD / 16;         // pairs of k-steps of S, blocks of 16 output columns
-  constexpr int AHEAD = few_ahead(HD);              // tiles whose addresses are looked up at once
-  constexpr int SCALES = 2 * DEPTH * TILE;          // K0 ... V0 ... of a wavefront, then twice as many tiles' scales:
+  constexpr int AHEAD = FEW_AHEAD;                  // tiles whose addresses are looked up at once
+  constexpr int SCALES = 4 * TILE;                  // K0 K1 V0 V1 of a wavefront, then twice as many tiles' scales:
   constexpr int KIND = 2 * AHEAD * KEYS * 2;        // bytes of those of keys, of values, and of their logarithms
-  constexpr int WAVE = few_bytes(HD, DEPTH);
+  constexpr int WAVE = few_bytes(HD);
   constexpr int PITCH = HD + 4;                     // of the partial results' rows, in floats
   constexpr int BIAS = NI / 2 * 1024;               // bytes that descriptors start ahead, so that no offset is negative
   static_assert(16 * (PITCH + 2) * 4 + 16 <= WAVE, "the partial results fit the tiles' LDS");
@@ -222,34 +222,20 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
       const int l = (IS_K ? 0 : 32) + 2 * (i & (AHEAD - 1)) + h, left = min(row_end - (tile0 + w + WAVES * i) * KEYS - 16 * h, 16);
       const uint32_t lo = __builtin_amdgcn_readlane(at_lo, l), hi = __builtin_amdgcn_readlane(at_hi, l);
       const u32x4_t desc = {lo, hi & 0xffffu, hi >> 31 ? (uint32_t)((left - 1) * stride + d + BIAS) : 0u, 0x00020000u};
-      transfer_once<NI / 2>(lds0 + ((IS_K ? 0 : DEPTH) + (i & (DEPTH - 1))) * TILE + h * (NI / 2) * 1024, IS_K ? koff : voff[h], desc);
+      transfer_once<NI / 2>(lds0 + ((IS_K ? 0 : 2) + (i & 1)) * TILE + h * (NI / 2) * 1024, IS_K ? koff : voff[h], desc);
     }
   };
   const std::true_type is_k{};
   const std::false_type is_v{};
 
-  // All transfers but the last n of K or V tiles have landed (n: at most 2 DEPTH - 1).
-  auto wait_tiles = [&](int n) __attribute__((always_inline)) {
-    static_assert((DEPTH == 2 || DEPTH == 4) && (2 * DEPTH - 1) * NI < 64, "as many as are told apart here");
-    if (DEPTH > 2 && n == 7) wait_vm<7 * NI>();
-    else if (DEPTH > 2 && n == 6) wait_vm<6 * NI>();
-    else if (DEPTH > 2 && n == 5) wait_vm<5 * NI>();
-    else if (DEPTH > 2 && n == 4) wait_vm<4 * NI>();
-    else if (n == 3) wait_vm<3 * NI>();
-    else if (n == 2) wait_vm<2 * NI>();
-    else if (n == 1) wait_vm<NI>();
-    else wait_vm<0>();
-  };
-
   look_up(0);
   asm volatile("" : "+v"(at_lo), "+v"(at_hi));
-#pragma unroll
-  for (int t = 0; t < DEPTH; t++) {
-    if (t < tiles) fetch(t, is_k);
-    if (t < tiles && t + 1 < DEPTH) fetch(t, is_v);
-  }
+  if (tiles > 0) fetch(0, is_k), fetch(0, is_v);
+  if (tiles > 1) fetch(1, is_k);
   keep_scales(0);
-  wait_tiles(2 * min(tiles, DEPTH) - (tiles >= DEPTH));
+  if (tiles > 1) wait_vm<3 * NI>();
+  else if (tiles > 0) wait_vm<2 * NI>();
+  else wait_vm<0>();
   half8_t qf[2 * KP];
   float first_sum = 0.0f;
 #pragma unroll
@@ -260,7 +246,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
 #pragma unroll
   for (int ks = 0; ks < 2 * KP; ks++) asm volatile("" : "+v"(qf[ks]));
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  if (tiles >= DEPTH) fetch(DEPTH - 1, is_v);
+  if (tiles > 1) fetch(1, is_v);
 #pragma unroll
   for (int ks = 0; ks < 2 * KP; ks++)
 #pragma unroll
@@ -298,12 +284,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
   half8_t all_ones;
 #pragma unroll
   for (int e = 0; e < 8; e++) all_ones[e] = (half_t)1;
-  for (int i = 0; i < tiles; i++) {
-    const int ahead = min(tiles - i, DEPTH);  // tiles that are in LDS or on their way
-    const bool more = i + DEPTH < tiles;      // the next of them is asked for as soon as the fragments of this one are in registers
-    wait_tiles(2 * ahead - 1);                // its keys have landed
-    const unsigned char* const cK = sm + (i & (DEPTH - 1)) * TILE;
-    const unsigned char* const cV = sm + (DEPTH + (i & (DEPTH - 1))) * TILE;
+  // Tile i; `next`: there is a tile i + 1, `more`: and a tile i + 2, whose keys and values are asked for as soon as the fragments
+  // of this one's are in registers.
+  auto tile = [&](int i, auto next, auto more) __attribute__((always_inline)) {
+    constexpr bool NEXT = decltype(next)::value, MORE = decltype(more)::value;
+    wait_vm<NEXT ? 3 * NI : NI>();  // its keys have landed
+    const unsigned char* const cK = sm + (i & 1) * TILE;
+    const unsigned char* const cV = sm + (2 + (i & 1)) * TILE;
     u32x4_t kc[2][KP];
     half4_t ks[2], vs[2], log_vs[2];
 #pragma unroll
@@ -325,24 +312,26 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
           s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(widened(kc[kb][kp][2 * h], kc[kb][kp][2 * h + 1]), qf[2 * kp + h], s[kb], 0, 0, 0);
-    if (more) {
+    if constexpr (MORE) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      const bool looks = ((i + DEPTH) & (AHEAD - 1)) == 0;
+      const bool looks = ((i + 2) & (AHEAD - 1)) == 0;
       if (looks) {
-        look_up(i + DEPTH);
+        look_up(i + 2);
         asm volatile("" : "+v"(at_lo), "+v"(at_hi));
       }
-      fetch(i + DEPTH, is_k);
-      if (looks) keep_scales(i + DEPTH);
+      fetch(i + 2, is_k);
+      if (looks) keep_scales(i + 2);
     }
-    wait_tiles(more ? 2 * DEPTH - 1 : 2 * ahead - 2);  // and its values
+    wait_vm<MORE ? 3 * NI : NEXT ? 2 * NI : 0>();  // and its values
     int2_t vc[DB];
 #pragma unroll
     for (int db = 0; db < DB; db++) vc[db] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2_t*)ADR_LDS_PTR(cV + offV[db]));
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if constexpr (MORE) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-    for (int db = 0; db < DB; db++) asm volatile("" : "+v"(vc[db]));
-    if (more) fetch(i + DEPTH, is_v);
+      for (int db = 0; db < DB; db++) asm volatile("" : "+v"(vc[db]));
+      fetch(i + 2, is_v);
+    }
     const int key0 = (tile0 + w + WAVES * i) * KEYS;
 #pragma unroll
     for (int kb = 0; kb < 2; kb++)
@@ -397,7 +386,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
     for (int db = 0; db < DB; db++)
       o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(widened((uint32_t)vc[db][0], (uint32_t)vc[db][1]),
                                                      __builtin_bit_cast(half8_t, pf), o[db], 0, 0, 0);
-  }
+  };
+  const std::true_type yes{};
+  const std::false_type no{};
+  int i = 0;
+  for (; i + 2 < tiles; i++) tile(i, yes, yes);
+  if (i + 1 < tiles) tile(i++, yes, no);
+  if (i < tiles) tile(i, no, no);
 
   Args z = arguments();
   // Merge the wavefronts' results: [wavefront][row][HD] sums, and (maximum, sum) of every row.
@@ -482,7 +477,7 @@ int64_t most_blocks(const SequencesArgs& a, int rows) {
 SequencesPlan sequences_u8_plan(const SequencesArgs& a, int cus, int64_t avail) {
   const SequencesPlan any = {SequencesPlan::ANY_LAYOUT, 0, 0, 0, 0, 0};
   if (!chunks(a) || knob(KNOB_SEQUENCES) == 1) return any;
-  SequencesPlan p = {SequencesPlan::FEW_ROWS, 4, 0, 0, 1, 0};
+  SequencesPlan p = {SequencesPlan::FEW_ROWS, 2, 0, 0, 1, 0};
   const int hd = a.d <= 64 ? 64 : 128;
   const int longest_rows = a.longest_rows > 0 ? std::min(a.longest_rows, a.rows) : a.rows;
   const int64_t most_keys = std::min((int64_t)a.table_width * a.page_size, (int64_t)MOST_KEYS);
@@ -494,6 +489,8 @@ SequencesPlan sequences_u8_plan(const SequencesArgs& a, int cus, int64_t avail) 
   const int each = hd == 64 ? 8 : 4;
   p.parts = unshared ? 0 : std::max(1, each * cus / a.kv_heads);
   const int forced = knob(KNOB_SEQUENCES) >= 2 && knob(KNOB_SEQUENCES) <= 8 ? knob(KNOB_SEQUENCES) : 0;
+  if (!forced && blocks <= cus) p.waves = 8;
+  if (forced) p.waves = forced == 3 ? 8 : 2;
   if (forced) p.parts = forced == 4 ? std::max(16, cus / a.kv_heads) : 0;
   const double most_tiles = ((double)a.rows * a.group / FEW + a.sequences) * (most_keys / FEW_KEYS + 2.0);
   for (p.shift = FEW_SHIFT; most_tiles > ldexp(0x1p29, p.shift) && p.shift < 25; p.shift++) {}
@@ -504,8 +501,6 @@ SequencesPlan sequences_u8_plan(const SequencesArgs& a, int cus, int64_t avail) 
   p.workspace_bytes = p.parts * part;
   return p;
 }
-
-constexpr int SHARED_DEPTH = 2;
 
 template <int HD, bool TREE>
 static hipError_t launch_blocks(hipStream_t stream, const SequencesArgs& a, const SequencesPlan& p, void* workspace) {
@@ -523,10 +518,11 @@ static hipError_t launch_blocks(hipStream_t stream, const SequencesArgs& a, cons
   const int at_once = std::min(FEW, 1024 / HD);
   const dim3 grid((unsigned)blocks), join((unsigned)((p.parts - 1) * a.kv_heads * (FEW / at_once)));
   if (p.parts > 0) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_u8_few_rows_kernel<HD, 2, SHARED_DEPTH, true, TREE>), grid, dim3(128), 2 * few_bytes(HD, SHARED_DEPTH), stream, job);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_u8_few_rows_kernel<HD, 2, true, TREE>), grid, dim3(128), 2 * few_bytes(HD), stream, job);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, FEW, true>), join, dim3(256), 0, stream, job);
   } else {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_u8_few_rows_kernel<HD, 4, 4, false, TREE>), grid, dim3(256), 4 * few_bytes(HD, 4), stream, job);
+    if (p.waves == 8) hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_u8_few_rows_kernel<HD, 8, false, TREE>), grid, dim3(512), 8 * few_bytes(HD), stream, job);
+    else hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_u8_few_rows_kernel<HD, 2, false, TREE>), grid, dim3(128), 2 * few_bytes(HD), stream, job);
   }
   return hipGetLastError();
 }

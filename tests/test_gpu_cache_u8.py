@@ -14,9 +14,9 @@ pytestmark = pytest.mark.gpu
 CAUSAL, NONE = MatmulMask.CAUSAL, MatmulMask.NONE
 SENTINEL = 777.0
 EPS = 1e-6
-FORMS = ["a row to a wavefront", "few rows", "few rows, shared", "many rows", "many rows, 2 groups", "many rows, shared",
+FORMS = ["a row to a wavefront", "few rows, 2 waves", "few rows, 8 waves", "few rows, shared", "many rows", "many rows, 2 groups", "many rows, shared",
          "many rows, 2 groups, shared"]
-KNOBS = [1, 2, 4, 5, 6, 7, 8]
+KNOBS = [1, 2, 3, 4, 5, 6, 7, 8]
 
 
 @pytest.fixture(scope="module")
