@@ -102,6 +102,13 @@ __device__ __forceinline__ void dma_global(uint32_t lds, const void* p) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, off"
                :: "s"(lds), "v"(p) : "memory");
 }
+// One transfer of 1 KiB, of what may be read again; one of 256 bytes, a word from each lane.
+__device__ __forceinline__ void dma_buffer(uint32_t lds, uint32_t voff, u32x4_t desc) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(lds), "v"(voff), "s"(desc) : "memory");
+}
+__device__ __forceinline__ void dma_global_word(uint32_t lds, const void* p) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, off" :: "s"(lds), "v"(p) : "memory");
+}
 template <int N>
 __device__ __forceinline__ void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");

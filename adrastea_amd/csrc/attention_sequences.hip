@@ -7,7 +7,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "attention_work.hpp"
+#include "attention_tiles.hpp"
 
 
 namespace adr {
@@ -345,613 +345,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
   }
 }
 
-// ---- many rows: prompts, and their pieces over what is in the cache ---------------------------------------
-//
-// A workgroup takes a block of 128 rows, wavefront w of it rows 32 w ... 32 w + 31 of the list, and walks tiles of 64
-// keys, double buffered in LDS by transfers from global memory; two workgroups share a compute unit.  Per tile a
-// wavefront computes S^T = K Q^T (MFMA 32x32x16, Q fragments resident in registers), so that every lane holds scores
-// of one row: the running maximum and sum are in-lane reductions plus one exchange with lane ^ 32, and a lane's own
-// last key is all that the mask needs.  The probabilities, narrowed to fp16, are already in the operand layout of the
-// second product O^T = V^T P^T, whose V^T fragments come from the row-major V tile by transposing LDS reads.  The two
-// products and the softmax between them are one instruction stream, as in attention_fwd_kernel (attention.hip, which
-// explains the arrangement): scores of tile i + 1 on the matrix cores beside the exponentials of tile i, P.V of tile i
-// beside the maximum of tile i + 1.  What is different here is where rows and keys come from: the heads of a group
-// share the block, so that a key row is read once for all of them and the part of a tile that the mask leaves empty
-// is 1 / group as wide, and each wavefront's 16 key rows of a tile have a base address of their own, on a page.
-//
-// GROUPS == 2: eight wavefronts, of which four take the first half of the block's keys and four the second, each through
-// tiles of its own; both ends meet in LDS.  Two workgroups beside each other do as much, but that takes twice as many blocks,
-// or parts that go through memory: 1024 rows over 8025 keys (256 blocks) 134 us, by halves through memory 143, one group on
-// each compute unit 144 (all three on one machine).
-//
-// Bound by issue as in attention_fwd_kernel, and where all is loop by power: one prompt of 16384 rows (32 / 8 heads of 128) 2006
-// to 2196 us by machine = 1096 to 1000 TFLOP/s, with the matrix cores busy 69 % of cycles at 1.6 GHz, where a product of 8192^3
-// reaches 1408.  The 256 blocks above, two groups each, leave some of that power: 53 % at 1.8 GHz, 136 to 146 us.  Short blocks are
-// bound by their beginnings and ends: us of a block among others, 2.0 from the end of one to the start of the next in its place,
-// 1.4 to find its sequence, 1.7 for addresses, 1.8 until the first keys are there, 1.9 a tile, 2.4 for the results.  Nine prompts
-// of 100 to 3996 rows, 25 tiles a block in the mean, 447 to 477 us = 933 to 874 TFLOP/s (what wavefronts whose rows end early, and
-// rows that the mask hides, compute of a tile is in the time and not in the operations).  HD = 128 keeps 24 to 38 vector registers
-// in scratch memory at those beginnings and ends, none in the loop; HD = 64 none.
-template <int HD, bool PAGED, bool SHARED, int GROUPS, bool TREE = false>
-__global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
-  constexpr int CPR = HD / 8, KEYS = 64, ROWS = 128;
-  constexpr int TILE = KEYS * HD * 2;  // bytes of one K or V tile
-  constexpr int NI = TILE / 1024 / 4;  // transfers per wavefront and tile: 16 rows
-  constexpr int DS = HD / 16;          // MFMA k-steps over the head dimension
-  constexpr int DT = HD / 32;          // 32-wide output column tiles
-  constexpr int ROWB = HD * 2;         // bytes per tile row
-  constexpr int BIAS = NI * 1024;      // bytes that descriptors start ahead, so that no offset is negative
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[GROUPS * 4 * TILE];  // K0 K1 V0 V1 of each group
-  __shared__ int lost_keys[4 * GROUPS];  // of each wavefront
-
-  // Consecutive workgroups go to different dies; where the key heads divide evenly, a die takes its share of them, so
-  // that the blocks which read the same keys meet in one L2.
-  Args a = arguments();
-  early<PAGED>(a);
-  const int kv_heads = a.kv_heads;
-  int hk, index;
-  if (kv_heads % 8 == 0) {
-    const int each = kv_heads >> 3, seq = blockIdx.x >> 3;
-    hk = (blockIdx.x & 7) * each + seq % each;
-    index = seq / each;
-  } else {
-    hk = blockIdx.x % kv_heads;
-    index = blockIdx.x / kv_heads;
-  }
-  const int tid = threadIdx.x, lane = tid & 63, group = GROUPS == 1 ? 0 : uniform(tid >> 8), w = uniform(tid >> 6 & 3);
-  const int frow = lane & 31, g = lane >> 5;
-  Part pt = {{}, 0, 1, 0, 0, 0};
-  if constexpr (SHARED) {
-    const bool some = part_at<ROWS, KEYS, PAGED>(a, index, lane, pt);
-    // (the second launch has a workgroup to each two slots)
-    if (tid == 0 && index >= pt.seams && index < a.parts / 2) a.seams[index * kv_heads + hk].parts = 0;
-    if (!some) return;
-    if (tid == 0 && pt.part == 0 && pt.parts > 1) a.seams[pt.seam * kv_heads + hk] = Seam{pt.parts, pt.slot, pt.b.q, pt.b.block};
-  } else {
-    Roster<ROWS, KEYS, PAGED, false> roster;
-    roster.load(a, 0, lane, 0, 0);
-    if (!roster.block_at(a, 0, index, lane, pt.b)) return;
-  }
-  const Sequence q = pt.b.q;
-  const int block = pt.b.block, part = pt.part, parts = pt.parts, slot0 = pt.slot;
-  const int rows = min(ROWS, q.rows * a.group - block * ROWS);  // of the block
-  const int wave_rows = min(32, rows - w * 32);                 // of the wavefront (may be negative)
-  const int list0 = block * ROWS + w * 32;
-  // (lanes without a row of their own compute the block's last one)
-  const int list_row = block * ROWS + min(w * 32 + frow, rows - 1), row = row_of_list(a, list_row), gh = list_row - row * a.group;
-  const int lane_end = end_of_row(a, q, row);
-  unsigned char* const sm = smem + group * (4 * TILE);
-  const uint32_t lds0 = (uint32_t)(uintptr_t)ADR_LDS_PTR(smem) + group * (4 * TILE);
-  const int d = a.d, k_stride = (int)a.sk.y, v_stride = (int)a.sv.y;
-  // The queries' fragments, by way of the values' LDS, so that nothing waits for them before the first keys are on their
-  // way.  (Chunks behind the head dimension are zeros below.)
-  static_assert(4 * DS * 1024 <= 2 * TILE, "the queries fit the values' tiles");
-  const half_t* const qrow = a.q + (int64_t)(hk * a.group + gh) * a.sq_z + (int64_t)(q.row0 + row) * a.sq_y;
-#pragma unroll
-  for (int ds = 0; ds < DS; ds++) {
-    const int col = ds * 16 + g * 8;
-    dma_global(lds0 + 2 * TILE + (w * DS + ds) * 1024, qrow + (col < d ? col : 0));
-  }
-
-  const int last_end = uniform(end_of_row(a, q, row_of_list(a, block * ROWS + rows - 1)));
-  const int all = (last_end + KEYS - 1) / KEYS;
-  // (exact, as above)
-  auto cut = [&](int i) __attribute__((always_inline)) { return uniform((int)((double)all * (double)i / (double)parts)); };
-  const int part0 = SHARED ? cut(part) : 0, part_tiles = (SHARED ? cut(part + 1) : all) - part0;
-  // (of each group; the second may have one less)
-  const int steps = (part_tiles + GROUPS - 1) / GROUPS, tile0 = part0 + group * steps;
-  const int row_end = min(last_end, min(part0 + part_tiles, tile0 + steps) * KEYS);
-  // Tiles that this wavefront computes: none without rows, none whose first key lies beyond its last row's.
-  int active = 0, first_edge = 0;
-  if (wave_rows > 0) {
-    active = uniform(clamp_to((end_of_row(a, q, row_of_list(a, list0 + wave_rows - 1)) + KEYS - 1) / KEYS - tile0, min(steps, part0 + part_tiles - tile0)));
-    // the first of them with keys that some row of the wavefront must not see
-    first_edge = uniform(TREE ? end_of_common(a, q, 0) : end_of_row(a, q, row_of_list(a, list0))) / KEYS - tile0;
-  }
-
-  // Wavefront w transfers rows 16 w ... 16 w + 15 of a tile, 1 KiB at a time: byte offsets of a lane's chunks in those
-  // rows, less the j KiB that the instruction adds; chunks behind the head dimension come as zeros.
-  uint32_t koff[NI], voff[NI];
-#pragma unroll
-  for (int j = 0; j < NI; j++) {
-    int krow, kc;
-    k_chunk_inv<CPR>(j * 64 + lane, krow, kc);
-    const int vrow = (j * 64 + lane) / CPR, vc = (lane % CPR) ^ v_swz<CPR>(vrow);
-    const uint32_t ko = (uint32_t)((krow * k_stride + kc * 8) * 2 + BIAS - j * 1024);
-    const uint32_t vo = (uint32_t)((vrow * v_stride + vc * 8) * 2 + BIAS - j * 1024);
-    koff[j] = kc * 8 < d ? ko : 0x7fff0000u;
-    voff[j] = vc * 8 < d ? vo : 0x7fff0000u;
-  }
-  // The wavefront's next 16 key and value rows: address, and bytes from there to the last key (0 behind it).  On
-  // pages, the addresses of 64 tiles at a time, a lane to each, worked out by the vector ALU.  (Addresses are even: an
-  // odd one says that there is one.)  Keys are ahead of values: theirs bring the pages, which the values take over.
-  struct Next {
-    uint64_t base, p, pages;
-    int64_t page_stride;
-    int bytes, key, stride;
-  };
-  bool lost = false;  // a key's page is not in the cache
-  int page = 0;
-  auto locate = [&](Next& t, auto is_k) __attribute__((always_inline)) {
-    const int left = min(row_end - t.key, 16);
-    t.bytes = left > 0 ? ((left - 1) * t.stride + d) * 2 + BIAS : 0;
-    if constexpr (PAGED) {
-      const int n = ((t.key - 16 * w) >> 6) - tile0;
-      if ((n & 63) == 0) {
-        const int key = t.key + lane * KEYS;
-        if constexpr (decltype(is_k)::value) {
-          page = -1;
-          if (key < row_end) {
-            page = a.table[(int64_t)q.index * a.table_pitch + (key >> a.page_shift)];
-            if (page < 0 || page >= a.pages) lost = true, page = -1;
-          }
-        }
-        const int slot = key & ((1 << a.page_shift) - 1);
-        t.pages = page < 0 ? 0 : (t.base + 2 * (page * t.page_stride + slot * (int64_t)t.stride)) | 1;
-      }
-      const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)t.pages, n & 63);
-      const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(t.pages >> 32), n & 63);
-      t.p = (uint64_t)hi << 32 | (lo & ~1u);
-      if (!(lo & 1)) t.bytes = 0;
-    }
-  };
-  const std::true_type is_k{};
-  const std::false_type is_v{};
-  auto first_tile = [&](const half_t* base, int64_t stride, int64_t page_stride, auto k) __attribute__((always_inline)) {
-    Next t;
-    t.base = (uint64_t)(base + (PAGED ? 0 : q.key0 * stride)) - BIAS;
-    t.page_stride = page_stride;
-    t.stride = (int)stride;
-    t.key = tile0 * KEYS + 16 * w;
-    t.pages = 0;
-    t.p = t.base + 2 * (t.key * stride);
-    locate(t, k);
-    return t;
-  };
-  Next nk = first_tile(a.k + hk * a.sk.z, a.sk.y, a.sk.p, is_k), nv = first_tile(a.v + hk * a.sv.z, a.sv.y, a.sv.p, is_v);
-  auto advance = [&](Next& t, auto k) __attribute__((always_inline)) {
-    t.key += KEYS;
-    if constexpr (!PAGED) t.p += (uint32_t)t.stride * (KEYS * 2u);
-    locate(t, k);
-  };
-  // Transfers 2 j and 2 j + 1 of the NI that bring a tile into buffer `buf` (0, 1: K; 2, 3: V).
-  auto transfer = [&](const Next& t, auto is_k, int buf, auto pair) __attribute__((always_inline)) {
-    constexpr int J = 2 * decltype(pair)::value;
-    const uint32_t dst = lds0 + w * (NI * 1024) + buf * TILE;
-    const u32x4_t desc = descriptor(t.p, t.bytes);
-    if constexpr (decltype(is_k)::value) dma_buffer_pair<J>(dst, koff[J], koff[J + 1], desc);
-    else dma_buffer_pair<J>(dst, voff[J], voff[J + 1], desc);
-  };
-  const std::integral_constant<int, 0> pair0{};
-  const std::integral_constant<int, NI / 2 - 1> pair1{};  // (the last pair; HD = 64 has one)
-  auto tile_transfers = [&](Next& t, auto k, int buf) __attribute__((always_inline)) {
-    transfer(t, k, buf, pair0);
-    if constexpr (NI > 2) transfer(t, k, buf, pair1);
-    advance(t, k);
-  };
-  // What is waited for at the end of each half: all transfers but those issued in it.
-  auto wait_landed = [&]() __attribute__((always_inline)) { wait_vm<NI>(); };
-
-  tile_transfers(nk, is_k, 0);
-  tile_transfers(nk, is_k, 1);
-  // LDS fragment offsets.  K: lane -> tile row frow (+32), chunk 2*ds + g.
-  int offK[DS];
-#pragma unroll
-  for (int ds = 0; ds < DS; ds++) offK[ds] = k_chunk_off<CPR>(frow, ds * 2 + g);
-  wait_vm<NI>();  // the queries and the first K tile have landed
-  half8_t qf[DS];  // (operand B of S^T = K Q^T: lane -> row frow, head-dimension group g)
-#pragma unroll
-  for (int ds = 0; ds < DS; ds++) {
-    qf[ds] = *(const half8_t*)(sm + 2 * TILE + (w * DS + ds) * 1024 + lane * 16);
-    if (ds * 16 + g * 8 >= d) qf[ds] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
-  }
-#pragma unroll
-  for (int ds = 0; ds < DS; ds++) asm volatile("" : "+v"(qf[ds]));
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (values come there behind the next barrier)
-  // V (transposing read): in each group of 16 lanes, lanes 4r..4r+3 address 16 consecutive halves of tile row r, and
-  // lane i of the group receives column i of that 4 x 16 block.  Group b = (lane / 16) % 2 takes columns 16b.. of the
-  // 32-column tile, g the rows 4g..4g+3.
-  int offV[DT];
-  {
-    const int s = lane & 15, b = (lane >> 4) & 1, r = s >> 2;
-    const int row = 4 * g + r;  // + 32*kt + 16*t + 8*h, all multiples of 8: row & 3 == r
-#pragma unroll
-    for (int dt = 0; dt < DT; dt++) {
-      const int chunk = 4 * dt + 2 * b + ((s & 3) >> 1);
-      offV[dt] = row * ROWB + ((chunk ^ v_swz<CPR>(row)) << 4) + (s & 1) * 8;
-    }
-  }
-
-  float16_t o[DT], sa[2], sb[2];  // sums of P.V; scores of two tiles in turn
-  u32x4_t pf[2][2];                 // probabilities, two to a register
-#pragma unroll
-  for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-    for (int r = 0; r < 16; r++) o[dt][r] = 0.0f;
-  float m_run = NO_SCORE, l_run = 0.0f;  // running maximum (log2 units) and this lane's sum
-
-  typedef short short4_t __attribute__((ext_vector_type(4)));
-  typedef __attribute__((address_space(3))) short4_t lds_short4_t;
-  // A half tile is NG groups of four MFMAs.  A group's fragments are read a group ahead, and used in
-  // the opposite order, so that one wait covers all four.
-  constexpr int NG = DS / 2;
-  half8_t kf[NG][4], vf[NG][4];
-
-  auto read_k = [&](const unsigned char* cK, int c) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < 4; j++) kf[c][j] = *(const half8_t*)(cK + offK[2 * c + (j >> 1)] + (j & 1) * 32 * ROWB);
-  };
-  // which of the products with V the j-th of group c is: keys 32 kt + 16 t ..., columns 32 dt ...
-  auto pv_of = [](int c, int j, int& kt, int& t, int& dt) __attribute__((always_inline)) {
-    const int p = 4 * c + j;
-    kt = p / (2 * DT), t = p / DT % 2, dt = p % DT;
-  };
-  auto read_v = [&](const unsigned char* cV, int c) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      int kt, t, dt;
-      pv_of(c, j, kt, t, dt);
-      const unsigned char* p0 = cV + offV[dt] + (32 * kt + 16 * t) * ROWB;
-      const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)ADR_LDS_PTR(p0));
-      const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)ADR_LDS_PTR(p0 + 8 * ROWB));
-      vf[c][j] = __builtin_shufflevector(__builtin_bit_cast(half4_t, lo), __builtin_bit_cast(half4_t, hi),
-                                         0, 1, 2, 3, 4, 5, 6, 7);
-    }
-  };
-
-  // First half of tile i: the scores of tile i + 1 on the matrix cores (K buffer KB), and the
-  // probabilities of tile i on the vector ALU.
-  auto half1 = [&](auto do_s, auto do_p, auto do_pv, auto kbuf, float16_t (&cur)[2], float16_t (&nxt)[2])
-                   __attribute__((always_inline)) {
-    constexpr bool S = decltype(do_s)::value, P = decltype(do_p)::value;
-    constexpr int KB = decltype(kbuf)::value, VB = 1 - KB;
-    const unsigned char* const cK = sm + KB * TILE;
-    const unsigned char* const cV = sm + (2 + VB) * TILE;
-    // Piece k of the softmax: VP scores, in three stages that run a piece apart, so that no instruction
-    // waits for the one before it: exponents (k + 1), powers of two (k), rounding and sum (k - 1).
-    // (The empty assembly keeps the stages where they are.  Sums by v_dot2 would be half the
-    // instructions, but those wait for the matrix cores.)
-    constexpr int NP = 4 * NG, VP = 32 / NP;
-    float sum[2] = {l_run, 0.0f};
-    float ex[VP], pw[VP];
-    auto stage_exponent = [&](int k) __attribute__((always_inline)) {
-#pragma unroll
-      for (int e = 0; e < VP; e++) ex[e] = fmaf(cur[k * VP >> 4][(k * VP & 15) + e], a.c, -m_run);
-    };
-    auto stage_power = [&]() __attribute__((always_inline)) {
-#pragma unroll
-      for (int e = 0; e < VP; e++) pw[e] = __builtin_amdgcn_exp2f(ex[e]);
-    };
-    auto stage_round = [&](int k) __attribute__((always_inline)) {
-#pragma unroll
-      for (int e = 0; e < VP; e += 2) {
-        const int x = k * VP + e;
-        const float2_t e2 = {pw[e], pw[e + 1]};
-        uint32_t bits = __builtin_bit_cast(uint32_t, __builtin_convertvector(e2, half2_t));
-        sum[0] += pw[e];
-        sum[1] += pw[e + 1];
-        asm volatile("" : "+v"(bits), "+v"(sum[0]), "+v"(sum[1]));
-        pf[x >> 4][x >> 3 & 1][(x & 7) / 2] = bits;
-      }
-    };
-    if constexpr (HD == 128) __builtin_amdgcn_s_setprio(1);
-    if constexpr (P) stage_exponent(0);
-    if constexpr (S) {
-#pragma unroll
-      for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) nxt[kt][r] = 0.0f;
-    }
-#pragma unroll
-    for (int c = 0; c < NG; c++) {
-      if constexpr (S) {
-        if (c + 1 < NG) read_k(cK, c + 1);
-      }
-      if constexpr (decltype(do_pv)::value) {
-        if (c + 1 == NG) read_v(cV, 0);
-      }
-      if (c == 0) transfer(nv, is_v, 2 + KB, pair0);
-      if constexpr (NI > 2) {
-        if (c == NG / 2) transfer(nv, is_v, 2 + KB, pair1);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        if constexpr (S) {
-          constexpr int last = 3;
-          const int f = last - j;
-          nxt[f & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[c][f], qf[2 * c + (f >> 1)], nxt[f & 1], 0, 0, 0);
-        }
-        if constexpr (P) {
-          const int k = 4 * c + j;
-          if (k > 0) stage_round(k - 1);
-          stage_power();
-          if (k + 1 < NP) stage_exponent(k + 1);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    if constexpr (P) {
-      stage_round(NP - 1);
-      l_run = sum[0] + sum[1];
-      asm volatile("" : "+v"(l_run));
-    }
-    if constexpr (HD == 128) __builtin_amdgcn_s_setprio(0);
-    advance(nv, is_v);
-    wait_landed();
-    barrier();
-  };
-
-  // Second half of tile i: P.V of tile i on the matrix cores (V buffer VB), and the maximum of the
-  // scores of tile i + 1 on the vector ALU.
-  auto half2 = [&](int i, auto do_pv, auto do_max, auto do_s, auto vbuf, float16_t (&nxt)[2])
-                   __attribute__((always_inline)) {
-    constexpr bool PV = decltype(do_pv)::value, MAX = decltype(do_max)::value;
-    constexpr int VB = decltype(vbuf)::value, KB = VB;  // K buffer of tile i + 2
-    const unsigned char* const cV = sm + (2 + VB) * TILE;
-    const unsigned char* const cK = sm + KB * TILE;
-    if constexpr (MAX) {
-      if (i + 1 >= first_edge) {
-        // this lane's first masked key, counted from its own first one
-        int end = lane_end - (tile0 + i + 1) * KEYS - 4 * g;
-#pragma unroll
-        for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) {
-            asm volatile("" : "+v"(end));  // (one comparison at a time: 32 would take as many scalar register pairs)
-            if (32 * kt + 8 * (r >> 2) + (r & 3) >= end) nxt[kt][r] = -INFINITY;
-          }
-        if constexpr (TREE) {
-#pragma unroll
-          for (int kt = 0; kt < 2; kt++) {
-            uint32_t seen = tree_window(a, q.row0 + row, (tile0 + i + 1) * KEYS + 32 * kt - (q.keys - q.rows)) >> 4 * g;
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-              asm volatile("" : "+v"(seen));
-              if (!(seen >> (8 * (r >> 2) + (r & 3)) & 1)) nxt[kt][r] = -INFINITY;
-            }
-          }
-        }
-      }
-    }
-    // (the maximum from the second group on, when the scores are there; done before the last one)
-    constexpr int FIRST = NG == 4 ? 4 : 2, PER = NG == 4 ? 2 : 4;
-    float mx2[2] = {NO_SCORE, NO_SCORE}, mx = 0.0f;
-#pragma unroll
-    for (int c = 0; c < NG; c++) {
-      if constexpr (PV) {
-        if (c + 1 < NG) read_v(cV, c + 1);
-      }
-      if constexpr (decltype(do_s)::value) {
-        if (c + 1 == NG) read_k(cK, 0);
-      }
-      if (c == 0) transfer(nk, is_k, 1 - KB, pair0);
-      if constexpr (NI > 2) {
-        if (c == NG / 2) transfer(nk, is_k, 1 - KB, pair1);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        if constexpr (PV) {
-          constexpr int last = 3;
-          const int f = last - j;
-          int kt, t, dt;
-          pv_of(c, f, kt, t, dt);
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[c][f], __builtin_bit_cast(half8_t, pf[kt][t]), o[dt], 0, 0, 0);
-        }
-        if constexpr (MAX) {
-          const int first = (4 * c + j - FIRST) * PER * 2;
-          if (first >= 0 && first < 32) {
-#pragma unroll
-            for (int e = 0; e < PER; e++) {
-              const int x = first + 2 * e;
-              mx2[e & 1] = fmaxf(fmaxf(mx2[e & 1], nxt[x >> 4][x & 15]), nxt[x >> 4][(x & 15) + 1]);
-            }
-          }
-          if (first == 32) mx = above(pair_max(fmaxf(mx2[0], mx2[1])) * a.c);  // in log2 units (c > 0)
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    if constexpr (MAX) {
-      if (__builtin_amdgcn_ballot_w64(mx > m_run + GROWN) != 0) {
-        const float m_new = fmaxf(m_run, mx - BELOW);
-        const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-        m_run = m_new;
-        l_run *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) o[dt][r] *= alpha;
-      }
-    }
-    advance(nk, is_k);
-    wait_landed();
-    barrier();
-  };
-  auto idle = [&](int i) __attribute__((always_inline)) {
-    tile_transfers(nv, is_v, 2 + ((i + 1) & 1));
-    wait_landed();
-    barrier();
-    tile_transfers(nk, is_k, (i + 1) & 1);
-    wait_landed();
-    barrier();
-  };
-
-  const std::true_type yes{};
-  const std::false_type no{};
-  const std::integral_constant<int, 0> even{};
-  const std::integral_constant<int, 1> odd{};
-
-  barrier();  // the first K tile has landed for every wavefront
-  int i = -1;
-  if (active > 0) {
-    read_k(sm, 0);
-    half1(yes, no, no, even, sb, sa);
-    half2(-1, no, yes, yes, odd, sa);
-    for (i = 0; i + 2 < active; i += 2) {
-      half1(yes, yes, yes, odd, sa, sb);
-      half2(i, yes, yes, yes, even, sb);
-      half1(yes, yes, yes, even, sb, sa);
-      half2(i + 1, yes, yes, yes, odd, sa);
-    }
-    if (i + 1 < active) {
-      half1(yes, yes, yes, odd, sa, sb);
-      half2(i, yes, yes, no, even, sb);
-      half1(no, yes, yes, even, sb, sa);
-      half2(i + 1, yes, no, no, odd, sa);
-    } else {
-      half1(no, yes, yes, odd, sa, sb);
-      half2(i, yes, no, no, even, sb);
-    }
-    i = active;
-  }
-  for (; i < steps; i++) idle(i);  // tiles this wavefront has no part in
-  wait_vm<0>();  // (transfers of no bytes write zeros)
-  if constexpr (PAGED) {
-    if (lane == 0) lost_keys[4 * group + w] = __ballot(lost) != 0;
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  }
-  barrier();  // every read of K and V tiles is done: LDS is free
-
-  // The groups' sums are joined by way of LDS: each finishes half of the columns.
-  constexpr int MINE = DT / GROUPS;
-  constexpr int EXCHANGE = GROUPS == 1 ? 0 : 256 * MINE * 64;  // bytes from a group
-  float16_t res[MINE];
-  if constexpr (GROUPS == 2) {
-    __shared__ float2 mls[2][256];
-    const int at = tid & 255;
-    float4_t* const theirs = (float4_t*)(smem + (1 - group) * (4 * TILE)) + at;
-    float4_t* const ours = (float4_t*)sm + at;
-    auto give = [&](auto first) __attribute__((always_inline)) {
-#pragma unroll
-      for (int d = 0; d < MINE; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float16_t& v = o[decltype(first)::value + d];
-          ours[(4 * d + i) * 256] = float4_t{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
-        }
-    };
-    if (group == 0) give(std::integral_constant<int, MINE>{});
-    else give(std::integral_constant<int, 0>{});
-    mls[group][at] = make_float2(m_run, l_run);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    barrier();
-    const float2 ml = mls[1 - group][at];
-    const float top = fmaxf(m_run, ml.x), f0 = __builtin_amdgcn_exp2f(m_run - top), f1 = __builtin_amdgcn_exp2f(ml.x - top);
-    m_run = top;
-    l_run = l_run * f0 + ml.y * f1;
-    auto take = [&](auto first) __attribute__((always_inline)) {
-#pragma unroll
-      for (int d = 0; d < MINE; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float16_t& v = o[decltype(first)::value + d];
-          const float4_t x = theirs[(4 * d + i) * 256];
-#pragma unroll
-          for (int j = 0; j < 4; j++) res[d][4 * i + j] = v[4 * i + j] * f0 + x[j] * f1;
-        }
-    };
-    if (group == 0) take(std::integral_constant<int, 0>{});
-    else take(std::integral_constant<int, MINE>{});
-  } else {
-#pragma unroll
-    for (int d = 0; d < DT; d++) res[d] = o[d];
-  }
-
-  Args z = arguments();
-  float l_tot = pair_sum(l_run);
-  if constexpr (PAGED) {
-    // (a page that is not in the cache may be some rows' only: all of the block come out as NaN, and where some do not see
-    // it they are computed again below)
-    int any = 0;
-#pragma unroll
-    for (int i = 0; i < 4 * GROUPS; i++) any |= lost_keys[i];
-    if (any) l_tot = NAN;
-  }
-  const int col0 = group * (32 * MINE);
-  if (!SHARED || parts == 1) {
-    // out[row][32d + 8i + 4g + j] = res[d][4i + j] / l, by way of LDS, so that whole rows are stored
-    constexpr int PITCH = ROWB / GROUPS + 16, CHUNKS = CPR / GROUPS;
-    static_assert(EXCHANGE + 4 * 32 * PITCH <= 4 * TILE, "the output's slots fit the LDS");
-    unsigned char* const slot = sm + EXCHANGE + w * (32 * PITCH);
-    const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
-    float zero[2] = {0.0f, 0.0f};  // (NaN behind a result that is not finite)
-#pragma unroll
-    for (int d = 0; d < MINE; d++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        half4_t h;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          h[j] = (half_t)(res[d][4 * i + j] * inv);
-          zero[j & 1] = fmaf((float)h[j], 0.0f, zero[j & 1]);
-        }
-        *(half4_t*)(slot + frow * PITCH + (32 * d + 8 * i + 4 * g) * 2) = h;
-      }
-    bool finite = zero[0] + zero[1] == 0.0f;
-    if (__ballot(!finite)) {
-      finite = true;
-#pragma unroll
-      for (int d = 0; d < MINE; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          half4_t h;
-          const float4_t v = {res[d][4 * i], res[d][4 * i + 1], res[d][4 * i + 2], res[d][4 * i + 3]};
-          finite &= round_means(h, v, inv);
-          *(half4_t*)(slot + frow * PITCH + (32 * d + 8 * i + 4 * g) * 2) = h;
-        }
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the slot is the wavefront's own)
-    constexpr int RPI = 64 / CHUNKS;  // rows of a store instruction
-    const int r0 = lane / CHUNKS, col = lane % CHUNKS * 8;
-    int token = row_of_list(z, list0 + r0), head = list0 + r0 - token * z.group;  // of the group
-    const int more_tokens = row_of_list(z, RPI), more_heads = RPI - more_tokens * z.group;
-    half_t* const out = z.out + (int64_t)(hk * z.group) * z.so_z + (int64_t)q.row0 * z.so_y + col0 + col;
-#pragma unroll
-    for (int i = 0; i < 32 / RPI; i++) {
-      if (i * RPI >= wave_rows) break;
-      const int r = r0 + i * RPI;
-      if (r < wave_rows && col0 + col < z.d)
-        *(half8_t*)(out + (int64_t)head * z.so_z + (int64_t)token * z.so_y) = *(const half8_t*)(slot + r * PITCH + col * 2);
-      token += more_tokens, head += more_heads;
-      if (head >= z.group) head -= z.group, token++;
-    }
-    // Rows that are computed again, a group's columns of them.
-    const uint64_t wrong = __ballot(!finite), far = __ballot(is_far(m_run));
-    if ((wrong | far) && wave_rows > 0) {
-      uint32_t again = (uint32_t)far | (uint32_t)(far >> 32);
-      const uint32_t bad = (uint32_t)wrong | (uint32_t)(wrong >> 32);
-      if (bad && (TREE || (q.rows > 1 && z.mask == ADR_MASK_CAUSAL)) &&
-          hidden_reaches(z, q, hk, end_of_common(z, q, row_of_list(z, list0 + min(__builtin_ctz(bad), wave_rows - 1))),
-                         end_of_row(z, q, row_of_list(z, block * ROWS + rows - 1)), lane))
-        again |= bad;
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (behind the stores above)
-      for (int r = 0; r < wave_rows; r++)
-        if (again >> r & 1)
-          row_by_wave(arguments(), q, (list0 + r) / z.group, hk * z.group + (list0 + r) % z.group, lane, col0, col0 + 32 * MINE);
-    }
-  } else if (frow < wave_rows) {
-    const int64_t prow = ((int64_t)(slot0 + part) * z.kv_heads + hk) * ROWS + w * 32 + frow;
-    float* const po = z.part_o + prow * HD + col0 + 4 * g;
-#pragma unroll
-    for (int d = 0; d < MINE; d++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        float4_t v;
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = res[d][4 * i + j];
-        *(float4_t*)(po + 32 * d + 8 * i) = v;
-      }
-    if (g == 0 && group == 0) z.part_ml[prow] = make_float2(m_run, l_tot);
-  }
-}
-
 }  // namespace
 
 // ---- the choice ---------------------------------------------------------------------------------------------
 
 namespace {
-
-int page_shift(int page_size) { return page_size >= 16 && (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1; }
 
 // What the matrix-core kernels take: whole chunks of 16 bytes at 16-byte addresses, 16 key rows within the reach of a
 // descriptor's 32-bit offsets, rows that do not overlap (a row behind the last key is told by its offset).
@@ -963,11 +361,6 @@ bool chunks(const SequencesArgs& a) {
          strides % 8 == 0 && strides >= 0 && near(a.sk.y) && near(a.sv.y) && (!a.table || page_shift(a.page_size) >= 0);
 }
 
-// Blocks of all key heads that there can be, and as many as a launch of 256 threads to each may have.
-int64_t most_blocks(const SequencesArgs& a, int rows) {
-  return ((int64_t)a.rows * a.group / rows + std::min(a.rows, a.sequences)) * a.kv_heads;
-}
-constexpr int64_t LAUNCH_BLOCKS = 0x7fffffff / 256;
 
 }  // namespace
 
@@ -1014,24 +407,7 @@ SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
     // two groups 78, by twice as many single ones 79; 256 rows: 117, 95, 47.5, 50.5; 64 rows, shared by two groups 27.9, by
     // as many single ones 25.3.)
     const double one = hd == 64 ? 0.67 : 1.1, two = hd == 64 ? 1.02 : 2.0, way = hd == 64 ? 0.012 : 0.018;
-    // (several sequences: taken to be three quarters as long as the longest)
-    const double tiles = longest / MANY_KEYS + 1, work = blocks * tiles * (a.sequences == 1 ? 1.0 : 0.75);
-    double best = 7 + (blocks <= cus ? one : two) * tiles;
-    p.waves = 4, p.parts = 0;
-    p.least = 4;
-    if (blocks <= cus && 8 + two * tiles / 2 < best) best = 8 + two * tiles / 2, p.waves = 8;
-    auto shared = [&](int waves, double most, double start, double tile) {
-      double n = std::min(most, sqrt(work * tile / way));
-      // (the blocks of one sequence are of one size, and go into equally many parts; of several, one goes into half a part
-      // too few in the mean)
-      if (a.sequences == 1) n = floor(n / blocks) * blocks;
-      if (a.sequences > 256 || n < (a.sequences == 1 ? 2.0 : 1.5) * blocks) return;
-      const double us = start + work * tile / (a.sequences == 1 ? n : n - blocks / 2) + n * way;
-      if (us < best) best = us, p.waves = waves, p.parts = (int)(n / a.kv_heads + 0.5);
-    };
-    shared(4, cus * 15 / 16.0, 12, one);  // (with as many as there are units some share one: 26.0, 240 of them 24.8)
-    shared(4, 2.0 * cus, 12, two);
-    shared(8, cus, 14, two / 2);
+    plan_tiles(p, a, cus, blocks, longest, one, two, way);
   }
   if (forced) {  // (shared in small parts, so that short sequences are divided too)
     const bool divides = forced == 4 || (forced > 6 && a.sequences <= 256 && full + sequences < 1000);

@@ -18,23 +18,12 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "attention_work.hpp"
+#include "attention_tiles.hpp"
 
 namespace adr {
 namespace {
 
 __global__ __launch_bounds__(256) void attention_u8_any_layout_kernel(Job) { rows_one_by_one<true>(arguments()); }
-
-// Eight codes c as c 2^-24.
-__device__ __forceinline__ half8_t widened(uint32_t w0, uint32_t w1) {
-  const u32x4_t r = {__builtin_amdgcn_perm(0u, w0, 0x0c010c00u), __builtin_amdgcn_perm(0u, w0, 0x0c030c02u),
-                     __builtin_amdgcn_perm(0u, w1, 0x0c010c00u), __builtin_amdgcn_perm(0u, w1, 0x0c030c02u)};
-  return __builtin_bit_cast(half8_t, r);
-}
-constexpr float WIDENED = 0x1p-24f;
-
-// The largest probability times scale may be this much above the reference, in log2 units.
-constexpr float GROWN_U8 = GROWN - 0.5f;
 
 // Where in a 256-byte line of the value tile a 16-byte chunk lies: the transposing reads of 32 lanes take a chunk each of rows
 // 4 g ... 4 g + 3 and 16 + 4 g ... 16 + 4 g + 3 of two g, and these 16 are on different banks.
@@ -453,8 +442,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
   }
 }
 
-int page_shift(int page_size) { return page_size >= 16 && (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1; }
-
 // What the matrix-core kernels take: whole chunks of 16 bytes at 16-byte addresses, 16 key rows within the reach of a
 // descriptor's 32-bit offsets, rows that do not overlap.
 bool chunks(const SequencesArgs& a) {
@@ -467,62 +454,84 @@ bool chunks(const SequencesArgs& a) {
          page_shift(a.page_size) >= 0;
 }
 
-constexpr int64_t LAUNCH_BLOCKS = 0x7fffffff / 256;
-int64_t most_blocks(const SequencesArgs& a, int rows) {
-  return ((int64_t)a.rows * a.group / rows + std::min(a.rows, a.sequences)) * a.kv_heads;
-}
-
 }  // namespace
 
 SequencesPlan sequences_u8_plan(const SequencesArgs& a, int cus, int64_t avail) {
   const SequencesPlan any = {SequencesPlan::ANY_LAYOUT, 0, 0, 0, 0, 0};
-  if (!chunks(a) || knob(KNOB_SEQUENCES) == 1) return any;
-  SequencesPlan p = {SequencesPlan::FEW_ROWS, 2, 0, 0, 1, 0};
-  const int hd = a.d <= 64 ? 64 : 128;
+  // (1: any layout; 2 ... 4: few rows, unshared with two or eight wavefronts, shared; 5 ... 8: many; as sequences_plan)
+  const int forced = knob(KNOB_SEQUENCES) >= 1 && knob(KNOB_SEQUENCES) <= 8 ? knob(KNOB_SEQUENCES) : 0;
+  if (!chunks(a) || forced == 1) return any;
   const int longest_rows = a.longest_rows > 0 ? std::min(a.longest_rows, a.rows) : a.rows;
+  SequencesPlan p = {(int64_t)longest_rows * a.group <= FEW ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES, 2, 0, 0, 1, 0};
+  if (forced) p.kind = forced <= 4 ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES;
+  const bool few = p.kind == SequencesPlan::FEW_ROWS;
+  const int rows = few ? FEW : MANY, keys = few ? FEW_KEYS : MANY_KEYS, hd = a.d <= 64 ? 64 : 128;
   const int64_t most_keys = std::min((int64_t)a.table_width * a.page_size, (int64_t)MOST_KEYS);
   const double longest = a.longest > 0 ? std::min<double>(a.longest, most_keys) : most_keys;
-  const double full = (double)a.rows * a.group / FEW, blocks = a.kv_heads * std::max(full, (double)std::min(a.rows, a.sequences));
-  (void)longest_rows;
-  const double alone = longest * hd * 3.3e-5, all = blocks * longest * hd * 2 / 6e6;
-  const bool unshared = blocks <= cus ? 4.0 + alone < 9.3 + all / 2 : alone < 9.0;
-  const int each = hd == 64 ? 8 : 4;
-  p.parts = unshared ? 0 : std::max(1, each * cus / a.kv_heads);
-  const int forced = knob(KNOB_SEQUENCES) >= 2 && knob(KNOB_SEQUENCES) <= 8 ? knob(KNOB_SEQUENCES) : 0;
-  if (!forced && blocks <= cus) p.waves = 8;
-  if (forced) p.waves = forced == 3 ? 8 : 2;
-  if (forced) p.parts = forced == 4 ? std::max(16, cus / a.kv_heads) : 0;
-  const double most_tiles = ((double)a.rows * a.group / FEW + a.sequences) * (most_keys / FEW_KEYS + 2.0);
+  const int sequences = std::min(a.rows, a.sequences);
+  const double full = (double)a.rows * a.group / rows, ends = (double)longest_rows * sequences > 4.0 * a.rows ? sequences : sequences / 2.0;
+  const double blocks = a.kv_heads * (few ? std::max(full, (double)sequences) : sequences <= 1 ? ceil(full) : std::max(full + ends, (double)sequences));
+  if (few) {
+    const double alone = longest * hd * 3.3e-5, all = blocks * longest * hd * 2 / 6e6;
+    const bool unshared = blocks <= cus ? 4.0 + alone < 9.3 + all / 2 : alone < 9.0;
+    const int each = hd == 64 ? 8 : 4;
+    p.parts = unshared ? 0 : std::max(1, each * cus / a.kv_heads);
+    if (unshared && blocks <= cus) p.waves = 8;
+  } else {
+    const double one = hd == 64 ? 0.67 : 1.1, two = hd == 64 ? 1.02 : 2.0, way = hd == 64 ? 0.012 : 0.018;
+    plan_tiles(p, a, cus, blocks, longest, one, two, way);
+  }
+  if (forced) {  // (shared in small parts, so that short sequences are divided too)
+    const bool divides = forced == 4 || (forced > 6 && a.sequences <= 256 && full + sequences < 1000);
+    p.waves = forced == 3 || forced == 6 || forced == 8 ? 8 : forced == 5 || forced == 7 ? 4 : 2;
+    p.parts = divides ? std::max(16, cus / a.kv_heads) : 0;
+    p.least = 1;
+  }
+  const double most_tiles = ((double)a.rows * a.group / rows + a.sequences) * (most_keys / keys + 2.0);
   for (p.shift = FEW_SHIFT; most_tiles > ldexp(0x1p29, p.shift) && p.shift < 25; p.shift++) {}
-  const int64_t part = (2 * (int64_t)FEW * (hd * 4 + 8) + (int64_t)sizeof(Seam)) * a.kv_heads;
+  const int64_t part = ((few ? 2 : 1) * (int64_t)rows * (hd * 4 + 8) + (int64_t)sizeof(Seam)) * a.kv_heads;
   p.parts = (int)std::min<int64_t>(p.parts, avail / part);
   if (p.parts < 2) p.parts = 0;
-  if (p.parts == 0 && most_blocks(a, FEW) > LAUNCH_BLOCKS) return any;
+  if (p.parts == 0 && most_blocks(a, rows) > LAUNCH_BLOCKS) return any;
   p.workspace_bytes = p.parts * part;
   return p;
 }
 
 template <int HD, bool TREE>
 static hipError_t launch_blocks(hipStream_t stream, const SequencesArgs& a, const SequencesPlan& p, void* workspace) {
+  const bool few = p.kind == SequencesPlan::FEW_ROWS;
+  const int rows = few ? FEW : MANY;
   Job job;
   (SequencesArgs&)job = a;
   job.page_shift = page_shift(a.page_size);
   job.parts = p.parts, job.shift = p.shift, job.least = p.least;
   job.per_head = 1.0 / a.group;
-  const int64_t part_rows = 2 * (int64_t)p.parts * a.kv_heads * FEW;
+  const int64_t part_rows = (int64_t)(few ? 2 : 1) * p.parts * a.kv_heads * rows;
   job.part_o = (float*)workspace;
   job.part_ml = (float2*)(job.part_o + part_rows * HD);
   job.seams = (Seam*)(job.part_ml + part_rows);
-  const int64_t blocks = p.parts == 0 ? most_blocks(a, FEW) : (int64_t)p.parts * a.kv_heads;
+  const int64_t most = most_blocks(a, rows), shared = (int64_t)p.parts * a.kv_heads;
+  const int64_t blocks = p.parts == 0 ? most : few ? shared : std::max(shared, most);
   if (blocks > LAUNCH_BLOCKS) return hipErrorInvalidConfiguration;
-  const int at_once = std::min(FEW, 1024 / HD);
-  const dim3 grid((unsigned)blocks), join((unsigned)((p.parts - 1) * a.kv_heads * (FEW / at_once)));
-  if (p.parts > 0) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_u8_few_rows_kernel<HD, 2, true, TREE>), grid, dim3(128), 2 * few_bytes(HD), stream, job);
+  const int at_once = std::min(rows, 1024 / HD);  // rows of the joining workgroups
+  const dim3 grid((unsigned)blocks), join((unsigned)((few ? p.parts - 1 : p.parts / 2) * a.kv_heads * (rows / at_once)));
+  const dim3 threads(64 * p.waves);
+  const size_t few_lds = (size_t)p.waves * few_bytes(HD);
+  if (few && p.parts > 0) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_u8_few_rows_kernel<HD, 2, true, TREE>), grid, threads, few_lds, stream, job);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, FEW, true>), join, dim3(256), 0, stream, job);
+  } else if (few && p.waves == 8) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_u8_few_rows_kernel<HD, 8, false, TREE>), grid, threads, few_lds, stream, job);
+  } else if (few) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_u8_few_rows_kernel<HD, 2, false, TREE>), grid, threads, few_lds, stream, job);
+  } else if (p.parts > 0) {
+    if (p.waves == 8) hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, true, true, 2, TREE, true>), grid, threads, 0, stream, job);
+    else hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, true, true, 1, TREE, true>), grid, threads, 0, stream, job);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_join_kernel<HD, MANY, true>), join, dim3(256), 0, stream, job);
+  } else if (p.waves == 8) {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, true, false, 2, TREE, true>), grid, threads, 0, stream, job);
   } else {
-    if (p.waves == 8) hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_u8_few_rows_kernel<HD, 8, false, TREE>), grid, dim3(512), 8 * few_bytes(HD), stream, job);
-    else hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_u8_few_rows_kernel<HD, 2, false, TREE>), grid, dim3(128), 2 * few_bytes(HD), stream, job);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(attention_tiles_kernel<HD, true, false, 1, TREE, true>), grid, threads, 0, stream, job);
   }
   return hipGetLastError();
 }

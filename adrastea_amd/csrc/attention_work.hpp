@@ -52,6 +52,17 @@ __device__ __forceinline__ bool round_means(half4_t& h, const float4_t& v, float
   return finite;
 }
 
+// Eight codes c as c 2^-24.
+__device__ __forceinline__ half8_t widened(uint32_t w0, uint32_t w1) {
+  const u32x4_t r = {__builtin_amdgcn_perm(0u, w0, 0x0c010c00u), __builtin_amdgcn_perm(0u, w0, 0x0c030c02u),
+                     __builtin_amdgcn_perm(0u, w1, 0x0c010c00u), __builtin_amdgcn_perm(0u, w1, 0x0c030c02u)};
+  return __builtin_bit_cast(half8_t, r);
+}
+constexpr float WIDENED = 0x1p-24f;
+
+// The largest probability times scale may be this much above the reference, in log2 units.
+constexpr float GROWN_U8 = GROWN - 0.5f;
+
 // What a kernel is given.  Share of the work: see below.
 struct Job : SequencesArgs {
   int page_shift;   // log2 of the slots of a page (16 at least: 16 keys from a multiple of 16 on lie on one page)
