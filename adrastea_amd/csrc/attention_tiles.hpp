@@ -40,7 +40,8 @@ namespace {
 // U8: the cache is one of codes (attention_u8.hip, which explains the arithmetic).  They lie in LDS as they come and are widened
 // behind its reads: a wavefront widens all of a tile, 128 instructions, where one that widened a quarter for all four would have half
 // of that and the tile's way through LDS once more.  A lane reads 16 codes of a key at once, for two steps of the product.
-// A tile's scales come with its keys, by a transfer of their own, and are looked at by the wavefront that asked for them.
+// Scales come for four tiles at a time, one for each wavefront, by transfers of their own: the table's entries, the scales' words, and
+// what is made of them, each a half tile behind the other.
 template <int HD, bool PAGED, bool SHARED, int GROUPS, bool TREE = false, bool U8 = false>
 __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
   static_assert(PAGED || !U8, "codes are in pages");
@@ -55,10 +56,11 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
   // K0 K1 V0 V1 of each group (of codes: room for the queries on their way, and the results)
   constexpr int GROUP_BYTES = !U8 ? 4 * TILE : HD == 128 ? 52 * 1024 : 28 * 1024;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[GROUPS * GROUP_BYTES];
-  // U8: two tiles' scales as they come, of each wavefront, and four tiles' as they are used: of keys, values, and their logarithms
-  __shared__ __attribute__((aligned(16))) uint32_t raw_scales[U8 ? 4 * GROUPS : 1][2][64];
-  __shared__ __attribute__((aligned(16))) half_t scales[U8 ? GROUPS : 1][4][3][KEYS];
-  __shared__ __attribute__((aligned(16))) half_t unit_scales[KEYS];
+  // U8: what has been asked for of a tile's 64 keys (pages, and words that hold a key's and a value's scale), of each wavefront; and
+  // eight tiles' scales as they are used: factors of the scores, scales of the values, and their logarithms
+  __shared__ __attribute__((aligned(16))) uint32_t asked[U8 ? 4 * GROUPS : 1][3][KEYS];
+  __shared__ __attribute__((aligned(16))) float scales[U8 ? GROUPS : 1][8][3][KEYS];
+  __shared__ __attribute__((aligned(16))) float unit_scales[KEYS];
   __shared__ int lost_keys[4 * GROUPS];  // of each wavefront
 
   // Consecutive workgroups go to different dies; where the key heads divide evenly, a die takes its share of them, so
@@ -152,7 +154,6 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     uint64_t base, p, pages;
     int64_t page_stride;
     int bytes, key, stride;
-    int page, left;  // U8, of the keys' tile: -1 on no page, and keys
   };
   bool lost = false;  // a key's page is not in the cache
   int page = 0;
@@ -173,7 +174,6 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
         const int slot = key & ((1 << a.page_shift) - 1);
         t.pages = page < 0 ? 0 : (t.base + BYTES * (page * t.page_stride + slot * (int64_t)t.stride)) | 1;
       }
-      if constexpr (U8 && decltype(is_k)::value) t.page = __builtin_amdgcn_readlane(page, n & 63), t.left = left;
       const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)t.pages, n & 63);
       const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(t.pages >> 32), n & 63);
       t.p = (uint64_t)hi << 32 | (lo & ~1u);
@@ -209,40 +209,50 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     else if constexpr (decltype(is_k)::value) dma_buffer_pair<J>(dst, koff[J], koff[J + 1], desc);
     else dma_buffer_pair<J>(dst, voff[J], voff[J + 1], desc);
   };
-  // U8.  The scales of the next tile's 16 rows: lanes 0 ... 15 (and 32 ... 47) those of keys, the others those of values, as the words
-  // that hold them.  A transfer in any case, so that the waits count right: of what is not there, some other word.
-  struct Asked {
-    int tile, left;  // of the group, and its keys; 0: none, or on no page
-    bool lost, upper;
+  // U8.  Scales of tile t of the group (a lane has a key), in three steps.  Transfers are made in any case, so that the waits count
+  // right: of what is not there, some other word.
+  uint32_t upper = 0;  // bits: the scale is in its word's upper half
+  const float factor = U8 ? a.c / WIDENED : a.c;  // of the scores (of codes: they are times 2^-24)
+  auto key_of = [&](int t) __attribute__((always_inline)) { return (tile0 + t) * KEYS + lane; };
+  auto page_word = [&](int t) __attribute__((always_inline)) {
+    const int key = key_of(t);
+    return key < row_end ? a.table + (int64_t)q.index * a.table_pitch + (key >> a.page_shift) : a.row_offsets;
   };
-  Asked asked[2] = {};  // the last two
-  auto ask_scales = [&](const Next& t) __attribute__((always_inline)) {
-    if constexpr (U8) {
-      const int tile = (t.key >> 6) - tile0, r = lane & 15;
-      const bool is_v = lane & 16, good = t.page >= 0 && r < t.left;
-      const int64_t slot = (t.key & ((1 << a.page_shift) - 1)) + r;
-      const half_t* p = is_v ? a.v_scale + hk * a.svs.z + t.page * a.svs.p + slot * a.svs.y
-                             : a.k_scale + hk * a.sks.z + t.page * a.sks.p + slot * a.sks.y;
-      if (!good) p = (const half_t*)a.row_offsets;
-      asked[0] = asked[1];
-      asked[1] = Asked{tile, t.page < 0 && t.left > 0 ? 0 : t.left, t.page < 0 && t.left > 0, ((uintptr_t)p & 2) != 0};
-      dma_global_word((uint32_t)(uintptr_t)ADR_LDS_PTR(&raw_scales[4 * group + w][tile & 1][0]), (const void*)((uintptr_t)p & ~(uintptr_t)3));
+  auto scale_words = [&](int t, int page, const half_t*& k, const half_t*& v) __attribute__((always_inline)) {
+    const int key = key_of(t), slot = key & ((1 << a.page_shift) - 1);
+    k = v = (const half_t*)a.row_offsets;
+    if (key < row_end && page >= 0 && page < a.pages) {
+      k = a.k_scale + hk * a.sks.z + page * a.sks.p + slot * a.sks.y;
+      v = a.v_scale + hk * a.svs.z + page * a.svs.p + slot * a.svs.y;
     }
   };
-  // Those that have landed, as they are used: 0 for keys that are not there, NaN and 0 for keys that count as NaN.
-  auto keep_scales = [&](const Asked& s) __attribute__((always_inline)) {
+  // As they are used: of keys that are not there whatever is finite, of those that count as NaN a factor of NaN and values of 0.
+  // (A factor of 0 is the smallest number instead: hidden scores stay -inf.)
+  auto keep = [&](int t, int page, half_t ks, half_t vs) __attribute__((always_inline)) {
+    const bool there = key_of(t) < row_end, good = page >= 0 && page < a.pages && scale_fits(ks) && scale_fits(vs);
+    const float k = !there ? 1.0f : !good ? NAN : (float)ks == 0.0f ? 0x1p-126f : (float)ks * factor;
+    const float v = there && good ? (float)vs : 0.0f;
+    float(*const to)[KEYS] = scales[U8 ? group : 0][t & 7];
+    to[0][lane] = k, to[1][lane] = v, to[2][lane] = __builtin_amdgcn_logf(fmaxf(fabsf(v), 0x1p-25f));
+  };
+  const uint32_t asked_lds = (uint32_t)(uintptr_t)ADR_LDS_PTR(&asked[U8 ? 4 * group + w : 0][0][0]);
+  auto whole_word = [](const void* p) __attribute__((always_inline)) { return (const void*)((uintptr_t)p & ~(uintptr_t)3); };
+  // In the second half of tile i; what is asked for there has landed at the end of the first half of tile i + 1.
+  auto scales_step = [&](int i) __attribute__((always_inline)) {
     if constexpr (U8) {
-      const uint32_t word = raw_scales[4 * group + w][s.tile & 1][lane];
-      half_t v = bits_to_half((uint16_t)(s.upper ? word >> 16 : word));
-      const int r = lane & 15;
-      const bool is_v = lane & 16, there = r < s.left;
-      if (!there) v = (half_t)0;
-      int bad = s.lost || !scale_fits(v);
-      bad |= __builtin_amdgcn_ds_swizzle(bad, 0x401f);  // lane ^ 16
-      if (bad) v = is_v ? (half_t)0 : (half_t)NAN;
-      half_t(*const to)[KEYS] = scales[group][s.tile & 3];
-      if (lane < 32) to[is_v][16 * w + r] = v;
-      if (is_v && lane < 32) to[2][16 * w + r] = (half_t)__builtin_amdgcn_logf(fmaxf(fabsf((float)v), 0x1p-25f));
+      if ((i & 3) == 0) {
+        dma_global_word(asked_lds, page_word(i + 4 + w));
+      } else if ((i & 3) == 1) {
+        const half_t *k, *v;
+        scale_words(i + 3 + w, (int)asked[4 * group + w][0][lane], k, v);
+        upper = ((uintptr_t)k >> 1 & 1) | ((uintptr_t)v & 2);
+        dma_global_word(asked_lds + KEYS * 4, whole_word(k));
+        dma_global_word(asked_lds + 2 * KEYS * 4, whole_word(v));
+      } else if ((i & 3) == 2) {
+        const uint32_t* const words = &asked[4 * group + w][0][lane];
+        const uint32_t k = words[KEYS], v = words[2 * KEYS];
+        keep(i + 2 + w, (int)words[0], bits_to_half((uint16_t)(upper & 1 ? k >> 16 : k)), bits_to_half((uint16_t)(upper & 2 ? v >> 16 : v)));
+      }
     }
   };
   const std::integral_constant<int, 0> pair0{};
@@ -250,22 +260,30 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
   auto tile_transfers = [&](Next& t, auto k, int buf) __attribute__((always_inline)) {
     transfer(t, k, buf, pair0);
     if constexpr (NI > 2) transfer(t, k, buf, pair1);
-    if constexpr (decltype(k)::value) ask_scales(t);
     advance(t, k);
   };
-  // What is waited for at the end of each half: all transfers but those issued in it, of values, or of keys (and their scales).
-  auto wait_landed = [&](auto k) __attribute__((always_inline)) { wait_vm<NI + (U8 && decltype(k)::value)>(); };
+  // What is waited for at the end of each half: all transfers but those issued in it, of values, or of keys, and of scales.
+  auto wait_landed = [&](auto k, int i) __attribute__((always_inline)) {
+    if (U8 && decltype(k)::value && (i & 3) == 0) wait_vm<NI + 1>();
+    else if (U8 && decltype(k)::value && (i & 3) == 1) wait_vm<NI + 2>();
+    else wait_vm<NI>();
+    if (U8 && decltype(k)::value && (i & 3) == 2) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (scales are there for the others)
+  };
 
   tile_transfers(nk, is_k, 0);
   tile_transfers(nk, is_k, 1);
-  const Asked first_scales = asked[0];
+  if constexpr (U8) {  // the first four tiles' scales, one to each wavefront
+    const half_t *k, *v;
+    const int page = *page_word(w);
+    scale_words(w, page, k, v);
+    keep(w, page, *k, *v);
+    unit_scales[lane] = 1.0f;  // (each wavefront: nobody waits for another's)
+  }
   // LDS fragment offsets.  K: lane -> tile row frow (+32), chunk 2*ds + g.
   int offK[DS];
 #pragma unroll
   for (int ds = 0; ds < DS; ds++) offK[ds] = k_chunk_off<CPR>(frow, U8 ? (ds >> 1) * 2 + g : ds * 2 + g);
-  wait_landed(is_k);  // the queries and the first K tile have landed
-  keep_scales(first_scales);
-  if constexpr (U8) unit_scales[lane] = (half_t)1;  // (each wavefront: nobody waits for another's)
+  wait_vm<NI>();  // the queries and the first K tile have landed
   half8_t qf[DS];  // (operand B of S^T = K Q^T: lane -> row frow, head-dimension group g)
 #pragma unroll
   for (int ds = 0; ds < DS; ds++) {
@@ -302,7 +320,7 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
 
   float16_t o[DT], sa[2], sb[2];  // sums of P.V; scores of two tiles in turn
   float sum_of_p = 0.0f;          // U8: of the rounded probabilities, in this lane
-  const float factor = U8 ? a.c / WIDENED : a.c;  // of the scores (of codes: they are times 2^-24)
+  const float* by = unit_scales;  // U8: factors of the scores of the tile whose probabilities come next
   constexpr float MOST = U8 ? GROWN_U8 : GROWN;
   u32x4_t pf[2][2];                 // probabilities, two to a register
 #pragma unroll
@@ -376,17 +394,18 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     constexpr int NP = 4 * NG, VP = 32 / NP;
     float sum[2] = {l_run, 0.0f};
     float ex[VP], pw[VP];
-    half4_t vs[2];  // U8: the scales of the tile's values, of four keys and the next four
-    auto read_vs = [&](int x) __attribute__((always_inline)) {
+    float4_t ks[2], vs[2];  // U8: the tile's factors and scales, of four keys and the next four
+    auto read_scales = [&](int x) __attribute__((always_inline)) {
       if constexpr (U8 && P) {
-        if (x < 8) vs[x & 1] = *(const half4_t*)&scales[group][i & 3][1][32 * (x >> 2) + 8 * (x & 3) + 4 * g];
+        const int key = 32 * (x >> 2) + 8 * (x & 3) + 4 * g;
+        if (x < 8) ks[x & 1] = *(const float4_t*)(by + key), vs[x & 1] = *(const float4_t*)&scales[group][i & 7][1][key];
       }
     };
-    read_vs(0);
-    read_vs(1);
+    read_scales(0);
+    read_scales(1);
     auto stage_exponent = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 0; e < VP; e++) ex[e] = fmaf(cur[k * VP >> 4][(k * VP & 15) + e], factor, -m_run);
+      for (int e = 0; e < VP; e++) ex[e] = fmaf(cur[k * VP >> 4][(k * VP & 15) + e], U8 ? ks[k * VP >> 2 & 1][(k * VP & 3) + e] : factor, -m_run);
     };
     auto stage_power = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -397,7 +416,7 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
       for (int e = 0; e < VP; e += 2) {
         const int x = k * VP + e;
         float2_t e2 = {pw[e], pw[e + 1]};
-        if constexpr (U8) e2 = float2_t{pw[e] * (float)vs[x >> 2 & 1][x & 3], pw[e + 1] * (float)vs[x >> 2 & 1][(x & 3) + 1]};
+        if constexpr (U8) e2 = float2_t{pw[e] * vs[x >> 2 & 1][x & 3], pw[e + 1] * vs[x >> 2 & 1][(x & 3) + 1]};
         uint32_t bits = __builtin_bit_cast(uint32_t, __builtin_convertvector(e2, half2_t));
         sum[0] += pw[e];
         sum[1] += pw[e + 1];
@@ -405,7 +424,7 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
         pf[x >> 4][x >> 3 & 1][(x & 7) / 2] = bits;
         if constexpr (U8) {
           sum_of_p = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, bits), half2_t{(half_t)1, (half_t)1}, sum_of_p, false);
-          if ((x & 3) == 2) read_vs((x >> 2) + 2);
+          if ((x & 3) == 2) read_scales((x >> 2) + 2);
         }
       }
     };
@@ -452,7 +471,7 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     }
     if constexpr (HD == 128) __builtin_amdgcn_s_setprio(0);
     advance(nv, is_v);
-    wait_landed(is_v);
+    wait_landed(is_v, i);
     barrier();
   };
 
@@ -464,18 +483,16 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     constexpr int VB = decltype(vbuf)::value, KB = VB;  // K buffer of tile i + 2
     const unsigned char* const cV = sm + (2 + VB) * TILE;
     const unsigned char* const cK = sm + KB * TILE;
-    keep_scales(asked[1]);  // (the transfer of the half before the last one)
-    // U8: the scales of the next tile's keys, and their values' logarithms, of four keys and the next four.  Where some keys are not
-    // seen, scores are scaled before those are taken out, and then by ones.
-    const half_t(*const next_scales)[KEYS] = scales[U8 ? group : 0][(i + 1) & 3];
-    const half_t* by = next_scales[0] + 4 * g;
-    half4_t ks[2], logs[2];
+    scales_step(i);
+    // U8: the factors of the next tile's scores, and its values' logarithms, of four keys and the next four.  Where some keys are not
+    // seen, scores are multiplied before those are taken out, and by ones from then on.
+    const float(*const next_scales)[KEYS] = scales[U8 ? group : 0][(i + 1) & 7];
+    if constexpr (U8 && MAX) by = next_scales[0];
+    float4_t ks[2], logs[2];
     auto read_scales = [&](int x) __attribute__((always_inline)) {
       if constexpr (U8 && MAX) {
-        if (x < 8) {
-          ks[x & 1] = *(const half4_t*)(by + 32 * (x >> 2) + 8 * (x & 3));
-          logs[x & 1] = *(const half4_t*)(next_scales[2] + 32 * (x >> 2) + 8 * (x & 3) + 4 * g);
-        }
+        const int key = 32 * (x >> 2) + 8 * (x & 3) + 4 * g;
+        if (x < 8) ks[x & 1] = *(const float4_t*)(by + key), logs[x & 1] = *(const float4_t*)(next_scales[2] + key);
       }
     };
     if constexpr (MAX) {
@@ -485,9 +502,9 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
         if constexpr (U8) {
 #pragma unroll
           for (int x = 0; x < 8; x++) {
-            const half4_t f = *(const half4_t*)(by + 32 * (x >> 2) + 8 * (x & 3));
+            const float4_t f = *(const float4_t*)(by + 32 * (x >> 2) + 8 * (x & 3) + 4 * g);
 #pragma unroll
-            for (int e = 0; e < 4; e++) nxt[x >> 2][4 * (x & 3) + e] *= (float)f[e];
+            for (int e = 0; e < 4; e++) nxt[x >> 2][4 * (x & 3) + e] *= f[e];
           }
           by = unit_scales;
         }
@@ -524,10 +541,7 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
       if constexpr (decltype(do_s)::value) {
         if (c + 1 == NG) read_k(cK, 0);
       }
-      if (c == 0) {
-        transfer(nk, is_k, 1 - KB, pair0);
-        ask_scales(nk);
-      }
+      if (c == 0) transfer(nk, is_k, 1 - KB, pair0);
       if constexpr (NI > 2) {
         if (c == NG / 2) transfer(nk, is_k, 1 - KB, pair1);
       }
@@ -548,9 +562,8 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
               const int x = first + 2 * e;
               float s0 = nxt[x >> 4][x & 15], s1 = nxt[x >> 4][(x & 15) + 1];
               if constexpr (U8) {
-                s0 *= (float)ks[x >> 2 & 1][x & 3], s1 *= (float)ks[x >> 2 & 1][(x & 3) + 1];
-                nxt[x >> 4][x & 15] = s0, nxt[x >> 4][(x & 15) + 1] = s1;
-                s0 = fmaf(s0, factor, (float)logs[x >> 2 & 1][x & 3]), s1 = fmaf(s1, factor, (float)logs[x >> 2 & 1][(x & 3) + 1]);
+                s0 = fmaf(s0, ks[x >> 2 & 1][x & 3], logs[x >> 2 & 1][x & 3]);
+                s1 = fmaf(s1, ks[x >> 2 & 1][(x & 3) + 1], logs[x >> 2 & 1][(x & 3) + 1]);
                 if ((x & 3) == 2) read_scales((x >> 2) + 2);
               }
               mx2[e & 1] = fmaxf(fmaxf(mx2[e & 1], s0), s1);
@@ -575,18 +588,16 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
       }
     }
     advance(nk, is_k);
-    if constexpr (U8) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the scales are there for the others)
-    wait_landed(is_k);
+    wait_landed(is_k, i);
     barrier();
   };
   auto idle = [&](int i) __attribute__((always_inline)) {
     tile_transfers(nv, is_v, 2 + ((i + 1) & 1));
-    wait_landed(is_v);
+    wait_landed(is_v, i);
     barrier();
-    keep_scales(asked[1]);
+    scales_step(i);
     tile_transfers(nk, is_k, (i + 1) & 1);
-    if constexpr (U8) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    wait_landed(is_k);
+    wait_landed(is_k, i);
     barrier();
   };
 
