@@ -462,24 +462,36 @@ SequencesPlan sequences_u8_plan(const SequencesArgs& a, int cus, int64_t avail) 
   const int forced = knob(KNOB_SEQUENCES) >= 1 && knob(KNOB_SEQUENCES) <= 8 ? knob(KNOB_SEQUENCES) : 0;
   if (!chunks(a) || forced == 1) return any;
   const int longest_rows = a.longest_rows > 0 ? std::min(a.longest_rows, a.rows) : a.rows;
-  SequencesPlan p = {(int64_t)longest_rows * a.group <= FEW ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES, 2, 0, 0, 1, 0};
-  if (forced) p.kind = forced <= 4 ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES;
-  const bool few = p.kind == SequencesPlan::FEW_ROWS;
-  const int rows = few ? FEW : MANY, keys = few ? FEW_KEYS : MANY_KEYS, hd = a.d <= 64 ? 64 : 128;
   const int64_t most_keys = std::min((int64_t)a.table_width * a.page_size, (int64_t)MOST_KEYS);
   const double longest = a.longest > 0 ? std::min<double>(a.longest, most_keys) : most_keys;
-  const int sequences = std::min(a.rows, a.sequences);
-  const double full = (double)a.rows * a.group / rows, ends = (double)longest_rows * sequences > 4.0 * a.rows ? sequences : sequences / 2.0;
-  const double blocks = a.kv_heads * (few ? std::max(full, (double)sequences) : sequences <= 1 ? ceil(full) : std::max(full + ends, (double)sequences));
+  const int sequences = std::min(a.rows, a.sequences), hd = a.d <= 64 ? 64 : 128;
+  // Blocks of all key heads, as far as the host can tell (as in sequences_plan), of either kernel.
+  auto blocks_of = [&](int rows) {
+    const double full = (double)a.rows * a.group / rows, ends = (double)longest_rows * sequences > 4.0 * a.rows ? sequences : sequences / 2.0;
+    return a.kv_heads * (sequences <= 1 ? ceil(full) : std::max(full + ends, (double)sequences));
+  };
+  // Blocks of few rows read the keys once each, at 24 bytes a ns and compute unit; of many rows, they compute a tile of 64 keys in 1.5 us.
+  // So three of the former to one of the latter take as much (drafts of 2 to 13 tokens, 4 heads to a key head, 24 sequences: 56 us, 70).
+  const bool one_block = (int64_t)longest_rows * a.group <= FEW;
+  const double few_blocks = one_block ? a.kv_heads * std::max((double)a.rows * a.group / FEW, (double)sequences) : blocks_of(FEW);
+  SequencesPlan p = {one_block || few_blocks < 3.0 * blocks_of(MANY) ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES, 2, 0, 0, 1, 0};
+  if (forced) p.kind = forced <= 4 ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES;
+  const bool few = p.kind == SequencesPlan::FEW_ROWS;
+  const int rows = few ? FEW : MANY, keys = few ? FEW_KEYS : MANY_KEYS;
+  const double full = (double)a.rows * a.group / rows, blocks = few ? few_blocks : blocks_of(MANY);
   if (few) {
-    const double alone = longest * hd * 3.3e-5, all = blocks * longest * hd * 2 / 6e6;
-    const bool unshared = blocks <= cus ? 4.0 + alone < 9.3 + all / 2 : alone < 9.0;
-    const int each = hd == 64 ? 8 : 4;
-    p.parts = unshared ? 0 : std::max(1, each * cus / a.kv_heads);
-    if (unshared && blocks <= cus) p.waves = 8;
+    // us, fitted to 1 to 200 sequences of up to 300 to 4000 keys, 8 key heads of 128: a block to eight wavefronts, which have a compute
+    // unit to themselves; to two; keys shared, whose sum counts and not the longest.  (64 sequences of up to 1000, 2000, 4000
+    // keys: 24.6, 32.9, 54.6; 25.8, 45.3, 84.6; shared, of 4000, 56.2.  100: 39, 52, 85; 30, 53, 101; 84.6.  8: 11.7, 17.2, 27.6;
+    // 20, 36, 68; shared, of 2000 and 4000, 15.1, 17.2.)
+    const double size = longest / 1000 * hd / 128, rounds = std::max(1.0, blocks / cus), all = blocks * longest * hd * 2 / 6e6;
+    const double eight = 2 + 5 * rounds + 5.4 * size * rounds, two = 6 + size * std::max(13 + 0.0125 * blocks, 0.028 * blocks);
+    const double shared = 12 + all * (sequences > 1 ? 0.53 : 1.0);
+    if (shared < std::min(eight, two)) p.parts = std::max(1, (hd == 64 ? 8 : 4) * cus / a.kv_heads);
+    else p.waves = eight < two ? 8 : 2;
   } else {
-    const double one = hd == 64 ? 0.67 : 1.1, two = hd == 64 ? 1.02 : 2.0, way = hd == 64 ? 0.012 : 0.018;
-    plan_tiles(p, a, cus, blocks, longest, one, two, way);
+    // (a tile takes a third longer than one of values in 16 bits)
+    plan_tiles(p, a, cus, blocks, longest, hd == 64 ? 0.85 : 1.4, hd == 64 ? 1.4 : 2.6, hd == 64 ? 0.012 : 0.018);
   }
   if (forced) {  // (shared in small parts, so that short sequences are divided too)
     const bool divides = forced == 4 || (forced > 6 && a.sequences <= 256 && full + sequences < 1000);
