@@ -54,6 +54,8 @@ __device__ __forceinline__ T sum_of(T v) {
   if constexpr (W > 16) v += partner<16>(v);
   return v;
 }
+__device__ __forceinline__ float absolute(float a) { return fabsf(a); }
+__device__ __forceinline__ double absolute(double a) { return fabs(a); }
 __device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
 template <int W, typename T>
@@ -107,15 +109,15 @@ __device__ __forceinline__ float step_of(float v) { return floorf(v); }
 __device__ __forceinline__ double step_of(double v) { return floor(v); }
 __device__ __forceinline__ float fused(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double fused(double a, double b, double c) { return fma(a, b, c); }
-// (inv: 1 / s, whose last bit may be wrong, so that the quotient is looked at again; 0 where s is 0 or NaN)
+// 128 + floor(y / s), by a product with 1 / s (0 where s is 0 or NaN): that is off by so little that a quotient which is an integer is
+// lifted over its border by `lift`, and no other one is.  Quotients of fp16 numbers, of 128 at most, are integers or 2^-12 from the
+// next one, and the product in 32 bits is off by 2^-15; in 64 bits those that lie within 2^-40 below an integer are lost.  The
+// numbers below 0 that come too near are told by their sign.
 template <typename T>
-__device__ __forceinline__ uint32_t code_of(T y, T s, T inv) {
-  if (!(inv > 0)) return 128;
-  T k = step_of(y * inv);
-  const T rest = fused(-k, s, y);
-  if (rest < 0) k -= 1;
-  if (rest >= s) k += 1;
-  return (uint32_t)(int)fminf(fmaxf((float)k + 128.0f, 0.0f), 255.0f);
+__device__ __forceinline__ uint32_t code_of(T y, T inv) {
+  constexpr T lift = sizeof(T) == 8 ? (T)0x1p-40 : (T)0x1p-13;
+  const int k = (int)step_of(fused(y, inv, lift));
+  return (uint32_t)(min(max(k, -128), y < 0 && inv > 0 ? -1 : 127) + 128);
 }
 template <typename T>
 __device__ __forceinline__ T inverse_of(half_t s) {
@@ -144,6 +146,34 @@ __device__ __forceinline__ Slot slot_of(const adr_paged_batch& b, int rows, int 
     if (row == r) s = at;
   }
   const int begin = clamp_to(b.row_offsets[s], rows), end = clamp_to(b.row_offsets[s + 1], rows), length = b.lengths[s];
+  Slot p = {row, 0, -1, 0};
+  if (row < begin || row >= end) {
+    p.row = -1;
+    return p;
+  }
+  const int64_t x = (int64_t)length - end + row;
+  p.position = (int)x;
+  if (x >= 0 && x < (int64_t)b.table_width * page_size) {
+    const int at = (int)x / page_size, page = b.table[(int64_t)s * b.table_pitch + at];
+    p.slot = (int)x - at * page_size;
+    p.page = page >= 0 && page < pages ? page : -1;
+  }
+  return p;
+}
+
+// The same of one row, by a wavefront.  Up to 63 sequences are known by one way to memory.
+__device__ __forceinline__ Slot slot_of_row(const adr_paged_batch& b, int rows, int pages, int page_size, int row, int lane) {
+  int s, begin, end, length;
+  if (b.sequences < 64) {
+    const int offset = lane <= b.sequences ? b.row_offsets[lane] : 0x7fffffff, of_lane = lane < b.sequences ? b.lengths[lane] : 0;
+    s = max(__popcll(__ballot(lane < b.sequences && offset <= row)), 1) - 1;
+    begin = __builtin_amdgcn_readlane(offset, s), end = __builtin_amdgcn_readlane(offset, s + 1);
+    length = __builtin_amdgcn_readlane(of_lane, s);
+  } else {
+    s = uniform(sequence_of_row(b.row_offsets, b.sequences, row, lane));
+    begin = b.row_offsets[s], end = b.row_offsets[s + 1], length = b.lengths[s];
+  }
+  begin = clamp_to(begin, rows), end = clamp_to(end, rows);
   Slot p = {row, 0, -1, 0};
   if (row < begin || row >= end) {
     p.row = -1;
@@ -194,6 +224,14 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
   const bool one = x1 >= a.d;  // (the last of an odd number: its chunk twice)
   if (one) x1 = x0, turn1 = false;
   const float per_value = 1.0f / (float)a.d;
+  // What does not depend on the row, and is asked for ahead of all else: the lane's own pair, and the queries' weights.
+  const int half = a.dims >> 1, own_pair = min(lane, max(half - 1, 0));
+  const double own_turns = half > 0 ? a.turns[own_pair] : 0.0;
+  const int own_axis = half > 0 && a.axis ? a.axis[own_pair] : 0;
+  half8_t qw0, qw1;
+#pragma unroll
+  for (int e = 0; e < 8; e++) qw0[e] = qw1[e] = (half_t)1;
+  if (a.q_weight) qw0 = *(const half8_t*)(a.q_weight + x0), qw1 = *(const half8_t*)(a.q_weight + x1);
   const uint32_t tasks = (uint32_t)a.rows * a.splits;  // (splits are more than one where there are few rows)
   for (uint64_t task = (uint64_t)blockIdx.x * 4 + wave; task < tasks; task += (uint64_t)gridDim.x * 4) {
     const int row = uniform((int)((uint32_t)task / (uint32_t)a.splits)), split = uniform((int)((uint32_t)task - (uint32_t)row * a.splits));
@@ -207,27 +245,22 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
       n0 = *(const half8_t*)(from + x0);
       n1 = *(const half8_t*)(from + x1);
     };
+    const int own_position = a.positions && half > 0
+                                 ? a.positions[(int64_t)((unsigned)own_axis < (unsigned)a.axes ? own_axis : 0) * a.positions_pitch + row] : 0;
     read(min(h0, all - 1));
     Slot at = {row, 0, -1, 0};
     if constexpr (CACHE != NO_CACHE) {
       const int pages = CACHE == U8 ? a.codes.pages : a.cache.pages, size = CACHE == U8 ? a.codes.page_size : a.cache.page_size;
-      at = slot_of(a.batch, a.rows, pages, size, row, row, row, lane);
+      at = slot_of_row(a.batch, a.rows, pages, size, row, lane);
       if (uniform(at.row) < 0) continue;
     }
-    for (int i = lane; i < a.dims >> 1; i += 64)
+    if (lane < half) turns[lane] = turn_of<angle_t>(a.positions ? own_position : at.position, own_turns, a.magnitude);
+    for (int i = lane + 64; i < half; i += 64)
       turns[i] = turn_of<angle_t>(position_of(a, row, i, at.position), a.turns[i], a.magnitude);
     __builtin_amdgcn_wave_barrier();
     const int end = CACHE != NO_CACHE && uniform(at.page) < 0 ? end_q : all;  // (keys and values without a slot go nowhere)
     if (h0 >= end) continue;
 
-    // The lane's eight pairs.
-    auto angles = [&](auto& mine8) __attribute__((always_inline)) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        mine8[e] = {1, 0};
-        if (e < 4 || !a.pairs ? turn0 : turn1) mine8[e] = {turns[8 * l + e].cosine, turns[8 * l + e].sine};
-      }
-    };
     auto store16 = [&](half_t* to, const half8_t& o0, const half8_t& o1) __attribute__((always_inline)) {
       *(half8_t*)(to + x0) = o0;
       *(half8_t*)(to + x1) = o1;
@@ -236,17 +269,13 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
     struct Coefficients {
       float uc[8], us[8], vc[8], vs[8];  // of each pair (u, v): u w cos, u w sin, v w cos, v w sin
     };
-    auto coefficients = [&](const half_t* weight, Coefficients& f) __attribute__((always_inline)) {
+    auto coefficients = [&](const half8_t& w0, const half8_t& w1, Coefficients& f) __attribute__((always_inline)) {
       Turn<float> t[8];
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         t[e] = {1, 0};
         if (e < 4 || !a.pairs ? turn0 : turn1) t[e] = {(float)turns[8 * l + e].cosine, (float)turns[8 * l + e].sine};
       }
-      half8_t w0, w1;
-#pragma unroll
-      for (int e = 0; e < 8; e++) w0[e] = w1[e] = (half_t)1;
-      if (weight) w0 = *(const half8_t*)(weight + x0), w1 = *(const half8_t*)(weight + x1);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const float wu = (float)(!a.pairs ? w0[e] : e < 4 ? w0[2 * e & 7] : w1[2 * e & 7]);
@@ -297,7 +326,7 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
       T top = 0, none = 0;
 #pragma unroll
       for (int e = 0; e < 16; e++) {
-        top = larger(top, y[e] < 0 ? -y[e] : y[e]);
+        top = larger(top, absolute(y[e]));
         none = fused(y[e], (T)0, none);  // (NaN behind what is not finite)
       }
       top = max_of<W>(top), none = sum_of<W>(none);
@@ -305,7 +334,7 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
       const T inv = inverse_of<T>(s);
       uint32_t c[4] = {};
 #pragma unroll
-      for (int e = 0; e < 16; e++) c[e / 4] |= code_of(y[e], (T)(float)s, inv) << 8 * (e % 4);
+      for (int e = 0; e < 16; e++) c[e / 4] |= code_of(y[e], inv) << 8 * (e % 4);
       *(u32x2_t*)(codes + x0) = u32x2_t{c[0], c[1]};
       *(u32x2_t*)(codes + x1) = u32x2_t{c[2], c[3]};
       *scale = s;
@@ -315,7 +344,7 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
     if (h < min(end, CACHE == F16 ? end_k : end_q)) {
       Coefficients f;
       if (h < end_q) {
-        coefficients(a.q_weight, f);
+        coefficients(qw0, qw1, f);
         half_t* to = a.q_out + h * (int64_t)a.so_z + row * (int64_t)a.so_y;
         for (; h < end_q; h += step, to += (int64_t)step * a.so_z) {
           const half8_t c0 = n0, c1 = n1;
@@ -324,7 +353,11 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
         }
       }
       if (CACHE == F16 && h < min(end, end_k)) {
-        coefficients(a.k_weight, f);
+        half8_t w0, w1;
+#pragma unroll
+        for (int e = 0; e < 8; e++) w0[e] = w1[e] = (half_t)1;
+        if (a.k_weight) w0 = *(const half8_t*)(a.k_weight + x0), w1 = *(const half8_t*)(a.k_weight + x1);
+        coefficients(w0, w1, f);
         const adr_paged_cache& c = a.cache;
         half_t* const to = (half_t*)c.key + at.page * c.stride_kp + at.slot * c.stride_ky;
         for (; h < end_k; h += step) {
@@ -337,10 +370,6 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
     if constexpr (CACHE == U8) {
       const adr_paged_cache_u8& c = a.codes;
       if (h < min(end, end_k)) {
-        Turn<double> t[8];
-        angles(t);
-        half8_t w0 = {}, w1 = {};
-        if (a.k_weight) w0 = *(const half8_t*)(a.k_weight + x0), w1 = *(const half8_t*)(a.k_weight + x1);
         uint8_t* const to = c.key + at.page * c.stride_kp + at.slot * c.stride_ky;
         half_t* const scale = (half_t*)c.key_scale + at.page * c.stride_ksp + at.slot * c.stride_ksy;
         for (; h < end_k; h += step) {
@@ -355,22 +384,26 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
             for (int e = 0; e < 8; e++) sum = fma(y[e], y[e], sum), sum1 = fma(y[8 + e], y[8 + e], sum1);
             sum = !mine ? 0.0 : one ? sum : sum + sum1;
             const double factor = 1.0 / sqrt(sum_of<W>(sum) / (double)a.d + (double)a.k_eps);
+            const half8_t w0 = *(const half8_t*)(a.k_weight + x0), w1 = *(const half8_t*)(a.k_weight + x1);
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] = y[e] * factor * (double)(float)w0[e], y[8 + e] = y[8 + e] * factor * (double)(float)w1[e];
           }
+          // (angles from LDS as they are used: in registers they would be 32 of them)
           if (a.pairs) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-              const double u = y[2 * e], v = y[2 * e + 1], x = u * t[e].cosine - v * t[e].sine, z = u * t[e].sine + v * t[e].cosine;
+              const Turn<double> t = turns[min(8 * l + e, MOST_PAIRS - 1)];
+              const double u = y[2 * e], v = y[2 * e + 1], x = u * t.cosine - v * t.sine, z = u * t.sine + v * t.cosine;
               y[2 * e] = (e < 4 ? turn0 : turn1) ? x : e >= 4 && one ? y[2 * e - 8] : u;
               y[2 * e + 1] = (e < 4 ? turn0 : turn1) ? z : e >= 4 && one ? y[2 * e - 7] : v;
             }
           } else if (turn0) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
+              const Turn<double> t = turns[8 * l + e];
               const double u = y[e], v = y[8 + e];
-              y[e] = u * t[e].cosine - v * t[e].sine;
-              y[8 + e] = u * t[e].sine + v * t[e].cosine;
+              y[e] = u * t.cosine - v * t.sine;
+              y[8 + e] = u * t.sine + v * t.cosine;
             }
           }
           place_codes(0.0, y, to + (h - end_q) * c.stride_kz, scale + (h - end_q) * c.stride_ksz);
@@ -412,7 +445,7 @@ __global__ __launch_bounds__(256) void place_any_layout_kernel(PlaceJob a) {
     Slot at = {row, 0, -1, 0};
     if constexpr (CACHE != NO_CACHE) {
       const int pages = CACHE == U8 ? a.codes.pages : a.cache.pages, size = CACHE == U8 ? a.codes.page_size : a.cache.page_size;
-      at = slot_of(a.batch, a.rows, pages, size, row, row, row, lane);
+      at = slot_of_row(a.batch, a.rows, pages, size, row, lane);
       if (at.row < 0 || (k >= 0 && at.page < 0)) continue;
     }
     const half_t* const from = k < 0   ? a.q + h * (int64_t)a.sq_z + row * (int64_t)a.sq_y
@@ -457,15 +490,15 @@ __global__ __launch_bounds__(256) void place_any_layout_kernel(PlaceJob a) {
         const int64_t x_step = v < 0 ? c.stride_kx : c.stride_vx;
         T top = 0, none = 0;
         each([&](int, T y0, int, T y1) __attribute__((always_inline)) {
-          top = larger(larger(top, y0 < 0 ? -y0 : y0), y1 < 0 ? -y1 : y1);
+          top = larger(larger(top, absolute(y0)), absolute(y1));
           none = fused(y0, (T)0, fused(y1, (T)0, none));
         });
         for (int i = 32; i > 0; i >>= 1) top = larger(top, __shfl_xor(top, i)), none += __shfl_xor(none, i);
         const half_t s = scale_of(none == 0 ? top : (T)INFINITY);
         const T inv = inverse_of<T>(s);
         each([&](int i0, T y0, int i1, T y1) __attribute__((always_inline)) {
-          to[i0 * x_step] = (uint8_t)code_of(y0, (T)(float)s, inv);
-          if (i1 >= 0) to[i1 * x_step] = (uint8_t)code_of(y1, (T)(float)s, inv);
+          to[i0 * x_step] = (uint8_t)code_of(y0, inv);
+          if (i1 >= 0) to[i1 * x_step] = (uint8_t)code_of(y1, inv);
         });
         if (lane == 0) *scale = s;
       } else {
