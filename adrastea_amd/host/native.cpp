@@ -23,7 +23,9 @@ PyObject *current_device, *raw_stream;                  // torch's functions
 PyObject *int32_type, *float16_type;                    // torch's types
 PyObject *s_shape, *s_stride, *s_dims, *s_strides, *s_storage, *s_layout, *s_offset, *s_data_ptr, *s_load, *s_store,
     *s_mask, *s_op, *s_scale, *s_beta, *s_bias, *s_is_contiguous, *s_get_device, *s_key, *s_value, *s_row_offsets, *s_lengths,
-    *s_table, *s_key_offsets, *s_longest_rows, *s_longest, *s_turns, *s_rotary_layout, *s_magnitude, *s_dtype;
+    *s_table, *s_key_offsets, *s_longest_rows, *s_longest, *s_turns, *s_rotary_layout, *s_magnitude, *s_dtype, *s_axis, *s_axes,
+    *s_weight, *s_eps, *s_key_scale, *s_value_scale, *s_bits;
+PyObject* axes_type;  // RotaryAxes
 
 decltype(&adr_matmul_f16) matmul_fn;
 decltype(&adr_attention_f16) attention_fn;
@@ -36,6 +38,13 @@ decltype(&adr_rotary_f16) rotary_fn;
 decltype(&adr_append_f16) append_fn;
 decltype(&adr_attention_paged_f16) paged_fn;
 decltype(&adr_attention_packed_f16) packed_fn;
+decltype(&adr_norm_rotary_f16) norm_rotary_fn;
+decltype(&adr_append_norm_f16) append_norm_fn;
+decltype(&adr_append_u8) append_u8_fn;
+decltype(&adr_read_u8) read_u8_fn;
+decltype(&adr_attention_paged_u8) paged_u8_fn;
+decltype(&adr_attention_tree_f16) tree_f16_fn;
+decltype(&adr_attention_tree_u8) tree_u8_fn;
 
 // A reference that is given back at the end of its scope.
 struct Ref {
@@ -636,6 +645,195 @@ PyObject* attention_packed_f16(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromLong(rc);
 }
 
+// ---- heads normed and turned, a cache in 8 bits, drafted trees.
+
+// A RotaryAxes, a Rotary (one axis) or None (nothing is turned)
+bool read_axes(PyObject* o, int64_t device, adr_rotary_axes& r) {
+  r = {nullptr, nullptr, 0, 0, 1.0f, 1};
+  if (o == Py_None) return true;
+  adr_rotary one;
+  if (!read_rotary(o, device, one)) return false;
+  r.turns = one.turns, r.dims = one.dims, r.layout = one.layout, r.magnitude = one.magnitude;
+  if ((PyObject*)Py_TYPE(o) != axes_type) return true;
+  const Ref axis(attr(o, s_axis));
+  int64_t n[MAX_RANK];
+  void* p;
+  if (!read_index(axis, 1, device, n, p) || n[0] * 2 != r.dims || !read_int32(o, s_axes, r.axes)) return false;
+  r.axis = (const int32_t*)p;
+  return true;
+}
+
+// positions[axes, rows], or [rows] for one axis, or None
+struct Positions {
+  const int32_t* ptr = nullptr;
+  int32_t pitch = 0;
+};
+bool read_axis_positions(PyObject* tensor, int64_t device, int64_t axes, int64_t rows, Positions& p) {
+  if (tensor == Py_None) return true;
+  const Ref type(attr(tensor, s_dtype)), shape(attr(tensor, s_shape)), strides(call(tensor, s_stride));
+  int64_t n[MAX_RANK], stride[MAX_RANK];
+  int rank = -1;
+  void* at;
+  if (type.p != int32_type || !shape.p || !strides.p || !PyTuple_Check(shape) || !read_ints(shape, n, rank) ||
+      !read_ints(strides, stride, rank) || rank > 2 || (rank == 1 && axes != 1) || n[rank - 1] != rows || stride[rank - 1] != 1 ||
+      (rank == 2 && n[0] != axes) || !on_device(tensor, device) || !read_ptr(tensor, at))
+    return false;
+  const int64_t pitch = axes > 1 ? stride[0] : rows;
+  if (pitch > INT32_MAX || pitch < INT32_MIN) return false;
+  p.ptr = (const int32_t*)at, p.pitch = (int32_t)pitch;
+  return true;
+}
+
+// A HeadNorm of d values, or None
+bool read_norm(PyObject* o, int64_t device, int64_t d, adr_head_norm& n) {
+  n = {nullptr, 0.0f};
+  if (o == Py_None) return true;
+  const Ref weight(attr(o, s_weight)), eps(attr(o, s_eps));
+  int64_t size[MAX_RANK];
+  void* p;
+  double e;
+  if (!read_index(weight, 1, device, size, p) || size[0] != d || !read_double(eps, e)) return false;
+  n = {(const uint16_t*)p, (float)e};
+  return true;
+}
+
+bool read_cache_u8(PyObject* o, int64_t device, adr_paged_cache_u8& c) {
+  const Ref views[4] = {Ref(attr(o, s_key)), Ref(attr(o, s_key_scale)), Ref(attr(o, s_value)), Ref(attr(o, s_value_scale))};
+  Layout l[4];
+  void* p[4];
+  for (int i = 0; i < 4; i++) {
+    if (!views[i].p || (PyObject*)Py_TYPE(views[i].p) != view_type || !read_layout(views[i], l[i]) || l[i].rank != (i & 1 ? 3 : 4) ||
+        !read_ptr(views[i], p[i]))
+      return false;
+    const Ref storage(attr(views[i], s_storage));
+    if (!storage.p || !on_device(storage, device)) return false;
+    for (int j = 0; j < l[i].rank; j++)
+      if (l[i].dims[j] != l[0].dims[j] || l[i].dims[j] > INT32_MAX) return false;
+  }
+  const int64_t(&k)[MAX_RANK] = l[0].strides, (&ks)[MAX_RANK] = l[1].strides, (&v)[MAX_RANK] = l[2].strides, (&vs)[MAX_RANK] = l[3].strides;
+  c = {(uint8_t*)p[0], (uint16_t*)p[1], (uint8_t*)p[2], (uint16_t*)p[3], (int32_t)l[0].dims[0], (int32_t)l[0].dims[1],
+       (int32_t)l[0].dims[2], (int32_t)l[0].dims[3], k[3], k[2], k[1], k[0], v[3], v[2], v[1], v[0], ks[2], ks[1], ks[0], vs[2], vs[1], vs[0]};
+  return true;
+}
+
+// norm_rotary_f16(output, input, positions, rotary, norm); the last three may be None
+PyObject* norm_rotary_f16(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t device;
+  adr_stream_t stream;
+  Rows o, x;
+  adr_rotary_axes r;
+  adr_head_norm norm;
+  Positions p;
+  if (n != 5 || !norm_rotary_fn || !read_device(device, stream) || !read_rows(a[0], device, o) || !read_rows(a[1], device, x) ||
+      !read_axes(a[3], device, r) || !read_axis_positions(a[2], device, r.axes, x.rows, p) || !read_norm(a[4], device, x.d, norm) ||
+      o.heads != x.heads || o.rows != x.rows || o.d != x.d)
+    return general();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = norm_rotary_fn(stream, (uint16_t*)o.ptr, (const uint16_t*)x.ptr, p.ptr, p.pitch, r, norm, x.heads, x.rows, x.d, o.x, o.y, o.z,
+                      x.x, x.y, x.z);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// (cache, batch, key, value, rotary, query_out, query, positions, query_norm, key_norm); the last six may be None
+template <typename Cache, typename Fn>
+PyObject* append_normed(PyObject* const* a, Py_ssize_t n, bool (*read)(PyObject*, int64_t, Cache&), Fn fn) {
+  int64_t device;
+  adr_stream_t stream;
+  Cache c;
+  adr_paged_batch b;
+  adr_rotary_axes r;
+  adr_head_norm norms[2];
+  Rows k, v, o = {}, q = {};
+  Positions p;
+  if (n != 10 || !fn || !read_device(device, stream) || !read(a[0], device, c) || !read_paged_batch(a[1], device, b) ||
+      !read_rows(a[2], device, k) || !read_rows(a[3], device, v) || k.heads != v.heads || k.rows != v.rows || k.d != v.d ||
+      k.heads != c.kv_heads || k.d != c.d || (a[5] == Py_None) != (a[6] == Py_None) || !read_axes(a[4], device, r) ||
+      !read_axis_positions(a[7], device, r.axes, k.rows, p) || !read_norm(a[8], device, c.d, norms[0]) ||
+      !read_norm(a[9], device, c.d, norms[1]))
+    return general();
+  if (a[6] != Py_None && (!read_rows(a[5], device, o) || !read_rows(a[6], device, q) || o.heads != q.heads || o.rows != q.rows ||
+                          o.d != q.d || q.rows != k.rows || q.d != k.d))
+    return general();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = fn(stream, c, b, (const uint16_t*)k.ptr, (const uint16_t*)v.ptr, (uint16_t*)o.ptr, (const uint16_t*)q.ptr, p.ptr, p.pitch, r,
+          norms[0], norms[1], q.heads, k.rows, k.x, k.y, k.z, v.x, v.y, v.z, o.x, o.y, o.z, q.x, q.y, q.z);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+PyObject* append_norm_f16(PyObject*, PyObject* const* a, Py_ssize_t n) { return append_normed(a, n, read_cache, append_norm_fn); }
+PyObject* append_u8(PyObject*, PyObject* const* a, Py_ssize_t n) { return append_normed(a, n, read_cache_u8, append_u8_fn); }
+
+// read_u8(key_out, value_out, cache, batch)
+PyObject* read_u8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t device;
+  adr_stream_t stream;
+  adr_paged_cache_u8 c;
+  adr_paged_batch b;
+  Rows k, v;
+  if (n != 4 || !read_u8_fn || !read_device(device, stream) || !read_rows(a[0], device, k) || !read_rows(a[1], device, v) ||
+      !read_cache_u8(a[2], device, c) || !read_paged_batch(a[3], device, b) || k.heads != v.heads || k.rows != v.rows || k.d != v.d ||
+      k.heads != c.kv_heads || k.d != c.d)
+    return general();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = read_u8_fn(stream, (uint16_t*)k.ptr, (uint16_t*)v.ptr, c, b, k.rows, k.x, k.y, k.z, v.x, v.y, v.z);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// attention_paged_u8(output, query, cache, batch, scale, temperature, mask)
+PyObject* attention_paged_u8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  int64_t device, mask;
+  adr_stream_t stream;
+  adr_paged_cache_u8 c;
+  adr_paged_batch b;
+  Rows o, q;
+  double scale, temp;
+  if (n != 7 || !paged_u8_fn || !read_device(device, stream) || !read_rows(a[0], device, o) || !read_rows(a[1], device, q) ||
+      !read_cache_u8(a[2], device, c) || !read_paged_batch(a[3], device, b) || !read_double(a[4], scale) || !read_double(a[5], temp) ||
+      !as_int(a[6], mask) || mask < 0 || mask > UINT32_MAX || o.heads != q.heads || o.rows != q.rows || o.d != q.d || q.d != c.d)
+    return general();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = paged_u8_fn(stream, (uint16_t*)o.ptr, (const uint16_t*)q.ptr, c, b, q.heads, q.rows, o.x, o.y, o.z, q.x, q.y, q.z, (float)scale,
+                   (float)temp, (uint32_t)mask);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// (output, query, cache, batch, tree, scale, temperature)
+template <typename Cache, typename Fn>
+PyObject* attention_tree(PyObject* const* a, Py_ssize_t n, bool (*read)(PyObject*, int64_t, Cache&), Fn fn) {
+  int64_t device, size[MAX_RANK], stride[MAX_RANK];
+  adr_stream_t stream;
+  Cache c;
+  adr_paged_batch b;
+  Rows o, q;
+  double scale, temp;
+  void* p;
+  if (n != 7 || !fn || !read_device(device, stream) || !read_rows(a[0], device, o) || !read_rows(a[1], device, q) ||
+      !read(a[2], device, c) || !read_paged_batch(a[3], device, b) || !read_double(a[5], scale) || !read_double(a[6], temp) ||
+      o.heads != q.heads || o.rows != q.rows || o.d != q.d || q.d != c.d)
+    return general();
+  const Ref bits(attr(a[4], s_bits));
+  if (!read_index(bits, 2, device, size, p) || size[0] != q.rows || size[1] > INT32_MAX) return general();
+  const Ref strides(call(bits, s_stride));
+  int rank = 2;
+  if (!strides.p || !read_ints(strides, stride, rank) || stride[1] != 1 || stride[0] > INT32_MAX || stride[0] < size[1]) return general();
+  const adr_draft_tree tree = {(const int32_t*)p, (int32_t)size[1], (int32_t)stride[0]};
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = fn(stream, (uint16_t*)o.ptr, (const uint16_t*)q.ptr, c, b, tree, q.heads, q.rows, o.x, o.y, o.z, q.x, q.y, q.z, (float)scale,
+          (float)temp);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+PyObject* attention_tree_f16(PyObject*, PyObject* const* a, Py_ssize_t n) { return attention_tree(a, n, read_cache, tree_f16_fn); }
+PyObject* attention_tree_u8(PyObject*, PyObject* const* a, Py_ssize_t n) { return attention_tree(a, n, read_cache_u8, tree_u8_fn); }
+
 #define ADR_METHOD(f) (PyCFunction)(void (*)(void))f, METH_FASTCALL | METH_KEYWORDS
 PyMethodDef of_def = {"of", ADR_METHOD(view_of), "View of a torch tensor with its own sizes and strides."};
 PyMethodDef permute_def = {"permute", ADR_METHOD(view_permute), nullptr};
@@ -704,6 +902,23 @@ PyObject* bind_sequences(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
+// bind_step(addresses of the functions above, kernels.RotaryAxes): beside bind_sequences
+PyObject* bind_step(PyObject*, PyObject* args) {
+  unsigned long long p[7];
+  PyObject* type;
+  if (!PyArg_ParseTuple(args, "KKKKKKKO", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, &type)) return nullptr;
+  Py_INCREF(type);
+  Py_XSETREF(axes_type, type);
+  norm_rotary_fn = (decltype(norm_rotary_fn))p[0];
+  append_norm_fn = (decltype(append_norm_fn))p[1];
+  append_u8_fn = (decltype(append_u8_fn))p[2];
+  read_u8_fn = (decltype(read_u8_fn))p[3];
+  paged_u8_fn = (decltype(paged_u8_fn))p[4];
+  tree_f16_fn = (decltype(tree_f16_fn))p[5];
+  tree_u8_fn = (decltype(tree_u8_fn))p[6];
+  Py_RETURN_NONE;
+}
+
 #define ADR_FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"install", install, METH_VARARGS, nullptr},
                          {"bind", bind, METH_VARARGS, nullptr},
@@ -719,6 +934,14 @@ PyMethodDef methods[] = {{"install", install, METH_VARARGS, nullptr},
                          ADR_FAST(append_f16),
                          ADR_FAST(attention_paged_f16),
                          ADR_FAST(attention_packed_f16),
+                         {"bind_step", bind_step, METH_VARARGS, nullptr},
+                         ADR_FAST(norm_rotary_f16),
+                         ADR_FAST(append_norm_f16),
+                         ADR_FAST(append_u8),
+                         ADR_FAST(read_u8),
+                         ADR_FAST(attention_paged_u8),
+                         ADR_FAST(attention_tree_f16),
+                         ADR_FAST(attention_tree_u8),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
@@ -732,7 +955,8 @@ PyMODINIT_FUNC PyInit__native() {
       {&s_is_contiguous, "is_contiguous"}, {&s_get_device, "get_device"}, {&s_key, "key"}, {&s_value, "value"},
       {&s_row_offsets, "row_offsets"}, {&s_lengths, "lengths"}, {&s_table, "table"}, {&s_key_offsets, "key_offsets"},
       {&s_longest_rows, "longest_rows"}, {&s_longest, "longest"}, {&s_turns, "turns"}, {&s_rotary_layout, "layout"},
-      {&s_magnitude, "magnitude"}, {&s_dtype, "dtype"}};
+      {&s_magnitude, "magnitude"}, {&s_dtype, "dtype"}, {&s_axis, "axis"}, {&s_axes, "axes"}, {&s_weight, "weight"},
+      {&s_eps, "eps"}, {&s_key_scale, "key_scale"}, {&s_value_scale, "value_scale"}, {&s_bits, "bits"}};
   for (const auto& n : names)
     if (!(*n.at = PyUnicode_InternFromString(n.name))) return nullptr;
   return PyModule_Create(&module);

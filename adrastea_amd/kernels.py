@@ -588,9 +588,20 @@ def _native_sequence_binding() -> tuple:
     return (*(C.cast(getattr(lib, name), C.c_void_p).value for name in _NATIVE_SEQUENCE_CALLS), torch.int32)
 
 
+_NATIVE_STEP_CALLS = ("adr_norm_rotary_f16", "adr_append_norm_f16", "adr_append_u8", "adr_read_u8", "adr_attention_paged_u8",
+                      "adr_attention_tree_f16", "adr_attention_tree_u8")
+
+
+@functools.lru_cache(maxsize=None)
+def _native_step_binding() -> tuple:
+    lib = _ffi.lib()
+    return (*(C.cast(getattr(lib, name), C.c_void_p).value for name in _NATIVE_STEP_CALLS), RotaryAxes)
+
+
 def _bind_native() -> None:
     _native.bind(*_native_binding())
     _native.bind_sequences(*_native_sequence_binding())
+    _native.bind_step(*_native_step_binding())
 
 
 class GpuKernels(CommonKernels):
@@ -784,6 +795,8 @@ class GpuKernels(CommonKernels):
     def norm_rotary_f16(self, output, input, positions=None, rotary=None, norm: Optional[HeadNorm] = None):
         """The heads of `input`, a [heads, rows, d] view, normed and then turned into `output` (which may be the same view).
         rotary: a RotaryAxes, a Rotary or None; positions: int32 [axes, rows] (or [rows])."""
+        if self._lowered("norm_rotary_f16", output, input, positions, rotary, norm):
+            return
         dims, si = _rows_view(input, "input")
         dims_out, so = _rows_view(output, "output")
         assert dims_out == dims, "output and input have one shape"
@@ -818,6 +831,8 @@ class GpuKernels(CommonKernels):
                         positions=None, query_norm: Optional[HeadNorm] = None, key_norm: Optional[HeadNorm] = None):
         """append_f16 of heads that are normed before they are turned, by positions on several axes (int32 [axes, rows]) where
         rotary is a RotaryAxes."""
+        if self._lowered("append_norm_f16", cache, batch, key, value, rotary, query_out, query, positions, query_norm, key_norm):
+            return
         self._append(self._lib.adr_append_norm_f16, "append_norm_f16", cache, batch, key, value, rotary, query_out, query,
                      positions, query_norm, key_norm)
 
@@ -825,12 +840,16 @@ class GpuKernels(CommonKernels):
                   positions=None, query_norm: Optional[HeadNorm] = None, key_norm: Optional[HeadNorm] = None):
         """append_norm_f16 into a cache in 8 bits: keys as normed and turned, and values, each with a scale of its own for each
         head, within half a scale of what they were."""
+        if self._lowered("append_u8", cache, batch, key, value, rotary, query_out, query, positions, query_norm, key_norm):
+            return
         self._append(self._lib.adr_append_u8, "append_u8", cache, batch, key, value, rotary, query_out, query, positions,
                      query_norm, key_norm)
 
     def read_u8(self, key_out, value_out, cache: PagedCacheU8, batch: PagedBatch):
         """What the codes of the batch's rows stand for, into [kv_heads, rows, d] views: row j of the r of sequence s is key
         lengths[s] - r + j.  (As many rows as keys: all of them.)"""
+        if self._lowered("read_u8", key_out, value_out, cache, batch):
+            return
         c, b = cache._desc, batch._desc
         dims, sk = _rows_view(key_out, "key_out")
         dims_v, sv = _rows_view(value_out, "value_out")
@@ -855,17 +874,23 @@ class GpuKernels(CommonKernels):
     def attention_paged_u8(self, output, query, cache: PagedCacheU8, batch: PagedBatch, scale: float, temperature: float = 1.0,
                            mask: int = MatmulMask.CAUSAL):
         """attention_paged_f16 over a cache in 8 bits."""
+        if self._workspace is None and self._lowered("attention_paged_u8", output, query, cache, batch, scale, temperature, mask):
+            return
         self._attention_paged("attention_paged_u8", output, query, cache, batch, (), (float(scale), float(temperature), int(mask)))
 
     def attention_tree_f16(self, output, query, cache: PagedCache, batch: PagedBatch, tree: DraftTree, scale: float,
                            temperature: float = 1.0):
         """Attention of drafted tokens, which are the last keys of their sequences: each row sees all keys in front of the
         draft, and of the draft what its bits say."""
+        if self._workspace is None and self._lowered("attention_tree_f16", output, query, cache, batch, tree, scale, temperature):
+            return
         self._attention_paged("attention_tree_f16", output, query, cache, batch, (tree._desc_of,), (float(scale), float(temperature)))
 
     def attention_tree_u8(self, output, query, cache: PagedCacheU8, batch: PagedBatch, tree: DraftTree, scale: float,
                           temperature: float = 1.0):
         """attention_tree_f16 over a cache in 8 bits."""
+        if self._workspace is None and self._lowered("attention_tree_u8", output, query, cache, batch, tree, scale, temperature):
+            return
         self._attention_paged("attention_tree_u8", output, query, cache, batch, (tree._desc_of,), (float(scale), float(temperature)))
 
     def _error_stats(self, fn, what, output, lhs, rhs):
