@@ -337,7 +337,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
     for (int r = w; r < rows; r += WAVES)
       if (again >> r & 1) {
         const int lr = block * ROWS + r;
-        row_by_wave(arguments(), q, lr / z.group, hk * z.group + lr % z.group, lane);
+        row_by_wave<TREE>(arguments(), q, lr / z.group, hk * z.group + lr % z.group, lane);
       }
   }
   if (!SHARED || next_place >= stretch1) break;

@@ -46,7 +46,7 @@ template <int HD, bool PAGED, bool SHARED, int GROUPS, bool TREE = false, bool U
 __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
   static_assert(PAGED || !U8, "codes are in pages");
   constexpr int BYTES = U8 ? 1 : 2;    // of a value of the tiles
-  constexpr int CPR = HD * BYTES / 16, KEYS = 64, ROWS = 128;
+  constexpr int CHUNK = 16 / BYTES, CPR = HD / CHUNK, KEYS = 64, ROWS = 128;
   constexpr int TILE = KEYS * HD * BYTES;  // bytes of one K or V tile
   constexpr int NI = TILE / 1024 / 4;  // transfers per wavefront and tile: 16 rows
   constexpr int DS = HD / 16;          // MFMA k-steps over the head dimension
@@ -142,10 +142,10 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     int krow, kc;
     k_chunk_inv<CPR>(j * 64 + lane, krow, kc);
     const int vrow = (j * 64 + lane) / CPR, vc = (lane % CPR) ^ value_swizzle(vrow);
-    const uint32_t ko = (uint32_t)(krow * k_stride * BYTES + kc * 16 + BIAS - j * 1024);
-    const uint32_t vo = (uint32_t)(vrow * v_stride * BYTES + vc * 16 + BIAS - j * 1024);
-    koff[j] = kc * 16 < d * BYTES ? ko : 0x7fff0000u;
-    voff[j] = vc * 16 < d * BYTES ? vo : 0x7fff0000u;
+    const uint32_t ko = (uint32_t)((krow * k_stride + kc * CHUNK) * BYTES + BIAS - j * 1024);
+    const uint32_t vo = (uint32_t)((vrow * v_stride + vc * CHUNK) * BYTES + BIAS - j * 1024);
+    koff[j] = kc * CHUNK < d ? ko : 0x7fff0000u;
+    voff[j] = vc * CHUNK < d ? vo : 0x7fff0000u;
   }
   // The wavefront's next 16 key and value rows: address, and bytes from there to the last key (0 behind it).  On
   // pages, the addresses of 64 tiles at a time, a lane to each, worked out by the vector ALU.  (Addresses are even: an
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
   // U8.  Scales of tile t of the group (a lane has a key), in three steps.  Transfers are made in any case, so that the waits count
   // right: of what is not there, some other word.
   uint32_t upper = 0;  // bits: the scale is in its word's upper half
-  const float factor = U8 ? a.c / WIDENED : a.c;  // of the scores (of codes: they are times 2^-24)
+  const float factor = U8 ? a.c / WIDENED : 0.0f;  // of the scores, which are times 2^-24
   auto key_of = [&](int t) __attribute__((always_inline)) { return (tile0 + t) * KEYS + lane; };
   auto page_word = [&](int t) __attribute__((always_inline)) {
     const int key = key_of(t);
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
     read_scales(1);
     auto stage_exponent = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 0; e < VP; e++) ex[e] = fmaf(cur[k * VP >> 4][(k * VP & 15) + e], U8 ? ks[k * VP >> 2 & 1][(k * VP & 3) + e] : factor, -m_run);
+      for (int e = 0; e < VP; e++) ex[e] = fmaf(cur[k * VP >> 4][(k * VP & 15) + e], U8 ? ks[k * VP >> 2 & 1][(k * VP & 3) + e] : a.c, -m_run);
     };
     auto stage_power = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -752,14 +752,14 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
       uint32_t again = (uint32_t)far | (uint32_t)(far >> 32);
       const uint32_t bad = (uint32_t)wrong | (uint32_t)(wrong >> 32);
       if (!U8 && bad && (TREE || (q.rows > 1 && z.mask == ADR_MASK_CAUSAL)) &&
-          hidden_reaches(z, q, hk, end_of_common(z, q, row_of_list(z, list0 + min(__builtin_ctz(bad), wave_rows - 1))),
+          hidden_reaches(z, q, hk, TREE ? end_of_common(z, q, 0) : end_of_row(z, q, row_of_list(z, list0 + min(__builtin_ctz(bad), wave_rows - 1))),
                          end_of_row(z, q, row_of_list(z, block * ROWS + rows - 1)), lane))
         again |= bad;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (behind the stores above)
       for (int r = 0; r < wave_rows; r++)
         if (again >> r & 1) {
-          if constexpr (U8) row_by_wave_u8(arguments(), q, (list0 + r) / z.group, hk * z.group + (list0 + r) % z.group, lane, col0, col0 + 32 * MINE);
-          else row_by_wave(arguments(), q, (list0 + r) / z.group, hk * z.group + (list0 + r) % z.group, lane, col0, col0 + 32 * MINE);
+          if constexpr (U8) row_by_wave_u8<TREE>(arguments(), q, (list0 + r) / z.group, hk * z.group + (list0 + r) % z.group, lane, col0, col0 + 32 * MINE);
+          else row_by_wave<TREE>(arguments(), q, (list0 + r) / z.group, hk * z.group + (list0 + r) % z.group, lane, col0, col0 + 32 * MINE);
         }
     }
   } else if (frow < wave_rows) {

@@ -434,7 +434,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
     for (int r = w; r < rows; r += WAVES)
       if (again >> r & 1) {
         const int lr = block * ROWS + r;
-        row_by_wave_u8(arguments(), q, lr / z.group, hk * z.group + lr % z.group, lane);
+        row_by_wave_u8<TREE>(arguments(), q, lr / z.group, hk * z.group + lr % z.group, lane);
       }
   }
   if (!SHARED || next_place >= stretch1) break;

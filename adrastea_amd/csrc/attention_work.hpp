@@ -168,8 +168,10 @@ __device__ __forceinline__ uint32_t tree_window(Args a, int64_t row, int rel) {
 
 // One row of one query head by one wavefront, at any strides: 64 keys at a time, a lane to a key for the scores
 // and a lane to every 64th column for the sums.  Only keys that the row sees are read.  Probabilities stay in 32 bits, and
-// scores unscaled until their maximum is subtracted: right for scores of any size.  (Columns col0 ... col1 - 1 are stored.)
+// scores unscaled until their maximum is subtracted: right for scores of any size.  (Columns col0 ... col1 - 1 are stored.  Without
+// TREE rows that see what is in front of them need fewer scalar registers of the kernels that end with this.)
 constexpr int GENERAL_MAX_D = 256;
+template <bool TREE = true>
 __device__ __forceinline__ void row_by_wave(Args a, const Sequence& q, int j, int h, int lane, int col0 = 0, int col1 = GENERAL_MAX_D) {
   const int64_t row = (int64_t)q.row0 + j;
   const half_t* const Q = a.q + h * (int64_t)a.sq_z + row * a.sq_y;
@@ -182,7 +184,7 @@ __device__ __forceinline__ void row_by_wave(Args a, const Sequence& q, int j, in
     float s = -INFINITY;
     int64_t ko = 0, vo = 0;
     bool good = true;
-    const bool seen = x < end && (a.mask != MASK_TREE || (tree_window(a, row, x - (q.keys - q.rows)) & 1));
+    const bool seen = x < end && (!TREE || a.mask != MASK_TREE || (tree_window(a, row, x - (q.keys - q.rows)) & 1));
     if (seen) {
       good = key_at(a, q, x, ko, vo);
       s = 0.0f;
@@ -198,18 +200,23 @@ __device__ __forceinline__ void row_by_wave(Args a, const Sequence& q, int j, in
     l = l * alpha + p;
 #pragma unroll
     for (int c = 0; c < GENERAL_MAX_D / 64; c++) o[c] *= alpha;
-    for (uint64_t left = __ballot(seen); left != 0; left &= left - 1) {
-      const int e = __builtin_ctzll(left);
+    auto add = [&](int e) __attribute__((always_inline)) {
       const float pe = __shfl(p, e);
       const int64_t at = __shfl(vo, e);
       if (!__shfl((int)good, e)) {
 #pragma unroll
         for (int c = 0; c < GENERAL_MAX_D / 64; c++) o[c] = NAN;
-        continue;
+        return;
       }
 #pragma unroll
       for (int c = 0; c < GENERAL_MAX_D / 64; c++)
         if (c * 64 + lane < a.d) o[c] = fmaf(pe, (float)V[at + (c * 64 + lane) * a.sv.x], o[c]);
+    };
+    if constexpr (TREE) {
+      for (uint64_t left = __ballot(seen); left != 0; left &= left - 1) add(__builtin_ctzll(left));
+    } else {
+      const int n = min(64, end - x0);
+      for (int e = 0; e < n; e++) add(e);
     }
   }
   for (int i = 32; i > 0; i >>= 1) l += __shfl_xor(l, i);
@@ -224,6 +231,7 @@ __device__ __forceinline__ void row_by_wave(Args a, const Sequence& q, int j, in
 // The same over codes.  A key counts as NaN where a scale of it is larger than those of the format, or no number.
 __device__ __forceinline__ bool scale_fits(half_t s) { return fabsf((float)s) <= 513.5f; }
 
+template <bool TREE = true>
 __device__ __forceinline__ void row_by_wave_u8(Args a, const Sequence& q, int j, int h, int lane, int col0 = 0, int col1 = GENERAL_MAX_D) {
   const int64_t row = (int64_t)q.row0 + j;
   const int hk = h / a.group;
@@ -236,7 +244,7 @@ __device__ __forceinline__ void row_by_wave_u8(Args a, const Sequence& q, int j,
     const int x = x0 + lane;
     float s = -INFINITY, value_scale = 0.0f;
     int64_t vo = 0;
-    const bool seen = x < end && (a.mask != MASK_TREE || (tree_window(a, row, x - (q.keys - q.rows)) & 1));
+    const bool seen = x < end && (!TREE || a.mask != MASK_TREE || (tree_window(a, row, x - (q.keys - q.rows)) & 1));
     bool good = false;
     if (seen) {
       const int at = x / a.page_size, slot = x - at * a.page_size;
@@ -268,8 +276,9 @@ __device__ __forceinline__ void row_by_wave_u8(Args a, const Sequence& q, int j,
     l = l * alpha + p;
 #pragma unroll
     for (int c = 0; c < GENERAL_MAX_D / 64; c++) o[c] *= alpha;
-    for (uint64_t left = __ballot(good); left != 0; left &= left - 1) {
-      const int e = __builtin_ctzll(left);
+    const int n = min(64, end - x0);
+    for (int e = 0; e < n; e++) {
+      if (!__shfl((int)good, e)) continue;
       const float pe = __shfl(p * value_scale, e);
       const int64_t at = __shfl(vo, e);
 #pragma unroll
