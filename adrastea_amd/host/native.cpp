@@ -25,7 +25,9 @@ PyObject *s_shape, *s_stride, *s_dims, *s_strides, *s_storage, *s_layout, *s_off
     *s_mask, *s_op, *s_scale, *s_beta, *s_bias, *s_is_contiguous, *s_get_device, *s_key, *s_value, *s_row_offsets, *s_lengths,
     *s_table, *s_key_offsets, *s_longest_rows, *s_longest, *s_turns, *s_rotary_layout, *s_magnitude, *s_dtype, *s_axis, *s_axes,
     *s_weight, *s_eps, *s_key_scale, *s_value_scale, *s_bits;
-PyObject* axes_type;  // RotaryAxes
+// RotaryAxes, HeadNorm, PagedCacheU8 and DraftTree.  Objects of others may have attributes of the same names that mean something else.
+PyObject *axes_type, *norm_type, *codes_type, *tree_type;
+bool is_a(PyObject* o, PyObject* type) { return type && PyType_IsSubtype(Py_TYPE(o), (PyTypeObject*)type); }
 
 decltype(&adr_matmul_f16) matmul_fn;
 decltype(&adr_attention_f16) attention_fn;
@@ -507,6 +509,7 @@ bool read_int32(PyObject* o, PyObject* name, int32_t& v) {
 }
 
 bool read_cache(PyObject* o, int64_t device, adr_paged_cache& c) {
+  if (is_a(o, codes_type)) return false;
   Layout l[2];
   const Ref views[2] = {Ref(attr(o, s_key)), Ref(attr(o, s_value))};
   void* p[2];
@@ -539,7 +542,7 @@ bool read_paged_batch(PyObject* o, int64_t device, adr_paged_batch& b) {
   return read_int32(o, s_longest_rows, b.longest_rows) && read_int32(o, s_longest, b.longest);
 }
 
-bool read_rotary(PyObject* o, int64_t device, adr_rotary& r) {
+bool read_turns(PyObject* o, int64_t device, adr_rotary& r) {
   const Ref turns(attr(o, s_turns)), magnitude(attr(o, s_magnitude));
   int64_t n[MAX_RANK];
   void* p;
@@ -551,6 +554,8 @@ bool read_rotary(PyObject* o, int64_t device, adr_rotary& r) {
   r = {(const double*)p, (int32_t)n[0] * 2, (uint32_t)layout, (float)m};
   return true;
 }
+
+bool read_rotary(PyObject* o, int64_t device, adr_rotary& r) { return !is_a(o, axes_type) && read_turns(o, device, r); }
 
 // rotary_f16(output, input, positions, rotary)
 PyObject* rotary_f16(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -652,9 +657,9 @@ bool read_axes(PyObject* o, int64_t device, adr_rotary_axes& r) {
   r = {nullptr, nullptr, 0, 0, 1.0f, 1};
   if (o == Py_None) return true;
   adr_rotary one;
-  if (!read_rotary(o, device, one)) return false;
+  if (!read_turns(o, device, one)) return false;
   r.turns = one.turns, r.dims = one.dims, r.layout = one.layout, r.magnitude = one.magnitude;
-  if ((PyObject*)Py_TYPE(o) != axes_type) return true;
+  if (!is_a(o, axes_type)) return true;
   const Ref axis(attr(o, s_axis));
   int64_t n[MAX_RANK];
   void* p;
@@ -688,6 +693,7 @@ bool read_axis_positions(PyObject* tensor, int64_t device, int64_t axes, int64_t
 bool read_norm(PyObject* o, int64_t device, int64_t d, adr_head_norm& n) {
   n = {nullptr, 0.0f};
   if (o == Py_None) return true;
+  if (!is_a(o, norm_type)) return false;
   const Ref weight(attr(o, s_weight)), eps(attr(o, s_eps));
   int64_t size[MAX_RANK];
   void* p;
@@ -698,6 +704,7 @@ bool read_norm(PyObject* o, int64_t device, int64_t d, adr_head_norm& n) {
 }
 
 bool read_cache_u8(PyObject* o, int64_t device, adr_paged_cache_u8& c) {
+  if (!is_a(o, codes_type)) return false;
   const Ref views[4] = {Ref(attr(o, s_key)), Ref(attr(o, s_key_scale)), Ref(attr(o, s_value)), Ref(attr(o, s_value_scale))};
   Layout l[4];
   void* p[4];
@@ -814,7 +821,7 @@ PyObject* attention_tree(PyObject* const* a, Py_ssize_t n, bool (*read)(PyObject
   Rows o, q;
   double scale, temp;
   void* p;
-  if (n != 7 || !fn || !read_device(device, stream) || !read_rows(a[0], device, o) || !read_rows(a[1], device, q) ||
+  if (n != 7 || !fn || !is_a(a[4], tree_type) || !read_device(device, stream) || !read_rows(a[0], device, o) || !read_rows(a[1], device, q) ||
       !read(a[2], device, c) || !read_paged_batch(a[3], device, b) || !read_double(a[5], scale) || !read_double(a[6], temp) ||
       o.heads != q.heads || o.rows != q.rows || o.d != q.d || q.d != c.d)
     return general();
@@ -902,13 +909,18 @@ PyObject* bind_sequences(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
-// bind_step(addresses of the functions above, kernels.RotaryAxes): beside bind_sequences
+// bind_step(addresses of the functions above, RotaryAxes, HeadNorm, PagedCacheU8, DraftTree): beside bind_sequences
 PyObject* bind_step(PyObject*, PyObject* args) {
   unsigned long long p[7];
-  PyObject* type;
-  if (!PyArg_ParseTuple(args, "KKKKKKKO", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, &type)) return nullptr;
-  Py_INCREF(type);
-  Py_XSETREF(axes_type, type);
+  PyObject* types[4];
+  if (!PyArg_ParseTuple(args, "KKKKKKKO!O!O!O!", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, &PyType_Type, types, &PyType_Type, types + 1,
+                        &PyType_Type, types + 2, &PyType_Type, types + 3))
+    return nullptr;
+  PyObject** const kept[4] = {&axes_type, &norm_type, &codes_type, &tree_type};
+  for (int i = 0; i < 4; i++) {
+    Py_INCREF(types[i]);
+    Py_XSETREF(*kept[i], types[i]);
+  }
   norm_rotary_fn = (decltype(norm_rotary_fn))p[0];
   append_norm_fn = (decltype(append_norm_fn))p[1];
   append_u8_fn = (decltype(append_u8_fn))p[2];

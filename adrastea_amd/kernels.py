@@ -336,6 +336,7 @@ _NO_NORM = _ffi.HeadNormDesc(None, 0.0)
 def _norm_desc(norm: Optional[HeadNorm], d: int) -> _ffi.HeadNormDesc:
     if norm is None:
         return _NO_NORM
+    assert isinstance(norm, HeadNorm), "a norm is a HeadNorm"
     _here(norm.weight)
     assert norm.weight.shape[0] == d, "a norm's weight has an entry for each value of a head"
     return _ffi.HeadNormDesc(norm.weight.data_ptr(), norm.eps)
@@ -474,7 +475,7 @@ def _hint(v: int) -> int:
 
 def _index(t, rank, what):
     import torch
-    assert t.dtype == torch.int32 and t.dim() == rank and (t.numel() == 0 or t.stride(-1) == 1), \
+    assert t.dtype == torch.int32 and t.dim() == rank and (t.numel() == 0 or t.stride(-1) == 1 or t.shape[-1] == 1), \
         f"{what}: an int32 tensor of rank {rank}, contiguous in its last dimension"
     return t
 
@@ -595,7 +596,7 @@ _NATIVE_STEP_CALLS = ("adr_norm_rotary_f16", "adr_append_norm_f16", "adr_append_
 @functools.lru_cache(maxsize=None)
 def _native_step_binding() -> tuple:
     lib = _ffi.lib()
-    return (*(C.cast(getattr(lib, name), C.c_void_p).value for name in _NATIVE_STEP_CALLS), RotaryAxes)
+    return (*(C.cast(getattr(lib, name), C.c_void_p).value for name in _NATIVE_STEP_CALLS), RotaryAxes, HeadNorm, PagedCacheU8, DraftTree)
 
 
 def _bind_native() -> None:
@@ -807,7 +808,8 @@ class GpuKernels(CommonKernels):
         if rc != 0:
             raise AdrasteaError(rc, "norm_rotary_f16")
 
-    def _append(self, fn, what, cache, batch, key, value, rotary, query_out, query, positions, query_norm, key_norm):
+    def _append(self, fn, what, kind, cache, batch, key, value, rotary, query_out, query, positions, query_norm, key_norm):
+        assert isinstance(cache, kind), f"the cache is a {kind.__name__}"
         c, b = cache._desc, batch._desc
         dims, sk = _rows_view(key, "key")
         dims_v, sv = _rows_view(value, "value")
@@ -833,7 +835,7 @@ class GpuKernels(CommonKernels):
         rotary is a RotaryAxes."""
         if self._lowered("append_norm_f16", cache, batch, key, value, rotary, query_out, query, positions, query_norm, key_norm):
             return
-        self._append(self._lib.adr_append_norm_f16, "append_norm_f16", cache, batch, key, value, rotary, query_out, query,
+        self._append(self._lib.adr_append_norm_f16, "append_norm_f16", PagedCache, cache, batch, key, value, rotary, query_out, query,
                      positions, query_norm, key_norm)
 
     def append_u8(self, cache: PagedCacheU8, batch: PagedBatch, key, value, rotary=None, query_out=None, query=None,
@@ -842,7 +844,7 @@ class GpuKernels(CommonKernels):
         head, within half a scale of what they were."""
         if self._lowered("append_u8", cache, batch, key, value, rotary, query_out, query, positions, query_norm, key_norm):
             return
-        self._append(self._lib.adr_append_u8, "append_u8", cache, batch, key, value, rotary, query_out, query, positions,
+        self._append(self._lib.adr_append_u8, "append_u8", PagedCacheU8, cache, batch, key, value, rotary, query_out, query, positions,
                      query_norm, key_norm)
 
     def read_u8(self, key_out, value_out, cache: PagedCacheU8, batch: PagedBatch):
@@ -850,6 +852,7 @@ class GpuKernels(CommonKernels):
         lengths[s] - r + j.  (As many rows as keys: all of them.)"""
         if self._lowered("read_u8", key_out, value_out, cache, batch):
             return
+        assert isinstance(cache, PagedCacheU8), "the cache is a PagedCacheU8"
         c, b = cache._desc, batch._desc
         dims, sk = _rows_view(key_out, "key_out")
         dims_v, sv = _rows_view(value_out, "value_out")
@@ -858,7 +861,8 @@ class GpuKernels(CommonKernels):
         if rc != 0:
             raise AdrasteaError(rc, "read_u8")
 
-    def _attention_paged(self, what, output, query, cache, batch, before, after):
+    def _attention_paged(self, what, output, query, kind, cache, batch, before, after):
+        assert isinstance(cache, kind), f"the cache is a {kind.__name__}"
         c, b = cache._desc, batch._desc
         dims, sq = _rows_view(query, "query")
         dims_o, so = _rows_view(output, "output")
@@ -876,7 +880,7 @@ class GpuKernels(CommonKernels):
         """attention_paged_f16 over a cache in 8 bits."""
         if self._workspace is None and self._lowered("attention_paged_u8", output, query, cache, batch, scale, temperature, mask):
             return
-        self._attention_paged("attention_paged_u8", output, query, cache, batch, (), (float(scale), float(temperature), int(mask)))
+        self._attention_paged("attention_paged_u8", output, query, PagedCacheU8, cache, batch, (), (float(scale), float(temperature), int(mask)))
 
     def attention_tree_f16(self, output, query, cache: PagedCache, batch: PagedBatch, tree: DraftTree, scale: float,
                            temperature: float = 1.0):
@@ -884,14 +888,14 @@ class GpuKernels(CommonKernels):
         draft, and of the draft what its bits say."""
         if self._workspace is None and self._lowered("attention_tree_f16", output, query, cache, batch, tree, scale, temperature):
             return
-        self._attention_paged("attention_tree_f16", output, query, cache, batch, (tree._desc_of,), (float(scale), float(temperature)))
+        self._attention_paged("attention_tree_f16", output, query, PagedCache, cache, batch, (tree._desc_of,), (float(scale), float(temperature)))
 
     def attention_tree_u8(self, output, query, cache: PagedCacheU8, batch: PagedBatch, tree: DraftTree, scale: float,
                           temperature: float = 1.0):
         """attention_tree_f16 over a cache in 8 bits."""
         if self._workspace is None and self._lowered("attention_tree_u8", output, query, cache, batch, tree, scale, temperature):
             return
-        self._attention_paged("attention_tree_u8", output, query, cache, batch, (tree._desc_of,), (float(scale), float(temperature)))
+        self._attention_paged("attention_tree_u8", output, query, PagedCacheU8, cache, batch, (tree._desc_of,), (float(scale), float(temperature)))
 
     def _error_stats(self, fn, what, output, lhs, rhs):
         if _native is not None:

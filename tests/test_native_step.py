@@ -62,7 +62,7 @@ def both(recorders, monkeypatch):
     """A call through the native path and through the general one: what each passed on (None: refused)."""
     _native.bind(ABI, *[0] * 8, lambda: -1, lambda device: 0x1001 + device)   # (tensors of the host say device -1)
     _native.bind_sequences(*[0] * 4, torch.int32)
-    _native.bind_step(*recorders.addresses, RotaryAxes)
+    _native.bind_step(*recorders.addresses, RotaryAxes, HeadNorm, PagedCacheU8, DraftTree)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
     monkeypatch.setattr(kernels, "_current_stream", lambda: 0x1000)
     k = GpuKernels.__new__(GpuKernels)
@@ -169,3 +169,54 @@ def test_what_one_refuses_the_other_does_not_take(both):
             ("attention_tree_u8", o, rows(8, 8, 64), codes(), batch(), tree, 0.1, 1.0)):
         native, general = both(name, *args)
         assert native is None and general is None, (name, args)
+
+
+def test_objects_of_other_kinds_are_refused(both):
+    """A cache of codes where one of 16 bits is asked for (its codes would be read as halves, twice as far), several axes where one
+    is, and objects that only have attributes of the same names, such as a norm of a model with weights of 32 bits."""
+    k, q, o, tree = rows(2, 9, 64), rows(8, 9, 64), rows(8, 9, 64), DraftTree(torch.zeros(9, 2, dtype=torch.int32))
+
+    class Like:
+        def __init__(self, of, **change):
+            self.__dict__.update({n: getattr(of, n) for n in of.__dataclass_fields__}, **change)
+    wide = torch.nn.RMSNorm(64, eps=1e-5)
+    for name, *args in (
+            ("attention_tree_f16", o, q, codes(), batch(), tree, 0.1, 1.0), ("attention_tree_u8", o, q, cache(), batch(), tree, 0.1, 1.0),
+            ("attention_paged_u8", o, q, cache(), batch(), 0.1, 1.0, 1), ("read_u8", k, k, cache(), batch()),
+            ("append_norm_f16", codes(), batch(), k, k, None, None, None, None, None, None),
+            ("append_u8", cache(), batch(), k, k, None, None, None, None, None, None),
+            ("append_u8", codes(), batch(), k, k, None, None, None, None, None, wide), ("norm_rotary_f16", o, q, None, None, wide),
+            ("norm_rotary_f16", o, q, None, None, Like(norm(), weight=torch.zeros(64))),
+            ("attention_paged_u8", o, q, Like(codes()), batch(), 0.1, 1.0, 1),
+            ("attention_tree_f16", o, q, cache(), batch(), Like(tree, bits=torch.zeros(9, 2, dtype=torch.int64)), 0.1, 1.0)):
+        native, general = both(name, *args)
+        assert native is None and general is None, (name, args)
+
+
+def test_calls_of_one_axis_and_16_bits_refuse_the_new_kinds(recorders, monkeypatch):
+    """rotary_f16, append_f16 and attention_paged_f16 through the native path, bound to where a call would be seen."""
+    at = recorders.addresses[0]
+    _native.bind(ABI, *[0] * 8, lambda: -1, lambda device: 0x1001 + device)
+    _native.bind_sequences(at, at, at, at, torch.int32)
+    _native.bind_step(*recorders.addresses, RotaryAxes, HeadNorm, PagedCacheU8, DraftTree)
+    k, q, o = rows(2, 9, 64), rows(8, 9, 64), rows(8, 9, 64)
+    try:
+        p = torch.zeros(9, dtype=torch.int32)
+        assert _native.rotary_f16(o, q, p, rotary(1)) is None
+        assert _native.append_f16(cache(), batch(), k, k, rotary(1), None, None, None) is None
+        assert _native.append_f16(codes(), batch(), k, k, None, None, None, None) is None
+        assert _native.attention_paged_f16(o, q, codes(), batch(), 0.1, 1.0, 1) is None
+        assert recorders.taken() == ""
+    finally:
+        _bind_native()
+
+
+@pytest.mark.parametrize("axes", [1, 3])
+def test_one_row_has_no_stride(both, axes):
+    """Positions and bits of one row, or of one word, whatever the stride that is not used."""
+    one = torch.zeros(1, axes, dtype=torch.int32).t()
+    native, general = both("norm_rotary_f16", rows(4, 1, 64), rows(4, 1, 64), one, rotary(axes), None)
+    assert general is not None and native in (None, general)
+    native, general = both("attention_tree_f16", rows(8, 9, 64), rows(8, 9, 64), cache(), batch(), DraftTree(torch.zeros(9, 4, dtype=torch.int32)[:, ::4]), 0.1,
+                           1.0)
+    assert general is not None and native in (None, general)
