@@ -130,6 +130,8 @@ HOST_TEST_SRC = os.path.join(CPP_TESTS, "test_host.cpp")
 HOST_TEST_BIN = os.path.join(CPP_TESTS, "bin", "test_host")
 SEQUENCES_TEST_SRC = os.path.join(CPP_TESTS, "test_sequences.cpp")
 SEQUENCES_TEST_BIN = os.path.join(CPP_TESTS, "bin", "test_sequences")
+STEP_TEST_SRC = os.path.join(CPP_TESTS, "test_step.cpp")
+STEP_TEST_BIN = os.path.join(CPP_TESTS, "bin", "test_step")
 
 
 def _build_host_test(force: bool, src: str, out: str) -> str:
@@ -151,9 +153,14 @@ def build_sequences_test(force: bool = False) -> str:
     return _build_host_test(force, SEQUENCES_TEST_SRC, SEQUENCES_TEST_BIN)
 
 
+def build_step_test(force: bool = False) -> str:
+    return _build_host_test(force, STEP_TEST_SRC, STEP_TEST_BIN)
+
+
 def build_host_test(force: bool = False) -> str:
     """Compiles the C++ host-side tests (header-only host/*.hpp over the C ABI) with g++."""
     build_sequences_test(force)
+    build_step_test(force)
     return _build_host_test(force, HOST_TEST_SRC, HOST_TEST_BIN)
 
 

@@ -114,6 +114,44 @@ struct PagedCache {
 using PagedBatch = adr_paged_batch;
 using PackedBatch = adr_packed_batch;
 using Rotary = adr_rotary;
+using RotaryAxes = adr_rotary_axes;
+using HeadNorm = adr_head_norm;
+using DraftTree = adr_draft_tree;
+
+// Keys and values in 8 bits: [pages, kv_heads, page_size, d] views of codes and [pages, kv_heads, page_size] views of their scales.
+struct PagedCacheU8 {
+  TensorView<uint8_t> key;
+  TensorView<f16> key_scale;
+  TensorView<uint8_t> value;
+  TensorView<f16> value_scale;
+  adr_paged_cache_u8 lower() const {
+    const auto &k = key.layout, &v = value.layout, &ks = key_scale.layout, &vs = value_scale.layout;
+    if (k.dims.size() != 4 || k.dims != v.dims) throw std::logic_error("PagedCacheU8: [pages, kv_heads, page_size, d] views");
+    const std::vector<size_t> scales(k.dims.begin(), k.dims.end() - 1);
+    if (ks.dims != scales || vs.dims != scales) throw std::logic_error("PagedCacheU8: [pages, kv_heads, page_size] views of scales");
+    adr_paged_cache_u8 c{};
+    c.key = key.ptr, c.key_scale = key_scale.ptr, c.value = value.ptr, c.value_scale = value_scale.ptr;
+    auto size = [&](int i) { return int32_of(k.dims[i], "PagedCacheU8"); };
+    c.pages = size(0), c.kv_heads = size(1), c.page_size = size(2), c.d = size(3);
+    c.stride_kx = (int64_t)k.strides[3], c.stride_ky = (int64_t)k.strides[2], c.stride_kz = (int64_t)k.strides[1], c.stride_kp = (int64_t)k.strides[0];
+    c.stride_vx = (int64_t)v.strides[3], c.stride_vy = (int64_t)v.strides[2], c.stride_vz = (int64_t)v.strides[1], c.stride_vp = (int64_t)v.strides[0];
+    c.stride_ksy = (int64_t)ks.strides[2], c.stride_ksz = (int64_t)ks.strides[1], c.stride_ksp = (int64_t)ks.strides[0];
+    c.stride_vsy = (int64_t)vs.strides[2], c.stride_vsz = (int64_t)vs.strides[1], c.stride_vsp = (int64_t)vs.strides[0];
+    return c;
+  }
+};
+
+// What a step appends: its keys and values, its queries with the view that they are turned into (both null: none), the positions on
+// each axis (device memory, `pitch` entries from axis to axis; null: the places in the cache), the rotation and the norms.
+struct Appended {
+  TensorView<const f16> key, value;
+  RotaryAxes rotary{nullptr, nullptr, 0, ADR_ROTARY_HALVES, 1.0f, 1};
+  HeadNorm query_norm{}, key_norm{};
+  TensorView<f16>* query_out = nullptr;
+  const TensorView<const f16>* query = nullptr;
+  const int32_t* positions = nullptr;
+  int32_t pitch = 0;
+};
 
 struct CommonKernels {
   virtual ~CommonKernels() = default;
@@ -155,6 +193,36 @@ struct CommonKernels {
                                     const PackedBatch& /*batch*/, float /*scale*/, float /*temperature*/ = 1.0f,
                                     MatmulMask /*mask*/ = MatmulMask::Causal) {
     throw AdrasteaError(ADR_ENOTIMPL, "attention_packed_f16");
+  }
+  // Heads normed and turned on several axes, a cache in 8 bits, drafted trees: see adr_norm_rotary_f16, adr_append_norm_f16,
+  // adr_append_u8, adr_read_u8, adr_attention_paged_u8, adr_attention_tree_f16 and adr_attention_tree_u8.
+  // The heads of `input` normed and turned into `output`, which may be the same view; positions [axes][pitch].
+  virtual void norm_rotary_f16(TensorView<f16>& /*output*/, const TensorView<const f16>& /*input*/, const int32_t* /*positions*/,
+                               int32_t /*pitch*/, const RotaryAxes& /*rotary*/, const HeadNorm& /*norm*/) {
+    throw AdrasteaError(ADR_ENOTIMPL, "norm_rotary_f16");
+  }
+  virtual void append_norm_f16(const PagedCache& /*cache*/, const PagedBatch& /*batch*/, const Appended& /*step*/) {
+    throw AdrasteaError(ADR_ENOTIMPL, "append_norm_f16");
+  }
+  virtual void append_u8(const PagedCacheU8& /*cache*/, const PagedBatch& /*batch*/, const Appended& /*step*/) {
+    throw AdrasteaError(ADR_ENOTIMPL, "append_u8");
+  }
+  // What the codes of the batch's rows stand for.
+  virtual void read_u8(TensorView<f16>& /*key_out*/, TensorView<f16>& /*value_out*/, const PagedCacheU8& /*cache*/, const PagedBatch& /*batch*/) {
+    throw AdrasteaError(ADR_ENOTIMPL, "read_u8");
+  }
+  virtual void attention_paged_u8(TensorView<f16>& /*output*/, const TensorView<const f16>& /*query*/, const PagedCacheU8& /*cache*/,
+                                  const PagedBatch& /*batch*/, float /*scale*/, float /*temperature*/ = 1.0f,
+                                  MatmulMask /*mask*/ = MatmulMask::Causal) {
+    throw AdrasteaError(ADR_ENOTIMPL, "attention_paged_u8");
+  }
+  virtual void attention_tree_f16(TensorView<f16>& /*output*/, const TensorView<const f16>& /*query*/, const PagedCache& /*cache*/,
+                                  const PagedBatch& /*batch*/, const DraftTree& /*tree*/, float /*scale*/, float /*temperature*/ = 1.0f) {
+    throw AdrasteaError(ADR_ENOTIMPL, "attention_tree_f16");
+  }
+  virtual void attention_tree_u8(TensorView<f16>& /*output*/, const TensorView<const f16>& /*query*/, const PagedCacheU8& /*cache*/,
+                                 const PagedBatch& /*batch*/, const DraftTree& /*tree*/, float /*scale*/, float /*temperature*/ = 1.0f) {
+    throw AdrasteaError(ADR_ENOTIMPL, "attention_tree_u8");
   }
 };
 
@@ -301,6 +369,55 @@ class GpuKernels : public CommonKernels {
     int rc = workspace_bytes_ > 0 ? call(adr_attention_packed_f16_ws, workspace_, workspace_bytes_) : call(adr_attention_packed_f16);
     if (rc) throw AdrasteaError(rc, what);
   }
+  void norm_rotary_f16(TensorView<f16>& output, const TensorView<const f16>& input, const int32_t* positions, int32_t pitch,
+                       const RotaryAxes& rotary, const HeadNorm& norm) override {
+    const Rows o = rows_of(output, "norm_rotary_f16"), i = rows_of(input, "norm_rotary_f16");
+    same(o, i, "norm_rotary_f16");
+    int rc = adr_norm_rotary_f16(stream_, output.ptr, input.ptr, positions, pitch, rotary, norm, i.heads, i.rows, i.d, o.x, o.y, o.z,
+                                 i.x, i.y, i.z);
+    if (rc) throw AdrasteaError(rc, "norm_rotary_f16");
+  }
+  void append_norm_f16(const PagedCache& cache, const PagedBatch& batch, const Appended& step) override {
+    append(adr_append_norm_f16, "append_norm_f16", cache.lower(), batch, step);
+  }
+  void append_u8(const PagedCacheU8& cache, const PagedBatch& batch, const Appended& step) override {
+    append(adr_append_u8, "append_u8", cache.lower(), batch, step);
+  }
+  void read_u8(TensorView<f16>& key_out, TensorView<f16>& value_out, const PagedCacheU8& cache, const PagedBatch& batch) override {
+    const adr_paged_cache_u8 c = cache.lower();
+    const Rows k = rows_of(key_out, "read_u8"), v = rows_of(value_out, "read_u8");
+    same(k, v, "read_u8");
+    if (k.heads != c.kv_heads || k.d != c.d) throw std::logic_error("read_u8: shape mismatch");
+    int rc = adr_read_u8(stream_, key_out.ptr, value_out.ptr, c, batch, k.rows, k.x, k.y, k.z, v.x, v.y, v.z);
+    if (rc) throw AdrasteaError(rc, "read_u8");
+  }
+  void attention_paged_u8(TensorView<f16>& output, const TensorView<const f16>& query, const PagedCacheU8& cache, const PagedBatch& batch,
+                          float scale, float temperature = 1.0f, MatmulMask mask = MatmulMask::Causal) override {
+    attend("attention_paged_u8", output, query, cache.lower(), [&](const Rows& o, const Rows& q, const adr_paged_cache_u8& c) {
+      return workspace_bytes_ > 0 ? adr_attention_paged_u8_ws(stream_, output.ptr, query.ptr, c, batch, q.heads, q.rows, o.x, o.y, o.z, q.x,
+                                                              q.y, q.z, scale, temperature, (uint32_t)mask, workspace_, workspace_bytes_)
+                                  : adr_attention_paged_u8(stream_, output.ptr, query.ptr, c, batch, q.heads, q.rows, o.x, o.y, o.z, q.x,
+                                                           q.y, q.z, scale, temperature, (uint32_t)mask);
+    });
+  }
+  void attention_tree_f16(TensorView<f16>& output, const TensorView<const f16>& query, const PagedCache& cache, const PagedBatch& batch,
+                          const DraftTree& tree, float scale, float temperature = 1.0f) override {
+    attend("attention_tree_f16", output, query, cache.lower(), [&](const Rows& o, const Rows& q, const adr_paged_cache& c) {
+      return workspace_bytes_ > 0 ? adr_attention_tree_f16_ws(stream_, output.ptr, query.ptr, c, batch, tree, q.heads, q.rows, o.x, o.y, o.z,
+                                                              q.x, q.y, q.z, scale, temperature, workspace_, workspace_bytes_)
+                                  : adr_attention_tree_f16(stream_, output.ptr, query.ptr, c, batch, tree, q.heads, q.rows, o.x, o.y, o.z,
+                                                           q.x, q.y, q.z, scale, temperature);
+    });
+  }
+  void attention_tree_u8(TensorView<f16>& output, const TensorView<const f16>& query, const PagedCacheU8& cache, const PagedBatch& batch,
+                         const DraftTree& tree, float scale, float temperature = 1.0f) override {
+    attend("attention_tree_u8", output, query, cache.lower(), [&](const Rows& o, const Rows& q, const adr_paged_cache_u8& c) {
+      return workspace_bytes_ > 0 ? adr_attention_tree_u8_ws(stream_, output.ptr, query.ptr, c, batch, tree, q.heads, q.rows, o.x, o.y, o.z,
+                                                             q.x, q.y, q.z, scale, temperature, workspace_, workspace_bytes_)
+                                  : adr_attention_tree_u8(stream_, output.ptr, query.ptr, c, batch, tree, q.heads, q.rows, o.x, o.y, o.z,
+                                                          q.x, q.y, q.z, scale, temperature);
+    });
+  }
   std::string plan(const TensorLayout& o, const TensorLayout& l, const TensorLayout& r, const MatmulOptions& opt) const {
     LoweredMatmul w = lower_matmul(o, l, r, opt);
     char name[64];
@@ -317,6 +434,30 @@ class GpuKernels : public CommonKernels {
     LoweredMatmul w = lower_matmul(o.layout, l.layout, r.layout, opt);
     int rc = fn(stream_, o.ptr, l.ptr, r.ptr, w.batches, w.m, w.k, w.n, w.so[0], w.so[1], w.so[2], w.sl[0], w.sl[1],
                 w.sl[2], w.sr[0], w.sr[1], w.sr[2], opt.store_.bias, w.beta, w.scale, w.store, w.load, w.mask);
+    if (rc) throw AdrasteaError(rc, what);
+  }
+  template <typename F, typename Cache>
+  void append(F fn, const char* what, const Cache& c, const PagedBatch& batch, const Appended& step) {
+    const Rows k = rows_of(step.key, what), v = rows_of(step.value, what);
+    same(k, v, what);
+    if (k.heads != c.kv_heads || k.d != c.d || !step.query != !step.query_out) throw std::logic_error(std::string(what) + ": shape mismatch");
+    Rows q{}, o{};
+    if (step.query) {
+      q = rows_of(*step.query, what), o = rows_of(*step.query_out, what);
+      same(q, o, what);
+      if (q.rows != k.rows || q.d != k.d) throw std::logic_error(std::string(what) + ": shape mismatch");
+    }
+    int rc = fn(stream_, c, batch, step.key.ptr, step.value.ptr, step.query ? step.query_out->ptr : nullptr,
+                step.query ? step.query->ptr : nullptr, step.positions, step.pitch, step.rotary, step.query_norm, step.key_norm, q.heads,
+                k.rows, k.x, k.y, k.z, v.x, v.y, v.z, o.x, o.y, o.z, q.x, q.y, q.z);
+    if (rc) throw AdrasteaError(rc, what);
+  }
+  template <typename Cache, typename F>
+  void attend(const char* what, const TensorView<f16>& output, const TensorView<const f16>& query, const Cache& c, F call) {
+    const Rows o = rows_of(output, what), q = rows_of(query, what);
+    same(o, q, what);
+    if (q.d != c.d) throw std::logic_error(std::string(what) + ": shape mismatch");
+    int rc = call(o, q, c);
     if (rc) throw AdrasteaError(rc, what);
   }
   adr_stream_t stream_;
@@ -357,6 +498,25 @@ class MatmulTracer : public CommonKernels {
                             const TensorView<const f16>& v, const PackedBatch& batch, float scale, float t = 1.0f,
                             MatmulMask mask = MatmulMask::Causal) override {
     inner_.attention_packed_f16(o, q, k, v, batch, scale, t, mask);
+  }
+  void norm_rotary_f16(TensorView<f16>& o, const TensorView<const f16>& i, const int32_t* positions, int32_t pitch, const RotaryAxes& rotary,
+                       const HeadNorm& norm) override {
+    inner_.norm_rotary_f16(o, i, positions, pitch, rotary, norm);
+  }
+  void append_norm_f16(const PagedCache& cache, const PagedBatch& batch, const Appended& step) override { inner_.append_norm_f16(cache, batch, step); }
+  void append_u8(const PagedCacheU8& cache, const PagedBatch& batch, const Appended& step) override { inner_.append_u8(cache, batch, step); }
+  void read_u8(TensorView<f16>& k, TensorView<f16>& v, const PagedCacheU8& cache, const PagedBatch& batch) override { inner_.read_u8(k, v, cache, batch); }
+  void attention_paged_u8(TensorView<f16>& o, const TensorView<const f16>& q, const PagedCacheU8& cache, const PagedBatch& batch,
+                          float scale, float t = 1.0f, MatmulMask mask = MatmulMask::Causal) override {
+    inner_.attention_paged_u8(o, q, cache, batch, scale, t, mask);
+  }
+  void attention_tree_f16(TensorView<f16>& o, const TensorView<const f16>& q, const PagedCache& cache, const PagedBatch& batch,
+                          const DraftTree& tree, float scale, float t = 1.0f) override {
+    inner_.attention_tree_f16(o, q, cache, batch, tree, scale, t);
+  }
+  void attention_tree_u8(TensorView<f16>& o, const TensorView<const f16>& q, const PagedCacheU8& cache, const PagedBatch& batch,
+                         const DraftTree& tree, float scale, float t = 1.0f) override {
+    inner_.attention_tree_u8(o, q, cache, batch, tree, scale, t);
   }
 
  private:
