@@ -89,9 +89,11 @@ def attention(q, k, v, scale, temp, seen):
 def close_enough(got, want, value_max, keys, codes):
     """As for the cache in 16 bits (sequences_reference.py).  Values of codes are not rounded, but a step of 2^-11 more of sum
     w |v| <= value_max is allowed (and 2^-25) for a kernel that rounds them to fp16 first.  Scores of codes are 32-bit sums of
-    d <= 128 products of codes up to 255, which begin at -127.5 sum(q): in the tests here sum |q| <= 110, scales <= 0.03 and
-    the factor is 1 / sqrt(d) >= 0.08, so that all of it adds up to less than 110 * 382 * 0.03 * 0.125 < 2^8 / 1.6 for d = 64 and
-    less than 2^7 for d = 128; an error of d 2^-24 of that is below 2^-11 in each exponent, as there."""
+    d <= 128 products of codes up to 255, which begin at -127.5 sum(q): whatever the order, what is summed so far is at most
+    127.5 sum |q|, as codes are at most 127.5 off 127.5.  In the tests here sum |q| <= 130, scales are below 0.042, a head's norm keeps
+    sum |q| below 80 where they are above 0.03, and the factor is at most 1 / (0.9 sqrt(d)): d roundings of 2^-24 of
+    127.5 * 130 * 0.03 / (0.9 * 11.3) for d = 128 make less than 2^-11 in each exponent, as there; of smaller d, where sum |q| is
+    below 1.3 d, less still."""
     want = np.asarray(want, np.float64)
     extra = value_max * 2.0 ** -11 + 2.0 ** -25 if codes else 0.0
     bound = (np.abs(want) * 2.0 ** -11 + 2.0 ** -25 + extra +
