@@ -373,8 +373,9 @@ SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
   const int forced = knob(KNOB_SEQUENCES) >= 1 && knob(KNOB_SEQUENCES) <= 8 ? knob(KNOB_SEQUENCES) : 0;
   if (forced == 1) return SequencesPlan{SequencesPlan::ANY_LAYOUT, 0, 0, 0, 0, 0};
   if (forced) p.kind = forced <= 4 ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES;
-  const bool few = p.kind == SequencesPlan::FEW_ROWS;
-  const int rows = few ? FEW : MANY, keys = few ? FEW_KEYS : MANY_KEYS, hd = a.d <= 64 ? 64 : 128;
+  bool few = p.kind == SequencesPlan::FEW_ROWS;
+  int rows = few ? FEW : MANY, keys = few ? FEW_KEYS : MANY_KEYS;
+  const int hd = a.d <= 64 ? 64 : 128;
   const int64_t most_keys = a.table ? std::min((int64_t)a.table_width * a.page_size, (int64_t)MOST_KEYS) : a.keys;
   const double longest = a.longest > 0 ? std::min<double>(a.longest, most_keys) : most_keys;
   // Blocks of all key heads, as far as the host can tell: a sequence's last one is full by half, but where one sequence has
@@ -383,7 +384,24 @@ SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail) {
   const double full = (double)a.rows * a.group / rows, ends = (double)longest_rows * sequences > 4.0 * a.rows ? sequences : sequences / 2.0;
   const double blocks = a.kv_heads * (few ? std::max(full, (double)sequences) : sequences <= 1 ? ceil(full) : std::max(full + ends, (double)sequences));
   p.least = 1;
-  if (few) {
+  if (a.mask == MASK_TREE && !forced) {
+    // Drafts are often more than a block of few rows, and seldom one of many: either kernel, by what it takes.
+    static const Costs of_64 = {{5.6, 9.2, 1.2, 1.2, 5.9}, {5.6, 4.8, 1.2, 2.1, 5.4}, {6.1, 1.2, 8.2, 0.64, 8.1},
+                                {6.8, 11, 2.2, 2.9, 8.7}, {7.6, 8.6, 1.3, 6.8, 11}, {9.1, 1.1, 0.015}, {9.9, 1.2, 0.022}, 0.67, 1.02, 0.012};
+    static const Costs of_128 = {{5.8, 11, 2.7, 2.3, 9.7}, {5.7, 7.3, 1.9, 4.5, 8.4}, {4.6, 1.5, 8.9, 1.7, 14},
+                                 {8.7, 16, 4.8, 3.9, 15}, {10, 12, 4.1, 8.9, 16}, {12, 1.1, 0.016}, {12, 1.0, 0.025}, 1.1, 2.0, 0.018};
+    auto blocks_of = [&](int rows) {
+      const double full = (double)a.rows * a.group / rows;
+      return a.kv_heads * (rows == FEW && (int64_t)longest_rows * a.group <= FEW ? std::max(full, (double)sequences)
+                           : sequences <= 1                                      ? ceil(full)
+                                                                                 : std::max(full + ends, (double)sequences));
+    };
+    const double few_blocks = blocks_of(FEW);
+    const int each = (hd == 64 ? 2 : 1) * (few_blocks >= 4.0 * cus ? 2 : 1);
+    plan_by_cost(p, a, cus, avail, few_blocks, blocks_of(MANY), longest, 4, std::max(1, each * cus / a.kv_heads), hd == 64 ? of_64 : of_128);
+    few = p.kind == SequencesPlan::FEW_ROWS;
+    rows = few ? FEW : MANY, keys = few ? FEW_KEYS : MANY_KEYS;
+  } else if (few) {
     // Two launches take the host and the device some 4 us more than one, and shared keys leave no workgroup with more
     // than the others.  us, fitted to 16 shapes of 12 to 32 heads, 1 to 256 sequences and 250 to 4000 keys: a block
     // by itself, four wavefronts to it, 4 + 8.5 per 1000 keys of 128 (one of 500 keys 7.8, shared 9.2; 700 9.1, 9.2; 1000

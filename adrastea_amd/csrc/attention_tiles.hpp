@@ -812,5 +812,59 @@ inline void plan_tiles(SequencesPlan& p, const SequencesArgs& a, int cus, double
   shared(8, cus, 14, two / 2);
 }
 
+// Of all forms the one that should take least, for calls that may go through either kernel whatever their rows are: few rows with two
+// wavefronts to a block, with `waves`, or shared; many rows with four or eight, or shared.
+//
+// us, with `keys` thousands of keys of the longest sequence and `blocks` for each compute unit: a block by itself takes start + alone *
+// keys, all of them `all` + (block + read * keys) * blocks, and the longer of the two counts, or a little more than either where they
+// are level.  Shared many rows as in plan_tiles.  Fitted to the times of every form over 36800 drawn batches (1 to 1024 rows and sequences,
+// 1 to 65000 keys, 12 to 40 heads of 64 to 128 in 1 to 32 key heads): over others, the form that is taken needs 1.03 times the time of the
+// best, all together; one in a hundred 1.3 times.  (By rows alone, as for attention_paged_f16, 1.15 and 1.9.)
+struct Cost {
+  double start, alone, all, block, read;
+  double us(double keys, double blocks) const {
+    const double x = start + alone * keys, y = all + (block + read * keys) * blocks;
+    return sqrt(sqrt(x * x * x * x + y * y * y * y));
+  }
+};
+struct SharedCost {
+  double start, tile, part;
+};
+struct Costs {
+  Cost two, waves, few_shared, four, eight;
+  SharedCost four_shared, eight_shared;
+  double tile, tiles, way;  // as in plan_tiles, for the number of parts
+};
+
+inline void plan_by_cost(SequencesPlan& p, const SequencesArgs& a, int cus, int64_t avail, double few_blocks, double many_blocks, double longest,
+                         int waves, int few_parts, const Costs& c) {
+  const double keys = longest / 1000, few = few_blocks / cus, many = many_blocks / cus;
+  double best = HUGE_VAL;
+  auto take = [&](double us, SequencesPlan::Kind kind, int with, int parts, int least) {
+    if (us < best) best = us, p.kind = kind, p.waves = with, p.parts = parts, p.least = least;
+  };
+  const int hd = a.d <= 64 ? 64 : 128;
+  auto fits = [&](int64_t slots) { return avail / ((slots * (hd * 4 + 8) + (int64_t)sizeof(Seam)) * a.kv_heads) >= 2; };
+  take(c.two.us(keys, few), SequencesPlan::FEW_ROWS, 2, 0, 1);
+  take(c.waves.us(keys, few), SequencesPlan::FEW_ROWS, waves, 0, 1);
+  if (a.sequences <= 256 && few_parts > 1 && fits(2 * FEW)) take(c.few_shared.us(keys, few), SequencesPlan::FEW_ROWS, 2, few_parts, 1);
+  if ((int64_t)(a.longest_rows > 0 ? std::min(a.longest_rows, a.rows) : a.rows) * a.group <= FEW) return;  // (a block for each sequence)
+  take(c.four.us(keys, many), SequencesPlan::TILES, 4, 0, 4);
+  take(c.eight.us(keys, many), SequencesPlan::TILES, 8, 0, 4);
+  if (a.sequences > 256 || !fits(MANY)) return;
+  const bool single = a.sequences == 1;
+  const double work = many_blocks * (longest / MANY_KEYS + 1) * (single ? 1.0 : 0.75);
+  auto shared = [&](int with, double most, double tile, const SharedCost& cost) {
+    double n = std::min(most, sqrt(work * tile / c.way));
+    if (single) n = floor(n / many_blocks) * many_blocks;
+    if (n < (single ? 2.0 : 1.5) * many_blocks) return;
+    take(cost.start + cost.tile * work * tile / (single ? n : n - many_blocks / 2) + cost.part * n, SequencesPlan::TILES, with,
+         (int)(n / a.kv_heads + 0.5), 4);
+  };
+  shared(4, cus * 15 / 16.0, c.tile, c.four_shared);
+  shared(4, 2.0 * cus, c.tiles, c.four_shared);
+  shared(8, cus, c.tiles / 2, c.eight_shared);
+}
+
 }  // namespace
 }  // namespace adr

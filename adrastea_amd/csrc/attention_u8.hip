@@ -470,29 +470,20 @@ SequencesPlan sequences_u8_plan(const SequencesArgs& a, int cus, int64_t avail) 
     const double full = (double)a.rows * a.group / rows, ends = (double)longest_rows * sequences > 4.0 * a.rows ? sequences : sequences / 2.0;
     return a.kv_heads * (sequences <= 1 ? ceil(full) : std::max(full + ends, (double)sequences));
   };
-  // Blocks of few rows read the keys once each, at 24 bytes a ns and compute unit; of many rows, they compute a tile of 64 keys in 1.5 us.
-  // So three of the former to one of the latter take as much (drafts of 2 to 13 tokens, 4 heads to a key head, 24 sequences: 56 us, 70).
   const bool one_block = (int64_t)longest_rows * a.group <= FEW;
   const double few_blocks = one_block ? a.kv_heads * std::max((double)a.rows * a.group / FEW, (double)sequences) : blocks_of(FEW);
-  SequencesPlan p = {one_block || few_blocks < 3.0 * blocks_of(MANY) ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES, 2, 0, 0, 1, 0};
+  static const Costs of_64 = {{5.4, 16, 5.0, 0.89, 2.3}, {6.4, 5.0, 2.6, 5.1, 4.2}, {6.9, 1.6, 10, 0.7, 7.4},
+                              {6.8, 20, 1.6, 3.4, 6.6}, {7.7, 14, 1.4, 7.2, 9.1}, {9.7, 1.3, 0.013}, {9.9, 1.5, 0.017}, 0.85, 1.4, 0.012};
+  static const Costs of_128 = {{6.8, 18, 4.0, 1.7, 3.7}, {7.4, 6.2, 2.7, 6.1, 5.5}, {8.3, 1.7, 11, 1.1, 8.3},
+                               {8.6, 26, 3.4, 4.3, 6.5}, {10, 20, 2.7, 8.8, 13}, {12, 0.99, 0.02}, {12, 1.1, 0.025}, 1.4, 2.6, 0.018};
+  // Shared few rows: as many workgroups as fit the LDS.
+  SequencesPlan p = {SequencesPlan::FEW_ROWS, 2, 0, 0, 1, 0};
+  plan_by_cost(p, a, cus, avail, few_blocks, blocks_of(MANY), longest, 8, std::max(1, (hd == 64 ? 8 : 4) * cus / a.kv_heads),
+               hd == 64 ? of_64 : of_128);
   if (forced) p.kind = forced <= 4 ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES;
   const bool few = p.kind == SequencesPlan::FEW_ROWS;
   const int rows = few ? FEW : MANY, keys = few ? FEW_KEYS : MANY_KEYS;
-  const double full = (double)a.rows * a.group / rows, blocks = few ? few_blocks : blocks_of(MANY);
-  if (few) {
-    // us, fitted to 1 to 200 sequences of up to 300 to 4000 keys, 8 key heads of 128: a block to eight wavefronts, which have a compute
-    // unit to themselves; to two; keys shared, whose sum counts and not the longest.  (64 sequences of up to 1000, 2000, 4000
-    // keys: 24.6, 32.9, 54.6; 25.8, 45.3, 84.6; shared, of 4000, 56.2.  100: 39, 52, 85; 30, 53, 101; 84.6.  8: 11.7, 17.2, 27.6;
-    // 20, 36, 68; shared, of 2000 and 4000, 15.1, 17.2.)
-    const double size = longest / 1000 * hd / 128, rounds = std::max(1.0, blocks / cus), all = blocks * longest * hd * 2 / 6e6;
-    const double eight = 2 + 5 * rounds + 5.4 * size * rounds, two = 6 + size * std::max(13 + 0.0125 * blocks, 0.028 * blocks);
-    const double shared = 12 + all * (sequences > 1 ? 0.53 : 1.0);
-    if (shared < std::min(eight, two)) p.parts = std::max(1, (hd == 64 ? 8 : 4) * cus / a.kv_heads);
-    else p.waves = eight < two ? 8 : 2;
-  } else {
-    // (a tile takes a third longer than one of values in 16 bits)
-    plan_tiles(p, a, cus, blocks, longest, hd == 64 ? 0.85 : 1.4, hd == 64 ? 1.4 : 2.6, hd == 64 ? 0.012 : 0.018);
-  }
+  const double full = (double)a.rows * a.group / rows;
   if (forced) {  // (shared in small parts, so that short sequences are divided too)
     const bool divides = forced == 4 || (forced > 6 && a.sequences <= 256 && full + sequences < 1000);
     p.waves = forced == 3 || forced == 6 || forced == 8 ? 8 : forced == 5 || forced == 7 ? 4 : 2;
