@@ -21,6 +21,7 @@ enum Cache { NO_CACHE, F16, U8 };
 
 struct PlaceJob : PlaceArgs {
   int lanes;   // that a head needs, of W
+  uint32_t first;
   int splits;  // wavefronts that share a row's heads
 };
 
@@ -193,18 +194,32 @@ __device__ __forceinline__ Slot slot_of_row(const adr_paged_batch& b, int rows, 
 
 // A wavefront has a row, or shares it with others where rows are few.  W lanes have a head, and the 64 / W heads that a wavefront
 // works on lie side by side; a lane has the 16 values that are turned together and so need no exchange: of halves chunk l
-// of 8 values and its partner, of pairs two chunks side by side; chunks that pass follow, two to a lane.  So angles and weights
-// stay in registers from head to head: each angle is computed by one lane of the wavefront, and comes to the others by way of LDS.
+// of 8 values and its partner, of pairs two chunks side by side; chunks that pass follow, two to a lane.  Each angle is computed by one
+// lane of the wavefront, and comes to the others by way of LDS.
 //
 // Loads and stores of the loops are under no condition, so that the next head's loads are waited for and not the stores in front
 // of them: lanes that are left over do what the last one with values does, and store the same.
+//
+// Memory bounds it, and how many wavefronts ask for it: a wavefront takes 14 us, nearly all of it waiting, so registers are what counts.
+// Angles are read from LDS for every head, weights widened for every head, and a wavefront has one task: kept from head to head, or
+// constants from task to task, they made 127 to 187 registers, two or three wavefronts to a SIMD; now 52, with codes 107.  us, then and
+// now: 7008 rows of 32 / 8 heads of 128 into a cache in 16 bits (172 MB) 44.6, 37.2, 4.6 TB/s, where a copy of as many bytes
+// has 5.2; 7364 rows of them into one in 8 bits (195 MB) 60.2, 48.9; one row of 24 tokens 5.8, 4.7; one token's queries 3.2, 2.7.
 template <int CACHE, int W>
 __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
   typedef typename std::conditional<CACHE == U8, double, float>::type angle_t;
   constexpr int GROUPS = 64 / W, MOST_PAIRS = 8 * W;
-  __shared__ Turn<angle_t> shared_turns[4][MOST_PAIRS];
+  __shared__ Turn<float> shared_rounded[4][MOST_PAIRS];
+  __shared__ Turn<double> shared_turns[4][CACHE == U8 ? MOST_PAIRS : 1];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), l = min(lane & (W - 1), a.lanes - 1);
-  Turn<angle_t>* const turns = shared_turns[wave];
+  // (pair 8 l + e at e W + l: a lane reads the eight of its l, beside the other lanes'.  Keys that become codes need them in 64 bits.)
+  Turn<float>* const rounded = shared_rounded[wave];
+  Turn<double>* const turns = shared_turns[wave];
+  auto keep = [&](int pair, const Turn<angle_t>& t) __attribute__((always_inline)) {
+    const int at = (pair & 7) * W + (pair >> 3);
+    rounded[at] = {(float)t.cosine, (float)t.sine};
+    if constexpr (CACHE == U8) turns[at] = t;
+  };
   const bool mine = (lane & (W - 1)) < a.lanes;
   const int end_q = a.q ? a.heads : 0, end_k = end_q + (CACHE == NO_CACHE ? 0 : a.kv_heads), all = 2 * end_k - end_q;
   // The lane's chunks (first values), and which are turned.
@@ -224,16 +239,10 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
   const bool one = x1 >= a.d;  // (the last of an odd number: its chunk twice)
   if (one) x1 = x0, turn1 = false;
   const float per_value = 1.0f / (float)a.d;
-  // What does not depend on the row, and is asked for ahead of all else: the lane's own pair, and the queries' weights.
-  const int half = a.dims >> 1, own_pair = min(lane, max(half - 1, 0));
-  const double own_turns = half > 0 ? a.turns[own_pair] : 0.0;
-  const int own_axis = half > 0 && a.axis ? a.axis[own_pair] : 0;
-  half8_t qw0, qw1;
-#pragma unroll
-  for (int e = 0; e < 8; e++) qw0[e] = qw1[e] = (half_t)1;
-  if (a.q_weight) qw0 = *(const half8_t*)(a.q_weight + x0), qw1 = *(const half8_t*)(a.q_weight + x1);
+  const int half = a.dims >> 1;
   const uint32_t tasks = (uint32_t)a.rows * a.splits;  // (splits are more than one where there are few rows)
-  for (uint64_t task = (uint64_t)blockIdx.x * 4 + wave; task < tasks; task += (uint64_t)gridDim.x * 4) {
+  const uint32_t task = a.first + blockIdx.x * 4 + wave;
+  if (task < tasks) {
     const int row = uniform((int)((uint32_t)task / (uint32_t)a.splits)), split = uniform((int)((uint32_t)task - (uint32_t)row * a.splits));
     const int step = GROUPS * a.splits, h0 = split * GROUPS + lane / W;
     // The chunks of a head, asked for a head ahead (behind the last one, that again).
@@ -245,79 +254,72 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
       n0 = *(const half8_t*)(from + x0);
       n1 = *(const half8_t*)(from + x1);
     };
-    const int own_position = a.positions && half > 0
-                                 ? a.positions[(int64_t)((unsigned)own_axis < (unsigned)a.axes ? own_axis : 0) * a.positions_pitch + row] : 0;
     read(min(h0, all - 1));
+    // Asked for ahead of where the row is: the lane's own angle, and the weights of the first heads.
+    const int own_pair = min(lane, max(half - 1, 0));
+    const double own_turns = half > 0 ? a.turns[own_pair] : 0.0;
+    const int own_axis = half > 0 && a.axis ? a.axis[own_pair] : 0;
+    half8_t w0 = {}, w1 = {};
+    auto weights = [&](const uint16_t* w) __attribute__((always_inline)) {
+      if (w) w0 = *(const half8_t*)(w + x0), w1 = *(const half8_t*)(w + x1);
+    };
+    weights((const uint16_t*)(end_q > 0 ? a.q_weight : a.k_weight));
+    const int own_position =
+        a.positions && half > 0 ? a.positions[(int64_t)((unsigned)own_axis < (unsigned)a.axes ? own_axis : 0) * a.positions_pitch + row] : 0;
     Slot at = {row, 0, -1, 0};
     if constexpr (CACHE != NO_CACHE) {
       const int pages = CACHE == U8 ? a.codes.pages : a.cache.pages, size = CACHE == U8 ? a.codes.page_size : a.cache.page_size;
       at = slot_of_row(a.batch, a.rows, pages, size, row, lane);
-      if (uniform(at.row) < 0) continue;
+      if (uniform(at.row) < 0) return;
     }
-    if (lane < half) turns[lane] = turn_of<angle_t>(a.positions ? own_position : at.position, own_turns, a.magnitude);
+    if (lane < half) keep(lane, turn_of<angle_t>(a.positions ? own_position : at.position, own_turns, a.magnitude));
     for (int i = lane + 64; i < half; i += 64)
-      turns[i] = turn_of<angle_t>(position_of(a, row, i, at.position), a.turns[i], a.magnitude);
+      keep(i, turn_of<angle_t>(position_of(a, row, i, at.position), a.turns[i], a.magnitude));
     __builtin_amdgcn_wave_barrier();
     const int end = CACHE != NO_CACHE && uniform(at.page) < 0 ? end_q : all;  // (keys and values without a slot go nowhere)
-    if (h0 >= end) continue;
+    if (h0 >= end) return;
 
     auto store16 = [&](half_t* to, const half8_t& o0, const half8_t& o1) __attribute__((always_inline)) {
       *(half8_t*)(to + x0) = o0;
       *(half8_t*)(to + x1) = o1;
     };
-    // Norm and turn 16 values in 32 bits: weights are part of the cosines and sines, and the norm's factor is applied at the end.
-    struct Coefficients {
-      float uc[8], us[8], vc[8], vs[8];  // of each pair (u, v): u w cos, u w sin, v w cos, v w sin
+    // The lane, as a number that the compiler does not know from head to head: what is read by it is read again.
+    auto fresh = [&]() __attribute__((always_inline)) {
+      int i = l;
+      asm volatile("" : "+v"(i));
+      return i;
     };
-    auto coefficients = [&](const half8_t& w0, const half8_t& w1, Coefficients& f) __attribute__((always_inline)) {
-      Turn<float> t[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        t[e] = {1, 0};
-        if (e < 4 || !a.pairs ? turn0 : turn1) t[e] = {(float)turns[8 * l + e].cosine, (float)turns[8 * l + e].sine};
-      }
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float wu = (float)(!a.pairs ? w0[e] : e < 4 ? w0[2 * e & 7] : w1[2 * e & 7]);
-        const float wv = (float)(!a.pairs ? w1[e] : e < 4 ? w0[(2 * e + 1) & 7] : w1[(2 * e + 1) & 7]);
-        f.uc[e] = wu * t[e].cosine, f.us[e] = wu * t[e].sine;
-        f.vc[e] = wv * t[e].cosine, f.vs[e] = wv * t[e].sine;
-      }
-    };
-    auto place_rounded = [&](half_t* to, const half8_t& c0, const half8_t& c1, bool norm, float eps, const Coefficients& f)
+    // Norm and turn 16 values in 32 bits; the norm's factor is applied at the end.
+    auto place_rounded = [&](half_t* to, const half8_t& c0, const half8_t& c1, bool norm, float eps)
                              __attribute__((always_inline)) {
-      float factor = 1.0f;
+      float factor = 1.0f, y[16];
+#pragma unroll
+      for (int e = 0; e < 8; e++) y[e] = (float)c0[e], y[8 + e] = (float)c1[e];
       if (norm) {
+        asm volatile("" : "+v"(w0), "+v"(w1));
         float sum = 0.0f, sum1 = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) sum = fmaf((float)c0[e], (float)c0[e], sum), sum1 = fmaf((float)c1[e], (float)c1[e], sum1);
+        for (int e = 0; e < 8; e++) sum = fmaf(y[e], y[e], sum), sum1 = fmaf(y[8 + e], y[8 + e], sum1);
         sum = !mine ? 0.0f : one ? sum : sum + sum1;
         factor = __builtin_amdgcn_rsqf(fmaf(sum_of<W>(sum), per_value, eps));
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] *= (float)w0[e], y[8 + e] *= (float)w1[e];
+      }
+      const int i = fresh();
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        // (what passes is not mixed with its neighbour, which may be infinite)
+        float& u = y[a.pairs ? 2 * e : e];
+        float& v = y[a.pairs ? 2 * e + 1 : 8 + e];
+        if (e < 4 || !a.pairs ? turn0 : turn1) {
+          const Turn<float> t = rounded[e * W + i];
+          const float x = u * t.cosine, z = u * t.sine;
+          u = fmaf(-v, t.sine, x), v = fmaf(v, t.cosine, z);
+        }
       }
       half8_t o0, o1;
-      auto turn = [&](float u, float v, int e, bool is_turned, half_t& ou, half_t& ov) __attribute__((always_inline)) {
-        const float tu = u * f.uc[e], tv = v * f.vc[e];
-        // (what passes has a cosine of 1, and is not mixed with its neighbour's infinity)
-        ou = (half_t)((is_turned ? fmaf(-v, f.vs[e], tu) : tu) * factor);
-        ov = (half_t)((is_turned ? fmaf(u, f.us[e], tv) : tv) * factor);
-      };
-      if (a.pairs) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          half_t x, y;
-          turn((float)c0[2 * e], (float)c0[2 * e + 1], e, turn0, x, y);
-          o0[2 * e] = x, o0[2 * e + 1] = y;
-          turn((float)c1[2 * e], (float)c1[2 * e + 1], e + 4, turn1, x, y);
-          o1[2 * e] = one ? o0[2 * e] : x, o1[2 * e + 1] = one ? o0[2 * e + 1] : y;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          half_t x, y;
-          turn((float)c0[e], (float)c1[e], e, turn0, x, y);
-          o0[e] = x, o1[e] = y;
-        }
-      }
+      for (int e = 0; e < 8; e++) o0[e] = (half_t)(y[e] * factor), o1[e] = (half_t)((one ? y[e] : y[8 + e]) * factor);
       store16(to, o0, o1);
     };
     // 16 values as codes, and the head's scale.
@@ -342,34 +344,29 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
 
     int h = h0;
     if (h < min(end, CACHE == F16 ? end_k : end_q)) {
-      Coefficients f;
       if (h < end_q) {
-        coefficients(qw0, qw1, f);
         half_t* to = a.q_out + h * (int64_t)a.so_z + row * (int64_t)a.so_y;
         for (; h < end_q; h += step, to += (int64_t)step * a.so_z) {
           const half8_t c0 = n0, c1 = n1;
           read(min(h + step, all - 1));
-          place_rounded(to, c0, c1, a.q_weight != nullptr, a.q_eps, f);
+          place_rounded(to, c0, c1, a.q_weight != nullptr, a.q_eps);
         }
       }
       if (CACHE == F16 && h < min(end, end_k)) {
-        half8_t w0, w1;
-#pragma unroll
-        for (int e = 0; e < 8; e++) w0[e] = w1[e] = (half_t)1;
-        if (a.k_weight) w0 = *(const half8_t*)(a.k_weight + x0), w1 = *(const half8_t*)(a.k_weight + x1);
-        coefficients(w0, w1, f);
+        weights((const uint16_t*)a.k_weight);
         const adr_paged_cache& c = a.cache;
         half_t* const to = (half_t*)c.key + at.page * c.stride_kp + at.slot * c.stride_ky;
         for (; h < end_k; h += step) {
           const half8_t c0 = n0, c1 = n1;
           read(min(h + step, all - 1));
-          place_rounded(to + (h - end_q) * c.stride_kz, c0, c1, a.k_weight != nullptr, a.k_eps, f);
+          place_rounded(to + (h - end_q) * c.stride_kz, c0, c1, a.k_weight != nullptr, a.k_eps);
         }
       }
     }
     if constexpr (CACHE == U8) {
       const adr_paged_cache_u8& c = a.codes;
       if (h < min(end, end_k)) {
+        weights((const uint16_t*)a.k_weight);
         uint8_t* const to = c.key + at.page * c.stride_kp + at.slot * c.stride_ky;
         half_t* const scale = (half_t*)c.key_scale + at.page * c.stride_ksp + at.slot * c.stride_ksy;
         for (; h < end_k; h += step) {
@@ -379,20 +376,20 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
 #pragma unroll
           for (int e = 0; e < 8; e++) y[e] = (double)(float)c0[e], y[8 + e] = (double)(float)c1[e];
           if (a.k_weight) {
+            asm volatile("" : "+v"(w0), "+v"(w1));
             double sum = 0.0, sum1 = 0.0;
 #pragma unroll
             for (int e = 0; e < 8; e++) sum = fma(y[e], y[e], sum), sum1 = fma(y[8 + e], y[8 + e], sum1);
             sum = !mine ? 0.0 : one ? sum : sum + sum1;
             const double factor = 1.0 / sqrt(sum_of<W>(sum) / (double)a.d + (double)a.k_eps);
-            const half8_t w0 = *(const half8_t*)(a.k_weight + x0), w1 = *(const half8_t*)(a.k_weight + x1);
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] = y[e] * factor * (double)(float)w0[e], y[8 + e] = y[8 + e] * factor * (double)(float)w1[e];
           }
-          // (angles from LDS as they are used: in registers they would be 32 of them)
+          const int i = fresh();
           if (a.pairs) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-              const Turn<double> t = turns[min(8 * l + e, MOST_PAIRS - 1)];
+              const Turn<double> t = turns[e * W + i];
               const double u = y[2 * e], v = y[2 * e + 1], x = u * t.cosine - v * t.sine, z = u * t.sine + v * t.cosine;
               y[2 * e] = (e < 4 ? turn0 : turn1) ? x : e >= 4 && one ? y[2 * e - 8] : u;
               y[2 * e + 1] = (e < 4 ? turn0 : turn1) ? z : e >= 4 && one ? y[2 * e - 7] : v;
@@ -400,7 +397,7 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
           } else if (turn0) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-              const Turn<double> t = turns[8 * l + e];
+              const Turn<double> t = turns[e * W + i];
               const double u = y[e], v = y[8 + e];
               y[e] = u * t.cosine - v * t.sine;
               y[8 + e] = u * t.sine + v * t.cosine;
@@ -610,11 +607,15 @@ hipError_t launch_place_into(hipStream_t stream, const PlaceArgs& a) {
   // wavefronts for each of 256 compute units.
   const int64_t steps = (heads + 64 / W - 1) / (64 / W);
   job.splits = (int)std::min<int64_t>(std::max<int64_t>((256 * 16 + a.rows - 1) / a.rows, 1), steps);
-  const unsigned grid = (unsigned)std::min<int64_t>(((int64_t)a.rows * job.splits + 3) / 4, MOST);
-  if (W == 4) hipLaunchKernelGGL(HIP_KERNEL_NAME(place_kernel<CACHE, 4>), dim3(grid), dim3(256), 0, stream, job);
-  else if (W == 8) hipLaunchKernelGGL(HIP_KERNEL_NAME(place_kernel<CACHE, 8>), dim3(grid), dim3(256), 0, stream, job);
-  else if (W == 16) hipLaunchKernelGGL(HIP_KERNEL_NAME(place_kernel<CACHE, 16>), dim3(grid), dim3(256), 0, stream, job);
-  else hipLaunchKernelGGL(HIP_KERNEL_NAME(place_kernel<CACHE, 32>), dim3(grid), dim3(256), 0, stream, job);
+  const int64_t tasks = (int64_t)a.rows * job.splits;
+  for (int64_t first = 0; first < tasks; first += 4 * MOST) {
+    job.first = (uint32_t)first;
+    const unsigned grid = (unsigned)std::min<int64_t>((tasks - first + 3) / 4, MOST);
+    if (W == 4) hipLaunchKernelGGL(HIP_KERNEL_NAME(place_kernel<CACHE, 4>), dim3(grid), dim3(256), 0, stream, job);
+    else if (W == 8) hipLaunchKernelGGL(HIP_KERNEL_NAME(place_kernel<CACHE, 8>), dim3(grid), dim3(256), 0, stream, job);
+    else if (W == 16) hipLaunchKernelGGL(HIP_KERNEL_NAME(place_kernel<CACHE, 16>), dim3(grid), dim3(256), 0, stream, job);
+    else hipLaunchKernelGGL(HIP_KERNEL_NAME(place_kernel<CACHE, 32>), dim3(grid), dim3(256), 0, stream, job);
+  }
   return hipGetLastError();
 }
 
