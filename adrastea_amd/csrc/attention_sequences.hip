@@ -45,7 +45,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_few_rows_kernel(Job) 
   Args first = arguments();
   early<PAGED, !SHARED>(first);
   const int kv_heads = first.kv_heads, hk = blockIdx.x % kv_heads, wg = blockIdx.x / kv_heads;
-  Roster<ROWS, KEYS, PAGED, SHARED> roster;
+  Roster<ROWS, KEYS, PAGED, SHARED, TREE && !SHARED> roster;
   const Line line = roster.line_of(first, threadIdx.x & 63);
   if (wg >= line.parts) {
     if (SHARED && threadIdx.x == 0) arguments().seams[wg * kv_heads + hk].parts = 0;
@@ -456,6 +456,7 @@ static hipError_t launch_blocks(hipStream_t stream, const SequencesArgs& a, cons
   job.parts = p.parts, job.shift = p.shift, job.least = p.least;
   job.part_o = (float*)workspace;
   job.per_head = 1.0 / a.group;
+  job.longest_first = p.longest_first;
   const int64_t part_rows = (int64_t)(few ? 2 : 1) * p.parts * a.kv_heads * rows;
   job.part_ml = (float2*)(job.part_o + (p.parts > 0 ? part_rows * HD : 0));
   job.seams = (Seam*)(job.part_ml + (p.parts > 0 ? part_rows : 0));

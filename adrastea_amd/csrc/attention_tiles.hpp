@@ -845,6 +845,7 @@ inline void plan_by_cost(SequencesPlan& p, const SequencesArgs& a, int cus, int6
   };
   const int hd = a.d <= 64 ? 64 : 128;
   auto fits = [&](int64_t slots) { return avail / ((slots * (hd * 4 + 8) + (int64_t)sizeof(Seam)) * a.kv_heads) >= 2; };
+  p.longest_first = a.sequences > 1 && few > 1.0;
   take(c.two.us(keys, few), SequencesPlan::FEW_ROWS, 2, 0, 1);
   take(c.waves.us(keys, few), SequencesPlan::FEW_ROWS, waves, 0, 1);
   if (a.sequences <= 256 && few_parts > 1 && fits(2 * FEW)) take(c.few_shared.us(keys, few), SequencesPlan::FEW_ROWS, 2, few_parts, 1);

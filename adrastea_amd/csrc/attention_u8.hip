@@ -84,7 +84,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
   Args first = arguments();
   early<true, !SHARED>(first);
   const int kv_heads = first.kv_heads, hk = blockIdx.x % kv_heads, wg = blockIdx.x / kv_heads;
-  Roster<ROWS, KEYS, true, SHARED> roster;
+  Roster<ROWS, KEYS, true, SHARED, !SHARED> roster;
   const Line line = roster.line_of(first, threadIdx.x & 63);
   if (wg >= line.parts) {
     if (SHARED && threadIdx.x == 0) arguments().seams[wg * kv_heads + hk].parts = 0;
@@ -509,6 +509,7 @@ static hipError_t launch_blocks(hipStream_t stream, const SequencesArgs& a, cons
   job.page_shift = page_shift(a.page_size);
   job.parts = p.parts, job.shift = p.shift, job.least = p.least;
   job.per_head = 1.0 / a.group;
+  job.longest_first = p.longest_first;
   const int64_t part_rows = (int64_t)(few ? 2 : 1) * p.parts * a.kv_heads * rows;
   job.part_o = (float*)workspace;
   job.part_ml = (float2*)(job.part_o + part_rows * HD);

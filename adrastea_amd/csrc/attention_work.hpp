@@ -73,6 +73,7 @@ struct Job : SequencesArgs {
   float* part_o;    // [slot][key head][ROWS][HD] unnormalised sums
   float2* part_ml;  // [slot][key head][ROWS] (maximum in log2 units, sum)
   struct Seam* seams;  // [parts][key head], of many rows half as many
+  int longest_first;   // Roster's sequences in the order of their keys
 };
 
 // The job is read where it is used, by scalar loads from the kernel's arguments (of which it is the only one): kept in
@@ -366,12 +367,17 @@ constexpr int MANY = 128, MANY_KEYS = 64;
 
 // The sequences on the line, 256 at a time: lane l has sequences base + 64 e + l, read from memory once for the whole
 // division where there are no more.
-template <int ROWS, int KEYS, bool PAGED, bool SHARED>
+//
+// ORDERED, where the job asks for it and there are at most 64: the sequences with the most keys come first.  Unshared blocks that are
+// more than the compute units start in this order, and no long one is the last (64 sequences of 3 to 4000 keys over codes, 512
+// blocks: the units were busy 63 % of the time).
+template <int ROWS, int KEYS, bool PAGED, bool SHARED, bool ORDERED = false>
 struct Roster {
   static constexpr int EACH = 4;
   typedef int each_t __attribute__((ext_vector_type(EACH)));
   each_t row0, rows, key0, keys;
   each_t upto;            // where on the line the sequence ends
+  int which;              // ORDERED: lane l's sequence
   int base, before, end;  // first sequence, and the part of the line that these are
 
   static __device__ __forceinline__ int blocks_of(Args a, int rows) {
@@ -390,6 +396,19 @@ struct Roster {
       if (base + 64 * e < a.sequences && base + 64 * e + lane < a.sequences) {
         const Sequence q = sequence_at(a, base + 64 * e + lane, PAGED);
         row0[e] = q.row0, rows[e] = q.rows, key0[e] = q.key0, keys[e] = q.keys;
+      }
+    }
+    if constexpr (ORDERED) {
+      which = lane;
+      if (a.longest_first && a.sequences <= 64) {
+        // (one number for each: its keys, then its place)
+        const int n = a.sequences, size = min(keys[0], 1 << 24) * 64 + 63 - lane;
+        int rank = 0;
+        for (int i = 0; i < n; i++) rank += __builtin_amdgcn_readlane(size, i) > size;
+        rank = 4 * (lane < n ? rank : lane);
+        auto moved = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_ds_permute(rank, v); };
+        which = moved(lane);
+        row0[0] = moved(row0[0]), rows[0] = moved(rows[0]), key0[0] = moved(key0[0]), keys[0] = moved(keys[0]);
       }
     }
 #pragma unroll
@@ -421,7 +440,7 @@ struct Roster {
       const uint64_t behind = __ballot(upto[e] > place);
       if (behind) {
         const int at = __builtin_ctzll(behind);
-        b.q = {base + 64 * e + at, __builtin_amdgcn_readlane(row0[e], at), __builtin_amdgcn_readlane(rows[e], at),
+        b.q = {ORDERED && e == 0 && base == 0 ? __builtin_amdgcn_readlane(which, at) : base + 64 * e + at, __builtin_amdgcn_readlane(row0[e], at), __builtin_amdgcn_readlane(rows[e], at),
                __builtin_amdgcn_readlane(key0[e], at), __builtin_amdgcn_readlane(keys[e], at)};
         const int blocks = blocks_of(a, b.q.rows), p = pieces_of(b.q.keys, shift);
         const int in = place - (__builtin_amdgcn_readlane(upto[e], at) - blocks * p);

@@ -64,6 +64,7 @@ struct SequencesPlan {
   int shift;  // log2 of the key tiles of a piece of the work
   int least;  // pieces that each workgroup has at least
   int64_t workspace_bytes;
+  bool longest_first = false;  // unshared blocks of few rows: the sequences with the most keys first
 };
 SequencesPlan sequences_plan(const SequencesArgs& a, int cus, int64_t avail);
 hipError_t launch_attention_sequences(hipStream_t stream, const SequencesArgs& a, const SequencesPlan& p,
