@@ -21,7 +21,7 @@ enum Cache { NO_CACHE, F16, U8 };
 
 struct PlaceJob : PlaceArgs {
   int lanes;   // that a head needs, of W
-  uint32_t first;
+  uint32_t first;  // task of the launch
   int splits;  // wavefronts that share a row's heads
 };
 
@@ -521,7 +521,8 @@ struct ReadJob : ReadArgs {
   int items;  // of a row and head, of keys or of values
 };
 
-// A thread to an item: 16 codes (VEC), or one.
+// A thread to an item: 16 codes (VEC), or one.  7364 rows of 8 heads of 128, 46 MB: 14.2 us, 3.2 TB/s, of which start and end are some 4;
+// 64 tokens 4.3.
 template <bool VEC>
 __global__ __launch_bounds__(256) void read_u8_kernel(ReadJob a) {
   const adr_paged_cache_u8& c = a.cache;

@@ -41,7 +41,9 @@ namespace {
 // behind its reads: a wavefront widens all of a tile, 128 instructions, where one that widened a quarter for all four would have half
 // of that and the tile's way through LDS once more.  A lane reads 16 codes of a key at once, for two steps of the product.
 // Scales come for four tiles at a time, one for each wavefront, by transfers of their own: the table's entries, the scales' words, and
-// what is made of them, each a half tile behind the other.
+// what is made of them, each a half tile behind the other.  A piece of 1024 rows over 8025 keys (32 / 8 heads of 128) 163 to 170 us = 770
+// to 740 TFLOP/s, where values in 16 bits take 136 to 146: 24000 vector instructions for each wavefront's 64 tiles, 375 a tile and
+// twice those of 16 bits, busy 64 % of the time beside matrix cores that are busy 36 %.
 template <int HD, bool PAGED, bool SHARED, int GROUPS, bool TREE = false, bool U8 = false>
 __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
   static_assert(PAGED || !U8, "codes are in pages");

@@ -616,7 +616,7 @@ class GpuKernels(CommonKernels):
     tensor of the host (in the reference: one more GpuBuffer held by GpuKernels); matmul_f16 then
     goes through adr_matmul_f16_ws, which may split K over workgroups for products with few
     output tiles and a long K, and attention_f16 through adr_attention_f16_ws, which may share keys
-    over workgroups for few query rows.  The buffer carries nothing between calls; one instance must
+    over workgroups for few query rows, as the attention over several sequences does.  The buffer carries nothing between calls; one instance must
     not be used from streams that run concurrently.  Without it (the default) the library takes such
     a buffer from its own per-stream cache (set_held_workspace_limit)."""
 
@@ -1065,8 +1065,9 @@ def attention_packed_workspace_bytes(batch: PackedBatch, heads: int, kv_heads: i
 
 
 def set_held_workspace_limit(nbytes: int) -> None:
-    """Bytes per buffer of the workspace pool that adr_matmul_f16, adr_matmul_nt_f16, adr_attention_f16, adr_attention_paged_f16 and
-    adr_attention_packed_f16 (and, on request, adr_matmul_nt_fp16u8) draw from, one buffer per (device, stream); 0 switches it off."""
+    """Bytes per buffer of the workspace pool that adr_matmul_f16, adr_matmul_nt_f16, adr_attention_f16, adr_attention_paged_f16,
+    adr_attention_packed_f16, adr_attention_paged_u8, adr_attention_tree_f16 and adr_attention_tree_u8 (and, on request,
+    adr_matmul_nt_fp16u8) draw from, one buffer per (device, stream); 0 switches it off."""
     rc = _ffi.lib().adr_set_held_workspace_limit(int(nbytes))
     if rc != 0:
         raise AdrasteaError(int(rc), "set_held_workspace_limit")

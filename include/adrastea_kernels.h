@@ -622,8 +622,8 @@ int64_t adr_attention_paged_u8_workspace_bytes(adr_paged_cache_u8 cache, adr_pag
  * of its keys, in the same order (adr_append_f16 puts them there, with their depths as `positions`).  Row j of the r of a
  * sequence sees all keys in front of the last r, and of those key i where bit i % 32 of word i / 32 of its bits is set (its
  * ancestors and itself): bits are [rows, words], rows `pitch` words apart, packed like the rows of the queries; tokens beyond
- * 32 * words are not seen.  Otherwise as adr_attention_paged_f16 and adr_attention_paged_u8, whose
- * _workspace_bytes hold for these too.
+ * 32 * words are not seen.  A row whose bits name no drafted token and that has no key in front of it gives zeros.
+ * Otherwise as adr_attention_paged_f16 and adr_attention_paged_u8, whose _workspace_bytes hold for these too.
  */
 typedef struct adr_draft_tree {
   const int32_t* bits;
@@ -688,7 +688,8 @@ int adr_matmul_f16_ws_plan(char* name, int32_t cap, int32_t batches, int32_t m, 
  * attention over several sequences, where the layout is one the matrix-core kernels take (1: a
  * wavefront per row, as for other layouts; blocks of few rows: 2, 3 unshared with two or four
  * wavefronts, 4 shared keys; blocks of many rows: 5, 6 unshared with one or two groups of
- * wavefronts, 7, 8 shared keys; shared keys need a workspace, without one they are unshared).
+ * wavefronts, 7, 8 shared keys; shared keys need a workspace, without one they are unshared;
+ * of keys in 8 bits 3 are eight wavefronts).
  * Unknown ids return ADR_EINVAL_ENUM.
  */
 int adr_debug_knob(int32_t id, int32_t value);
