@@ -202,9 +202,10 @@ __device__ __forceinline__ Slot slot_of_row(const adr_paged_batch& b, int rows, 
 //
 // Memory bounds it, and how many wavefronts ask for it: a wavefront takes 14 us, nearly all of it waiting, so registers are what counts.
 // Angles are read from LDS for every head, weights widened for every head, and a wavefront has one task: kept from head to head, or
-// constants from task to task, they made 127 to 187 registers, two or three wavefronts to a SIMD; now 52, with codes 107.  us, then and
-// now: 7008 rows of 32 / 8 heads of 128 into a cache in 16 bits (172 MB) 44.6, 37.2, 4.6 TB/s, where a copy of as many bytes
-// has 5.2; 7364 rows of them into one in 8 bits (195 MB) 60.2, 48.9; one row of 24 tokens 5.8, 4.7; one token's queries 3.2, 2.7.
+// constants from task to task, they made 127 to 187 registers, two or three wavefronts to a SIMD; now 66, with codes 107.  us, then and
+// now: 7008 rows of 32 / 8 heads of 128 into a cache in 16 bits (172 MB) 44.6, 37.7, 4.6 TB/s, where a copy of as many bytes
+// has 5.2; 7364 rows of 40 / 8 into one in 8 bits (195 MB) 60.2, 47.5, where the vector ALU is busy two thirds of the time as well; 48
+// tokens 5.8, 4.4; one token's queries 3.2, 2.4; 4097 patches of 16 heads of 80 7.8, 7.3.
 template <int CACHE, int W>
 __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
   typedef typename std::conditional<CACHE == U8, double, float>::type angle_t;
@@ -299,27 +300,30 @@ __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
         asm volatile("" : "+v"(w0), "+v"(w1));
         float sum = 0.0f, sum1 = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) sum = fmaf(y[e], y[e], sum), sum1 = fmaf(y[8 + e], y[8 + e], sum1);
+        for (int e = 0; e < 8; e++) sum = fmaf((float)c0[e], (float)c0[e], sum), sum1 = fmaf((float)c1[e], (float)c1[e], sum1);
         sum = !mine ? 0.0f : one ? sum : sum + sum1;
         factor = __builtin_amdgcn_rsqf(fmaf(sum_of<W>(sum), per_value, eps));
 #pragma unroll
-        for (int e = 0; e < 8; e++) y[e] *= (float)w0[e], y[8 + e] *= (float)w1[e];
+        for (int e = 0; e < 8; e++) y[e] = fmaf((float)c0[e], (float)w0[e], 0.0f), y[8 + e] = fmaf((float)c1[e], (float)w1[e], 0.0f);
       }
       const int i = fresh();
+      // (what passes is not mixed with its neighbour, which may be infinite)
+      auto turn = [&](float& u, float& v, int e, bool is_turned) __attribute__((always_inline)) {
+        if (e == 4) asm volatile("" ::: "memory");  // (four at a time: eight are six registers more)
+        const Turn<float> t = rounded[e * W + i];
+        const float x = fmaf(-v, t.sine, u * t.cosine), z = fmaf(v, t.cosine, u * t.sine);
+        u = is_turned ? x : u, v = is_turned ? z : v;
+      };
+      if (a.pairs) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        // (what passes is not mixed with its neighbour, which may be infinite)
-        float& u = y[a.pairs ? 2 * e : e];
-        float& v = y[a.pairs ? 2 * e + 1 : 8 + e];
-        if (e < 4 || !a.pairs ? turn0 : turn1) {
-          const Turn<float> t = rounded[e * W + i];
-          const float x = u * t.cosine, z = u * t.sine;
-          u = fmaf(-v, t.sine, x), v = fmaf(v, t.cosine, z);
-        }
+        for (int e = 0; e < 8; e++) turn(y[2 * e], y[2 * e + 1], e, e < 4 ? turn0 : turn1);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) turn(y[e], y[8 + e], e, turn0);
       }
       half8_t o0, o1;
 #pragma unroll
-      for (int e = 0; e < 8; e++) o0[e] = (half_t)(y[e] * factor), o1[e] = (half_t)((one ? y[e] : y[8 + e]) * factor);
+      for (int e = 0; e < 8; e++) o0[e] = (half_t)fmaf(y[e], factor, 0.0f), o1[e] = (half_t)fmaf(one ? y[e] : y[8 + e], factor, 0.0f);
       store16(to, o0, o1);
     };
     // 16 values as codes, and the head's scale.
