@@ -1,4 +1,4 @@
-"""The checker of step_long.py on the CPU: what a kernel over codes may round passes it, and what it may lose does not."""
+"""The bound of step_long.py on the CPU: what a kernel over codes may round passes it, and what it may lose does not."""
 import pytest
 import torch
 
