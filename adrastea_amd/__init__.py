@@ -11,6 +11,7 @@ from .tensor import TensorLayout, TensorView  # noqa: F401
 from .kernels import (  # noqa: F401
     CommonKernels, GpuKernels, MatmulLoad, MatmulMask, MatmulOptions, MatmulStore, MatmulTracer,
     AdrasteaError, DraftTree, HeadNorm, PackedBatch, PagedBatch, PagedCache, PagedCacheU8, Rotary, RotaryAxes, RotaryLayout,
-    RotaryScaling, rotary_frequencies, attention_paged_u8_workspace_bytes, attention_paged_workspace_bytes, attention_packed_workspace_bytes, set_held_workspace_limit, held_workspace_limit, held_workspace_bytes,
+    RotaryScaling, rotary_frequencies, attention_paged_u8_workspace_bytes, attention_paged_workspace_bytes, attention_packed_workspace_bytes,
+    attention_tree_workspace_bytes, set_held_workspace_limit, held_workspace_limit, held_workspace_bytes,
     held_workspace_declined, release_held_workspace, set_u8_dequantise_first,
 )

@@ -26,6 +26,7 @@ SYMBOLS = (
     "adr_norm_rotary_f16", "adr_append_norm_f16", "adr_append_u8", "adr_read_u8",
     "adr_attention_paged_u8", "adr_attention_paged_u8_ws", "adr_attention_paged_u8_workspace_bytes",
     "adr_attention_tree_f16", "adr_attention_tree_f16_ws", "adr_attention_tree_u8", "adr_attention_tree_u8_ws",
+    "adr_attention_tree_f16_workspace_bytes", "adr_attention_tree_u8_workspace_bytes",
     "adr_debug_knob", "adr_microbench_empty", "adr_microbench_mfma_f16", "adr_microbench_stream_read",
     "adr_strerror", "adr_abi_version",
 )
@@ -184,6 +185,9 @@ def lib():
     L.adr_attention_paged_f16_workspace_bytes.restype = C.c_int64
     L.adr_attention_packed_f16_workspace_bytes.restype = C.c_int64
     L.adr_attention_paged_u8_workspace_bytes.restype = C.c_int64
+    L.adr_attention_tree_f16_workspace_bytes.argtypes = [cache, batch, i32, i32]
+    L.adr_attention_tree_u8_workspace_bytes.argtypes = [codes, batch, i32, i32]
+    L.adr_attention_tree_f16_workspace_bytes.restype = L.adr_attention_tree_u8_workspace_bytes.restype = C.c_int64
     L.adr_held_workspace_limit.restype = C.c_int64
     L.adr_held_workspace_bytes.restype = C.c_int64
     L.adr_held_workspace_declined.restype = C.c_int64

@@ -1081,10 +1081,7 @@ int64_t adr_attention_paged_f16_workspace_bytes(adr_paged_cache cache, adr_paged
   bool nothing;
   if (int rc = paged_args(a, cache, batch, heads, rows, &nothing)) return rc;
   a.so_x = a.sq_x = 1;
-  if (nothing) return 0;
-  const int64_t bytes = sequences_plan(a, device_info_for_plan().cus, INT64_MAX).workspace_bytes;
-  a.mask = MASK_TREE;  // (of a draft that may be one)
-  return std::max(bytes, sequences_plan(a, device_info_for_plan().cus, INT64_MAX).workspace_bytes);
+  return nothing ? 0 : sequences_plan(a, device_info_for_plan().cus, INT64_MAX).workspace_bytes;
 }
 
 int adr_attention_packed_f16(adr_stream_t stream, uint16_t* output, const uint16_t* query, const uint16_t* key,
@@ -1271,6 +1268,19 @@ int64_t adr_attention_paged_u8_workspace_bytes(adr_paged_cache_u8 cache, adr_pag
   if (int rc = paged_args(a, cache, batch, heads, rows, &nothing)) return rc;
   a.so_x = a.sq_x = 1;
   return nothing ? 0 : sequences_u8_plan(a, device_info_for_plan().cus, INT64_MAX).workspace_bytes;
+}
+
+int64_t adr_attention_tree_f16_workspace_bytes(adr_paged_cache cache, adr_paged_batch batch, int32_t heads, int32_t rows) {
+  SequencesArgs a = {};
+  bool nothing;
+  if (int rc = paged_args(a, cache, batch, heads, rows, &nothing)) return rc;
+  a.so_x = a.sq_x = 1, a.mask = MASK_TREE;
+  return nothing ? 0 : sequences_plan(a, device_info_for_plan().cus, INT64_MAX).workspace_bytes;
+}
+
+// (the same kernels, whatever the mask)
+int64_t adr_attention_tree_u8_workspace_bytes(adr_paged_cache_u8 cache, adr_paged_batch batch, int32_t heads, int32_t rows) {
+  return adr_attention_paged_u8_workspace_bytes(cache, batch, heads, rows);
 }
 
 #define ADR_TREE_ENTRIES(suffix, cache_t)                                                                                        \

@@ -1055,6 +1055,17 @@ def attention_paged_u8_workspace_bytes(cache: PagedCacheU8, batch: PagedBatch, h
     return int(n)
 
 
+def attention_tree_workspace_bytes(cache, batch: PagedBatch, heads: int, rows: int) -> int:
+    """Scratch bytes adr_attention_tree_f16_ws, or of a PagedCacheU8 adr_attention_tree_u8_ws, would use for `rows` packed drafted
+    tokens of `heads` query heads (0: it would share no keys)."""
+    _int32("heads and rows", heads, rows)
+    name = "adr_attention_tree_u8_workspace_bytes" if isinstance(cache, PagedCacheU8) else "adr_attention_tree_f16_workspace_bytes"
+    n = getattr(_ffi.lib(), name)(cache._desc, batch._desc, heads, rows)
+    if n < 0:
+        raise AdrasteaError(int(n), name[4:])
+    return int(n)
+
+
 def attention_packed_workspace_bytes(batch: PackedBatch, heads: int, kv_heads: int, rows: int, keys: int, d: int) -> int:
     """Scratch bytes adr_attention_packed_f16_ws would use for these sizes (0: it would share no keys)."""
     _int32("heads, rows and keys", heads, kv_heads, rows, keys, d)

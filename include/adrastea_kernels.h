@@ -623,7 +623,7 @@ int64_t adr_attention_paged_u8_workspace_bytes(adr_paged_cache_u8 cache, adr_pag
  * sequence sees all keys in front of the last r, and of those key i where bit i % 32 of word i / 32 of its bits is set (its
  * ancestors and itself): bits are [rows, words], rows `pitch` words apart, packed like the rows of the queries; tokens beyond
  * 32 * words are not seen.  A row whose bits name no drafted token and that has no key in front of it gives zeros.
- * Otherwise as adr_attention_paged_f16 and adr_attention_paged_u8, whose _workspace_bytes hold for these too.
+ * Otherwise as adr_attention_paged_f16 and adr_attention_paged_u8.
  */
 typedef struct adr_draft_tree {
   const int32_t* bits;
@@ -645,6 +645,8 @@ int adr_attention_tree_u8_ws(adr_stream_t stream, uint16_t* output, const uint16
                              adr_paged_batch batch, adr_draft_tree tree, int32_t heads, int32_t rows, int32_t stride_ox,
                              int32_t stride_oy, int32_t stride_oz, int32_t stride_qx, int32_t stride_qy, int32_t stride_qz,
                              float scale, float temp, void* workspace, int64_t workspace_bytes);
+int64_t adr_attention_tree_f16_workspace_bytes(adr_paged_cache cache, adr_paged_batch batch, int32_t heads, int32_t rows);
+int64_t adr_attention_tree_u8_workspace_bytes(adr_paged_cache_u8 cache, adr_paged_batch batch, int32_t heads, int32_t rows);
 
 /*
  * Diagnostics (no counterpart in the reference).

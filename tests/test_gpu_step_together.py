@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from adrastea_amd import (attention_paged_u8_workspace_bytes, DraftTree, GpuKernels, HeadNorm, MatmulMask, PagedBatch, PagedCache, PagedCacheU8,
+from adrastea_amd import (attention_paged_u8_workspace_bytes, attention_tree_workspace_bytes, DraftTree, GpuKernels, HeadNorm, MatmulMask, PagedBatch, PagedCache, PagedCacheU8,
                           RotaryAxes, TensorLayout, TensorView, _ffi, rotary_frequencies)
 import sequences_reference as ref
 import step_reference as step
@@ -471,6 +471,23 @@ def test_workspace_bytes(seqs):
         assert torch.equal(got, want)
     for part in (nbytes // 2, nbytes // 7, 64):
         run(GpuKernels(workspace_bytes=part))
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("rows,past", [([8], [5000]), ([61], [2100]), ([100, 3], [3000, 40])])
+def test_workspaces_of_trees(rows, past, bits):
+    """As above: the same bits with what is reported as through the pool; with less still right."""
+    lib, rng = _ffi.lib(), np.random.default_rng(4)
+    t = Drafts([random_parents(r, rng) for r in rows], past, 8, 2, 128, 16, bits, seed=67)
+    want, nbytes = t.want(0.1), attention_tree_workspace_bytes(t.cache, t.batch, 8, t.rows)
+    assert nbytes > 0
+    lib.adr_set_held_workspace_limit(_ffi.HELD_WORKSPACE_DEFAULT_BYTES)
+    pool = t.run(GpuKernels(), 0.1).copy()
+    lib.adr_set_held_workspace_limit(0)
+    t.check(pool, want)
+    assert np.array_equal(t.run(GpuKernels(workspace_bytes=nbytes), 0.1), pool)
+    for part in (nbytes // 2, nbytes // 7, 64):
+        t.check(t.run(GpuKernels(workspace_bytes=part), 0.1), want)
 
 
 def test_calls_allocate_nothing():

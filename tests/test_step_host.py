@@ -143,6 +143,15 @@ def test_workspace_arguments_are_checked():
         assert want >= 0 and lib.adr_attention_paged_u8_workspace_bytes(codes(pages=10000, **none), unknown, heads, rows) == want
 
 
+def test_workspaces_of_trees():
+    lib = _ffi.lib()
+    for call, c in ((lib.adr_attention_tree_f16_workspace_bytes, cache), (lib.adr_attention_tree_u8_workspace_bytes, codes)):
+        assert call(c(), batch(), 3, 5) == SHAPE and call(c(kv_heads=-2), batch(), 4, 5) == SHAPE and call(c(), batch(), 4, 0) == 0
+        wide = dict(sequences=1, table_width=2000, table_pitch=2000)
+        assert call(c(pages=10000), batch(**wide), 32, 8) > 0          # (a long context's keys are shared)
+        assert call(c(pages=10000), batch(sequences=1, table_width=1, table_pitch=1), 32, 8) == 0
+
+
 def test_handles_check_types():
     with pytest.raises(AssertionError):
         HeadNorm(torch.ones(4))
