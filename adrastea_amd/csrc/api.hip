@@ -1125,7 +1125,8 @@ namespace {
 int validate_axes(const adr_rotary_axes& r, int32_t d, const int32_t* positions, int32_t pitch, int32_t rows) {
   if (int rc = validate_rotary(adr_rotary{r.turns, r.dims, r.layout, r.magnitude}, d)) return rc;
   if (r.axes < 1 || r.axes > ADR_ROTARY_MAX_AXES) return ADR_EINVAL_SHAPE;
-  return positions && r.axes > 1 && pitch < rows ? ADR_EINVAL_SHAPE : ADR_OK;
+  // (0: one row of positions for every axis)
+  return positions && r.axes > 1 && pitch != 0 && pitch < rows ? ADR_EINVAL_SHAPE : ADR_OK;
 }
 
 bool eps_fits(const adr_head_norm& n) { return !n.weight || (n.eps >= 0.0f && n.eps <= 3.402823466e38f); }

@@ -142,7 +142,7 @@ struct PagedCacheU8 {
 };
 
 // What a step appends: its keys and values, its queries with the view that they are turned into (both null: none), the positions on
-// each axis (device memory, `pitch` entries from axis to axis; null: the places in the cache), the rotation and the norms.
+// each axis (device memory, `pitch` entries from axis to axis, 0: the same for all; null: the places in the cache), the rotation and the norms.
 struct Appended {
   TensorView<const f16> key, value;
   RotaryAxes rotary{nullptr, nullptr, 0, ADR_ROTARY_HALVES, 1.0f, 1};

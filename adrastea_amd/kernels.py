@@ -343,7 +343,7 @@ def _norm_desc(norm: Optional[HeadNorm], d: int) -> _ffi.HeadNormDesc:
 
 
 def _axis_positions(positions, axes: int, rows: int):
-    """Address and pitch of positions [axes, rows], or [rows] for one axis."""
+    """Address and pitch of positions [axes, rows], or [rows] for one axis.  (Of positions that are expanded over the axes 0.)"""
     rank = positions.dim()
     assert rank == 2 or (rank == 1 and axes == 1), "positions: [axes, rows]"
     shape = _index(positions, rank, "positions").shape

@@ -534,7 +534,8 @@ int64_t adr_attention_packed_f16_workspace_bytes(adr_packed_batch batch, int32_t
  * memory, [dims / 2], entries outside 0 .. axes - 1 count as 0; null: all pairs follow the first axis.  How the pairs are
  * divided, and whether each axis has frequencies of its own, is in `axis` and `turns`.
  *
- * adr_norm_rotary_f16: as adr_rotary_f16, with both; positions [axes][positions_pitch], of which `rows` entries each are used.
+ * adr_norm_rotary_f16: as adr_rotary_f16, with both; positions [axes][positions_pitch], of which `rows` entries each are used.  A pitch of
+ * 0: the same entries for every axis, as rows of text have them; other pitches are `rows` at least (ADR_EINVAL_SHAPE).
  * adr_append_norm_f16: as adr_append_f16, with both: `query_norm` for the queries, `key_norm` for the keys, values as they are.
  * Without `positions` every axis is at the row's place in the cache.  32-bit arithmetic (angles in 64), one rounding.
  */
