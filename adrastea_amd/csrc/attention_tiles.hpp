@@ -37,7 +37,7 @@ namespace {
 // rows that the mask hides, compute of a tile is in the time and not in the operations).  HD = 128 keeps 24 to 38 vector registers
 // in scratch memory at those beginnings and ends, none in the loop; HD = 64 none.
 //
-// U8: the cache is one of codes (attention_u8.hip, which explains the arithmetic).  They lie in LDS as they come and are widened
+// U8: the cache is one of codes (attention_u8.hip, which explains the arithmetic, and why probabilities have 11 bits here and 22 in few rows).  They lie in LDS as they come and are widened
 // behind its reads: a wavefront widens all of a tile, 128 instructions, where one that widened a quarter for all four would have half
 // of that and the tile's way through LDS once more.  A lane reads 16 codes of a key at once, for two steps of the product.
 // Scales come for four tiles at a time, one for each wavefront, by transfers of their own: the table's entries, the scales' words, and

@@ -5,8 +5,13 @@
 // The matrix cores are given the codes as they are: a byte, widened, is the fp16 number c 2^-24, exact, and below the normal
 // numbers, which are not flushed.  So scores are 32-bit sums of exact products that begin at -127.5 sum(q) and are multiplied by the
 // key's scale once; a value's scale goes into the probability, the only thing that is rounded, and 127.5 times the sum of the
-// rounded probabilities (one more product, with ones) is taken off at the end.  (With values rounded to fp16 the results of a batch of
-// tokens were 0.00033 off in the mean, of their root mean square, now 0.00027, where the last rounding to fp16 alone is 0.00021.)
+// rounded probabilities (one more product, with ones) is taken off at the end.
+//
+// Few rows round it to two fp16 numbers, the second what the first leaves: 22 bits.  Results are then off by 0.00021 of their root mean
+// square, which is the last rounding to fp16; with one number it was 0.00025 to 0.00032.  The matrix cores have room for the second
+// product (us, with one -> with both: a batch of tokens 50.9 -> 51.2, long contexts 201.0 -> 202.1, one user 11.5 -> 11.7, drafts 44.5 ->
+// 44.9).  Many rows round it to one: 0.00028, as values in 16 bits have it.  The loop has no registers for the other, which goes
+// through scratch: a prompt's piece 167 -> 274 us, one user's draft 26.8 -> 35.5.
 //
 // What is kept within fp16's range is thus the probability times the value's scale: a row's reference follows the largest
 // s c + log2 vs, as attention_sequences.hip says of s c, with vs taken as 2^-25 where it is less (a key of such values may have
@@ -332,7 +337,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
 #pragma unroll
     for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) s[kb][r] *= (float)ks[kb][r];
+      for (int r = 0; r < 4; r++) s[kb][r] = fmaf(s[kb][r], (float)ks[kb][r], 0.0f);  // (one instruction, with the scale as it is)
     if (key0 + KEYS > common_end) {  // keys that some row does not see
       const int left = end - key0;   // of this lane's row from its first one on
       uint32_t seen = ~0u;
@@ -362,26 +367,33 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
       for (int db = 0; db < DB; db++) o[db] *= alpha;
     }
     float sum[2] = {0.0f, 0.0f};
-    u32x4_t pf;
+    u32x4_t pf, rest;
 #pragma unroll
     for (int kb = 0; kb < 2; kb++)
 #pragma unroll
       for (int r = 0; r < 4; r += 2) {
-        float2_t e;
+        float2_t e, p;  // (and what rounding takes off p, by one instruction: the product once more, less the rounded one)
 #pragma unroll
         for (int j = 0; j < 2; j++) {
           e[j] = __builtin_amdgcn_exp2f(fmaf(s[kb][r + j], c, -m_run));
           sum[j] += e[j];
-          e[j] *= (float)vs[kb][r + j];
+          p[j] = fmaf(e[j], (float)vs[kb][r + j], 0.0f);
         }
-        pf[kb * 2 + r / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(e, half2_t));
+        const half2_t h = __builtin_convertvector(p, half2_t);
+#pragma unroll
+        for (int j = 0; j < 2; j++) p[j] = fmaf(e[j], (float)vs[kb][r + j], -(float)h[j]);
+        pf[kb * 2 + r / 2] = __builtin_bit_cast(uint32_t, h);
+        rest[kb * 2 + r / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, half2_t));
       }
     l_run += sum[0] + sum[1];
     ones = __builtin_amdgcn_mfma_f32_16x16x32_f16(all_ones, __builtin_bit_cast(half8_t, pf), ones, 0, 0, 0);
+    ones = __builtin_amdgcn_mfma_f32_16x16x32_f16(all_ones, __builtin_bit_cast(half8_t, rest), ones, 0, 0, 0);
 #pragma unroll
-    for (int db = 0; db < DB; db++)
-      o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(widened((uint32_t)vc[db][0], (uint32_t)vc[db][1]),
-                                                     __builtin_bit_cast(half8_t, pf), o[db], 0, 0, 0);
+    for (int db = 0; db < DB; db++) {
+      const half8_t v = widened((uint32_t)vc[db][0], (uint32_t)vc[db][1]);
+      o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, __builtin_bit_cast(half8_t, pf), o[db], 0, 0, 0);
+      o[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, __builtin_bit_cast(half8_t, rest), o[db], 0, 0, 0);
+    }
   };
   const std::true_type yes{};
   const std::false_type no{};
