@@ -9,7 +9,7 @@
 //
 // Few rows round it to two fp16 numbers, the second what the first leaves: 22 bits.  Results are then off by 0.00021 of their root mean
 // square, which is the last rounding to fp16; with one number it was 0.00025 to 0.00032.  The matrix cores have room for the second
-// product (us, with one -> with both: a batch of tokens 50.9 -> 51.2, long contexts 201.0 -> 202.1, one user 11.5 -> 11.7, drafts 44.5 ->
+// product (us, with one -> with both: a batch of tokens 51.3 -> 52.0, long contexts 200.9 -> 202.1, one user 11.5 -> 11.7, drafts 44.3 ->
 // 44.9).  Many rows round it to one: 0.00028, as values in 16 bits have it.  The loop has no registers for the other, which goes
 // through scratch: a prompt's piece 167 -> 274 us, one user's draft 26.8 -> 35.5.
 //
@@ -495,9 +495,12 @@ SequencesPlan sequences_u8_plan(const SequencesArgs& a, int cus, int64_t avail) 
                               {6.8, 20, 1.6, 3.4, 6.6}, {7.7, 14, 1.4, 7.2, 9.1}, {9.7, 1.3, 0.013}, {9.9, 1.5, 0.017}, 0.85, 1.4, 0.012};
   static const Costs of_128 = {{6.8, 18, 4.0, 1.7, 3.7}, {7.4, 6.2, 2.7, 6.1, 5.5}, {8.3, 1.7, 11, 1.1, 8.3},
                                {8.6, 26, 3.4, 4.3, 6.5}, {10, 20, 2.7, 8.8, 13}, {12, 0.99, 0.02}, {12, 1.1, 0.025}, 1.4, 2.6, 0.018};
-  // Shared few rows: as many workgroups as fit the LDS.
+  // Shared few rows: as many workgroups as a unit holds at once, six of heads up to 64 by their 150 registers (three wavefronts to a SIMD), four of
+  // 128 by their LDS.  Stretches are equal, and more workgroups are a second round.  us, six and eight of heads of 64: eight sequences
+  // of 20000 to 40000 keys (20 / 20) 118, 132; 40 of 500 to 8000 (32 / 4) 29, 35; one of 30000 (12 / 12) 19, 25.  Four and six of 128: eight
+  // (40 / 8) 92, 109.
   SequencesPlan p = {SequencesPlan::FEW_ROWS, 2, 0, 0, 1, 0};
-  plan_by_cost(p, a, cus, avail, few_blocks, blocks_of(MANY), longest, 8, std::max(1, (hd == 64 ? 8 : 4) * cus / a.kv_heads),
+  plan_by_cost(p, a, cus, avail, few_blocks, blocks_of(MANY), longest, 8, std::max(1, (hd == 64 ? 6 : 4) * cus / a.kv_heads),
                hd == 64 ? of_64 : of_128);
   if (forced) p.kind = forced <= 4 ? SequencesPlan::FEW_ROWS : SequencesPlan::TILES;
   const bool few = p.kind == SequencesPlan::FEW_ROWS;
