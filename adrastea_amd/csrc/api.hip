@@ -2,6 +2,7 @@
 // Declarations and the reference interface each one replaces: include/adrastea_kernels.h.
 #include <string.h>
 
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 
@@ -1129,6 +1130,9 @@ int validate_axes(const adr_rotary_axes& r, int32_t d, const int32_t* positions,
   return positions && r.axes > 1 && pitch != 0 && pitch < rows ? ADR_EINVAL_SHAPE : ADR_OK;
 }
 
+// (The kernels' reciprocal square root takes what is below the normal numbers for 0.  A mean of squares of fp16 numbers is 2^-57 at least
+// where it is not 0, so that 2^-126 in the place of a smaller eps is the same sum.)
+float eps_of(const adr_head_norm& n) { return n.eps > 0.0f ? std::max(n.eps, 0x1p-126f) : 0.0f; }
 bool eps_fits(const adr_head_norm& n) { return !n.weight || (n.eps >= 0.0f && n.eps <= 3.402823466e38f); }
 
 void set_turns(PlaceArgs& a, const adr_rotary_axes& r, const int32_t* positions, int32_t pitch) {
@@ -1169,8 +1173,8 @@ int append_normed(adr_stream_t stream, const Cache& cache, PlaceArgs& a, const a
   a.sk_x = k[0], a.sk_y = k[1], a.sk_z = k[2];
   a.sv_x = v[0], a.sv_y = v[1], a.sv_z = v[2];
   set_turns(a, rotary, positions, positions_pitch);
-  if (query) a.q_weight = (const half_t*)query_norm.weight, a.q_eps = query_norm.eps;
-  a.k_weight = (const half_t*)key_norm.weight, a.k_eps = key_norm.eps;
+  if (query) a.q_weight = (const half_t*)query_norm.weight, a.q_eps = eps_of(query_norm);
+  a.k_weight = (const half_t*)key_norm.weight, a.k_eps = eps_of(key_norm);
   a.heads = query ? heads : 0, a.kv_heads = cache.kv_heads, a.rows = rows, a.d = cache.d;
   a.batch = batch;
   return (int)launch_place((hipStream_t)stream, a);
@@ -1195,7 +1199,7 @@ int adr_norm_rotary_f16(adr_stream_t stream, uint16_t* output, const uint16_t* i
   a.so_x = stride_ox, a.so_y = stride_oy, a.so_z = stride_oz;
   a.sq_x = stride_ix, a.sq_y = stride_iy, a.sq_z = stride_iz;
   set_turns(a, rotary, positions, positions_pitch);
-  a.q_weight = (const half_t*)norm.weight, a.q_eps = norm.eps;
+  a.q_weight = (const half_t*)norm.weight, a.q_eps = eps_of(norm);
   a.heads = heads, a.rows = rows, a.d = d;
   return (int)launch_place((hipStream_t)stream, a);
 }
