@@ -577,16 +577,18 @@ __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
       }
     }
     if constexpr (MAX) {
-      if (__builtin_amdgcn_ballot_w64(mx > m_run + MOST) != 0) {
+      // (codes, every 16th tile as well: the offset of what is summed so far is taken off it, as attention_u8.hip says)
+      if (__builtin_amdgcn_ballot_w64(mx > m_run + MOST) != 0 || (U8 && (i & 15) == 15)) {
         const float m_new = fmaxf(m_run, mx - BELOW);
         const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
         m_run = m_new;
         l_run *= alpha;
-        if constexpr (U8) sum_of_p *= alpha;
+        float offset = 0.0f;
+        if constexpr (U8) offset = pair_sum(sum_of_p) * (127.5f * WIDENED) * alpha, sum_of_p = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-          for (int r = 0; r < 16; r++) o[dt][r] *= alpha;
+          for (int r = 0; r < 16; r++) o[dt][r] = U8 ? fmaf(o[dt][r], alpha, -offset) : o[dt][r] * alpha;
       }
     }
     advance(nk, is_k);
