@@ -135,18 +135,9 @@ struct Slot {
   int page, slot; // page -1: in no page of the cache
 };
 
-// The sequences of rows first ... last, of which each lane has one, at most a lane's worth of them: one search for the first, and the
-// 64 offsets from there on decide for the others.
-__device__ __forceinline__ Slot slot_of(const adr_paged_batch& b, int rows, int pages, int page_size, int first, int last, int row, int lane) {
-  const int s0 = sequence_of_row(b.row_offsets, b.sequences, first, lane);
-  const int ahead = s0 + lane < b.sequences ? b.row_offsets[s0 + lane] : 0x7fffffff;
-  int s = s0;
-  for (int r = first; r <= last; r++) {
-    const int n = __popcll(__ballot(ahead <= r));
-    const int at = n < 64 ? s0 + max(n, 1) - 1 : sequence_of_row(b.row_offsets, b.sequences, r, lane);
-    if (row == r) s = at;
-  }
-  const int begin = clamp_to(b.row_offsets[s], rows), end = clamp_to(b.row_offsets[s + 1], rows), length = b.lengths[s];
+// Of a row of sequence s, whose rows and keys the batch says to be these.
+__device__ __forceinline__ Slot slot_in(const adr_paged_batch& b, int rows, int pages, int page_size, int row, int s, int begin, int end, int length) {
+  begin = clamp_to(begin, rows), end = clamp_to(end, rows);
   Slot p = {row, 0, -1, 0};
   if (row < begin || row >= end) {
     p.row = -1;
@@ -162,6 +153,20 @@ __device__ __forceinline__ Slot slot_of(const adr_paged_batch& b, int rows, int 
   return p;
 }
 
+// The sequences of rows first ... last, of which each lane has one, at most a lane's worth of them: one search for the first, and the
+// 64 offsets from there on decide for the others.
+__device__ __forceinline__ Slot slot_of(const adr_paged_batch& b, int rows, int pages, int page_size, int first, int last, int row, int lane) {
+  const int s0 = sequence_of_row(b.row_offsets, b.sequences, first, lane);
+  const int ahead = s0 + lane < b.sequences ? b.row_offsets[s0 + lane] : 0x7fffffff;
+  int s = s0;
+  for (int r = first; r <= last; r++) {
+    const int n = __popcll(__ballot(ahead <= r));
+    const int at = n < 64 ? s0 + max(n, 1) - 1 : sequence_of_row(b.row_offsets, b.sequences, r, lane);
+    if (row == r) s = at;
+  }
+  return slot_in(b, rows, pages, page_size, row, s, b.row_offsets[s], b.row_offsets[s + 1], b.lengths[s]);
+}
+
 // The same of one row, by a wavefront.  Up to 63 sequences are known by one way to memory.
 __device__ __forceinline__ Slot slot_of_row(const adr_paged_batch& b, int rows, int pages, int page_size, int row, int lane) {
   int s, begin, end, length;
@@ -174,20 +179,7 @@ __device__ __forceinline__ Slot slot_of_row(const adr_paged_batch& b, int rows, 
     s = uniform(sequence_of_row(b.row_offsets, b.sequences, row, lane));
     begin = b.row_offsets[s], end = b.row_offsets[s + 1], length = b.lengths[s];
   }
-  begin = clamp_to(begin, rows), end = clamp_to(end, rows);
-  Slot p = {row, 0, -1, 0};
-  if (row < begin || row >= end) {
-    p.row = -1;
-    return p;
-  }
-  const int64_t x = (int64_t)length - end + row;
-  p.position = (int)x;
-  if (x >= 0 && x < (int64_t)b.table_width * page_size) {
-    const int at = (int)x / page_size, page = b.table[(int64_t)s * b.table_pitch + at];
-    p.slot = (int)x - at * page_size;
-    p.page = page >= 0 && page < pages ? page : -1;
-  }
-  return p;
+  return slot_in(b, rows, pages, page_size, row, s, begin, end, length);
 }
 
 // ---- 16 bytes at a time -------------------------------------------------------------------------------------
