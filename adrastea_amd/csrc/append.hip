@@ -194,10 +194,10 @@ __device__ __forceinline__ Slot slot_of_row(const adr_paged_batch& b, int rows, 
 //
 // Memory bounds it, and how many wavefronts ask for it: a wavefront takes 14 us, nearly all of it waiting, so registers are what counts.
 // Angles are read from LDS for every head, weights widened for every head, and a wavefront has one task: kept from head to head, or
-// constants from task to task, they made 127 to 187 registers, two or three wavefronts to a SIMD; now 66, with codes 107.  us, then and
-// now: 7008 rows of 32 / 8 heads of 128 into a cache in 16 bits (172 MB) 44.6, 37.7, 4.6 TB/s, where a copy of as many bytes
-// has 5.2; 7364 rows of 40 / 8 into one in 8 bits (195 MB) 60.2, 47.5, where the vector ALU is busy two thirds of the time as well; 48
-// tokens 5.8, 4.4; one token's queries 3.2, 2.4; 4097 patches of 16 heads of 80 7.8, 7.3.
+// constants from task to task, they made 127 to 187 registers, two or three wavefronts to a SIMD; now 74, six wavefronts, and with codes 107,
+// four.  us, then and now: 7008 rows of 32 / 8 heads of 128 into a cache in 16 bits (172 MB) 44.6, 38.2, 4.5 TB/s, where a copy of as many
+// bytes has 5.2; 7364 rows of 40 / 8 into one in 8 bits (195 MB) 60.2, 47.9, where the vector ALU is busy 59 % of the time as well; 48
+// tokens 5.8, 4.3; one token's queries 3.2, 2.5; 4097 patches of 16 heads of 80 7.8, 6.8.
 template <int CACHE, int W>
 __global__ __launch_bounds__(256) void place_kernel(PlaceJob a) {
   typedef typename std::conditional<CACHE == U8, double, float>::type angle_t;
@@ -517,8 +517,9 @@ struct ReadJob : ReadArgs {
   int items;  // of a row and head, of keys or of values
 };
 
-// A thread to an item: 16 codes (VEC), or one.  7364 rows of 8 heads of 128, 46 MB: 14.2 us, 3.2 TB/s, of which start and end are some 4;
-// 64 tokens 4.3.
+// A thread to an item: 16 codes (VEC), or one.  7364 rows of 8 heads of 128, 46 MB: 14.2 us, 3.2 TB/s, of which start and end are some 4; 64
+// tokens 4.3.  Before its codes a wavefront goes to memory four times, one after the other (the search, offsets, length, table), for 1 KB of
+// them; the vector ALU is busy 68 % of the time.
 template <bool VEC>
 __global__ __launch_bounds__(256) void read_u8_kernel(ReadJob a) {
   const adr_paged_cache_u8& c = a.cache;

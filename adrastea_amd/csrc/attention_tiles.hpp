@@ -34,16 +34,19 @@ namespace {
 // bound by their beginnings and ends: us of a block among others, 2.0 from the end of one to the start of the next in its place,
 // 1.4 to find its sequence, 1.7 for addresses, 1.8 until the first keys are there, 1.9 a tile, 2.4 for the results.  Nine prompts
 // of 100 to 3996 rows, 25 tiles a block in the mean, 447 to 477 us = 933 to 874 TFLOP/s (what wavefronts whose rows end early, and
-// rows that the mask hides, compute of a tile is in the time and not in the operations).  HD = 128 keeps 24 to 38 vector registers
-// in scratch memory at those beginnings and ends, none in the loop; HD = 64 none.
+// rows that the mask hides, compute of a tile is in the time and not in the operations).  HD = 128 keeps 24 to 40 vector registers
+// in scratch memory at those beginnings and ends, none in the loop; HD = 64 none.  With trees 37 to 45, 4 to 10 of them in the loop, where a
+// row's bits are looked at.
 //
-// U8: the cache is one of codes (attention_u8.hip, which explains the arithmetic, and why probabilities have 11 bits here and 22 in few rows).  They lie in LDS as they come and are widened
-// behind its reads: a wavefront widens all of a tile, 128 instructions, where one that widened a quarter for all four would have half
-// of that and the tile's way through LDS once more.  A lane reads 16 codes of a key at once, for two steps of the product.
-// Scales come for four tiles at a time, one for each wavefront, by transfers of their own: the table's entries, the scales' words, and
-// what is made of them, each a half tile behind the other.  A piece of 1024 rows over 8025 keys (32 / 8 heads of 128) 163 to 170 us = 770
-// to 740 TFLOP/s, where values in 16 bits take 136 to 146: 24000 vector instructions for each wavefront's 64 tiles, 375 a tile and
-// twice those of 16 bits, busy 64 % of the time beside matrix cores that are busy 36 %.
+// U8: the cache is one of codes (attention_u8.hip, which explains the arithmetic, and why probabilities have 11 bits here and 22 in few
+// rows).  They lie in LDS as they come and are widened behind its reads: a wavefront widens all of a tile, 128 instructions, where one that
+// widened a quarter for all four would have half of that and the tile's way through LDS once more.  A lane reads 16 codes of a key at once, for
+// two steps of the product.  Scales come for four tiles at a time, one for each wavefront, by transfers of their own: the table's entries, the
+// scales' words, and what is made of them, each a half tile behind the other.  A piece of 1024 rows over 8025 keys (32 / 8 heads of 128) 163 to
+// 170 us = 770 to 740 TFLOP/s, where values in 16 bits take 136 to 146: 425 vector instructions for each of a wavefront's tiles (25100 for 59, starts and
+// ends among them), the vector ALU busy 64 % of the time beside matrix cores that are busy 36 %.  HD = 128 keeps 40 to 64 vector registers in
+// scratch, none in the loop; with trees 56 to 70, some 40 of them in the loop over two tiles, where bits are looked at; HD = 64 none, or with
+// trees and shared keys nine words.
 template <int HD, bool PAGED, bool SHARED, int GROUPS, bool TREE = false, bool U8 = false>
 __global__ __launch_bounds__(256 * GROUPS, 2) void attention_tiles_kernel(Job) {
   static_assert(PAGED || !U8, "codes are in pages");

@@ -71,12 +71,12 @@ __device__ __forceinline__ Scales read_scales(const half_t* p, int64_t step, boo
 // A block of 16 rows against its keys, as attention_few_rows_kernel: tiles of 32 keys, two of each wavefront's in LDS.  A tile's
 // codes go from LDS to registers as they are, values through the transposing read of bytes, and become fp16 there.
 //
-// Long contexts are bound by memory: eight sequences of 50000 to 110000 keys (40 / 8 heads of 128, 1.22 GB) 193 us, 6.3 TB/s.
+// Long contexts are bound by memory: eight sequences of 50000 to 110000 keys (40 / 8 heads of 128, 1.22 GB) 195 us, 6.2 TB/s.
 // One wavefront alone takes 1.1 to 1.3 us a tile, so that blocks get eight where they
-// are few: one of 777 keys (32 / 32 heads) 11.6 us, with four 12.7, with two 14.1.  64 sequences of 3 to 4000 keys (32 / 8, 251 MB)
-// 51.8: a unit has two blocks one after the other, each with some 8 us before its first tile and behind its last, in which nothing
+// are few: one of 777 keys (32 / 32 heads) 11.7 us, with four 12.7, with two 14.1.  64 sequences of 3 to 4000 keys (32 / 8, 251 MB)
+// 51.5: a unit has two blocks one after the other, each with some 8 us before its first tile and behind its last, in which nothing
 // else is on its way there (four wavefronts, two blocks beside each other, 56; two 85).  24 drafts of 2 to 13 tokens over up to 6000 keys
-// 45.5 (longest sequences first; in the batch's order 59.5).
+// 44.8 (longest sequences first; in the batch's order 59.5).
 constexpr int FEW_AHEAD = 8;
 constexpr int few_bytes(int hd) { return 4 * FEW_KEYS * hd + 3 * 2 * FEW_AHEAD * FEW_KEYS * 2; }  // of LDS, a wavefront
 
