@@ -403,7 +403,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attention_u8_few_rows_kernel(Jo
   int i = 0;
   for (; i + 2 < tiles; i++) {
     tile(i, yes, yes);
-    if ((i & 15) == 15) {
+    if ((i & 15) == 15) {  // (the offset of what is summed so far)
 #pragma unroll
       for (int db = 0; db < DB; db++) o[db] -= ones * (127.5f * WIDENED);
       ones = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
